@@ -204,7 +204,8 @@ def prepare(case, seed):
 
 # ---- moments in 8 bits, in plain form ----
 #
-# A block of 256 values shares the exponent e of its largest magnitude. A magnitude a, with
+# A block of 256 values shares the exponent e of its largest magnitude, one more where that could
+# round up to the next power of two. A magnitude a, with
 # k = max(exponent of a, e - range), is a whole number q of 2^(k - 3), and its code is
 # 8 (k - (e - range)) + q, at most 8 range + 15. a / 2^(k - 3) is rounded to a whole number up where
 # its fraction exceeds a number u in [0, 1), else down.
@@ -222,7 +223,8 @@ def _pow2(e):
 
 def _to_codes(x, span, u, signed):
     a = x.abs().view(-1, _BLOCK)
-    e = _exponent(a.amax(dim=1, keepdim=True).contiguous()).clamp(min=span + 4)
+    top = a.amax(dim=1, keepdim=True).contiguous()
+    e = ((top.view(torch.int32) + (1 << 20)) >> 23).clamp(min=span + 4, max=254)
     k = torch.maximum(_exponent(a), e - span)
     t = a * _pow2(257 - k)  # a / 2^(k - 127 - 3), exact
     low = torch.floor(t)

@@ -48,6 +48,13 @@ from .repro_conv import (  # noqa: F401
     repro_conv2d_grad_weight_ws,
     repro_conv2d_ws,
 )
+from .repro_adamw import (  # noqa: F401
+    AdamW,
+    adamw8_state,
+    adamw8_step,
+    adamw8_values,
+    adamw_step,
+)
 from .layers import (  # noqa: F401
     Conv2d,
     FiniteGuard,

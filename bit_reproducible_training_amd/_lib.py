@@ -71,6 +71,20 @@ class rg_conv_shape(ctypes.Structure):
                 ("N", "C", "H", "W", "F", "KH", "KW", "SY", "SX", "PY", "PX")]
 
 
+class rg_adamw_config(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("step", ctypes.c_longlong)]
+
+
+class rg_adamw_tensor(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("p", "g", "m", "v")] + [("n", ctypes.c_longlong)]
+
+
+class rg_adamw8_tensor(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("p", "g", "m", "m_exp", "v", "v_exp")] + \
+               [("n", ctypes.c_longlong)]
+
+
 _CONV_WS = (ctypes.c_int, [ctypes.POINTER(rg_conv_shape), ctypes.c_int,
                            ctypes.POINTER(ctypes.c_size_t)])
 _CONV_RUN = (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
@@ -179,6 +193,16 @@ _SIGNATURES = {
 
 EXPORTED = tuple(_SIGNATURES)
 
+# The same for include/repro_adamw.h.
+_STEP_SIGNATURES = {
+    "rg_adamw_config_init": (None, [ctypes.POINTER(rg_adamw_config)]),
+    "rg_adamw_fp32": (ctypes.c_int, [ctypes.POINTER(rg_adamw_tensor), ctypes.c_int,
+                                     ctypes.POINTER(rg_adamw_config), ctypes.c_void_p]),
+    "rg_adamw8_fp32": (ctypes.c_int, [ctypes.POINTER(rg_adamw8_tensor), ctypes.c_int,
+                                      ctypes.POINTER(rg_adamw_config), ctypes.c_void_p]),
+    "rg_adamw8_values": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_longlong, ctypes.c_void_p]),
+}
+
 
 def _bind_after_torch():
     """Makes the library use the same HIP runtime as PyTorch.
@@ -211,7 +235,7 @@ def _load():
             "librepro_gemm.so is not built (%s); run __graft_entry__.build() or "
             "python -m bit_reproducible_training_amd._build" % LIB_PATH)
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in _SIGNATURES.items():
+    for name, (res, args) in list(_SIGNATURES.items()) + list(_STEP_SIGNATURES.items()):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -1,0 +1,359 @@
+// The AdamW step over a list of tensors, with the moments in float32 or in 8 bits.
+//
+// A launch takes up to a fixed number of tensors in its arguments (no table in device memory to
+// copy there first), and its blocks are dealt to them by chunks: a block finds its tensor by
+// bisection over the tensors' first chunks, which are wavefront-uniform.
+#include "rg_internal.h"
+#include "repro_adamw.h"
+#include "repro_adamw_math.h"
+
+#include <cmath>
+#include <cstdint>
+
+namespace rg {
+namespace {
+
+using repro_adamw::BLOCK;
+using repro_adamw::Scalars;
+
+static_assert(BLOCK == RG_ADAMW8_BLOCK && BLOCK == 4 * 64, "a wavefront holds a block, four values a lane");
+
+constexpr int THREADS = 256;
+constexpr long long MOST = 1ll << 30;  // values of one entry: a longer tensor takes several
+
+struct Entry {
+    float* p;
+    const float* g;
+    float* m;
+    float* v;
+    uint32_t n, first;  // values; the entry's first chunk in this launch
+};
+struct Entry8 {
+    float* p;
+    const float* g;
+    uint8_t *m, *m_exp, *v, *v_exp;
+    uint32_t n, first;
+    uint32_t block;  // the call's blocks before this entry
+};
+// As many as the 4 KiB of a launch's arguments hold.
+template <class E>
+struct List {
+    static constexpr int MAX = (4096 - 64) / sizeof(E);
+    Scalars s;
+    int count;
+    E e[MAX];
+};
+static_assert(sizeof(List<Entry>) <= 4096 && sizeof(List<Entry8>) <= 4096, "launch arguments");
+
+template <class E>
+__device__ __forceinline__ int entry_of(const List<E>& list, uint32_t chunk) {
+    int lo = 0, hi = list.count;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (list.e[mid].first <= chunk) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// A chunk is 4 U values a thread. 16-byte accesses where all four arrays allow them, else single
+// values, neighbouring threads on neighbouring values either way.
+template <int U>
+__global__ void __launch_bounds__(THREADS)
+adamw_kernel(const List<Entry> list) {
+    const Entry& t = list.e[entry_of(list, blockIdx.x)];
+    const Scalars s = list.s;
+    const uint32_t base = (blockIdx.x - t.first) * (uint32_t)(THREADS * 4 * U);
+    const uint32_t left = t.n - base;
+    float* __restrict__ p = t.p + base;
+    const float* __restrict__ g = t.g + base;
+    float* __restrict__ m = t.m + base;
+    float* __restrict__ v = t.v + base;
+    const uintptr_t off = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(g) |
+                          reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v);
+    if ((off & 15) == 0 && left >= (uint32_t)(THREADS * 4 * U)) {
+        float4 pv[U], gv[U], mv[U], vv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t i = u * THREADS + threadIdx.x;
+            pv[u] = reinterpret_cast<const float4*>(p)[i];
+            gv[u] = reinterpret_cast<const float4*>(g)[i];
+            mv[u] = reinterpret_cast<const float4*>(m)[i];
+            vv[u] = reinterpret_cast<const float4*>(v)[i];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t i = u * THREADS + threadIdx.x;
+            pv[u].x = repro_adamw::update(pv[u].x, gv[u].x, mv[u].x, vv[u].x, s);
+            pv[u].y = repro_adamw::update(pv[u].y, gv[u].y, mv[u].y, vv[u].y, s);
+            pv[u].z = repro_adamw::update(pv[u].z, gv[u].z, mv[u].z, vv[u].z, s);
+            pv[u].w = repro_adamw::update(pv[u].w, gv[u].w, mv[u].w, vv[u].w, s);
+            reinterpret_cast<float4*>(p)[i] = pv[u];
+            reinterpret_cast<float4*>(m)[i] = mv[u];
+            reinterpret_cast<float4*>(v)[i] = vv[u];
+        }
+        return;
+    }
+    const uint32_t n = left < (uint32_t)(THREADS * 4 * U) ? left : (uint32_t)(THREADS * 4 * U);
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
+        float mi = m[i], vi = v[i];
+        p[i] = repro_adamw::update(p[i], g[i], mi, vi, s);
+        m[i] = mi;
+        v[i] = vi;
+    }
+}
+
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t a) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, off, 64));
+    return a;
+}
+
+// A wavefront takes U blocks of BLOCK values, its lane l the values 4 l .. 4 l + 3 of each.
+template <int U>
+__global__ void __launch_bounds__(THREADS)
+adamw8_kernel(const List<Entry8> list) {
+    const Entry8& t = list.e[entry_of(list, blockIdx.x)];
+    const Scalars s = list.s;
+    const int lane = threadIdx.x & 63;
+    const uint32_t blocks = (t.n + BLOCK - 1) / BLOCK;
+    const uint32_t b0 = (blockIdx.x - t.first) * (uint32_t)(THREADS / 64 * U) + (threadIdx.x >> 6);
+    const bool wide = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & 15) == 0;
+    float pv[U][4], gv[U][4];
+    uint32_t mc[U], vc[U];
+    int me[U], ve[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t b = b0 + u * (THREADS / 64);
+        mc[u] = vc[u] = 0;
+        me[u] = ve[u] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pv[u][i] = gv[u][i] = 0.0f;
+        if (b >= blocks) continue;
+        const uint32_t at = b * BLOCK + 4 * lane;
+        mc[u] = reinterpret_cast<const uint32_t*>(t.m + (size_t)b * BLOCK)[lane];
+        vc[u] = reinterpret_cast<const uint32_t*>(t.v + (size_t)b * BLOCK)[lane];
+        me[u] = t.m_exp[b];
+        ve[u] = t.v_exp[b];
+        if (wide && at + 4 <= t.n) {
+            const float4 pp = *reinterpret_cast<const float4*>(t.p + at);
+            const float4 gg = *reinterpret_cast<const float4*>(t.g + at);
+            pv[u][0] = pp.x, pv[u][1] = pp.y, pv[u][2] = pp.z, pv[u][3] = pp.w;
+            gv[u][0] = gg.x, gv[u][1] = gg.y, gv[u][2] = gg.z, gv[u][3] = gg.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (at + i < t.n) {
+                    pv[u][i] = t.p[at + i];
+                    gv[u][i] = t.g[at + i];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t b = b0 + u * (THREADS / 64);
+        if (b >= blocks) continue;  // uniform in a wavefront
+        const uint32_t at = b * BLOCK + 4 * lane;
+        float m[4], v[4];
+        uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            m[i] = repro_adamw::decode_m((uint8_t)(mc[u] >> (8 * i)), me[u]);
+            v[i] = repro_adamw::decode_v((uint8_t)(vc[u] >> (8 * i)), ve[u]);
+            pv[u][i] = repro_adamw::update(pv[u][i], gv[u][i], m[i], v[i], s);
+            if (at + i >= t.n) m[i] = v[i] = 0.0f;  // past the tensor: codes of zero
+            top_m = max(top_m, repro_adamw::magnitude_bits(m[i]));
+            top_v = max(top_v, repro_adamw::magnitude_bits(v[i]));
+        }
+        const int em = repro_adamw::shared_exponent(wave_max_bits(top_m), repro_adamw::SPAN_M);
+        const int ev = repro_adamw::shared_exponent(wave_max_bits(top_v), repro_adamw::SPAN_V);
+        uint32_t cm = 0, cv = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float um, uv;
+            repro_adamw::rounding((t.block + b) * BLOCK + 4 * lane + i, s.salt, um, uv);
+            cm |= (uint32_t)repro_adamw::encode_m(m[i], em, um) << (8 * i);
+            cv |= (uint32_t)repro_adamw::encode_v(v[i], ev, uv) << (8 * i);
+        }
+        reinterpret_cast<uint32_t*>(t.m + (size_t)b * BLOCK)[lane] = cm;
+        reinterpret_cast<uint32_t*>(t.v + (size_t)b * BLOCK)[lane] = cv;
+        if (lane == 0) {
+            t.m_exp[b] = (uint8_t)em;
+            t.v_exp[b] = (uint8_t)ev;
+        }
+        if (wide && at + 4 <= t.n) {
+            *reinterpret_cast<float4*>(t.p + at) = make_float4(pv[u][0], pv[u][1], pv[u][2], pv[u][3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (at + i < t.n) t.p[at + i] = pv[u][i];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(THREADS)
+adamw8_values_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ m_exp,
+                     const uint8_t* __restrict__ v, const uint8_t* __restrict__ v_exp,
+                     float* __restrict__ m_values, float* __restrict__ v_values, long long blocks) {
+    const int lane = threadIdx.x & 63;
+    for (long long b = (long long)blockIdx.x * (THREADS / 64) + (threadIdx.x >> 6); b < blocks;
+         b += (long long)gridDim.x * (THREADS / 64)) {
+        const uint32_t mc = reinterpret_cast<const uint32_t*>(m + b * BLOCK)[lane];
+        const uint32_t vc = reinterpret_cast<const uint32_t*>(v + b * BLOCK)[lane];
+        const int me = m_exp[b], ve = v_exp[b];
+        float mo[4], vo[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            mo[i] = repro_adamw::decode_m((uint8_t)(mc >> (8 * i)), me);
+            vo[i] = repro_adamw::decode_v((uint8_t)(vc >> (8 * i)), ve);
+        }
+        reinterpret_cast<float4*>(m_values + b * BLOCK)[lane] = make_float4(mo[0], mo[1], mo[2], mo[3]);
+        reinterpret_cast<float4*>(v_values + b * BLOCK)[lane] = make_float4(vo[0], vo[1], vo[2], vo[3]);
+    }
+}
+
+bool config_ok(const rg_adamw_config* c) {
+    return c != nullptr && c->lr >= 0.0 && c->eps >= 0.0 && c->weight_decay >= 0.0 && c->beta1 >= 0.0 &&
+           c->beta1 < 1.0 && c->beta2 >= 0.0 && c->beta2 < 1.0 && c->step >= 1;
+}
+
+bool off(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+// Fills lists of entries and launches each as it is full. add(entry, chunks) appends, flush() ends.
+template <class E, class Launch>
+struct Dealer {
+    List<E> list;
+    uint32_t chunks = 0;
+    int rc = hipSuccess;
+    Launch launch;
+    Dealer(const Scalars& s, Launch l) : launch(l) {
+        list.s = s;
+        list.count = 0;
+    }
+    void flush() {
+        if (list.count == 0 || rc != hipSuccess) return;
+        launch(list, chunks);
+        rc = hipGetLastError();
+        list.count = 0;
+        chunks = 0;
+    }
+    void add(E e, uint32_t n) {
+        if (list.count == List<E>::MAX || (uint64_t)chunks + n > 0xFFFFFFu) flush();  // 2^32 threads
+        e.first = chunks;
+        list.e[list.count++] = e;
+        chunks += n;
+    }
+};
+
+template <class E, class Launch>
+Dealer<E, Launch> make_dealer(const Scalars& s, Launch l) {
+    return Dealer<E, Launch>(s, l);
+}
+
+Scalars scalars_of(const rg_adamw_config* c) {
+    return repro_adamw::make_scalars(c->lr, c->beta1, c->beta2, c->eps, c->weight_decay, c->step);
+}
+
+}  // namespace
+}  // namespace rg
+
+extern "C" {
+
+void rg_adamw_config_init(rg_adamw_config* cfg) {
+    if (!cfg) return;
+    cfg->lr = 1e-3;
+    cfg->beta1 = 0.9;
+    cfg->beta2 = 0.999;
+    cfg->eps = 1e-8;
+    cfg->weight_decay = 1e-2;
+    cfg->step = 1;
+}
+
+int rg_adamw_fp32(const rg_adamw_tensor* tensors, int count, const rg_adamw_config* cfg, void* stream) {
+    using namespace rg;
+    if (!config_ok(cfg) || count < 0 || (count > 0 && !tensors)) return hipErrorInvalidValue;
+    for (int i = 0; i < count; ++i) {
+        const rg_adamw_tensor& t = tensors[i];
+        if (t.n < 0) return hipErrorInvalidValue;
+        if (t.n > 0 && (!t.p || !t.g || !t.m || !t.v || off(t.p, 4) || off(t.g, 4) || off(t.m, 4) || off(t.v, 4)))
+            return hipErrorInvalidValue;
+    }
+    constexpr int U = 4;
+    constexpr uint32_t CHUNK = THREADS * 4 * U;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    auto dealer = make_dealer<Entry>(scalars_of(cfg), [&](const List<Entry>& list, uint32_t chunks) {
+        hipLaunchKernelGGL(adamw_kernel<U>, dim3(chunks), dim3(THREADS), 0, st, list);
+    });
+    for (int i = 0; i < count; ++i) {
+        const rg_adamw_tensor& t = tensors[i];
+        for (long long a = 0; a < t.n; a += MOST) {
+            Entry e;
+            e.p = t.p + a;
+            e.g = t.g + a;
+            e.m = t.m + a;
+            e.v = t.v + a;
+            e.n = (uint32_t)(t.n - a < MOST ? t.n - a : MOST);
+            dealer.add(e, (e.n + CHUNK - 1) / CHUNK);
+        }
+    }
+    dealer.flush();
+    return dealer.rc;
+}
+
+int rg_adamw8_fp32(const rg_adamw8_tensor* tensors, int count, const rg_adamw_config* cfg, void* stream) {
+    using namespace rg;
+    if (!config_ok(cfg) || count < 0 || (count > 0 && !tensors)) return hipErrorInvalidValue;
+    for (int i = 0; i < count; ++i) {
+        const rg_adamw8_tensor& t = tensors[i];
+        if (t.n < 0) return hipErrorInvalidValue;
+        if (t.n > 0 && (!t.p || !t.g || !t.m || !t.m_exp || !t.v || !t.v_exp || off(t.p, 4) || off(t.g, 4) ||
+                        off(t.m, 4) || off(t.v, 4)))
+            return hipErrorInvalidValue;
+    }
+    constexpr int U = 2;
+    constexpr uint32_t CHUNK = THREADS / 64 * U;  // blocks
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    auto dealer = make_dealer<Entry8>(scalars_of(cfg), [&](const List<Entry8>& list, uint32_t chunks) {
+        hipLaunchKernelGGL(adamw8_kernel<U>, dim3(chunks), dim3(THREADS), 0, st, list);
+    });
+    uint32_t before = 0;
+    for (int i = 0; i < count; ++i) {
+        const rg_adamw8_tensor& t = tensors[i];
+        for (long long a = 0; a < t.n; a += MOST) {
+            Entry8 e;
+            e.p = t.p + a;
+            e.g = t.g + a;
+            e.m = t.m + a;
+            e.m_exp = t.m_exp + a / BLOCK;
+            e.v = t.v + a;
+            e.v_exp = t.v_exp + a / BLOCK;
+            e.n = (uint32_t)(t.n - a < MOST ? t.n - a : MOST);
+            e.block = before;
+            const uint32_t blocks = (e.n + BLOCK - 1) / BLOCK;
+            before += blocks;
+            dealer.add(e, (blocks + CHUNK - 1) / CHUNK);
+        }
+    }
+    dealer.flush();
+    return dealer.rc;
+}
+
+int rg_adamw8_values(const unsigned char* m, const unsigned char* m_exp, const unsigned char* v,
+                     const unsigned char* v_exp, float* m_values, float* v_values, long long blocks,
+                     void* stream) {
+    using namespace rg;
+    if (blocks < 0 || blocks > 2147483647ll) return hipErrorInvalidValue;
+    if (blocks == 0) return hipSuccess;
+    if (!m || !m_exp || !v || !v_exp || !m_values || !v_values || off(m, 4) || off(v, 4) || off(m_values, 16) ||
+        off(v_values, 16))
+        return hipErrorInvalidValue;
+    const long long needed = (blocks + THREADS / 64 - 1) / (THREADS / 64);
+    const unsigned grid = (unsigned)(needed < (1 << 22) ? needed : (1 << 22));
+    hipLaunchKernelGGL(adamw8_values_kernel, dim3(grid), dim3(THREADS), 0, static_cast<hipStream_t>(stream), m,
+                       m_exp, v, v_exp, m_values, v_values, blocks);
+    return hipGetLastError();
+}
+
+}  // extern "C"

@@ -20,6 +20,8 @@
 #include <string>
 #include <vector>
 
+#include "repro_adamw.h"
+#include "repro_adamw_cpu.h"
 #include "repro_conv.h"
 #include "repro_conv_cpu.h"
 #include "repro_gemm.h"
@@ -357,6 +359,157 @@ void scan_finite_pair(Tensor x, int op_x, Tensor y, int op_y, Tensor flag) {
           "finite scan");
 }
 
+// ---- AdamW ----
+
+rg_adamw_config adamw_config(double lr, double beta1, double beta2, double eps, double weight_decay, int64_t step) {
+    need(lr >= 0 && eps >= 0 && weight_decay >= 0, "adamw: lr, eps and weight_decay must not be negative");
+    need(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adamw: betas must be in [0, 1)");
+    need(step >= 1, "adamw: step must be at least 1");
+    rg_adamw_config c;
+    rg_adamw_config_init(&c);
+    c.lr = lr;
+    c.beta1 = beta1;
+    c.beta2 = beta2;
+    c.eps = eps;
+    c.weight_decay = weight_decay;
+    c.step = step;
+    return c;
+}
+
+repro_adamw::Scalars adamw_scalars(const rg_adamw_config& c) {
+    return repro_adamw::make_scalars(c.lr, c.beta1, c.beta2, c.eps, c.weight_decay, c.step);
+}
+
+// The step goes through a tensor's memory in its own order, so all of a value's tensors must be
+// dense, without overlaps and laid out alike.
+void need_alike(const Tensor& p, const Tensor& t, const char* name) {
+    need(t.scalar_type() == torch::kFloat32, std::string("adamw: ") + name + " must be float32");
+    need(t.device() == p.device(), std::string("adamw: ") + name + " must be on its parameter's device");
+    need(t.sizes() == p.sizes() && (p.is_contiguous() ? t.is_contiguous() : t.strides() == p.strides()),
+         std::string("adamw: ") + name + " must have its parameter's shape and strides");
+    need(!t.is_neg(), std::string("adamw: ") + name + " must not be a lazily negated view");
+}
+
+// The first parameter's device kind (true: GPU); every parameter float32, dense and on that device.
+bool adamw_parameters(const std::vector<Tensor>& params, const std::vector<Tensor>& grads) {
+    need(params.size() == grads.size(), "adamw: as many gradients as parameters");
+    for (size_t i = 0; i < params.size(); ++i) {
+        const Tensor& p = params[i];
+        need(p.device() == params[0].device(), "adamw: parameters must be on one device");
+        need(p.is_cuda() || p.is_cpu(), "adamw: parameters must be on the CPU or a GPU");
+        need(p.is_non_overlapping_and_dense(), "adamw: parameters must be dense");
+        need_alike(p, p, "a parameter");
+        need_alike(p, grads[i], "a gradient");
+    }
+    return !params.empty() && params[0].is_cuda();
+}
+
+void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m,
+                const std::vector<Tensor>& v, double lr, double beta1, double beta2, double eps,
+                double weight_decay, int64_t step) {
+    const rg_adamw_config cfg = adamw_config(lr, beta1, beta2, eps, weight_decay, step);
+    const bool gpu = adamw_parameters(params, grads);
+    need(m.size() == params.size() && v.size() == params.size(), "adamw: as many moments as parameters");
+    std::vector<rg_adamw_tensor> list(params.size());
+    for (size_t i = 0; i < params.size(); ++i) {
+        need_alike(params[i], m[i], "a first moment");
+        need_alike(params[i], v[i], "a second moment");
+        list[i] = {params[i].data_ptr<float>(), grads[i].data_ptr<float>(), m[i].data_ptr<float>(),
+                   v[i].data_ptr<float>(), (long long)params[i].numel()};
+    }
+    if (list.empty()) return;
+    if (gpu) {
+        c10::DeviceGuard guard(params[0].device());
+        check(rg_adamw_fp32(list.data(), (int)list.size(), &cfg, stream_of(params[0])), "adamw");
+        return;
+    }
+    const repro_adamw::Scalars s = adamw_scalars(cfg);
+    py::gil_scoped_release nogil;
+    for (const rg_adamw_tensor& t : list) repro_adamw::cpu_adamw(t.p, t.g, t.m, t.v, t.n, s);
+}
+
+int64_t adamw8_blocks(int64_t n) { return (n + RG_ADAMW8_BLOCK - 1) / RG_ADAMW8_BLOCK; }
+
+void need_codes(const Tensor& t, const Tensor& p, int64_t n, const char* name) {
+    need(t.scalar_type() == torch::kUInt8 && t.is_contiguous() && t.device() == p.device() && t.numel() == n,
+         std::string("adamw: ") + name + " must be contiguous uint8 of " + std::to_string(n) + " values on the parameters' device");
+    need((reinterpret_cast<uintptr_t>(t.data_ptr()) & 3) == 0, std::string("adamw: ") + name + " must be at a multiple of 4 bytes");
+}
+
+void need_exponents(const Tensor& t, const Tensor& p, int64_t n) {
+    need(t.scalar_type() == torch::kUInt8 && t.is_contiguous() && t.device() == p.device() && t.numel() == n,
+         "adamw: exponents must be contiguous uint8, one a block, on the parameters' device");
+}
+
+// The moments' codes and exponents: one tensor of each for all parameters (each parameter at whole
+// blocks, in order), or one for each parameter.
+void adamw8_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m,
+                 const std::vector<Tensor>& m_exp, const std::vector<Tensor>& v, const std::vector<Tensor>& v_exp,
+                 bool flat, double lr, double beta1, double beta2, double eps, double weight_decay,
+                 int64_t step) {
+    const rg_adamw_config cfg = adamw_config(lr, beta1, beta2, eps, weight_decay, step);
+    const bool gpu = adamw_parameters(params, grads);
+    const size_t states = flat ? 1 : params.size();
+    need(m.size() == states && m_exp.size() == states && v.size() == states && v_exp.size() == states,
+         "adamw: as many moments as parameters");
+    if (params.empty()) return;
+    const auto need_state = [&](size_t k, int64_t blocks) {
+        need_codes(m[k], params[0], blocks * RG_ADAMW8_BLOCK, "the first moments");
+        need_codes(v[k], params[0], blocks * RG_ADAMW8_BLOCK, "the second moments");
+        need_exponents(m_exp[k], params[0], blocks);
+        need_exponents(v_exp[k], params[0], blocks);
+    };
+    int64_t total = 0;
+    for (const Tensor& p : params) total += adamw8_blocks(p.numel());
+    if (flat) need_state(0, total);
+    int64_t at = 0;
+    std::vector<rg_adamw8_tensor> list(params.size());
+    for (size_t i = 0; i < params.size(); ++i) {
+        const int64_t blocks = adamw8_blocks(params[i].numel());
+        if (!flat) need_state(i, blocks);
+        const size_t k = flat ? 0 : i;
+        list[i] = {params[i].data_ptr<float>(), grads[i].data_ptr<float>(),
+                   m[k].data_ptr<uint8_t>() + at * RG_ADAMW8_BLOCK, m_exp[k].data_ptr<uint8_t>() + at,
+                   v[k].data_ptr<uint8_t>() + at * RG_ADAMW8_BLOCK, v_exp[k].data_ptr<uint8_t>() + at,
+                   (long long)params[i].numel()};
+        if (flat) at += blocks;
+    }
+    if (gpu) {
+        c10::DeviceGuard guard(params[0].device());
+        check(rg_adamw8_fp32(list.data(), (int)list.size(), &cfg, stream_of(params[0])), "adamw8");
+        return;
+    }
+    const repro_adamw::Scalars s = adamw_scalars(cfg);
+    py::gil_scoped_release nogil;
+    int64_t first = 0;
+    for (const rg_adamw8_tensor& t : list) {
+        repro_adamw::cpu_adamw8(t.p, t.g, t.m, t.m_exp, t.v, t.v_exp, t.n, first, s);
+        first += adamw8_blocks(t.n);
+    }
+}
+
+std::vector<Tensor> adamw8_values(const Tensor& m, const Tensor& m_exp, const Tensor& v, const Tensor& v_exp) {
+    const int64_t blocks = m_exp.numel();
+    need(m.is_cuda() || m.is_cpu(), "adamw: tensors must be on the CPU or a GPU");
+    need_codes(m, m, blocks * RG_ADAMW8_BLOCK, "the first moments");
+    need_codes(v, m, blocks * RG_ADAMW8_BLOCK, "the second moments");
+    need_exponents(m_exp, m, blocks);
+    need_exponents(v_exp, m, blocks);
+    Tensor mo = torch::empty({blocks * RG_ADAMW8_BLOCK}, m.options().dtype(torch::kFloat32));
+    Tensor vo = torch::empty_like(mo);
+    if (m.is_cuda()) {
+        c10::DeviceGuard guard(m.device());
+        check(rg_adamw8_values(m.data_ptr<uint8_t>(), m_exp.data_ptr<uint8_t>(), v.data_ptr<uint8_t>(),
+                               v_exp.data_ptr<uint8_t>(), mo.data_ptr<float>(), vo.data_ptr<float>(), blocks,
+                               stream_of(m)),
+              "adamw8 values");
+    } else {
+        repro_adamw::cpu_adamw8_values(m.data_ptr<uint8_t>(), m_exp.data_ptr<uint8_t>(), mo.data_ptr<float>(), blocks, true);
+        repro_adamw::cpu_adamw8_values(v.data_ptr<uint8_t>(), v_exp.data_ptr<uint8_t>(), vo.data_ptr<float>(), blocks, false);
+    }
+    return {mo, vo};
+}
+
 }  // namespace
 
 // 64-bit FNV-1a over the raw bytes of a contiguous CPU tensor, continuing from h: the hash the
@@ -388,6 +541,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("conv2d_bias", &conv2d_bias);
     m.def("exact_sum_watch", &exact_sum_watch);
     m.def("scan_finite_pair", &scan_finite_pair);
+    m.def("adamw_step", &adamw_step);
+    m.def("adamw8_step", &adamw8_step);
+    m.def("adamw8_values", &adamw8_values);
     m.def("cpu_threads", &repro_gemm::cpu_thread_count);
     m.def("set_error_class", [](py::object cls) {
         Py_XINCREF(cls.ptr());

@@ -55,6 +55,12 @@ from .repro_adamw import (  # noqa: F401
     adamw8_values,
     adamw_step,
 )
+from .repro_norm import (  # noqa: F401
+    Norm,
+    ResidualNorm,
+    norm,
+    residual_norm,
+)
 from .layers import (  # noqa: F401
     Conv2d,
     FiniteGuard,

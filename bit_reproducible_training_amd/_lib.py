@@ -85,6 +85,11 @@ class rg_adamw8_tensor(ctypes.Structure):
                [("n", ctypes.c_longlong)]
 
 
+class rg_norm_config(ctypes.Structure):
+    _fields_ = [("N", ctypes.c_longlong), ("D", ctypes.c_int), ("rms", ctypes.c_int), ("post", ctypes.c_int),
+                ("gate_rows", ctypes.c_longlong), ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
 _CONV_WS = (ctypes.c_int, [ctypes.POINTER(rg_conv_shape), ctypes.c_int,
                            ctypes.POINTER(ctypes.c_size_t)])
 _CONV_RUN = (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
@@ -193,13 +198,20 @@ _SIGNATURES = {
 
 EXPORTED = tuple(_SIGNATURES)
 
-# The same for include/repro_adamw.h.
+# The same for include/repro_adamw.h and include/repro_norm.h.
 _STEP_SIGNATURES = {
     "rg_adamw_config_init": (None, [ctypes.POINTER(rg_adamw_config)]),
     "rg_adamw_fp32": (ctypes.c_int, [ctypes.POINTER(rg_adamw_tensor), ctypes.c_int,
                                      ctypes.POINTER(rg_adamw_config), ctypes.c_void_p]),
     "rg_adamw8_fp32": (ctypes.c_int, [ctypes.POINTER(rg_adamw8_tensor), ctypes.c_int,
                                       ctypes.POINTER(rg_adamw_config), ctypes.c_void_p]),
+    "rg_norm_config_init": (None, [ctypes.POINTER(rg_norm_config)]),
+    "rg_residual_norm_fp32": (ctypes.c_int, [ctypes.POINTER(rg_norm_config)] + [ctypes.c_void_p] * 11 +
+                              [ctypes.c_int, ctypes.c_void_p]),
+    "rg_residual_norm_grad_workspace": (ctypes.c_int, [ctypes.POINTER(rg_norm_config), ctypes.c_int,
+                                                       ctypes.POINTER(ctypes.c_size_t)]),
+    "rg_residual_norm_grad_fp32": (ctypes.c_int, [ctypes.POINTER(rg_norm_config)] + [ctypes.c_void_p] * 17 +
+                                   [ctypes.c_size_t, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "rg_adamw8_values": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_longlong, ctypes.c_void_p]),
 }
 

@@ -26,6 +26,8 @@
 #include "repro_conv_cpu.h"
 #include "repro_gemm.h"
 #include "repro_gemm_cpu.h"
+#include "repro_norm.h"
+#include "repro_norm_cpu.h"
 #include "repro_sum.h"
 #include "repro_sum_cpu.h"
 
@@ -510,6 +512,136 @@ std::vector<Tensor> adamw8_values(const Tensor& m, const Tensor& m_exp, const Te
     return {mo, vo};
 }
 
+// ---- norms ----
+
+using OptTensor = c10::optional<Tensor>;
+
+// A float32 tensor of `numel` values on x's device, contiguous; undefined where there is none.
+Tensor norm_operand(const OptTensor& t, const Tensor& x, int64_t numel, const char* name) {
+    if (!t.has_value()) return Tensor();
+    need(t->scalar_type() == torch::kFloat32, std::string("norm: ") + name + " must be float32");
+    need(t->device() == x.device(), std::string("norm: ") + name + " must be on x's device");
+    need(t->numel() == numel, std::string("norm: ") + name + " has the wrong number of values");
+    return t->resolve_neg().contiguous();
+}
+
+const float* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+float* out_or_null(Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+rg_norm_config norm_config(const Tensor& x, const OptTensor& gate, bool rms, bool post, double eps, double scale) {
+    require_f32(x, "x");
+    need(x.is_cuda() || x.is_cpu(), "norm: tensors must be on the CPU or a GPU");
+    need(x.dim() == 2, "norm: x must be [rows, values]");
+    need(x.size(1) >= 1 && x.size(1) <= RG_NORM_MAX_D,
+         "norm: a row must have 1 to " + std::to_string(RG_NORM_MAX_D) + " values");
+    need(eps >= 0, "norm: eps must not be negative");
+    rg_norm_config c;
+    rg_norm_config_init(&c);
+    c.N = x.size(0);
+    c.D = (int)x.size(1);
+    c.rms = rms ? 1 : 0;
+    c.post = post ? 1 : 0;
+    c.eps = (float)eps;
+    c.scale = (float)scale;
+    if (gate.has_value() && c.N > 0) {
+        const int64_t rows = gate->numel() / c.D;
+        need(rows >= 1 && gate->numel() == rows * c.D && rows <= c.N && c.N % rows == 0,
+             "norm: the gate's rows must divide x's");
+        c.gate_rows = rows;
+    }
+    return c;
+}
+
+// x, f [N][D] -> {r (undefined without f), y, stats (undefined unless wanted)}
+std::vector<OptTensor> residual_norm(Tensor x, OptTensor f_, OptTensor gate_, OptTensor post_weight_, OptTensor post_bias_,
+                                     OptTensor weight_, OptTensor bias_, bool rms, bool post, double eps, double scale,
+                                     bool want_stats, OptTensor flag, int op_id) {
+    rg_norm_config c = norm_config(x, gate_, rms, post, eps, scale);
+    x = x.resolve_neg().contiguous();
+    const int64_t D = c.D;
+    const Tensor f = norm_operand(f_, x, x.numel(), "f");
+    const Tensor gate = norm_operand(gate_, x, gate_.has_value() ? gate_->numel() : 0, "the gate");
+    const Tensor pw = norm_operand(post_weight_, x, D, "post_weight"), pb = norm_operand(post_bias_, x, D, "post_bias");
+    const Tensor w = norm_operand(weight_, x, D, "weight"), b = norm_operand(bias_, x, D, "bias");
+    need(f.defined() || (!gate.defined() && !post), "norm: a gate or a post norm needs f");
+    need(post || (!pw.defined() && !pb.defined()), "norm: post_weight and post_bias need the post norm");
+    Tensor y = torch::empty_like(x), r, stats;
+    if (f.defined()) r = torch::empty_like(x);
+    if (want_stats) stats = torch::empty({c.N, 4}, x.options());
+    if (x.is_cuda()) {
+        c10::DeviceGuard guard(x.device());
+        if (flag.has_value()) require_flag(*flag, x, "residual_norm");
+        check(rg_residual_norm_fp32(&c, x.data_ptr<float>(), data_or_null(f), c.N > 0 ? data_or_null(gate) : nullptr,
+                                    data_or_null(pw), data_or_null(pb), data_or_null(w), data_or_null(b),
+                                    out_or_null(r), y.data_ptr<float>(), out_or_null(stats),
+                                    flag.has_value() ? flag->data_ptr<int>() : nullptr, op_id, stream_of(x)),
+              "residual norm");
+    } else {
+        py::gil_scoped_release nogil;
+        repro_norm::cpu_residual_norm(c, x.data_ptr<float>(), data_or_null(f), data_or_null(gate), data_or_null(pw),
+                                      data_or_null(pb), data_or_null(w), data_or_null(b), out_or_null(r),
+                                      y.data_ptr<float>(), out_or_null(stats));
+    }
+    const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    return {opt(r), opt(y), opt(stats)};
+}
+
+// {dx, df, dgate, dpost_weight, dpost_bias, dweight, dbias}, those that `want` asks for.
+std::vector<OptTensor> residual_norm_grad(OptTensor dr_, OptTensor dy_, Tensor r, OptTensor f_, OptTensor gate_,
+                                          OptTensor post_weight_, OptTensor post_bias_, OptTensor weight_, Tensor stats,
+                                          bool rms, bool post, double eps, double scale, std::vector<bool> want,
+                                          OptTensor flag, int op_id) {
+    rg_norm_config c = norm_config(r, gate_, rms, post, eps, scale);
+    need(want.size() == 7, "norm: seven gradients");
+    need(r.is_contiguous(), "norm: r must be contiguous");
+    const int64_t D = c.D;
+    const Tensor dr = norm_operand(dr_, r, r.numel(), "dr"), dy = norm_operand(dy_, r, r.numel(), "dy");
+    const Tensor f = norm_operand(f_, r, r.numel(), "f");
+    const Tensor gate = norm_operand(gate_, r, gate_.has_value() ? gate_->numel() : 0, "the gate");
+    const Tensor pw = norm_operand(post_weight_, r, D, "post_weight"), pb = norm_operand(post_bias_, r, D, "post_bias");
+    const Tensor w = norm_operand(weight_, r, D, "weight");
+    need(stats.scalar_type() == torch::kFloat32 && stats.device() == r.device() && stats.is_contiguous() &&
+             stats.numel() == 4 * c.N,
+         "norm: stats must be the forward pass's");
+    need(dr.defined() || dy.defined(), "norm: a gradient of r or y is needed");
+    const auto rows = r.options();
+    const auto maybe = [&](int i, at::IntArrayRef shape) { return want[i] ? torch::empty(shape, rows) : Tensor(); };
+    Tensor dx = maybe(0, {c.N, D}), df = maybe(1, {c.N, D}), dgate = maybe(2, {std::max<int64_t>(c.gate_rows, 1), D});
+    Tensor dpw = maybe(3, {D}), dpb = maybe(4, {D}), dw = maybe(5, {D}), db = maybe(6, {D});
+    if (!dy.defined()) {  // y was not used: its weight's gradients are zero
+        for (Tensor* t : {&dw, &db})
+            if (t->defined()) t->zero_();
+    }
+    Tensor kernel_dw = dy.defined() ? dw : Tensor(), kernel_db = dy.defined() ? db : Tensor();
+    if (c.N == 0) {
+        for (Tensor* t : {&dgate, &dpw, &dpb, &dw, &db})
+            if (t->defined()) t->zero_();
+    } else if (r.is_cuda()) {
+        c10::DeviceGuard guard(r.device());
+        if (flag.has_value()) require_flag(*flag, r, "residual_norm_grad");
+        const bool sums = dgate.defined() || dpw.defined() || dpb.defined() || kernel_dw.defined() || kernel_db.defined();
+        size_t bytes = 0;
+        check(rg_residual_norm_grad_workspace(&c, sums ? 1 : 0, &bytes), "norm gradient plan");
+        Tensor ws = workspace_like(bytes, r);
+        check(rg_residual_norm_grad_fp32(&c, data_or_null(dr), data_or_null(dy), r.data_ptr<float>(), data_or_null(f),
+                                         data_or_null(gate), data_or_null(pw), data_or_null(pb), data_or_null(w),
+                                         stats.data_ptr<float>(), out_or_null(dx), out_or_null(df), out_or_null(dgate),
+                                         out_or_null(dpw), out_or_null(dpb), out_or_null(kernel_dw),
+                                         out_or_null(kernel_db), ws.data_ptr(), (size_t)ws.numel(),
+                                         flag.has_value() ? flag->data_ptr<int>() : nullptr, op_id, stream_of(r)),
+              "norm gradient");
+    } else {
+        py::gil_scoped_release nogil;
+        repro_norm::cpu_residual_norm_grad(c, data_or_null(dr), data_or_null(dy), r.data_ptr<float>(), data_or_null(f),
+                                           data_or_null(gate), data_or_null(pw), data_or_null(pb), data_or_null(w),
+                                           stats.data_ptr<float>(), out_or_null(dx), out_or_null(df),
+                                           out_or_null(dgate), out_or_null(dpw), out_or_null(dpb),
+                                           out_or_null(kernel_dw), out_or_null(kernel_db));
+    }
+    const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    return {opt(dx), opt(df), opt(dgate), opt(dpw), opt(dpb), opt(dw), opt(db)};
+}
+
 }  // namespace
 
 // 64-bit FNV-1a over the raw bytes of a contiguous CPU tensor, continuing from h: the hash the
@@ -544,6 +676,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw_step", &adamw_step);
     m.def("adamw8_step", &adamw8_step);
     m.def("adamw8_values", &adamw8_values);
+    m.def("residual_norm", &residual_norm);
+    m.def("residual_norm_grad", &residual_norm_grad);
     m.def("cpu_threads", &repro_gemm::cpu_thread_count);
     m.def("set_error_class", [](py::object cls) {
         Py_XINCREF(cls.ptr());

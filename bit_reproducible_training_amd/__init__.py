@@ -55,6 +55,10 @@ from .repro_adamw import (  # noqa: F401
     adamw8_values,
     adamw_step,
 )
+from .repro_loss import (  # noqa: F401
+    LinearCrossEntropy,
+    linear_cross_entropy,
+)
 from .repro_norm import (  # noqa: F401
     Norm,
     ResidualNorm,

@@ -22,7 +22,7 @@ BUILD_DIR = os.path.join(CSRC, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "librepro_gemm.so")
 
 SOURCES = ["rg_slice.hip", "rg_contract.hip", "rg_probe.hip", "rg_sum.hip", "rg_conv.hip", "rg_conv_fused.hip", "rg_conv_dw.hip",
-           "rg_adamw.hip", "rg_norm.hip", "rg_api.cpp"]
+           "rg_loss.hip", "rg_norm.hip", "rg_adamw.hip", "rg_api.cpp"]
 BINDING_SOURCE = "rg_torch.cpp"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

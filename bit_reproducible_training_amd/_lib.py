@@ -85,6 +85,11 @@ class rg_adamw8_tensor(ctypes.Structure):
                [("n", ctypes.c_longlong)]
 
 
+class rg_loss_config(ctypes.Structure):
+    _fields_ = [("N", ctypes.c_longlong), ("D", ctypes.c_int), ("V", ctypes.c_int), ("slices", ctypes.c_int),
+                ("reduction", ctypes.c_int), ("ignore_index", ctypes.c_longlong)]
+
+
 class rg_norm_config(ctypes.Structure):
     _fields_ = [("N", ctypes.c_longlong), ("D", ctypes.c_int), ("rms", ctypes.c_int), ("post", ctypes.c_int),
                 ("gate_rows", ctypes.c_longlong), ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
@@ -198,13 +203,20 @@ _SIGNATURES = {
 
 EXPORTED = tuple(_SIGNATURES)
 
-# The same for include/repro_adamw.h and include/repro_norm.h.
-_STEP_SIGNATURES = {
+# The same for include/repro_adamw.h, include/repro_norm.h and include/repro_loss.h.
+_MODEL_SIGNATURES = {
     "rg_adamw_config_init": (None, [ctypes.POINTER(rg_adamw_config)]),
     "rg_adamw_fp32": (ctypes.c_int, [ctypes.POINTER(rg_adamw_tensor), ctypes.c_int,
                                      ctypes.POINTER(rg_adamw_config), ctypes.c_void_p]),
     "rg_adamw8_fp32": (ctypes.c_int, [ctypes.POINTER(rg_adamw8_tensor), ctypes.c_int,
                                       ctypes.POINTER(rg_adamw_config), ctypes.c_void_p]),
+    "rg_loss_config_init": (None, [ctypes.POINTER(rg_loss_config)]),
+    "rg_loss_group_tokens": (ctypes.c_int, [ctypes.c_int]),
+    "rg_linear_cross_entropy_workspace": (ctypes.c_int, [ctypes.POINTER(rg_loss_config), ctypes.c_int, ctypes.c_int,
+                                                         ctypes.POINTER(ctypes.c_size_t)]),
+    "rg_linear_cross_entropy": (ctypes.c_int, [ctypes.POINTER(rg_loss_config)] + [ctypes.c_void_p] * 8 +
+                                [ctypes.c_size_t, ctypes.c_void_p]),
+    "rg_scale_fp32": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "rg_norm_config_init": (None, [ctypes.POINTER(rg_norm_config)]),
     "rg_residual_norm_fp32": (ctypes.c_int, [ctypes.POINTER(rg_norm_config)] + [ctypes.c_void_p] * 11 +
                               [ctypes.c_int, ctypes.c_void_p]),
@@ -247,7 +259,7 @@ def _load():
             "librepro_gemm.so is not built (%s); run __graft_entry__.build() or "
             "python -m bit_reproducible_training_amd._build" % LIB_PATH)
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in list(_SIGNATURES.items()) + list(_STEP_SIGNATURES.items()):
+    for name, (res, args) in list(_SIGNATURES.items()) + list(_MODEL_SIGNATURES.items()):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

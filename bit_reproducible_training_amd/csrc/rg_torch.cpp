@@ -26,6 +26,8 @@
 #include "repro_conv_cpu.h"
 #include "repro_gemm.h"
 #include "repro_gemm_cpu.h"
+#include "repro_loss.h"
+#include "repro_loss_cpu.h"
 #include "repro_norm.h"
 #include "repro_norm_cpu.h"
 #include "repro_sum.h"
@@ -642,6 +644,76 @@ std::vector<OptTensor> residual_norm_grad(OptTensor dr_, OptTensor dy_, Tensor r
     return {opt(dx), opt(df), opt(dgate), opt(dpw), opt(dpb), opt(dw), opt(db)};
 }
 
+// ---- cross entropy of a vocabulary projection ----
+
+// {loss, dx, dweight}: x [N][D], weight [V][D], target [N]; factors [N] or none; the gradients that are wanted.
+std::vector<OptTensor> linear_cross_entropy(Tensor x, Tensor weight, Tensor target, OptTensor factors_, int S,
+                                            int reduction, int64_t ignore_index, bool want_loss, bool want_dx,
+                                            bool want_dw) {
+    require_f32(x, "x");
+    require_f32(weight, "weight");
+    const bool gpu = on_gpu(x, weight, "linear_cross_entropy");
+    need(target.device() == x.device(), "linear_cross_entropy: tensors must be on the same device");
+    need(target.scalar_type() == torch::kInt64, "linear_cross_entropy: target must be int64");
+    need(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1) && target.dim() == 1 && target.size(0) == x.size(0),
+         "linear_cross_entropy: x must be [tokens, size], weight [words, size], target [tokens]");
+    need(x.size(1) >= 1 && weight.size(0) >= 1, "linear_cross_entropy: sizes must be positive");
+    need(x.size(0) <= INT32_MAX && x.size(1) <= INT32_MAX && weight.size(0) <= INT32_MAX, "linear_cross_entropy: sizes must be below 2^31");
+    need(S >= 1 && S <= 3, "linear_cross_entropy: slices must be 1..3");
+    need(reduction >= RG_LOSS_MEAN && reduction <= RG_LOSS_NONE, "linear_cross_entropy: unknown reduction");
+    x = x.resolve_neg().contiguous();
+    weight = weight.resolve_neg().contiguous();
+    target = target.contiguous();
+    Tensor factors;
+    if (factors_.has_value()) {
+        factors = factors_->resolve_neg().contiguous();
+        require_f32(factors, "factors");
+        need(factors.device() == x.device() && factors.numel() == x.size(0), "linear_cross_entropy: one factor for each token");
+    }
+    rg_loss_config c;
+    rg_loss_config_init(&c);
+    c.N = x.size(0);
+    c.D = (int)x.size(1);
+    c.V = (int)weight.size(0);
+    c.slices = S;
+    c.reduction = reduction;
+    c.ignore_index = ignore_index;
+    Tensor loss, dx, dw;
+    if (want_loss) loss = reduction == RG_LOSS_NONE ? torch::empty({c.N}, x.options()) : torch::empty({}, x.options());
+    if (want_dx) dx = torch::empty_like(x);
+    if (want_dw) dw = torch::empty_like(weight);
+    const auto* t = target.data_ptr<int64_t>();
+    if (gpu) {
+        c10::DeviceGuard guard(x.device());
+        size_t bytes = 0;
+        check(rg_linear_cross_entropy_workspace(&c, want_dx, want_dw, &bytes), "linear cross entropy plan");
+        Tensor ws = workspace_like(bytes, x);
+        check(rg_linear_cross_entropy(&c, x.data_ptr<float>(), weight.data_ptr<float>(),
+                                      reinterpret_cast<const long long*>(t), data_or_null(factors), out_or_null(loss),
+                                      out_or_null(dx), out_or_null(dw), ws.data_ptr(), (size_t)ws.numel(), stream_of(x)),
+              "linear cross entropy");
+    } else {
+        py::gil_scoped_release nogil;
+        repro_loss::cpu_linear_cross_entropy(c, x.data_ptr<float>(), weight.data_ptr<float>(), t, data_or_null(factors),
+                                             out_or_null(loss), out_or_null(dx), out_or_null(dw));
+    }
+    const auto opt = [](const Tensor& v) { return v.defined() ? OptTensor(v) : OptTensor(); };
+    return {opt(loss), opt(dx), opt(dw)};
+}
+
+// t *= factor[0] for a contiguous t; no write where the factor is 1.
+void scale_(Tensor t, Tensor factor) {
+    require_f32(t, "t");
+    require_f32(factor, "factor");
+    need(t.is_contiguous() && factor.numel() == 1, "scale_: a contiguous tensor and one factor");
+    if (on_gpu(t, factor, "scale_")) {
+        c10::DeviceGuard guard(t.device());
+        check(rg_scale_fp32(t.data_ptr<float>(), factor.data_ptr<float>(), (size_t)t.numel(), stream_of(t)), "scale");
+        return;
+    }
+    t.mul_(factor);
+}
+
 }  // namespace
 
 // 64-bit FNV-1a over the raw bytes of a contiguous CPU tensor, continuing from h: the hash the
@@ -678,6 +750,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw8_values", &adamw8_values);
     m.def("residual_norm", &residual_norm);
     m.def("residual_norm_grad", &residual_norm_grad);
+    m.def("linear_cross_entropy", &linear_cross_entropy);
+    m.def("scale_", &scale_);
     m.def("cpu_threads", &repro_gemm::cpu_thread_count);
     m.def("set_error_class", [](py::object cls) {
         Py_XINCREF(cls.ptr());

@@ -134,7 +134,7 @@ def name_layers(model, prefix=""):
     """Gives every reproducible layer of `model` its path in the model (prefix + the name from
     named_modules()) as repro_name, which the guard's messages use. Returns the model."""
     for path, module in model.named_modules():
-        if isinstance(module, (Linear, Conv2d)):
+        if isinstance(getattr(type(module), "repro_name", None), str):
             module.repro_name = prefix + path
     return model
 

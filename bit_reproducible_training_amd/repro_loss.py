@@ -1,0 +1,90 @@
+"""The softmax cross entropy of a language model's head: x W^T, the loss and its gradients, without
+keeping the logits.
+
+  linear_cross_entropy   the loss of hidden states against target words, differentiable
+  LinearCrossEntropy     a module with the head's weight, which reports to the layers' guard
+
+The three products (logits, the gradients of x and of the weight) are the reproducible GEMM's; the
+softmax's exponentials, logarithms and sums have their own definition (include/repro_loss_math.h). So loss
+and gradients have the same bits on every run, on the GPU and on the CPU. Tokens are taken in groups, and
+a group's logits are used for its gradients at once, so training takes three products and the memory
+of one group's logits (512 MB, or those of 128 tokens): with the sum or the mean of the losses,
+the forward pass leaves the gradients for the backward pass to hand out. Without a reduction, whose
+gradients need what arrives there, the backward pass computes the logits again.
+"""
+import torch
+
+from ._lib import _backend
+from .layers import _CallInfo, _watch_operands, get_slices, guard
+
+__all__ = ["LinearCrossEntropy", "linear_cross_entropy"]
+
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
+
+
+class _LossOp(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, target, settings):
+        slices, reduction, ignore_index, wanted = settings
+        early = reduction != 2
+        loss, dx, dw = _backend.linear_cross_entropy(x, weight, target, None, slices, reduction, ignore_index, True,
+                                                     wanted[0] and early, wanted[1] and early)
+        if any(wanted):
+            ctx.settings = settings
+            ctx.ready = (dx, dw) if early else None
+            ctx.save_for_backward(x, weight, target)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        slices, reduction, ignore_index, wanted = ctx.settings
+        x, weight, target = ctx.saved_tensors
+        if reduction == 2:
+            _, dx, dw = _backend.linear_cross_entropy(x, weight, target, dloss, slices, reduction, ignore_index, False,
+                                                      *wanted)
+            return dx, dw, None, None
+        ready, ctx.ready = ctx.ready, None
+        if ready is None:  # handed out by an earlier backward pass
+            ready = _backend.linear_cross_entropy(x, weight, target, None, slices, reduction, ignore_index, False,
+                                                  *wanted)[1:]
+        for g in ready:
+            if g is not None:
+                _backend.scale_(g, dloss)
+        return (*ready, None, None)
+
+
+def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mean", slices=None):
+    """The cross entropy of softmax(x weight^T) against target, for float32 x [..., size], weight
+    [words, size] and int64 target [...]; reduction "mean" (over the tokens that count), "sum", or
+    "none" (a loss for each token). Tokens whose target is ignore_index are left out; one whose target
+    is no word has a NaN loss and no gradients. slices: the products' S (the layers' by default)."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError('reduction must be "mean", "sum" or "none"')
+    if x.dim() < 1 or x.shape[-1] < 1 or tuple(target.shape) != tuple(x.shape[:-1]):
+        raise ValueError("linear_cross_entropy: x must be [..., size] and target [...]")
+    grad = torch.is_grad_enabled()
+    settings = (get_slices() if slices is None else int(slices), _REDUCTIONS[reduction], int(ignore_index),
+                (grad and x.requires_grad, grad and weight.requires_grad))
+    loss = _LossOp.apply(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1), settings)
+    return loss.view(target.shape) if reduction == "none" else loss
+
+
+class LinearCrossEntropy(torch.nn.Module):
+    """A head of num_words words over hidden states of in_features values with its loss:
+    forward(x, target) is linear_cross_entropy of them. The weight [num_words, in_features] may be
+    shared with an embedding."""
+
+    repro_name = "linear_cross_entropy"
+
+    def __init__(self, in_features, num_words, ignore_index=-100, reduction="mean"):
+        super().__init__()
+        if reduction not in _REDUCTIONS:
+            raise ValueError('reduction must be "mean", "sum" or "none"')
+        self.ignore_index, self.reduction = ignore_index, reduction
+        self.weight = torch.nn.Parameter(torch.empty(num_words, in_features))
+        torch.nn.init.normal_(self.weight, std=0.02)
+
+    def forward(self, x, target):
+        _watch_operands(_CallInfo(self.repro_name, get_slices(), guard()), x, self.weight)
+        return linear_cross_entropy(x, self.weight, target, ignore_index=self.ignore_index, reduction=self.reduction)

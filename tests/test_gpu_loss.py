@@ -1,0 +1,136 @@
+"""The vocabulary projection's cross entropy and its gradients on the GPU against the CPU's: the same bits."""
+import math
+
+import pytest
+import torch
+
+import bit_reproducible_training_amd as rg
+from bit_reproducible_training_amd import _lib
+from test_loss import case, check, results
+
+pytestmark = pytest.mark.gpu
+
+
+def assert_same(got, want):
+    for name, a, b in zip(("loss", "dx", "dw"), got, want):
+        a, b = a.cpu(), b.cpu()
+        nan = b.isnan()
+        assert torch.equal(a.isnan(), nan), name
+        assert torch.equal(a[~nan].view(torch.int32), b[~nan].view(torch.int32)), name
+
+
+# One word, one part and its ends, one token, sizes off every multiple, long rows, few and many tokens a word.
+CASES = [(1, 1, 1, None), (1, 7, 3, None), (3, 4, 63, None), (5, 16, 64, 2), (17, 33, 65, 1), (64, 64, 1024, None),
+         (130, 40, 1003, 5), (2, 768, 50257, None), (96, 128, 4099, None), (33, 100, 16385, 3), (700, 20, 130, 1),
+         (1030, 65, 200, 3), (300, 1028, 77, 9)]
+
+
+@pytest.mark.parametrize("n,d,v,words", CASES)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_gives_the_cpu_bits(n, d, v, words, reduction):
+    x, w, t = case(n, d, v, seed=n + v, lean=3.0, ignored=range(1, n, 7), words=words)
+    up = torch.randn(n, generator=torch.Generator().manual_seed(1)) if reduction == "none" else None
+    got = results(x.cuda(), w.cuda(), t.cuda(), reduction, None if up is None else up.cuda())
+    assert_same(got, results(x, w, t, reduction, up))
+    check(got, x, w, t, reduction=reduction, up=up)
+
+
+@pytest.mark.parametrize("S", [1, 2, 3])
+def test_slices(S):
+    x, w, t = case(70, 50, 333, seed=S)
+    got = results(x.cuda(), w.cuda(), t.cuda(), "sum", slices=S)
+    assert_same(got, results(x, w, t, "sum", slices=S))
+    check(got, x, w, t, reduction="sum", S=S)
+
+
+def test_groups_of_tokens():
+    v = 2 ** 20 + 3
+    n = 2 * _lib.lib.rg_loss_group_tokens(v) + 5
+    x, w, t = case(n, 3, v, seed=2, std=1.0, words=40)
+    assert_same(results(x.cuda(), w.cuda(), t.cuda()), results(x, w, t))
+
+
+def test_parts_of_the_gradient_and_of_the_output():
+    x, w, t = case(200, 40, 500, seed=3)
+    want = results(x, w, t)
+    x, w, t = x.cuda(), w.cuda(), t.cuda()
+    leaf = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(rg.linear_cross_entropy(leaf, w, t), [leaf])
+    leaf = w.clone().requires_grad_()
+    (dw,) = torch.autograd.grad(rg.linear_cross_entropy(x, leaf, t), [leaf])
+    with torch.no_grad():
+        assert_same((rg.linear_cross_entropy(x, w, t), dx, dw), want)
+
+
+def test_tokens_that_do_not_count_and_no_tokens():
+    for reduction in ("mean", "sum", "none"):
+        x, w, t = case(40, 12, 90, seed=4)
+        t[::3], t[4], t[5] = -100, 90, -7
+        assert_same(results(x.cuda(), w.cuda(), t.cuda(), reduction), results(x, w, t, reduction))
+        t[:] = -100
+        assert_same(results(x.cuda(), w.cuda(), t.cuda(), reduction), results(x, w, t, reduction))
+        assert_same(results(x[:0].cuda(), w.cuda(), t[:0].cuda(), reduction), results(x[:0], w, t[:0], reduction))
+
+
+def test_non_finite_inputs_give_the_cpu_bits():
+    x, w, t = case(20, 12, 90, seed=4)
+    x[3, 2], x[7, 1], w[9, 9] = math.nan, math.inf, -math.inf
+    x[11], w[11] = 3e38, 3e38  # a logit past the range
+    got, want = results(x.cuda(), w.cuda(), t.cuda(), "none"), results(x, w, t, "none")
+    assert_same(got[:1], want[:1])
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_operands_off_16_bytes(shift):
+    x, w, t = case(50, 36, 200, seed=shift)
+
+    def moved(v):
+        flat = torch.empty(v.numel() + 8, device="cuda", dtype=v.dtype)
+        return flat[shift:shift + v.numel()].view(v.shape).copy_(v)
+
+    assert_same(results(moved(x), moved(w), moved(t)), results(x, w, t))
+
+
+def test_scaled_losses_and_second_backwards():
+    x, w, t = case(100, 30, 400, seed=6)
+    want = results(x, w, t, up=torch.tensor(0.3))
+    x, w, t = x.cuda().requires_grad_(), w.cuda().requires_grad_(), t.cuda()
+    loss = rg.linear_cross_entropy(x, w, t)
+    for _ in range(2):
+        got = torch.autograd.grad(loss, (x, w), torch.tensor(0.3, device="cuda"), retain_graph=True)
+        assert_same((loss, *got), want)
+
+
+def test_another_stream_and_graph_replays():
+    x, w, t = case(150, 64, 1000, seed=9)
+    want = results(x, w, t)
+    x, w, t = x.cuda(), w.cuda(), t.cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert_same(results(x, w, t), want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = results(x, w, t)
+    for k in range(3):
+        for v in got:
+            v.fill_(math.nan)
+        (torch.randn(1000, 1000, device="cuda") @ torch.randn(1000, 1000, device="cuda")).sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_same(got, want)
+
+
+def test_repeated_runs_give_the_same_bits():
+    x, w, t = case(1500, 96, 3000, seed=10, words=30)
+    x, w, t = x.cuda(), w.cuda(), t.cuda()
+    first = results(x, w, t)
+    for _ in range(5):
+        assert_same(results(x, w, t), first)
+
+
+def test_refuses_tensors_on_two_devices():
+    x, w, t = case(6, 8, 20, device="cuda")
+    for bad in ((x, w.cpu(), t), (x, w, t.cpu()), (x.cpu(), w, t)):
+        with pytest.raises(ValueError):
+            rg.linear_cross_entropy(*bad)

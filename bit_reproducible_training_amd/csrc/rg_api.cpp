@@ -458,6 +458,63 @@ GemmAddressing dense_addressing(const Layout& L) {
     return a;
 }
 
+static SliceDesc make_slice_desc(const float* src, int R, int K, int Rp, int Kp, bool strided, long long ld, int batch,
+                                 long long bstride, int nch, int kch, float* pm, void* out, int* expo) {
+    SliceDesc d;
+    d.src = src;
+    d.R = R;
+    d.K = K;
+    d.Rp = Rp;
+    d.Kp = Kp;
+    d.ld = ld;
+    d.batch = batch;
+    d.bstride = batch > 1 ? bstride : 0;
+    d.strided = strided ? 1 : 0;
+    const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && ld % 4 == 0 && d.bstride % 4 == 0;
+    d.vec = aligned && (strided ? (R % 4 == 0) : (K % 4 == 0)) ? 1 : 0;
+    d.nch = nch;
+    d.kch = kch;
+    d.pmax = pm;
+    d.out = out;
+    d.expo = expo;
+    d.im2col = 0;
+    std::memset(&d.g, 0, sizeof d.g);
+    d.nanrows = nullptr;
+    slice_grid(d);
+    d.spin_limit = slice_spin_limit();
+    pslice_grid(d);
+    return d;
+}
+
+size_t slice_scratch_bytes(int R, int K, bool strided) {
+    int nch, kch;
+    choose_chunks(R, R, K, strided, &nch, &kch);
+    const int Kp = round_up(K, STEP_K);
+    const int parts = pslice_route(strided, Kp) ? pslice_parts(strided, Kp) : 0;
+    return (size_t)std::max(nch, parts) * round_up(R, STEP_K) * sizeof(float);
+}
+
+int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
+                 hipStream_t stream) {
+    int nch, kch;
+    choose_chunks(R, R, K, strided, &nch, &kch);
+    const SliceDesc d = make_slice_desc(src, R, K, round_up(R, STEP_K), round_up(K, STEP_K), strided, strided ? R : K, 1,
+                                        0, nch, kch, scratch, out, expo);
+    SliceDesc none = d;
+    none.max_blocks = 0;
+    none.split_blocks = 0;
+    if (onepass_eligible(d)) {
+        launch_onepass(d, true, d, false, S, stream);
+    } else if (pslice_route(strided, d.Kp)) {
+        launch_mark(pslice_slots(d), MarkRange(), stream);
+        launch_pslice(d, true, d, false, S, stream);
+    } else {
+        launch_absmax(d, none, stream);
+        launch_split(d, none, S, false, stream);
+    }
+    return hipGetLastError();
+}
+
 int gemm_launch(const float* A, const float* B, float* C, const Layout& L, char* base,
                 hipStream_t stream, void* const* stage_events, const GemmOptions& opt,
                 const GemmAddressing& addr) {
@@ -487,31 +544,7 @@ int gemm_launch(const float* A, const float* B, float* C, const Layout& L, char*
 
     auto desc = [&](const float* src, int R, int Rp, bool strided, long long ld, long long bstride,
                     int nch, int kch, float* pm, void* out, int* expo) {
-        SliceDesc d;
-        d.src = src;
-        d.R = R;
-        d.K = L.K;
-        d.Rp = Rp;
-        d.Kp = L.Kp;
-        d.ld = ld;
-        d.batch = L.batch;
-        d.bstride = L.batch > 1 ? bstride : 0;
-        d.strided = strided ? 1 : 0;
-        const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && ld % 4 == 0 &&
-                             d.bstride % 4 == 0;
-        d.vec = aligned && (strided ? (R % 4 == 0) : (L.K % 4 == 0)) ? 1 : 0;
-        d.nch = nch;
-        d.kch = kch;
-        d.pmax = pm;
-        d.out = out;
-        d.expo = expo;
-        d.im2col = 0;
-        std::memset(&d.g, 0, sizeof d.g);
-        d.nanrows = nullptr;
-        slice_grid(d);
-        d.spin_limit = slice_spin_limit();
-        pslice_grid(d);
-        return d;
+        return make_slice_desc(src, R, L.K, Rp, L.Kp, strided, ld, L.batch, bstride, nch, kch, pm, out, expo);
     };
     SliceDesc da = desc(A, L.M, L.Mp, L.a_strided, addr.lda, addr.stride_a, L.nch_a,
                         L.kch_a, pma, qa, ea);

@@ -385,6 +385,13 @@ int gemm_launch(const float* A, const float* B, float* C, const Layout& L, char*
                 hipStream_t stream, void* const* events, const GemmOptions& opt,
                 const GemmAddressing& addr);
 
+// One operand's slicing by itself, for callers that keep its digits for several products: op(X) of R
+// rows of K values (row access, or column access with rows R apart) into panels of round_up(R, 64) by
+// round_up(K, 64) at `out` and exponents at `expo`; scratch of slice_scratch_bytes.
+size_t slice_scratch_bytes(int R, int K, bool strided);
+int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
+                 hipStream_t stream);
+
 // Kernel launchers (asynchronous on `stream`).
 void launch_absmax(const SliceDesc& a, const SliceDesc& b, hipStream_t stream);
 void launch_split(const SliceDesc& a, const SliceDesc& b, int S, bool int32_out, hipStream_t stream);

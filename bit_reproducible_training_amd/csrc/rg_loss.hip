@@ -3,10 +3,10 @@
 // Tokens are taken in groups (repro_loss::group_tokens), a group's logits z are one product, and its
 // gradient dz two more with them: three products in all, where pieces of the vocabulary, whose
 // softmax is not known before the last piece, need z a second time.
+#include "rg_digits.h"
 #include "rg_internal.h"
 #include "repro_loss.h"
 #include "repro_loss_math.h"
-#include "repro_sum.h"
 
 #include <algorithm>
 #include <cmath>
@@ -27,62 +27,54 @@ struct __attribute__((packed, aligned(4))) Four {
     float v[4];
 };
 
-// What is known of the targets before any product. word: the target, LEFT_OUT or INVALID. The tokens
-// of a word are listed together in ascending order, from place[first token of the word].
+// What is known of the targets before any product. word: the target, LEFT_OUT or INVALID. A word's
+// tokens are listed together from place[word], in ascending order in `list` and as they came in `arrived`.
 constexpr int LEFT_OUT = -1, INVALID = -2;
 struct Targets {
-    int* word;    // [N]
-    int* first;   // [N] the first token of its word
-    int* rank;    // [N] its word's tokens before it
-    int* count;   // [N] its word's tokens (where rank is 0)
-    int* place;   // [N] (where rank is 0)
-    int* list;    // [N]
-    int* used;    // places given out, tokens that count
+    int* word;     // [N]
+    int* slot;     // [N] the token's place among its word's as they came (which differs from run to run)
+    int* arrived;  // [N]
+    int* list;     // [N]
+    int* count;    // [V]
+    int* place;    // [V] (of words that occur)
+    int* counted;  // [1] tokens that are not left out
 };
 
-__global__ void loss_clear(int* used) { used[0] = used[1] = 0; }
-
-// A wavefront takes a token and compares its word with every token's, which the block's 16
-// wavefronts read through LDS together.
-constexpr int WORDS_THREADS = 1024, WORDS_TILE = 4096;
-__global__ void __launch_bounds__(WORDS_THREADS)
+// One block: the words' counts by atomics, then places for their tokens. A word's place and its tokens'
+// order in `arrived` change from run to run and reach no result: loss_tokens puts them in order. (Every
+// token compared with every other one took 170 us for 8192 tokens, and 64 times that for 65536.)
+__global__ void __launch_bounds__(1024)
 loss_words(const long long* __restrict__ target, long long ignore_index, int N, int V, Targets t) {
-    __shared__ int tile[WORDS_TILE];
-    const int lane = threadIdx.x & 63;
-    const int n = blockIdx.x * (WORDS_THREADS / 64) + (threadIdx.x >> 6);
-    const auto read = [&](int i) {
-        const long long v = target[i];
-        return v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
-    };
-    const int mine = n < N ? read(n) : LEFT_OUT;
-    int before = 0, all = 0, first = N;
-    for (int base = 0; base < N; base += WORDS_TILE) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < WORDS_TILE && base + i < N; i += WORDS_THREADS) tile[i] = read(base + i);
-        __syncthreads();
-        const int held = min(WORDS_TILE, N - base);
-        for (int i = lane; i < held; i += 64) {
-            const bool same = tile[i] == mine;
-            all += same;
-            before += same && base + i < n;
-            first = same ? min(first, base + i) : first;
+    __shared__ int places, kept;
+    if (threadIdx.x == 0) places = kept = 0;
+    for (int v = threadIdx.x; v < V; v += 1024) __hip_atomic_store(&t.count[v], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __threadfence();
+    __syncthreads();
+    int mine = 0;
+    for (int n = threadIdx.x; n < N; n += 1024) {
+        const long long v = target[n];
+        const int w = v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
+        t.word[n] = w;
+        mine += w != LEFT_OUT;
+        if (w >= 0) t.slot[n] = atomicAdd(&t.count[w], 1);
+    }
+    if (mine > 0) atomicAdd(&kept, mine);
+    __threadfence();
+    __syncthreads();
+    for (int n = threadIdx.x; n < N; n += 1024) {
+        const int w = t.word[n];
+        if (w >= 0 && t.slot[n] == 0) {
+            const int c = __hip_atomic_load(&t.count[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(&t.place[w], atomicAdd(&places, c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        all += __shfl_xor(all, off, 64);
-        before += __shfl_xor(before, off, 64);
-        first = min(first, __shfl_xor(first, off, 64));
+    __threadfence();
+    __syncthreads();
+    for (int n = threadIdx.x; n < N; n += 1024) {
+        const int w = t.word[n];
+        if (w >= 0) t.arrived[__hip_atomic_load(&t.place[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + t.slot[n]] = n;
     }
-    if (lane != 0 || n >= N) return;
-    t.word[n] = mine;
-    t.rank[n] = before;
-    t.first[n] = first;
-    if (mine >= 0 && before == 0) {
-        t.count[n] = all;
-        t.place[n] = atomicAdd(&t.used[0], all);  // which place a word gets changes no result
-    }
-    if (mine != LEFT_OUT) atomicAdd(&t.used[1], 1);
+    if (threadIdx.x == 0) t.counted[0] = kept;
 }
 
 template <int CTRL>
@@ -109,23 +101,18 @@ __device__ __forceinline__ float wave_sum(float v) {
     return row_sum16(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// The parts' largest logits and sums: a lane takes a chunk of 4 words, 16 lanes a part.
+// The parts' largest logits and sums: a lane takes a chunk of 4 words, 16 lanes a part. Rows of z are ldz
+// apart, a multiple of 32.
 __global__ void __launch_bounds__(256)
-loss_parts(const float* __restrict__ z, int V, int parts, float2* __restrict__ out) {
+loss_parts(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ out) {
     const int row = blockIdx.y;
     const int part = blockIdx.x * 16 + (threadIdx.x >> 4);
     if (part >= parts) return;  // uniform over a part's 16 lanes
     const int at = part * PART + 4 * (threadIdx.x & 15);
-    const float* q = z + (size_t)row * V;
-    float v[4];
-    if (at + 4 <= V) {
-        const Four f = *reinterpret_cast<const Four*>(q + at);
+    const float4 f = at < V ? *reinterpret_cast<const float4*>(z + (size_t)row * ldz + at) : make_float4(0, 0, 0, 0);
+    float v[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = f.v[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = at + i < V ? q[at + i] : -INFINITY;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
     const float a = row_max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = at + i < V ? exp_nonpositive(v[i] - a) : 0.0f;
@@ -133,112 +120,312 @@ loss_parts(const float* __restrict__ z, int V, int parts, float2* __restrict__ o
     if ((threadIdx.x & 15) == 0) out[(size_t)row * parts + part] = make_float2(a, b);
 }
 
-// A token from its parts (a wavefront each), and its place in its word's list.
+__device__ __forceinline__ float wave_fmax(float m) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    return m;
+}
+
+// A token from its parts (a wavefront each), its place among its word's, and the exponent of its row of
+// dz: that of the largest of the words other than the target (exp_nonpositive never falls).
 __global__ void __launch_bounds__(256)
-loss_tokens(const float* __restrict__ z, int V, int parts, const float2* __restrict__ part, int first, int rows,
-            Targets t, const float* __restrict__ factors, int mean, Token* __restrict__ tokens,
-            float* __restrict__ losses) {
+loss_tokens(const float* __restrict__ z, int ldz, int V, int parts, const float2* __restrict__ part, int first,
+            int rows, Targets t, const float* __restrict__ factors, int mean, Token* __restrict__ tokens,
+            int* __restrict__ exponents) {
     const int lane = threadIdx.x & 63;
     const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= rows) return;
     const int n = first + r, word = t.word[n];
     Token k = repro_loss::ignored_token();
+    int exponent = 0;
     if (word >= 0) {
         const float2* p = part + (size_t)r * parts;
-        float m = -INFINITY;
-        for (int i = lane; i < parts; i += 64) m = fmaxf(m, p[i].x);
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        const float* q = z + (size_t)r * ldz;
+        const int own = word / PART;
+        float m = -INFINITY, other = -INFINITY;  // other: without the target's part
+        for (int i = lane; i < parts; i += 64) {
+            const float a = p[i].x;
+            m = fmaxf(m, a);
+            other = fmaxf(other, i == own ? -INFINITY : a);
+        }
+        const int beside = own * PART + lane;
+        if (beside < V && beside != word) other = fmaxf(other, q[beside]);
+        m = wave_fmax(m);
+        other = wave_fmax(other);
         float s = 0.0f;
         for (int i = lane; i < parts; i += 64) s = s + p[i].y * exp_nonpositive(p[i].x - m);
         s = wave_sum(s);
-        const float g = factors ? factors[n] : mean ? 1.0f / (float)t.used[1] : 1.0f;
-        k = repro_loss::finish_token(m, s, z[(size_t)r * V + word], g);
-        if (lane == 0) t.list[t.place[t.first[n]] + t.rank[n]] = n;
+        const float g = factors ? factors[n] : mean ? 1.0f / (float)t.counted[0] : 1.0f;
+        k = repro_loss::finish_token(m, s, q[word], g);
+        const float top = fabsf(exp_nonpositive(other - k.top) * k.factor);
+        exponent = repro_gemm::scale_exponent(top);  // 0 for a NaN
+        const int place = t.place[word], count = t.count[word];
+        int before = 0;
+        for (int i = lane; i < count; i += 64) before += t.arrived[place + i] < n;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
+        if (lane == 0) t.list[place + before] = n;
     } else if (word == INVALID) {
         k.loss = NAN;
     }
     if (lane == 0) {
         tokens[n] = k;
-        losses[n] = k.loss;
+        exponents[r] = exponent;
     }
 }
 
-// z becomes its gradient, without the target words' share.
-__global__ void __launch_bounds__(256)
-loss_gradient(float* __restrict__ z, int V, int first, const Token* __restrict__ tokens, const int* __restrict__ words) {
-    const int row = blockIdx.y;
-    const Token k = tokens[first + row];
-    const int word = words[first + row];
-    float* q = z + (size_t)row * V;
-    const int at = 4 * (blockIdx.x * 256 + threadIdx.x);
-    if (at >= V) return;
-    Four f;
+// ---- dz, as the digits that the two products with it read ----
+//
+// A block takes WORDS words over all of a group's tokens and keeps dz there in registers, so z is
+// read once: the words' largest magnitudes, and with them the digits of dz^T for dw, come from there as
+// well as the digits of dz for dx, whose tokens' exponents are known. A thread's 4 tokens x 4 words are
+// packed along the words and along the tokens; four lanes exchange them into 16-byte pieces of a panel,
+// so that a wavefront's stores are whole runs of 1 KiB (rows) and 256 bytes (columns).
+// Lane bits 0, 1: q, the words 4 q ..; 2, 3: j, the tokens 16 j ..; 4, 5: i, the tokens 16 j + 4 i ..
+constexpr int WORDS = 16, DIGIT_THREADS = 512, STEP_TOKENS = DIGIT_THREADS;  // 64 tokens a wavefront
+
+template <int CTRL>
+__device__ __forceinline__ int lane_swapped(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
+}
+// d[k] of lane q becomes d[q] of lane k, among lanes 4 n .. 4 n + 3
+__device__ __forceinline__ void transpose_quad(int (&d)[4], int lane) {
+    const bool odd = lane & 1, high = lane & 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float v = at + i < V ? q[at + i] : 0.0f;
-        f.v[i] = word < 0 || at + i == word ? 0.0f : exp_nonpositive(v - k.top) * k.factor;
+    for (int k = 0; k < 4; k += 2) {
+        const int got = lane_swapped<0xB1>(odd ? d[k] : d[k + 1]);
+        d[k] = odd ? got : d[k];
+        d[k + 1] = odd ? d[k + 1] : got;
     }
-    if (at + 4 <= V) *reinterpret_cast<Four*>(q + at) = f;
-    else
-        for (int i = 0; i < 4; ++i)
-            if (at + i < V) q[at + i] = f.v[i];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int got = lane_swapped<0x4E>(high ? d[k] : d[k + 2]);
+        d[k] = high ? got : d[k];
+        d[k + 2] = high ? d[k + 2] : got;
+    }
+}
+// d[c] of row i of 16 lanes becomes d[i] of row c
+__device__ __forceinline__ void transpose_rows(int (&d)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; k += 2) {
+        const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)d[k], (uint32_t)d[k + 1], false, false);
+        d[k] = (int)s[0];
+        d[k + 1] = (int)s[1];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const auto s = __builtin_amdgcn_permlane32_swap((uint32_t)d[k], (uint32_t)d[k + 2], false, false);
+        d[k] = (int)s[0];
+        d[k + 2] = (int)s[1];
+    }
 }
 
-// The target words' share of dx.
+struct DigitsOut {
+    int8_t* by_token;     // op(A) of dx: rows tokens, k words; null where not wanted
+    size_t token_bytes;   // of a panel of 32 tokens over all words
+    int8_t* by_word;      // op(A) of dw: rows words, k tokens; null where not wanted
+    size_t word_bytes;
+    int* word_exponents;  // [V]
+    int padded;           // the group's tokens, padded as dw's k
+};
+
+template <int S, int STEPS>
+__global__ void __launch_bounds__(DIGIT_THREADS, 4)
+loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, const Token* __restrict__ tokens,
+            const int* __restrict__ words, const int* __restrict__ exponents, DigitsOut out) {
+    __shared__ uint32_t tops[DIGIT_THREADS / 64][WORDS];
+    // Neighbouring blocks of words, which share cache lines, run on one XCD (workgroup i on XCD i mod 8).
+    const int whole = gridDim.x / 16 * 16, id = blockIdx.x;
+    const int block = id < whole ? id / 16 * 16 + id % 8 * 2 + id / 8 % 2 : id;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int q = lane & 3, i = lane >> 4, j = (lane >> 2) & 3;
+    const int v0 = block * WORDS, v = v0 + 4 * q;
+    const int base = wave * 64 + 16 * j + 4 * i;  // + STEP_TOKENS * step
+    float d[STEPS][4][4];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = s * STEP_TOKENS + base + k;
+            const float4 f = r < rows ? *reinterpret_cast<const float4*>(z + (size_t)r * ldz + v) : make_float4(0, 0, 0, 0);
+            d[s][k][0] = f.x, d[s][k][1] = f.y, d[s][k][2] = f.z, d[s][k][3] = f.w;
+        }
+    uint32_t top[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = s * STEP_TOKENS + base + k;
+            int word = LEFT_OUT;
+            float2 t = make_float2(0.0f, 0.0f);
+            if (r < rows) {
+                word = words[first + r];
+                t = *reinterpret_cast<const float2*>(&tokens[first + r]);  // top, factor
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float e = exp_nonpositive(d[s][k][c] - t.x) * t.y;
+                d[s][k][c] = word < 0 || v + c == word ? 0.0f : e;
+                top[c] = max(top[c], repro_gemm::magnitude_key(d[s][k][c]));
+            }
+        }
+    if (out.by_word != nullptr) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int off = 4; off < 64; off <<= 1) top[c] = max(top[c], (uint32_t)__shfl_xor((int)top[c], off, 64));
+            if (lane < 4) tops[wave][4 * q + c] = top[c];
+        }
+        __syncthreads();
+        RowScale scale[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int w = 0; w < DIGIT_THREADS / 64; ++w) m = max(m, tops[w][4 * q + c]);
+            const int e = repro_gemm::scale_exponent(__uint_as_float(m));
+            scale[c] = row_scale<S>(e);
+            if (threadIdx.x < 4 && v + c < V) out.word_exponents[v + c] = e;
+        }
+        const int mine = v0 + 4 * q + i;  // the word whose pieces this lane stores
+        int8_t* to = out.by_word + (size_t)(mine >> 5) * out.word_bytes + (mine & 31) * 16;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int t0 = s * STEP_TOKENS + wave * 64;
+            if (t0 >= out.padded) continue;
+            v4i w[S];  // w[p][c]: digit p of word c's four tokens
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int x[4] = {round_fixed(d[s][0][c], scale[c]), round_fixed(d[s][1][c], scale[c]),
+                                  round_fixed(d[s][2][c], scale[c]), round_fixed(d[s][3][c], scale[c])};
+                pack_word<S>(x, w, c);
+            }
+            const int k0 = t0 + 16 * j;
+#pragma unroll
+            for (int p = 0; p < S; ++p) {
+                int a[4] = {w[p][0], w[p][1], w[p][2], w[p][3]};
+                transpose_rows(a);
+                *reinterpret_cast<v4i*>(to + ((size_t)(k0 >> 5) * S + p) * PANEL_BYTES + (k0 & 16) * 32) = v4i{a[0], a[1], a[2], a[3]};
+            }
+        }
+    }
+    if (out.by_token != nullptr) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int t0 = s * STEP_TOKENS + wave * 64;
+            if (t0 >= rows) continue;
+            v4i w[S];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int r = s * STEP_TOKENS + base + k;
+                const RowScale scale = row_scale<S>(r < rows ? exponents[r] : 0);
+                const int x[4] = {round_fixed(d[s][k][0], scale), round_fixed(d[s][k][1], scale),
+                                  round_fixed(d[s][k][2], scale), round_fixed(d[s][k][3], scale)};
+                pack_word<S>(x, w, k);
+            }
+            const int r = s * STEP_TOKENS + base + q;  // the token whose piece this lane stores
+            int8_t* to = out.by_token + (size_t)(r >> 5) * out.token_bytes + (size_t)(v0 >> 5) * (S * PANEL_BYTES) +
+                         (r & 31) * 16 + (v0 & 16) * 32;
+#pragma unroll
+            for (int p = 0; p < S; ++p) {
+                int a[4] = {w[p][0], w[p][1], w[p][2], w[p][3]};
+                transpose_quad(a, lane);
+                *reinterpret_cast<v4i*>(to + p * PANEL_BYTES) = v4i{a[0], a[1], a[2], a[3]};
+            }
+        }
+    }
+}
+
+// ---- the target words' share ----
+//
+// Blocks below N take dw (a word each, at its first token; a wavefront 256 columns at a time), the
+// others dx (a token each). A word's tokens are read 64 at a time by the lanes, which then know
+// the rows of x to load, 16 at once.
 __global__ void __launch_bounds__(256)
-loss_target_dx(float* __restrict__ dx, const float* __restrict__ w, int D, const Token* __restrict__ tokens,
-               const int* __restrict__ words, int N) {
-    for (int n = blockIdx.x; n < N; n += gridDim.x) {
-        const int word = words[n];
-        if (word < 0) continue;
+loss_target(float* __restrict__ dx, float* __restrict__ dw, const float* __restrict__ x, const float* __restrict__ w,
+            int D, const Token* __restrict__ tokens, Targets t, int N) {
+    const int lane = threadIdx.x & 63;
+    int n = blockIdx.x;
+    if (dw == nullptr || n >= N) {
+        n = dw == nullptr ? n : n - N;
+        const int word = t.word[n];
+        if (word < 0) return;
         const float c = tokens[n].target;
         const float* q = w + (size_t)word * D;
         float* o = dx + (size_t)n * D;
         for (int i = threadIdx.x; i < D; i += 256) o[i] = o[i] + c * q[i];
+        return;
     }
-}
-
-// The target words' share of dw: a block takes a word (at its first token), a wavefront 256 columns
-// at a time, 16 of the word's tokens in flight.
-__global__ void __launch_bounds__(256)
-loss_target_dw(float* __restrict__ dw, const float* __restrict__ x, int D, const Token* __restrict__ tokens, Targets t,
-               int N) {
-    const int n = blockIdx.x, word = t.word[n];
-    if (word < 0 || t.rank[n] != 0) return;
-    const int count = t.count[n];
-    const int* list = t.list + t.place[n];
-    const int lane = threadIdx.x & 63;
+    const int word = t.word[n];
+    if (word < 0) return;
+    const int count = t.count[word];
+    const int* list = t.list + t.place[word];
+    if (list[0] != n) return;
     for (int base = 256 * (threadIdx.x >> 6); base < D; base += 1024) {
         const int at = base + 4 * lane;
+        const bool full = at + 4 <= D;
         float s[16][4];
 #pragma unroll
         for (int h = 0; h < 16; ++h)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[h][i] = 0.0f;
-        for (int k0 = 0; k0 < count; k0 += 16) {
+            for (int k = 0; k < 4; ++k) s[h][k] = 0.0f;
+        for (int k0 = 0; k0 < count; k0 += 64) {
+            int m = 0;
+            float c = 0.0f;
+            if (k0 + lane < count) {
+                m = list[k0 + lane];
+                c = tokens[m].target;
+            }
+            const int held = min(64, count - k0);
+            for (int b = 0; b < held; b += 16) {
 #pragma unroll
-            for (int h = 0; h < 16; ++h) {
-                if (k0 + h >= count) break;
-                const int m = list[k0 + h];
-                const float c = tokens[m].target;
-                const float* q = x + (size_t)m * D;
+                for (int h = 0; h < 16; ++h) {
+                    if (b + h >= held) break;
+                    const float* q = x + (size_t)__builtin_amdgcn_readlane(m, b + h) * D + at;
+                    const float ch = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), b + h));
+                    if (full) {
+                        const Four f = *reinterpret_cast<const Four*>(q);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (at + i < D) s[h][i] = s[h][i] + c * q[at + i];
+                        for (int k = 0; k < 4; ++k) s[h][k] = s[h][k] + ch * f.v[k];
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (at + k < D) s[h][k] = s[h][k] + ch * q[k];
+                    }
+                }
             }
         }
 #pragma unroll
         for (int h = 8; h > 0; h /= 2)
 #pragma unroll
-            for (int k = 0; k < h; ++k)
+            for (int a = 0; a < h; ++a)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[k][i] = s[k][i] + s[k + h][i];
-        float* o = dw + (size_t)word * D;
+                for (int k = 0; k < 4; ++k) s[a][k] = s[a][k] + s[a + h][k];
+        float* o = dw + (size_t)word * D + at;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (at + i < D) o[at + i] = o[at + i] + s[0][i];
+        for (int k = 0; k < 4; ++k)
+            if (at + k < D) o[k] = o[k] + s[0][k];
     }
+}
+
+// The losses, or their sum or mean (one block).
+__global__ void __launch_bounds__(1024)
+loss_reduce(const Token* __restrict__ tokens, int N, int reduction, const int* __restrict__ counted, float* __restrict__ loss) {
+    static_assert(repro_loss::STRANDS == 1024, "a thread a strand");
+    if (reduction == RG_LOSS_NONE) {
+        for (int n = blockIdx.x * 1024 + threadIdx.x; n < N; n += gridDim.x * 1024) loss[n] = tokens[n].loss;
+        return;
+    }
+    __shared__ double lds[1024];
+    double s = 0.0;
+#pragma unroll 8
+    for (int n = threadIdx.x; n < N; n += 1024) s = s + (double)tokens[n].loss;
+    lds[threadIdx.x] = s;
+    for (int h = 512; h > 0; h /= 2) {
+        __syncthreads();
+        if ((int)threadIdx.x < h) lds[threadIdx.x] = lds[threadIdx.x] + lds[threadIdx.x + h];
+    }
+    if (threadIdx.x == 0) loss[0] = (float)(reduction == RG_LOSS_MEAN ? lds[0] / (double)counted[0] : lds[0]);
 }
 
 __global__ void __launch_bounds__(256) loss_add(float* __restrict__ a, const float* __restrict__ b, size_t n) {
@@ -252,75 +439,108 @@ __global__ void __launch_bounds__(256) scale_kernel(float* __restrict__ a, const
     if (f == 1.0f) return;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) a[i] = a[i] * f;
 }
-__global__ void loss_mean(float* loss, const int* used) { loss[0] = loss[0] / (float)used[1]; }
 
 unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 1u << 20); }
 
 bool sizes_ok(const rg_loss_config* c) {
-    return c && c->N >= 0 && c->N <= 2147483647ll && c->D >= 1 && c->V >= 1 && c->slices >= 1 && c->slices <= 3 &&
+    return c && c->N >= 0 && c->N <= RG_LOSS_MAX_TOKENS && c->D >= 1 && c->D <= RG_LOSS_MAX_WORDS && c->V >= 1 &&
+           c->V <= RG_LOSS_MAX_WORDS && c->slices >= 1 && c->slices <= 3 &&
            c->reduction >= RG_LOSS_MEAN && c->reduction <= RG_LOSS_NONE;
 }
 
-rg_config product(int slices, bool ta, bool tb) {
-    rg_config g;
-    rg_config_init(&g);
-    g.slices = slices;
-    g.trans_a = ta;
-    g.trans_b = tb;
-    return g;
+int round_up(int x, int m) { return (x + m - 1) / m * m; }
+
+// A product from digits that are in memory: the tile plan (no kernel that slices by itself).
+int plan_product(int M, int N, int K, int S, Layout* L) {
+    rg_config c;
+    rg_config_init(&c);
+    c.slices = S;
+    PlanExtras extras;
+    extras.one_launch = false;
+    return layout_for_current_device(M, N, K, &c, L, extras);
 }
 
-// Where everything lies in the workspace.
+struct Digits {
+    size_t q, e;  // offsets of the panels and exponents
+};
+
+// Where everything lies in the workspace, and the products of a whole group [0] and of the last [1].
 struct Space {
-    int group, parts;
-    size_t words, tokens, losses, part, z, dw, gemm, sum, gemm_bytes, sum_bytes, total;
+    int group, last, parts, ldz;
+    Layout z[2], dx[2], dw[2];
+    Digits x_rows, w_rows, w_cols, x_cols, by_token, by_word;
+    size_t words, tokens, part, logits, more, partial, scratch, total;
 };
 
 int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
-    const size_t N = (size_t)c->N;
-    s->group = (int)std::min<long long>(repro_loss::group_tokens(c->V), c->N);
-    s->parts = (c->V + PART - 1) / PART;
-    size_t at = 0;
+    const int N = (int)c->N, D = c->D, V = c->V, S = c->slices;
+    s->group = std::min(repro_loss::group_tokens(V), N);
+    s->last = (N - 1) % s->group + 1;
+    s->parts = (V + PART - 1) / PART;
+    s->ldz = round_up(V, 32);
+    // Rows past a matrix's own that a tile may read: their products are not stored.
+    constexpr int BEYOND = 192;
+    size_t at = 0, partial = 0, scratch = 0;
     const auto take = [&](size_t bytes) {
         const size_t here = at;
         at += align_up(bytes);
         return here;
     };
-    s->words = take((6 * N + 2) * sizeof(int));
-    s->tokens = take(N * sizeof(Token));
-    s->losses = take(N * sizeof(float));
-    s->part = take((size_t)s->group * s->parts * sizeof(float2));
-    s->z = take((size_t)s->group * c->V * sizeof(float));
-    s->dw = take(dw && c->N > s->group ? (size_t)c->V * c->D * sizeof(float) : 0);
-    s->gemm_bytes = s->sum_bytes = 0;
-    const auto need = [&](int M, int N_, int K, bool ta, bool tb) {
-        const rg_config g = product(c->slices, ta, tb);
-        rg_plan p;
-        const int rc = rg_make_plan(M, N_, K, &g, &p);
-        if (rc == hipSuccess) s->gemm_bytes = std::max(s->gemm_bytes, p.workspace_bytes);
-        return rc;
+    const auto digits = [&](int rows, int K) {
+        Digits d;
+        d.q = take((size_t)(round_up(rows, 64) + BEYOND) * round_up(K, STEP_K) * S);
+        d.e = take((size_t)(round_up(rows, 64) + BEYOND) * sizeof(int));
+        return d;
     };
-    // a whole group and the last one
-    for (const int rows : {s->group, c->N > 0 ? (int)((c->N - 1) % s->group) + 1 : 0}) {
-        if (rows == 0) continue;
-        int rc = need(rows, c->V, c->D, false, true);
-        if (rc == hipSuccess && dx) rc = need(rows, c->D, c->V, false, false);
-        if (rc == hipSuccess && dw) rc = need(c->V, c->D, rows, true, false);
+    for (int k = 0; k < 2; ++k) {
+        const int rows = k ? s->last : s->group;
+        int rc = plan_product(rows, V, D, S, &s->z[k]);
+        if (rc == hipSuccess && dx) rc = plan_product(rows, D, V, S, &s->dx[k]);
+        if (rc == hipSuccess && dw) rc = plan_product(V, D, rows, S, &s->dw[k]);
         if (rc != hipSuccess) return rc;
+        for (const Layout* L : {&s->z[k], dx ? &s->dx[k] : nullptr, dw ? &s->dw[k] : nullptr})
+            if (L && L->has_partial) partial = std::max(partial, (size_t)L->split * L->M * L->N * sizeof(int64_t));
     }
-    s->gemm = take(s->gemm_bytes);
-    if (c->N > 0 && c->reduction != RG_LOSS_NONE) {
-        rg_sum_config sc;
-        rg_sum_config_init(&sc);
-        rg_sum_plan p;
-        const int rc = rg_make_sum_plan(1, 1, (int)c->N, &sc, &p);
-        if (rc != hipSuccess) return rc;
-        s->sum_bytes = p.workspace_bytes;
+    s->words = take(((size_t)4 * N + 2 * (size_t)V + 1) * sizeof(int));
+    s->tokens = take((size_t)N * sizeof(Token));
+    s->part = take((size_t)s->group * s->parts * sizeof(float2));
+    s->logits = take((size_t)s->group * s->ldz * sizeof(float));
+    s->x_rows = digits(N, D);
+    s->w_rows = digits(V, D);
+    scratch = std::max(slice_scratch_bytes(N, D, false), slice_scratch_bytes(V, D, false));
+    if (dx) {
+        s->w_cols = digits(D, V);
+        scratch = std::max(scratch, slice_scratch_bytes(D, V, true));
     }
-    s->sum = take(s->sum_bytes);
+    s->by_token = digits(s->group, dx ? V : 0);
+    if (dw) {
+        s->x_cols = digits(D, s->group);
+        scratch = std::max({scratch, slice_scratch_bytes(D, s->group, true), slice_scratch_bytes(D, s->last, true)});
+        s->by_word = digits(V, s->group);
+    }
+    s->more = take(dw && N > s->group ? (size_t)V * D * sizeof(float) : 0);
+    s->partial = take(partial);
+    s->scratch = take(scratch);
     s->total = at;
     return hipSuccess;
 }
+
+// C (rows ldc apart) = the product of two operands' digits.
+void launch_product(const Layout& L, const int8_t* qa, const int* ea, const int8_t* qb, const int* eb, float* C,
+                    long long ldc, int64_t* partial, hipStream_t st) {
+    const OutAddr out{ldc, 0, nullptr};
+    launch_contract_mfma(L, qa, qb, ea, eb, C, out, L.has_partial ? partial : nullptr, st);
+    if (L.has_partial) launch_reduce_round(L, partial, ea, eb, C, out, st);
+}
+
+template <int S>
+void launch_digits_s(int V, int rows, hipStream_t st, const float* z, int ldz, int first, const Token* tokens,
+                     const int* words, const int* exponents, const DigitsOut& out) {
+    const dim3 grid((V + WORDS - 1) / WORDS), block(DIGIT_THREADS);
+    auto kernel = rows <= STEP_TOKENS ? loss_digits<S, 1> : rows <= 2 * STEP_TOKENS ? loss_digits<S, 2> : loss_digits<S, 4>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, st, z, ldz, V, first, rows, tokens, words, exponents, out);
+}
+static_assert(repro_loss::MAX_GROUP <= 4 * STEP_TOKENS, "a block holds a group's tokens");
 
 }  // namespace
 }  // namespace rg
@@ -340,6 +560,8 @@ int rg_loss_group_tokens(int V) { return V < 1 ? 0 : repro_loss::group_tokens(V)
 
 int rg_linear_cross_entropy_workspace(const rg_loss_config* cfg, int want_dx, int want_dw, size_t* bytes) {
     if (!rg::sizes_ok(cfg) || !bytes) return hipErrorInvalidValue;
+    *bytes = 0;
+    if (cfg->N == 0) return hipSuccess;
     rg::Space s;
     const int rc = rg::plan_space(cfg, want_dx != 0, want_dw != 0, &s);
     if (rc == hipSuccess) *bytes = s.total;
@@ -355,12 +577,12 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     if (off(x, 4) || off(w, 4) || off(target, 8) || off(factors, 4) || off(loss, 4) || off(dx, 4) || off(dw, 4))
         return hipErrorInvalidValue;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int D = cfg->D, V = cfg->V, N = (int)cfg->N;
-    const auto fill = [&](float* p, float v, size_t n) {
-        if (p) hipLaunchKernelGGL(loss_fill, dim3(grid_of(n)), dim3(256), 0, st, p, v, n);
-    };
+    const int D = cfg->D, V = cfg->V, N = (int)cfg->N, S = cfg->slices;
     if (N == 0) {
         if (!dw && (!loss || cfg->reduction == RG_LOSS_NONE)) return hipSuccess;
+        const auto fill = [&](float* p, float v, size_t n) {
+            if (p) hipLaunchKernelGGL(loss_fill, dim3(grid_of(n)), dim3(256), 0, st, p, v, n);
+        };
         if (cfg->reduction != RG_LOSS_NONE) fill(loss, cfg->reduction == RG_LOSS_MEAN ? NAN : 0.0f, 1);
         fill(dw, 0.0f, (size_t)V * D);
         return hipGetLastError();
@@ -369,59 +591,66 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     Space s;
     int rc = plan_space(cfg, dx != nullptr, dw != nullptr, &s);
     if (rc != hipSuccess) return rc;
-    if (!workspace || off(workspace, 16) || workspace_bytes < s.total) return hipErrorInvalidValue;
+    if (!workspace || off(workspace, 256) || workspace_bytes < s.total) return hipErrorInvalidValue;
     char* base = static_cast<char*>(workspace);
+    const auto panels = [&](const Digits& d) { return reinterpret_cast<int8_t*>(base + d.q); };
+    const auto exponents = [&](const Digits& d) { return reinterpret_cast<int*>(base + d.e); };
     Targets t;
     t.word = reinterpret_cast<int*>(base + s.words);
-    t.first = t.word + N;
-    t.rank = t.first + N;
-    t.count = t.rank + N;
-    t.place = t.count + N;
-    t.list = t.place + N;
-    t.used = t.list + N;
+    t.slot = t.word + N;
+    t.arrived = t.slot + N;
+    t.list = t.arrived + N;
+    t.count = t.list + N;
+    t.place = t.count + V;
+    t.counted = t.place + V;
     Token* tokens = reinterpret_cast<Token*>(base + s.tokens);
-    float* losses = reinterpret_cast<float*>(base + s.losses);
     float2* part = reinterpret_cast<float2*>(base + s.part);
-    float* z = reinterpret_cast<float*>(base + s.z);
-    float* more = reinterpret_cast<float*>(base + s.dw);
-    hipLaunchKernelGGL(loss_clear, dim3(1), dim3(1), 0, st, t.used);
-    hipLaunchKernelGGL(loss_words, dim3((N + 15) / 16), dim3(WORDS_THREADS), 0, st, target, cfg->ignore_index, N, V, t);
+    float* z = reinterpret_cast<float*>(base + s.logits);
+    float* more = reinterpret_cast<float*>(base + s.more);
+    int64_t* partial = reinterpret_cast<int64_t*>(base + s.partial);
+    float* scratch = reinterpret_cast<float*>(base + s.scratch);
+
+    hipLaunchKernelGGL(loss_words, dim3(1), dim3(1024), 0, st, target, cfg->ignore_index, N, V, t);
+    // The digits that every group's products share.
+    rc = launch_slice(x, N, D, false, S, panels(s.x_rows), exponents(s.x_rows), scratch, st);
+    if (rc == hipSuccess) rc = launch_slice(w, V, D, false, S, panels(s.w_rows), exponents(s.w_rows), scratch, st);
+    if (rc == hipSuccess && dx) rc = launch_slice(w, D, V, true, S, panels(s.w_cols), exponents(s.w_cols), scratch, st);
+    if (rc != hipSuccess) return rc;
     for (int first = 0; first < N; first += s.group) {
-        const int rows = std::min(s.group, N - first);
-        const float* xg = x + (size_t)first * D;
-        rg_config g = product(cfg->slices, false, true);
-        rc = rg_gemm_fp32_ws(xg, w, z, rows, V, D, &g, base + s.gemm, s.gemm_bytes, st, nullptr);
-        if (rc != hipSuccess) return rc;
-        hipLaunchKernelGGL(loss_parts, dim3((s.parts + 15) / 16, rows), dim3(256), 0, st, z, V, s.parts, part);
-        hipLaunchKernelGGL(loss_tokens, dim3((rows + 3) / 4), dim3(256), 0, st, z, V, s.parts, part, first, rows, t,
-                           factors, cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, losses);
-        if (dx || dw)
-            hipLaunchKernelGGL(loss_gradient, dim3((V + 1023) / 1024, rows), dim3(256), 0, st, z, V, first, tokens, t.word);
-        if (dx) {
-            g = product(cfg->slices, false, false);
-            rc = rg_gemm_fp32_ws(z, w, dx + (size_t)first * D, rows, D, V, &g, base + s.gemm, s.gemm_bytes, st, nullptr);
-            if (rc != hipSuccess) return rc;
-        }
+        const int rows = std::min(s.group, N - first), k = first + s.group < N ? 0 : 1;
+        launch_product(s.z[k], panels(s.x_rows) + (size_t)first * round_up(D, STEP_K) * S, exponents(s.x_rows) + first,
+                       panels(s.w_rows), exponents(s.w_rows), z, s.ldz, partial, st);
+        hipLaunchKernelGGL(loss_parts, dim3((s.parts + 15) / 16, rows), dim3(256), 0, st, z, s.ldz, V, s.parts, part);
+        hipLaunchKernelGGL(loss_tokens, dim3((rows + 3) / 4), dim3(256), 0, st, z, s.ldz, V, s.parts, part, first, rows,
+                           t, factors, cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, exponents(s.by_token));
+        if (!dx && !dw) continue;
+        DigitsOut out;
+        out.by_token = dx ? panels(s.by_token) : nullptr;
+        out.token_bytes = (size_t)round_up(V, STEP_K) * S * PANEL_ROWS;
+        out.padded = round_up(rows, STEP_K);
+        out.by_word = dw ? panels(s.by_word) : nullptr;
+        out.word_bytes = (size_t)out.padded * S * PANEL_ROWS;
+        out.word_exponents = dw ? exponents(s.by_word) : nullptr;
+        if (S == 1) launch_digits_s<1>(V, rows, st, z, s.ldz, first, tokens, t.word, exponents(s.by_token), out);
+        else if (S == 2) launch_digits_s<2>(V, rows, st, z, s.ldz, first, tokens, t.word, exponents(s.by_token), out);
+        else launch_digits_s<3>(V, rows, st, z, s.ldz, first, tokens, t.word, exponents(s.by_token), out);
+        if (dx)
+            launch_product(s.dx[k], panels(s.by_token), exponents(s.by_token), panels(s.w_cols), exponents(s.w_cols),
+                           dx + (size_t)first * D, D, partial, st);
         if (dw) {
-            g = product(cfg->slices, true, false);
-            rc = rg_gemm_fp32_ws(z, xg, first == 0 ? dw : more, V, D, rows, &g, base + s.gemm, s.gemm_bytes, st, nullptr);
+            rc = launch_slice(x + (size_t)first * D, D, rows, true, S, panels(s.x_cols), exponents(s.x_cols), scratch, st);
             if (rc != hipSuccess) return rc;
+            launch_product(s.dw[k], panels(s.by_word), exponents(s.by_word), panels(s.x_cols), exponents(s.x_cols),
+                           first == 0 ? dw : more, D, partial, st);
             const size_t n = (size_t)V * D;
             if (first > 0) hipLaunchKernelGGL(loss_add, dim3(grid_of(n)), dim3(256), 0, st, dw, more, n);
         }
     }
-    if (dx) hipLaunchKernelGGL(loss_target_dx, dim3(std::min(N, 1 << 20)), dim3(256), 0, st, dx, w, D, tokens, t.word, N);
-    if (dw) hipLaunchKernelGGL(loss_target_dw, dim3(N), dim3(256), 0, st, dw, x, D, tokens, t, N);
-    if (loss && cfg->reduction == RG_LOSS_NONE) {
-        rc = hipMemcpyAsync(loss, losses, (size_t)N * sizeof(float), hipMemcpyDeviceToDevice, st);
-        if (rc != hipSuccess) return rc;
-    } else if (loss) {
-        rg_sum_config sc;
-        rg_sum_config_init(&sc);
-        rc = rg_sum_fp32_ws(losses, loss, 1, 1, N, &sc, base + s.sum, s.sum_bytes, st);
-        if (rc != hipSuccess) return rc;
-        if (cfg->reduction == RG_LOSS_MEAN) hipLaunchKernelGGL(loss_mean, dim3(1), dim3(1), 0, st, loss, t.used);
-    }
+    if (dx || dw)
+        hipLaunchKernelGGL(loss_target, dim3((dx ? N : 0) + (dw ? N : 0)), dim3(256), 0, st, dx, dw, x, w, D, tokens, t, N);
+    if (loss)
+        hipLaunchKernelGGL(loss_reduce, dim3(cfg->reduction == RG_LOSS_NONE ? std::min((N + 1023) / 1024, 1024) : 1),
+                           dim3(1024), 0, st, tokens, N, cfg->reduction, t.counted, loss);
     return hipGetLastError();
 }
 

@@ -658,7 +658,8 @@ std::vector<OptTensor> linear_cross_entropy(Tensor x, Tensor weight, Tensor targ
     need(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1) && target.dim() == 1 && target.size(0) == x.size(0),
          "linear_cross_entropy: x must be [tokens, size], weight [words, size], target [tokens]");
     need(x.size(1) >= 1 && weight.size(0) >= 1, "linear_cross_entropy: sizes must be positive");
-    need(x.size(0) <= INT32_MAX && x.size(1) <= INT32_MAX && weight.size(0) <= INT32_MAX, "linear_cross_entropy: sizes must be below 2^31");
+    need(x.size(0) <= RG_LOSS_MAX_TOKENS && x.size(1) <= RG_LOSS_MAX_WORDS && weight.size(0) <= RG_LOSS_MAX_WORDS,
+         "linear_cross_entropy: too many tokens, values or words");
     need(S >= 1 && S <= 3, "linear_cross_entropy: slices must be 1..3");
     need(reduction >= RG_LOSS_MEAN && reduction <= RG_LOSS_NONE, "linear_cross_entropy: unknown reduction");
     x = x.resolve_neg().contiguous();

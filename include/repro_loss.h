@@ -32,9 +32,13 @@ extern "C" {
 
 enum { RG_LOSS_MEAN = 0, RG_LOSS_SUM = 1, RG_LOSS_NONE = 2 };
 
+#define RG_LOSS_MAX_TOKENS (1 << 22)
+#define RG_LOSS_MAX_WORDS (1 << 28)
+
 typedef struct rg_loss_config {
-    long long N;            /* tokens, 0 .. 2^31 - 1 */
-    int D, V;               /* V as the GEMM's inner length: at S = 3 up to about 1,000,000 */
+    long long N;            /* tokens, 0 .. RG_LOSS_MAX_TOKENS */
+    int D, V;               /* 1 .. RG_LOSS_MAX_WORDS, and what the GEMM takes as its inner length: at
+                             * S = 3 about 1,000,000 */
     int slices;             /* S in 1..3 */
     int reduction;          /* RG_LOSS_* */
     long long ignore_index;
@@ -43,8 +47,8 @@ typedef struct rg_loss_config {
 /* Three slices, the mean, ignore_index -100; sizes 0. */
 void rg_loss_config_init(rg_loss_config* cfg);
 
-/* Tokens of a group for a vocabulary of V words: a power of two, at least 128, of at most 2^27 logits
- * past that. 0 for V < 1. */
+/* Tokens of a group for a vocabulary of V words: a power of two from 128 to 2048, of at most 2^27 logits
+ * where it is past 128. 0 for V < 1. */
 int rg_loss_group_tokens(int V);
 
 /* Bytes that rg_linear_cross_entropy needs for these sizes; want_dx, want_dw: whether it is asked for
@@ -54,7 +58,7 @@ int rg_linear_cross_entropy_workspace(const rg_loss_config* cfg, int want_dx, in
 /* loss: one float, or N for RG_LOSS_NONE; dx [N][D]; dw [V][D]; each may be null. factors (N floats, may
  * be null): g_n instead of the reduction's. N = 0: loss 0 (the mean NaN), dw zero.
  * 1 (invalid value): null cfg, sizes, slices or reduction out of range; with N > 0 null x, w or target, an
- * address off 4 bytes (off 8: target), or a workspace that is null or too small. */
+ * address off 4 bytes (off 8: target), or a workspace that is null, off 256 bytes or too small. */
 int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const float* w, const long long* target,
                             const float* factors, float* loss, float* dx, float* dw, void* workspace,
                             size_t workspace_bytes, void* stream);

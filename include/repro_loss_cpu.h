@@ -11,14 +11,14 @@
 #include "repro_gemm_cpu.h"
 #include "repro_loss.h"
 #include "repro_loss_math.h"
-#include "repro_sum_cpu.h"
 
 namespace repro_loss {
 
 namespace cpu_detail {
 
 // Balanced tree over n values, first level v[i] + v[i + n / 2].
-inline float halves(float* v, int n) {
+template <class T>
+T halves(T* v, int n) {
     for (int h = n / 2; h > 0; h /= 2)
         for (int i = 0; i < h; ++i) v[i] = v[i] + v[i + h];
     return v[0];
@@ -120,9 +120,10 @@ inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, co
         std::copy(rows.begin(), rows.end(), loss);
         return;
     }
-    loss[0] = 0.0f;
-    if (N > 0) repro_sum::cpu_sum(rows.data(), loss, (int)N, 1, 1, false);
-    if (c.reduction == RG_LOSS_MEAN) loss[0] = loss[0] / (float)count;
+    std::vector<double> sum(STRANDS, 0.0);
+    for (int64_t n = 0; n < N; ++n) sum[n % STRANDS] = sum[n % STRANDS] + (double)rows[n];
+    const double all = cpu_detail::halves(sum.data(), STRANDS);
+    loss[0] = (float)(c.reduction == RG_LOSS_MEAN ? all / (double)count : all);
 }
 
 }  // namespace repro_loss

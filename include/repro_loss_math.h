@@ -8,10 +8,11 @@ namespace repro_loss {
 
 using repro_gemm::bits_to_float;
 
-// e^x for x <= 0, within one unit in the last place; 0 below -87, where results leave the normal range; NaN
+// e^x for x <= 0, within 1.04 units in the last place; 0 below -87, where results leave the normal range; NaN
 // for NaN. x = n ln 2 + r with |r| <= ln 2 / 2 (ln 2 in two parts, the first short enough for n times it to be
 // exact: Cody and Waite's reduction), and Taylor's polynomial to r^7 / 7!, whose remainder is under
-// 2^-27 of the result.
+// 2^-27 of the result. It never falls as x rises (checked for every float32): the largest of a row's
+// values is that of its largest x.
 RG_HD inline float exp_nonpositive(float x) {
     if (!(x >= -87.0f)) return x == x ? 0.0f : x;
     const float n = __builtin_rintf(x * 1.44269504f);
@@ -23,8 +24,7 @@ RG_HD inline float exp_nonpositive(float x) {
     p = __builtin_fmaf(p, r, 1.0f / 24.0f);
     p = __builtin_fmaf(p, r, 1.0f / 6.0f);
     p = __builtin_fmaf(p, r, 0.5f);
-    p = __builtin_fmaf(p, r, 1.0f);
-    p = __builtin_fmaf(p, r, 1.0f);
+    p = 1.0f + __builtin_fmaf(r * r, p, r);
     return p * bits_to_float((uint32_t)((int)n + 127) << 23);
 }
 
@@ -55,11 +55,17 @@ RG_HD inline double log_positive(float s) {
 // balanced tree whose first level adds l and l + 32, the next l and l + 16, and so on.
 constexpr int PART = 64;
 
+// The losses' sum is taken in binary64: token n to strand n mod STRANDS, in ascending order from +0, and the
+// strands as a balanced tree whose first level adds l and l + STRANDS / 2, and so on; a mean is divided by the
+// count there, and either is rounded to float32 once.
+constexpr int STRANDS = 1024;
+
 // Tokens are taken in groups of this many, whose logits are held together (at most 2^27 of them,
 // 512 MB, past 128 tokens). It is part of the result: a group's contribution to the weight's gradient
 // is rounded once, and the groups' are added in ascending order.
+constexpr int MAX_GROUP = 2048;
 inline int group_tokens(long long V) {
-    int r = 1 << 15;
+    int r = MAX_GROUP;
     while (r > 128 && r * V > (1ll << 27)) r /= 2;
     return r;
 }

@@ -140,7 +140,7 @@ def test_a_group_of_tokens_and_more(monkeypatch):
     assert torch.equal(dw[untouched], (halves[0][2] + halves[1][2])[untouched])
     for a in (1, 64, 1003, 4096, 4097, 50257, 2 ** 30):
         r = _lib.lib.rg_loss_group_tokens(a)
-        assert r & (r - 1) == 0 and 128 <= r <= 2 ** 15 and (r * a <= 2 ** 27 or r == 128)
+        assert r & (r - 1) == 0 and 128 <= r <= 2048 and (r * a <= 2 ** 27 or r == 128)
     assert _lib.lib.rg_loss_group_tokens(0) == 0
 
 

@@ -38,10 +38,12 @@ constexpr int contract_waves_per_simd() {
     return w < need ? need : (w > cap ? cap : w);
 }
 
-// BIAS: bias[c] is added to the rounded outputs of column c, one IEEE addition each. (An instantiation
+// EPI: WITH_BIAS adds bias[c] to the rounded outputs of column c, ONTO adds the rounded outputs to C,
+// one IEEE addition each (at one part; split sums are added by the reduction). (An instantiation
 // of its own: with the null pointer tested or -0.0 added instead, GEMMs without a bias took 0.3-0.9%
 // longer, 4096^3 435.5 -> 438.6 us.)
-template <int S, int WTI, int WTJ, int WGM, int WGN, bool BIAS>
+enum { PLAIN, WITH_BIAS, ONTO };
+template <int S, int WTI, int WTJ, int WGM, int WGN, int EPI>
 __global__ void __launch_bounds__(64 * WGM * WGN, (contract_waves_per_simd<S, WTI, WTJ, WGM, WGN>()))
 contract_mfma(const int8_t* __restrict__ QA, const int8_t* __restrict__ QB,
               const int* __restrict__ eA, const int* __restrict__ eB, float* __restrict__ C,
@@ -115,7 +117,7 @@ contract_mfma(const int8_t* __restrict__ QA, const int8_t* __restrict__ QB,
     int er_lane = 0;
     int ec[WTJ];
     float bv[WTJ];
-    if constexpr (BIAS) {
+    if constexpr (EPI == WITH_BIAS) {
 #pragma unroll
         for (int tj = 0; tj < WTJ; ++tj)
             bv[tj] = bias[min(tn * BN + (wn * WTJ + tj) * 32 + (lane & 31), N - 1)];
@@ -305,6 +307,14 @@ contract_mfma(const int8_t* __restrict__ QA, const int8_t* __restrict__ QB,
 #pragma unroll
             for (int tj = 0; tj < WTJ; ++tj) {
                 float* cp = C + (size_t)(row0 + ti * 32) * ldc + col[tj];
+                float onto[16];  // the tile's old values, all in flight before its roundings
+                if constexpr (EPI == ONTO) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int r = 8 * (e >> 2) + (e & 3);
+                        onto[e] = inside || (col[tj] < N && row0 + ti * 32 + r < M) ? cp[(size_t)r * ldc] : 0.0f;
+                    }
+                }
                 // Four rows at a time (registers e = 4q .. 4q+3: rows 8q .. 8q+3 of the lane's
                 // column), so few values are live at once.
 #pragma unroll
@@ -329,9 +339,13 @@ contract_mfma(const int8_t* __restrict__ QA, const int8_t* __restrict__ QB,
                             v[i] = round_to_float_rare(combine_levels<L>(lv), er[4 * q + i] + ec[tj]);
                         }
                     }
-                    if constexpr (BIAS) {
+                    if constexpr (EPI == WITH_BIAS) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) v[i] += bv[tj];
+                    }
+                    if constexpr (EPI == ONTO) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[i] += onto[4 * q + i];
                     }
                     // Non-temporal stores: C is not read again here, and streaming it past the
                     // caches made the contraction faster (4096^3 steady state 0.466 -> 0.459 ms,
@@ -782,7 +796,7 @@ __global__ void __launch_bounds__(256)
 reduce_round(const int64_t* __restrict__ partial, const int* __restrict__ eA,
              const int* __restrict__ eB, float* __restrict__ C, int M, int N, int split, int e0,
              int batch, int Mp, int Np, long long ldc, long long c_item,
-             const float* __restrict__ bias) {
+             const float* __restrict__ bias, bool onto) {
     constexpr int OPB = 256 / TPO;  // outputs per block
     const int t = threadIdx.x;
     const int ol = t % OPB, sub = t / OPB;
@@ -802,6 +816,7 @@ reduce_round(const int64_t* __restrict__ partial, const int* __restrict__ eA,
             ea = eA[(size_t)item * Mp + r];
             eb = eB[(size_t)item * Np + c];
             if (bias != nullptr) bv = bias[c];
+            if (onto) bv = C[(size_t)item * c_item + (size_t)r * ldc + c];
         }
         const int64_t* p0 = partial + (size_t)item * split * MN + rc;
         for (int p = sub; p < split; p += TPO * RU) {
@@ -857,7 +872,7 @@ void launch_test_round(const int* levels, const int64_t* T, const int* E, float*
     else round_levels_kernel<5><<<blocks, 256, 0, stream>>>(levels, E, out, n);
 }
 
-template <int S, bool BIAS>
+template <int S, int EPI>
 static void launch_mfma_s(const Layout& L, const int8_t* qa, const int8_t* qb, const int* ea,
                           const int* eb, float* C, OutAddr out, int64_t* partial,
                           hipStream_t stream) {
@@ -873,32 +888,34 @@ static void launch_mfma_s(const Layout& L, const int8_t* qa, const int8_t* qb, c
     // 12 wavefronts; the planner never gives them to S < 3.)
     if constexpr (S == 3) {
         if (L.ti == 1 && L.tj == 3) {
-            contract_mfma<S, 1, 1, 2, 6, BIAS><<<grid, 768, 0, stream>>>(RG_CONTRACT_ARGS);
+            contract_mfma<S, 1, 1, 2, 6, EPI><<<grid, 768, 0, stream>>>(RG_CONTRACT_ARGS);
             return;
         }
         if (L.ti == 3 && L.tj == 1) {
-            contract_mfma<S, 1, 1, 6, 2, BIAS><<<grid, 768, 0, stream>>>(RG_CONTRACT_ARGS);
+            contract_mfma<S, 1, 1, 6, 2, EPI><<<grid, 768, 0, stream>>>(RG_CONTRACT_ARGS);
             return;
         }
     }
     if (L.ti == 2 && L.tj == 2)
-        contract_mfma<S, 2, 1, 2, 4, BIAS><<<grid, 512, 0, stream>>>(RG_CONTRACT_ARGS);
+        contract_mfma<S, 2, 1, 2, 4, EPI><<<grid, 512, 0, stream>>>(RG_CONTRACT_ARGS);
     else if (L.ti == 2 && L.tj == 1)
-        contract_mfma<S, 1, 1, 4, 2, BIAS><<<grid, 512, 0, stream>>>(RG_CONTRACT_ARGS);
+        contract_mfma<S, 1, 1, 4, 2, EPI><<<grid, 512, 0, stream>>>(RG_CONTRACT_ARGS);
     else if (L.ti == 1 && L.tj == 2)
-        contract_mfma<S, 1, 1, 2, 4, BIAS><<<grid, 512, 0, stream>>>(RG_CONTRACT_ARGS);
+        contract_mfma<S, 1, 1, 2, 4, EPI><<<grid, 512, 0, stream>>>(RG_CONTRACT_ARGS);
     else
-        contract_mfma<S, 1, 1, 2, 2, BIAS><<<grid, 256, 0, stream>>>(RG_CONTRACT_ARGS);
+        contract_mfma<S, 1, 1, 2, 2, EPI><<<grid, 256, 0, stream>>>(RG_CONTRACT_ARGS);
 #undef RG_CONTRACT_ARGS
 }
 
 void launch_contract_mfma(const Layout& L, const int8_t* qa, const int8_t* qb, const int* ea,
                           const int* eb, float* C, OutAddr out, int64_t* partial,
                           hipStream_t stream) {
-    const bool bias = out.bias != nullptr && partial == nullptr;  // (partials: the reduction adds it)
-#define RG_MFMA_S(SS)                                                                       \
-    (bias ? launch_mfma_s<SS, true>(L, qa, qb, ea, eb, C, out, partial, stream)             \
-          : launch_mfma_s<SS, false>(L, qa, qb, ea, eb, C, out, partial, stream))
+    // (partials: the reduction adds)
+    const int epi = partial != nullptr ? PLAIN : out.bias != nullptr ? WITH_BIAS : out.onto ? ONTO : PLAIN;
+#define RG_MFMA_S(SS)                                                                                \
+    (epi == WITH_BIAS ? launch_mfma_s<SS, WITH_BIAS>(L, qa, qb, ea, eb, C, out, partial, stream)     \
+     : epi == ONTO    ? launch_mfma_s<SS, ONTO>(L, qa, qb, ea, eb, C, out, partial, stream)          \
+                      : launch_mfma_s<SS, PLAIN>(L, qa, qb, ea, eb, C, out, partial, stream))
     switch (L.S) {
         case 1: RG_MFMA_S(1); break;
         case 2: RG_MFMA_S(2); break;
@@ -990,10 +1007,10 @@ void launch_reduce_round(const Layout& L, const int64_t* partial, const int* ea,
 #define RG_REDUCE(T)                                                                              \
     (many ? reduce_round<T, 8><<<blocks, 256, 0, stream>>>(partial, ea, eb, C, L.M, L.N, L.split,  \
                                                            -14 * (L.S - 1), L.batch, L.Mp, L.Np, \
-                                                           out.ldc, out.c_item, out.bias)       \
+                                                           out.ldc, out.c_item, out.bias, out.onto) \
           : reduce_round<T, 1><<<blocks, 256, 0, stream>>>(partial, ea, eb, C, L.M, L.N, L.split,  \
                                                            -14 * (L.S - 1), L.batch, L.Mp, L.Np, \
-                                                           out.ldc, out.c_item, out.bias))
+                                                           out.ldc, out.c_item, out.bias, out.onto))
     switch (tpo) {
         case 1: RG_REDUCE(1); break;
         case 4: RG_REDUCE(4); break;

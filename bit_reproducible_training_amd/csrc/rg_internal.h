@@ -405,6 +405,7 @@ void launch_group_max2(const SliceDesc* a, int group_a, const SliceDesc* b, int 
 struct OutAddr {
     long long ldc, c_item;
     const float* bias = nullptr;  // N values added to the rounded outputs of their columns, or null
+    bool onto = false;            // the rounded outputs are added to C (without a bias)
 };
 void launch_contract_mfma(const Layout& L, const int8_t* qa, const int8_t* qb, const int* ea,
                           const int* eb, float* C, OutAddr out, int64_t* partial,

@@ -35,46 +35,85 @@ struct Targets {
     int* slot;     // [N] the token's place among its word's as they came (which differs from run to run)
     int* arrived;  // [N]
     int* list;     // [N]
+    int2* lead;    // [N] of a word's first token: its tokens and their place in `list`; else 0 tokens
     int* count;    // [V]
     int* place;    // [V] (of words that occur)
     int* counted;  // [1] tokens that are not left out
 };
 
 // One block: the words' counts by atomics, then places for their tokens. A word's place and its tokens'
-// order in `arrived` change from run to run and reach no result: loss_tokens puts them in order. (Every
-// token compared with every other one took 170 us for 8192 tokens, and 64 times that for 65536.)
-__global__ void __launch_bounds__(1024)
-loss_words(const long long* __restrict__ target, long long ignore_index, int N, int V, Targets t) {
+// order in `arrived` change from run to run and reach no result: loss_tokens puts them in order. The
+// block waits for memory nearly all the time, so a thread has BATCH tokens in flight, and the block runs
+// beside those of the first group's loss_parts, which take longer from some 1000 tokens of 50257 words
+// on (8192 tokens: 73 us as a launch of its own with a token at a time; every token compared with every
+// other one, 170 us, and 64 times that for 65536). lists: whether the tokens are listed.
+__device__ void words_block(const long long* __restrict__ target, long long ignore_index, int N, int V, bool lists,
+                            const Targets& t) {
+    constexpr int BATCH = 8;
     __shared__ int places, kept;
+    const int threads = blockDim.x;
+    const auto load = [](const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const auto store = [](int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
     if (threadIdx.x == 0) places = kept = 0;
-    for (int v = threadIdx.x; v < V; v += 1024) __hip_atomic_store(&t.count[v], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (lists)
+        for (int v = threadIdx.x; v < V; v += threads) store(&t.count[v], 0);
     __threadfence();
     __syncthreads();
     int mine = 0;
-    for (int n = threadIdx.x; n < N; n += 1024) {
-        const long long v = target[n];
-        const int w = v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
-        t.word[n] = w;
-        mine += w != LEFT_OUT;
-        if (w >= 0) t.slot[n] = atomicAdd(&t.count[w], 1);
+    for (int base = threadIdx.x; base < N; base += threads * BATCH) {
+        int w[BATCH], slot[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int n = base + i * threads;
+            const long long v = n < N ? target[n] : ignore_index;
+            w[i] = v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
+            mine += w[i] != LEFT_OUT;
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) slot[i] = lists && w[i] >= 0 ? atomicAdd(&t.count[w[i]], 1) : 0;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int n = base + i * threads;
+            if (n >= N) break;
+            t.word[n] = w[i];
+            if (lists) t.slot[n] = slot[i];
+        }
     }
     if (mine > 0) atomicAdd(&kept, mine);
     __threadfence();
     __syncthreads();
-    for (int n = threadIdx.x; n < N; n += 1024) {
-        const int w = t.word[n];
-        if (w >= 0 && t.slot[n] == 0) {
-            const int c = __hip_atomic_load(&t.count[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_store(&t.place[w], atomicAdd(&places, c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) t.counted[0] = kept;
+    if (!lists) return;
+    for (int base = threadIdx.x; base < N; base += threads * BATCH) {
+        int w[BATCH], c[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int n = base + i * threads;
+            w[i] = n < N && t.slot[n] == 0 ? t.word[n] : LEFT_OUT;
         }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) c[i] = w[i] >= 0 ? load(&t.count[w[i]]) : 0;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (w[i] >= 0) store(&t.place[w[i]], atomicAdd(&places, c[i]));
     }
     __threadfence();
     __syncthreads();
-    for (int n = threadIdx.x; n < N; n += 1024) {
-        const int w = t.word[n];
-        if (w >= 0) t.arrived[__hip_atomic_load(&t.place[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + t.slot[n]] = n;
+    for (int base = threadIdx.x; base < N; base += threads * BATCH) {
+        int w[BATCH], at[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int n = base + i * threads;
+            w[i] = n < N ? t.word[n] : LEFT_OUT;
+            at[i] = n < N ? t.slot[n] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (w[i] >= 0) at[i] += load(&t.place[w[i]]);
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (w[i] >= 0) t.arrived[at[i]] = base + i * threads;
     }
-    if (threadIdx.x == 0) t.counted[0] = kept;
 }
 
 template <int CTRL>
@@ -101,23 +140,45 @@ __device__ __forceinline__ float wave_sum(float v) {
     return row_sum16(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// The parts' largest logits and sums: a lane takes a chunk of 4 words, 16 lanes a part. Rows of z are ldz
-// apart, a multiple of 32.
+// What words_block is to do in a launch, if anything (N = 0: nothing).
+struct WordsWork {
+    const long long* target;
+    long long ignore_index;
+    int N;
+    bool lists;
+};
+
+// The parts' largest logits and sums: a lane takes a chunk of 4 words, 16 lanes a part, EACH times. Rows of z are ldz
+// apart, a multiple of 32. The first row of blocks is not a token's: its first block is words_block.
+constexpr int EACH = 4;
 __global__ void __launch_bounds__(256)
-loss_parts(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ out) {
-    const int row = blockIdx.y;
-    const int part = blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (part >= parts) return;  // uniform over a part's 16 lanes
-    const int at = part * PART + 4 * (threadIdx.x & 15);
-    const float4 f = at < V ? *reinterpret_cast<const float4*>(z + (size_t)row * ldz + at) : make_float4(0, 0, 0, 0);
-    float v[4] = {f.x, f.y, f.z, f.w};
+loss_parts(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ out, WordsWork work, Targets t) {
+    if (blockIdx.y == 0) {
+        if (blockIdx.x == 0 && work.N > 0) words_block(work.target, work.ignore_index, work.N, V, work.lists, t);
+        return;
+    }
+    const int row = blockIdx.y - 1, chunk = 4 * (threadIdx.x & 15);
+    const float* q = z + (size_t)row * ldz + chunk;
+    const int first = blockIdx.x * (16 * EACH) + (threadIdx.x >> 4);
+    float4 f[EACH];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
-    const float a = row_max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+    for (int u = 0; u < EACH; ++u) {
+        const int at = (first + 16 * u) * PART;
+        f[u] = at + chunk < V ? *reinterpret_cast<const float4*>(q + at) : make_float4(0, 0, 0, 0);
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = at + i < V ? exp_nonpositive(v[i] - a) : 0.0f;
-    const float b = row_sum16((v[0] + v[1]) + (v[2] + v[3]));
-    if ((threadIdx.x & 15) == 0) out[(size_t)row * parts + part] = make_float2(a, b);
+    for (int u = 0; u < EACH; ++u) {
+        const int part = first + 16 * u, at = part * PART + chunk;
+        if (part >= parts) return;  // uniform over a part's 16 lanes
+        float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
+        const float a = row_max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = at + i < V ? exp_nonpositive(v[i] - a) : 0.0f;
+        const float b = row_sum16((v[0] + v[1]) + (v[2] + v[3]));
+        if (chunk == 0) out[(size_t)row * parts + part] = make_float2(a, b);
+    }
 }
 
 __device__ __forceinline__ float wave_fmax(float m) {
@@ -130,7 +191,7 @@ __device__ __forceinline__ float wave_fmax(float m) {
 // dz: that of the largest of the words other than the target (exp_nonpositive never falls).
 __global__ void __launch_bounds__(256)
 loss_tokens(const float* __restrict__ z, int ldz, int V, int parts, const float2* __restrict__ part, int first,
-            int rows, Targets t, const float* __restrict__ factors, int mean, Token* __restrict__ tokens,
+            int rows, Targets t, bool lists, const float* __restrict__ factors, int mean, Token* __restrict__ tokens,
             int* __restrict__ exponents) {
     const int lane = threadIdx.x & 63;
     const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -159,16 +220,22 @@ loss_tokens(const float* __restrict__ z, int ldz, int V, int parts, const float2
         k = repro_loss::finish_token(m, s, q[word], g);
         const float top = fabsf(exp_nonpositive(other - k.top) * k.factor);
         exponent = repro_gemm::scale_exponent(top);  // 0 for a NaN
-        const int place = t.place[word], count = t.count[word];
-        int before = 0;
-        for (int i = lane; i < count; i += 64) before += t.arrived[place + i] < n;
+        if (lists) {
+            const int place = t.place[word], count = t.count[word];
+            int before = 0;
+            for (int i = lane; i < count; i += 64) before += t.arrived[place + i] < n;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
-        if (lane == 0) t.list[place + before] = n;
+            for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
+            if (lane == 0) {
+                t.list[place + before] = n;
+                t.lead[n] = make_int2(before == 0 ? count : 0, place);
+            }
+        }
     } else if (word == INVALID) {
         k.loss = NAN;
     }
     if (lane == 0) {
+        if (lists && word < 0) t.lead[n] = make_int2(0, 0);
         tokens[n] = k;
         exponents[r] = exponent;
     }
@@ -220,6 +287,13 @@ __device__ __forceinline__ void transpose_rows(int (&d)[4]) {
     }
 }
 
+// round_fixed of a finite value within its row's scale, in the low 7 S bits: the scale is a power of two at least
+// |x| / 127 (to one rounding), so |x| 2^n is at most 127 * 2^(7 (S - 1)) when rounded and no clamp is
+// needed; what falls below float32's range here rounds to 0 either way.
+__device__ __forceinline__ int fixed_bits(float x, int n) {
+    return __float_as_int(__builtin_amdgcn_ldexpf(x, n) + ROUND_MAGIC);
+}
+
 struct DigitsOut {
     int8_t* by_token;     // op(A) of dx: rows tokens, k words; null where not wanted
     size_t token_bytes;   // of a panel of 32 tokens over all words
@@ -260,13 +334,13 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
             float2 t = make_float2(0.0f, 0.0f);
             if (r < rows) {
                 word = words[first + r];
-                t = *reinterpret_cast<const float2*>(&tokens[first + r]);  // top, factor
+                t = *reinterpret_cast<const float2*>(&tokens[first + r]);  // top, factor (0: a row of zeros)
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const float e = exp_nonpositive(d[s][k][c] - t.x) * t.y;
-                d[s][k][c] = word < 0 || v + c == word ? 0.0f : e;
-                top[c] = max(top[c], repro_gemm::magnitude_key(d[s][k][c]));
+                const float e = repro_loss::dz_of(d[s][k][c], t.x, t.y);
+                d[s][k][c] = v + c == word ? 0.0f : e;
+                top[c] = max(top[c], __float_as_uint(d[s][k][c]) & 0x7FFFFFFFu);
             }
         }
     if (out.by_word != nullptr) {
@@ -277,14 +351,14 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
             if (lane < 4) tops[wave][4 * q + c] = top[c];
         }
         __syncthreads();
-        RowScale scale[4];
+        int scale[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
             uint32_t m = 0;
 #pragma unroll
             for (int w = 0; w < DIGIT_THREADS / 64; ++w) m = max(m, tops[w][4 * q + c]);
             const int e = repro_gemm::scale_exponent(__uint_as_float(m));
-            scale[c] = row_scale<S>(e);
+            scale[c] = 7 * (S - 1) - e;
             if (threadIdx.x < 4 && v + c < V) out.word_exponents[v + c] = e;
         }
         const int mine = v0 + 4 * q + i;  // the word whose pieces this lane stores
@@ -296,8 +370,8 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
             v4i w[S];  // w[p][c]: digit p of word c's four tokens
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const int x[4] = {round_fixed(d[s][0][c], scale[c]), round_fixed(d[s][1][c], scale[c]),
-                                  round_fixed(d[s][2][c], scale[c]), round_fixed(d[s][3][c], scale[c])};
+                const int x[4] = {fixed_bits(d[s][0][c], scale[c]), fixed_bits(d[s][1][c], scale[c]),
+                                  fixed_bits(d[s][2][c], scale[c]), fixed_bits(d[s][3][c], scale[c])};
                 pack_word<S>(x, w, c);
             }
             const int k0 = t0 + 16 * j;
@@ -318,9 +392,9 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int r = s * STEP_TOKENS + base + k;
-                const RowScale scale = row_scale<S>(r < rows ? exponents[r] : 0);
-                const int x[4] = {round_fixed(d[s][k][0], scale), round_fixed(d[s][k][1], scale),
-                                  round_fixed(d[s][k][2], scale), round_fixed(d[s][k][3], scale)};
+                const int scale = 7 * (S - 1) - (r < rows ? exponents[r] : 0);
+                const int x[4] = {fixed_bits(d[s][k][0], scale), fixed_bits(d[s][k][1], scale),
+                                  fixed_bits(d[s][k][2], scale), fixed_bits(d[s][k][3], scale)};
                 pack_word<S>(x, w, k);
             }
             const int r = s * STEP_TOKENS + base + q;  // the token whose piece this lane stores
@@ -338,74 +412,87 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
 
 // ---- the target words' share ----
 //
-// Blocks below N take dw (a word each, at its first token; a wavefront 256 columns at a time), the
-// others dx (a token each). A word's tokens are read 64 at a time by the lanes, which then know
-// the rows of x to load, 16 at once.
+// A wavefront takes a token and 256 columns, of dx (blockIdx.z 0) or of dw, where a word's first token
+// stands for all of its tokens, 16 at a time. Most words have one, whose row's address is known without the list.
 __global__ void __launch_bounds__(256)
 loss_target(float* __restrict__ dx, float* __restrict__ dw, const float* __restrict__ x, const float* __restrict__ w,
             int D, const Token* __restrict__ tokens, Targets t, int N) {
     const int lane = threadIdx.x & 63;
-    int n = blockIdx.x;
-    if (dw == nullptr || n >= N) {
-        n = dw == nullptr ? n : n - N;
-        const int word = t.word[n];
+    const int n = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int at = blockIdx.y * 256 + 4 * lane;
+    if (n >= N || at >= D) return;
+    const bool full = at + 4 <= D;
+    const auto load = [&](const float* p, float (&v)[4]) {
+        if (full) {
+            const Four f = *reinterpret_cast<const Four*>(p + at);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = f.v[k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = at + k < D ? p[at + k] : 0.0f;
+        }
+    };
+    const auto onto = [&](float* p, const float (&v)[4]) {
+        float old[4];
+        load(p, old);
+        Four f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f.v[k] = old[k] + v[k];
+        if (full) {
+            *reinterpret_cast<Four*>(p + at) = f;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (at + k < D) p[at + k] = f.v[k];
+        }
+    };
+    const int word = t.word[n];
+    const float mine = tokens[n].target;
+    float v[4];
+    if (blockIdx.z == 0 && dx != nullptr) {
         if (word < 0) return;
-        const float c = tokens[n].target;
-        const float* q = w + (size_t)word * D;
-        float* o = dx + (size_t)n * D;
-        for (int i = threadIdx.x; i < D; i += 256) o[i] = o[i] + c * q[i];
+        load(w + (size_t)word * D, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = mine * v[k];
+        onto(dx + (size_t)n * D, v);
         return;
     }
-    const int word = t.word[n];
-    if (word < 0) return;
-    const int count = t.count[word];
-    const int* list = t.list + t.place[word];
-    if (list[0] != n) return;
-    for (int base = 256 * (threadIdx.x >> 6); base < D; base += 1024) {
-        const int at = base + 4 * lane;
-        const bool full = at + 4 <= D;
-        float s[16][4];
+    const int2 lead = t.lead[n];
+    if (lead.x == 0) return;
+    if (lead.x == 1) {
+        load(x + (size_t)n * D, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = 0.0f + mine * v[k];
+        onto(dw + (size_t)word * D, v);
+        return;
+    }
+    const int* list = t.list + lead.y;
+    float s[16][4];
+#pragma unroll
+    for (int h = 0; h < 16; ++h)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[h][k] = 0.0f;
+    for (int k0 = 0; k0 < lead.x; k0 += 16) {
+        // No branches: the 16 rows are in flight together (past the end the last one, whose value is not taken).
+        float c[16], q[16][4];
+#pragma unroll
+        for (int h = 0; h < 16; ++h) {
+            const int m = list[min(k0 + h, lead.x - 1)];
+            c[h] = tokens[m].target;
+            load(x + (size_t)m * D, q[h]);
+        }
 #pragma unroll
         for (int h = 0; h < 16; ++h)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[h][k] = 0.0f;
-        for (int k0 = 0; k0 < count; k0 += 64) {
-            int m = 0;
-            float c = 0.0f;
-            if (k0 + lane < count) {
-                m = list[k0 + lane];
-                c = tokens[m].target;
-            }
-            const int held = min(64, count - k0);
-            for (int b = 0; b < held; b += 16) {
-#pragma unroll
-                for (int h = 0; h < 16; ++h) {
-                    if (b + h >= held) break;
-                    const float* q = x + (size_t)__builtin_amdgcn_readlane(m, b + h) * D + at;
-                    const float ch = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(c), b + h));
-                    if (full) {
-                        const Four f = *reinterpret_cast<const Four*>(q);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) s[h][k] = s[h][k] + ch * f.v[k];
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (at + k < D) s[h][k] = s[h][k] + ch * q[k];
-                    }
-                }
-            }
-        }
-#pragma unroll
-        for (int h = 8; h > 0; h /= 2)
-#pragma unroll
-            for (int a = 0; a < h; ++a)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[a][k] = s[a][k] + s[a + h][k];
-        float* o = dw + (size_t)word * D + at;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (at + k < D) o[k] = o[k] + s[0][k];
+            for (int k = 0; k < 4; ++k) s[h][k] = k0 + h < lead.x ? s[h][k] + c[h] * q[h][k] : s[h][k];
     }
+#pragma unroll
+    for (int h = 8; h > 0; h /= 2)
+#pragma unroll
+        for (int a = 0; a < h; ++a)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[a][k] = s[a][k] + s[a + h][k];
+    onto(dw + (size_t)word * D, s[0]);
 }
 
 // The losses, or their sum or mean (one block).
@@ -428,9 +515,6 @@ loss_reduce(const Token* __restrict__ tokens, int N, int reduction, const int* _
     if (threadIdx.x == 0) loss[0] = (float)(reduction == RG_LOSS_MEAN ? lds[0] / (double)counted[0] : lds[0]);
 }
 
-__global__ void __launch_bounds__(256) loss_add(float* __restrict__ a, const float* __restrict__ b, size_t n) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) a[i] = a[i] + b[i];
-}
 __global__ void __launch_bounds__(256) loss_fill(float* __restrict__ a, float v, size_t n) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) a[i] = v;
 }
@@ -443,7 +527,7 @@ __global__ void __launch_bounds__(256) scale_kernel(float* __restrict__ a, const
 unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 1u << 20); }
 
 bool sizes_ok(const rg_loss_config* c) {
-    return c && c->N >= 0 && c->N <= RG_LOSS_MAX_TOKENS && c->D >= 1 && c->D <= RG_LOSS_MAX_WORDS && c->V >= 1 &&
+    return c && c->N >= 0 && c->N <= RG_LOSS_MAX_TOKENS && c->D >= 1 && c->D <= RG_LOSS_MAX_SIZE && c->V >= 1 &&
            c->V <= RG_LOSS_MAX_WORDS && c->slices >= 1 && c->slices <= 3 &&
            c->reduction >= RG_LOSS_MEAN && c->reduction <= RG_LOSS_NONE;
 }
@@ -469,7 +553,7 @@ struct Space {
     int group, last, parts, ldz;
     Layout z[2], dx[2], dw[2];
     Digits x_rows, w_rows, w_cols, x_cols, by_token, by_word;
-    size_t words, tokens, part, logits, more, partial, scratch, total;
+    size_t words, tokens, part, logits, partial, scratch, total;
 };
 
 int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
@@ -501,7 +585,7 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
         for (const Layout* L : {&s->z[k], dx ? &s->dx[k] : nullptr, dw ? &s->dw[k] : nullptr})
             if (L && L->has_partial) partial = std::max(partial, (size_t)L->split * L->M * L->N * sizeof(int64_t));
     }
-    s->words = take(((size_t)4 * N + 2 * (size_t)V + 1) * sizeof(int));
+    s->words = take(((size_t)6 * N + 2 * (size_t)V + 1) * sizeof(int));
     s->tokens = take((size_t)N * sizeof(Token));
     s->part = take((size_t)s->group * s->parts * sizeof(float2));
     s->logits = take((size_t)s->group * s->ldz * sizeof(float));
@@ -518,17 +602,16 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
         scratch = std::max({scratch, slice_scratch_bytes(D, s->group, true), slice_scratch_bytes(D, s->last, true)});
         s->by_word = digits(V, s->group);
     }
-    s->more = take(dw && N > s->group ? (size_t)V * D * sizeof(float) : 0);
     s->partial = take(partial);
     s->scratch = take(scratch);
     s->total = at;
     return hipSuccess;
 }
 
-// C (rows ldc apart) = the product of two operands' digits.
+// C (rows ldc apart) = the product of two operands' digits, or that added to C.
 void launch_product(const Layout& L, const int8_t* qa, const int* ea, const int8_t* qb, const int* eb, float* C,
-                    long long ldc, int64_t* partial, hipStream_t st) {
-    const OutAddr out{ldc, 0, nullptr};
+                    long long ldc, bool onto, int64_t* partial, hipStream_t st) {
+    const OutAddr out{ldc, 0, nullptr, onto};
     launch_contract_mfma(L, qa, qb, ea, eb, C, out, L.has_partial ? partial : nullptr, st);
     if (L.has_partial) launch_reduce_round(L, partial, ea, eb, C, out, st);
 }
@@ -596,7 +679,8 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     const auto panels = [&](const Digits& d) { return reinterpret_cast<int8_t*>(base + d.q); };
     const auto exponents = [&](const Digits& d) { return reinterpret_cast<int*>(base + d.e); };
     Targets t;
-    t.word = reinterpret_cast<int*>(base + s.words);
+    t.lead = reinterpret_cast<int2*>(base + s.words);
+    t.word = reinterpret_cast<int*>(t.lead + N);
     t.slot = t.word + N;
     t.arrived = t.slot + N;
     t.list = t.arrived + N;
@@ -606,11 +690,9 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     Token* tokens = reinterpret_cast<Token*>(base + s.tokens);
     float2* part = reinterpret_cast<float2*>(base + s.part);
     float* z = reinterpret_cast<float*>(base + s.logits);
-    float* more = reinterpret_cast<float*>(base + s.more);
     int64_t* partial = reinterpret_cast<int64_t*>(base + s.partial);
     float* scratch = reinterpret_cast<float*>(base + s.scratch);
 
-    hipLaunchKernelGGL(loss_words, dim3(1), dim3(1024), 0, st, target, cfg->ignore_index, N, V, t);
     // The digits that every group's products share.
     rc = launch_slice(x, N, D, false, S, panels(s.x_rows), exponents(s.x_rows), scratch, st);
     if (rc == hipSuccess) rc = launch_slice(w, V, D, false, S, panels(s.w_rows), exponents(s.w_rows), scratch, st);
@@ -619,10 +701,11 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     for (int first = 0; first < N; first += s.group) {
         const int rows = std::min(s.group, N - first), k = first + s.group < N ? 0 : 1;
         launch_product(s.z[k], panels(s.x_rows) + (size_t)first * round_up(D, STEP_K) * S, exponents(s.x_rows) + first,
-                       panels(s.w_rows), exponents(s.w_rows), z, s.ldz, partial, st);
-        hipLaunchKernelGGL(loss_parts, dim3((s.parts + 15) / 16, rows), dim3(256), 0, st, z, s.ldz, V, s.parts, part);
+                       panels(s.w_rows), exponents(s.w_rows), z, s.ldz, false, partial, st);
+        const WordsWork work{target, cfg->ignore_index, first == 0 ? N : 0, dw != nullptr};
+        hipLaunchKernelGGL(loss_parts, dim3((s.parts + 16 * EACH - 1) / (16 * EACH), rows + 1), dim3(256), 0, st, z, s.ldz, V, s.parts, part, work, t);
         hipLaunchKernelGGL(loss_tokens, dim3((rows + 3) / 4), dim3(256), 0, st, z, s.ldz, V, s.parts, part, first, rows,
-                           t, factors, cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, exponents(s.by_token));
+                           t, dw != nullptr, factors, cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, exponents(s.by_token));
         if (!dx && !dw) continue;
         DigitsOut out;
         out.by_token = dx ? panels(s.by_token) : nullptr;
@@ -636,18 +719,17 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
         else launch_digits_s<3>(V, rows, st, z, s.ldz, first, tokens, t.word, exponents(s.by_token), out);
         if (dx)
             launch_product(s.dx[k], panels(s.by_token), exponents(s.by_token), panels(s.w_cols), exponents(s.w_cols),
-                           dx + (size_t)first * D, D, partial, st);
+                           dx + (size_t)first * D, D, false, partial, st);
         if (dw) {
             rc = launch_slice(x + (size_t)first * D, D, rows, true, S, panels(s.x_cols), exponents(s.x_cols), scratch, st);
             if (rc != hipSuccess) return rc;
             launch_product(s.dw[k], panels(s.by_word), exponents(s.by_word), panels(s.x_cols), exponents(s.x_cols),
-                           first == 0 ? dw : more, D, partial, st);
-            const size_t n = (size_t)V * D;
-            if (first > 0) hipLaunchKernelGGL(loss_add, dim3(grid_of(n)), dim3(256), 0, st, dw, more, n);
+                           dw, D, first > 0, partial, st);
         }
     }
     if (dx || dw)
-        hipLaunchKernelGGL(loss_target, dim3((dx ? N : 0) + (dw ? N : 0)), dim3(256), 0, st, dx, dw, x, w, D, tokens, t, N);
+        hipLaunchKernelGGL(loss_target, dim3((N + 3) / 4, (D + 255) / 256, dx && dw ? 2 : 1), dim3(256), 0, st, dx, dw, x,
+                           w, D, tokens, t, N);
     if (loss)
         hipLaunchKernelGGL(loss_reduce, dim3(cfg->reduction == RG_LOSS_NONE ? std::min((N + 1023) / 1024, 1024) : 1),
                            dim3(1024), 0, st, tokens, N, cfg->reduction, t.counted, loss);

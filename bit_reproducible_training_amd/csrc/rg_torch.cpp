@@ -12,6 +12,8 @@
 // argument errors raise ValueError.
 #include <torch/extension.h>
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -38,14 +40,17 @@ namespace {
 using torch::Tensor;
 
 // A non-zero hipError_t from the library, raised in Python as error_class(code, what).
-struct LibraryError {
+// (A std::exception: the autograd engine's threads hand on no others.)
+struct LibraryError : std::exception {
     int code;
-    std::string what;
+    std::string message;
+    LibraryError(int c, const char* w) : code(c), message(w) {}
+    const char* what() const noexcept override { return message.c_str(); }
 };
 PyObject* g_error_class = nullptr;  // set once by the package (set_error_class)
 
 void check(int code, const char* what) {
-    if (code != 0) throw LibraryError{code, what};
+    if (code != 0) throw LibraryError(code, what);
 }
 
 void need(bool ok, const std::string& what) {
@@ -62,6 +67,15 @@ bool on_gpu(const Tensor& a, const Tensor& b, const char* op) {
     need(a.is_cuda() || a.is_cpu(), std::string(op) + ": tensors must be on the CPU or a GPU");
     return a.is_cuda();
 }
+
+// Lets other Python threads run while the CPU computes, where this thread has the interpreter (a backward
+// pass of the binding's own functions has not).
+struct Unlocked {
+    c10::optional<py::gil_scoped_release> released;
+    Unlocked() {
+        if (PyGILState_Check()) released.emplace();
+    }
+};
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
@@ -384,34 +398,54 @@ repro_adamw::Scalars adamw_scalars(const rg_adamw_config& c) {
     return repro_adamw::make_scalars(c.lr, c.beta1, c.beta2, c.eps, c.weight_decay, c.step);
 }
 
+// The tensors of a Python list or tuple, which holds them while the call runs (taking a few hundred of them as a
+// vector, with its reference counts, and building every check's message took longer than the step).
+struct Listed {
+    py::object held;
+    std::vector<const Tensor*> t;
+    Listed(const py::handle& list, const char* name) {
+        held = py::reinterpret_steal<py::object>(PySequence_Fast(list.ptr(), "adamw takes lists of tensors"));
+        if (!held) throw py::error_already_set();
+        const Py_ssize_t n = PySequence_Fast_GET_SIZE(held.ptr());
+        PyObject** items = PySequence_Fast_ITEMS(held.ptr());
+        t.reserve(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            if (!THPVariable_Check(items[i])) need(false, std::string("adamw: ") + name + " must be tensors");
+            t.push_back(&THPVariable_Unpack(items[i]));
+        }
+    }
+    size_t size() const { return t.size(); }
+    const Tensor& operator[](size_t i) const { return *t[i]; }
+};
+
 // The step goes through a tensor's memory in its own order, so all of a value's tensors must be
 // dense, without overlaps and laid out alike.
 void need_alike(const Tensor& p, const Tensor& t, const char* name) {
-    need(t.scalar_type() == torch::kFloat32, std::string("adamw: ") + name + " must be float32");
-    need(t.device() == p.device(), std::string("adamw: ") + name + " must be on its parameter's device");
-    need(t.sizes() == p.sizes() && (p.is_contiguous() ? t.is_contiguous() : t.strides() == p.strides()),
-         std::string("adamw: ") + name + " must have its parameter's shape and strides");
-    need(!t.is_neg(), std::string("adamw: ") + name + " must not be a lazily negated view");
+    if (t.scalar_type() == torch::kFloat32 && t.device() == p.device() && t.sizes() == p.sizes() && !t.is_neg() &&
+        (p.is_contiguous() ? t.is_contiguous() : t.strides() == p.strides()))
+        return;
+    need(false, std::string("adamw: ") + name + " must be float32, on its parameter's device, with its shape and strides" +
+                    (t.is_neg() ? " (and no lazily negated view)" : ""));
 }
 
 // The first parameter's device kind (true: GPU); every parameter float32, dense and on that device.
-bool adamw_parameters(const std::vector<Tensor>& params, const std::vector<Tensor>& grads) {
+bool adamw_parameters(const Listed& params, const Listed& grads) {
     need(params.size() == grads.size(), "adamw: as many gradients as parameters");
     for (size_t i = 0; i < params.size(); ++i) {
         const Tensor& p = params[i];
-        need(p.device() == params[0].device(), "adamw: parameters must be on one device");
-        need(p.is_cuda() || p.is_cpu(), "adamw: parameters must be on the CPU or a GPU");
-        need(p.is_non_overlapping_and_dense(), "adamw: parameters must be dense");
+        if (p.device() != params[0].device()) need(false, "adamw: parameters must be on one device");
+        if (!p.is_cuda() && !p.is_cpu()) need(false, "adamw: parameters must be on the CPU or a GPU");
+        if (!p.is_non_overlapping_and_dense()) need(false, "adamw: parameters must be dense");
         need_alike(p, p, "a parameter");
         need_alike(p, grads[i], "a gradient");
     }
-    return !params.empty() && params[0].is_cuda();
+    return params.size() > 0 && params[0].is_cuda();
 }
 
-void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m,
-                const std::vector<Tensor>& v, double lr, double beta1, double beta2, double eps,
-                double weight_decay, int64_t step) {
+void adamw_step(py::handle params_, py::handle grads_, py::handle m_, py::handle v_, double lr, double beta1,
+                double beta2, double eps, double weight_decay, int64_t step) {
     const rg_adamw_config cfg = adamw_config(lr, beta1, beta2, eps, weight_decay, step);
+    const Listed params(params_, "parameters"), grads(grads_, "gradients"), m(m_, "moments"), v(v_, "moments");
     const bool gpu = adamw_parameters(params, grads);
     need(m.size() == params.size() && v.size() == params.size(), "adamw: as many moments as parameters");
     std::vector<rg_adamw_tensor> list(params.size());
@@ -428,35 +462,38 @@ void adamw_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gr
         return;
     }
     const repro_adamw::Scalars s = adamw_scalars(cfg);
-    py::gil_scoped_release nogil;
+    Unlocked unlocked;
     for (const rg_adamw_tensor& t : list) repro_adamw::cpu_adamw(t.p, t.g, t.m, t.v, t.n, s);
 }
 
 int64_t adamw8_blocks(int64_t n) { return (n + RG_ADAMW8_BLOCK - 1) / RG_ADAMW8_BLOCK; }
 
 void need_codes(const Tensor& t, const Tensor& p, int64_t n, const char* name) {
-    need(t.scalar_type() == torch::kUInt8 && t.is_contiguous() && t.device() == p.device() && t.numel() == n,
-         std::string("adamw: ") + name + " must be contiguous uint8 of " + std::to_string(n) + " values on the parameters' device");
-    need((reinterpret_cast<uintptr_t>(t.data_ptr()) & 3) == 0, std::string("adamw: ") + name + " must be at a multiple of 4 bytes");
+    if (t.scalar_type() == torch::kUInt8 && t.is_contiguous() && t.device() == p.device() && t.numel() == n &&
+        (reinterpret_cast<uintptr_t>(t.data_ptr()) & 3) == 0)
+        return;
+    need(false, std::string("adamw: ") + name + " must be contiguous uint8 of " + std::to_string(n) +
+                    " values, at a multiple of 4 bytes, on the parameters' device");
 }
 
 void need_exponents(const Tensor& t, const Tensor& p, int64_t n) {
-    need(t.scalar_type() == torch::kUInt8 && t.is_contiguous() && t.device() == p.device() && t.numel() == n,
-         "adamw: exponents must be contiguous uint8, one a block, on the parameters' device");
+    if (!(t.scalar_type() == torch::kUInt8 && t.is_contiguous() && t.device() == p.device() && t.numel() == n))
+        need(false, "adamw: exponents must be contiguous uint8, one a block, on the parameters' device");
 }
 
 // The moments' codes and exponents: one tensor of each for all parameters (each parameter at whole
 // blocks, in order), or one for each parameter.
-void adamw8_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& m,
-                 const std::vector<Tensor>& m_exp, const std::vector<Tensor>& v, const std::vector<Tensor>& v_exp,
-                 bool flat, double lr, double beta1, double beta2, double eps, double weight_decay,
+void adamw8_step(py::handle params_, py::handle grads_, py::handle m_, py::handle m_exp_, py::handle v_,
+                 py::handle v_exp_, bool flat, double lr, double beta1, double beta2, double eps, double weight_decay,
                  int64_t step) {
     const rg_adamw_config cfg = adamw_config(lr, beta1, beta2, eps, weight_decay, step);
+    const Listed params(params_, "parameters"), grads(grads_, "gradients"), m(m_, "moments"), m_exp(m_exp_, "exponents"),
+        v(v_, "moments"), v_exp(v_exp_, "exponents");
     const bool gpu = adamw_parameters(params, grads);
     const size_t states = flat ? 1 : params.size();
     need(m.size() == states && m_exp.size() == states && v.size() == states && v_exp.size() == states,
          "adamw: as many moments as parameters");
-    if (params.empty()) return;
+    if (params.size() == 0) return;
     const auto need_state = [&](size_t k, int64_t blocks) {
         need_codes(m[k], params[0], blocks * RG_ADAMW8_BLOCK, "the first moments");
         need_codes(v[k], params[0], blocks * RG_ADAMW8_BLOCK, "the second moments");
@@ -464,7 +501,7 @@ void adamw8_step(const std::vector<Tensor>& params, const std::vector<Tensor>& g
         need_exponents(v_exp[k], params[0], blocks);
     };
     int64_t total = 0;
-    for (const Tensor& p : params) total += adamw8_blocks(p.numel());
+    for (const Tensor* p : params.t) total += adamw8_blocks(p->numel());
     if (flat) need_state(0, total);
     int64_t at = 0;
     std::vector<rg_adamw8_tensor> list(params.size());
@@ -484,7 +521,7 @@ void adamw8_step(const std::vector<Tensor>& params, const std::vector<Tensor>& g
         return;
     }
     const repro_adamw::Scalars s = adamw_scalars(cfg);
-    py::gil_scoped_release nogil;
+    Unlocked unlocked;
     int64_t first = 0;
     for (const rg_adamw8_tensor& t : list) {
         repro_adamw::cpu_adamw8(t.p, t.g, t.m, t.m_exp, t.v, t.v_exp, t.n, first, s);
@@ -521,9 +558,8 @@ using OptTensor = c10::optional<Tensor>;
 // A float32 tensor of `numel` values on x's device, contiguous; undefined where there is none.
 Tensor norm_operand(const OptTensor& t, const Tensor& x, int64_t numel, const char* name) {
     if (!t.has_value()) return Tensor();
-    need(t->scalar_type() == torch::kFloat32, std::string("norm: ") + name + " must be float32");
-    need(t->device() == x.device(), std::string("norm: ") + name + " must be on x's device");
-    need(t->numel() == numel, std::string("norm: ") + name + " has the wrong number of values");
+    if (t->scalar_type() != torch::kFloat32 || t->device() != x.device() || t->numel() != numel)
+        need(false, std::string("norm: ") + name + " must be float32, on x's device, with " + std::to_string(numel) + " values");
     return t->resolve_neg().contiguous();
 }
 
@@ -533,14 +569,14 @@ float* out_or_null(Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullp
 rg_norm_config norm_config(const Tensor& x, const OptTensor& gate, bool rms, bool post, double eps, double scale) {
     require_f32(x, "x");
     need(x.is_cuda() || x.is_cpu(), "norm: tensors must be on the CPU or a GPU");
-    need(x.dim() == 2, "norm: x must be [rows, values]");
-    need(x.size(1) >= 1 && x.size(1) <= RG_NORM_MAX_D,
-         "norm: a row must have 1 to " + std::to_string(RG_NORM_MAX_D) + " values");
+    need(x.dim() >= 1 && x.size(-1) >= 1, "norm: x must be [..., values]");
+    need(x.size(-1) <= RG_NORM_MAX_D, "norm: a row must have at most 16384 values");
+    static_assert(RG_NORM_MAX_D == 16384, "the message above");
     need(eps >= 0, "norm: eps must not be negative");
     rg_norm_config c;
     rg_norm_config_init(&c);
-    c.N = x.size(0);
-    c.D = (int)x.size(1);
+    c.D = (int)x.size(-1);
+    c.N = x.numel() / c.D;
     c.rms = rms ? 1 : 0;
     c.post = post ? 1 : 0;
     c.eps = (float)eps;
@@ -554,7 +590,7 @@ rg_norm_config norm_config(const Tensor& x, const OptTensor& gate, bool rms, boo
     return c;
 }
 
-// x, f [N][D] -> {r (undefined without f), y, stats (undefined unless wanted)}
+// x, f [..., D] -> {r (undefined without f), y, stats (undefined unless wanted)}
 std::vector<OptTensor> residual_norm(Tensor x, OptTensor f_, OptTensor gate_, OptTensor post_weight_, OptTensor post_bias_,
                                      OptTensor weight_, OptTensor bias_, bool rms, bool post, double eps, double scale,
                                      bool want_stats, OptTensor flag, int op_id) {
@@ -579,7 +615,7 @@ std::vector<OptTensor> residual_norm(Tensor x, OptTensor f_, OptTensor gate_, Op
                                     flag.has_value() ? flag->data_ptr<int>() : nullptr, op_id, stream_of(x)),
               "residual norm");
     } else {
-        py::gil_scoped_release nogil;
+        Unlocked unlocked;
         repro_norm::cpu_residual_norm(c, x.data_ptr<float>(), data_or_null(f), data_or_null(gate), data_or_null(pw),
                                       data_or_null(pb), data_or_null(w), data_or_null(b), out_or_null(r),
                                       y.data_ptr<float>(), out_or_null(stats));
@@ -608,7 +644,8 @@ std::vector<OptTensor> residual_norm_grad(OptTensor dr_, OptTensor dy_, Tensor r
     need(dr.defined() || dy.defined(), "norm: a gradient of r or y is needed");
     const auto rows = r.options();
     const auto maybe = [&](int i, at::IntArrayRef shape) { return want[i] ? torch::empty(shape, rows) : Tensor(); };
-    Tensor dx = maybe(0, {c.N, D}), df = maybe(1, {c.N, D}), dgate = maybe(2, {std::max<int64_t>(c.gate_rows, 1), D});
+    Tensor dx = maybe(0, r.sizes()), df = maybe(1, r.sizes());
+    Tensor dgate = want[2] ? torch::empty(gate.sizes(), rows) : Tensor();
     Tensor dpw = maybe(3, {D}), dpb = maybe(4, {D}), dw = maybe(5, {D}), db = maybe(6, {D});
     if (!dy.defined()) {  // y was not used: its weight's gradients are zero
         for (Tensor* t : {&dw, &db})
@@ -633,7 +670,7 @@ std::vector<OptTensor> residual_norm_grad(OptTensor dr_, OptTensor dy_, Tensor r
                                          flag.has_value() ? flag->data_ptr<int>() : nullptr, op_id, stream_of(r)),
               "norm gradient");
     } else {
-        py::gil_scoped_release nogil;
+        Unlocked unlocked;
         repro_norm::cpu_residual_norm_grad(c, data_or_null(dr), data_or_null(dy), r.data_ptr<float>(), data_or_null(f),
                                            data_or_null(gate), data_or_null(pw), data_or_null(pb), data_or_null(w),
                                            stats.data_ptr<float>(), out_or_null(dx), out_or_null(df),
@@ -644,9 +681,94 @@ std::vector<OptTensor> residual_norm_grad(OptTensor dr_, OptTensor dy_, Tensor r
     return {opt(dx), opt(df), opt(dgate), opt(dpw), opt(dpb), opt(dw), opt(db)};
 }
 
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients that are not differentiable themselves: where a graph of the backward pass is wanted, using it
+// raises an error (and is not left out of it silently).
+void differentiable_once(variable_list& grads, const char* op) {
+    if (!at::GradMode::is_enabled()) return;
+    for (Tensor& g : grads) {
+        if (!g.defined()) continue;
+        torch::autograd::DelayedError error(std::string(op) + " is differentiable only once", 1);
+        g = error.apply({g.detach().requires_grad_()})[0];
+    }
+}
+
+OptTensor opt_of(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor or_undefined(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+// Where a module reports a NaN or infinity: an int32 cell of x's device (or nowhere) and the numbers of its
+// labels for the input and the gradient.
+struct Watch {
+    OptTensor cell;
+    int64_t input, gradient;
+};
+
+// Autograd in the binding (from Python, a norm's two passes took 130 us of host time, of the kernels' 46).
+// The operands are x, f, gate, post_weight, post_bias, weight, bias.
+struct NormFunction : torch::autograd::Function<NormFunction> {
+    static variable_list forward(AutogradContext* ctx, Tensor x, OptTensor f, OptTensor gate, OptTensor post_weight,
+                                 OptTensor post_bias, OptTensor weight, OptTensor bias, bool rms, bool post, double eps,
+                                 double scale, Watch watch, std::vector<bool> want) {
+        bool any = false;
+        for (const bool w : want) any = any || w;
+        auto out = residual_norm(x, f, gate, post_weight, post_bias, weight, bias, rms, post, eps, scale, any, watch.cell,
+                                 (int)watch.input);
+        if (any) {
+            ctx->save_for_backward({f.has_value() ? *out[0] : x, or_undefined(f), or_undefined(gate), or_undefined(post_weight),
+                                    or_undefined(post_bias), or_undefined(weight), *out[2]});
+            ctx->saved_data["settings"] = std::make_tuple(rms, post, eps, scale);
+            ctx->saved_data["cell"] = watch.cell;
+            ctx->saved_data["label"] = watch.gradient;
+            ctx->saved_data["want"] = c10::List<bool>({want[0], want[1], want[2], want[3], want[4], want[5], want[6]});
+        }
+        ctx->set_materialize_grads(false);
+        if (f.has_value()) return {*out[0], *out[1]};
+        return {*out[1]};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor dr = grads.size() > 1 ? grads[0] : Tensor(), dy = grads.back();
+        variable_list result(13);
+        if (!dr.defined() && !dy.defined()) return result;
+        const variable_list s = ctx->get_saved_variables();
+        const auto settings = ctx->saved_data["settings"].toTuple();
+        const auto list = ctx->saved_data["want"].toBoolList();
+        const std::vector<bool> want(list.begin(), list.end());
+        const auto out = residual_norm_grad(
+            opt_of(dr), opt_of(dy), s[0].resolve_neg().contiguous(), opt_of(s[1]), opt_of(s[2]), opt_of(s[3]), opt_of(s[4]),
+            opt_of(s[5]), s[6], settings->elements()[0].toBool(), settings->elements()[1].toBool(),
+            settings->elements()[2].toDouble(), settings->elements()[3].toDouble(), want,
+            ctx->saved_data["cell"].toOptional<Tensor>(), (int)ctx->saved_data["label"].toInt());
+        for (int i = 0; i < 7; ++i) result[i] = or_undefined(out[i]);
+        differentiable_once(result, "residual_norm");
+        return result;
+    }
+};
+
+// (y) or (r, y), differentiable; x and f of any leading dimensions.
+variable_list norm_apply(const Tensor& x, const OptTensor& f, const OptTensor& gate, const OptTensor& post_weight,
+                         const OptTensor& post_bias, const OptTensor& weight, const OptTensor& bias, bool rms, bool post,
+                         double eps, double scale, const OptTensor& cell, int64_t input_label, int64_t gradient_label) {
+    need(x.dim() >= 1 && x.size(-1) >= 1, "norm: x must be [..., values]");
+    need(!f.has_value() || f->sizes() == x.sizes(), "norm: f must have x's shape");
+    const int64_t d = x.size(-1);
+    need(!gate.has_value() || (gate->dim() >= 1 && gate->size(-1) == d), "norm: the gate's last dimension must be x's");
+    const std::pair<const OptTensor*, const char*> vectors[] = {
+        {&weight, "weight"}, {&bias, "bias"}, {&post_weight, "post_weight"}, {&post_bias, "post_bias"}};
+    for (const auto& v : vectors)
+        if (v.first->has_value() && !((*v.first)->dim() == 1 && (*v.first)->size(0) == d))
+            need(false, std::string("norm: ") + v.second + " must be [" + std::to_string(d) + "]");
+    std::vector<bool> want = {at::GradMode::is_enabled() && x.requires_grad()};
+    for (const OptTensor* t : {&f, &gate, &post_weight, &post_bias, &weight, &bias})
+        want.push_back(at::GradMode::is_enabled() && t->has_value() && (*t)->requires_grad());
+    return NormFunction::apply(x, f, gate, post_weight, post_bias, weight, bias, rms, post,
+                               eps, scale, Watch{cell, input_label, gradient_label}, want);
+}
+
 // ---- cross entropy of a vocabulary projection ----
 
-// {loss, dx, dweight}: x [N][D], weight [V][D], target [N]; factors [N] or none; the gradients that are wanted.
+// {loss, dx, dweight}: x [..., D], weight [V, D], target [...]; a factor for each token or none; what is wanted.
 std::vector<OptTensor> linear_cross_entropy(Tensor x, Tensor weight, Tensor target, OptTensor factors_, int S,
                                             int reduction, int64_t ignore_index, bool want_loss, bool want_dx,
                                             bool want_dw) {
@@ -655,10 +777,10 @@ std::vector<OptTensor> linear_cross_entropy(Tensor x, Tensor weight, Tensor targ
     const bool gpu = on_gpu(x, weight, "linear_cross_entropy");
     need(target.device() == x.device(), "linear_cross_entropy: tensors must be on the same device");
     need(target.scalar_type() == torch::kInt64, "linear_cross_entropy: target must be int64");
-    need(x.dim() == 2 && weight.dim() == 2 && x.size(1) == weight.size(1) && target.dim() == 1 && target.size(0) == x.size(0),
-         "linear_cross_entropy: x must be [tokens, size], weight [words, size], target [tokens]");
-    need(x.size(1) >= 1 && weight.size(0) >= 1, "linear_cross_entropy: sizes must be positive");
-    need(x.size(0) <= RG_LOSS_MAX_TOKENS && x.size(1) <= RG_LOSS_MAX_WORDS && weight.size(0) <= RG_LOSS_MAX_WORDS,
+    need(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1) && target.sizes() == x.sizes().slice(0, x.dim() - 1),
+         "linear_cross_entropy: x must be [..., size], weight [words, size], target [...]");
+    need(x.size(-1) >= 1 && weight.size(0) >= 1, "linear_cross_entropy: sizes must be positive");
+    need(target.numel() <= RG_LOSS_MAX_TOKENS && x.size(-1) <= RG_LOSS_MAX_SIZE && weight.size(0) <= RG_LOSS_MAX_WORDS,
          "linear_cross_entropy: too many tokens, values or words");
     need(S >= 1 && S <= 3, "linear_cross_entropy: slices must be 1..3");
     need(reduction >= RG_LOSS_MEAN && reduction <= RG_LOSS_NONE, "linear_cross_entropy: unknown reduction");
@@ -669,18 +791,18 @@ std::vector<OptTensor> linear_cross_entropy(Tensor x, Tensor weight, Tensor targ
     if (factors_.has_value()) {
         factors = factors_->resolve_neg().contiguous();
         require_f32(factors, "factors");
-        need(factors.device() == x.device() && factors.numel() == x.size(0), "linear_cross_entropy: one factor for each token");
+        need(factors.device() == x.device() && factors.numel() == target.numel(), "linear_cross_entropy: one factor for each token");
     }
     rg_loss_config c;
     rg_loss_config_init(&c);
-    c.N = x.size(0);
-    c.D = (int)x.size(1);
+    c.N = target.numel();
+    c.D = (int)x.size(-1);
     c.V = (int)weight.size(0);
     c.slices = S;
     c.reduction = reduction;
     c.ignore_index = ignore_index;
     Tensor loss, dx, dw;
-    if (want_loss) loss = reduction == RG_LOSS_NONE ? torch::empty({c.N}, x.options()) : torch::empty({}, x.options());
+    if (want_loss) loss = torch::empty(reduction == RG_LOSS_NONE ? target.sizes() : at::IntArrayRef(), x.options());
     if (want_dx) dx = torch::empty_like(x);
     if (want_dw) dw = torch::empty_like(weight);
     const auto* t = target.data_ptr<int64_t>();
@@ -694,12 +816,71 @@ std::vector<OptTensor> linear_cross_entropy(Tensor x, Tensor weight, Tensor targ
                                       out_or_null(dx), out_or_null(dw), ws.data_ptr(), (size_t)ws.numel(), stream_of(x)),
               "linear cross entropy");
     } else {
-        py::gil_scoped_release nogil;
+        Unlocked unlocked;
         repro_loss::cpu_linear_cross_entropy(c, x.data_ptr<float>(), weight.data_ptr<float>(), t, data_or_null(factors),
                                              out_or_null(loss), out_or_null(dx), out_or_null(dw));
     }
     const auto opt = [](const Tensor& v) { return v.defined() ? OptTensor(v) : OptTensor(); };
     return {opt(loss), opt(dx), opt(dw)};
+}
+
+void scale_(Tensor t, Tensor factor);
+
+// The loss, differentiable. With the sum or the mean, the forward pass leaves the gradients in the context
+// for the first backward pass to scale and hand out; a later one, and one without a reduction, computes them.
+struct LossFunction : torch::autograd::Function<LossFunction> {
+    static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, Tensor target, int64_t S, int64_t reduction,
+                          int64_t ignore_index, bool want_x, bool want_w) {
+        const bool early = reduction != RG_LOSS_NONE;
+        auto out = linear_cross_entropy(x, weight, target, OptTensor(), (int)S, (int)reduction, ignore_index, true,
+                                        want_x && early, want_w && early);
+        if (want_x || want_w) {
+            ctx->save_for_backward({x, weight, target});
+            ctx->saved_data["settings"] = std::make_tuple(S, reduction, ignore_index, want_x, want_w);
+            ctx->saved_data["ready"] = early;
+            if (early) {
+                ctx->saved_data["dx"] = out[1];
+                ctx->saved_data["dw"] = out[2];
+            }
+        }
+        return *out[0];
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list s = ctx->get_saved_variables();
+        const auto settings = ctx->saved_data["settings"].toTuple();
+        const auto& e = settings->elements();
+        const int S = (int)e[0].toInt(), reduction = (int)e[1].toInt();
+        const int64_t ignore_index = e[2].toInt();
+        const bool want_x = e[3].toBool(), want_w = e[4].toBool();
+        variable_list result(8);
+        OptTensor dx, dw;
+        if (ctx->saved_data["ready"].toBool()) {
+            dx = ctx->saved_data["dx"].toOptional<Tensor>();
+            dw = ctx->saved_data["dw"].toOptional<Tensor>();
+            ctx->saved_data["ready"] = false;
+            ctx->saved_data.erase("dx");
+            ctx->saved_data.erase("dw");
+        } else {
+            auto out = linear_cross_entropy(s[0], s[1], s[2], reduction == RG_LOSS_NONE ? OptTensor(grads[0]) : OptTensor(),
+                                            S, reduction, ignore_index, false, want_x, want_w);
+            dx = out[1];
+            dw = out[2];
+        }
+        if (reduction != RG_LOSS_NONE)
+            for (const OptTensor* g : {&dx, &dw})
+                if (g->has_value()) scale_(**g, grads[0]);
+        result[0] = or_undefined(dx);
+        result[1] = or_undefined(dw);
+        differentiable_once(result, "linear_cross_entropy");
+        return result;
+    }
+};
+
+Tensor loss_apply(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t S, int64_t reduction,
+                  int64_t ignore_index) {
+    const bool grad = at::GradMode::is_enabled();
+    return LossFunction::apply(x, weight, target, S, reduction, ignore_index, grad && x.requires_grad(),
+                               grad && weight.requires_grad());
 }
 
 // t *= factor[0] for a contiguous t; no write where the factor is 1.
@@ -749,10 +930,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw_step", &adamw_step);
     m.def("adamw8_step", &adamw8_step);
     m.def("adamw8_values", &adamw8_values);
-    m.def("residual_norm", &residual_norm);
-    m.def("residual_norm_grad", &residual_norm_grad);
-    m.def("linear_cross_entropy", &linear_cross_entropy);
-    m.def("scale_", &scale_);
+    m.def("norm_apply", &norm_apply);
+    m.def("loss_apply", &loss_apply);
     m.def("cpu_threads", &repro_gemm::cpu_thread_count);
     m.def("set_error_class", [](py::object cls) {
         Py_XINCREF(cls.ptr());
@@ -764,10 +943,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             if (p) std::rethrow_exception(p);
         } catch (const LibraryError& e) {
             if (!g_error_class) {
-                PyErr_SetString(PyExc_RuntimeError, (e.what + ": hip error " + std::to_string(e.code)).c_str());
+                PyErr_SetString(PyExc_RuntimeError, (e.message + ": hip error " + std::to_string(e.code)).c_str());
                 return;
             }
-            PyObject* err = PyObject_CallFunction(g_error_class, "is", e.code, e.what.c_str());
+            PyObject* err = PyObject_CallFunction(g_error_class, "is", e.code, e.what());
             if (err) {
                 PyErr_SetObject(g_error_class, err);
                 Py_DECREF(err);

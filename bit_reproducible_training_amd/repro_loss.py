@@ -22,38 +22,6 @@ __all__ = ["LinearCrossEntropy", "linear_cross_entropy"]
 _REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
-class _LossOp(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, target, settings):
-        slices, reduction, ignore_index, wanted = settings
-        early = reduction != 2
-        loss, dx, dw = _backend.linear_cross_entropy(x, weight, target, None, slices, reduction, ignore_index, True,
-                                                     wanted[0] and early, wanted[1] and early)
-        if any(wanted):
-            ctx.settings = settings
-            ctx.ready = (dx, dw) if early else None
-            ctx.save_for_backward(x, weight, target)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dloss):
-        slices, reduction, ignore_index, wanted = ctx.settings
-        x, weight, target = ctx.saved_tensors
-        if reduction == 2:
-            _, dx, dw = _backend.linear_cross_entropy(x, weight, target, dloss, slices, reduction, ignore_index, False,
-                                                      *wanted)
-            return dx, dw, None, None
-        ready, ctx.ready = ctx.ready, None
-        if ready is None:  # handed out by an earlier backward pass
-            ready = _backend.linear_cross_entropy(x, weight, target, None, slices, reduction, ignore_index, False,
-                                                  *wanted)[1:]
-        for g in ready:
-            if g is not None:
-                _backend.scale_(g, dloss)
-        return (*ready, None, None)
-
-
 def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mean", slices=None):
     """The cross entropy of softmax(x weight^T) against target, for float32 x [..., size], weight
     [words, size] and int64 target [...]; reduction "mean" (over the tokens that count), "sum", or
@@ -61,13 +29,8 @@ def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mea
     is no word has a NaN loss and no gradients. slices: the products' S (the layers' by default)."""
     if reduction not in _REDUCTIONS:
         raise ValueError('reduction must be "mean", "sum" or "none"')
-    if x.dim() < 1 or x.shape[-1] < 1 or tuple(target.shape) != tuple(x.shape[:-1]):
-        raise ValueError("linear_cross_entropy: x must be [..., size] and target [...]")
-    grad = torch.is_grad_enabled()
-    settings = (get_slices() if slices is None else int(slices), _REDUCTIONS[reduction], int(ignore_index),
-                (grad and x.requires_grad, grad and weight.requires_grad))
-    loss = _LossOp.apply(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1), settings)
-    return loss.view(target.shape) if reduction == "none" else loss
+    return _backend.loss_apply(x, weight, target, get_slices() if slices is None else int(slices), _REDUCTIONS[reduction],
+                               int(ignore_index))
 
 
 class LinearCrossEntropy(torch.nn.Module):

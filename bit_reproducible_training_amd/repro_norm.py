@@ -20,82 +20,26 @@ __all__ = ["Norm", "ResidualNorm", "norm", "residual_norm"]
 _KINDS = {"layer": False, "rms": True}
 
 
-class _NormOp(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, f, gate, post_weight, post_bias, weight, bias, settings, watch, wanted):
-        operands = (x, f, gate, post_weight, post_bias, weight, bias)
-        flag, number = watch.cell(x) if watch else (None, 0)
-        r, y, stats = _backend.residual_norm(*operands, *settings, wanted, flag, number)
-        if wanted:
-            ctx.save_for_backward(x if f is None else r, f, gate, post_weight, post_bias, weight, stats)
-            ctx.settings, ctx.watch = settings, watch
-        ctx.set_materialize_grads(False)
-        return (y,) if f is None else (r, y)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, *grads):
-        dr, dy = (None, grads[0]) if len(grads) == 1 else grads
-        if dr is None and dy is None:
-            return (None,) * 10
-        r, f, gate, post_weight, post_bias, weight, stats = ctx.saved_tensors
-        flag, number = ctx.watch.gradient_cell(r) if ctx.watch else (None, 0)
-        out = _backend.residual_norm_grad(dr, dy, r.contiguous(), f, gate, post_weight, post_bias, weight, stats,
-                                          *ctx.settings, list(ctx.needs_input_grad[:7]), flag, number)
-        if out[2] is not None:
-            out[2] = out[2].view(gate.shape)
-        return (*out, None, None, None)
-
-
-class _Watch:
-    """Where a module reports a NaN or infinity: the guard's cells, on a GPU in the norm's own launch."""
-
-    def __init__(self, name):
-        self.name, self.guard = name, guard()
-
-    def cell(self, x):
-        return self._cell(x, self.name + " input")
-
-    def gradient_cell(self, x):
-        return self._cell(x, self.name + " gradient")
-
-    def _cell(self, x, label):
-        if not x.is_cuda:
-            return None, 0
-        return self.guard._cell(x.device), self.guard._number(label)
-
-
-def _rows(t, d):
-    return None if t is None else t.reshape(-1, d)
-
-
-def _apply(x, f, weight, bias, kind, eps, gate, scale, post_norm, post_weight, post_bias, watch):
+def _apply(x, f, weight, bias, kind, eps, gate, scale, post_norm, post_weight, post_bias, name=None):
     if kind not in _KINDS:
         raise ValueError('kind must be "layer" or "rms"')
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("norm: x must be [..., values]")
-    if f is not None and f.shape != x.shape:
-        raise ValueError("norm: f must have x's shape")
-    d = x.shape[-1]
-    for name, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight), ("post_bias", post_bias)):
-        if t is not None and tuple(t.shape) != (d,):
-            raise ValueError("norm: %s must be [%d]" % (name, d))
-    if gate is not None and (gate.dim() < 1 or gate.shape[-1] != d):
-        raise ValueError("norm: the gate's last dimension must be x's")
-    if watch is not None and not x.is_cuda:
-        watch.guard.scan(x, watch.name + " input")
-        if f is not None:
-            watch.guard.scan(f, watch.name + " input")
-    settings = (_KINDS[kind], bool(post_norm), float(eps), float(scale))
-    operands = (_rows(x, d), _rows(f, d), gate, post_weight, post_bias, weight, bias)
-    wanted = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands)
-    out = _NormOp.apply(*operands, settings, watch, wanted)
-    return tuple(t.view(x.shape) for t in out)
+    cell, input_label, gradient_label = None, 0, 0
+    if name is not None:  # a module's: the guard hears of a NaN or infinity, on a GPU in the norm's own launch
+        watcher = guard()
+        if x.is_cuda:
+            cell = watcher._cell(x.device)
+            input_label, gradient_label = watcher._number(name + " input"), watcher._number(name + " gradient")
+        else:
+            watcher.scan(x, name + " input")
+            if f is not None:
+                watcher.scan(f, name + " input")
+    return _backend.norm_apply(x, f, gate, post_weight, post_bias, weight, bias, _KINDS[kind], bool(post_norm),
+                               float(eps), float(scale), cell, input_label, gradient_label)
 
 
 def norm(x, weight=None, bias=None, *, kind="layer", eps=1e-5):
     """Norm(x) * weight + bias over the last dimension (1 to 16384 values) of a float32 tensor."""
-    return _apply(x, None, weight, bias, kind, eps, None, 1.0, False, None, None, None)[0]
+    return _apply(x, None, weight, bias, kind, eps, None, 1.0, False, None, None)[0]
 
 
 def residual_norm(x, f, weight=None, bias=None, *, kind="layer", eps=1e-5, gate=None, scale=1.0, post_norm=False,
@@ -106,7 +50,8 @@ def residual_norm(x, f, weight=None, bias=None, *, kind="layer", eps=1e-5, gate=
     rows (its leading elements): each run of rows / G rows takes one of its rows. So [D] gates channels,
     [batch, D] gates each sequence of an x of [batch, tokens, D], and x's shape each value. Gradients
     reach every tensor; r and y may be used or not."""
-    return _apply(x, f, weight, bias, kind, eps, gate, scale, post_norm, post_weight, post_bias, None)
+    r, y = _apply(x, f, weight, bias, kind, eps, gate, scale, post_norm, post_weight, post_bias)
+    return r, y
 
 
 class Norm(torch.nn.Module):
@@ -125,7 +70,7 @@ class Norm(torch.nn.Module):
 
     def forward(self, x):
         return _apply(x, None, self.weight, self.bias, self.kind, self.eps, None, 1.0, False, None, None,
-                      _Watch(self.repro_name))[0]
+                      self.repro_name)[0]
 
 
 class ResidualNorm(Norm):
@@ -141,5 +86,6 @@ class ResidualNorm(Norm):
         self.post_bias = torch.nn.Parameter(torch.zeros(size)) if post_norm and self.bias is not None else None
 
     def forward(self, x, f, gate=None):
-        return _apply(x, f, self.weight, self.bias, self.kind, self.eps, gate, self.scale, self.post_norm,
-                      self.post_weight, self.post_bias, _Watch(self.repro_name))
+        r, y = _apply(x, f, self.weight, self.bias, self.kind, self.eps, gate, self.scale, self.post_norm,
+                      self.post_weight, self.post_bias, self.repro_name)
+        return r, y

@@ -33,12 +33,13 @@ extern "C" {
 enum { RG_LOSS_MEAN = 0, RG_LOSS_SUM = 1, RG_LOSS_NONE = 2 };
 
 #define RG_LOSS_MAX_TOKENS (1 << 22)
+#define RG_LOSS_MAX_SIZE (1 << 23)
 #define RG_LOSS_MAX_WORDS (1 << 28)
 
 typedef struct rg_loss_config {
     long long N;            /* tokens, 0 .. RG_LOSS_MAX_TOKENS */
-    int D, V;               /* 1 .. RG_LOSS_MAX_WORDS, and what the GEMM takes as its inner length: at
-                             * S = 3 about 1,000,000 */
+    int D, V;               /* 1 .. RG_LOSS_MAX_SIZE and 1 .. RG_LOSS_MAX_WORDS, and what the GEMM takes
+                             * as its inner length: at S = 3 about 1,000,000 */
     int slices;             /* S in 1..3 */
     int reduction;          /* RG_LOSS_* */
     long long ignore_index;

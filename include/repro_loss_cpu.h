@@ -75,7 +75,7 @@ inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, co
                 float m, s;
                 cpu_detail::largest_and_sum(q, V, m, s);
                 t = finish_token(m, s, q[word], g);
-                for (int v = 0; v < V; ++v) q[v] = exp_nonpositive(q[v] - t.top) * t.factor;
+                for (int v = 0; v < V; ++v) q[v] = dz_of(q[v], t.top, t.factor);
                 q[word] = 0.0f;
             } else {
                 if (word != c.ignore_index) t.loss = NAN;

@@ -13,8 +13,7 @@ using repro_gemm::bits_to_float;
 // exact: Cody and Waite's reduction), and Taylor's polynomial to r^7 / 7!, whose remainder is under
 // 2^-27 of the result. It never falls as x rises (checked for every float32): the largest of a row's
 // values is that of its largest x.
-RG_HD inline float exp_nonpositive(float x) {
-    if (!(x >= -87.0f)) return x == x ? 0.0f : x;
+RG_HD inline float exp_in_range(float x) {
     const float n = __builtin_rintf(x * 1.44269504f);
     float r = __builtin_fmaf(n, -0.693145751953125f, x);   // 0x1.62e4p-1
     r = __builtin_fmaf(n, -1.42860677e-6f, r);             // ln 2 - 0x1.62e4p-1
@@ -26,6 +25,14 @@ RG_HD inline float exp_nonpositive(float x) {
     p = __builtin_fmaf(p, r, 0.5f);
     p = 1.0f + __builtin_fmaf(r * r, p, r);
     return p * bits_to_float((uint32_t)((int)n + 127) << 23);
+}
+
+RG_HD inline float exp_nonpositive(float x) { return x >= -87.0f ? exp_in_range(x) : x == x ? 0.0f : x; }
+
+// One word's share of dz (the target's is elsewhere): 0 in a row whose factor is 0, whatever its logits.
+RG_HD inline float dz_of(float z, float top, float factor) {
+    const float x = z - top;
+    return x >= -87.0f && factor != 0.0f ? exp_in_range(x) * factor : 0.0f;
 }
 
 // ln s in binary64 for a positive normal float32, NaN or infinity (returned as they are): s = 2^e m with m in
@@ -77,11 +84,17 @@ struct Token {
     float loss;
 };
 
+// Where a logit or the weight is not finite, the token's row of dz is 0 (factor 0) and its target word's
+// share NaN, so that dx and the target's row of dw are.
 RG_HD inline Token finish_token(float m, float s, float zt, float weight) {
     Token t;
     t.top = m;
     t.factor = weight / s;
     t.target = exp_nonpositive(zt - m) * t.factor - weight;
+    if (!(__builtin_fabsf(t.factor) < 3.4028235e38f) || !(__builtin_fabsf(m) < 3.4028235e38f)) {
+        t.factor = 0.0f;
+        t.target = __builtin_nanf("");
+    }
     t.loss = (float)(((double)m - (double)zt) + log_positive(s));
     return t;
 }

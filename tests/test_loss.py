@@ -279,3 +279,32 @@ def test_module_reports_to_the_guard():
     m(x, t)
     assert rg.guard().first_offender() == "head input"
     rg.guard().reset()
+
+
+def test_gradients_are_differentiable_no_further():
+    x, w, t = case(6, 8, 20)
+    x.requires_grad_()
+    loss = rg.linear_cross_entropy(x, w, t)
+    (dx,) = torch.autograd.grad(loss, [x], create_graph=True)
+    assert torch.equal(dx, results(x, w, t)[1])
+    with pytest.raises(RuntimeError, match="only once"):
+        dx.sum().backward()
+
+
+def test_backward_passes_of_several_threads():
+    """The binding's backward passes run with and without the interpreter's lock."""
+    import threading
+
+    x, w, t = case(40, 16, 300, seed=3)
+    want = results(x, w, t)
+    got = [None] * 4
+
+    def work(i):
+        got[i] = results(x, w, t)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))

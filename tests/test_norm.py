@@ -287,3 +287,12 @@ def test_modules_report_to_the_guard():
     rg.guard().reset()
     n = rg.Norm(16, kind="rms")
     assert n.bias is None and torch.equal(n(x), rg.norm(x, n.weight, kind="rms"))
+
+
+def test_gradients_are_differentiable_no_further():
+    t, settings, up = case(5, 16, "layer", None)
+    x = t["x"].requires_grad_()
+    r, y = call(t, settings)
+    (dx,) = torch.autograd.grad((r, y), [x], up, create_graph=True)
+    with pytest.raises(RuntimeError, match="only once"):
+        dx.sum().backward()

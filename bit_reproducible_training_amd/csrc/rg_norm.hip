@@ -93,33 +93,58 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v + rotated<0x121>(v);
 }
 
-// Sums over a row, in the order of repro_norm_math.h. `turn` alternates the exchange's halves, so one
-// barrier a sum is enough.
+// Sums over a row, in the order of repro_norm_math.h. One wavefront needs no exchange. With as many threads as
+// strands a thread holds a strand; with twice as many, its chunks are added after the exchange. `turn`
+// alternates the exchange's halves, so one barrier a sum is enough.
 template <int WAVES, int NK>
 struct RowSum {
-    static constexpr int T = 64 * WAVES;
-    float* lds;  // 2 * 2 * T floats (WAVES > 1)
+    static constexpr int T = 64 * WAVES, CHUNKS = T * NK;
+    static constexpr int STRANDS = CHUNKS <= 1024 ? 256 : 1024;  // a row of at most 4096 values: 256
+    static constexpr bool JOINED = T <= STRANDS;                 // a thread adds up its strand itself
+    static constexpr int HELD = JOINED ? T : CHUNKS;             // values exchanged for a sum
+    static constexpr int LDS = WAVES == 1 ? 1 : 4 * HELD;
+    float* lds;  // LDS floats
     int t, D, turn;
 
     template <class F>
-    __device__ __forceinline__ float strand(F value) const {
-        float s = 0.0f;
+    __device__ __forceinline__ float chunk(int k, F value) const {
+        float v[4];
 #pragma unroll
-        for (int k = 0; k < NK; ++k) {
-            float v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = 4 * (t + T * k) + i < D ? value(k, i) : 0.0f;
-            const float q = (v[0] + v[1]) + (v[2] + v[3]);
-            s = k == 0 ? q : (4 * (t + T * k) < D ? s + q : s);
-        }
-        return s;
+        for (int i = 0; i < 4; ++i) v[i] = 4 * (t + T * k) + i < D ? value(k, i) : 0.0f;
+        return (v[0] + v[1]) + (v[2] + v[3]);
     }
-    __device__ __forceinline__ static float tree(const float* __restrict__ p, int lane) {
-        float v[WAVES];
+    template <class F>
+    __device__ __forceinline__ void put(float* __restrict__ p, F value) const {
+        if constexpr (JOINED) {
+            float s = chunk(0, value);
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v[w] = p[64 * w + lane];
+            for (int k = 1; k < NK; ++k) {
+                const float q = chunk(k, value);
+                s = 4 * (t + T * k) < D ? s + q : s;
+            }
+            p[t] = s;
+        } else {
 #pragma unroll
-        for (int n = WAVES / 2; n > 0; n /= 2)
+            for (int k = 0; k < NK; ++k) p[t + T * k] = chunk(k, value);
+        }
+    }
+    __device__ __forceinline__ float take(const float* __restrict__ p) const {
+        constexpr int N = JOINED ? WAVES : STRANDS / 64;
+        const int lane = t & 63;
+        float v[N];
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+            v[w] = p[64 * w + lane];
+            if constexpr (!JOINED) {
+#pragma unroll
+                for (int c = STRANDS; c < CHUNKS; c += STRANDS) {
+                    const float q = p[c + 64 * w + lane];
+                    v[w] = 4 * (c + 64 * w + lane) < D ? v[w] + q : v[w];
+                }
+            }
+        }
+#pragma unroll
+        for (int n = N / 2; n > 0; n /= 2)
 #pragma unroll
             for (int w = 0; w < n; ++w) v[w] = v[2 * w] + v[2 * w + 1];
         return wave_sum(v[0]);
@@ -129,19 +154,14 @@ struct RowSum {
         if constexpr (WAVES == 1) {
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = 4 * (t + T * k) + i < D ? value(k, i) : 0.0f;
-                s[k] = (v[0] + v[1]) + (v[2] + v[3]);
-            }
+            for (int k = 0; k < NK; ++k) s[k] = chunk(k, value);
             return wave_sum((s[0] + s[1]) + (s[2] + s[3]));
         } else {
-            float* p = lds + turn * 2 * T;
+            float* p = lds + turn * 2 * HELD;
             turn ^= 1;
-            p[t] = strand(value);
+            put(p, value);
             __syncthreads();
-            return tree(p, t & 63);
+            return take(p);
         }
     }
     template <class F, class G>
@@ -150,13 +170,13 @@ struct RowSum {
             a = one(f);
             b = one(g);
         } else {
-            float* p = lds + turn * 2 * T;
+            float* p = lds + turn * 2 * HELD;
             turn ^= 1;
-            p[t] = strand(f);
-            p[T + t] = strand(g);
+            put(p, f);
+            put(p + HELD, g);
             __syncthreads();
-            a = tree(p, t & 63);
-            b = tree(p + T, t & 63);
+            a = take(p);
+            b = take(p + HELD);
         }
     }
 };
@@ -191,7 +211,7 @@ norm_forward(Sizes z, long long group, const float* __restrict__ x, const float*
              const float* __restrict__ bias, float* __restrict__ r, float* __restrict__ y,
              float* __restrict__ stats, int* flag, int op_id) {
     constexpr int T = 64 * WAVES, ROWS = WAVES == 1 ? 4 : 1;
-    __shared__ float lds[WAVES == 1 ? 1 : 4 * T];
+    __shared__ float lds[RowSum<WAVES, NK>::LDS];
     const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
     RowSum<WAVES, NK> sum{lds, t, z.D, 0};
     const int sub = WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
@@ -253,7 +273,7 @@ struct Parts {
 };
 
 template <int WAVES, int NK, bool POST, bool GATED>
-__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES)
+__global__ void __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES, WAVES == 1 ? 2 : 4)
 norm_backward(Sizes z, Partition pt, const float* __restrict__ dr, const float* __restrict__ dy,
               const float* __restrict__ r, const float* __restrict__ f, const float* __restrict__ gate,
               const float* __restrict__ post_weight, const float* __restrict__ post_bias,
@@ -261,7 +281,7 @@ norm_backward(Sizes z, Partition pt, const float* __restrict__ dr, const float* 
               float* __restrict__ df, float* __restrict__ dgate, Parts parts, int* flag, int op_id) {
     constexpr int T = 64 * WAVES;
     using Row = Chunks<T, NK>;
-    __shared__ float lds[WAVES == 1 ? 4 * T * NK * 4 : 4 * T];
+    __shared__ float lds[WAVES == 1 ? 4 * T * NK * 4 : RowSum<WAVES, NK>::LDS];
     const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
     const int sub = WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     RowSum<WAVES, NK> sum{lds, t, z.D, 0};
@@ -471,13 +491,14 @@ void with_row(int D, F run) {
     constexpr integral_constant<int, 2> two;
     constexpr integral_constant<int, 3> three;
     constexpr integral_constant<int, 4> four;
+    constexpr integral_constant<int, 8> eight;
     constexpr integral_constant<int, 16> sixteen;
     if (D <= 256) of(one, one);
     else if (D <= 512) of(one, two);
     else if (D <= 768) of(one, three);
     else if (D <= 1024) of(one, four);
-    else if (D <= 2048) of(four, two);
-    else if (D <= 4096) of(four, four);
+    else if (D <= 2048) of(eight, one);
+    else if (D <= 4096) of(eight, two);
     else if (D <= 8192) of(sixteen, two);
     else of(sixteen, four);
 }

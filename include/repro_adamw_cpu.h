@@ -39,10 +39,9 @@ inline void cpu_adamw8(float* p, const float* g, uint8_t* m, uint8_t* m_exp, uin
         m_exp[b] = (uint8_t)shared_exponent(top_m, SPAN_M);
         v_exp[b] = (uint8_t)shared_exponent(top_v, SPAN_V);
         for (int i = 0; i < BLOCK; ++i) {
-            float um, uv;
-            rounding((uint32_t)((first + b) * BLOCK + i), s.salt, um, uv);
-            m[base + i] = encode_m(mv[i], m_exp[b], um);
-            v[base + i] = encode_v(vv[i], v_exp[b], uv);
+            const uint32_t u = rounding((uint32_t)((first + b) * BLOCK + i), s.salt);
+            m[base + i] = encode_m(mv[i], m_exp[b], u & 0xFFFFu);
+            v[base + i] = encode_v(vv[i], v_exp[b], u >> 16);
         }
     });
 }

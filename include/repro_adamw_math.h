@@ -74,15 +74,8 @@ RG_HD inline uint32_t mix(uint32_t h) {
 }
 
 // The rounding numbers of the value at `position` (counted over the call's tensors, each starting at
-// a whole block): 16 bits for each moment, as values in [0, 1).
-RG_HD inline void rounding(uint32_t position, uint32_t salt, float& um, float& uv) {
-    const uint32_t h = mix(position ^ salt);
-    um = (float)(int)(h & 0xFFFFu) * (1.0f / 65536.0f);
-    uv = (float)(int)(h >> 16) * (1.0f / 65536.0f);
-}
-
-// 2^(field - 127), 0 where that is below the normal range.
-RG_HD inline float pow2_field(int field) { return bits_to_float((uint32_t)(field > 0 ? field : 0) << 23); }
+// a whole block), 16 bits for each moment, the first one's the lower.
+RG_HD inline uint32_t rounding(uint32_t position, uint32_t salt) { return mix(position ^ salt); }
 
 // Magnitude whose exponent a block shares; infinities and NaN count as the largest finite number.
 RG_HD inline uint32_t magnitude_bits(float x) {
@@ -95,33 +88,39 @@ RG_HD inline int shared_exponent(uint32_t largest_bits, int span) {
     return e > span + 4 ? e : span + 4;
 }
 
-RG_HD inline int encode_magnitude(uint32_t bits, int e, int span, float u, bool keep_positive) {
-    const int own = (int)(bits >> 23), low = e - span;
-    const int k = own > low ? own : low;
-    const float t = bits_to_float(bits) * pow2_field(257 - k);  // exact, below 16
+// The code of a magnitude, for a rounding number u16 / 65536. From 2^(e - span) on a code is the magnitude's
+// exponent and upper three mantissa bits, so rounding is an addition to the float's bits whose carry
+// goes where it should: 2^20 - 1 - 16 u16 carries where the lower 20 bits exceed 16 u16. Below, the
+// magnitude is counted in steps of 2^(e - span - 130).
+RG_HD inline int encode_magnitude(uint32_t bits, int e, int span, uint32_t u16, bool keep_positive) {
+    const int low = e - span;  // an exponent field of at least 4
+    const int large = (int)((bits + 0xFFFFFu - (u16 << 4)) >> 20) - 8 * (low - 1);
+    const float t = bits_to_float(bits) * bits_to_float((uint32_t)(257 - low) << 23);  // exact where below 8
     const float whole = __builtin_floorf(t);
-    int q = (int)whole + (t - whole > u ? 1 : 0);
-    if (keep_positive && bits != 0 && q == 0) q = 1;
-    const int code = 8 * (k - low) + q, top = 8 * span + 15;
+    int small = (int)whole + (t - whole > (float)(int)u16 * (1.0f / 65536.0f) ? 1 : 0);
+    if (keep_positive) small = bits != 0 && small == 0 ? 1 : small;
+    const int code = bits < (uint32_t)low << 23 ? small : large, top = 8 * span + 15;
     return code < top ? code : top;
 }
 
+// A code's magnitude: its bits, or below 2^(e - span) those beside 2^(e - span), which is taken away.
 RG_HD inline float decode_magnitude(int code, int e, int span) {
-    const int up = (code >> 3) - 1;
-    const int q = code < 8 ? code : 8 + (code & 7);
-    return (float)q * pow2_field(e - span + (up > 0 ? up : 0) - 3);
+    const int low = e > span + 4 ? e - span : 4;  // (before the first step e is 0, as the codes are)
+    const uint32_t large = ((uint32_t)code << 20) + ((uint32_t)(low - 1) << 23);
+    const float one = bits_to_float((uint32_t)low << 23);
+    return code < 8 ? bits_to_float(large + (1u << 23)) - one : bits_to_float(large);
 }
 
-RG_HD inline uint8_t encode_m(float m, int e, float u) {
-    const int c = encode_magnitude(magnitude_bits(m), e, SPAN_M, u, false);
+RG_HD inline uint8_t encode_m(float m, int e, uint32_t u16) {
+    const int c = encode_magnitude(magnitude_bits(m), e, SPAN_M, u16, false);
     return (uint8_t)(m < 0.0f ? c + 128 : c);
 }
 RG_HD inline float decode_m(uint8_t code, int e) {
     const float a = decode_magnitude(code & 127, e, SPAN_M);
     return code & 128 ? -a : a;
 }
-RG_HD inline uint8_t encode_v(float v, int e, float u) {
-    return (uint8_t)encode_magnitude(magnitude_bits(v), e, SPAN_V, u, true);
+RG_HD inline uint8_t encode_v(float v, int e, uint32_t u16) {
+    return (uint8_t)encode_magnitude(magnitude_bits(v), e, SPAN_V, u16, true);
 }
 RG_HD inline float decode_v(uint8_t code, int e) { return decode_magnitude(code, e, SPAN_V); }
 

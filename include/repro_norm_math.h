@@ -39,7 +39,7 @@ struct Partition {
 inline Partition partition(long long N, int D, long long G) {
     Partition p;
     p.join = D <= 1024 ? 4 : 1;
-    const long long aim = D <= 1024 ? 2048 : D <= 4096 ? 1024 : 512;
+    const long long aim = D <= 1024 ? 2048 : 512;
     const long long rows = (N + aim - 1) / aim;
     p.rows = (int)(rows > 4 ? rows : 4);
     p.group_rows = G > 0 ? N / G : N;

@@ -215,14 +215,23 @@ norm_forward(Sizes z, long long group, const float* __restrict__ x, const float*
     const int t = WAVES == 1 ? threadIdx.x & 63 : threadIdx.x;
     RowSum<WAVES, NK> sum{lds, t, z.D, 0};
     const int sub = WAVES == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
-    for (long long n = (long long)blockIdx.x * ROWS + sub; n < z.N; n += (long long)gridDim.x * ROWS) {
+    const long long step = (long long)gridDim.x * ROWS;
+    constexpr bool AHEAD = WAVES > 1;  // the next row's values are in flight while a row is worked on
+    Chunks<T, NK> next_x, next_f;
+    const auto fetch = [&](long long n) {
+        if (n >= z.N) return;
+        next_x.load(x + (size_t)n * z.D, z.D, t);
+        if (f != nullptr) next_f.load(f + (size_t)n * z.D, z.D, t);
+    };
+    long long n = (long long)blockIdx.x * ROWS + sub;
+    if (AHEAD) fetch(n);
+    for (; n < z.N; n += step) {
         const size_t at = (size_t)n * z.D;
-        Chunks<T, NK> v, w;
-        v.load(x + at, z.D, t);
+        if (!AHEAD) fetch(n);
+        Chunks<T, NK> v = next_x, u = next_f, w;
+        if (AHEAD) fetch(n + step);
         repro_norm::RowStats sf{0.0f, 0.0f};
         if (f != nullptr) {
-            Chunks<T, NK> u;
-            u.load(f + at, z.D, t);
             if constexpr (POST) {
                 sf = stats_of<WAVES, NK>(u, sum, z);
                 Chunks<T, NK> b;
@@ -291,17 +300,36 @@ norm_backward(Sizes z, Partition pt, const float* __restrict__ dr, const float* 
     Row acc[SUMS];
 #pragma unroll
     for (int q = 0; q < SUMS; ++q) acc[q].clear();
+    // Where four values a thread make a row, its weights stay in registers and the next row's values are in
+    // flight while a row is worked on.
+    constexpr bool AHEAD = WAVES > 1 && NK == 1;
+    Row next_r, next_dy, next_dr, next_f, held_w, held_pw, held_pb;
+    float4 next_st;
+    const auto fetch = [&](long long k0) {
+        if (k0 >= end) return;
+        const long long n = section * pt.section_rows + k0;
+        const size_t at = (size_t)n * z.D;
+        next_st = *reinterpret_cast<const float4*>(stats + 4 * n);
+        next_r.load(r + at, z.D, t);
+        if (dy != nullptr) next_dy.load(dy + at, z.D, t);
+        if (dr != nullptr) next_dr.load(dr + at, z.D, t);
+        if (f != nullptr) next_f.load(f + at, z.D, t);
+    };
+    if (AHEAD) {
+        fetch(first);
+        if (weight != nullptr) held_w.load(weight, z.D, t);
+        if (POST && post_weight != nullptr) held_pw.load(post_weight, z.D, t);
+        if (POST && GATED && post_bias != nullptr) held_pb.load(post_bias, z.D, t);
+    }
     for (long long k0 = first; k0 < end; ++k0) {
         const long long n = section * pt.section_rows + k0;
         const size_t at = (size_t)n * z.D;
-        const float4 st = *reinterpret_cast<const float4*>(stats + 4 * n);
-        Row hat, d, a, u, w;
-        hat.load(r + at, z.D, t);
-        if (dy != nullptr) a.load(dy + at, z.D, t);
-        if (dr != nullptr) d.load(dr + at, z.D, t);
-        if (f != nullptr) u.load(f + at, z.D, t);
+        if (!AHEAD) fetch(k0);
+        const float4 st = next_st;
+        Row hat = next_r, a = next_dy, d = next_dr, u = next_f, w = held_w;
+        if (AHEAD) fetch(k0 + 1);
         if (dy != nullptr) {
-            if (weight != nullptr) w.load(weight, z.D, t);
+            if (!AHEAD && weight != nullptr) w.load(weight, z.D, t);
 #pragma unroll
             for (int k = 0; k < NK; ++k)
 #pragma unroll
@@ -349,10 +377,11 @@ norm_backward(Sizes z, Partition pt, const float* __restrict__ dr, const float* 
             for (int k = 0; k < NK; ++k)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) hat.v[k][i] = centred(u.v[k][i], st.z, z.layer) * st.w;
-            if (post_weight != nullptr) w.load(post_weight, z.D, t);
+            if (AHEAD) w = held_pw;
+            else if (post_weight != nullptr) w.load(post_weight, z.D, t);
             if (GATED) {
-                Row b;
-                if (post_bias != nullptr) b.load(post_bias, z.D, t);
+                Row b = held_pb;
+                if (!AHEAD && post_bias != nullptr) b.load(post_bias, z.D, t);
 #pragma unroll
                 for (int k = 0; k < NK; ++k)
 #pragma unroll
@@ -482,9 +511,14 @@ bool sizes_ok(const rg_norm_config* c) {
 
 Sizes sizes_of(const rg_norm_config* c) { return Sizes{c->N, c->D, c->eps, c->scale, c->rms == 0}; }
 
-// run(WAVES, NK) with the values that hold a row of D.
+// Blocks of a forward launch whose rows take a block each: two a compute unit, each with a row ahead.
+constexpr long long FORWARD_BLOCKS = 512;
+
+// run(WAVES, NK) with the values that hold a row of D. Rows of 2049 to 4096 values take eight wavefronts in the
+// forward pass (sixteen wait for each other at its barriers: 4096 rows of 4096 59 -> 82 us) and sixteen
+// in the backward pass, whose sums over rows would not leave registers for two rows otherwise.
 template <class F>
-void with_row(int D, F run) {
+void with_row(int D, bool forward, F run) {
     using std::integral_constant;
     const auto of = [&](auto waves, auto nk) { run(waves, nk); };
     constexpr integral_constant<int, 1> one;
@@ -498,7 +532,8 @@ void with_row(int D, F run) {
     else if (D <= 768) of(one, three);
     else if (D <= 1024) of(one, four);
     else if (D <= 2048) of(eight, one);
-    else if (D <= 4096) of(eight, two);
+    else if (D <= 4096 && forward) of(eight, two);
+    else if (D <= 4096) of(sixteen, one);
     else if (D <= 8192) of(sixteen, two);
     else of(sixteen, four);
 }
@@ -531,11 +566,12 @@ int rg_residual_norm_fp32(const rg_norm_config* cfg, const float* x, const float
         return hipErrorInvalidValue;
     const Sizes z = sizes_of(cfg);
     const long long group = cfg->gate_rows > 0 ? cfg->N / cfg->gate_rows : 1;
-    with_row(cfg->D, [&](auto waves, auto nk) {
+    with_row(cfg->D, true, [&](auto waves, auto nk) {
         constexpr int WV = decltype(waves)::value, NK = decltype(nk)::value;
         constexpr int rows = WV == 1 ? 4 : 1;
         const long long needed = (cfg->N + rows - 1) / rows;
-        const dim3 grid((unsigned)(needed < (1 << 20) ? needed : (1 << 20))), block(WV == 1 ? 256 : 64 * WV);
+        const long long most = WV == 1 ? 1 << 20 : FORWARD_BLOCKS;
+        const dim3 grid((unsigned)(needed < most ? needed : most)), block(WV == 1 ? 256 : 64 * WV);
         auto kernel = cfg->post ? norm_forward<WV, NK, true> : norm_forward<WV, NK, false>;
         hipLaunchKernelGGL(kernel, grid, block, 0, static_cast<hipStream_t>(stream), z, group, x, f, gate, post_weight,
                            post_bias, weight, bias, r, y, stats, flag, op_id);
@@ -591,7 +627,7 @@ int rg_residual_norm_grad_fp32(const rg_norm_config* cfg, const float* dr, const
     }
     const Sizes z = sizes_of(cfg);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    with_row(cfg->D, [&](auto waves, auto nk) {
+    with_row(cfg->D, false, [&](auto waves, auto nk) {
         constexpr int WV = decltype(waves)::value, NK = decltype(nk)::value;
         auto kernel = cfg->post ? (gate ? norm_backward<WV, NK, true, true> : norm_backward<WV, NK, true, false>)
                                 : (gate ? norm_backward<WV, NK, false, true> : norm_backward<WV, NK, false, false>);

@@ -216,7 +216,8 @@ _MODEL_SIGNATURES = {
                                                          ctypes.POINTER(ctypes.c_size_t)]),
     "rg_linear_cross_entropy": (ctypes.c_int, [ctypes.POINTER(rg_loss_config)] + [ctypes.c_void_p] * 8 +
                                 [ctypes.c_size_t, ctypes.c_void_p]),
-    "rg_scale_fp32": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "rg_scale_fp32": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_size_t,
+                                     ctypes.c_void_p, ctypes.c_void_p]),
     "rg_norm_config_init": (None, [ctypes.POINTER(rg_norm_config)]),
     "rg_residual_norm_fp32": (ctypes.c_int, [ctypes.POINTER(rg_norm_config)] + [ctypes.c_void_p] * 11 +
                               [ctypes.c_int, ctypes.c_void_p]),

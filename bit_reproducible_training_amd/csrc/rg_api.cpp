@@ -494,12 +494,27 @@ size_t slice_scratch_bytes(int R, int K, bool strided) {
     return (size_t)std::max(nch, parts) * round_up(R, STEP_K) * sizeof(float);
 }
 
-int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
-                 hipStream_t stream) {
+static SliceDesc slice_alone(const float* src, int R, int K, bool strided, int8_t* out, int* expo, float* scratch) {
     int nch, kch;
     choose_chunks(R, R, K, strided, &nch, &kch);
-    const SliceDesc d = make_slice_desc(src, R, K, round_up(R, STEP_K), round_up(K, STEP_K), strided, strided ? R : K, 1,
-                                        0, nch, kch, scratch, out, expo);
+    return make_slice_desc(src, R, K, round_up(R, STEP_K), round_up(K, STEP_K), strided, strided ? R : K, 1, 0, nch, kch,
+                           scratch, out, expo);
+}
+
+int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, const float* b, int Rb, int8_t* qb, int* eb, int K, int S,
+                      float* scratch, hipStream_t stream) {
+    const SliceDesc da = slice_alone(a, Ra, K, false, qa, ea, scratch), db = slice_alone(b, Rb, K, false, qb, eb, scratch);
+    if (!onepass_eligible(da)) {
+        const int rc = launch_slice(a, Ra, K, false, S, qa, ea, scratch, stream);
+        return rc != hipSuccess ? rc : launch_slice(b, Rb, K, false, S, qb, eb, scratch, stream);
+    }
+    launch_onepass(da, true, db, true, S, stream);
+    return hipGetLastError();
+}
+
+int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
+                 hipStream_t stream) {
+    const SliceDesc d = slice_alone(src, R, K, strided, out, expo, scratch);
     SliceDesc none = d;
     none.max_blocks = 0;
     none.split_blocks = 0;

@@ -391,6 +391,9 @@ int gemm_launch(const float* A, const float* B, float* C, const Layout& L, char*
 size_t slice_scratch_bytes(int R, int K, bool strided);
 int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
                  hipStream_t stream);
+// Two row-access operands of one K, in one launch where one pass takes them.
+int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, const float* b, int Rb, int8_t* qb, int* eb, int K, int S,
+                      float* scratch, hipStream_t stream);
 
 // Kernel launchers (asynchronous on `stream`).
 void launch_absmax(const SliceDesc& a, const SliceDesc& b, hipStream_t stream);

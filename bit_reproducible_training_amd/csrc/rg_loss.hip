@@ -41,80 +41,91 @@ struct Targets {
     int* counted;  // [1] tokens that are not left out
 };
 
-// One block: the words' counts by atomics, then places for their tokens. A word's place and its tokens'
-// order in `arrived` change from run to run and reach no result: loss_tokens puts them in order. The
-// block waits for memory nearly all the time, so a thread has BATCH tokens in flight, and the block runs
-// beside those of the first group's loss_parts, which take longer from some 1000 tokens of 50257 words
-// on (8192 tokens: 73 us as a launch of its own with a token at a time; every token compared with every
-// other one, 170 us, and 64 times that for 65536). lists: whether the tokens are listed.
-__device__ void words_block(const long long* __restrict__ target, long long ignore_index, int N, int V, bool lists,
-                            const Targets& t) {
-    constexpr int BATCH = 8;
+// The words' counts by atomics, then places for their tokens. A word's place and its tokens' order in
+// `arrived` change from run to run and reach no result: loss_tokens puts them in order. lists: whether
+// the tokens are listed.
+// Each block owns the words of every gridDim.x-th cache line of `count` (gridDim.x a power of two) and reads all targets, so blocks
+// need nothing of each other: the places before its own are those of the tokens of the blocks before it. The
+// scattered accesses are what takes time, at one compute unit's rate (8192 tokens of 50257 words: 66 us by
+// one block, 26 by 16; every token compared with every other one took 170, and 64 times that for 65536).
+// A thread has BATCH tokens in flight.
+__global__ void __launch_bounds__(1024)
+loss_words(const long long* __restrict__ target, long long ignore_index, int N, int V, bool lists, Targets t) {
+    constexpr int BATCH = 8, threads = 1024, LINE = 32;
     __shared__ int places, kept;
-    const int threads = blockDim.x;
+    const int blocks = gridDim.x, self = blockIdx.x;
+    // A block's memory operations all meet in its XCD's L2: loads that pass the L1 by, after a barrier that waits
+    // for every wavefront's stores and atomics there, see them. (Device-scope fences between the phases
+    // write the whole L2 back: 20 us each here.)
     const auto load = [](const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    const auto store = [](int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    const auto phase_end = []() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    const auto read = [&](int n) {
+        const long long v = n < N ? target[n] : ignore_index;
+        return v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
+    };
     if (threadIdx.x == 0) places = kept = 0;
-    if (lists)
-        for (int v = threadIdx.x; v < V; v += threads) store(&t.count[v], 0);
-    __threadfence();
-    __syncthreads();
-    int mine = 0;
+    if (lists) {
+        const int lines = (V + LINE - 1) / LINE;
+        for (int i = threadIdx.x; i < (lines - self + blocks - 1) / blocks * LINE; i += threads) {
+            const int v = (i / LINE * blocks + self) * LINE + i % LINE;
+            if (v < V) t.count[v] = 0;
+        }
+    }
+    phase_end();
+    int count = 0, before = 0;
     for (int base = threadIdx.x; base < N; base += threads * BATCH) {
         int w[BATCH], slot[BATCH];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int n = base + i * threads;
-            const long long v = n < N ? target[n] : ignore_index;
-            w[i] = v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
-            mine += w[i] != LEFT_OUT;
-        }
+        for (int i = 0; i < BATCH; ++i) w[i] = read(base + i * threads);
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) slot[i] = lists && w[i] >= 0 ? atomicAdd(&t.count[w[i]], 1) : 0;
+        for (int i = 0; i < BATCH; ++i) {
+            const int owner = w[i] / LINE & (blocks - 1);
+            count += w[i] != LEFT_OUT;
+            before += w[i] >= 0 && owner < self;
+            slot[i] = -1;
+            if (lists && w[i] >= 0 && owner == self) slot[i] = atomicAdd(&t.count[w[i]], 1);
+        }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             const int n = base + i * threads;
             if (n >= N) break;
-            t.word[n] = w[i];
-            if (lists) t.slot[n] = slot[i];
+            if (self == 0) t.word[n] = w[i];
+            if (slot[i] >= 0) t.slot[n] = slot[i];
         }
     }
-    if (mine > 0) atomicAdd(&kept, mine);
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) t.counted[0] = kept;
+    if (count > 0) atomicAdd(&kept, count);
+    if (before > 0) atomicAdd(&places, before);
+    phase_end();
+    if (self == 0 && threadIdx.x == 0) t.counted[0] = kept;
     if (!lists) return;
-    for (int base = threadIdx.x; base < N; base += threads * BATCH) {
-        int w[BATCH], c[BATCH];
+    for (int pass = 0; pass < 2; ++pass) {  // places for the block's words, then its tokens there
+        for (int base = threadIdx.x; base < N; base += threads * BATCH) {
+            int w[BATCH], slot[BATCH], at[BATCH];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int n = base + i * threads;
-            w[i] = n < N && t.slot[n] == 0 ? t.word[n] : LEFT_OUT;
+            for (int i = 0; i < BATCH; ++i) w[i] = read(base + i * threads);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                w[i] = w[i] >= 0 && (w[i] / LINE & (blocks - 1)) == self ? w[i] : LEFT_OUT;
+                slot[i] = w[i] >= 0 ? t.slot[base + i * threads] : 0;
+                if (pass == 0 && slot[i] > 0) w[i] = LEFT_OUT;
+            }
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) at[i] = w[i] >= 0 ? load(pass == 0 ? &t.count[w[i]] : &t.place[w[i]]) : 0;
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                if (w[i] < 0) continue;
+                if (pass == 0) t.place[w[i]] = atomicAdd(&places, at[i]);
+                else t.arrived[at[i] + slot[i]] = base + i * threads;
+            }
         }
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) c[i] = w[i] >= 0 ? load(&t.count[w[i]]) : 0;
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-            if (w[i] >= 0) store(&t.place[w[i]], atomicAdd(&places, c[i]));
-    }
-    __threadfence();
-    __syncthreads();
-    for (int base = threadIdx.x; base < N; base += threads * BATCH) {
-        int w[BATCH], at[BATCH];
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int n = base + i * threads;
-            w[i] = n < N ? t.word[n] : LEFT_OUT;
-            at[i] = n < N ? t.slot[n] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-            if (w[i] >= 0) at[i] += load(&t.place[w[i]]);
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i)
-            if (w[i] >= 0) t.arrived[at[i]] = base + i * threads;
+        phase_end();
     }
 }
+// Listed tokens from which 16 blocks take them (96 tokens of 1003 words: 7.3 us by one block, 9.5 by 16).
+constexpr int MANY_WORDS = 1024;
 
 template <int CTRL>
 __device__ __forceinline__ float rotated(float v) {
@@ -140,24 +151,12 @@ __device__ __forceinline__ float wave_sum(float v) {
     return row_sum16(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
-// What words_block is to do in a launch, if anything (N = 0: nothing).
-struct WordsWork {
-    const long long* target;
-    long long ignore_index;
-    int N;
-    bool lists;
-};
-
 // The parts' largest logits and sums: a lane takes a chunk of 4 words, 16 lanes a part, EACH times. Rows of z are ldz
-// apart, a multiple of 32. The first row of blocks is not a token's: its first block is words_block.
+// apart, a multiple of 32.
 constexpr int EACH = 4;
 __global__ void __launch_bounds__(256)
-loss_parts(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ out, WordsWork work, Targets t) {
-    if (blockIdx.y == 0) {
-        if (blockIdx.x == 0 && work.N > 0) words_block(work.target, work.ignore_index, work.N, V, work.lists, t);
-        return;
-    }
-    const int row = blockIdx.y - 1, chunk = 4 * (threadIdx.x & 15);
+loss_parts(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ out) {
+    const int row = blockIdx.y, chunk = 4 * (threadIdx.x & 15);
     const float* q = z + (size_t)row * ldz + chunk;
     const int first = blockIdx.x * (16 * EACH) + (threadIdx.x >> 4);
     float4 f[EACH];
@@ -343,6 +342,31 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
                 top[c] = max(top[c], __float_as_uint(d[s][k][c]) & 0x7FFFFFFFu);
             }
         }
+    if (out.by_token != nullptr) {
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int t0 = s * STEP_TOKENS + wave * 64;
+            if (t0 >= rows) continue;
+            v4i w[S];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int r = s * STEP_TOKENS + base + k;
+                const int scale = 7 * (S - 1) - (r < rows ? exponents[r] : 0);
+                const int x[4] = {fixed_bits(d[s][k][0], scale), fixed_bits(d[s][k][1], scale),
+                                  fixed_bits(d[s][k][2], scale), fixed_bits(d[s][k][3], scale)};
+                pack_word<S>(x, w, k);
+            }
+            const int r = s * STEP_TOKENS + base + q;  // the token whose piece this lane stores
+            int8_t* to = out.by_token + (size_t)(r >> 5) * out.token_bytes + (size_t)(v0 >> 5) * (S * PANEL_BYTES) +
+                         (r & 31) * 16 + (v0 & 16) * 32;
+#pragma unroll
+            for (int p = 0; p < S; ++p) {
+                int a[4] = {w[p][0], w[p][1], w[p][2], w[p][3]};
+                transpose_quad(a, lane);
+                *reinterpret_cast<v4i*>(to + p * PANEL_BYTES) = v4i{a[0], a[1], a[2], a[3]};
+            }
+        }
+    }
     if (out.by_word != nullptr) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -380,31 +404,6 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
                 int a[4] = {w[p][0], w[p][1], w[p][2], w[p][3]};
                 transpose_rows(a);
                 *reinterpret_cast<v4i*>(to + ((size_t)(k0 >> 5) * S + p) * PANEL_BYTES + (k0 & 16) * 32) = v4i{a[0], a[1], a[2], a[3]};
-            }
-        }
-    }
-    if (out.by_token != nullptr) {
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            const int t0 = s * STEP_TOKENS + wave * 64;
-            if (t0 >= rows) continue;
-            v4i w[S];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int r = s * STEP_TOKENS + base + k;
-                const int scale = 7 * (S - 1) - (r < rows ? exponents[r] : 0);
-                const int x[4] = {fixed_bits(d[s][k][0], scale), fixed_bits(d[s][k][1], scale),
-                                  fixed_bits(d[s][k][2], scale), fixed_bits(d[s][k][3], scale)};
-                pack_word<S>(x, w, k);
-            }
-            const int r = s * STEP_TOKENS + base + q;  // the token whose piece this lane stores
-            int8_t* to = out.by_token + (size_t)(r >> 5) * out.token_bytes + (size_t)(v0 >> 5) * (S * PANEL_BYTES) +
-                         (r & 31) * 16 + (v0 & 16) * 32;
-#pragma unroll
-            for (int p = 0; p < S; ++p) {
-                int a[4] = {w[p][0], w[p][1], w[p][2], w[p][3]};
-                transpose_quad(a, lane);
-                *reinterpret_cast<v4i*>(to + p * PANEL_BYTES) = v4i{a[0], a[1], a[2], a[3]};
             }
         }
     }
@@ -518,10 +517,22 @@ loss_reduce(const Token* __restrict__ tokens, int N, int reduction, const int* _
 __global__ void __launch_bounds__(256) loss_fill(float* __restrict__ a, float v, size_t n) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) a[i] = v;
 }
-__global__ void __launch_bounds__(256) scale_kernel(float* __restrict__ a, const float* __restrict__ factor, size_t n) {
+__device__ __forceinline__ void scale_all(float* __restrict__ a, size_t n, float f) {
+    const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x, all = (size_t)gridDim.x * 256;
+    for (size_t i = id; i < n / 4; i += all) {
+        Four v = reinterpret_cast<Four*>(a)[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v.v[k] = v.v[k] * f;
+        reinterpret_cast<Four*>(a)[i] = v;
+    }
+    if (id < n % 4) a[n - 1 - id] = a[n - 1 - id] * f;
+}
+__global__ void __launch_bounds__(256)
+scale_kernel(float* __restrict__ a, size_t na, float* __restrict__ b, size_t nb, const float* __restrict__ factor) {
     const float f = factor[0];
     if (f == 1.0f) return;
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) a[i] = a[i] * f;
+    scale_all(a, na, f);
+    scale_all(b, nb, f);
 }
 
 unsigned grid_of(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 1u << 20); }
@@ -585,7 +596,7 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
         for (const Layout* L : {&s->z[k], dx ? &s->dx[k] : nullptr, dw ? &s->dw[k] : nullptr})
             if (L && L->has_partial) partial = std::max(partial, (size_t)L->split * L->M * L->N * sizeof(int64_t));
     }
-    s->words = take(((size_t)6 * N + 2 * (size_t)V + 1) * sizeof(int));
+    s->words = take(((size_t)6 * N + 2 * (size_t)round_up(V, 32) + 1) * sizeof(int));
     s->tokens = take((size_t)N * sizeof(Token));
     s->part = take((size_t)s->group * s->parts * sizeof(float2));
     s->logits = take((size_t)s->group * s->ldz * sizeof(float));
@@ -679,31 +690,33 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     const auto panels = [&](const Digits& d) { return reinterpret_cast<int8_t*>(base + d.q); };
     const auto exponents = [&](const Digits& d) { return reinterpret_cast<int*>(base + d.e); };
     Targets t;
-    t.lead = reinterpret_cast<int2*>(base + s.words);
+    t.count = reinterpret_cast<int*>(base + s.words);  // whole cache lines
+    t.place = t.count + round_up(V, 32);
+    t.lead = reinterpret_cast<int2*>(t.place + round_up(V, 32));
     t.word = reinterpret_cast<int*>(t.lead + N);
     t.slot = t.word + N;
     t.arrived = t.slot + N;
     t.list = t.arrived + N;
-    t.count = t.list + N;
-    t.place = t.count + V;
-    t.counted = t.place + V;
+    t.counted = t.list + N;
     Token* tokens = reinterpret_cast<Token*>(base + s.tokens);
     float2* part = reinterpret_cast<float2*>(base + s.part);
     float* z = reinterpret_cast<float*>(base + s.logits);
     int64_t* partial = reinterpret_cast<int64_t*>(base + s.partial);
     float* scratch = reinterpret_cast<float*>(base + s.scratch);
 
+    hipLaunchKernelGGL(loss_words, dim3(dw && N > MANY_WORDS ? 16 : 1), dim3(1024), 0, st, target, cfg->ignore_index, N, V,
+                       dw != nullptr, t);
     // The digits that every group's products share.
-    rc = launch_slice(x, N, D, false, S, panels(s.x_rows), exponents(s.x_rows), scratch, st);
-    if (rc == hipSuccess) rc = launch_slice(w, V, D, false, S, panels(s.w_rows), exponents(s.w_rows), scratch, st);
+    rc = launch_slice_rows(x, N, panels(s.x_rows), exponents(s.x_rows), w, V, panels(s.w_rows), exponents(s.w_rows), D, S,
+                           scratch, st);
     if (rc == hipSuccess && dx) rc = launch_slice(w, D, V, true, S, panels(s.w_cols), exponents(s.w_cols), scratch, st);
     if (rc != hipSuccess) return rc;
     for (int first = 0; first < N; first += s.group) {
         const int rows = std::min(s.group, N - first), k = first + s.group < N ? 0 : 1;
         launch_product(s.z[k], panels(s.x_rows) + (size_t)first * round_up(D, STEP_K) * S, exponents(s.x_rows) + first,
                        panels(s.w_rows), exponents(s.w_rows), z, s.ldz, false, partial, st);
-        const WordsWork work{target, cfg->ignore_index, first == 0 ? N : 0, dw != nullptr};
-        hipLaunchKernelGGL(loss_parts, dim3((s.parts + 16 * EACH - 1) / (16 * EACH), rows + 1), dim3(256), 0, st, z, s.ldz, V, s.parts, part, work, t);
+        hipLaunchKernelGGL(loss_parts, dim3((s.parts + 16 * EACH - 1) / (16 * EACH), rows), dim3(256), 0, st, z, s.ldz, V,
+                           s.parts, part);
         hipLaunchKernelGGL(loss_tokens, dim3((rows + 3) / 4), dim3(256), 0, st, z, s.ldz, V, s.parts, part, first, rows,
                            t, dw != nullptr, factors, cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, exponents(s.by_token));
         if (!dx && !dw) continue;
@@ -736,11 +749,11 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     return hipGetLastError();
 }
 
-int rg_scale_fp32(float* x, const float* factor, size_t n, void* stream) {
-    if (n == 0) return hipSuccess;
-    if (!x || !factor) return hipErrorInvalidValue;
-    const unsigned grid = (unsigned)std::min<size_t>((n + 1023) / 1024, 8192);
-    hipLaunchKernelGGL(rg::scale_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), x, factor, n);
+int rg_scale_fp32(float* x, size_t nx, float* y, size_t ny, const float* factor, void* stream) {
+    if (nx + ny == 0) return hipSuccess;
+    if ((nx > 0 && !x) || (ny > 0 && !y) || !factor) return hipErrorInvalidValue;
+    const unsigned grid = (unsigned)std::min<size_t>((nx + ny + 1023) / 1024, 4096);
+    hipLaunchKernelGGL(rg::scale_kernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), x, nx, y, ny, factor);
     return hipGetLastError();
 }
 

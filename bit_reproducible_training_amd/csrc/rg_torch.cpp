@@ -824,7 +824,22 @@ std::vector<OptTensor> linear_cross_entropy(Tensor x, Tensor weight, Tensor targ
     return {opt(loss), opt(dx), opt(dw)};
 }
 
-void scale_(Tensor t, Tensor factor);
+// Both (either may be undefined, both contiguous) times factor[0]; no write on a GPU where that is 1.
+void scale(const Tensor& a, const Tensor& b, const Tensor& factor) {
+    const Tensor& t = a.defined() ? a : b;
+    if (!t.defined()) return;
+    if (t.is_cuda()) {
+        c10::DeviceGuard guard(t.device());
+        check(rg_scale_fp32(a.defined() ? a.data_ptr<float>() : nullptr, a.defined() ? a.numel() : 0,
+                            b.defined() ? b.data_ptr<float>() : nullptr, b.defined() ? b.numel() : 0,
+                            factor.data_ptr<float>(), stream_of(t)),
+              "scale");
+        return;
+    }
+    at::NoGradGuard no_grad;
+    for (const Tensor* g : {&a, &b})
+        if (g->defined()) g->mul_(factor);
+}
 
 // The loss, differentiable. With the sum or the mean, the forward pass leaves the gradients in the context
 // for the first backward pass to scale and hand out; a later one, and one without a reduction, computes them.
@@ -866,11 +881,9 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
             dx = out[1];
             dw = out[2];
         }
-        if (reduction != RG_LOSS_NONE)
-            for (const OptTensor* g : {&dx, &dw})
-                if (g->has_value()) scale_(**g, grads[0]);
         result[0] = or_undefined(dx);
         result[1] = or_undefined(dw);
+        if (reduction != RG_LOSS_NONE) scale(result[0], result[1], grads[0].resolve_neg().contiguous());
         differentiable_once(result, "linear_cross_entropy");
         return result;
     }
@@ -881,19 +894,6 @@ Tensor loss_apply(const Tensor& x, const Tensor& weight, const Tensor& target, i
     const bool grad = at::GradMode::is_enabled();
     return LossFunction::apply(x, weight, target, S, reduction, ignore_index, grad && x.requires_grad(),
                                grad && weight.requires_grad());
-}
-
-// t *= factor[0] for a contiguous t; no write where the factor is 1.
-void scale_(Tensor t, Tensor factor) {
-    require_f32(t, "t");
-    require_f32(factor, "factor");
-    need(t.is_contiguous() && factor.numel() == 1, "scale_: a contiguous tensor and one factor");
-    if (on_gpu(t, factor, "scale_")) {
-        c10::DeviceGuard guard(t.device());
-        check(rg_scale_fp32(t.data_ptr<float>(), factor.data_ptr<float>(), (size_t)t.numel(), stream_of(t)), "scale");
-        return;
-    }
-    t.mul_(factor);
 }
 
 }  // namespace

@@ -64,9 +64,9 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
                             const float* factors, float* loss, float* dx, float* dw, void* workspace,
                             size_t workspace_bytes, void* stream);
 
-/* x[i] <- x[i] * factor[0] for n floats, factor in device memory; nothing is written where it is 1 (the
- * gradient of a loss that is not scaled further). 1 (invalid value): null pointers with n > 0. */
-int rg_scale_fp32(float* x, const float* factor, size_t n, void* stream);
+/* The nx floats of x and the ny of y times factor[0], in device memory; nothing is written where it is 1 (the
+ * gradients of a loss that is not scaled further). 1 (invalid value): null pointers to what is to be scaled. */
+int rg_scale_fp32(float* x, size_t nx, float* y, size_t ny, const float* factor, void* stream);
 
 #ifdef __cplusplus
 }

@@ -264,7 +264,8 @@ def test_c_entry_refuses_bad_arguments():
         args = [p, p, p, p, p, p, p]
         args[i] = p + 2
         assert lib.rg_linear_cross_entropy(ctypes.byref(config()), *args, p, 1 << 40, None) == bad
-    assert lib.rg_scale_fp32(None, None, 4, None) == bad and lib.rg_scale_fp32(None, None, 0, None) == 0
+    assert lib.rg_scale_fp32(None, 4, None, 0, p, None) == bad and lib.rg_scale_fp32(p, 4, p, 4, None, None) == bad
+    assert lib.rg_scale_fp32(None, 0, None, 0, None, None) == 0
 
 
 def test_module_reports_to_the_guard():

@@ -151,6 +151,105 @@ __device__ __forceinline__ float wave_sum(float v) {
     return row_sum16(__uint_as_float(s[0]) + __uint_as_float(s[1]));
 }
 
+// ---- the logits of few tokens ----
+//
+// Few tokens' logits are bound by reading the weight once; slicing it first writes 3 bytes for each 4 it reads
+// and reads them again. Here a block holds 32 words in registers: its wavefronts take k panels (32 words x 32
+// values) in turn, 16 values of a word a lane, find the words' scales together, round, and contract
+// the digits from registers with the tokens' digits, a tile of 32 at most. The wavefronts' exact integer sums
+// meet in LDS. A block is mostly latency, so more tokens or values lose again: losses of 1 and 32 tokens of
+// GPT-2 small's head 63 and 71 us against 88 and 96 by slicing and contracting; of 64 (two tiles) 98 against 102, of 128
+// 139 against 118; with 1600 values a word (eight wavefronts) 181 against 178.
+constexpr int FEW_TOKENS = 32, FEW_WAVES = 4, FEW_MAX_D = 1024;
+
+template <int S, int PW>
+__global__ void __launch_bounds__(64 * FEW_WAVES, 2)
+loss_few(const float* __restrict__ w, int V, int D, int panels, const int8_t* __restrict__ qx, const int* __restrict__ ex,
+         int N, float* __restrict__ z, int ldz) {
+    constexpr int L = 2 * S - 1;
+    __shared__ int64_t sums[FEW_WAVES][16][64];
+    __shared__ uint32_t tops[FEW_WAVES][32];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int word = blockIdx.x * 32 + (lane & 31);
+    const float* row = w + (size_t)min(word, V - 1) * D;
+    float f[PW][16];
+#pragma unroll
+    for (int p = 0; p < PW; ++p) {
+        const int k0 = (wave + FEW_WAVES * p) * PANEL_K + 16 * (lane >> 5);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+            if (k0 + j + 4 <= D) {
+                const Four q = *reinterpret_cast<const Four*>(row + k0 + j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[p][j + i] = q.v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[p][j + i] = k0 + j + i < D ? row[k0 + j + i] : 0.0f;
+            }
+        }
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int p = 0; p < PW; ++p)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = max(top, repro_gemm::magnitude_key(f[p][j]));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    if (lane < 32) tops[wave][lane] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FEW_WAVES; ++i) top = max(top, tops[i][lane & 31]);
+    const int ew = repro_gemm::scale_exponent(__uint_as_float(top));
+    const RowScale scale = row_scale<S>(ew);
+    v16i acc[L];
+#pragma unroll
+    for (int l = 0; l < L; ++l)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[l][e] = 0;
+#pragma unroll
+    for (int p = 0; p < PW; ++p) {
+        // Past the last panel the weight's digits are zero: any of the tokens' will do.
+        const int8_t* qa = qx + (size_t)min(wave + FEW_WAVES * p, panels - 1) * (S * PANEL_BYTES) + lane * 16;
+        v4i a[S], b[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) a[i] = *reinterpret_cast<const v4i*>(qa + i * PANEL_BYTES);
+        int x[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = round_fixed(f[p][j], scale);
+        pack16<S>(x, b);
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                acc[i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i + j], 0, 0, 0);
+    }
+    // Register e of the tile holds token 8 (e / 4) + 4 (lane / 32) + e % 4 and its lane's word.
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        if (8 * (e >> 2) >= N) break;  // uniform: nobody's
+        int lv[L];
+#pragma unroll
+        for (int l = 0; l < L; ++l) lv[l] = acc[l][e];
+        sums[wave][e][lane] = combine_levels<L>(lv);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16 / FEW_WAVES; ++i) {
+        if (8 * i >= N) break;
+        const int e = wave + FEW_WAVES * i, n = 8 * i + 4 * (lane >> 5) + wave;
+        int64_t t = 0;
+#pragma unroll
+        for (int k = 0; k < FEW_WAVES; ++k) t += sums[k][e][lane];
+        if (n < N && word < V) z[(size_t)n * ldz + word] = round_output(t, ex[n] + ew - 14 * (S - 1));
+    }
+}
+
+template <int S>
+void launch_few_s(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, hipStream_t st) {
+    const int panels = (D + STEP_K - 1) / STEP_K * (STEP_K / PANEL_K);  // as the slicing pads
+    auto kernel = panels <= 8 ? loss_few<S, 2> : panels <= 16 ? loss_few<S, 4> : panels <= 24 ? loss_few<S, 6> : loss_few<S, 8>;
+    hipLaunchKernelGGL(kernel, dim3((V + 31) / 32), dim3(64 * FEW_WAVES), 0, st, w, V, D, panels, qx, ex, N, z, ldz);
+}
+
 // The parts' largest logits and sums: a lane takes a chunk of 4 words, 16 lanes a part, EACH times. Rows of z are ldz
 // apart, a multiple of 32.
 constexpr int EACH = 4;
@@ -562,6 +661,7 @@ struct Digits {
 // Where everything lies in the workspace, and the products of a whole group [0] and of the last [1].
 struct Space {
     int group, last, parts, ldz;
+    bool few;  // the logits by loss_few
     Layout z[2], dx[2], dw[2];
     Digits x_rows, w_rows, w_cols, x_cols, by_token, by_word;
     size_t words, tokens, part, logits, partial, scratch, total;
@@ -573,6 +673,7 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
     s->last = (N - 1) % s->group + 1;
     s->parts = (V + PART - 1) / PART;
     s->ldz = round_up(V, 32);
+    s->few = N <= FEW_TOKENS && D <= FEW_MAX_D;
     // Rows past a matrix's own that a tile may read: their products are not stored.
     constexpr int BEYOND = 192;
     size_t at = 0, partial = 0, scratch = 0;
@@ -589,11 +690,11 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
     };
     for (int k = 0; k < 2; ++k) {
         const int rows = k ? s->last : s->group;
-        int rc = plan_product(rows, V, D, S, &s->z[k]);
+        int rc = s->few ? hipSuccess : plan_product(rows, V, D, S, &s->z[k]);
         if (rc == hipSuccess && dx) rc = plan_product(rows, D, V, S, &s->dx[k]);
         if (rc == hipSuccess && dw) rc = plan_product(V, D, rows, S, &s->dw[k]);
         if (rc != hipSuccess) return rc;
-        for (const Layout* L : {&s->z[k], dx ? &s->dx[k] : nullptr, dw ? &s->dw[k] : nullptr})
+        for (const Layout* L : {s->few ? nullptr : &s->z[k], dx ? &s->dx[k] : nullptr, dw ? &s->dw[k] : nullptr})
             if (L && L->has_partial) partial = std::max(partial, (size_t)L->split * L->M * L->N * sizeof(int64_t));
     }
     s->words = take(((size_t)6 * N + 2 * (size_t)round_up(V, 32) + 1) * sizeof(int));
@@ -601,7 +702,7 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
     s->part = take((size_t)s->group * s->parts * sizeof(float2));
     s->logits = take((size_t)s->group * s->ldz * sizeof(float));
     s->x_rows = digits(N, D);
-    s->w_rows = digits(V, D);
+    s->w_rows = digits(s->few ? 0 : V, D);
     scratch = std::max(slice_scratch_bytes(N, D, false), slice_scratch_bytes(V, D, false));
     if (dx) {
         s->w_cols = digits(D, V);
@@ -707,14 +808,22 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     hipLaunchKernelGGL(loss_words, dim3(dw && N > MANY_WORDS ? 16 : 1), dim3(1024), 0, st, target, cfg->ignore_index, N, V,
                        dw != nullptr, t);
     // The digits that every group's products share.
-    rc = launch_slice_rows(x, N, panels(s.x_rows), exponents(s.x_rows), w, V, panels(s.w_rows), exponents(s.w_rows), D, S,
-                           scratch, st);
+    if (s.few)
+        rc = launch_slice(x, N, D, false, S, panels(s.x_rows), exponents(s.x_rows), scratch, st);
+    else
+        rc = launch_slice_rows(x, N, panels(s.x_rows), exponents(s.x_rows), w, V, panels(s.w_rows), exponents(s.w_rows), D, S,
+                               scratch, st);
     if (rc == hipSuccess && dx) rc = launch_slice(w, D, V, true, S, panels(s.w_cols), exponents(s.w_cols), scratch, st);
     if (rc != hipSuccess) return rc;
     for (int first = 0; first < N; first += s.group) {
         const int rows = std::min(s.group, N - first), k = first + s.group < N ? 0 : 1;
-        launch_product(s.z[k], panels(s.x_rows) + (size_t)first * round_up(D, STEP_K) * S, exponents(s.x_rows) + first,
-                       panels(s.w_rows), exponents(s.w_rows), z, s.ldz, false, partial, st);
+        if (s.few) {
+            auto launch_few = S == 1 ? launch_few_s<1> : S == 2 ? launch_few_s<2> : launch_few_s<3>;
+            launch_few(w, V, D, panels(s.x_rows), exponents(s.x_rows), N, z, s.ldz, st);
+        } else {
+            launch_product(s.z[k], panels(s.x_rows) + (size_t)first * round_up(D, STEP_K) * S, exponents(s.x_rows) + first,
+                           panels(s.w_rows), exponents(s.w_rows), z, s.ldz, false, partial, st);
+        }
         hipLaunchKernelGGL(loss_parts, dim3((s.parts + 16 * EACH - 1) / (16 * EACH), rows), dim3(256), 0, st, z, s.ldz, V,
                            s.parts, part);
         hipLaunchKernelGGL(loss_tokens, dim3((rows + 3) / 4), dim3(256), 0, st, z, s.ldz, V, s.parts, part, first, rows,

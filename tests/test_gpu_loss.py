@@ -22,7 +22,10 @@ def assert_same(got, want):
 # One word, one part and its ends, one token, sizes off every multiple, long rows, few and many tokens a word.
 CASES = [(1, 1, 1, None), (1, 7, 3, None), (3, 4, 63, None), (5, 16, 64, 2), (17, 33, 65, 1), (64, 64, 1024, None),
          (130, 40, 1003, 5), (2, 768, 50257, None), (96, 128, 4099, None), (33, 100, 16385, 3), (700, 20, 130, 1),
-         (1030, 65, 200, 3), (300, 1028, 77, 9)]
+         (1030, 65, 200, 3), (300, 1028, 77, 9),
+         # few tokens: one, 8, 32 and past them, widths of each register class and past them
+         (1, 33, 31, None), (8, 257, 33, 4), (9, 512, 100, 4), (32, 770, 97, 10), (33, 64, 97, 10), (31, 1024, 40, 2),
+         (24, 1025, 70, 5), (64, 1024, 95, 9)]
 
 
 @pytest.mark.parametrize("n,d,v,words", CASES)

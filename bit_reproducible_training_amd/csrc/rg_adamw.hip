@@ -106,13 +106,91 @@ adamw_kernel(const List<Entry> list) {
     }
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t rotated(uint32_t a) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)a, CTRL, 0xF, 0xF, true);
+}
+// The largest over the wavefront, as a scalar: half waves, rows of 16, and rotations inside a row.
 __device__ __forceinline__ uint32_t wave_max_bits(uint32_t a) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) a = max(a, (uint32_t)__shfl_xor((int)a, off, 64));
-    return a;
+    auto s = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    a = max((uint32_t)s[0], (uint32_t)s[1]);
+    s = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    a = max((uint32_t)s[0], (uint32_t)s[1]);
+    a = max(a, rotated<0x128>(a));
+    a = max(a, rotated<0x124>(a));
+    a = max(a, rotated<0x122>(a));
+    a = max(a, rotated<0x121>(a));
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
 }
 
-// A wavefront takes U blocks of BLOCK values, its lane l the values 4 l .. 4 l + 3 of each.
+// One block of BLOCK values by a wavefront, its lane l the values 4 l .. 4 l + 3. FULL: the tensor holds the
+// whole block and 16-byte accesses are allowed.
+template <bool FULL>
+struct Block8 {
+    float p[4], g[4];
+    uint32_t m, v;  // codes
+    int me, ve;
+
+    __device__ __forceinline__ void load(const Entry8& t, uint32_t b, int lane) {
+        const uint32_t at = b * BLOCK + 4 * lane;
+        m = reinterpret_cast<const uint32_t*>(t.m + (size_t)b * BLOCK)[lane];
+        v = reinterpret_cast<const uint32_t*>(t.v + (size_t)b * BLOCK)[lane];
+        me = t.m_exp[b];
+        ve = t.v_exp[b];
+        if constexpr (FULL) {
+            const float4 pp = *reinterpret_cast<const float4*>(t.p + at), gg = *reinterpret_cast<const float4*>(t.g + at);
+            p[0] = pp.x, p[1] = pp.y, p[2] = pp.z, p[3] = pp.w;
+            g[0] = gg.x, g[1] = gg.y, g[2] = gg.z, g[3] = gg.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p[i] = at + i < t.n ? t.p[at + i] : 0.0f;
+                g[i] = at + i < t.n ? t.g[at + i] : 0.0f;
+            }
+        }
+    }
+    __device__ __forceinline__ void step(const Entry8& t, uint32_t b, int lane, const Scalars& s) {
+        const uint32_t at = b * BLOCK + 4 * lane;
+        const int em0 = __builtin_amdgcn_readfirstlane(me), ev0 = __builtin_amdgcn_readfirstlane(ve);
+        float mv[4], vv[4];
+        uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            mv[i] = repro_adamw::decode_m((uint8_t)(m >> (8 * i)), em0);
+            vv[i] = repro_adamw::decode_v((uint8_t)(v >> (8 * i)), ev0);
+            p[i] = repro_adamw::update(p[i], g[i], mv[i], vv[i], s);
+            if (!FULL && at + i >= t.n) mv[i] = vv[i] = 0.0f;  // past the tensor: codes of zero
+            top_m = max(top_m, repro_adamw::magnitude_bits(mv[i]));
+            top_v = max(top_v, repro_adamw::magnitude_bits(vv[i]));
+        }
+        const int em = repro_adamw::shared_exponent(wave_max_bits(top_m), repro_adamw::SPAN_M);
+        const int ev = repro_adamw::shared_exponent(wave_max_bits(top_v), repro_adamw::SPAN_V);
+        uint32_t cm = 0, cv = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t u = repro_adamw::rounding((t.block + b) * BLOCK + 4 * lane + i, s.salt);
+            cm |= (uint32_t)repro_adamw::encode_m(mv[i], em, u & 0xFFFFu) << (8 * i);
+            cv |= (uint32_t)repro_adamw::encode_v(vv[i], ev, u >> 16) << (8 * i);
+        }
+        reinterpret_cast<uint32_t*>(t.m + (size_t)b * BLOCK)[lane] = cm;
+        reinterpret_cast<uint32_t*>(t.v + (size_t)b * BLOCK)[lane] = cv;
+        if (lane == 0) {
+            t.m_exp[b] = (uint8_t)em;
+            t.v_exp[b] = (uint8_t)ev;
+        }
+        if constexpr (FULL) {
+            *reinterpret_cast<float4*>(t.p + at) = make_float4(p[0], p[1], p[2], p[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (at + i < t.n) t.p[at + i] = p[i];
+        }
+    }
+};
+
+// A wavefront takes U blocks in turn, all of them loaded before the first is stepped. (Eight a wavefront in a loop,
+// fewer searches of the list: no faster. The arithmetic bounds it: about 100 vector instructions a
+// value, 484 us for 124 million of them.)
 template <int U>
 __global__ void __launch_bounds__(THREADS)
 adamw8_kernel(const List<Entry8> list) {
@@ -121,77 +199,21 @@ adamw8_kernel(const List<Entry8> list) {
     const Scalars s = list.s;
     const int lane = threadIdx.x & 63;
     const uint32_t blocks = (t.n + BLOCK - 1) / BLOCK;
-    const uint32_t b0 = (blockIdx.x - list.first[entry]) * (uint32_t)(THREADS / 64 * U) + (threadIdx.x >> 6);
+    const uint32_t b0 = (blockIdx.x - list.first[entry]) * (uint32_t)(THREADS / 64 * U) +
+                        (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool wide = ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g)) & 15) == 0;
-    float pv[U][4], gv[U][4];
-    uint32_t mc[U], vc[U];
-    int me[U], ve[U];
+    if (wide && b0 + (U - 1) * (THREADS / 64) < t.n / BLOCK) {
+        Block8<true> k[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t b = b0 + u * (THREADS / 64);
-        mc[u] = vc[u] = 0;
-        me[u] = ve[u] = 0;
+        for (int u = 0; u < U; ++u) k[u].load(t, b0 + u * (THREADS / 64), lane);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pv[u][i] = gv[u][i] = 0.0f;
-        if (b >= blocks) continue;
-        const uint32_t at = b * BLOCK + 4 * lane;
-        mc[u] = reinterpret_cast<const uint32_t*>(t.m + (size_t)b * BLOCK)[lane];
-        vc[u] = reinterpret_cast<const uint32_t*>(t.v + (size_t)b * BLOCK)[lane];
-        me[u] = t.m_exp[b];
-        ve[u] = t.v_exp[b];
-        if (wide && at + 4 <= t.n) {
-            const float4 pp = *reinterpret_cast<const float4*>(t.p + at);
-            const float4 gg = *reinterpret_cast<const float4*>(t.g + at);
-            pv[u][0] = pp.x, pv[u][1] = pp.y, pv[u][2] = pp.z, pv[u][3] = pp.w;
-            gv[u][0] = gg.x, gv[u][1] = gg.y, gv[u][2] = gg.z, gv[u][3] = gg.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (at + i < t.n) {
-                    pv[u][i] = t.p[at + i];
-                    gv[u][i] = t.g[at + i];
-                }
-            }
-        }
+        for (int u = 0; u < U; ++u) k[u].step(t, b0 + u * (THREADS / 64), lane, s);
+        return;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t b = b0 + u * (THREADS / 64);
-        if (b >= blocks) continue;  // uniform in a wavefront
-        const uint32_t at = b * BLOCK + 4 * lane;
-        float m[4], v[4];
-        uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            m[i] = repro_adamw::decode_m((uint8_t)(mc[u] >> (8 * i)), me[u]);
-            v[i] = repro_adamw::decode_v((uint8_t)(vc[u] >> (8 * i)), ve[u]);
-            pv[u][i] = repro_adamw::update(pv[u][i], gv[u][i], m[i], v[i], s);
-            if (at + i >= t.n) m[i] = v[i] = 0.0f;  // past the tensor: codes of zero
-            top_m = max(top_m, repro_adamw::magnitude_bits(m[i]));
-            top_v = max(top_v, repro_adamw::magnitude_bits(v[i]));
-        }
-        const int em = repro_adamw::shared_exponent(wave_max_bits(top_m), repro_adamw::SPAN_M);
-        const int ev = repro_adamw::shared_exponent(wave_max_bits(top_v), repro_adamw::SPAN_V);
-        uint32_t cm = 0, cv = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t u = repro_adamw::rounding((t.block + b) * BLOCK + 4 * lane + i, s.salt);
-            cm |= (uint32_t)repro_adamw::encode_m(m[i], em, u & 0xFFFFu) << (8 * i);
-            cv |= (uint32_t)repro_adamw::encode_v(v[i], ev, u >> 16) << (8 * i);
-        }
-        reinterpret_cast<uint32_t*>(t.m + (size_t)b * BLOCK)[lane] = cm;
-        reinterpret_cast<uint32_t*>(t.v + (size_t)b * BLOCK)[lane] = cv;
-        if (lane == 0) {
-            t.m_exp[b] = (uint8_t)em;
-            t.v_exp[b] = (uint8_t)ev;
-        }
-        if (wide && at + 4 <= t.n) {
-            *reinterpret_cast<float4*>(t.p + at) = make_float4(pv[u][0], pv[u][1], pv[u][2], pv[u][3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (at + i < t.n) t.p[at + i] = pv[u][i];
-        }
+    for (uint32_t b = b0; b < blocks && b < b0 + U * (THREADS / 64); b += THREADS / 64) {
+        Block8<false> k;
+        k.load(t, b, lane);
+        k.step(t, b, lane, s);
     }
 }
 

@@ -605,7 +605,7 @@ int rg_residual_norm_grad_fp32(const rg_norm_config* cfg, const float* dr, const
         return hipErrorInvalidValue;
     const Partition pt = repro_norm::partition(cfg->N, cfg->D, cfg->gate_rows);
     const long long P = pt.sections * pt.partials;
-    if (P > 0x7FFFFF) return hipErrorInvalidValue;
+    if (P >= 1ll << 22) return hipErrorInvalidValue;  // a launch has fewer than 2^32 threads
     float* out[SUMS] = {dweight, dbias, dpost_weight, dpost_bias, pt.gate_inside ? nullptr : dgate};
     bool any = false;
     for (float* o : out) any = any || o;

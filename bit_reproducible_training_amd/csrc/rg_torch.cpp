@@ -442,6 +442,12 @@ bool adamw_parameters(const Listed& params, const Listed& grads) {
     return params.size() > 0 && params[0].is_cuda();
 }
 
+// What autograd has saved of a tensor is not its value any more.
+void changed(const Listed& list) {
+    for (const Tensor* t : list.t)
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void adamw_step(py::handle params_, py::handle grads_, py::handle m_, py::handle v_, double lr, double beta1,
                 double beta2, double eps, double weight_decay, int64_t step) {
     const rg_adamw_config cfg = adamw_config(lr, beta1, beta2, eps, weight_decay, step);
@@ -456,6 +462,7 @@ void adamw_step(py::handle params_, py::handle grads_, py::handle m_, py::handle
                    v[i].data_ptr<float>(), (long long)params[i].numel()};
     }
     if (list.empty()) return;
+    for (const Listed* changing : {&params, &m, &v}) changed(*changing);
     if (gpu) {
         c10::DeviceGuard guard(params[0].device());
         check(rg_adamw_fp32(list.data(), (int)list.size(), &cfg, stream_of(params[0])), "adamw");
@@ -515,6 +522,7 @@ void adamw8_step(py::handle params_, py::handle grads_, py::handle m_, py::handl
                    (long long)params[i].numel()};
         if (flat) at += blocks;
     }
+    for (const Listed* changing : {&params, &m, &m_exp, &v, &v_exp}) changed(*changing);
     if (gpu) {
         c10::DeviceGuard guard(params[0].device());
         check(rg_adamw8_fp32(list.data(), (int)list.size(), &cfg, stream_of(params[0])), "adamw8");

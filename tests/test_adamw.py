@@ -301,3 +301,14 @@ def test_optimizer_refuses_bad_settings():
     for bad in (dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0), dict(betas=(0.9, 1.0)), dict(state_bits=16)):
         with pytest.raises(ValueError):
             rg.AdamW(p, **bad)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_step_is_a_change_that_autograd_sees(bits):
+    p = torch.nn.Parameter(torch.randn(5))
+    opt = rg.AdamW([p], state_bits=bits)
+    loss = (p * p).sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()

@@ -42,15 +42,14 @@ struct Targets {
 };
 
 // The words' counts by atomics, then places for their tokens. A word's place and its tokens' order in
-// `arrived` change from run to run and reach no result: loss_tokens puts them in order. lists: whether
-// the tokens are listed.
+// `arrived` change from run to run and reach no result: loss_rows puts them in order.
 // Each block owns the words of every gridDim.x-th cache line of `count` (gridDim.x a power of two) and reads all targets, so blocks
 // need nothing of each other: the places before its own are those of the tokens of the blocks before it. The
 // scattered accesses are what takes time, at one compute unit's rate (8192 tokens of 50257 words: 66 us by
-// one block, 26 by 16; every token compared with every other one took 170, and 64 times that for 65536).
+// one block, 24 by 16).
 // A thread has BATCH tokens in flight.
 __global__ void __launch_bounds__(1024)
-loss_words(const long long* __restrict__ target, long long ignore_index, int N, int V, bool lists, Targets t) {
+loss_words(const long long* __restrict__ target, long long ignore_index, int N, int V, Targets t) {
     constexpr int BATCH = 8, threads = 1024, LINE = 32;
     __shared__ int places, kept;
     const int blocks = gridDim.x, self = blockIdx.x;
@@ -67,12 +66,10 @@ loss_words(const long long* __restrict__ target, long long ignore_index, int N, 
         return v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
     };
     if (threadIdx.x == 0) places = kept = 0;
-    if (lists) {
-        const int lines = (V + LINE - 1) / LINE;
-        for (int i = threadIdx.x; i < (lines - self + blocks - 1) / blocks * LINE; i += threads) {
-            const int v = (i / LINE * blocks + self) * LINE + i % LINE;
-            if (v < V) t.count[v] = 0;
-        }
+    const int lines = (V + LINE - 1) / LINE;
+    for (int i = threadIdx.x; i < (lines - self + blocks - 1) / blocks * LINE; i += threads) {
+        const int v = (i / LINE * blocks + self) * LINE + i % LINE;
+        if (v < V) t.count[v] = 0;
     }
     phase_end();
     int count = 0, before = 0;
@@ -86,7 +83,7 @@ loss_words(const long long* __restrict__ target, long long ignore_index, int N, 
             count += w[i] != LEFT_OUT;
             before += w[i] >= 0 && owner < self;
             slot[i] = -1;
-            if (lists && w[i] >= 0 && owner == self) slot[i] = atomicAdd(&t.count[w[i]], 1);
+            if (w[i] >= 0 && owner == self) slot[i] = atomicAdd(&t.count[w[i]], 1);
         }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
@@ -100,7 +97,6 @@ loss_words(const long long* __restrict__ target, long long ignore_index, int N, 
     if (before > 0) atomicAdd(&places, before);
     phase_end();
     if (self == 0 && threadIdx.x == 0) t.counted[0] = kept;
-    if (!lists) return;
     for (int pass = 0; pass < 2; ++pass) {  // places for the block's words, then its tokens there
         for (int base = threadIdx.x; base < N; base += threads * BATCH) {
             int w[BATCH], slot[BATCH], at[BATCH];
@@ -124,8 +120,67 @@ loss_words(const long long* __restrict__ target, long long ignore_index, int N, 
         phase_end();
     }
 }
-// Listed tokens from which 16 blocks take them (96 tokens of 1003 words: 7.3 us by one block, 9.5 by 16).
-constexpr int MANY_WORDS = 1024;
+
+// The same for fewer tokens without counts in memory: a token's place is the number of tokens of smaller words, and
+// its place among its word's that of earlier ones, so `list` and `lead` are written at once. A block
+// takes RANKED tokens, 16 lanes each, which compare them with every token, SHELF at a time from LDS.
+constexpr int RANKED = 16, SHELF = 2048;
+__global__ void __launch_bounds__(16 * RANKED)
+loss_ranks(const long long* __restrict__ target, long long ignore_index, int N, int V, bool lists, Targets t) {
+    constexpr int threads = 16 * RANKED;
+    __shared__ __align__(16) int shelf[SHELF];
+    __shared__ int kept;
+    const int l = threadIdx.x & 15, n = blockIdx.x * RANKED + (threadIdx.x >> 4);
+    const auto read = [&](int i) {
+        const long long v = i < N ? target[i] : ignore_index;
+        return v == ignore_index ? LEFT_OUT : v >= 0 && v < V ? (int)v : INVALID;
+    };
+    const int word = read(n);
+    if (threadIdx.x == 0) kept = 0;
+    int smaller = 0, same = 0, before = 0, count = 0;
+    const bool counts = blockIdx.x == 0;
+    for (int first = 0; first < N && (lists || counts); first += SHELF) {
+        const int here = min(SHELF, (N - first + 63) / 64 * 64);
+        __syncthreads();
+        for (int i = threadIdx.x; i < here; i += threads) {
+            const int w = read(first + i);
+            shelf[i] = w;
+            count += w != LEFT_OUT;
+        }
+        __syncthreads();
+        if (!lists) continue;
+        for (int i = 4 * l; i < here; i += 64) {
+            const int4 four = *reinterpret_cast<const int4*>(&shelf[i]);
+            const int w[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                smaller += (uint32_t)w[k] < (uint32_t)word;  // not LEFT_OUT and INVALID: the largest numbers
+                same += w[k] == word;
+                before += w[k] == word && first + i + k < n;
+            }
+        }
+    }
+    if (counts) {
+        if (count > 0) atomicAdd(&kept, count);
+        __syncthreads();
+        if (threadIdx.x == 0) t.counted[0] = kept;
+    }
+    if (n >= N) return;
+    if (l == 0) t.word[n] = word;
+    if (!lists) return;
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) {
+        smaller += __shfl_xor(smaller, off, 16);
+        same += __shfl_xor(same, off, 16);
+        before += __shfl_xor(before, off, 16);
+    }
+    if (l != 0) return;
+    t.lead[n] = make_int2(word >= 0 && before == 0 ? same : 0, smaller);
+    if (word >= 0) t.list[smaller + before] = n;
+}
+// Tokens up to which loss_ranks lists them. us of loss_ranks and of loss_words for 96 tokens RANK96, 1024 RANK1024, 4096
+// RANK4096, 8192 RANK8192.
+constexpr int FEW_WORDS = 4096;
 
 template <int CTRL>
 __device__ __forceinline__ float rotated(float v) {
@@ -250,92 +305,107 @@ void launch_few_s(const float* w, int V, int D, const int8_t* qx, const int* ex,
     hipLaunchKernelGGL(kernel, dim3((V + 31) / 32), dim3(64 * FEW_WAVES), 0, st, w, V, D, panels, qx, ex, N, z, ldz);
 }
 
-// The parts' largest logits and sums: a lane takes a chunk of 4 words, 16 lanes a part, EACH times. Rows of z are ldz
-// apart, a multiple of 32.
-constexpr int EACH = 4;
-__global__ void __launch_bounds__(256)
-loss_parts(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ out) {
-    const int row = blockIdx.y, chunk = 4 * (threadIdx.x & 15);
-    const float* q = z + (size_t)row * ldz + chunk;
-    const int first = blockIdx.x * (16 * EACH) + (threadIdx.x >> 4);
-    float4 f[EACH];
-#pragma unroll
-    for (int u = 0; u < EACH; ++u) {
-        const int at = (first + 16 * u) * PART;
-        f[u] = at + chunk < V ? *reinterpret_cast<const float4*>(q + at) : make_float4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < EACH; ++u) {
-        const int part = first + 16 * u, at = part * PART + chunk;
-        if (part >= parts) return;  // uniform over a part's 16 lanes
-        float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
-        const float a = row_max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = at + i < V ? exp_nonpositive(v[i] - a) : 0.0f;
-        const float b = row_sum16((v[0] + v[1]) + (v[2] + v[3]));
-        if (chunk == 0) out[(size_t)row * parts + part] = make_float2(a, b);
-    }
-}
-
 __device__ __forceinline__ float wave_fmax(float m) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
     return m;
 }
 
-// A token from its parts (a wavefront each), its place among its word's, and the exponent of its row of
-// dz: that of the largest of the words other than the target (exp_nonpositive never falls).
-__global__ void __launch_bounds__(256)
-loss_tokens(const float* __restrict__ z, int ldz, int V, int parts, const float2* __restrict__ part, int first,
-            int rows, Targets t, bool lists, const float* __restrict__ factors, int mean, Token* __restrict__ tokens,
-            int* __restrict__ exponents) {
-    const int lane = threadIdx.x & 63;
-    const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
-    const int n = first + r, word = t.word[n];
-    Token k = repro_loss::ignored_token();
-    int exponent = 0;
-    if (word >= 0) {
-        const float2* p = part + (size_t)r * parts;
-        const float* q = z + (size_t)r * ldz;
-        const int own = word / PART;
-        float m = -INFINITY, other = -INFINITY;  // other: without the target's part
-        for (int i = lane; i < parts; i += 64) {
-            const float a = p[i].x;
-            m = fmaxf(m, a);
-            other = fmaxf(other, i == own ? -INFINITY : a);
+// A token by a block, in one read of its row of z: the parts' largest logits and sums (16 lanes a part, a lane
+// a chunk of 4 words, EACH parts in flight; the 64 strands' parts are those of the block's 64 groups of lanes),
+// from them the token, its place among its word's (arrived: where loss_words has listed them), and the
+// exponent of its row of dz: that of the largest of the words other than the target
+// (exp_nonpositive never falls). Reading z bounds it: 2048 rows of 50257 ROWS_US us, ROWS_TB TB/s. (By two launches,
+// parts and then tokens, ROWS_TWO; with the words' chunks in order, so that both were read here, 190.)
+// IN_LDS: the parts' maxima and sums are kept there, else in part[row].
+// Rows of z are ldz apart, a multiple of 32.
+constexpr int EACH = 4, STRIP = 1024 / 16;
+constexpr int LDS_PARTS = 4096;
+static_assert(STRIP == 64, "a group of lanes is a strand");
+
+template <bool IN_LDS>
+__global__ void __launch_bounds__(1024, 8)
+loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ part, int first, Targets t,
+          bool arrived, const float* __restrict__ factors, int mean, Token* __restrict__ tokens,
+          int* __restrict__ exponents) {
+    extern __shared__ float2 lds_part[];
+    __shared__ float maxima[STRIP], others[STRIP];
+    __shared__ float target_logit;
+    const int r = blockIdx.x, n = first + r, word = t.word[n], lane = threadIdx.x & 63;
+    if (word < 0) {  // uniform over the block
+        if (threadIdx.x == 0) {
+            Token k = repro_loss::ignored_token();
+            if (word == INVALID) k.loss = NAN;
+            if (arrived) t.lead[n] = make_int2(0, 0);
+            tokens[n] = k;
+            exponents[r] = 0;
         }
-        const int beside = own * PART + lane;
-        if (beside < V && beside != word) other = fmaxf(other, q[beside]);
-        m = wave_fmax(m);
-        other = wave_fmax(other);
-        float s = 0.0f;
-        for (int i = lane; i < parts; i += 64) s = s + p[i].y * exp_nonpositive(p[i].x - m);
-        s = wave_sum(s);
-        const float g = factors ? factors[n] : mean ? 1.0f / (float)t.counted[0] : 1.0f;
-        k = repro_loss::finish_token(m, s, q[word], g);
-        const float top = fabsf(exp_nonpositive(other - k.top) * k.factor);
-        exponent = repro_gemm::scale_exponent(top);  // 0 for a NaN
-        if (lists) {
-            const int place = t.place[word], count = t.count[word];
-            int before = 0;
-            for (int i = lane; i < count; i += 64) before += t.arrived[place + i] < n;
+        return;
+    }
+    float2* kept = IN_LDS ? lds_part : part + (size_t)r * parts;
+    const int strand = threadIdx.x >> 4, chunk = 4 * (threadIdx.x & 15), own = word / PART;
+    const float* q = z + (size_t)r * ldz + chunk;
+    float m = -INFINITY, other = -INFINITY;  // other: without the target
+    for (int base = strand; base < parts; base += STRIP * EACH) {
+        float4 f[EACH];
 #pragma unroll
-            for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
-            if (lane == 0) {
-                t.list[place + before] = n;
-                t.lead[n] = make_int2(before == 0 ? count : 0, place);
-            }
+        for (int u = 0; u < EACH; ++u) {
+            const int at = (base + STRIP * u) * PART;
+            f[u] = base + STRIP * u < parts && at + chunk < V ? *reinterpret_cast<const float4*>(q + at) : make_float4(0, 0, 0, 0);
         }
-    } else if (word == INVALID) {
-        k.loss = NAN;
+#pragma unroll
+        for (int u = 0; u < EACH; ++u) {
+            const int p = base + STRIP * u, at = p * PART + chunk;
+            if (p >= parts) break;  // uniform over a part's 16 lanes
+            float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
+            const float a = row_max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
+            m = fmaxf(m, a);
+            float o = a;
+            if (p == own) {
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = at + i == word ? -INFINITY : v[i];
+                    if (at + i == word) target_logit = v[i];
+                }
+                o = row_max16(fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])));
+            }
+            other = fmaxf(other, o);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = at + i < V ? exp_nonpositive(v[i] - a) : 0.0f;
+            const float b = row_sum16((v[0] + v[1]) + (v[2] + v[3]));
+            if (chunk == 0) kept[p] = make_float2(a, b);
+        }
+    }
+    if (chunk == 0) {
+        maxima[strand] = m;
+        others[strand] = other;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    m = wave_fmax(maxima[lane]);
+    other = wave_fmax(others[lane]);
+    float s = 0.0f;
+    for (int p = lane; p < parts; p += STRIP) s = s + kept[p].y * exp_nonpositive(kept[p].x - m);
+    s = wave_sum(s);
+    const float g = factors ? factors[n] : mean ? 1.0f / (float)t.counted[0] : 1.0f;
+    const Token k = repro_loss::finish_token(m, s, target_logit, g);
+    if (arrived) {
+        const int place = t.place[word], count = t.count[word];
+        int before = 0;
+        for (int i = lane; i < count; i += 64) before += t.arrived[place + i] < n;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
+        if (lane == 0) {
+            t.list[place + before] = n;
+            t.lead[n] = make_int2(before == 0 ? count : 0, place);
+        }
     }
     if (lane == 0) {
-        if (lists && word < 0) t.lead[n] = make_int2(0, 0);
         tokens[n] = k;
-        exponents[r] = exponent;
+        exponents[r] = repro_gemm::scale_exponent(fabsf(exp_nonpositive(other - k.top) * k.factor));  // 0 for a NaN
     }
 }
 
@@ -508,15 +578,47 @@ loss_digits(const float* __restrict__ z, int ldz, int V, int first, int rows, co
     }
 }
 
+// The sum or mean of the losses, by a block.
+template <int THREADS>
+__device__ __forceinline__ void reduce_losses(const Token* __restrict__ tokens, int N, int reduction,
+                                              const int* __restrict__ counted, float* __restrict__ loss) {
+    constexpr int OWN = repro_loss::STRANDS / THREADS;
+    __shared__ double lds[repro_loss::STRANDS];
+    double s[OWN];
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) s[k] = 0.0;
+#pragma unroll 4
+    for (int base = 0; base < N; base += repro_loss::STRANDS) {
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            const int n = base + k * THREADS + threadIdx.x;
+            if (n < N) s[k] = s[k] + (double)tokens[n].loss;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) lds[k * THREADS + threadIdx.x] = s[k];
+    for (int h = repro_loss::STRANDS / 2; h > 0; h /= 2) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < h; i += THREADS) lds[i] = lds[i] + lds[i + h];
+    }
+    if (threadIdx.x == 0) loss[0] = (float)(reduction == RG_LOSS_MEAN ? lds[0] / (double)counted[0] : lds[0]);
+}
+
 // ---- the target words' share ----
 //
 // A wavefront takes a token and 256 columns, of dx (blockIdx.z 0) or of dw, where a word's first token
 // stands for all of its tokens, 16 at a time. Most words have one, whose row's address is known without the list.
+// loss: where the losses' sum or mean is wanted, the first block of the launch takes it (a launch of its own: 5 us), and
+// the tokens start with the second.
 __global__ void __launch_bounds__(256)
 loss_target(float* __restrict__ dx, float* __restrict__ dw, const float* __restrict__ x, const float* __restrict__ w,
-            int D, const Token* __restrict__ tokens, Targets t, int N) {
+            int D, const Token* __restrict__ tokens, Targets t, int N, int reduction, float* __restrict__ loss) {
+    if (loss != nullptr && blockIdx.x == 0) {
+        if (blockIdx.y == 0 && blockIdx.z == 0) reduce_losses<256>(tokens, N, reduction, t.counted, loss);
+        return;
+    }
     const int lane = threadIdx.x & 63;
-    const int n = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = (blockIdx.x - (loss != nullptr)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int at = blockIdx.y * 256 + 4 * lane;
     if (n >= N || at >= D) return;
     const bool full = at + 4 <= D;
@@ -596,21 +698,8 @@ loss_target(float* __restrict__ dx, float* __restrict__ dw, const float* __restr
 // The losses, or their sum or mean (one block).
 __global__ void __launch_bounds__(1024)
 loss_reduce(const Token* __restrict__ tokens, int N, int reduction, const int* __restrict__ counted, float* __restrict__ loss) {
-    static_assert(repro_loss::STRANDS == 1024, "a thread a strand");
-    if (reduction == RG_LOSS_NONE) {
-        for (int n = blockIdx.x * 1024 + threadIdx.x; n < N; n += gridDim.x * 1024) loss[n] = tokens[n].loss;
-        return;
-    }
-    __shared__ double lds[1024];
-    double s = 0.0;
-#pragma unroll 8
-    for (int n = threadIdx.x; n < N; n += 1024) s = s + (double)tokens[n].loss;
-    lds[threadIdx.x] = s;
-    for (int h = 512; h > 0; h /= 2) {
-        __syncthreads();
-        if ((int)threadIdx.x < h) lds[threadIdx.x] = lds[threadIdx.x] + lds[threadIdx.x + h];
-    }
-    if (threadIdx.x == 0) loss[0] = (float)(reduction == RG_LOSS_MEAN ? lds[0] / (double)counted[0] : lds[0]);
+    if (reduction != RG_LOSS_NONE) return reduce_losses<1024>(tokens, N, reduction, counted, loss);
+    for (int n = blockIdx.x * 1024 + threadIdx.x; n < N; n += gridDim.x * 1024) loss[n] = tokens[n].loss;
 }
 
 __global__ void __launch_bounds__(256) loss_fill(float* __restrict__ a, float v, size_t n) {
@@ -699,7 +788,7 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
     }
     s->words = take(((size_t)6 * N + 2 * (size_t)round_up(V, 32) + 1) * sizeof(int));
     s->tokens = take((size_t)N * sizeof(Token));
-    s->part = take((size_t)s->group * s->parts * sizeof(float2));
+    s->part = take(s->parts <= LDS_PARTS ? 0 : (size_t)s->group * s->parts * sizeof(float2));
     s->logits = take((size_t)s->group * s->ldz * sizeof(float));
     s->x_rows = digits(N, D);
     s->w_rows = digits(s->few ? 0 : V, D);
@@ -805,8 +894,12 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     int64_t* partial = reinterpret_cast<int64_t*>(base + s.partial);
     float* scratch = reinterpret_cast<float*>(base + s.scratch);
 
-    hipLaunchKernelGGL(loss_words, dim3(dw && N > MANY_WORDS ? 16 : 1), dim3(1024), 0, st, target, cfg->ignore_index, N, V,
-                       dw != nullptr, t);
+    const bool ranked = !dw || N <= FEW_WORDS;
+    if (ranked)
+        hipLaunchKernelGGL(loss_ranks, dim3((N + RANKED - 1) / RANKED), dim3(16 * RANKED), 0, st, target, cfg->ignore_index,
+                           N, V, dw != nullptr, t);
+    else
+        hipLaunchKernelGGL(loss_words, dim3(16), dim3(1024), 0, st, target, cfg->ignore_index, N, V, t);
     // The digits that every group's products share.
     if (s.few)
         rc = launch_slice(x, N, D, false, S, panels(s.x_rows), exponents(s.x_rows), scratch, st);
@@ -824,10 +917,10 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
             launch_product(s.z[k], panels(s.x_rows) + (size_t)first * round_up(D, STEP_K) * S, exponents(s.x_rows) + first,
                            panels(s.w_rows), exponents(s.w_rows), z, s.ldz, false, partial, st);
         }
-        hipLaunchKernelGGL(loss_parts, dim3((s.parts + 16 * EACH - 1) / (16 * EACH), rows), dim3(256), 0, st, z, s.ldz, V,
-                           s.parts, part);
-        hipLaunchKernelGGL(loss_tokens, dim3((rows + 3) / 4), dim3(256), 0, st, z, s.ldz, V, s.parts, part, first, rows,
-                           t, dw != nullptr, factors, cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, exponents(s.by_token));
+        const bool in_lds = s.parts <= LDS_PARTS;
+        hipLaunchKernelGGL(in_lds ? loss_rows<true> : loss_rows<false>, dim3(rows), dim3(1024),
+                           in_lds ? s.parts * sizeof(float2) : 0, st, z, s.ldz, V, s.parts, part, first, t, !ranked, factors,
+                           cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, exponents(s.by_token));
         if (!dx && !dw) continue;
         DigitsOut out;
         out.by_token = dx ? panels(s.by_token) : nullptr;
@@ -849,10 +942,11 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
                            dw, D, first > 0, partial, st);
         }
     }
+    const bool joined = loss && cfg->reduction != RG_LOSS_NONE && (dx || dw);
     if (dx || dw)
-        hipLaunchKernelGGL(loss_target, dim3((N + 3) / 4, (D + 255) / 256, dx && dw ? 2 : 1), dim3(256), 0, st, dx, dw, x,
-                           w, D, tokens, t, N);
-    if (loss)
+        hipLaunchKernelGGL(loss_target, dim3((N + 3) / 4 + joined, (D + 255) / 256, dx && dw ? 2 : 1), dim3(256), 0, st, dx,
+                           dw, x, w, D, tokens, t, N, cfg->reduction, joined ? loss : nullptr);
+    if (loss && !joined)
         hipLaunchKernelGGL(loss_reduce, dim3(cfg->reduction == RG_LOSS_NONE ? std::min((N + 1023) / 1024, 1024) : 1),
                            dim3(1024), 0, st, tokens, N, cfg->reduction, t.counted, loss);
     return hipGetLastError();

@@ -9,7 +9,6 @@
 // whose first level adds l and l + 32, the next l and l + 16, and so on.
 //
 // Sum over rows (the gradients of weights, biases and gates): see Partition.
-#include <vector>
 
 #include "repro_gemm_math.h"
 

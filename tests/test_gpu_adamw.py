@@ -108,3 +108,18 @@ def test_tensors_on_two_devices_are_refused():
         rg.adamw_step(p, [g[0].cpu()], m, v, step=1)
     with pytest.raises(ValueError):
         rg.adamw_step(p + [torch.zeros(3)], g + [torch.zeros(3)], m + [torch.zeros(3)], v + [torch.zeros(3)], step=1)
+
+
+@pytest.mark.parametrize("count", [3, 127, 128, 129, 300])
+def test_moments_in_one_row_or_apart_take_the_same_step(count):
+    sizes = [(1 + (37 * i) % 700,) for i in range(count)]
+    p, g, _, _ = tensors(sizes, count, "cuda")
+    q = [t.clone() for t in p]
+    row = rg.adamw8_state(p)
+    apart = [[torch.zeros(len_, dtype=torch.uint8, device="cuda") for len_ in lens]
+             for lens in ([-(-t.numel() // 256) * k for t in p] for k in (256, 1, 256, 1))]
+    for step in (1, 2):
+        rg.adamw8_step(p, g, *row, step=step)
+        rg.adamw8_step(q, g, *apart, step=step)
+    assert same([t.cpu() for t in p], q)
+    assert all(torch.equal(a, torch.cat(b)) for a, b in zip(row, apart))

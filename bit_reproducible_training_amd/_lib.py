@@ -1,5 +1,5 @@
-"""Loads librepro_gemm.so (the C ABI in include/repro_gemm.h, include/repro_sum.h and
-include/repro_conv.h) through ctypes, and the compiled PyTorch binding (_backend) that calls the
+"""Loads librepro_gemm.so (the C ABI in include/repro_gemm.h, repro_sum.h, repro_conv.h,
+repro_loss.h, repro_norm.h and repro_adamw.h) through ctypes, and the compiled PyTorch binding (_backend) that calls the
 same library for tensors.
 
 Both must have been built (bit_reproducible_training_amd._build.build(), or

@@ -3,6 +3,10 @@
 // Tokens are taken in groups (repro_loss::group_tokens), a group's logits z are one product, and its
 // gradient dz two more with them: three products in all, where pieces of the vocabulary, whose
 // softmax is not known before the last piece, need z a second time.
+//
+// The matrix cores bound it: of 7.74 ms for 8192 tokens of 768 values against 50257 words (S = 3, four groups, dx and
+// dw) the products take 6.05, at 313 TFLOP/s of float32 work, the digits of dz 0.99, the rows' statistics
+// 0.38, slicing x and the weight 0.18, the target words 0.07.
 #include "rg_digits.h"
 #include "rg_internal.h"
 #include "repro_loss.h"
@@ -178,8 +182,8 @@ loss_ranks(const long long* __restrict__ target, long long ignore_index, int N, 
     t.lead[n] = make_int2(word >= 0 && before == 0 ? same : 0, smaller);
     if (word >= 0) t.list[smaller + before] = n;
 }
-// Tokens up to which loss_ranks lists them. us of loss_ranks and of loss_words for 96 tokens RANK96, 1024 RANK1024, 4096
-// RANK4096, 8192 RANK8192.
+// Tokens up to which loss_ranks lists them (us by it and by loss_words: 96 tokens 5.0 and 10.7, 1024 8.5 and 13.8, 2048 13.2
+// and 16.8, 4096 19.4 and 19.7, 8192 36.6 and 26.2).
 constexpr int FEW_WORDS = 4096;
 
 template <int CTRL>
@@ -312,19 +316,20 @@ __device__ __forceinline__ float wave_fmax(float m) {
 }
 
 // A token by a block, in one read of its row of z: the parts' largest logits and sums (16 lanes a part, a lane
-// a chunk of 4 words, EACH parts in flight; the 64 strands' parts are those of the block's 64 groups of lanes),
-// from them the token, its place among its word's (arrived: where loss_words has listed them), and the
-// exponent of its row of dz: that of the largest of the words other than the target
-// (exp_nonpositive never falls). Reading z bounds it: 2048 rows of 50257 ROWS_US us, ROWS_TB TB/s. (By two launches,
-// parts and then tokens, ROWS_TWO; with the words' chunks in order, so that both were read here, 190.)
+// a chunk of 4 words, EACH parts in flight), from them the token, its place among its word's (arrived: where
+// loss_words has listed them), and the exponent of its row of dz: that of the largest of the words
+// other than the target (exp_nonpositive never falls).
+// 2047 rows of 50257 take 88 us, 4.7 TB/s, with about 20 vector instructions a logit, the exponential's 13 among
+// them, in the same time; 1024 rows 61. By two launches, parts and then tokens, 96 and 67; with the next
+// parts in flight 103 and 65; by 512 threads 84 and 61, by 256 87 and 62, but for one token 5 and 15 us more.
 // IN_LDS: the parts' maxima and sums are kept there, else in part[row].
 // Rows of z are ldz apart, a multiple of 32.
-constexpr int EACH = 4, STRIP = 1024 / 16;
+constexpr int EACH = 4, ROW_THREADS = 1024, STRIP = ROW_THREADS / 16;
 constexpr int LDS_PARTS = 4096;
-static_assert(STRIP == 64, "a group of lanes is a strand");
+static_assert(STRIP == 64, "a wavefront reads the groups' maxima");
 
 template <bool IN_LDS>
-__global__ void __launch_bounds__(1024, 8)
+__global__ void __launch_bounds__(ROW_THREADS, 8)
 loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __restrict__ part, int first, Targets t,
           bool arrived, const float* __restrict__ factors, int mean, Token* __restrict__ tokens,
           int* __restrict__ exponents) {
@@ -343,10 +348,10 @@ loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __rest
         return;
     }
     float2* kept = IN_LDS ? lds_part : part + (size_t)r * parts;
-    const int strand = threadIdx.x >> 4, chunk = 4 * (threadIdx.x & 15), own = word / PART;
+    const int group = threadIdx.x >> 4, chunk = 4 * (threadIdx.x & 15), own = word / PART;
     const float* q = z + (size_t)r * ldz + chunk;
     float m = -INFINITY, other = -INFINITY;  // other: without the target
-    for (int base = strand; base < parts; base += STRIP * EACH) {
+    for (int base = group; base < parts; base += STRIP * EACH) {
         float4 f[EACH];
 #pragma unroll
         for (int u = 0; u < EACH; ++u) {
@@ -358,8 +363,10 @@ loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __rest
             const int p = base + STRIP * u, at = p * PART + chunk;
             if (p >= parts) break;  // uniform over a part's 16 lanes
             float v[4] = {f[u].x, f[u].y, f[u].z, f[u].w};
+            if (p == parts - 1) {  // words past the last: e^-inf
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
+                for (int i = 0; i < 4; ++i) v[i] = at + i < V ? v[i] : -INFINITY;
+            }
             const float a = row_max16(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
             m = fmaxf(m, a);
             float o = a;
@@ -374,21 +381,25 @@ loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __rest
             }
             other = fmaxf(other, o);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = at + i < V ? exp_nonpositive(v[i] - a) : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                const float x = v[i] - a;
+                v[i] = x >= -87.0f ? repro_loss::exp_in_range(x) : 0.0f;
+            }
+            // Logits are never NaN (a product is a rounded whole number), so v - a is only where a is infinite.
             const float b = row_sum16((v[0] + v[1]) + (v[2] + v[3]));
-            if (chunk == 0) kept[p] = make_float2(a, b);
+            if (chunk == 0) kept[p] = make_float2(a, fabsf(a) < INFINITY ? b : NAN);
         }
     }
     if (chunk == 0) {
-        maxima[strand] = m;
-        others[strand] = other;
+        maxima[group] = m;
+        others[group] = other;
     }
     __syncthreads();
     if (threadIdx.x >= 64) return;
     m = wave_fmax(maxima[lane]);
     other = wave_fmax(others[lane]);
     float s = 0.0f;
-    for (int p = lane; p < parts; p += STRIP) s = s + kept[p].y * exp_nonpositive(kept[p].x - m);
+    for (int p = lane; p < parts; p += 64) s = s + kept[p].y * exp_nonpositive(kept[p].x - m);
     s = wave_sum(s);
     const float g = factors ? factors[n] : mean ? 1.0f / (float)t.counted[0] : 1.0f;
     const Token k = repro_loss::finish_token(m, s, target_logit, g);
@@ -918,7 +929,7 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
                            panels(s.w_rows), exponents(s.w_rows), z, s.ldz, false, partial, st);
         }
         const bool in_lds = s.parts <= LDS_PARTS;
-        hipLaunchKernelGGL(in_lds ? loss_rows<true> : loss_rows<false>, dim3(rows), dim3(1024),
+        hipLaunchKernelGGL(in_lds ? loss_rows<true> : loss_rows<false>, dim3(rows), dim3(ROW_THREADS),
                            in_lds ? s.parts * sizeof(float2) : 0, st, z, s.ldz, V, s.parts, part, first, t, !ranked, factors,
                            cfg->reduction == RG_LOSS_MEAN ? 1 : 0, tokens, exponents(s.by_token));
         if (!dx && !dw) continue;

@@ -6,11 +6,10 @@
 // taken from there. A row of at most 1024 values is one wavefront's, whose sums need no barrier; wider
 // ones take 8 or 16, which hold the next row while they work on one.
 //
-// HBM bounds both passes: 16 bytes a value forward (x, f, r, y) and up to 24 backward (dr, dy, r, f, dx, df).
-// 8192 rows of 768 (layer norm of x, no f: 8 and 12 bytes): 17.7 and 23.3 us, small enough for the caches to hold
-// part of it. 4096 rows of 4096 with both norms and a gate: 55 and 90 us, 4.8 and 4.5 TB/s, where a copy of 1 GiB
-// reaches 5.1. Sums over rows (the weights' gradients) stay in registers over a block's rows and meet in
-// norm_totals, 4 to 6 us.
+// HBM bounds both passes: 16 bytes a value forward (x, f, r, y) and 16 to 24 backward (dr, dy, r, dx, and f and df).
+// 8192 rows of 768: 17.3 us forward (101 MB, partly in the caches: 5.8 TB/s) and 23.2 backward. 4096 rows of
+// 4096 with both norms and a gate: 56 and 91 us, 4.8 and 4.4 TB/s, where a copy of 1 GiB reaches 5.1. Sums over
+// rows (the weights' gradients) stay in registers over a block's rows and meet in norm_totals, 4 to 7 us.
 #include "rg_internal.h"
 #include "repro_norm.h"
 #include "repro_norm_math.h"

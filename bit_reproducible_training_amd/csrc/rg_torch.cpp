@@ -1,7 +1,7 @@
 // PyTorch binding of the reproducible operations: the compiled counterpart of the reference's
 // repro_torch/src/bindings.cpp:43-175,286-297 (_backend.gemm, exact_sum, conv2d,
 // conv2d_grad_weight, conv2d_grad_input, scan_finite), with the same names, arguments, checks
-// and results.
+// and results; and the vocabulary loss, the residual norms (with their autograd nodes) and the AdamW steps.
 //
 // A GPU tensor runs on the MI355X library (librepro_gemm.so, through its C ABI) on PyTorch's
 // current HIP stream of the tensor's device, with the workspace taken from PyTorch's caching

@@ -184,7 +184,7 @@ loss_ranks(const long long* __restrict__ target, long long ignore_index, int N, 
 }
 // Tokens up to which loss_ranks lists them (us by it and by loss_words: 96 tokens 5.0 and 10.7, 1024 8.5 and 13.8, 2048 13.2
 // and 16.8, 4096 19.4 and 19.7, 8192 36.6 and 26.2).
-constexpr int FEW_WORDS = 4096;
+constexpr int RANKS_MAX = 4096;
 
 template <int CTRL>
 __device__ __forceinline__ float rotated(float v) {
@@ -213,28 +213,31 @@ __device__ __forceinline__ float wave_sum(float v) {
 // ---- the logits of few tokens ----
 //
 // Few tokens' logits are bound by reading the weight once; slicing it first writes 3 bytes for each 4 it reads
-// and reads them again. Here a block holds 32 words in registers: its wavefronts take k panels (32 words x 32
-// values) in turn, 16 values of a word a lane, find the words' scales together, round, and contract
-// the digits from registers with the tokens' digits, a tile of 32 at most. The wavefronts' exact integer sums
-// meet in LDS. A block is mostly latency, so more tokens or values lose again: losses of 1 and 32 tokens of
-// GPT-2 small's head 63 and 71 us against 88 and 96 by slicing and contracting; of 64 (two tiles) 98 against 102, of 128
-// 139 against 118; with 1600 values a word (eight wavefronts) 181 against 178.
-constexpr int FEW_TOKENS = 32, FEW_WAVES = 4, FEW_MAX_D = 1024;
+// and reads them again. Here a block holds 16 words in registers: its wavefronts take pieces of 64 values of
+// each in turn, 16 values of a word a lane, find the words' scales together, round, and contract the digits
+// from registers with the tokens' digits, TILES times 16 tokens. The wavefronts' exact integer sums
+// meet in LDS. Reading the weight bounds it, at half of HBM's rate, as a block's loads, rounding and products follow
+// each other and registers allow few blocks at once. Whole calls without gradients, us, here and by slicing and contracting:
+// GPT-2 small's head with 1, 32 and 64 tokens 54, 63 and 91 against 88, 96 and 99; 1600 values a word 117, 152 and 193
+// against 180, 186 and 191; 32000 words of 2048 with 32 and 64 tokens 100 and 128 against 146 and 150; 1000 of 256 with
+// 8 18 against 17. (32 words a block, for one token of GPT-2 small's head 64.)
+constexpr int FEW_TOKENS = 64, FEW_WAVES = 4, FEW_WORDS_EACH = 16, FEW_K = 2 * PANEL_K, FEW_MAX_D = 8 * FEW_WAVES * FEW_K;
+static_assert(STEP_K % FEW_K == 0, "tokens' digits come in whole pieces");
 
-template <int S, int PW>
-__global__ void __launch_bounds__(64 * FEW_WAVES, 2)
-loss_few(const float* __restrict__ w, int V, int D, int panels, const int8_t* __restrict__ qx, const int* __restrict__ ex,
+template <int S, int PW, int TILES>
+__global__ void __launch_bounds__(64 * FEW_WAVES, PW <= 3 ? 4 : PW <= 4 ? 3 : 2)
+loss_few(const float* __restrict__ w, int V, int D, int pieces, const int8_t* __restrict__ qx, const int* __restrict__ ex,
          int N, float* __restrict__ z, int ldz) {
     constexpr int L = 2 * S - 1;
-    __shared__ int64_t sums[FEW_WAVES][16][64];
-    __shared__ uint32_t tops[FEW_WAVES][32];
+    __shared__ int64_t sums[FEW_WAVES][4 * TILES][64];
+    __shared__ uint32_t tops[FEW_WAVES][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int word = blockIdx.x * 32 + (lane & 31);
+    const int word = blockIdx.x * FEW_WORDS_EACH + (lane & 15);
     const float* row = w + (size_t)min(word, V - 1) * D;
     float f[PW][16];
 #pragma unroll
     for (int p = 0; p < PW; ++p) {
-        const int k0 = (wave + FEW_WAVES * p) * PANEL_K + 16 * (lane >> 5);
+        const int k0 = (wave + FEW_WAVES * p) * FEW_K + 16 * (lane >> 4);
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
             if (k0 + j + 4 <= D) {
@@ -252,61 +255,81 @@ loss_few(const float* __restrict__ w, int V, int D, int panels, const int8_t* __
     for (int p = 0; p < PW; ++p)
 #pragma unroll
         for (int j = 0; j < 16; ++j) top = max(top, repro_gemm::magnitude_key(f[p][j]));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    if (lane < 32) tops[wave][lane] = top;
+    if (lane < 16) tops[wave][lane] = top;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < FEW_WAVES; ++i) top = max(top, tops[i][lane & 31]);
+    for (int i = 0; i < FEW_WAVES; ++i) top = max(top, tops[i][lane & 15]);
     const int ew = repro_gemm::scale_exponent(__uint_as_float(top));
     const RowScale scale = row_scale<S>(ew);
-    v16i acc[L];
+    v4i acc[TILES][L];
 #pragma unroll
-    for (int l = 0; l < L; ++l)
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) acc[l][e] = 0;
+        for (int l = 0; l < L; ++l) acc[t][l] = v4i{0, 0, 0, 0};
 #pragma unroll
     for (int p = 0; p < PW; ++p) {
-        // Past the last panel the weight's digits are zero: any of the tokens' will do.
-        const int8_t* qa = qx + (size_t)min(wave + FEW_WAVES * p, panels - 1) * (S * PANEL_BYTES) + lane * 16;
-        v4i a[S], b[S];
+        // Past the last piece the weight's digits are zero: any of the tokens' will do. A panel is 32 tokens x
+        // 32 values, its halves of 16 values one after the other.
+        const int8_t* qa = qx + (size_t)min(wave + FEW_WAVES * p, pieces - 1) * (2 * S * PANEL_BYTES) +
+                           (lane >> 5) * (S * PANEL_BYTES) + (lane >> 4 & 1) * 512 + (lane & 15) * 16;
+        v4i a[TILES][S], b[S];
 #pragma unroll
-        for (int i = 0; i < S; ++i) a[i] = *reinterpret_cast<const v4i*>(qa + i * PANEL_BYTES);
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < S; ++i) a[t][i] = *reinterpret_cast<const v4i*>(qa + (size_t)(t >> 1) * pieces * (2 * S * PANEL_BYTES) + i * PANEL_BYTES + (t & 1) * 256);
         int x[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = round_fixed(f[p][j], scale);
         pack16<S>(x, b);
 #pragma unroll
-        for (int i = 0; i < S; ++i)
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-            for (int j = 0; j < S; ++j)
-                acc[i + j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i + j], 0, 0, 0);
+            for (int i = 0; i < S; ++i)
+#pragma unroll
+                for (int j = 0; j < S; ++j)
+                    acc[t][i + j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[t][i], b[j], acc[t][i + j], 0, 0, 0);
     }
-    // Register e of the tile holds token 8 (e / 4) + 4 (lane / 32) + e % 4 and its lane's word.
+    // Register e of tile t holds token 16 t + 4 (lane / 16) + e and its lane's word.
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        if (8 * (e >> 2) >= N) break;  // uniform: nobody's
-        int lv[L];
+    for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int l = 0; l < L; ++l) lv[l] = acc[l][e];
-        sums[wave][e][lane] = combine_levels<L>(lv);
-    }
+        for (int e = 0; e < 4; ++e) {
+            int lv[L];
+#pragma unroll
+            for (int l = 0; l < L; ++l) lv[l] = acc[t][l][e];
+            sums[wave][4 * t + e][lane] = combine_levels<L>(lv);
+        }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 16 / FEW_WAVES; ++i) {
-        if (8 * i >= N) break;
-        const int e = wave + FEW_WAVES * i, n = 8 * i + 4 * (lane >> 5) + wave;
-        int64_t t = 0;
+    for (int t = 0; t < TILES; ++t) {
+        const int n = 16 * t + 4 * (lane >> 4) + wave;
+        int64_t sum = 0;
 #pragma unroll
-        for (int k = 0; k < FEW_WAVES; ++k) t += sums[k][e][lane];
-        if (n < N && word < V) z[(size_t)n * ldz + word] = round_output(t, ex[n] + ew - 14 * (S - 1));
+        for (int k = 0; k < FEW_WAVES; ++k) sum += sums[k][4 * t + wave][lane];
+        if (n < N && word < V) z[(size_t)n * ldz + word] = round_output(sum, ex[n] + ew - 14 * (S - 1));
     }
 }
 
+template <int S, int TILES>
+void launch_few_tiles(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, hipStream_t st) {
+    const int pieces = (D + STEP_K - 1) / STEP_K * (STEP_K / FEW_K);  // as the slicing pads
+    const int each = ((D + FEW_K - 1) / FEW_K + FEW_WAVES - 1) / FEW_WAVES;
+    auto kernel = each <= 1   ? loss_few<S, 1, TILES>
+                  : each <= 2 ? loss_few<S, 2, TILES>
+                  : each <= 3 ? loss_few<S, 3, TILES>
+                  : each <= 4 ? loss_few<S, 4, TILES>
+                  : each <= 6 ? loss_few<S, 6, TILES>
+                              : loss_few<S, 8, TILES>;
+    hipLaunchKernelGGL(kernel, dim3((V + FEW_WORDS_EACH - 1) / FEW_WORDS_EACH), dim3(64 * FEW_WAVES), 0, st, w, V, D, pieces, qx,
+                       ex, N, z, ldz);
+}
 template <int S>
 void launch_few_s(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, hipStream_t st) {
-    const int panels = (D + STEP_K - 1) / STEP_K * (STEP_K / PANEL_K);  // as the slicing pads
-    auto kernel = panels <= 8 ? loss_few<S, 2> : panels <= 16 ? loss_few<S, 4> : panels <= 24 ? loss_few<S, 6> : loss_few<S, 8>;
-    hipLaunchKernelGGL(kernel, dim3((V + 31) / 32), dim3(64 * FEW_WAVES), 0, st, w, V, D, panels, qx, ex, N, z, ldz);
+    if (N <= 16) launch_few_tiles<S, 1>(w, V, D, qx, ex, N, z, ldz, st);
+    else if (N <= 32) launch_few_tiles<S, 2>(w, V, D, qx, ex, N, z, ldz, st);
+    else launch_few_tiles<S, 4>(w, V, D, qx, ex, N, z, ldz, st);
 }
 
 __device__ __forceinline__ float wave_fmax(float m) {
@@ -905,7 +928,7 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     int64_t* partial = reinterpret_cast<int64_t*>(base + s.partial);
     float* scratch = reinterpret_cast<float*>(base + s.scratch);
 
-    const bool ranked = !dw || N <= FEW_WORDS;
+    const bool ranked = !dw || N <= RANKS_MAX;
     if (ranked)
         hipLaunchKernelGGL(loss_ranks, dim3((N + RANKED - 1) / RANKED), dim3(16 * RANKED), 0, st, target, cfg->ignore_index,
                            N, V, dw != nullptr, t);

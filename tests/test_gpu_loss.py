@@ -137,3 +137,22 @@ def test_refuses_tensors_on_two_devices():
     for bad in ((x, w.cpu(), t), (x, w, t.cpu()), (x.cpu(), w, t)):
         with pytest.raises(ValueError):
             rg.linear_cross_entropy(*bad)
+
+
+@pytest.mark.parametrize("S", [1, 2, 3])
+@pytest.mark.parametrize("n", [1, 16, 17, 32, 33, 64, 65])
+def test_few_tokens_of_every_width(n, S):
+    for d in (1, 256, 257, 600, 1000, 1025, 1540, 1700, 2047, 2048, 2049):
+        x, w, t = case(n, d, 50, seed=n + d, lean=2.0)
+        with torch.no_grad():
+            got = rg.linear_cross_entropy(x.cuda(), w.cuda(), t.cuda(), reduction="none", slices=S)
+            want = rg.linear_cross_entropy(x, w, t, reduction="none", slices=S)
+        assert torch.equal(got.cpu().view(torch.int32), want.view(torch.int32)), d
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 9001])
+@pytest.mark.parametrize("words", [1, 700])
+def test_many_tokens_of_the_same_words(n, words):
+    x, w, t = case(n, 5, 700, seed=n, words=words, ignored=range(3, n, 11))
+    t[5::97], t[7::101] = 700, -3
+    assert_same(results(x.cuda(), w.cuda(), t.cuda()), results(x, w, t))

@@ -218,9 +218,10 @@ __device__ __forceinline__ float wave_sum(float v) {
 // from registers with the tokens' digits, TILES times 16 tokens. The wavefronts' exact integer sums
 // meet in LDS. Reading the weight bounds it, at half of HBM's rate, as a block's loads, rounding and products follow
 // each other and registers allow few blocks at once. Whole calls without gradients, us, here and by slicing and contracting:
-// GPT-2 small's head with 1, 32 and 64 tokens 54, 63 and 91 against 88, 96 and 99; 1600 values a word 117, 152 and 193
-// against 180, 186 and 191; 32000 words of 2048 with 32 and 64 tokens 100 and 128 against 146 and 150; 1000 of 256 with
-// 8 18 against 17. (32 words a block, for one token of GPT-2 small's head 64.)
+// GPT-2 small's head with 1, 32 and 64 tokens 54, 63 and 92 against 88, 96 and 99; 1600 values a word 115, 134 and 185
+// against 180, 186 and 191; 32000 words of 2048 with 32 and 64 tokens 101 and 128 against 146 and 150; 1000 of 256 with
+// 8 the same 17. (32 words a block, for one token of GPT-2 small's head 64; registers for 8 pieces where 7 do, for 32
+// tokens of 1600 values 153.)
 constexpr int FEW_TOKENS = 64, FEW_WAVES = 4, FEW_WORDS_EACH = 16, FEW_K = 2 * PANEL_K, FEW_MAX_D = 8 * FEW_WAVES * FEW_K;
 static_assert(STEP_K % FEW_K == 0, "tokens' digits come in whole pieces");
 
@@ -316,13 +317,10 @@ template <int S, int TILES>
 void launch_few_tiles(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, hipStream_t st) {
     const int pieces = (D + STEP_K - 1) / STEP_K * (STEP_K / FEW_K);  // as the slicing pads
     const int each = ((D + FEW_K - 1) / FEW_K + FEW_WAVES - 1) / FEW_WAVES;
-    auto kernel = each <= 1   ? loss_few<S, 1, TILES>
-                  : each <= 2 ? loss_few<S, 2, TILES>
-                  : each <= 3 ? loss_few<S, 3, TILES>
-                  : each <= 4 ? loss_few<S, 4, TILES>
-                  : each <= 6 ? loss_few<S, 6, TILES>
-                              : loss_few<S, 8, TILES>;
-    hipLaunchKernelGGL(kernel, dim3((V + FEW_WORDS_EACH - 1) / FEW_WORDS_EACH), dim3(64 * FEW_WAVES), 0, st, w, V, D, pieces, qx,
+    decltype(&loss_few<S, 1, TILES>) kernels[] = {loss_few<S, 1, TILES>, loss_few<S, 2, TILES>, loss_few<S, 3, TILES>,
+                                                  loss_few<S, 4, TILES>, loss_few<S, 5, TILES>, loss_few<S, 6, TILES>,
+                                                  loss_few<S, 7, TILES>, loss_few<S, 8, TILES>};
+    hipLaunchKernelGGL(kernels[each - 1], dim3((V + FEW_WORDS_EACH - 1) / FEW_WORDS_EACH), dim3(64 * FEW_WAVES), 0, st, w, V, D, pieces, qx,
                        ex, N, z, ldz);
 }
 template <int S>

@@ -4,7 +4,7 @@
 // copy there first), and its blocks are dealt to them by chunks: a block finds its tensor by the
 // tensors' first chunks, all read at once.
 //
-// In float32 HBM bounds it: 28 bytes a value, 600 us for 124 million values of 148 tensors, 5.8 TB/s where a
+// In float32 HBM bounds it: 28 bytes a value, 640 us for 124 million values of 148 tensors, 5.4 TB/s where a
 // copy of 1 GiB reaches 5.1. With moments in 8 bits 16 bytes a value remain and the vector units bound it, see there.
 #include "rg_internal.h"
 #include "repro_adamw.h"
@@ -85,12 +85,11 @@ __device__ __forceinline__ int entry_of(const List<E>& list, uint32_t chunk) {
     return __popcll(__ballot(a <= chunk)) + __popcll(__ballot(b <= chunk)) - 1;
 }
 
-// What a step reads once, and the moments, which the next step reads after everything else, past the caches; the new
-// parameters stay there for what follows (124 million values 642 -> 600 us; with the parameters past them too 597; the
-// loads alone 612; in the 8-bit step, which the vector units bound, 1%).
+// What a step reads is written again or not needed any more: its loads leave nothing in the caches (124 million values 658
+// -> 640 us; with the moments' stores past the caches too 642. In the 8-bit step 435 -> 423, but reading the moments back
+// right after it took 10 longer).
 typedef float v4f __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ v4f load_once(const float* p) { return __builtin_nontemporal_load(reinterpret_cast<const v4f*>(p)); }
-__device__ __forceinline__ void store_away(float* p, v4f v) { __builtin_nontemporal_store(v, reinterpret_cast<v4f*>(p)); }
 
 // A chunk is 4 U values a thread. 16-byte accesses where all four arrays allow them, else single
 // values, neighbouring threads on neighbouring values either way.
@@ -129,8 +128,8 @@ adamw_kernel(const List<Entry> list) {
                 vv[u][k] = vk;
             }
             reinterpret_cast<v4f*>(p)[i] = pv[u];
-            store_away(m + 4 * i, mv[u]);
-            store_away(v + 4 * i, vv[u]);
+            reinterpret_cast<v4f*>(m)[i] = mv[u];
+            reinterpret_cast<v4f*>(v)[i] = vv[u];
         }
         return;
     }
@@ -228,7 +227,7 @@ struct Block8 {
 
 // A wavefront takes U blocks in turn, all of them loaded before the first is stepped. (Eight a wavefront in a loop,
 // fewer searches of the list: no faster. The arithmetic bounds it: about 100 vector instructions a
-// value, 465 us for 124 million of them.)
+// value, 430 to 465 us for 124 million of them.)
 template <int U, class E>
 __global__ void __launch_bounds__(THREADS)
 adamw8_kernel(const List<E> list) {

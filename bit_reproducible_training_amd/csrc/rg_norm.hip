@@ -8,8 +8,9 @@
 //
 // HBM bounds both passes: 16 bytes a value forward (x, f, r, y) and 16 to 24 backward (dr, dy, r, dx, and f and df).
 // 8192 rows of 768: 17.3 us forward (101 MB, partly in the caches: 5.8 TB/s) and 23.2 backward. 4096 rows of
-// 4096 with both norms and a gate: 56 and 91 us, 4.8 and 4.4 TB/s, where a copy of 1 GiB reaches 5.1. Sums over
-// rows (the weights' gradients) stay in registers over a block's rows and meet in norm_totals, 4 to 7 us.
+// 4096 with both norms and a gate: 56 and 91 us, 4.8 and 4.4 TB/s, where a copy of 1 GiB reaches 5.1 (with loads
+// and stores past the caches 53 and 88, but 19.6 and 26.8 for the 8192 rows of 768, which find each other's rows
+// there). Sums over rows (the weights' gradients) stay in registers over a block's rows and meet in norm_totals, 4 to 7 us.
 #include "rg_internal.h"
 #include "repro_norm.h"
 #include "repro_norm_math.h"

@@ -406,9 +406,10 @@ loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __rest
                 const float x = v[i] - a;
                 v[i] = x >= -87.0f ? repro_loss::exp_in_range(x) : 0.0f;
             }
-            // Logits are never NaN (a product is a rounded whole number), so v - a is only where a is infinite.
+            // Logits are never NaN (a product is a rounded whole number), so v - a is only where a is infinite, and
+            // counted as 0 above: the sum of a part whose logits are all -infinity, while +infinity has none.
             const float b = row_sum16((v[0] + v[1]) + (v[2] + v[3]));
-            if (chunk == 0) kept[p] = make_float2(a, fabsf(a) < INFINITY ? b : NAN);
+            if (chunk == 0) kept[p] = make_float2(a, a < INFINITY ? b : NAN);
         }
     }
     if (chunk == 0) {

@@ -38,7 +38,7 @@ inline void largest_and_sum(const float* z, int V, float& m, float& s) {
             for (int i = 0; i < 4; ++i) e[i] = 4 * c + i < n ? exp_nonpositive(q[4 * c + i] - a[p]) : 0.0f;
             chunk[c] = (e[0] + e[1]) + (e[2] + e[3]);
         }
-        b[p] = halves(chunk, PART / 4);
+        b[p] = a[p] == -INFINITY ? 0.0f : halves(chunk, PART / 4);
     }
     m = a[0];
     for (int p = 1; p < parts; ++p) m = std::fmax(m, a[p]);

@@ -57,7 +57,7 @@ RG_HD inline double log_positive(float s) {
 // A token's logits z are taken in parts of PART consecutive words (the last may be shorter). A part has its
 // largest logit a and its sum b of e^(z - a): chunks of 4 consecutive words (missing ones 0) give
 // (v0 + v1) + (v2 + v3), and the chunks are added as a balanced tree whose first level adds chunks c and
-// c + 8, the next c and c + 4, and so on. The token's largest logit is m = max a, and its sum s that of
+// c + 8, the next c and c + 4, and so on; b is 0 where a is -infinity. The token's largest logit is m = max a, and its sum s that of
 // b e^(a - m): part p goes to strand p mod 64, in ascending order from +0, and the strands are added as a
 // balanced tree whose first level adds l and l + 32, the next l and l + 16, and so on.
 constexpr int PART = 64;

@@ -156,3 +156,16 @@ def test_many_tokens_of_the_same_words(n, words):
     x, w, t = case(n, 5, 700, seed=n, words=words, ignored=range(3, n, 11))
     t[5::97], t[7::101] = 700, -3
     assert_same(results(x.cuda(), w.cuda(), t.cuda()), results(x, w, t))
+
+
+@pytest.mark.parametrize("below,above", [(0, 64), (64, 0), (54, 300), (4096, 0), (0, 270000)])
+@pytest.mark.parametrize("n", [1, 40, 70])
+def test_parts_whose_logits_are_all_minus_infinity(n, below, above):
+    from test_loss import words_past_the_range
+
+    x, w, t, _ = words_past_the_range(n, below, above)
+    got = results(x.cuda(), w.cuda(), t.cuda())
+    assert torch.isfinite(got[0]) and torch.isfinite(got[2]).all()
+    assert_same(got, results(x, w, t))
+    for t in (torch.zeros_like(t), t):
+        assert_same(results(x.cuda(), -w.cuda(), t.cuda()), results(x, -w, t))

@@ -309,3 +309,42 @@ def test_backward_passes_of_several_threads():
     for th in threads:
         th.join()
     assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+
+
+def words_past_the_range(n, below, above):
+    """One value a row, so every finite logit is exact: `below` words whose logits are -infinity (products below
+    float32's range), ten of -1 to 1.25, and `above` more of -infinity. (x, w, t, the first finite word)"""
+    c = torch.arange(10) / 4.0 - 1.0
+    lost = torch.tensor([-2.0 ** 70])
+    w = torch.cat([lost.expand(below), c * 2.0 ** -70, lost.expand(above)])[:, None].contiguous()
+    x = torch.full((n, 1), 2.0 ** 70)
+    return x, w, below + torch.arange(n) % 10, below
+
+
+@pytest.mark.parametrize("below,above", [(0, 64), (63, 0), (64, 0), (64, 64), (128, 5), (54, 300), (4096, 0)])
+@pytest.mark.parametrize("n", [1, 3])
+def test_parts_whose_logits_are_all_minus_infinity(n, below, above):
+    """They have no share: the softmax is that of the ten words. Exponentials, sums and the quotient: 24 and 6
+    roundings relative to a probability, as in bounds(); a word's row of dz is rounded at half a step of its largest value."""
+    x, w, t, first = words_past_the_range(n, below, above)
+    rows, _, dw = results(x, w, t, "none")
+    z = torch.arange(10, dtype=torch.float64) / 4 - 1
+    lse = torch.logsumexp(z, 0)
+    want = lse - z[t - first]
+    assert torch.all((rows.double() - want).abs() <= 24 * EPS32 + 2 * EPS32 * want)
+    p = torch.exp(z - lse)
+    counts = torch.bincount(t - first, minlength=10)
+    want = (p * n - counts) * 2.0 ** 70
+    got = dw[first:first + 10, 0].double()
+    assert torch.all((got - want).abs() <= 2.0 ** 70 * (n * p * (40 * EPS32 + step(1.0, 3)) + 8 * EPS32 * counts))
+    assert not dw[:first].any() and not dw[first + 10:].any()
+
+
+def test_targets_and_rows_of_minus_infinity():
+    x, w, t, first = words_past_the_range(2, 64, 3)
+    rows, dx, dw = results(x, w, torch.tensor([0, first]), "none")  # a target of probability 0, and an ordinary one
+    assert rows[0] == math.inf and torch.isfinite(rows[1]) and torch.isfinite(dw).all() and torch.isfinite(dx).all()
+    rows, dx, dw = results(x, w[:64], torch.tensor([0, 1]), "none")  # no word has a probability
+    assert rows.isnan().all() and dx.isnan().all() and dw[:2].isnan().all()
+    rows, _, _ = results(x, -w, torch.tensor([first, 0]), "none")  # +infinity
+    assert rows.isnan().all()

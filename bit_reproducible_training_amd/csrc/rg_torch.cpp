@@ -754,6 +754,21 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     }
 };
 
+// Whether the gate's leading sizes, without 1s at their end, are x's first ones (1s of x that the gate has not are passed
+// over), so that every row has a place among the gate's; or x is rows without further structure, which
+// the gate takes in runs. Other gates would be read one way by their count and another by broadcasting.
+bool gate_lines_up(const Tensor& gate, const Tensor& x) {
+    const auto g = gate.sizes(), s = x.sizes();
+    size_t n = g.size() - 1, at = 0;
+    while (n > 0 && g[n - 1] == 1) --n;
+    if (s.size() == 2 && n <= 1) return true;
+    for (size_t i = 0; i < n; ++i, ++at) {
+        while (at + 1 < s.size() && s[at] == 1 && g[i] != 1) ++at;
+        if (at + 1 >= s.size() || s[at] != g[i]) return false;
+    }
+    return true;
+}
+
 // (y) or (r, y), differentiable; x and f of any leading dimensions.
 variable_list norm_apply(const Tensor& x, const OptTensor& f, const OptTensor& gate, const OptTensor& post_weight,
                          const OptTensor& post_bias, const OptTensor& weight, const OptTensor& bias, bool rms, bool post,
@@ -762,6 +777,7 @@ variable_list norm_apply(const Tensor& x, const OptTensor& f, const OptTensor& g
     need(!f.has_value() || f->sizes() == x.sizes(), "norm: f must have x's shape");
     const int64_t d = x.size(-1);
     need(!gate.has_value() || (gate->dim() >= 1 && gate->size(-1) == d), "norm: the gate's last dimension must be x's");
+    need(!gate.has_value() || gate_lines_up(*gate, x), "norm: the gate's leading sizes must be x's first ones");
     const std::pair<const OptTensor*, const char*> vectors[] = {
         {&weight, "weight"}, {&bias, "bias"}, {&post_weight, "post_weight"}, {&post_bias, "post_bias"}};
     for (const auto& v : vectors)

@@ -46,9 +46,10 @@ def residual_norm(x, f, weight=None, bias=None, *, kind="layer", eps=1e-5, gate=
                   post_weight=None, post_bias=None):
     """(r, y): r = x + scale * gate * u and y = Norm(r) * weight + bias, where u is f, or with
     post_norm Norm(f) * post_weight + post_bias. x and f are float32 [..., D] of one shape; weights
-    and biases [D], or None. gate is None or [..., D] with G leading elements, G a divisor of x's
-    rows (its leading elements): each run of rows / G rows takes one of its rows. So [D] gates channels,
-    [batch, D] gates each sequence of an x of [batch, tokens, D], and x's shape each value. Gradients
+    and biases [D], or None. gate is None or [..., D] whose leading sizes are the first of x's leading sizes (1s at
+    their end do not count): [D] gates channels, [batch, D] or [batch, 1, D] each sequence of an x of
+    [batch, tokens, D], and x's shape each value. For an x of [rows, D] it may be [G, D], G a divisor of
+    rows, and each run of rows / G rows takes one of its rows. Other gates are refused. Gradients
     reach every tensor; r and y may be used or not."""
     r, y = _apply(x, f, weight, bias, kind, eps, gate, scale, post_norm, post_weight, post_bias)
     return r, y

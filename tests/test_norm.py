@@ -296,3 +296,31 @@ def test_gradients_are_differentiable_no_further():
     (dx,) = torch.autograd.grad((r, y), [x], up, create_graph=True)
     with pytest.raises(RuntimeError, match="only once"):
         dx.sum().backward()
+
+
+def test_gates_that_line_up_with_rows():
+    """The gate's leading sizes, 1s at their end left out, are x's first ones (x's own 1s aside): the value of a row
+    is that of its place among them."""
+    x, f = torch.randn(2, 3, 4, 5), torch.randn(2, 3, 4, 5)
+    for lead in ((), (1,), (1, 1, 1), (2,), (2, 1), (2, 1, 1), (2, 3), (2, 3, 1), (2, 3, 4)):
+        gate = torch.randn(*lead, 5)
+        full = gate.reshape(*lead, *(1,) * (3 - len(lead)), 5).expand(2, 3, 4, 5)
+        assert torch.equal(rg.residual_norm(x, f, gate=gate)[0], x + full * f), lead
+    one = torch.randn(4, 5)
+    assert torch.equal(rg.residual_norm(x[:1, :1], f[:1, :1], gate=one)[0], x[:1, :1] + one * f[:1, :1])
+    rows = torch.randn(2, 5)  # rows without further structure, in runs
+    assert torch.equal(rg.residual_norm(x.view(24, 5), f.view(24, 5), gate=rows)[0],
+                       x.view(24, 5) + rows.repeat_interleave(12, 0) * f.view(24, 5))
+
+
+@pytest.mark.parametrize("lead", [(4,), (1, 4), (1, 3), (3,), (3, 4), (1, 3, 4), (2, 4), (2, 1, 4), (4, 3, 2), (6,), (24,),
+                                  (2, 3, 4, 2), (12, 2)])
+def test_gates_that_do_not_line_up_are_refused(lead):
+    """Broadcasting or counts would read these in ways that differ."""
+    x = torch.zeros(2, 3, 4, 5)
+    with pytest.raises(ValueError, match="gate"):
+        rg.residual_norm(x, x, gate=torch.ones(*lead, 5))
+    with pytest.raises(ValueError, match="gate"):
+        rg.ResidualNorm(5)(x, x, torch.ones(*lead, 5))
+    with pytest.raises(ValueError, match="gate"):
+        rg.residual_norm(x.view(24, 5), x.view(24, 5), gate=torch.ones(2, 4, 5))

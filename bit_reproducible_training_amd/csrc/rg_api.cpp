@@ -480,6 +480,7 @@ static SliceDesc make_slice_desc(const float* src, int R, int K, int Rp, int Kp,
     d.im2col = 0;
     std::memset(&d.g, 0, sizeof d.g);
     d.nanrows = nullptr;
+    d.k_factors = nullptr;
     slice_grid(d);
     d.spin_limit = slice_spin_limit();
     pslice_grid(d);
@@ -513,8 +514,10 @@ int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, const float* 
 }
 
 int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
-                 hipStream_t stream) {
-    const SliceDesc d = slice_alone(src, R, K, strided, out, expo, scratch);
+                 hipStream_t stream, const float* k_factors) {
+    SliceDesc d = slice_alone(src, R, K, strided, out, expo, scratch);
+    if (k_factors && !(strided && onepass_eligible(d))) return hipErrorInvalidValue;
+    d.k_factors = k_factors;
     SliceDesc none = d;
     none.max_blocks = 0;
     none.split_blocks = 0;

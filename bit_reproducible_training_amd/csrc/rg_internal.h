@@ -251,6 +251,9 @@ struct SliceDesc {
     // exponent 0, the exponent of a maximum that a NaN wins (the convolution's window and
     // position maxima; the maxima computed here skip NaN).
     const unsigned* nanrows;
+    // Null, or a factor for each k, four floats apart: the values of a k whose factor is 0 count as 0 (the one
+    // pass on a column-access operand of one item; the vocabulary loss's tokens that have no share).
+    const float* k_factors;
 };
 
 // Bit pattern of a partial-maximum slot not yet written by this call (a NaN; no maximum of
@@ -387,10 +390,10 @@ int gemm_launch(const float* A, const float* B, float* C, const Layout& L, char*
 
 // One operand's slicing by itself, for callers that keep its digits for several products: op(X) of R
 // rows of K values (row access, or column access with rows R apart) into panels of round_up(R, 64) by
-// round_up(K, 64) at `out` and exponents at `expo`; scratch of slice_scratch_bytes.
+// round_up(K, 64) at `out` and exponents at `expo`; scratch of slice_scratch_bytes. k_factors as in SliceDesc.
 size_t slice_scratch_bytes(int R, int K, bool strided);
 int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
-                 hipStream_t stream);
+                 hipStream_t stream, const float* k_factors = nullptr);
 // Two row-access operands of one K, in one launch where one pass takes them.
 int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, const float* b, int Rb, int8_t* qb, int* eb, int K, int S,
                       float* scratch, hipStream_t stream);

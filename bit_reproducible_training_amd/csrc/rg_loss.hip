@@ -864,6 +864,8 @@ void launch_digits_s(int V, int rows, hipStream_t st, const float* z, int ldz, i
     hipLaunchKernelGGL(kernel, grid, block, 0, st, z, ldz, V, first, rows, tokens, words, exponents, out);
 }
 static_assert(repro_loss::MAX_GROUP <= 4 * STEP_TOKENS, "a block holds a group's tokens");
+static_assert(repro_loss::MAX_GROUP <= ONEPASS_MAX_K_COLUMNS && sizeof(Token) == 4 * sizeof(float),
+              "a group's tokens are sliced in one pass, which reads their factors");
 
 }  // namespace
 }  // namespace rg
@@ -975,7 +977,8 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
             launch_product(s.dx[k], panels(s.by_token), exponents(s.by_token), panels(s.w_cols), exponents(s.w_cols),
                            dx + (size_t)first * D, D, false, partial, st);
         if (dw) {
-            rc = launch_slice(x + (size_t)first * D, D, rows, true, S, panels(s.x_cols), exponents(s.x_cols), scratch, st);
+            rc = launch_slice(x + (size_t)first * D, D, rows, true, S, panels(s.x_cols), exponents(s.x_cols), scratch, st,
+                              &tokens[first].factor);
             if (rc != hipSuccess) return rc;
             launch_product(s.dw[k], panels(s.by_word), exponents(s.by_word), panels(s.x_cols), exponents(s.x_cols),
                            dw, D, first > 0, partial, st);

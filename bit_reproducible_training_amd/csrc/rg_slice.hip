@@ -675,6 +675,15 @@ __device__ __forceinline__ void slice_onepass(const SliceDesc& d, long long blk)
             }
             v[i] = make_float4(x[0], x[1], x[2], x[3]);
         }
+        if (G && d.k_factors != nullptr) {
+            const auto kept = [&](float value, int i, int j) {
+                const int k = (kp0 + i) * PANEL_K + 8 * j + (lane >> 3);
+                return k < d.K && d.k_factors[4 * (size_t)k] != 0.0f ? value : 0.0f;
+            };
+#pragma unroll
+            for (int i = 0; i < NF4; ++i)
+                v[i] = make_float4(kept(v[i].x, i, 0), kept(v[i].y, i, 1), kept(v[i].z, i, 2), kept(v[i].w, i, 3));
+        }
 #pragma unroll
         for (int i = 0; i < NF4; ++i) m = fmaxf(m, max4(v[i]));
 #pragma unroll
@@ -691,6 +700,13 @@ __device__ __forceinline__ void slice_onepass(const SliceDesc& d, long long blk)
             if (k < d.K && c < d.R) {
                 const float* q = base + (size_t)k * d.ld + c;
                 v[i] = *reinterpret_cast<const float4*>(q);
+            }
+        }
+        if (G && d.k_factors != nullptr) {
+#pragma unroll
+            for (int i = 0; i < NF4; ++i) {
+                const int k = (kp0 + i) * PANEL_K + (lane >> 1);
+                if (!(k < d.K && d.k_factors[4 * (size_t)k] != 0.0f)) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
         }
 #pragma unroll
@@ -835,9 +851,9 @@ bool onepass_eligible(const SliceDesc& d) {
 void launch_onepass(const SliceDesc& a, bool use_a, const SliceDesc& b, bool use_b, int S,
                     hipStream_t stream) {
     const int kp = use_a ? a.Kp : b.Kp;
-    // Gathering (implicit im2col) instantiations only when an operand gathers, so the plain
+    // Gathering (implicit im2col) or leaving out values of k: instantiations of their own, so the plain
     // GEMM's kernels carry none of that code.
-    const bool gather = (use_a && a.im2col) || (use_b && b.im2col);
+    const bool gather = (use_a && (a.im2col || a.k_factors)) || (use_b && (b.im2col || b.k_factors));
     if (kp <= 256) {  // wave strips: 8 strips per block
         const long long na = use_a ? ((long long)a.batch * (a.Rp / 8) + 7) / 8 : 0;
         const long long nb = use_b ? ((long long)b.batch * (b.Rp / 8) + 7) / 8 : 0;

@@ -57,7 +57,7 @@ inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, co
     for (int64_t n = 0; n < N; ++n) count += target[n] != c.ignore_index;
     const float weight = c.reduction == RG_LOSS_MEAN ? 1.0f / (float)count : 1.0f;
     std::vector<Token> tokens(N);
-    std::vector<float> z, part;
+    std::vector<float> z, part, counted;
     const int64_t group = group_tokens(V);
     if (dw) std::fill(dw, dw + (size_t)V * D, 0.0f);
     for (int64_t first = 0; first < N; first += group) {
@@ -94,7 +94,10 @@ inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, co
         }
         if (dw) {
             float* out = first == 0 ? dw : (part.resize((size_t)V * D), part.data());
-            repro_gemm::cpu_gemm(z.data(), xg, out, V, D, rows, true, false, c.slices);
+            counted.assign(xg, xg + (size_t)rows * D);
+            for (int r = 0; r < rows; ++r)
+                if (tokens[first + r].factor == 0.0f) std::fill_n(counted.begin() + (size_t)r * D, D, 0.0f);
+            repro_gemm::cpu_gemm(z.data(), counted.data(), out, V, D, rows, true, false, c.slices);
             if (first > 0)
                 for (size_t i = 0; i < (size_t)V * D; ++i) dw[i] = dw[i] + part[i];
         }

@@ -77,7 +77,9 @@ inline int group_tokens(long long V) {
     return r;
 }
 
-// One token: what its logits' gradient is made of. `weight` is the loss's factor.
+// One token: what its logits' gradient is made of. `weight` is the loss's factor. Where `factor` is 0, so is the
+// token's row of dz, and its row of x counts as zeros in the product for dw: what it holds (padding may hold
+// anything) does not set the scale that the other tokens' values are rounded at.
 struct Token {
     float top, factor;  // dz_v = e^(z_v - top) * factor for the words that are not the target
     float target;       // dz of the target word: weight * (its probability - 1)

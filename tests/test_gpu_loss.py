@@ -169,3 +169,20 @@ def test_parts_whose_logits_are_all_minus_infinity(n, below, above):
     assert_same(got, results(x, w, t))
     for t in (torch.zeros_like(t), t):
         assert_same(results(x.cuda(), -w.cuda(), t.cuda()), results(x, -w, t))
+
+
+@pytest.mark.parametrize("n", [7, 300, 2100])
+@pytest.mark.parametrize("d", [33, 36])
+def test_hidden_states_of_tokens_that_do_not_count_reach_nothing(n, d):
+    """Padding between and after the tokens, in one group and in two."""
+    x, w, t = case(n, d, 90, seed=n, lean=2.0)
+    keep = torch.rand(n, generator=torch.Generator().manual_seed(3)) < 0.7
+    keep[0], keep[-1] = True, False
+    t[~keep] = -100
+    for large in (1e12, math.inf, math.nan):
+        x[~keep, 1::2] = large
+        got = results(x.cuda(), w.cuda(), t.cuda())
+        assert_same(got, results(x, w, t))
+        if n < 2048:
+            part = results(x[keep].cuda(), w.cuda(), t[keep].cuda())
+            assert torch.equal(got[2], part[2]) and torch.equal(got[1][keep.cuda()], part[1])

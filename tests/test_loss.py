@@ -348,3 +348,26 @@ def test_targets_and_rows_of_minus_infinity():
     assert rows.isnan().all() and dx.isnan().all() and dw[:2].isnan().all()
     rows, _, _ = results(x, -w, torch.tensor([first, 0]), "none")  # +infinity
     assert rows.isnan().all()
+
+
+@pytest.mark.parametrize("large", [1e12, -3e38, math.inf, math.nan])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_hidden_states_of_tokens_that_do_not_count_reach_nothing(large, reduction):
+    """Padding may hold anything: of tokens that are left out, whose target is no word, or whose finite loss has a factor
+    of 0, nothing reaches the others' gradients. Without them the results are the same bits."""
+    x, w, t = case(30, 12, 50, seed=11, lean=2.0)
+    up = torch.randn(30, generator=torch.Generator().manual_seed(2))
+    keep = torch.ones(30, dtype=torch.bool)
+    keep[[0, 7, 8, 29]] = False
+    part = results(x[keep], w, t[keep], reduction, up[keep] if reduction == "none" else None)
+    t[~keep] = -100
+    if reduction == "none":
+        t[7] = 50
+        if large == 1e12:
+            t[8], up[8] = 3, 0.0
+    x[~keep, ::2] = large
+    got = results(x, w, t, reduction, up if reduction == "none" else None)
+    assert torch.equal(got[2], part[2]) and torch.equal(got[1][keep], part[1])
+    if math.isfinite(large):
+        assert not got[1][~keep].any()
+    assert torch.equal(got[0], part[0]) if reduction == "mean" else torch.equal(got[0][keep], part[0])

@@ -481,6 +481,8 @@ static SliceDesc make_slice_desc(const float* src, int R, int K, int Rp, int Kp,
     std::memset(&d.g, 0, sizeof d.g);
     d.nanrows = nullptr;
     d.k_factors = nullptr;
+    d.nonfinite = nullptr;
+    d.nonfinite_step = 0;
     slice_grid(d);
     d.spin_limit = slice_spin_limit();
     pslice_grid(d);
@@ -502,14 +504,19 @@ static SliceDesc slice_alone(const float* src, int R, int K, bool strided, int8_
                            scratch, out, expo);
 }
 
-int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, const float* b, int Rb, int8_t* qb, int* eb, int K, int S,
-                      float* scratch, hipStream_t stream) {
-    const SliceDesc da = slice_alone(a, Ra, K, false, qa, ea, scratch), db = slice_alone(b, Rb, K, false, qb, eb, scratch);
+int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, int* nonfinite_a, const float* b, int Rb, int8_t* qb,
+                      int* eb, int* nonfinite_b, int K, int S, float* scratch, hipStream_t stream) {
+    SliceDesc da = slice_alone(a, Ra, K, false, qa, ea, scratch), db = da;
+    if (b) db = slice_alone(b, Rb, K, false, qb, eb, scratch);
     if (!onepass_eligible(da)) {
+        launch_mark_nonfinite(a, Ra, nonfinite_a, b, b ? Rb : 0, nonfinite_b, K, stream);
         const int rc = launch_slice(a, Ra, K, false, S, qa, ea, scratch, stream);
-        return rc != hipSuccess ? rc : launch_slice(b, Rb, K, false, S, qb, eb, scratch, stream);
+        return rc != hipSuccess || !b ? rc : launch_slice(b, Rb, K, false, S, qb, eb, scratch, stream);
     }
-    launch_onepass(da, true, db, true, S, stream);
+    da.nonfinite = nonfinite_a;
+    da.nonfinite_step = 1;
+    db.nonfinite = nonfinite_b;
+    launch_onepass(da, true, db, b != nullptr, S, stream);
     return hipGetLastError();
 }
 

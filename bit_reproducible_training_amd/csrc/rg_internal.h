@@ -254,6 +254,10 @@ struct SliceDesc {
     // Null, or a factor for each k, four floats apart: the values of a k whose factor is 0 count as 0 (the one
     // pass on a column-access operand of one item; the vocabulary loss's tokens that have no share).
     const float* k_factors;
+    // Null, or where rows that hold a NaN or an infinity are marked (the one pass on a row-access operand of one
+    // item): 1 at nonfinite[row * nonfinite_step], nothing elsewhere.
+    int* nonfinite;
+    int nonfinite_step;
 };
 
 // Bit pattern of a partial-maximum slot not yet written by this call (a NaN; no maximum of
@@ -394,9 +398,13 @@ int gemm_launch(const float* A, const float* B, float* C, const Layout& L, char*
 size_t slice_scratch_bytes(int R, int K, bool strided);
 int launch_slice(const float* src, int R, int K, bool strided, int S, int8_t* out, int* expo, float* scratch,
                  hipStream_t stream, const float* k_factors = nullptr);
-// Two row-access operands of one K, in one launch where one pass takes them.
-int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, const float* b, int Rb, int8_t* qb, int* eb, int K, int S,
-                      float* scratch, hipStream_t stream);
+// Two row-access operands of one K (b may be null), in one launch where one pass takes them. nonfinite_a[r] is set to 1
+// for the rows of a that hold a NaN or an infinity, nonfinite_b[0] where b holds one; nothing else is written there.
+int launch_slice_rows(const float* a, int Ra, int8_t* qa, int* ea, int* nonfinite_a, const float* b, int Rb, int8_t* qb,
+                      int* eb, int* nonfinite_b, int K, int S, float* scratch, hipStream_t stream);
+// The marks by themselves: rows of K values, K apart.
+void launch_mark_nonfinite(const float* a, int Ra, int* nonfinite_a, const float* b, int Rb, int* nonfinite_b, int K,
+                           hipStream_t stream);
 
 // Kernel launchers (asynchronous on `stream`).
 void launch_absmax(const SliceDesc& a, const SliceDesc& b, hipStream_t stream);

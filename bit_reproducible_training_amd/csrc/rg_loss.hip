@@ -43,6 +43,8 @@ struct Targets {
     int* count;    // [V]
     int* place;    // [V] (of words that occur)
     int* counted;  // [1] tokens that are not left out
+    int* broken;   // [N] 1 where the token's row of x holds a NaN or an infinity (cleared with the rest, set by the slicing)
+    int* broken_weight;  // [1] 1 where the weight does
 };
 
 // The words' counts by atomics, then places for their tokens. A word's place and its tokens' order in
@@ -93,14 +95,20 @@ loss_words(const long long* __restrict__ target, long long ignore_index, int N, 
         for (int i = 0; i < BATCH; ++i) {
             const int n = base + i * threads;
             if (n >= N) break;
-            if (self == 0) t.word[n] = w[i];
+            if (self == 0) {
+                t.word[n] = w[i];
+                t.broken[n] = 0;
+            }
             if (slot[i] >= 0) t.slot[n] = slot[i];
         }
     }
     if (count > 0) atomicAdd(&kept, count);
     if (before > 0) atomicAdd(&places, before);
     phase_end();
-    if (self == 0 && threadIdx.x == 0) t.counted[0] = kept;
+    if (self == 0 && threadIdx.x == 0) {
+        t.counted[0] = kept;
+        t.broken_weight[0] = 0;
+    }
     for (int pass = 0; pass < 2; ++pass) {  // places for the block's words, then its tokens there
         for (int base = threadIdx.x; base < N; base += threads * BATCH) {
             int w[BATCH], slot[BATCH], at[BATCH];
@@ -167,10 +175,16 @@ loss_ranks(const long long* __restrict__ target, long long ignore_index, int N, 
     if (counts) {
         if (count > 0) atomicAdd(&kept, count);
         __syncthreads();
-        if (threadIdx.x == 0) t.counted[0] = kept;
+        if (threadIdx.x == 0) {
+            t.counted[0] = kept;
+            t.broken_weight[0] = 0;
+        }
     }
     if (n >= N) return;
-    if (l == 0) t.word[n] = word;
+    if (l == 0) {
+        t.word[n] = word;
+        t.broken[n] = 0;
+    }
     if (!lists) return;
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) {
@@ -228,7 +242,7 @@ static_assert(STEP_K % FEW_K == 0, "tokens' digits come in whole pieces");
 template <int S, int PW, int TILES>
 __global__ void __launch_bounds__(64 * FEW_WAVES, PW <= 3 ? 4 : PW <= 4 ? 3 : 2)
 loss_few(const float* __restrict__ w, int V, int D, int pieces, const int8_t* __restrict__ qx, const int* __restrict__ ex,
-         int N, float* __restrict__ z, int ldz) {
+         int N, float* __restrict__ z, int ldz, int* __restrict__ broken_weight) {
     constexpr int L = 2 * S - 1;
     __shared__ int64_t sums[FEW_WAVES][4 * TILES][64];
     __shared__ uint32_t tops[FEW_WAVES][16];
@@ -255,7 +269,9 @@ loss_few(const float* __restrict__ w, int V, int D, int pieces, const int8_t* __
 #pragma unroll
     for (int p = 0; p < PW; ++p)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) top = max(top, repro_gemm::magnitude_key(f[p][j]));
+        for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(f[p][j]) & 0x7FFFFFFFu);
+    // (A NaN or an infinity breaks every token: what its word's logits are does not matter.)
+    if (top >= 0x7F800000u) broken_weight[0] = 1;
     top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
     if (lane < 16) tops[wave][lane] = top;
@@ -314,20 +330,22 @@ loss_few(const float* __restrict__ w, int V, int D, int pieces, const int8_t* __
 }
 
 template <int S, int TILES>
-void launch_few_tiles(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, hipStream_t st) {
+void launch_few_tiles(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, int* broken_weight,
+                      hipStream_t st) {
     const int pieces = (D + STEP_K - 1) / STEP_K * (STEP_K / FEW_K);  // as the slicing pads
     const int each = ((D + FEW_K - 1) / FEW_K + FEW_WAVES - 1) / FEW_WAVES;
     decltype(&loss_few<S, 1, TILES>) kernels[] = {loss_few<S, 1, TILES>, loss_few<S, 2, TILES>, loss_few<S, 3, TILES>,
                                                   loss_few<S, 4, TILES>, loss_few<S, 5, TILES>, loss_few<S, 6, TILES>,
                                                   loss_few<S, 7, TILES>, loss_few<S, 8, TILES>};
     hipLaunchKernelGGL(kernels[each - 1], dim3((V + FEW_WORDS_EACH - 1) / FEW_WORDS_EACH), dim3(64 * FEW_WAVES), 0, st, w, V, D, pieces, qx,
-                       ex, N, z, ldz);
+                       ex, N, z, ldz, broken_weight);
 }
 template <int S>
-void launch_few_s(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, hipStream_t st) {
-    if (N <= 16) launch_few_tiles<S, 1>(w, V, D, qx, ex, N, z, ldz, st);
-    else if (N <= 32) launch_few_tiles<S, 2>(w, V, D, qx, ex, N, z, ldz, st);
-    else launch_few_tiles<S, 4>(w, V, D, qx, ex, N, z, ldz, st);
+void launch_few_s(const float* w, int V, int D, const int8_t* qx, const int* ex, int N, float* z, int ldz, int* broken_weight,
+                  hipStream_t st) {
+    if (N <= 16) launch_few_tiles<S, 1>(w, V, D, qx, ex, N, z, ldz, broken_weight, st);
+    else if (N <= 32) launch_few_tiles<S, 2>(w, V, D, qx, ex, N, z, ldz, broken_weight, st);
+    else launch_few_tiles<S, 4>(w, V, D, qx, ex, N, z, ldz, broken_weight, st);
 }
 
 __device__ __forceinline__ float wave_fmax(float m) {
@@ -424,7 +442,8 @@ loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __rest
     for (int p = lane; p < parts; p += 64) s = s + kept[p].y * exp_nonpositive(kept[p].x - m);
     s = wave_sum(s);
     const float g = factors ? factors[n] : mean ? 1.0f / (float)t.counted[0] : 1.0f;
-    const Token k = repro_loss::finish_token(m, s, target_logit, g);
+    const bool broken = t.broken[n] != 0 || t.broken_weight[0] != 0;
+    const Token k = broken ? repro_loss::broken_token() : repro_loss::finish_token(m, s, target_logit, g);
     if (arrived) {
         const int place = t.place[word], count = t.count[word];
         int before = 0;
@@ -438,7 +457,8 @@ loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __rest
     }
     if (lane == 0) {
         tokens[n] = k;
-        exponents[r] = repro_gemm::scale_exponent(fabsf(exp_nonpositive(other - k.top) * k.factor));  // 0 for a NaN
+        // 0 for a NaN, and a broken token's row of zeros
+        exponents[r] = broken ? 0 : repro_gemm::scale_exponent(fabsf(exp_nonpositive(other - k.top) * k.factor));
     }
 }
 
@@ -825,7 +845,7 @@ int plan_space(const rg_loss_config* c, bool dx, bool dw, Space* s) {
         for (const Layout* L : {s->few ? nullptr : &s->z[k], dx ? &s->dx[k] : nullptr, dw ? &s->dw[k] : nullptr})
             if (L && L->has_partial) partial = std::max(partial, (size_t)L->split * L->M * L->N * sizeof(int64_t));
     }
-    s->words = take(((size_t)6 * N + 2 * (size_t)round_up(V, 32) + 1) * sizeof(int));
+    s->words = take(((size_t)7 * N + 2 * (size_t)round_up(V, 32) + 2) * sizeof(int));
     s->tokens = take((size_t)N * sizeof(Token));
     s->part = take(s->parts <= LDS_PARTS ? 0 : (size_t)s->group * s->parts * sizeof(float2));
     s->logits = take((size_t)s->group * s->ldz * sizeof(float));
@@ -929,6 +949,8 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     t.arrived = t.slot + N;
     t.list = t.arrived + N;
     t.counted = t.list + N;
+    t.broken_weight = t.counted + 1;
+    t.broken = t.broken_weight + 1;
     Token* tokens = reinterpret_cast<Token*>(base + s.tokens);
     float2* part = reinterpret_cast<float2*>(base + s.part);
     float* z = reinterpret_cast<float*>(base + s.logits);
@@ -942,18 +964,15 @@ int rg_linear_cross_entropy(const rg_loss_config* cfg, const float* x, const flo
     else
         hipLaunchKernelGGL(loss_words, dim3(16), dim3(1024), 0, st, target, cfg->ignore_index, N, V, t);
     // The digits that every group's products share.
-    if (s.few)
-        rc = launch_slice(x, N, D, false, S, panels(s.x_rows), exponents(s.x_rows), scratch, st);
-    else
-        rc = launch_slice_rows(x, N, panels(s.x_rows), exponents(s.x_rows), w, V, panels(s.w_rows), exponents(s.w_rows), D, S,
-                               scratch, st);
+    rc = launch_slice_rows(x, N, panels(s.x_rows), exponents(s.x_rows), t.broken, s.few ? nullptr : w, V, panels(s.w_rows),
+                           exponents(s.w_rows), t.broken_weight, D, S, scratch, st);
     if (rc == hipSuccess && dx) rc = launch_slice(w, D, V, true, S, panels(s.w_cols), exponents(s.w_cols), scratch, st);
     if (rc != hipSuccess) return rc;
     for (int first = 0; first < N; first += s.group) {
         const int rows = std::min(s.group, N - first), k = first + s.group < N ? 0 : 1;
         if (s.few) {
             auto launch_few = S == 1 ? launch_few_s<1> : S == 2 ? launch_few_s<2> : launch_few_s<3>;
-            launch_few(w, V, D, panels(s.x_rows), exponents(s.x_rows), N, z, s.ldz, st);
+            launch_few(w, V, D, panels(s.x_rows), exponents(s.x_rows), N, z, s.ldz, t.broken_weight, st);
         } else {
             launch_product(s.z[k], panels(s.x_rows) + (size_t)first * round_up(D, STEP_K) * S, exponents(s.x_rows) + first,
                            panels(s.w_rows), exponents(s.w_rows), z, s.ldz, false, partial, st);

@@ -656,6 +656,12 @@ __device__ __forceinline__ void slice_onepass(const SliceDesc& d, long long blk)
                 }
             }
         }
+        if (G && d.nonfinite != nullptr) {
+            unsigned mb = 0;
+#pragma unroll
+            for (int i = 0; i < NF4; ++i) mb = max(mb, max4_bits(v[i]));
+            if (mb >= 0x7F800000u) d.nonfinite[(size_t)row * d.nonfinite_step] = 1;
+        }
 #pragma unroll
         for (int i = 0; i < NF4; ++i) m = fmaxf(m, max4(v[i]));
 #pragma unroll
@@ -851,9 +857,10 @@ bool onepass_eligible(const SliceDesc& d) {
 void launch_onepass(const SliceDesc& a, bool use_a, const SliceDesc& b, bool use_b, int S,
                     hipStream_t stream) {
     const int kp = use_a ? a.Kp : b.Kp;
-    // Gathering (implicit im2col) or leaving out values of k: instantiations of their own, so the plain
-    // GEMM's kernels carry none of that code.
-    const bool gather = (use_a && (a.im2col || a.k_factors)) || (use_b && (b.im2col || b.k_factors));
+    // Gathering (implicit im2col), leaving out values of k or marking rows: instantiations of their own, so the
+    // plain GEMM's kernels carry none of that code.
+    const auto more = [](const SliceDesc& d) { return d.im2col || d.k_factors || d.nonfinite; };
+    const bool gather = (use_a && more(a)) || (use_b && more(b));
     if (kp <= 256) {  // wave strips: 8 strips per block
         const long long na = use_a ? ((long long)a.batch * (a.Rp / 8) + 7) / 8 : 0;
         const long long nb = use_b ? ((long long)b.batch * (b.Rp / 8) + 7) / 8 : 0;
@@ -902,6 +909,36 @@ void launch_onepass(const SliceDesc& a, bool use_a, const SliceDesc& b, bool use
     }
 #undef RG_ONEPASS_S
 #undef RG_ONEPASS
+}
+
+// A row by a block, 16 bytes a load at any multiple of 4. Rows past the one pass only, whose slicing takes two reads or
+// an exchange of maxima: a read of its own, 35 us for 170 MB.
+struct __attribute__((packed, aligned(4))) MarkFour {
+    unsigned v[4];
+};
+__global__ void __launch_bounds__(256)
+mark_nonfinite(const float* __restrict__ a, int Ra, int* __restrict__ nonfinite_a, const float* __restrict__ b, int Rb,
+               int* __restrict__ nonfinite_b, int K) {
+    for (long long r = blockIdx.x; r < (long long)Ra + Rb; r += gridDim.x) {
+        const float* row = r < Ra ? a + (size_t)r * K : b + (size_t)(r - Ra) * K;
+        unsigned mb = 0;
+#pragma unroll 4
+        for (int k = 4 * threadIdx.x; k < K - 3; k += 4 * 256) {
+            const MarkFour q = *reinterpret_cast<const MarkFour*>(row + k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mb = max(mb, q.v[i] & 0x7FFFFFFFu);
+        }
+        const int rest = K / 4 * 4 + threadIdx.x;
+        if (rest < K) mb = max(mb, __float_as_uint(row[rest]) & 0x7FFFFFFFu);
+        if (mb >= 0x7F800000u) *(r < Ra ? nonfinite_a + r : nonfinite_b) = 1;
+    }
+}
+
+void launch_mark_nonfinite(const float* a, int Ra, int* nonfinite_a, const float* b, int Rb, int* nonfinite_b, int K,
+                           hipStream_t stream) {
+    const long long rows = (long long)Ra + Rb;
+    const unsigned blocks = (unsigned)(rows < (1 << 20) ? rows : 1 << 20);
+    mark_nonfinite<<<blocks, 256, 0, stream>>>(a, Ra, nonfinite_a, b, Rb, nonfinite_b, K);
 }
 
 void launch_onepass_absmax(const SliceDesc& one, const SliceDesc& two, int S, hipStream_t stream) {

@@ -26,7 +26,9 @@ def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mea
     """The cross entropy of softmax(x weight^T) against target, for float32 x [..., size], weight
     [words, size] and int64 target [...]; reduction "mean" (over the tokens that count), "sum", or
     "none" (a loss for each token). Tokens whose target is ignore_index are left out; one whose target
-    is no word has a NaN loss and no gradients. slices: the products' S (the layers' by default)."""
+    is no word has a NaN loss and no gradients. A token whose row of x holds a NaN or an infinity, or whose largest
+    logit is infinite, has a NaN loss, a NaN row in x's gradient and makes its target's row of the weight's NaN; where the
+    weight holds one, every token that counts is such. slices: the products' S (the layers' by default)."""
     if reduction not in _REDUCTIONS:
         raise ValueError('reduction must be "mean", "sum" or "none"')
     return _backend.loss_apply(x, weight, target, get_slices() if slices is None else int(slices), _REDUCTIONS[reduction],

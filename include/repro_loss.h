@@ -9,6 +9,9 @@
  * A target equal to ignore_index leaves its token out (loss and gradients 0); another one outside
  * [0, V) gives the token a loss of NaN and no gradients. The losses are reduced to their sum, their
  * mean over the tokens that count (0 of them: NaN), or not; g_n is 1, 1 / count, or the caller's.
+ * A token whose row of x holds a NaN or an infinity, or whose largest logit is one, has a NaN loss, a NaN row of dx, and
+ * makes its target's row of dw NaN; where w holds one, that is so for every token. Nothing that the rows of tokens
+ * that do not count hold reaches loss, dw or the other tokens' dx.
  *
  * The three products are the reproducible GEMM's (S int8 slices); the target word's share of the
  * gradients, g_n (softmax - 1), stays out of dz there, where it would set the scale that the other words'

@@ -47,6 +47,12 @@ inline void largest_and_sum(const float* z, int V, float& m, float& s) {
     s = halves(strand, 64);
 }
 
+inline bool all_finite(const float* v, size_t n) {
+    for (size_t i = 0; i < n; ++i)
+        if (!finite_bits(v[i])) return false;
+    return true;
+}
+
 }  // namespace cpu_detail
 
 inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, const float* w, const int64_t* target,
@@ -56,6 +62,9 @@ inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, co
     int64_t count = 0;
     for (int64_t n = 0; n < N; ++n) count += target[n] != c.ignore_index;
     const float weight = c.reduction == RG_LOSS_MEAN ? 1.0f / (float)count : 1.0f;
+    std::vector<char> finite(V);  // the weight's words
+    repro_gemm::cpu_for(V, [&](int v) { finite[v] = cpu_detail::all_finite(w + (size_t)v * D, D); });
+    const bool finite_weight = std::find(finite.begin(), finite.end(), 0) == finite.end();
     std::vector<Token> tokens(N);
     std::vector<float> z, part, counted;
     const int64_t group = group_tokens(V);
@@ -72,9 +81,13 @@ inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, co
             const float g = factors ? factors[first + r] : weight;
             t = ignored_token();
             if (word >= 0 && word < V && word != c.ignore_index) {
-                float m, s;
-                cpu_detail::largest_and_sum(q, V, m, s);
-                t = finish_token(m, s, q[word], g);
+                if (finite_weight && cpu_detail::all_finite(xg + (size_t)r * D, D)) {
+                    float m, s;
+                    cpu_detail::largest_and_sum(q, V, m, s);
+                    t = finish_token(m, s, q[word], g);
+                } else {
+                    t = broken_token();
+                }
                 for (int v = 0; v < V; ++v) q[v] = dz_of(q[v], t.top, t.factor);
                 q[word] = 0.0f;
             } else {

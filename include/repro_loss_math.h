@@ -86,8 +86,8 @@ struct Token {
     float loss;
 };
 
-// Where a logit or the weight is not finite, the token's row of dz is 0 (factor 0) and its target word's
-// share NaN, so that dx and the target's row of dw are.
+// Where the largest logit or the loss's factor is not finite, the token's row of dz is 0 (factor 0) and its target
+// word's share NaN, so that its row of dx and the target's row of dw are.
 RG_HD inline Token finish_token(float m, float s, float zt, float weight) {
     Token t;
     t.top = m;
@@ -100,6 +100,10 @@ RG_HD inline Token finish_token(float m, float s, float zt, float weight) {
     t.loss = (float)(((double)m - (double)zt) + log_positive(s));
     return t;
 }
+// Of a token whose row of x holds a NaN or an infinity, and of every token where the weight holds one (the products'
+// fixed-point numbers stand for neither, so the logits may look ordinary): the same, and a NaN loss.
+RG_HD inline Token broken_token() { return Token{0.0f, 0.0f, __builtin_nanf(""), __builtin_nanf("")}; }
+RG_HD inline bool finite_bits(float x) { return (repro_gemm::float_to_bits(x) & 0x7F800000u) != 0x7F800000u; }
 // Of a token that is left out: no gradient, no loss.
 RG_HD inline Token ignored_token() { return Token{0.0f, 0.0f, 0.0f, 0.0f}; }
 

@@ -186,3 +186,24 @@ def test_hidden_states_of_tokens_that_do_not_count_reach_nothing(n, d):
         if n < 2048:
             part = results(x[keep].cuda(), w.cuda(), t[keep].cuda())
             assert torch.equal(got[2], part[2]) and torch.equal(got[1][keep.cuda()], part[1])
+
+
+@pytest.mark.parametrize("n,d,v", [(9, 12, 90), (20, 1601, 130), (70, 30, 90), (130, 768, 333), (70, 4100, 80), (66, 4103, 70), (2100, 36, 70)])
+def test_a_nan_or_infinity_gives_the_cpu_bits_everywhere(n, d, v):
+    """In x and in the weight, in a token's and a word's first and last values, on every way to the logits."""
+    for bad in (math.nan, math.inf, -math.inf):
+        for where in ("x", "w", "x last", "w last"):
+            x, w, t = case(n, d, v, seed=n, lean=2.0, ignored=(1,))
+            (x if where[0] == "x" else w)[(-1, -1) if "last" in where else (2, 0)] = bad
+            for reduction in ("mean", "none"):
+                got, want = results(x.cuda(), w.cuda(), t.cuda(), reduction), results(x, w, t, reduction)
+                assert_same(got, want)
+            assert got[0].isnan().sum() == (1 if where[0] == "x" else n - 1)
+
+
+def test_left_out_tokens_may_hold_anything():
+    x, w, t = case(150, 64, 200, seed=2)
+    want = results(x.cuda(), w.cuda(), t.where(torch.arange(150) % 3 > 0, -100).cuda())
+    t[::3] = -100
+    x[::3] = math.nan
+    assert_same(results(x.cuda(), w.cuda(), t.cuda()), [v.cpu() for v in want])

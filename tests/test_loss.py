@@ -371,3 +371,37 @@ def test_hidden_states_of_tokens_that_do_not_count_reach_nothing(large, reductio
     if math.isfinite(large):
         assert not got[1][~keep].any()
     assert torch.equal(got[0], part[0]) if reduction == "mean" else torch.equal(got[0][keep], part[0])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_a_nan_or_infinity_in_x_reaches_its_token(bad, reduction):
+    """Its loss, its row of dx and its target's row of dw are NaN; the other tokens' are those of a call without it."""
+    x, w, t = case(17, 12, 40, seed=12, lean=2.0)
+    t[5] = 39
+    t[t == 39] = 38
+    t[5] = 39  # no other token's target
+    keep = torch.arange(17) != 5
+    up = torch.ones(17)
+    part = results(x[keep], w, t[keep], "none")
+    x[5, 3] = bad
+    loss, dx, dw = results(x, w, t, reduction, up if reduction == "none" else torch.tensor(17.0))
+    assert loss.isnan() if reduction == "mean" else loss[5].isnan() and torch.equal(loss[keep], part[0])
+    assert dx[5].isnan().all() and dw[39].isnan().all()
+    if reduction == "none":
+        assert torch.equal(dx[keep], part[1]) and torch.equal(dw[:39], part[2][:39])
+    else:
+        assert torch.isfinite(dx[keep]).all() and torch.isfinite(dw[:39]).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_nan_or_infinity_in_the_weight_reaches_every_token(bad):
+    x, w, t = case(9, 12, 40, seed=13)
+    t[t == 30] = 3
+    t[4] = -100
+    w[30, 11] = bad  # a word that is no token's target
+    keep = torch.arange(9) != 4
+    rows, dx, dw = results(x, w, t, "none")
+    assert rows[keep].isnan().all() and rows[4] == 0
+    assert dx[keep].isnan().all() and not dx[4].any() and dw[t[keep]].isnan().all()
+    assert results(x, w, t, "sum")[0].isnan()

@@ -598,6 +598,11 @@ rg_norm_config norm_config(const Tensor& x, const OptTensor& gate, bool rms, boo
     return c;
 }
 
+// Lowers a CPU's flag, where there is one.
+void report(const OptTensor& flag, bool bad, int op_id) {
+    if (bad && flag.has_value()) flag->data_ptr<int>()[0] = std::min(flag->data_ptr<int>()[0], op_id);
+}
+
 // x, f [..., D] -> {r (undefined without f), y, stats (undefined unless wanted)}
 std::vector<OptTensor> residual_norm(Tensor x, OptTensor f_, OptTensor gate_, OptTensor post_weight_, OptTensor post_bias_,
                                      OptTensor weight_, OptTensor bias_, bool rms, bool post, double eps, double scale,
@@ -624,9 +629,11 @@ std::vector<OptTensor> residual_norm(Tensor x, OptTensor f_, OptTensor gate_, Op
               "residual norm");
     } else {
         Unlocked unlocked;
+        bool bad = false;
         repro_norm::cpu_residual_norm(c, x.data_ptr<float>(), data_or_null(f), data_or_null(gate), data_or_null(pw),
                                       data_or_null(pb), data_or_null(w), data_or_null(b), out_or_null(r),
-                                      y.data_ptr<float>(), out_or_null(stats));
+                                      y.data_ptr<float>(), out_or_null(stats), &bad);
+        report(flag, bad, op_id);
     }
     const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     return {opt(r), opt(y), opt(stats)};
@@ -679,11 +686,13 @@ std::vector<OptTensor> residual_norm_grad(OptTensor dr_, OptTensor dy_, Tensor r
               "norm gradient");
     } else {
         Unlocked unlocked;
+        bool bad = false;
         repro_norm::cpu_residual_norm_grad(c, data_or_null(dr), data_or_null(dy), r.data_ptr<float>(), data_or_null(f),
                                            data_or_null(gate), data_or_null(pw), data_or_null(pb), data_or_null(w),
                                            stats.data_ptr<float>(), out_or_null(dx), out_or_null(df),
                                            out_or_null(dgate), out_or_null(dpw), out_or_null(dpb),
-                                           out_or_null(kernel_dw), out_or_null(kernel_db));
+                                           out_or_null(kernel_dw), out_or_null(kernel_db), &bad);
+        report(flag, bad, op_id);
     }
     const auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     return {opt(dx), opt(df), opt(dgate), opt(dpw), opt(dpb), opt(dw), opt(db)};

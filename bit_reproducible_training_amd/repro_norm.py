@@ -24,15 +24,11 @@ def _apply(x, f, weight, bias, kind, eps, gate, scale, post_norm, post_weight, p
     if kind not in _KINDS:
         raise ValueError('kind must be "layer" or "rms"')
     cell, input_label, gradient_label = None, 0, 0
-    if name is not None:  # a module's: the guard hears of a NaN or infinity, on a GPU in the norm's own launch
+    if name is not None and (x.is_cuda or x.is_cpu):
+        # a module's: the guard hears of rows whose norm is not finite and of gradients, in the norm's own passes
         watcher = guard()
-        if x.is_cuda:
-            cell = watcher._cell(x.device)
-            input_label, gradient_label = watcher._number(name + " input"), watcher._number(name + " gradient")
-        else:
-            watcher.scan(x, name + " input")
-            if f is not None:
-                watcher.scan(f, name + " input")
+        cell = watcher._cell(x.device)
+        input_label, gradient_label = watcher._number(name + " input"), watcher._number(name + " gradient")
     return _backend.norm_apply(x, f, gate, post_weight, post_bias, weight, bias, _KINDS[kind], bool(post_norm),
                                float(eps), float(scale), cell, input_label, gradient_label)
 

@@ -1,8 +1,10 @@
 #pragma once
 // repro_norm_cpu.h -- the reproducible residual addition with the norms before and after a block on the
 // host CPU (header-only C++17; no GPU needed), bit-identical to rg_residual_norm_fp32 and
-// rg_residual_norm_grad_fp32 (include/repro_norm.h), whose arguments these take. Arguments are not checked
-// (the binding does).
+// rg_residual_norm_grad_fp32 (include/repro_norm.h), whose arguments these take; `bad`, when not null, is set where
+// those lower their flag. Arguments are not checked (the binding does).
+#include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <vector>
 
@@ -62,7 +64,8 @@ inline float total(const float* part, long long P, int D, int i) {
 
 inline void cpu_residual_norm(const rg_norm_config& c, const float* x, const float* f, const float* gate,
                               const float* post_weight, const float* post_bias, const float* weight,
-                              const float* bias, float* r, float* y, float* stats) {
+                              const float* bias, float* r, float* y, float* stats, bool* bad = nullptr) {
+    std::atomic<bool> found{false};
     const int D = c.D;
     const bool layer = !c.rms;
     const long long group = c.gate_rows > 0 ? c.N / c.gate_rows : 1;
@@ -87,6 +90,7 @@ inline void cpu_residual_norm(const rg_norm_config& c, const float* x, const flo
         for (int i = 0; i < D; ++i)
             y[at + i] = affine(centred(v[i], s.mean, layer) * s.rstd, weight, weight ? weight[i] : 0.0f, bias,
                                bias ? bias[i] : 0.0f);
+        if (!(s.rstd > 0.0f)) found.store(true, std::memory_order_relaxed);
         if (stats) {
             stats[4 * (size_t)n] = s.mean;
             stats[4 * (size_t)n + 1] = s.rstd;
@@ -94,13 +98,15 @@ inline void cpu_residual_norm(const rg_norm_config& c, const float* x, const flo
             stats[4 * (size_t)n + 3] = sf.rstd;
         }
     });
+    if (bad && found) *bad = true;
 }
 
 inline void cpu_residual_norm_grad(const rg_norm_config& c, const float* dr, const float* dy, const float* r,
                                    const float* f, const float* gate, const float* post_weight,
                                    const float* post_bias, const float* weight, const float* stats, float* dx,
                                    float* df, float* dgate, float* dpost_weight, float* dpost_bias,
-                                   float* dweight, float* dbias) {
+                                   float* dweight, float* dbias, bool* bad = nullptr) {
+    std::atomic<bool> found{false};
     const int D = c.D;
     const bool layer = !c.rms;
     const Partition pt = partition(c.N, D, c.gate_rows);
@@ -136,6 +142,7 @@ inline void cpu_residual_norm_grad(const rg_norm_config& c, const float* dr, con
                         d = dr ? d + b : b;
                     }
                     if (dx) dx[at + i] = d;
+                    if (!std::isfinite(d)) found.store(true, std::memory_order_relaxed);
                     a[i] = d * c.scale;
                 }
                 if (!f) continue;
@@ -177,6 +184,7 @@ inline void cpu_residual_norm_grad(const rg_norm_config& c, const float* dr, con
             }
         }
     });
+    if (bad && found) *bad = true;
     float* out[] = {dweight, dbias, dpost_weight, dpost_bias};
     for (int q = W; q <= PB; ++q)
         if (out[q])

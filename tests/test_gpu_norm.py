@@ -127,3 +127,28 @@ def test_refuses_tensors_on_two_devices():
                 lambda: rg.residual_norm(x, x, gate=torch.ones(8))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("d", [40, 1100])
+def test_the_guard_hears_the_same_on_both_devices(kind, d):
+    g = torch.Generator().manual_seed(d)
+    for what in range(6):
+        heard = []
+        for device in ("cpu", "cuda"):
+            rg.guard().reset()
+            m = rg.ResidualNorm(d, kind=kind).to(device)
+            m.repro_name = "nine"
+            x, f = torch.randn(9, d, generator=g.manual_seed(what)), torch.randn(9, d, generator=g)
+            up = [torch.randn(9, d, generator=g) for _ in range(2)]
+            if what < 2:
+                (x, f)[what][3, d - 1] = math.inf
+            elif what == 2:
+                x[5] *= 1e25
+            elif what < 5:
+                up[what - 3][8, d - 1] = math.nan
+            x = x.to(device).requires_grad_()
+            torch.autograd.grad(m(x, f.to(device)), x, [u.to(device) for u in up])
+            heard.append(rg.guard().first_offender())
+        rg.guard().reset()
+        assert heard[0] == heard[1] == (None if what == 5 else "nine gradient" if what > 2 else "nine input")

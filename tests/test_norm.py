@@ -324,3 +324,33 @@ def test_gates_that_do_not_line_up_are_refused(lead):
         rg.ResidualNorm(5)(x, x, torch.ones(*lead, 5))
     with pytest.raises(ValueError, match="gate"):
         rg.residual_norm(x.view(24, 5), x.view(24, 5), gate=torch.ones(2, 4, 5))
+
+
+@pytest.mark.parametrize("what", ["gradient", "input", "squares", "gate"])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_the_guard_hears_what_it_hears_on_a_gpu(what, kind):
+    rg.guard().reset()
+    m = rg.ResidualNorm(40, kind=kind)
+    m.repro_name = "eight"
+    x, f, gate = torch.randn(9, 40, requires_grad=True), torch.randn(9, 40), torch.ones(40)
+    up = torch.zeros(9, 40)
+    if what == "gradient":
+        up[4, 39] = math.nan
+    elif what == "input":
+        f[8, 0] = -math.inf
+    elif what == "gate":
+        gate[3] = math.nan
+    else:
+        f[2] = 1e25 * torch.randn(40)  # finite, its squares are not
+    r, y = m(x, f, gate)
+    assert rg.guard().first_offender() == (None if what == "gradient" else "eight input")
+    if what == "gradient":
+        torch.autograd.grad(y, x, up)
+        assert rg.guard().first_offender() == "eight gradient"
+        rg.guard().reset()
+        torch.autograd.grad(m(x, f, gate)[0], x, torch.full((9, 40), math.inf))
+        assert rg.guard().first_offender() == "eight gradient"
+    rg.guard().reset()
+    n = rg.Norm(40, kind=kind)
+    torch.autograd.grad(n(x), n.weight, up.fill_(1.0))
+    rg.guard().check()

@@ -276,7 +276,7 @@ norm_forward(Sizes z, long long group, const float* __restrict__ x, const float*
         v.store(y + at, z.D, t);
         if (t == 0) {
             if (stats != nullptr) *reinterpret_cast<float4*>(stats + 4 * n) = make_float4(s.mean, s.rstd, sf.mean, sf.rstd);
-            if (flag != nullptr && !(s.rstd > 0.0f)) report(flag, op_id);
+            if (flag != nullptr && !(s.rstd > 0.0f && (!POST || sf.rstd > 0.0f))) report(flag, op_id);
         }
     }
 }

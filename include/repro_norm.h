@@ -41,8 +41,8 @@ typedef struct rg_norm_config {
 void rg_norm_config_init(rg_norm_config* cfg);
 
 /* The forward pass. stats: N * 4 floats (mean and 1 / deviation of r, then of f) for the backward pass,
- * or null. r null exactly where f is. flag, when not null, is lowered to op_id if a row's norm is not
- * finite (a NaN or infinity in the row, or squares past float32's range).
+ * or null. r null exactly where f is. flag, when not null, is lowered to op_id if a norm of a row of r (post: or of f)
+ * is not finite (a NaN or infinity in the row, or squares past float32's range).
  * 1 (invalid value): null cfg, x or y; N < 0, D out of range, eps negative or NaN; f and r not null together; a post
  * norm or gate without f, gate_rows not a divisor of N, or gate and gate_rows not given together. */
 int rg_residual_norm_fp32(const rg_norm_config* cfg, const float* x, const float* f, const float* gate,

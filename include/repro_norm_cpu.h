@@ -90,7 +90,7 @@ inline void cpu_residual_norm(const rg_norm_config& c, const float* x, const flo
         for (int i = 0; i < D; ++i)
             y[at + i] = affine(centred(v[i], s.mean, layer) * s.rstd, weight, weight ? weight[i] : 0.0f, bias,
                                bias ? bias[i] : 0.0f);
-        if (!(s.rstd > 0.0f)) found.store(true, std::memory_order_relaxed);
+        if (!(s.rstd > 0.0f && (!c.post || sf.rstd > 0.0f))) found.store(true, std::memory_order_relaxed);
         if (stats) {
             stats[4 * (size_t)n] = s.mean;
             stats[4 * (size_t)n + 1] = s.rstd;

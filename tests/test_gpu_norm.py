@@ -152,3 +152,16 @@ def test_the_guard_hears_the_same_on_both_devices(kind, d):
             heard.append(rg.guard().first_offender())
         rg.guard().reset()
         assert heard[0] == heard[1] == (None if what == 5 else "nine gradient" if what > 2 else "nine input")
+
+
+@pytest.mark.parametrize("d", [40, 1100])
+def test_the_guard_hears_a_block_whose_squares_pass_the_range(d):
+    rg.guard().reset()
+    m = rg.ResidualNorm(d, kind="rms", post_norm=True).cuda()
+    x, f = torch.randn(5, d, device="cuda"), torch.randn(5, d, device="cuda")
+    m(x, f)
+    rg.guard().check()
+    f[3] *= 1e25
+    m(x, f)
+    assert rg.guard().first_offender() == "residual_norm input"
+    rg.guard().reset()

@@ -354,3 +354,18 @@ def test_the_guard_hears_what_it_hears_on_a_gpu(what, kind):
     n = rg.Norm(40, kind=kind)
     torch.autograd.grad(n(x), n.weight, up.fill_(1.0))
     rg.guard().check()
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_the_guard_hears_a_block_whose_squares_pass_the_range(kind):
+    """Normalised first, such an output becomes zeros, and r is an ordinary row."""
+    rg.guard().reset()
+    m = rg.ResidualNorm(40, kind=kind, post_norm=True)
+    x, f = torch.randn(5, 40), torch.randn(5, 40)
+    m(x, f)
+    rg.guard().check()
+    f[3] *= 1e25
+    r, y = m(x, f)
+    assert torch.isfinite(r).all() and torch.isfinite(y).all()
+    assert rg.guard().first_offender() == "residual_norm input"
+    rg.guard().reset()

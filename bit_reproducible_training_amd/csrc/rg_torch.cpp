@@ -878,13 +878,15 @@ void scale(const Tensor& a, const Tensor& b, const Tensor& factor) {
 // for the first backward pass to scale and hand out; a later one, and one without a reduction, computes them.
 struct LossFunction : torch::autograd::Function<LossFunction> {
     static Tensor forward(AutogradContext* ctx, Tensor x, Tensor weight, Tensor target, int64_t S, int64_t reduction,
-                          int64_t ignore_index, bool want_x, bool want_w) {
+                          int64_t ignore_index, OptTensor cell, int64_t label, bool want_x, bool want_w) {
         const bool early = reduction != RG_LOSS_NONE;
         auto out = linear_cross_entropy(x, weight, target, OptTensor(), (int)S, (int)reduction, ignore_index, true,
                                         want_x && early, want_w && early);
         if (want_x || want_w) {
             ctx->save_for_backward({x, weight, target});
             ctx->saved_data["settings"] = std::make_tuple(S, reduction, ignore_index, want_x, want_w);
+            ctx->saved_data["cell"] = cell;
+            ctx->saved_data["label"] = label;
             ctx->saved_data["ready"] = early;
             if (early) {
                 ctx->saved_data["dx"] = out[1];
@@ -900,7 +902,9 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
         const int S = (int)e[0].toInt(), reduction = (int)e[1].toInt();
         const int64_t ignore_index = e[2].toInt();
         const bool want_x = e[3].toBool(), want_w = e[4].toBool();
-        variable_list result(8);
+        variable_list result(10);
+        const auto cell = ctx->saved_data["cell"].toOptional<Tensor>();
+        if (cell.has_value()) scan_finite(grads[0].resolve_neg(), *cell, (int)ctx->saved_data["label"].toInt());
         OptTensor dx, dw;
         if (ctx->saved_data["ready"].toBool()) {
             dx = ctx->saved_data["dx"].toOptional<Tensor>();
@@ -922,10 +926,11 @@ struct LossFunction : torch::autograd::Function<LossFunction> {
     }
 };
 
+// cell and label: where the gradient that arrives reports a NaN or infinity, or nowhere.
 Tensor loss_apply(const Tensor& x, const Tensor& weight, const Tensor& target, int64_t S, int64_t reduction,
-                  int64_t ignore_index) {
+                  int64_t ignore_index, const OptTensor& cell, int64_t label) {
     const bool grad = at::GradMode::is_enabled();
-    return LossFunction::apply(x, weight, target, S, reduction, ignore_index, grad && x.requires_grad(),
+    return LossFunction::apply(x, weight, target, S, reduction, ignore_index, cell, label, grad && x.requires_grad(),
                                grad && weight.requires_grad());
 }
 

@@ -29,10 +29,13 @@ def linear_cross_entropy(x, weight, target, *, ignore_index=-100, reduction="mea
     is no word has a NaN loss and no gradients. A token whose row of x holds a NaN or an infinity, or whose largest
     logit is infinite, has a NaN loss, a NaN row in x's gradient and makes its target's row of the weight's NaN; where the
     weight holds one, every token that counts is such. slices: the products' S (the layers' by default)."""
+    return _apply(x, weight, target, ignore_index, reduction, get_slices() if slices is None else int(slices), None, 0)
+
+
+def _apply(x, weight, target, ignore_index, reduction, slices, cell, gradient_label):
     if reduction not in _REDUCTIONS:
         raise ValueError('reduction must be "mean", "sum" or "none"')
-    return _backend.loss_apply(x, weight, target, get_slices() if slices is None else int(slices), _REDUCTIONS[reduction],
-                               int(ignore_index))
+    return _backend.loss_apply(x, weight, target, slices, _REDUCTIONS[reduction], int(ignore_index), cell, gradient_label)
 
 
 class LinearCrossEntropy(torch.nn.Module):
@@ -51,5 +54,7 @@ class LinearCrossEntropy(torch.nn.Module):
         torch.nn.init.normal_(self.weight, std=0.02)
 
     def forward(self, x, target):
-        _watch_operands(_CallInfo(self.repro_name, get_slices(), guard()), x, self.weight)
-        return linear_cross_entropy(x, self.weight, target, ignore_index=self.ignore_index, reduction=self.reduction)
+        info = _CallInfo(self.repro_name, get_slices(), guard())
+        _watch_operands(info, x, self.weight)
+        return _apply(x, self.weight, target, self.ignore_index, self.reduction, info.slices, info.guard._cell(x.device),
+                      info.guard._number(info.name + " gradient"))

@@ -207,3 +207,19 @@ def test_left_out_tokens_may_hold_anything():
     t[::3] = -100
     x[::3] = math.nan
     assert_same(results(x.cuda(), w.cuda(), t.cuda()), [v.cpu() for v in want])
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_the_guard_hears_a_gradient_that_is_not_finite(reduction):
+    rg.guard().reset()
+    torch.manual_seed(0)
+    m = rg.LinearCrossEntropy(8, 20, reduction=reduction).cuda()
+    x, t = torch.randn(5, 8, device="cuda"), torch.randint(0, 20, (5,), device="cuda")
+    loss = m(x, t)
+    up = torch.ones_like(loss)
+    torch.autograd.grad(loss, m.weight, up, retain_graph=True)
+    rg.guard().check()
+    up.view(-1)[-1] = math.nan
+    torch.autograd.grad(loss, m.weight, up)
+    assert rg.guard().first_offender() == "linear_cross_entropy gradient"
+    rg.guard().reset()

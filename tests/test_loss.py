@@ -405,3 +405,21 @@ def test_a_nan_or_infinity_in_the_weight_reaches_every_token(bad):
     assert rows[keep].isnan().all() and rows[4] == 0
     assert dx[keep].isnan().all() and not dx[4].any() and dw[t[keep]].isnan().all()
     assert results(x, w, t, "sum")[0].isnan()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_the_guard_hears_a_gradient_that_is_not_finite(reduction):
+    rg.guard().reset()
+    torch.manual_seed(0)
+    m = rg.LinearCrossEntropy(8, 20, reduction=reduction)
+    m.repro_name = "top"
+    x, t = torch.randn(5, 8), torch.randint(0, 20, (5,))
+    loss = m(x, t)
+    up = torch.ones_like(loss)
+    (clean,) = torch.autograd.grad(loss, m.weight, up, retain_graph=True)
+    rg.guard().check()
+    assert torch.equal(clean, results(x, m.weight, t, reduction)[2])
+    up.view(-1)[-1] = math.inf
+    torch.autograd.grad(loss, m.weight, up)
+    assert rg.guard().first_offender() == "top gradient"
+    rg.guard().reset()

@@ -110,15 +110,15 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             bits = group["state_bits"]
-            by_step = {}
+            by_step, steps = {}, {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
                 if p.grad.is_sparse:
                     raise RuntimeError("AdamW takes dense gradients")
                 state = self._state_of(p, bits)
-                state["step"] += 1
-                by_step.setdefault((int(state["step"]), p.device), []).append((p, state))
+                steps[p] = steps.get(p, int(state["step"])) + 1  # (one that is listed twice takes two steps)
+                by_step.setdefault((steps[p], p.device), []).append((p, state))
             for (step, _), held in by_step.items():
                 params = [p for p, _ in held]
                 grads = [_laid_out_as(p.grad, p) for p in params]
@@ -130,6 +130,8 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     adamw_step(params, grads, [s["exp_avg"] for _, s in held], [s["exp_avg_sq"] for _, s in held],
                                **settings)
+                for _, state in held:  # a step that is refused is not counted
+                    state["step"] = step
         return loss
 
 

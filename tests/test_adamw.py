@@ -312,3 +312,40 @@ def test_a_step_is_a_change_that_autograd_sees(bits):
     opt.step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_refused_step_is_not_counted(bits):
+    import copy
+
+    p = [torch.nn.Parameter(torch.randn(5)), torch.nn.Parameter(torch.randn(6))]
+    opt = rg.AdamW(p, state_bits=bits)
+    for t in p:
+        t.grad = torch.randn(t.shape)
+    opt.step()
+    before = [t.detach().clone() for t in p]
+    opt.param_groups[0]["lr"] = -1.0
+    with pytest.raises(ValueError):
+        opt.step()
+    assert [opt.state[t]["step"] for t in p] == [1, 1] and all(torch.equal(a, b) for a, b in zip(before, p))
+    opt.param_groups[0]["lr"] = 1e-3
+    again = [torch.nn.Parameter(t) for t in before]
+    other = rg.AdamW(again, state_bits=bits)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))  # (float32 moments would be shared)
+    for t, q in zip(p, again):
+        q.grad = t.grad
+    opt.step()
+    other.step()
+    assert all(torch.equal(a, b) for a, b in zip(p, again)) and opt.state[p[0]]["step"] == 2
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group with duplicate")
+def test_a_parameter_that_is_listed_twice_takes_two_steps():
+    p, q = torch.nn.Parameter(torch.randn(9)), None
+    q = torch.nn.Parameter(p.detach().clone())
+    p.grad = q.grad = torch.randn(9)
+    twice, once = rg.AdamW([p, p]), rg.AdamW([q])
+    twice.step()
+    once.step()
+    once.step()
+    assert torch.equal(p, q) and twice.state[p]["step"] == 2

@@ -26,7 +26,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         m <- m b1 + g (1 - b1),  v <- v b2 + g^2 (1 - b2),
         p <- p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - b2^step) + eps) lr / (1 - b1^step).
     params, grads, exp_avgs and exp_avg_sqs are lists of float32 tensors on one GPU or on the CPU; a
-    parameter's four tensors are dense and laid out alike. step is 1 for the first."""
+    parameter's four tensors are dense and laid out alike, and no two that are updated overlap. step is 1 for
+    the first."""
     _backend.adamw_step(params, grads, exp_avgs, exp_avg_sqs, float(lr), float(betas[0]), float(betas[1]), float(eps),
                         float(weight_decay), int(step))
 

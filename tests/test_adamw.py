@@ -349,3 +349,26 @@ def test_a_parameter_that_is_listed_twice_takes_two_steps():
     once.step()
     once.step()
     assert torch.equal(p, q) and twice.state[p]["step"] == 2
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_tensors_of_a_step_that_overlap_are_refused(device):
+    """Values that two threads of a launch would read and write."""
+    new = lambda n=600: torch.zeros(n, device=device)  # noqa: E731
+    z, flat = new(), new(1000)
+    for p, m, v in [([z, z], [new(), new()], [new(), new()]), ([new(), new()], [z, z], [new(), new()]),
+                    ([new(), new()], [new(), new()], [z, z]), ([new()], [z], [z]), ([z], [z], [new()]), ([z], [new()], [z]),
+                    ([flat[400:], flat[:600], new()], [new(), new(), new()], [new(), new(), new()][:3])]:
+        p = [t[:600] for t in p]
+        with pytest.raises(ValueError, match="overlap"):
+            rg.adamw_step(p, [torch.ones_like(t) for t in p], m, v, step=1)
+    apart = [flat[400:], new(0), flat[:400]]  # in no order, and an empty one
+    rg.adamw_step(apart, *([torch.zeros_like(t) for t in apart] for _ in range(3)), step=1)
+    with pytest.raises(ValueError, match="overlap"):
+        rg.adamw8_step([z, z], [new(), new()], *rg.adamw8_state([z, z]), step=1)
+    state = rg.adamw8_state([z])
+    for k in range(4):
+        states = [[s, s if i == k else s.clone()] for i, s in enumerate(state)]
+        with pytest.raises(ValueError, match="overlap"):
+            rg.adamw8_step([new(), new()], [new(), new()], *states, step=1)
+    rg.adamw8_step([new(), new()], [z, z], *([s, s.clone()] for s in state), step=1)  # gradients are only read

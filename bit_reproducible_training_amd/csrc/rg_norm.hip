@@ -470,7 +470,7 @@ norm_backward(Sizes z, Partition pt, const float* __restrict__ dr, const float* 
     }
 }
 
-// out[j][i] = the sum of P partials' column i: a block takes 64 columns, its wavefront h the partials
+// out[j][i] = the sum of P partials' column i: a block takes 64 columns of one sum j, its wavefront h the partials
 // p with p mod 16 = h.
 struct Totals {
     const float* part[4 + 1];
@@ -485,28 +485,25 @@ norm_totals(Totals z, int D) {
     __shared__ float lds[16][64];
     const int lane = threadIdx.x & 63, h = threadIdx.x >> 6;
     const int i = blockIdx.x * 64 + lane;
-    for (long long j = blockIdx.y; j < z.sums - 1 + z.repeat; j += gridDim.y) {
-        const int q = j < z.sums ? (int)j : z.sums - 1;
-        const long long again = j - q, P = z.partials[q];
-        const float* __restrict__ p = z.part[q] + again * P * D;
-        float s = 0.0f;
-        if (i < D) {
+    const int j = blockIdx.y, q = j < z.sums ? j : z.sums - 1;
+    const long long again = j - q, P = z.partials[q];
+    const float* __restrict__ p = z.part[q] + again * P * D;
+    float s = 0.0f;
+    if (i < D) {
 #pragma unroll 8
-            for (long long k = h; k < P; k += 16) s = s + p[k * D + i];
-        }
-        lds[h][lane] = s;
-        __syncthreads();
-        if (h == 0 && i < D) {
-            float v[16];
+        for (long long k = h; k < P; k += 16) s = s + p[k * D + i];
+    }
+    lds[h][lane] = s;
+    __syncthreads();
+    if (h == 0 && i < D) {
+        float v[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = lds[k][lane];
+        for (int k = 0; k < 16; ++k) v[k] = lds[k][lane];
 #pragma unroll
-            for (int n = 8; n > 0; n /= 2)
+        for (int n = 8; n > 0; n /= 2)
 #pragma unroll
-                for (int k = 0; k < n; ++k) v[k] = v[2 * k] + v[2 * k + 1];
-            z.out[q][again * D + i] = v[0];
-        }
-        __syncthreads();
+            for (int k = 0; k < n; ++k) v[k] = v[2 * k] + v[2 * k + 1];
+        z.out[q][again * D + i] = v[0];
     }
 }
 
@@ -611,7 +608,6 @@ int rg_residual_norm_grad_fp32(const rg_norm_config* cfg, const float* dr, const
         return hipErrorInvalidValue;
     const Partition pt = repro_norm::partition(cfg->N, cfg->D, cfg->gate_rows);
     const long long P = pt.sections * pt.partials;
-    if (P >= 1ll << 22) return hipErrorInvalidValue;  // a launch has fewer than 2^32 threads
     float* out[SUMS] = {dweight, dbias, dpost_weight, dpost_bias, pt.gate_inside ? nullptr : dgate};
     bool any = false;
     for (float* o : out) any = any || o;
@@ -642,8 +638,8 @@ int rg_residual_norm_grad_fp32(const rg_norm_config* cfg, const float* dr, const
     });
     int rc = hipGetLastError();
     if (rc == hipSuccess && totals.sums > 0) {
-        const long long jobs = totals.sums - 1 + totals.repeat;
-        hipLaunchKernelGGL(norm_totals, dim3((cfg->D + 63) / 64, (unsigned)(jobs < 4096 ? jobs : 4096)), dim3(1024), 0,
+        // (The partition has at most 4096 partials and 2048 sections.)
+        hipLaunchKernelGGL(norm_totals, dim3((cfg->D + 63) / 64, (unsigned)(totals.sums - 1 + totals.repeat)), dim3(1024), 0,
                            st, totals, cfg->D);
         rc = hipGetLastError();
     }

@@ -53,11 +53,9 @@ int rg_residual_norm_fp32(const rg_norm_config* cfg, const float* x, const float
 /* The gradients. dr and dy: of r and y, one of them may be null (all zero); r (x where f is null), f and
  * stats as in the forward pass. Each output may be null: dx, df [N][D], dgate [gate_rows][D], and the
  * weights' and biases' [D]. The workspace holds at least the given bytes (0 where no sum over rows is
- * asked for: sums = 0). flag as above, for a row's sums of gradients.
+ * asked for: sums = 0). flag as above, where a value of dx is not finite.
  * 1 (invalid value): as above; dr and dy both null, an output whose input is absent, stats off 16 bytes (in
- * either pass), a
- * workspace that is needed and null, too small or off 4 bytes; 2^22 partial sums or more (a gate of
- * that many groups of at least four rows). */
+ * either pass), a workspace that is needed and null, too small or off 4 bytes. */
 int rg_residual_norm_grad_workspace(const rg_norm_config* cfg, int sums, size_t* bytes);
 int rg_residual_norm_grad_fp32(const rg_norm_config* cfg, const float* dr, const float* dy, const float* r,
                                const float* f, const float* gate, const float* post_weight,

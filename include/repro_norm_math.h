@@ -26,7 +26,8 @@ RG_HD inline int strands_of(int D) { return D <= 4096 ? 256 : 1024; }
 // strand, a section is a group, and its gate's gradient is the sum of its partials. Else there is one
 // section, a strand holds whole groups, and adds up each group's gradient by itself.
 // Strands are short enough to give a GPU work and long enough that their partials are little to
-// write beside the rows; they depend on the sizes alone, so the results do too.
+// write beside the rows; they depend on the sizes alone, so the results do too. There are at most 2 * aim partials
+// (below) and `aim` sections: groups are sections only where they are at least as long as N / aim.
 struct Partition {
     long long sections, section_rows;  // the last section may be shorter only where it is the only one
     int rows, join;

@@ -369,3 +369,20 @@ def test_the_guard_hears_a_block_whose_squares_pass_the_range(kind):
     assert torch.isfinite(r).all() and torch.isfinite(y).all()
     assert rg.guard().first_offender() == "residual_norm input"
     rg.guard().reset()
+
+
+def test_partial_sums_over_rows_are_few():
+    """At most two for each strand that a GPU is given (2048 for rows of up to 1024 values, else 512): a launch of a block for
+    each, and of a row of blocks for each sum, always fits. The workspace has five sums' partials."""
+    g = torch.Generator().manual_seed(1)
+    size = ctypes.c_size_t()
+    for d, aim in ((8, 2048), (1024, 2048), (1025, 512), (16384, 512)):
+        for k in range(400):
+            n = int(2.0 ** (40 * torch.rand(1, generator=g, dtype=torch.float64).item()))
+            rows = 2 ** int(torch.randint(0, 41, (1,), generator=g))  # groups of at least four rows, and shorter ones
+            for total, gate in ((n, 0), (n, 1), (n, n), (n // rows * rows, n // rows)):
+                if total == 0:
+                    continue
+                c = _lib.rg_norm_config(N=total, D=d, rms=0, post=0, gate_rows=gate, eps=1e-5, scale=1.0)
+                assert _lib.lib.rg_residual_norm_grad_workspace(ctypes.byref(c), 1, ctypes.byref(size)) == 0
+                assert 0 < size.value // (5 * 4 * d) <= 2 * aim, (total, d, gate)

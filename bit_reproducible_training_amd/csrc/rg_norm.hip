@@ -72,12 +72,6 @@ struct Chunks {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[k][i] = 0.0f;
     }
-    __device__ __forceinline__ void fill(float x) {
-#pragma unroll
-        for (int k = 0; k < NK; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[k][i] = x;
-    }
 };
 
 template <int CTRL>
@@ -520,8 +514,8 @@ constexpr long long FORWARD_BLOCKS = 512;
 // run(WAVES, NK) with the values that hold a row of D. Rows of 2049 to 4096 values take eight wavefronts in the
 // forward pass (sixteen wait for each other at its barriers: 4096 rows of 4096 59 -> 82 us) and sixteen
 // in the backward pass, whose sums over rows would not leave registers for two rows otherwise.
-template <class F>
-void with_row(int D, bool forward, F run) {
+template <bool FORWARD, class F>
+void with_row(int D, F run) {
     using std::integral_constant;
     const auto of = [&](auto waves, auto nk) { run(waves, nk); };
     constexpr integral_constant<int, 1> one;
@@ -535,9 +529,10 @@ void with_row(int D, bool forward, F run) {
     else if (D <= 768) of(one, three);
     else if (D <= 1024) of(one, four);
     else if (D <= 2048) of(eight, one);
-    else if (D <= 4096 && forward) of(eight, two);
-    else if (D <= 4096) of(sixteen, one);
-    else if (D <= 8192) of(sixteen, two);
+    else if (D <= 4096) {
+        if constexpr (FORWARD) of(eight, two);
+        else of(sixteen, one);
+    } else if (D <= 8192) of(sixteen, two);
     else of(sixteen, four);
 }
 
@@ -569,7 +564,7 @@ int rg_residual_norm_fp32(const rg_norm_config* cfg, const float* x, const float
         return hipErrorInvalidValue;
     const Sizes z = sizes_of(cfg);
     const long long group = cfg->gate_rows > 0 ? cfg->N / cfg->gate_rows : 1;
-    with_row(cfg->D, true, [&](auto waves, auto nk) {
+    with_row<true>(cfg->D, [&](auto waves, auto nk) {
         constexpr int WV = decltype(waves)::value, NK = decltype(nk)::value;
         constexpr int rows = WV == 1 ? 4 : 1;
         const long long needed = (cfg->N + rows - 1) / rows;
@@ -629,7 +624,7 @@ int rg_residual_norm_grad_fp32(const rg_norm_config* cfg, const float* dr, const
     }
     const Sizes z = sizes_of(cfg);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    with_row(cfg->D, false, [&](auto waves, auto nk) {
+    with_row<false>(cfg->D, [&](auto waves, auto nk) {
         constexpr int WV = decltype(waves)::value, NK = decltype(nk)::value;
         auto kernel = cfg->post ? (gate ? norm_backward<WV, NK, true, true> : norm_backward<WV, NK, true, false>)
                                 : (gate ? norm_backward<WV, NK, false, true> : norm_backward<WV, NK, false, false>);

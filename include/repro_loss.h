@@ -37,7 +37,7 @@ enum { RG_LOSS_MEAN = 0, RG_LOSS_SUM = 1, RG_LOSS_NONE = 2 };
 
 #define RG_LOSS_MAX_TOKENS (1 << 22)
 #define RG_LOSS_MAX_SIZE (1 << 23)
-#define RG_LOSS_MAX_WORDS (1 << 28)
+#define RG_LOSS_MAX_WORDS (1 << 25) /* 64 threads a word are the most of a launch, fewer than 2^32 */
 
 typedef struct rg_loss_config {
     long long N;            /* tokens, 0 .. RG_LOSS_MAX_TOKENS */

@@ -423,3 +423,13 @@ def test_the_guard_hears_a_gradient_that_is_not_finite(reduction):
     torch.autograd.grad(loss, m.weight, up)
     assert rg.guard().first_offender() == "top gradient"
     rg.guard().reset()
+
+
+def test_more_words_than_launches_take_are_refused():
+    """A launch has fewer than 2^32 threads, and slicing takes 64 a word."""
+    words = 2 ** 25
+    assert 64 * words < 2 ** 32
+    c, size = _lib.rg_loss_config(N=4, D=300, V=words + 1, slices=3, reduction=0, ignore_index=-100), ctypes.c_size_t()
+    assert _lib.lib.rg_linear_cross_entropy_workspace(ctypes.byref(c), 0, 1, ctypes.byref(size)) == _lib.HIP_ERROR_INVALID_VALUE
+    with pytest.raises(ValueError, match="too many"):
+        rg.linear_cross_entropy(torch.zeros(2, 1), torch.zeros(1, 1).expand(words + 1, 1), torch.zeros(2, dtype=torch.int64))

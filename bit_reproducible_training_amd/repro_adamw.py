@@ -26,8 +26,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.
         m <- m b1 + g (1 - b1),  v <- v b2 + g^2 (1 - b2),
         p <- p (1 - lr weight_decay) - m / (sqrt(v) / sqrt(1 - b2^step) + eps) lr / (1 - b1^step).
     params, grads, exp_avgs and exp_avg_sqs are lists of float32 tensors on one GPU or on the CPU; a
-    parameter's four tensors are dense and laid out alike, and no two that are updated overlap. step is 1 for
-    the first."""
+    parameter's four tensors are dense and laid out alike, and none that is updated overlaps another of the call (neighbours
+    in a list and a parameter's own are checked). step is 1 for the first."""
     _backend.adamw_step(params, grads, exp_avgs, exp_avg_sqs, float(lr), float(betas[0]), float(betas[1]), float(eps),
                         float(weight_decay), int(step))
 
@@ -111,29 +111,36 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             bits = group["state_bits"]
-            by_step, steps = {}, {}
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                if p.grad.is_sparse:
-                    raise RuntimeError("AdamW takes dense gradients")
-                state = self._state_of(p, bits)
-                steps[p] = steps.get(p, int(state["step"])) + 1  # (one that is listed twice takes two steps)
-                by_step.setdefault((steps[p], p.device), []).append((p, state))
-            for (step, _), held in by_step.items():
-                params = [p for p, _ in held]
-                grads = [_laid_out_as(p.grad, p) for p in params]
-                settings = dict(step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                                weight_decay=group["weight_decay"])
-                if bits == 8:
-                    names = ("exp_avg", "exp_avg_exponent", "exp_avg_sq", "exp_avg_sq_exponent")
-                    adamw8_step(params, grads, *([s[n] for _, s in held] for n in names), **settings)
-                else:
-                    adamw_step(params, grads, [s["exp_avg"] for _, s in held], [s["exp_avg_sq"] for _, s in held],
-                               **settings)
-                for _, state in held:  # a step that is refused is not counted
-                    state["step"] = step
+            by_step = {}
+            try:
+                for p in group["params"]:
+                    if p.grad is None:
+                        continue
+                    if p.grad.is_sparse:
+                        raise RuntimeError("AdamW takes dense gradients")
+                    state = self._state_of(p, bits)
+                    state["step"] += 1
+                    by_step.setdefault((int(state["step"]), p.device), []).append((p, state))
+                while by_step:
+                    key = next(iter(by_step))
+                    self._take(group, bits, key[0], by_step[key])
+                    del by_step[key]
+            except BaseException:  # steps that were not taken do not count
+                for held in by_step.values():
+                    for _, state in held:
+                        state["step"] -= 1
+                raise
         return loss
+
+    def _take(self, group, bits, step, held):
+        params = [p for p, _ in held]
+        grads = [_laid_out_as(p.grad, p) for p in params]
+        settings = dict(step=step, lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"])
+        if bits == 8:
+            names = ("exp_avg", "exp_avg_exponent", "exp_avg_sq", "exp_avg_sq_exponent")
+            adamw8_step(params, grads, *([s[n] for _, s in held] for n in names), **settings)
+        else:
+            adamw_step(params, grads, [s["exp_avg"] for _, s in held], [s["exp_avg_sq"] for _, s in held], **settings)
 
 
 def _laid_out_as(grad, p):

@@ -53,10 +53,12 @@ struct Targets {
 // need nothing of each other: the places before its own are those of the tokens of the blocks before it. The
 // scattered accesses are what takes time, at one compute unit's rate (8192 tokens of 50257 words: 66 us by
 // one block, 24 by 16).
-// A thread has BATCH tokens in flight.
+// A thread has BATCH tokens in flight. Batches of LISTED tokens come one after another, so a word's tokens of earlier
+// batches stand before those of later ones in `arrived`, and only one batch's are left to be ordered.
+constexpr int BATCH = 8, LISTED = 1024 * BATCH;
 __global__ void __launch_bounds__(1024)
 loss_words(const long long* __restrict__ target, long long ignore_index, int N, int V, Targets t) {
-    constexpr int BATCH = 8, threads = 1024, LINE = 32;
+    constexpr int threads = 1024, LINE = 32;
     __shared__ int places, kept;
     const int blocks = gridDim.x, self = blockIdx.x;
     // A block's memory operations all meet in its XCD's L2: loads that pass the L1 by, after a barrier that waits
@@ -79,7 +81,9 @@ loss_words(const long long* __restrict__ target, long long ignore_index, int N, 
     }
     phase_end();
     int count = 0, before = 0;
-    for (int base = threadIdx.x; base < N; base += threads * BATCH) {
+    for (int start = 0; start < N; start += LISTED) {
+        const int base = start + threadIdx.x;
+        if (start > 0) phase_end();
         int w[BATCH], slot[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) w[i] = read(base + i * threads);
@@ -110,7 +114,7 @@ loss_words(const long long* __restrict__ target, long long ignore_index, int N, 
         t.broken_weight[0] = 0;
     }
     for (int pass = 0; pass < 2; ++pass) {  // places for the block's words, then its tokens there
-        for (int base = threadIdx.x; base < N; base += threads * BATCH) {
+        for (int base = threadIdx.x; base < N; base += LISTED) {
             int w[BATCH], slot[BATCH], at[BATCH];
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) w[i] = read(base + i * threads);
@@ -445,11 +449,15 @@ loss_rows(const float* __restrict__ z, int ldz, int V, int parts, float2* __rest
     const bool broken = t.broken[n] != 0 || t.broken_weight[0] != 0;
     const Token k = broken ? repro_loss::broken_token() : repro_loss::finish_token(m, s, target_logit, g);
     if (arrived) {
-        const int place = t.place[word], count = t.count[word];
+        // All of `arrived` that a batch could hold before and after the token's own slot; what stands further before came
+        // with an earlier one. (131072 tokens of one word, 256 words of 64 values: 29 ms the call; compared with all of them, 55.)
+        const int place = t.place[word], count = t.count[word], slot = t.slot[n];
+        const int from = max(0, slot - (LISTED - 1)), to = min(count, slot + LISTED);
         int before = 0;
-        for (int i = lane; i < count; i += 64) before += t.arrived[place + i] < n;
+        for (int i = from + lane; i < to; i += 64) before += t.arrived[place + i] < n;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) before += __shfl_xor(before, off, 64);
+        before += from;
         if (lane == 0) {
             t.list[place + before] = n;
             t.lead[n] = make_int2(before == 0 ? count : 0, place);

@@ -223,3 +223,14 @@ def test_the_guard_hears_a_gradient_that_is_not_finite(reduction):
     torch.autograd.grad(loss, m.weight, up)
     assert rg.guard().first_offender() == "linear_cross_entropy gradient"
     rg.guard().reset()
+
+
+@pytest.mark.parametrize("words", [1, 2, 90])
+def test_a_frequent_word_over_several_batches_of_tokens(words):
+    """Tokens are listed 8192 at a time: a word's in three batches, and in the middle one only."""
+    n = 20011
+    x, w, t = case(n, 5, 90, seed=words, words=words, ignored=range(3, n, 11))
+    t[8192:16384:3] = 71
+    want = results(x, w, t)
+    assert_same(results(x.cuda(), w.cuda(), t.cuda()), want)
+    assert_same(results(x.cuda(), w.cuda(), t.cuda()), want)

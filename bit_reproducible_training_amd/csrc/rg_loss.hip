@@ -4,9 +4,9 @@
 // gradient dz two more with them: three products in all, where pieces of the vocabulary, whose
 // softmax is not known before the last piece, need z a second time.
 //
-// The matrix cores bound it: of 7.92 ms for 8192 tokens of 768 values against 50257 words (S = 3, four groups, dx and
-// dw) the products take 6.32, at 300 TFLOP/s of float32 work, the digits of dz 0.94, the rows' statistics
-// 0.35, slicing x and the weight 0.18, the target words 0.07.
+// The matrix cores bound it: of 7.86 ms for 8192 tokens of 768 values against 50257 words (S = 3, four groups, dx and
+// dw) the products take 6.24, at 304 TFLOP/s of float32 work, the digits of dz 0.94, the rows' statistics
+// 0.36, slicing x and the weight 0.19, the target words 0.07.
 #include "rg_digits.h"
 #include "rg_internal.h"
 #include "repro_loss.h"

@@ -64,7 +64,8 @@ def adamw8_values(exp_avg, exp_avg_exponent, exp_avg_sq, exp_avg_sq_exponent):
 
 
 class AdamW(torch.optim.Optimizer):
-    """torch.optim.AdamW's arguments and update, reproducible bit for bit; state_bits=8 keeps the
+    """torch.optim.AdamW's lr, betas, eps and weight_decay and its update (amsgrad, maximize, capturable and the
+    choice of an implementation are not there), reproducible bit for bit; state_bits=8 keeps the
     moments in 8 bits. Parameters are float32, each group's on one device. A parameter without a
     gradient is left out of a step; each counts its own steps."""
 

@@ -6,11 +6,15 @@ keeping the logits.
 
 The three products (logits, the gradients of x and of the weight) are the reproducible GEMM's; the
 softmax's exponentials, logarithms and sums have their own definition (include/repro_loss_math.h). So loss
-and gradients have the same bits on every run, on the GPU and on the CPU. Tokens are taken in groups, and
-a group's logits are used for its gradients at once, so training takes three products and the memory
-of one group's logits (512 MB, or those of 128 tokens): with the sum or the mean of the losses,
-the forward pass leaves the gradients for the backward pass to hand out. Without a reduction, whose
-gradients need what arrives there, the backward pass computes the logits again.
+and gradients have the same bits on every run, on the GPU and on the CPU. Tokens are taken in groups (of
+up to 2048, whose logits fill at most 512 MB, or of 128), and a group's logits are used for its gradients at once,
+so training takes three products. With the sum or the mean of the losses, the forward pass leaves the
+gradients for the backward pass to hand out. Without a reduction, whose gradients need what arrives there, the
+backward pass computes the logits again.
+
+Memory on a GPU while a call runs: for one group 4 bytes a logit, and with both gradients 2 slices bytes more
+(the digits of the logits' gradient in both orientations: at 3 slices 2.5 times the logits in all); 2 slices bytes
+for each value of the weight and about as much for each of x; the products' partial sums.
 """
 import torch
 

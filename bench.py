@@ -45,10 +45,10 @@ STEADY_STEPS = 50
 # from inside this process, so a figure is reported only while its sources are unchanged; otherwise it is null.
 CSRC = os.path.join(REPO, "bit_reproducible_training_amd", "csrc")
 TRAFFIC = {
-    "contract": (671575240, ("rg_contract.hip", "rg_internal.h", "rg_digits.h", "rg_mfma.h"),
-                 "928f2bec4bb4f70baebee00ecbad20b3f3a0eeb78f962178086fa61885a86197"),
-    "slicing": (235603489, ("rg_slice.hip", "rg_internal.h", "rg_digits.h"),
-                "0b4fdbb3b3b4853ad503bdc61b6173fca2ba2e76e25c970930c72537eb804157"),
+    "contract": (671576064, ("rg_contract.hip", "rg_internal.h", "rg_digits.h", "rg_mfma.h"),
+                 "a89a4c8b5333c39d04f9413f7bee82dfcdf5a8fa7a4995a8b054ef5215c5aed2"),
+    "slicing": (235614720, ("rg_slice.hip", "rg_internal.h", "rg_digits.h"),
+                "819a845df417649edcf7e0c2eee36f3c4973b29972131aadd8135c7cc2975644"),
 }
 FIXTURE = os.path.join(REPO, "tests", "golden", "baseline_configs.json")
 

@@ -92,12 +92,23 @@ class AdamW(torch.optim.Optimizer):
                 state["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
         return state
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:
+            group.setdefault("state_bits", 32)
+
     def load_state_dict(self, state_dict):
         """As torch's, except that 8-bit moments stay what they are (torch converts a state to its
-        parameter's type)."""
+        parameter's type). A state of torch.optim.AdamW is taken up, with moments in float32."""
+        for group in state_dict["param_groups"]:
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("AdamW has no amsgrad and no maximize")
         saved = {k: {n: t for n, t in s.items() if isinstance(t, torch.Tensor) and t.dtype == torch.uint8}
                  for k, s in state_dict["state"].items()}
         super().load_state_dict(state_dict)
+        for state in self.state.values():
+            if "step" in state:
+                state["step"] = int(state["step"])  # torch's is a tensor
         numbers = [n for g in state_dict["param_groups"] for n in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for number, p in zip(numbers, params):

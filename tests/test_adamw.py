@@ -372,3 +372,33 @@ def test_tensors_of_a_step_that_overlap_are_refused(device):
         with pytest.raises(ValueError, match="overlap"):
             rg.adamw8_step([new(), new()], [new(), new()], *states, step=1)
     rg.adamw8_step([new(), new()], [z, z], *([s, s.clone()] for s in state), step=1)  # gradients are only read
+
+
+def test_a_state_of_torchs_adamw_is_taken_up():
+    """Its steps go on: against torch's own from the same state, within the roundings of two more steps of each (16 and 4
+    as in check_step, twice, for both)."""
+    import copy
+
+    torch.manual_seed(2)
+    p = [torch.nn.Parameter(torch.randn(40)), torch.nn.Parameter(torch.randn(3, 5))]
+    theirs = torch.optim.AdamW(p, lr=1e-2, betas=(0.9, 0.98), weight_decay=0.1)
+    grads = [[torch.randn(t.shape) for t in p] for _ in range(5)]
+    for g in grads[:3]:
+        for t, v in zip(p, g):
+            t.grad = v
+        theirs.step()
+    q = [torch.nn.Parameter(t.detach().clone()) for t in p]
+    ours = rg.AdamW(q, state_bits=8)
+    ours.load_state_dict(copy.deepcopy(theirs.state_dict()))
+    for g in grads[3:]:
+        for a, b, v in zip(p, q, g):
+            a.grad, b.grad = v, v.clone()
+        theirs.step()
+        ours.step()
+    for a, b in zip(p, q):
+        assert torch.all((a.double() - b.double()).abs() <= 2 * 2 * EPS32 * (4 * a.detach().double().abs() + 20 * 2 * 1e-2))
+    assert all(int(ours.state[t]["step"]) == 5 and ours.state[t]["exp_avg"].dtype == torch.float32 for t in q)
+    for unknown in (dict(amsgrad=True), dict(maximize=True)):
+        state = torch.optim.AdamW([torch.nn.Parameter(torch.zeros(2))], **unknown).state_dict()
+        with pytest.raises(ValueError):
+            rg.AdamW([torch.nn.Parameter(torch.zeros(2))]).load_state_dict(state)

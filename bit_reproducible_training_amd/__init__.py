@@ -2,11 +2,11 @@
 exact recombination. Bit-identical to the CPU definition on every input. Around it: the
 reproducible convolution (forward and both gradients) on the same contraction, the exact
 (superaccumulator) sum and non-finite scan the layers need, and the reproducible Linear and
-Conv2d layers (autograd) built on them; and for language models the vocabulary loss, residual norms and
-AdamW steps, each with the same bits on the GPU and on the CPU.
+Conv2d layers (autograd) built on them; and for language models attention, the bias of relative positions, dropout, the
+vocabulary loss, residual norms and AdamW steps, each with the same bits on the GPU and on the CPU.
 
 The compute path is librepro_gemm.so (HIP kernels + C ABI, include/repro_gemm.h, repro_sum.h,
-repro_conv.h, repro_loss.h, repro_norm.h, repro_adamw.h); this package is its Python host mirror. Importing it fails if the
+repro_conv.h, repro_loss.h, repro_norm.h, repro_adamw.h, repro_attention.h, repro_dropout.h); this package is its Python host mirror. Importing it fails if the
 library is not built.
 """
 from .repro_gemm import (  # noqa: F401
@@ -55,6 +55,16 @@ from .repro_adamw import (  # noqa: F401
     adamw8_step,
     adamw8_values,
     adamw_step,
+)
+from .repro_attention import (  # noqa: F401
+    Attention,
+    RelativePositionBias,
+    attention,
+    relative_position_bias,
+)
+from .repro_dropout import (  # noqa: F401
+    Dropout,
+    dropout,
 )
 from .repro_loss import (  # noqa: F401
     LinearCrossEntropy,

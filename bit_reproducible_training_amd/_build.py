@@ -22,7 +22,7 @@ BUILD_DIR = os.path.join(CSRC, "_build")
 LIB_PATH = os.path.join(PKG_DIR, "librepro_gemm.so")
 
 SOURCES = ["rg_slice.hip", "rg_contract.hip", "rg_probe.hip", "rg_sum.hip", "rg_conv.hip", "rg_conv_fused.hip", "rg_conv_dw.hip",
-           "rg_loss.hip", "rg_norm.hip", "rg_adamw.hip", "rg_api.cpp"]
+           "rg_loss.hip", "rg_norm.hip", "rg_adamw.hip", "rg_attention.hip", "rg_relative_bias.hip", "rg_dropout.hip", "rg_api.cpp"]
 BINDING_SOURCE = "rg_torch.cpp"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -65,7 +65,7 @@ def _binding_compile_cmd(obj):
     import torch
 
     tdir = os.path.dirname(torch.__file__)
-    return ["g++", "-O2", "-std=c++17", "-fPIC", "-fno-fast-math", "-ffp-contract=off", "-pthread",
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-fno-fast-math", "-ffp-contract=off", "-mfma", "-pthread",
             "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-DTORCH_EXTENSION_NAME=_backend",
             "-DTORCH_API_INCLUDE_EXTENSION_H",
             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI),

@@ -1,6 +1,6 @@
 """Loads librepro_gemm.so (the C ABI in include/repro_gemm.h, repro_sum.h, repro_conv.h,
-repro_loss.h, repro_norm.h and repro_adamw.h) through ctypes, and the compiled PyTorch binding (_backend) that calls the
-same library for tensors.
+repro_loss.h, repro_norm.h, repro_adamw.h, repro_attention.h and repro_dropout.h) through ctypes, and the compiled
+PyTorch binding (_backend) that calls the same library for tensors.
 
 Both must have been built (bit_reproducible_training_amd._build.build(), or
 __graft_entry__.build()). There is no fallback: if either is missing or does not load,
@@ -93,6 +93,18 @@ class rg_loss_config(ctypes.Structure):
 class rg_norm_config(ctypes.Structure):
     _fields_ = [("N", ctypes.c_longlong), ("D", ctypes.c_int), ("rms", ctypes.c_int), ("post", ctypes.c_int),
                 ("gate_rows", ctypes.c_longlong), ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
+class rg_attention_config(ctypes.Structure):
+    _fields_ = [("B", ctypes.c_longlong), ("Tq", ctypes.c_longlong), ("Tk", ctypes.c_longlong), ("H", ctypes.c_int),
+                ("KVH", ctypes.c_int), ("D", ctypes.c_int), ("causal", ctypes.c_int), ("query_start", ctypes.c_longlong),
+                ("scale", ctypes.c_double), ("dropout", ctypes.c_double), ("seed", ctypes.c_ulonglong)] + \
+               [(n + "_stride", ctypes.c_longlong * 3) for n in ("q", "k", "v", "mask")]
+
+
+class rg_relative_bias_config(ctypes.Structure):
+    _fields_ = [("Tq", ctypes.c_longlong), ("Tk", ctypes.c_longlong), ("query_start", ctypes.c_longlong)] + \
+               [(n, ctypes.c_int) for n in ("H", "count", "both", "dense")] + [("borders", ctypes.POINTER(ctypes.c_int))]
 
 
 _CONV_WS = (ctypes.c_int, [ctypes.POINTER(rg_conv_shape), ctypes.c_int,
@@ -228,6 +240,27 @@ _MODEL_SIGNATURES = {
     "rg_adamw8_values": (ctypes.c_int, [ctypes.c_void_p] * 6 + [ctypes.c_longlong, ctypes.c_void_p]),
 }
 
+# The same for include/repro_attention.h and include/repro_dropout.h.
+_SEQUENCE_SIGNATURES = {
+    "rg_attention_config_init": (None, [ctypes.POINTER(rg_attention_config)]),
+    "rg_attention_pack_mask": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_longlong] * 4 +
+                               [ctypes.POINTER(ctypes.c_longlong), ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]),
+    "rg_attention_workspace": (ctypes.c_int, [ctypes.POINTER(rg_attention_config), ctypes.POINTER(ctypes.c_size_t)]),
+    "rg_attention_fp32": (ctypes.c_int, [ctypes.POINTER(rg_attention_config)] + [ctypes.c_void_p] * 11 +
+                          [ctypes.c_size_t, ctypes.c_void_p]),
+    "rg_attention_grad_workspace": (ctypes.c_int, [ctypes.POINTER(rg_attention_config), ctypes.c_int,
+                                                   ctypes.POINTER(ctypes.c_size_t)]),
+    "rg_attention_grad_fp32": (ctypes.c_int, [ctypes.POINTER(rg_attention_config)] + [ctypes.c_void_p] * 15 +
+                               [ctypes.c_size_t, ctypes.c_void_p]),
+    "rg_relative_bias_fp32": (ctypes.c_int, [ctypes.POINTER(rg_relative_bias_config)] + [ctypes.c_void_p] * 3),
+    "rg_relative_bias_grad_workspace": (ctypes.c_int, [ctypes.POINTER(rg_relative_bias_config),
+                                                       ctypes.POINTER(ctypes.c_size_t)]),
+    "rg_relative_bias_grad_fp32": (ctypes.c_int, [ctypes.POINTER(rg_relative_bias_config)] + [ctypes.c_void_p] * 3 +
+                                   [ctypes.c_size_t, ctypes.c_void_p]),
+    "rg_dropout_fp32": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_double, ctypes.c_ulonglong,
+                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+}
+
 
 def _bind_after_torch():
     """Makes the library use the same HIP runtime as PyTorch.
@@ -260,7 +293,8 @@ def _load():
             "librepro_gemm.so is not built (%s); run __graft_entry__.build() or "
             "python -m bit_reproducible_training_amd._build" % LIB_PATH)
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in list(_SIGNATURES.items()) + list(_MODEL_SIGNATURES.items()):
+    for name, (res, args) in list(_SIGNATURES.items()) + list(_MODEL_SIGNATURES.items()) + \
+            list(_SEQUENCE_SIGNATURES.items()):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

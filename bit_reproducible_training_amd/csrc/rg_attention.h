@@ -1,0 +1,197 @@
+#pragma once
+// What the attention's kernels share: its operands, which pairs are seen, and a wavefront's work on one row or key in the
+// order of repro_attention_math.h. Internal.
+#include "rg_internal.h"
+#include "repro_attention.h"
+#include "repro_attention_math.h"
+#include "repro_dropout_math.h"
+
+namespace rg {
+namespace attention {
+
+using repro_attention::CHUNK;
+using repro_attention::ds_of;
+using repro_attention::e2;
+using repro_attention::finite_top;
+using repro_attention::KEY_BLOCK;
+using repro_attention::larger;
+using repro_attention::LOG2E;
+using repro_attention::QUERY_CHUNK;
+using repro_attention::reciprocal;
+using repro_attention::TILE;
+
+struct Problem {
+    const float *q, *k, *v;
+    const long long* key_lengths;
+    const unsigned long long* mask;
+    const float* bias;
+    const unsigned long long* seed_at;
+    unsigned long long seed;
+    int B, Tq, Tk, H, KVH, D, group, causal, start;
+    float factor, scale, keep_factor;
+    uint32_t threshold;
+    long long q_stride[3], k_stride[3], v_stride[3], mask_stride[3];
+};
+struct Gradients {
+    const float *dy, *stats, *delta;
+};
+
+// Rows of 64-bit strides: a cache may be longer than 2^32 values.
+__device__ __forceinline__ const float* query_at(const Problem& z, int b, int h, int i) {
+    return z.q + b * z.q_stride[0] + i * z.q_stride[1] + h * z.q_stride[2];
+}
+__device__ __forceinline__ const float* key_at(const Problem& z, int b, int h, int j) {
+    return z.k + b * z.k_stride[0] + j * z.k_stride[1] + h / z.group * z.k_stride[2];
+}
+__device__ __forceinline__ const float* value_at(const Problem& z, int b, int h, int j) {
+    return z.v + b * z.v_stride[0] + j * z.v_stride[1] + h / z.group * z.v_stride[2];
+}
+// The batch item's keys.
+__device__ __forceinline__ int keys_of(const Problem& z, int b) {
+    if (!z.key_lengths) return z.Tk;
+    const long long n = z.key_lengths[b];
+    return n < 0 ? 0 : n < z.Tk ? (int)n : z.Tk;
+}
+// The keys from which on query i sees none, the mask aside.
+__device__ __forceinline__ int key_end(const Problem& z, int b, int i) {
+    const int n = keys_of(z, b);
+    return z.causal ? max(0, min(n, i + z.start + 1)) : n;
+}
+__device__ __forceinline__ bool seen(const Problem& z, int b, int h, int i, int j, int end) {
+    if (j >= end) return false;
+    if (!z.mask) return true;
+    return (z.mask[b * z.mask_stride[0] + h * z.mask_stride[1] + i * z.mask_stride[2] + (j >> 6)] >> (j & 63) & 1) != 0;
+}
+__device__ __forceinline__ float dot(const float* a, const float* b, int D) {
+    float s = 0.0f;
+    for (int d = 0; d < D; ++d) s = __builtin_fmaf(a[d], b[d], s);
+    return s;
+}
+__device__ __forceinline__ float score(const Problem& z, int b, int h, int i, int j) {
+    const float s = dot(query_at(z, b, h, i), key_at(z, b, h, j), z.D);
+    return z.bias ? __builtin_fmaf(s, z.factor, z.bias[(size_t)h * (z.Tq + z.Tk - 1) + j - i + z.Tq - 1] * LOG2E)
+                  : s * z.factor;
+}
+__device__ __forceinline__ bool kept(const Problem& z, uint64_t seed, int b, int h, int i, int j) {
+    if (z.threshold == 0) return true;
+    return repro_dropout::pair_words(j >> 2, i, b * z.H + h, seed).w[j & 3] >= z.threshold;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int n = 32; n > 0; n >>= 1) v = v + __shfl_xor(v, n, 64);
+    return v;
+}
+
+// A row's share of a chunk of keys; lane d holds o_d and o_{d + 64}.
+struct RowChunk {
+    float m, even, odd, o0, o1;
+};
+__device__ __forceinline__ RowChunk row_chunk(const Problem& z, uint64_t seed, int b, int h, int i, int first, int end, int lane) {
+    RowChunk r{-__builtin_inff(), 0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j0 = first; j0 < first + CHUNK && j0 < end; j0 += TILE) {
+        const int j = j0 + lane;
+        const bool see = seen(z, b, h, i, j, end);
+        const float t = see ? score(z, b, h, i, j) : -__builtin_inff();
+        const float next = larger(r.m, wave_max(t));
+        const float a = e2(r.m - finite_top(next));
+        r.m = next;
+        r.even = r.even * a, r.odd = r.odd * a, r.o0 = r.o0 * a, r.o1 = r.o1 * a;
+        const float p = see ? e2(t - finite_top(next)) : 0.0f;
+        const float u = see && kept(z, seed, b, h, i, j) ? p : 0.0f;
+        const unsigned long long which = __ballot(see);
+        for (int n = 0; n < TILE; n += 2) {
+            r.even = r.even + __shfl(p, n, 64);
+            r.odd = r.odd + __shfl(p, n + 1, 64);
+        }
+        for (int n = 0; n < TILE; ++n) {
+            const float w = __shfl(u, n, 64);
+            if ((which >> n & 1) == 0) continue;
+            const float* v = value_at(z, b, h, j0 + n);
+            if (lane < z.D) r.o0 = __builtin_fmaf(w, v[lane], r.o0);
+            if (lane + 64 < z.D) r.o1 = __builtin_fmaf(w, v[lane + 64], r.o1);
+        }
+    }
+    return r;
+}
+struct Joined {
+    float top = -__builtin_inff(), total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    __device__ __forceinline__ void join(const RowChunk& r) {
+        const float both = larger(top, r.m), a = e2(top - finite_top(both)), e = e2(r.m - finite_top(both));
+        top = both;
+        total = __builtin_fmaf(r.even + r.odd, e, total * a);
+        o0 = __builtin_fmaf(r.o0, e, o0 * a);
+        o1 = __builtin_fmaf(r.o1, e, o1 * a);
+    }
+};
+
+// u = p kept factor and ds of one pair, 0 where it is not seen.
+struct Pair {
+    float u, ds;
+};
+__device__ __forceinline__ Pair pair(const Problem& z, const Gradients& g, uint64_t seed, int b, int h, int i, int j, bool see) {
+    if (!see) return Pair{0.0f, 0.0f};
+    const size_t n = ((size_t)b * z.H + h) * z.Tq + i;
+    const float p = e2(score(z, b, h, i, j) - g.stats[2 * n]) * g.stats[2 * n + 1];
+    float u = p, dp = dot(g.dy + (((size_t)b * z.Tq + i) * z.H + h) * z.D, value_at(z, b, h, j), z.D);
+    if (z.threshold != 0) {
+        const bool keep = kept(z, seed, b, h, i, j);
+        u = keep ? p * z.keep_factor : 0.0f;
+        dp = keep ? dp * z.keep_factor : 0.0f;
+    }
+    return Pair{u, ds_of(p, dp, g.delta[n])};
+}
+
+// A key's share of a chunk of queries under a head; lane d holds dv_d, dv_{d + 64}, dk_d and dk_{d + 64}.
+struct KeyPart {
+    float v0, v1, k0, k1;
+};
+__device__ __forceinline__ KeyPart key_part(const Problem& z, const Gradients& g, uint64_t seed, int b, int h, int j, int first,
+                                            int lane) {
+    KeyPart r{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = first; i0 < first + QUERY_CHUNK && i0 < z.Tq; i0 += 64) {
+        const int i = i0 + lane;
+        const bool see = i < z.Tq && seen(z, b, h, i, j, key_end(z, b, i));
+        const Pair w = pair(z, g, seed, b, h, i, j, see);
+        const unsigned long long which = __ballot(see);
+        for (int n = 0; n < 64; ++n) {
+            const float u = __shfl(w.u, n, 64), ds = __shfl(w.ds, n, 64);
+            if ((which >> n & 1) == 0) continue;
+            const float* a = g.dy + (((size_t)b * z.Tq + i0 + n) * z.H + h) * z.D;
+            const float* x = query_at(z, b, h, i0 + n);
+            if (lane < z.D) {
+                r.v0 = __builtin_fmaf(u, a[lane], r.v0);
+                r.k0 = __builtin_fmaf(ds, x[lane], r.k0);
+            }
+            if (lane + 64 < z.D) {
+                r.v1 = __builtin_fmaf(u, a[lane + 64], r.v1);
+                r.k1 = __builtin_fmaf(ds, x[lane + 64], r.k1);
+            }
+        }
+    }
+    return r;
+}
+// A query's share of a block of keys; lane d holds dq_d and dq_{d + 64}.
+struct QueryPart {
+    float q0, q1;
+};
+__device__ __forceinline__ QueryPart query_part(const Problem& z, const Gradients& g, uint64_t seed, int b, int h, int i, int first,
+                                                int end, int lane) {
+    QueryPart r{0.0f, 0.0f};
+    for (int j0 = first; j0 < first + KEY_BLOCK && j0 < end; j0 += 64) {
+        const bool see = seen(z, b, h, i, j0 + lane, end);
+        const float mine = pair(z, g, seed, b, h, i, j0 + lane, see).ds;
+        const unsigned long long which = __ballot(see);
+        for (int n = 0; n < 64; ++n) {
+            const float ds = __shfl(mine, n, 64);
+            if ((which >> n & 1) == 0) continue;
+            const float* x = key_at(z, b, h, j0 + n);
+            if (lane < z.D) r.q0 = __builtin_fmaf(ds, x[lane], r.q0);
+            if (lane + 64 < z.D) r.q1 = __builtin_fmaf(ds, x[lane + 64], r.q1);
+        }
+    }
+    return r;
+}
+
+}  // namespace attention
+}  // namespace rg

@@ -1,0 +1,270 @@
+// Attention over states of another or the same length, and its gradients: one wavefront a row, in the order
+// of repro_attention_math.h.
+#include "rg_attention.h"
+
+#include <cmath>
+
+namespace rg {
+namespace attention {
+
+// The mask's truth values as words of 64 keys.
+__global__ void __launch_bounds__(256)
+pack_mask(const unsigned char* mask, long long heads, long long queries, long long Tk, long long s0, long long s1, long long s2,
+          long long key_stride, long long count, unsigned long long* words) {
+    const long long W = (Tk + 63) / 64;
+    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < count; n += (long long)gridDim.x * 4) {
+        const long long row = n / W, w = n % W, i = row % queries, h = row / queries % heads, b = row / queries / heads;
+        const long long j = 64 * w + (threadIdx.x & 63);
+        const bool seen = j < Tk && mask[b * s0 + h * s1 + i * s2 + j * key_stride] != 0;
+        const unsigned long long bits = __ballot(seen);
+        if ((threadIdx.x & 63) == 0) words[n] = bits;
+    }
+}
+
+__global__ void __launch_bounds__(256)
+forward_rows(Problem z, float* y, float* stats, unsigned long long* used) {
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    if (used && blockIdx.x == 0 && threadIdx.x == 0) *used = seed;
+    const int lane = threadIdx.x & 63;
+    const long long rows = (long long)z.B * z.H * z.Tq;
+    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
+        const int i = (int)(n % z.Tq), t = (int)(n / z.Tq), b = t / z.H, h = t % z.H;
+        const int end = key_end(z, b, i);
+        Joined all;
+        for (int first = 0; first < end; first += CHUNK) all.join(row_chunk(z, seed, b, h, i, first, end, lane));
+        const float inverse = reciprocal(all.total), f = z.threshold == 0 ? inverse : inverse * z.keep_factor;
+        float* out = y + (((size_t)b * z.Tq + i) * z.H + h) * z.D;
+        if (lane < z.D) out[lane] = all.o0 * f + 0.0f;
+        if (lane + 64 < z.D) out[lane + 64] = all.o1 * f + 0.0f;
+        if (stats && lane == 0) {
+            stats[2 * n] = finite_top(all.top);
+            stats[2 * n + 1] = inverse;
+        }
+    }
+}
+
+// delta = sum over d of dy y, for each row [B][H][Tq].
+__global__ void __launch_bounds__(256)
+row_deltas(Problem z, const float* dy, const float* y, float* delta) {
+    const int lane = threadIdx.x & 63;
+    const long long rows = (long long)z.B * z.H * z.Tq;
+    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
+        const int i = (int)(n % z.Tq), t = (int)(n / z.Tq), b = t / z.H, h = t % z.H;
+        const size_t at = (((size_t)b * z.Tq + i) * z.H + h) * z.D;
+        float s = lane < z.D ? dy[at + lane] * y[at + lane] : 0.0f;
+        if (lane + 64 < z.D) s = __builtin_fmaf(dy[at + lane + 64], y[at + lane + 64], s);
+        s = wave_sum(s);
+        if (lane == 0) delta[n] = s;
+    }
+}
+
+__global__ void __launch_bounds__(256)
+backward_keys(Problem z, Gradients g, float* dk, float* dv) {
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    const int lane = threadIdx.x & 63;
+    const long long rows = (long long)z.B * z.KVH * z.Tk;
+    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
+        const int j = (int)(n % z.Tk), kvh = (int)(n / z.Tk % z.KVH), b = (int)(n / z.Tk / z.KVH);
+        KeyPart s = {};
+        for (int h = kvh * z.group; h < (kvh + 1) * z.group; ++h)
+            for (int first = 0; first < z.Tq; first += QUERY_CHUNK) {
+                const KeyPart p = key_part(z, g, seed, b, h, j, first, lane);
+                s.v0 = s.v0 + p.v0, s.v1 = s.v1 + p.v1, s.k0 = s.k0 + p.k0, s.k1 = s.k1 + p.k1;
+            }
+        const size_t at = (((size_t)b * z.Tk + j) * z.KVH + kvh) * z.D;
+        if (lane < z.D) {
+            dv[at + lane] = s.v0 + 0.0f;
+            dk[at + lane] = s.k0 * z.scale + 0.0f;
+        }
+        if (lane + 64 < z.D) {
+            dv[at + lane + 64] = s.v1 + 0.0f;
+            dk[at + lane + 64] = s.k1 * z.scale + 0.0f;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256)
+backward_queries(Problem z, Gradients g, float* dq) {
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    const int lane = threadIdx.x & 63;
+    const long long rows = (long long)z.B * z.H * z.Tq;
+    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
+        const int i = (int)(n % z.Tq), t = (int)(n / z.Tq), b = t / z.H, h = t % z.H;
+        const int end = key_end(z, b, i);
+        float s0 = 0.0f, s1 = 0.0f;
+        for (int first = 0; first < end; first += KEY_BLOCK) {
+            const QueryPart p = query_part(z, g, seed, b, h, i, first, end, lane);
+            s0 = s0 + p.q0, s1 = s1 + p.q1;
+        }
+        const size_t at = (((size_t)b * z.Tq + i) * z.H + h) * z.D;
+        if (lane < z.D) dq[at + lane] = s0 * z.scale + 0.0f;
+        if (lane + 64 < z.D) dq[at + lane + 64] = s1 * z.scale + 0.0f;
+    }
+}
+
+// The bias's gradient: a thread a distance of a head.
+__global__ void __launch_bounds__(256)
+backward_bias(Problem z, Gradients g, float* dbias) {
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    const int columns = z.Tq + z.Tk - 1;
+    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < (long long)z.H * columns; n += (long long)gridDim.x * 256) {
+        const int h = (int)(n / columns), away = (int)(n % columns) - (z.Tq - 1);
+        float s = 0.0f;
+        for (int b = 0; b < z.B; ++b)
+            for (int block = 0; block < z.Tk; block += KEY_BLOCK)
+                for (int first = 0; first < z.Tq; first += QUERY_CHUNK) {
+                    const int high = min(block + KEY_BLOCK, z.Tk);
+                    int i = max(first, block - away);
+                    const int last = min(min(first + QUERY_CHUNK, z.Tq), high - away);
+                    if (i >= last) continue;
+                    float part = 0.0f;
+                    for (; i < last; ++i) {
+                        const Pair w = pair(z, g, seed, b, h, i, i + away, seen(z, b, h, i, i + away, key_end(z, b, i)));
+                        part = part + w.ds;
+                    }
+                    s = s + part;
+                }
+        dbias[n] = s + 0.0f;
+    }
+}
+
+namespace {
+
+bool off(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
+
+bool sizes_ok(const rg_attention_config* c) {
+    if (!c || c->B < 0 || c->Tq < 0 || c->Tk < 0 || c->H < 1 || c->KVH < 1 || c->H % c->KVH != 0 || c->D < 1 ||
+        c->D > RG_ATTENTION_MAX_D || c->Tq > RG_ATTENTION_MAX_LENGTH || c->Tk > RG_ATTENTION_MAX_LENGTH ||
+        c->B > RG_ATTENTION_MAX_HEADS || c->B * c->H > RG_ATTENTION_MAX_HEADS || !std::isfinite(c->scale) ||
+        !std::isfinite((float)(c->scale * 1.4426950408889634)) || !(c->dropout >= 0.0 && c->dropout < 1.0))
+        return false;
+    for (int n = 0; n < 3; ++n)
+        if (c->q_stride[n] < 0 || c->k_stride[n] < 0 || c->v_stride[n] < 0 || c->mask_stride[n] < 0) return false;
+    return true;
+}
+
+Problem problem_of(const rg_attention_config* c, const float* q, const float* k, const float* v, const long long* key_lengths,
+                   const unsigned long long* mask, const float* bias, const unsigned long long* seed_at) {
+    Problem z;
+    z.q = q, z.k = k, z.v = v, z.key_lengths = key_lengths, z.mask = mask, z.bias = bias, z.seed_at = seed_at;
+    z.seed = c->seed;
+    z.B = (int)c->B, z.Tq = (int)c->Tq, z.Tk = (int)c->Tk, z.H = c->H, z.KVH = c->KVH, z.D = c->D, z.group = c->H / c->KVH;
+    // past the ends, the queries all see every key or none
+    const long long s = c->query_start;
+    z.causal = c->causal && s < c->Tk;
+    z.start = (int)(s > c->Tk ? c->Tk : s < -c->Tq ? -c->Tq : s);
+    z.factor = repro_attention::score_factor(c->scale);
+    z.scale = (float)c->scale;
+    z.keep_factor = repro_dropout::factor_of(c->dropout);
+    z.threshold = repro_dropout::threshold_of(c->dropout);
+    for (int n = 0; n < 3; ++n) {
+        z.q_stride[n] = c->q_stride[n];
+        z.k_stride[n] = c->k_stride[n];
+        z.v_stride[n] = c->v_stride[n];
+        z.mask_stride[n] = c->mask_stride[n];
+    }
+    return z;
+}
+
+bool operands_ok(const rg_attention_config* c, const float* q, const float* k, const float* v, const long long* key_lengths,
+                 const unsigned long long* mask, const float* bias, const unsigned long long* seed_at) {
+    const bool rows = c->B > 0 && c->Tq > 0, keys = c->B > 0 && c->Tk > 0;
+    return !(rows && !q) && !(keys && (!k || !v)) && !off(q, 4) && !off(k, 4) && !off(v, 4) && !off(key_lengths, 8) &&
+           !off(mask, 8) && !off(bias, 4) && !off(seed_at, 8);
+}
+
+unsigned grid_of(long long items, int a_block) {
+    const long long blocks = (items + a_block - 1) / a_block;
+    return (unsigned)(blocks < 1 ? 1 : blocks < (1 << 20) ? blocks : 1 << 20);
+}
+
+}  // namespace
+}  // namespace attention
+}  // namespace rg
+
+extern "C" {
+
+void rg_attention_config_init(rg_attention_config* cfg) {
+    if (!cfg) return;
+    *cfg = rg_attention_config{};
+    cfg->B = 1;
+    cfg->H = cfg->KVH = 1;
+    cfg->scale = 1.0;
+}
+
+int rg_attention_pack_mask(const unsigned char* mask, long long items, long long heads, long long queries, long long Tk,
+                           const long long stride[3], long long key_stride, unsigned long long* words, void* stream) {
+    using namespace rg::attention;
+    if (items < 0 || heads < 0 || queries < 0 || Tk < 0 || items > RG_ATTENTION_MAX_HEADS || heads > RG_ATTENTION_MAX_HEADS ||
+        queries > RG_ATTENTION_MAX_LENGTH || Tk > RG_ATTENTION_MAX_LENGTH || off(words, 8))
+        return hipErrorInvalidValue;
+    const long long rows = items * heads * queries, W = (Tk + 63) / 64;
+    if (rows == 0 || W == 0) return hipSuccess;
+    if (!mask || !words || !stride) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(pack_mask, dim3(grid_of(rows * W, 4)), dim3(256), 0, static_cast<hipStream_t>(stream), mask, heads,
+                       queries, Tk, stride[0], stride[1], stride[2], key_stride, rows * W, words);
+    return hipGetLastError();
+}
+
+int rg_attention_workspace(const rg_attention_config* cfg, size_t* bytes) {
+    using namespace rg::attention;
+    if (!sizes_ok(cfg) || !bytes) return hipErrorInvalidValue;
+    *bytes = 0;
+    return hipSuccess;
+}
+
+int rg_attention_fp32(const rg_attention_config* cfg, const float* q, const float* k, const float* v,
+                      const long long* key_lengths, const unsigned long long* mask, const float* relative_bias,
+                      const unsigned long long* seed_at, unsigned long long* used, float* y, float* stats, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    using namespace rg::attention;
+    (void)workspace;
+    (void)workspace_bytes;
+    if (!sizes_ok(cfg) || !operands_ok(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at) || off(y, 4) ||
+        off(stats, 8) || off(used, 8))
+        return hipErrorInvalidValue;
+    const long long rows = cfg->B * cfg->H * cfg->Tq;
+    if (rows > 0 && !y) return hipErrorInvalidValue;
+    if (rows == 0 && !used) return hipSuccess;
+    const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at);
+    hipLaunchKernelGGL(forward_rows, dim3(grid_of(rows, 4)), dim3(256), 0, static_cast<hipStream_t>(stream), z, y, stats, used);
+    return hipGetLastError();
+}
+
+int rg_attention_grad_workspace(const rg_attention_config* cfg, int want_bias, size_t* bytes) {
+    using namespace rg::attention;
+    (void)want_bias;
+    if (!sizes_ok(cfg) || !bytes) return hipErrorInvalidValue;
+    *bytes = (size_t)(cfg->B * cfg->H * cfg->Tq) * sizeof(float);
+    return hipSuccess;
+}
+
+int rg_attention_grad_fp32(const rg_attention_config* cfg, const float* dy, const float* q, const float* k, const float* v,
+                           const long long* key_lengths, const unsigned long long* mask, const float* relative_bias,
+                           const unsigned long long* seed_at, const float* y, const float* stats, float* dq, float* dk,
+                           float* dv, float* drelative_bias, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace rg::attention;
+    if (!sizes_ok(cfg) || !operands_ok(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at) || off(dy, 4) || off(y, 4) ||
+        off(stats, 8) || off(dq, 4) || off(dk, 4) || off(dv, 4) || off(drelative_bias, 4) || (drelative_bias && !relative_bias))
+        return hipErrorInvalidValue;
+    const long long rows = cfg->B * cfg->H * cfg->Tq, keys = cfg->B * cfg->KVH * cfg->Tk;
+    size_t needed = 0;
+    (void)rg_attention_grad_workspace(cfg, drelative_bias != nullptr, &needed);
+    if ((rows > 0 && (!dy || !y || !stats || !dq)) || (keys > 0 && (!dk || !dv)) ||
+        (needed > 0 && (!workspace || workspace_bytes < needed || off(workspace, 16))))
+        return hipErrorInvalidValue;
+    const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at);
+    const Gradients g{dy, stats, static_cast<float*>(workspace)};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (rows > 0) {
+        hipLaunchKernelGGL(row_deltas, dim3(grid_of(rows, 4)), dim3(256), 0, st, z, dy, y, static_cast<float*>(workspace));
+        hipLaunchKernelGGL(backward_queries, dim3(grid_of(rows, 4)), dim3(256), 0, st, z, g, dq);
+    }
+    if (keys > 0) hipLaunchKernelGGL(backward_keys, dim3(grid_of(keys, 4)), dim3(256), 0, st, z, g, dk, dv);
+    if (drelative_bias && z.Tq + z.Tk > 1)
+        hipLaunchKernelGGL(backward_bias, dim3(grid_of((long long)z.H * (z.Tq + z.Tk - 1), 256)), dim3(256), 0, st, z, g,
+                           drelative_bias);
+    return hipGetLastError();
+}
+
+}  // extern "C"

@@ -1,7 +1,8 @@
 // PyTorch binding of the reproducible operations: the compiled counterpart of the reference's
 // repro_torch/src/bindings.cpp:43-175,286-297 (_backend.gemm, exact_sum, conv2d,
 // conv2d_grad_weight, conv2d_grad_input, scan_finite), with the same names, arguments, checks
-// and results; and the vocabulary loss, the residual norms (with their autograd nodes) and the AdamW steps.
+// and results; and the vocabulary loss, the residual norms, attention, the bias of relative positions and dropout (with their
+// autograd nodes) and the AdamW steps.
 //
 // A GPU tensor runs on the MI355X library (librepro_gemm.so, through its C ABI) on PyTorch's
 // current HIP stream of the tensor's device, with the workspace taken from PyTorch's caching
@@ -18,6 +19,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -25,8 +27,12 @@
 
 #include "repro_adamw.h"
 #include "repro_adamw_cpu.h"
+#include "repro_attention.h"
+#include "repro_attention_cpu.h"
 #include "repro_conv.h"
 #include "repro_conv_cpu.h"
+#include "repro_dropout.h"
+#include "repro_dropout_cpu.h"
 #include "repro_gemm.h"
 #include "repro_gemm_cpu.h"
 #include "repro_loss.h"
@@ -971,6 +977,388 @@ Tensor loss_apply(const Tensor& x, const Tensor& weight, const Tensor& target, i
                                grad && weight.requires_grad());
 }
 
+// A leaf keeps the stream that the first graph over it was made on for as long as such a graph lives, and a backward pass
+// waits for that stream; one that is being captured cannot wait for a stream outside of its capture, and PyTorch ends the process
+// over it. So the forward pass is refused there.
+void need_capturable(std::initializer_list<const Tensor*> operands, const char* op) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const Tensor* t : operands) {
+        if (!t->defined() || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!node || !node->stream().has_value()) continue;
+        const auto current = c10::hip::getCurrentHIPStream(t->get_device());
+        if (node->stream()->id() == current.unwrap().id()) continue;
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        check((int)hipStreamIsCapturing(current.stream(), &status), op);
+        need(status == hipStreamCaptureStatusNone,
+             std::string(op) + ": a graph over an operand that was made outside of this capture is still alive; free it before");
+    }
+}
+
+// ---- dropout ----
+
+// A seed: a number, or an int64 tensor of one element on the operands' device, which is read when the kernels run.
+struct Seed {
+    uint64_t value;
+    Tensor at;
+};
+
+Seed seed_of(uint64_t value, const OptTensor& at, const Tensor& x, const char* op) {
+    if (!at.has_value()) return Seed{value, Tensor()};
+    need(at->scalar_type() == torch::kInt64 && at->numel() == 1 && at->device() == x.device(),
+         std::string(op) + ": a seed must be a number or an int64 tensor of one element on the operands' device");
+    if (x.is_cpu()) return Seed{(uint64_t)at->data_ptr<int64_t>()[0], Tensor()};
+    return Seed{0, at->contiguous()};
+}
+const unsigned long long* seed_data(const Tensor& at) {
+    return at.defined() ? reinterpret_cast<const unsigned long long*>(at.data_ptr<int64_t>()) : nullptr;
+}
+
+void need_probability(double p, const char* op) {
+    need(p >= 0.0 && p < 1.0, std::string(op) + ": the probability to drop must be in [0, 1)");
+}
+
+// used, when defined, receives the seed that was read.
+Tensor dropout_run(const Tensor& x_, double p, const Seed& seed, const Tensor& used) {
+    const Tensor x = x_.resolve_neg().contiguous();
+    Tensor y = torch::empty_like(x);
+    if (x.is_cuda()) {
+        c10::DeviceGuard guard(x.device());
+        check(rg_dropout_fp32(x.data_ptr<float>(), y.data_ptr<float>(), (size_t)x.numel(), p, seed.value, seed_data(seed.at),
+                              const_cast<unsigned long long*>(seed_data(used)), stream_of(x)),
+              "dropout");
+    } else {
+        Unlocked unlocked;
+        repro_dropout::cpu_dropout(x.data_ptr<float>(), y.data_ptr<float>(), (size_t)x.numel(), p, seed.value);
+    }
+    return y;
+}
+
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+    static Tensor forward(AutogradContext* ctx, Tensor x, double p, int64_t seed, OptTensor at, bool want) {
+        const Seed s = seed_of((uint64_t)seed, at, x, "dropout");
+        Tensor used;
+        if (want && s.at.defined()) used = torch::empty({1}, s.at.options());
+        const Tensor y = dropout_run(x, p, s, used);
+        if (want) {
+            if (used.defined()) ctx->saved_data["used"] = used;
+            ctx->saved_data["seed"] = (int64_t)s.value;
+            ctx->saved_data["p"] = p;
+        }
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        Seed s{(uint64_t)ctx->saved_data["seed"].toInt(), Tensor()};
+        if (ctx->saved_data.count("used")) s.at = ctx->saved_data["used"].toTensor();
+        variable_list result(5);
+        result[0] = dropout_run(grads[0], ctx->saved_data["p"].toDouble(), s, Tensor());
+        differentiable_once(result, "dropout");
+        return result;
+    }
+};
+
+Tensor dropout_apply(const Tensor& x, double p, uint64_t seed, const OptTensor& at) {
+    require_f32(x, "x");
+    need(x.is_cuda() || x.is_cpu(), "dropout: tensors must be on the CPU or a GPU");
+    need_probability(p, "dropout");
+    seed_of(seed, at, x, "dropout");
+    need_capturable({&x}, "dropout");
+    return DropoutFunction::apply(x, p, (int64_t)seed, at, at::GradMode::is_enabled() && x.requires_grad());
+}
+
+// ---- attention ----
+
+// [B, T, heads, D] with its values next to each other; any other strides stay.
+Tensor attention_operand(const Tensor& t_) {
+    const Tensor t = t_.resolve_neg();
+    return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+void set_strides(long long* to, const Tensor& t) {
+    for (int n = 0; n < 3; ++n) to[n] = t.size(n) > 1 ? t.stride(n) : 0;
+}
+
+struct AttentionSettings {
+    double scale;
+    bool causal;
+    int64_t query_start;
+    double dropout;
+    int64_t seed;
+};
+
+rg_attention_config attention_config(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionSettings& s) {
+    rg_attention_config c;
+    rg_attention_config_init(&c);
+    c.B = q.size(0);
+    c.Tq = q.size(1);
+    c.H = (int)q.size(2);
+    c.D = (int)q.size(3);
+    c.Tk = k.size(1);
+    c.KVH = (int)k.size(2);
+    c.causal = s.causal ? 1 : 0;
+    c.query_start = s.query_start;
+    c.scale = s.scale;
+    c.dropout = s.dropout;
+    c.seed = (unsigned long long)s.seed;
+    set_strides(c.q_stride, q);
+    set_strides(c.k_stride, k);
+    set_strides(c.v_stride, v);
+    return c;
+}
+// The packed mask's strides; [items, heads, queries, words], sizes 1 shared.
+void set_mask(rg_attention_config& c, const Tensor& words) {
+    if (!words.defined()) return;
+    const long long row = words.size(3);
+    const long long strides[3] = {row * words.size(1) * words.size(2), row * words.size(2), row};
+    for (int n = 0; n < 3; ++n) c.mask_stride[n] = words.size(n) > 1 ? strides[n] : 0;
+}
+const unsigned long long* words_or_null(const Tensor& t) {
+    return t.defined() ? reinterpret_cast<const unsigned long long*>(t.data_ptr<int64_t>()) : nullptr;
+}
+const long long* lengths_or_null(const Tensor& t) {
+    return t.defined() ? reinterpret_cast<const long long*>(t.data_ptr<int64_t>()) : nullptr;
+}
+
+// The mask (bool, broadcast to [B, H, Tq, Tk]) as words of 64 keys.
+Tensor packed_mask(const Tensor& mask_, const Tensor& q, int64_t Tk) {
+    need(mask_.scalar_type() == torch::kBool && mask_.device() == q.device() && mask_.dim() <= 4,
+         "attention: the mask must be bool, on the operands' device, with at most 4 dimensions");
+    Tensor mask = mask_;
+    while (mask.dim() < 4) mask = mask.unsqueeze(0);
+    const int64_t want[4] = {q.size(0), q.size(2), q.size(1), Tk};
+    for (int n = 0; n < 4; ++n)
+        need(mask.size(n) == want[n] || mask.size(n) == 1, "attention: the mask must broadcast to [batch, heads, queries, keys]");
+    const long long stride[3] = {mask.stride(0), mask.stride(1), mask.stride(2)};
+    const long long key_stride = mask.size(3) == Tk ? mask.stride(3) : 0;
+    Tensor words = torch::empty({mask.size(0), mask.size(1), mask.size(2), (Tk + 63) / 64}, q.options().dtype(torch::kInt64));
+    const auto* from = reinterpret_cast<const unsigned char*>(mask.data_ptr<bool>());
+    auto* to = reinterpret_cast<unsigned long long*>(words.data_ptr<int64_t>());
+    if (words.numel() == 0) return words;
+    if (q.is_cuda()) {
+        c10::DeviceGuard guard(q.device());
+        check(rg_attention_pack_mask(from, mask.size(0), mask.size(1), mask.size(2), Tk, stride, key_stride, to, stream_of(q)),
+              "attention mask");
+    } else {
+        Unlocked unlocked;
+        repro_attention::cpu_pack_mask(from, mask.size(0), mask.size(1), mask.size(2), Tk, stride, key_stride, to);
+    }
+    return words;
+}
+
+// The operands are q, k, v and the relative bias; lengths and words prepared by attention_apply.
+struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
+    static Tensor forward(AutogradContext* ctx, Tensor q_, Tensor k_, Tensor v_, OptTensor bias_, OptTensor lengths,
+                          OptTensor words_, AttentionSettings s, OptTensor seed_at, bool want, bool want_bias) {
+        const Tensor q = attention_operand(q_), k = attention_operand(k_), v = attention_operand(v_);
+        const Tensor bias = bias_.has_value() ? bias_->resolve_neg().contiguous() : Tensor();
+        const Tensor words = or_undefined(words_), keys = or_undefined(lengths);
+        const Seed seed = seed_of((uint64_t)s.seed, seed_at, q, "attention");
+        s.seed = (int64_t)seed.value;
+        rg_attention_config c = attention_config(q, k, v, s);
+        set_mask(c, words);
+        Tensor y = torch::empty(q.sizes(), q.options()), stats, used;
+        if (want) stats = torch::empty({c.B, c.H, c.Tq, 2}, q.options());
+        if (want && seed.at.defined()) used = torch::empty({1}, seed.at.options());
+        if (q.is_cuda()) {
+            c10::DeviceGuard guard(q.device());
+            size_t bytes = 0;
+            check(rg_attention_workspace(&c, &bytes), "attention plan");
+            Tensor ws;
+            if (bytes > 0) ws = workspace_like(bytes, q);
+            check(rg_attention_fp32(&c, q.data_ptr<float>(), k.data_ptr<float>(), v.data_ptr<float>(), lengths_or_null(keys),
+                                    words_or_null(words), data_or_null(bias), seed_data(seed.at),
+                                    const_cast<unsigned long long*>(seed_data(used)), y.data_ptr<float>(), out_or_null(stats),
+                                    bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+                  "attention");
+        } else {
+            Unlocked unlocked;
+            repro_attention::cpu_attention(c, q.data_ptr<float>(), k.data_ptr<float>(), v.data_ptr<float>(),
+                                           lengths_or_null(keys), words_or_null(words), data_or_null(bias),
+                                           y.data_ptr<float>(), out_or_null(stats));
+        }
+        if (want) {
+            ctx->save_for_backward({q_, k_, v_, or_undefined(bias_), keys, words, y, stats});
+            if (used.defined()) ctx->saved_data["used"] = used;
+            ctx->saved_data["settings"] = std::make_tuple(s.scale, s.causal, s.query_start, s.dropout, s.seed, want_bias);
+        }
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const auto settings = ctx->saved_data["settings"].toTuple();
+        const auto& e = settings->elements();
+        const AttentionSettings s{e[0].toDouble(), e[1].toBool(), e[2].toInt(), e[3].toDouble(), e[4].toInt()};
+        const bool want_bias = e[5].toBool();
+        const Tensor q = attention_operand(saved[0]), k = attention_operand(saved[1]), v = attention_operand(saved[2]);
+        const Tensor bias = saved[3].defined() ? saved[3].resolve_neg().contiguous() : Tensor();
+        const Tensor &keys = saved[4], &words = saved[5], &y = saved[6], &stats = saved[7];
+        const Tensor dy = grads[0].resolve_neg().contiguous();
+        Tensor used;
+        if (ctx->saved_data.count("used")) used = ctx->saved_data["used"].toTensor();
+        rg_attention_config c = attention_config(q, k, v, s);
+        set_mask(c, words);
+        Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options()),
+               dv = torch::empty(k.sizes(), k.options()), dbias;
+        if (want_bias) dbias = torch::empty(bias.sizes(), bias.options());
+        if (q.is_cuda()) {
+            c10::DeviceGuard guard(q.device());
+            size_t bytes = 0;
+            check(rg_attention_grad_workspace(&c, want_bias, &bytes), "attention gradient plan");
+            Tensor ws = workspace_like(bytes, q);
+            check(rg_attention_grad_fp32(&c, dy.data_ptr<float>(), q.data_ptr<float>(), k.data_ptr<float>(), v.data_ptr<float>(),
+                                         lengths_or_null(keys), words_or_null(words), data_or_null(bias), seed_data(used),
+                                         y.data_ptr<float>(), stats.data_ptr<float>(), dq.data_ptr<float>(), dk.data_ptr<float>(),
+                                         dv.data_ptr<float>(), out_or_null(dbias), ws.data_ptr(), (size_t)ws.numel(),
+                                         stream_of(q)),
+                  "attention gradient");
+        } else {
+            Unlocked unlocked;
+            repro_attention::cpu_attention_grad(c, dy.data_ptr<float>(), q.data_ptr<float>(), k.data_ptr<float>(),
+                                                v.data_ptr<float>(), lengths_or_null(keys), words_or_null(words),
+                                                data_or_null(bias), y.data_ptr<float>(), stats.data_ptr<float>(),
+                                                dq.data_ptr<float>(), dk.data_ptr<float>(), dv.data_ptr<float>(),
+                                                out_or_null(dbias));
+        }
+        variable_list result(10);
+        result[0] = dq;
+        result[1] = dk;
+        result[2] = dv;
+        result[3] = dbias;
+        differentiable_once(result, "attention");
+        return result;
+    }
+};
+
+// q [B, Tq, H, D], k and v [B, Tk, KVH, D] -> [B, Tq, H, D], differentiable.
+Tensor attention_apply(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, int64_t query_start,
+                       const OptTensor& key_lengths, const OptTensor& mask, const OptTensor& bias, double dropout, uint64_t seed,
+                       const OptTensor& seed_at) {
+    const std::pair<const Tensor*, const char*> operands[] = {{&q, "q"}, {&k, "k"}, {&v, "v"}};
+    for (const auto& t : operands) {
+        require_f32(*t.first, t.second);
+        if (t.first->dim() != 4) need(false, std::string("attention: ") + t.second + " must be [batch, positions, heads, size]");
+    }
+    on_gpu(q, k, "attention");
+    on_gpu(q, v, "attention");
+    need(k.sizes() == v.sizes() && k.size(0) == q.size(0) && k.size(3) == q.size(3),
+         "attention: k and v must have one shape, with q's batch and size");
+    need(q.size(3) >= 1 && q.size(3) <= RG_ATTENTION_MAX_D, "attention: a head's size must be 1 to 128");
+    static_assert(RG_ATTENTION_MAX_D == 128, "the message above");
+    need(q.size(2) >= 1 && k.size(2) >= 1 && q.size(2) % k.size(2) == 0, "attention: k's heads must divide q's");
+    need(q.size(1) <= RG_ATTENTION_MAX_LENGTH && k.size(1) <= RG_ATTENTION_MAX_LENGTH &&
+             q.size(0) * q.size(2) <= RG_ATTENTION_MAX_HEADS && q.size(0) <= RG_ATTENTION_MAX_HEADS,
+         "attention: too many positions or heads");
+    need(std::isfinite((float)(scale * 1.4426950408889634)), "attention: the scale must be finite");
+    need_probability(dropout, "attention");
+    seed_of(seed, seed_at, q, "attention");
+    const Tensor given_bias = or_undefined(bias);
+    need_capturable({&q, &k, &v, &given_bias}, "attention");
+    OptTensor lengths, words;
+    if (key_lengths.has_value()) {
+        need((key_lengths->scalar_type() == torch::kInt64 || key_lengths->scalar_type() == torch::kInt32) &&
+                 key_lengths->device() == q.device() && key_lengths->dim() == 1 && key_lengths->size(0) == q.size(0),
+             "attention: key_lengths must be int64 or int32 [batch], on the operands' device");
+        lengths = key_lengths->to(torch::kInt64).contiguous();
+    }
+    if (mask.has_value()) words = packed_mask(*mask, q, k.size(1));
+    if (bias.has_value()) {
+        require_f32(*bias, "relative_bias");
+        need(bias->device() == q.device() && bias->dim() == 2 && bias->size(0) == q.size(2) &&
+                 bias->size(1) == std::max<int64_t>(q.size(1) + k.size(1) - 1, 0),
+             "attention: relative_bias must be [heads, queries + keys - 1], on the operands' device");
+    }
+    const bool grad = at::GradMode::is_enabled(), want_bias = grad && bias.has_value() && bias->requires_grad();
+    const bool want = want_bias || (grad && (q.requires_grad() || k.requires_grad() || v.requires_grad()));
+    return AttentionFunction::apply(q, k, v, bias, lengths, words,
+                                    AttentionSettings{scale, causal, query_start, dropout, (int64_t)seed}, seed_at, want,
+                                    want_bias);
+}
+
+// ---- the bias of relative positions ----
+
+rg_relative_bias_config relative_bias_config(int64_t H, int64_t Tq, int64_t Tk, int64_t start, const c10::List<int64_t>& borders,
+                                             bool both, bool dense, std::vector<int>& held) {
+    for (const int64_t b : borders) held.push_back((int)b);
+    rg_relative_bias_config c{};
+    c.Tq = Tq;
+    c.Tk = Tk;
+    c.query_start = start;
+    c.H = (int)H;
+    c.count = (int)held.size();
+    c.both = both ? 1 : 0;
+    c.dense = dense ? 1 : 0;
+    c.borders = held.data();
+    return c;
+}
+
+struct RelativeBiasFunction : torch::autograd::Function<RelativeBiasFunction> {
+    static Tensor forward(AutogradContext* ctx, Tensor table_, int64_t Tq, int64_t Tk, int64_t start, c10::List<int64_t> borders,
+                          bool both, bool dense, bool want) {
+        const Tensor table = table_.resolve_neg().contiguous();
+        const int64_t H = table.size(1);
+        std::vector<int> held;
+        const rg_relative_bias_config c = relative_bias_config(H, Tq, Tk, start, borders, both, dense, held);
+        Tensor out = dense ? torch::empty({H, Tq, Tk}, table.options())
+                           : torch::empty({H, std::max<int64_t>(Tq + Tk - 1, 0)}, table.options());
+        if (table.is_cuda()) {
+            c10::DeviceGuard guard(table.device());
+            check(rg_relative_bias_fp32(&c, table.data_ptr<float>(), out.data_ptr<float>(), stream_of(table)), "relative bias");
+        } else if (out.numel() > 0) {
+            Unlocked unlocked;
+            repro_attention::cpu_relative_bias(c, table.data_ptr<float>(), out.data_ptr<float>());
+        }
+        if (want) {
+            ctx->saved_data["sizes"] = std::make_tuple(H, Tq, Tk, start, both, dense);
+            ctx->saved_data["borders"] = borders;
+        }
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor dout = grads[0].resolve_neg().contiguous();
+        const auto sizes = ctx->saved_data["sizes"].toTuple();
+        const auto& e = sizes->elements();
+        const int64_t H = e[0].toInt(), Tq = e[1].toInt(), Tk = e[2].toInt();
+        std::vector<int> held;
+        const rg_relative_bias_config c = relative_bias_config(H, Tq, Tk, e[3].toInt(), ctx->saved_data["borders"].toIntList(),
+                                                               e[4].toBool(), e[5].toBool(), held);
+        Tensor dtable = torch::empty({(int64_t)(held.size() + 1) * (c.both ? 2 : 1), H}, dout.options());
+        if (dout.is_cuda()) {
+            c10::DeviceGuard guard(dout.device());
+            size_t bytes = 0;
+            check(rg_relative_bias_grad_workspace(&c, &bytes), "relative bias gradient plan");
+            Tensor ws = workspace_like(bytes, dout);
+            check(rg_relative_bias_grad_fp32(&c, dout.data_ptr<float>(), dtable.data_ptr<float>(), ws.data_ptr(),
+                                             (size_t)ws.numel(), stream_of(dout)),
+                  "relative bias gradient");
+        } else {
+            Unlocked unlocked;
+            if (dout.numel() > 0) repro_attention::cpu_relative_bias_grad(c, dout.data_ptr<float>(), dtable.data_ptr<float>());
+            else dtable.zero_();
+        }
+        variable_list result(8);
+        result[0] = dtable;
+        differentiable_once(result, "relative_position_bias");
+        return result;
+    }
+};
+
+// table [buckets, H], the borders between one side's buckets -> [H, Tq, Tk] (dense) or [H, Tq + Tk - 1].
+Tensor relative_bias_apply(const Tensor& table, int64_t Tq, int64_t Tk, int64_t start, const std::vector<int64_t>& borders,
+                           bool both, bool dense) {
+    require_f32(table, "table");
+    need(table.is_cuda() || table.is_cpu(), "relative_position_bias: tensors must be on the CPU or a GPU");
+    need(!borders.empty() && borders.size() <= RG_RELATIVE_BIAS_MAX_BORDERS && table.dim() == 2 && table.size(1) >= 1 &&
+             table.size(0) == (int64_t)(borders.size() + 1) * (both ? 2 : 1),
+         "relative_position_bias: the table must be [buckets, heads]");
+    need(table.size(1) <= 4096, "relative_position_bias: at most 4096 heads");
+    need(Tq >= 0 && Tk >= 0 && Tq <= RG_ATTENTION_MAX_LENGTH && Tk <= RG_ATTENTION_MAX_LENGTH,
+         "relative_position_bias: lengths must be 0 to 4194304");
+    static_assert(RG_ATTENTION_MAX_LENGTH == 4194304, "the message above");
+    need(start >= -(1ll << 32) && start <= (1ll << 32), "relative_position_bias: query_start is out of range");
+    need_capturable({&table}, "relative_position_bias");
+    return RelativeBiasFunction::apply(table, Tq, Tk, start, c10::List<int64_t>(borders), both, dense,
+                                       at::GradMode::is_enabled() && table.requires_grad());
+}
+
 }  // namespace
 
 // 64-bit FNV-1a over the raw bytes of a contiguous CPU tensor, continuing from h: the hash the
@@ -1007,6 +1395,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw8_values", &adamw8_values);
     m.def("norm_apply", &norm_apply);
     m.def("loss_apply", &loss_apply);
+    m.def("dropout_apply", &dropout_apply);
+    m.def("attention_apply", &attention_apply);
+    m.def("relative_bias_apply", &relative_bias_apply);
     m.def("cpu_threads", &repro_gemm::cpu_thread_count);
     m.def("set_error_class", [](py::object cls) {
         Py_XINCREF(cls.ptr());

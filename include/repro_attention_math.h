@@ -1,0 +1,83 @@
+#pragma once
+// What defines the reproducible attention and the bias of relative positions: the exponential and the order of
+// every sum, callable from host and device code. Every operation is rounded once (build without -ffast-math
+// and without FP contraction; fused multiply-adds are written out). Products are chains of fused
+// multiply-adds in ascending order from +0, which is what the matrix cores' float32 instructions compute.
+//
+// Forward, for a query and a head:
+//   score  s_j = fma chain over d of q_d k_jd;  t_j = s_j c (+ bias_j log2 e, fused), c = scale log2 e
+//   keys are taken in chunks of CHUNK, a chunk in tiles of TILE: m' = max(m, visible t of the tile), a = e2(m - m');
+//   p_j = e2(t_j - m'); l_even = l_even a, then + p_j of the even keys in ascending order, l_odd likewise;
+//   o_d = o_d a, then the chain over the tile's keys of p_j v_jd
+//   chunks are joined in ascending order: M' = max(M, m), a = e2(M - M'), b = e2(m - M'),
+//   L = fma(l_even + l_odd, b, L a), O_d = fma(o_d, b, O_d a)
+//   y_d = O_d (1 / L)
+// A masked key has p = 0 and nothing else of it takes part; a tile or chunk without visible keys changes nothing. So a
+// row's bits depend on its query and the keys it sees alone, not on the batch, the other queries or the padding.
+// -infinity as a maximum counts as 0 in the exponents; a row that sees nothing has L = 0, which 1 / L is 0 for.
+// With dropout the dropped p_j are 0 in the chain over v (not in l) and y is multiplied by factor / L.
+//
+// Backward: p_ij = e2(t_ij - M_i) (1 / L_i), delta_i = sum_d dy_d y_d, u_ij = p_ij kept factor,
+//   ds_ij = p_ij ((dy_i . v_j) kept factor - delta_i)
+// Queries are taken in chunks of QUERY_CHUNK and keys in blocks of KEY_BLOCK:
+//   dv_j = sum over the group's heads, then the chunks, both ascending, of the chunk's chain of u_ij dy_i; dk_j likewise of
+//   ds_ij q_i, times scale; dq_i = sum over the key blocks of the block's chain of ds_ij k_j, times scale
+//   the bias's gradient at distance j - i: over the batch, the key blocks, the chunks, ascending, the sum of ds_ij
+//   of one block and chunk in ascending order of i
+#include "repro_gemm_math.h"
+
+namespace repro_attention {
+
+using repro_gemm::bits_to_float;
+using repro_gemm::float_to_bits;
+
+constexpr int TILE = 64, CHUNK = 256, QUERY_CHUNK = 256, KEY_BLOCK = 128, MAX_D = 128;
+constexpr float LOG2E = 1.44269504f;
+inline float score_factor(double scale) { return (float)(scale * 1.4426950408889634); }
+
+// 2^t for t <= 0, within 1.1 units in the last place; 0 below -126, NaN for NaN, 1 for 0. t = n + f with n a whole number and
+// |f| <= 1/2, read off a sum with 1.5 2^23; 2^f by a polynomial whose coefficients were fitted to the least
+// largest relative error (2^-25.9).
+RG_HD inline float e2(float t) {
+    const float shifted = t + 12583039.0f;  // 1.5 2^23 + 127: the low bits are n + 127
+    const float f = t - (shifted - 12583039.0f);
+    float p = 0.00015353362f;
+    p = __builtin_fmaf(p, f, 0.0013398875f);
+    p = __builtin_fmaf(p, f, 0.009618437f);
+    p = __builtin_fmaf(p, f, 0.055503324f);
+    p = __builtin_fmaf(p, f, 0.24022648f);
+    p = __builtin_fmaf(p, f, 0.6931472f);
+    p = __builtin_fmaf(p, f, 1.0f);
+    const float r = p * bits_to_float(float_to_bits(shifted) << 23);
+    return t < -126.0f ? 0.0f : r;
+}
+RG_HD inline float finite_top(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+// The larger of the two; the other where one is NaN.
+RG_HD inline float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+// 1 / L, and 0 for a row that sees nothing.
+RG_HD inline float reciprocal(float total) { return total == 0.0f ? 0.0f : 1.0f / total; }
+RG_HD inline float ds_of(float p, float dp, float delta) { return p * (dp - delta); }
+
+// The sum of x_i over a row of D <= 128 values of products x_d = a_d b_d: lane l of 64 has fma(a_{l+64}, b_{l+64}, a_l b_l)
+// (missing values 0), and the lanes are added as a balanced tree whose first level adds l and l + 32, the next l and l + 16.
+
+// ---- the bias of relative positions ----
+//
+// The bucket of a distance n >= 0 is the number of borders <= n (ascending, made by the caller); a bidirectional table's
+// keys after the query have the upper half of the buckets.
+RG_HD inline int bucket_of(long long relative, const int* borders, int count, bool both) {
+    const long long n = relative > 0 ? (both ? relative : 0) : -relative;
+    int low = 0, high = count;
+    while (low < high) {
+        const int mid = (low + high) / 2;
+        if (borders[mid] <= n) low = mid + 1;
+        else high = mid;
+    }
+    return both && relative > 0 ? low + count + 1 : low;
+}
+// The gradient of a dense bias: rows in runs of RUN give each distance a sum in ascending order, the runs' are added in ascending
+// order; a bucket's distances (column n of [H][Tq + Tk - 1] goes to strand n mod STRANDS, in ascending order) are added, and
+// the strands as a balanced tree whose first level adds s and s + STRANDS / 2.
+constexpr int RUN = 64, STRANDS = 256;
+
+}  // namespace repro_attention

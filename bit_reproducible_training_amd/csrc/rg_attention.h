@@ -6,6 +6,8 @@
 #include "repro_attention_math.h"
 #include "repro_dropout_math.h"
 
+#include <type_traits>
+
 namespace rg {
 namespace attention {
 
@@ -28,6 +30,7 @@ struct Problem {
     const unsigned long long* seed_at;
     unsigned long long seed;
     int B, Tq, Tk, H, KVH, D, group, causal, start;
+    int quads;  // whether the rows of q, k and v can be read 16 bytes at a time
     float factor, scale, keep_factor;
     uint32_t threshold;
     long long q_stride[3], k_stride[3], v_stride[3], mask_stride[3];
@@ -125,6 +128,18 @@ struct Joined {
     }
 };
 
+__device__ __forceinline__ void finish_row(const Problem& z, const Joined& all, int b, int h, int i, int lane, float* y, float* stats) {
+    const float inverse = reciprocal(all.total), f = z.threshold == 0 ? inverse : inverse * z.keep_factor;
+    float* out = y + (((size_t)b * z.Tq + i) * z.H + h) * z.D;
+    if (lane < z.D) out[lane] = all.o0 * f + 0.0f;
+    if (lane + 64 < z.D) out[lane + 64] = all.o1 * f + 0.0f;
+    if (stats && lane == 0) {
+        const size_t n = ((size_t)b * z.H + h) * z.Tq + i;
+        stats[2 * n] = finite_top(all.top);
+        stats[2 * n + 1] = inverse;
+    }
+}
+
 // u = p kept factor and ds of one pair, 0 where it is not seen.
 struct Pair {
     float u, ds;
@@ -192,6 +207,35 @@ __device__ __forceinline__ QueryPart query_part(const Problem& z, const Gradient
     }
     return r;
 }
+
+// ---- host ----
+
+constexpr long long MAX_BLOCKS = 1 << 23;  // of 256 threads: a launch takes fewer than 2^32
+
+inline unsigned grid_of(long long items, int a_block) {
+    const long long blocks = (items + a_block - 1) / a_block;
+    return (unsigned)(blocks < 1 ? 1 : blocks < (1 << 20) ? blocks : 1 << 20);
+}
+// run(DB) with the blocks of 32 values that hold a head's.
+template <class F>
+void with_size(int D, F run) {
+    if (D <= 32) run(std::integral_constant<int, 1>());
+    else if (D <= 64) run(std::integral_constant<int, 2>());
+    else if (D <= 96) run(std::integral_constant<int, 3>());
+    else run(std::integral_constant<int, 4>());
+}
+template <class F>
+void with_flags(bool a, bool b, F run) {
+    const auto second = [&](auto x) {
+        if (b) run(x, std::true_type());
+        else run(x, std::false_type());
+    };
+    if (a) second(std::true_type());
+    else second(std::false_type());
+}
+
+size_t forward_workspace(const Problem& z);
+int forward(const Problem& z, float* y, float* stats, unsigned long long* used, void* workspace, hipStream_t stream);
 
 }  // namespace attention
 }  // namespace rg

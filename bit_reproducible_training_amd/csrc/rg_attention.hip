@@ -1,5 +1,4 @@
-// Attention over states of another or the same length, and its gradients: one wavefront a row, in the order
-// of repro_attention_math.h.
+// Attention over states of another or the same length: the entries and the small kernels.
 #include "rg_attention.h"
 
 #include <cmath>
@@ -18,28 +17,6 @@ pack_mask(const unsigned char* mask, long long heads, long long queries, long lo
         const bool seen = j < Tk && mask[b * s0 + h * s1 + i * s2 + j * key_stride] != 0;
         const unsigned long long bits = __ballot(seen);
         if ((threadIdx.x & 63) == 0) words[n] = bits;
-    }
-}
-
-__global__ void __launch_bounds__(256)
-forward_rows(Problem z, float* y, float* stats, unsigned long long* used) {
-    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
-    if (used && blockIdx.x == 0 && threadIdx.x == 0) *used = seed;
-    const int lane = threadIdx.x & 63;
-    const long long rows = (long long)z.B * z.H * z.Tq;
-    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
-        const int i = (int)(n % z.Tq), t = (int)(n / z.Tq), b = t / z.H, h = t % z.H;
-        const int end = key_end(z, b, i);
-        Joined all;
-        for (int first = 0; first < end; first += CHUNK) all.join(row_chunk(z, seed, b, h, i, first, end, lane));
-        const float inverse = reciprocal(all.total), f = z.threshold == 0 ? inverse : inverse * z.keep_factor;
-        float* out = y + (((size_t)b * z.Tq + i) * z.H + h) * z.D;
-        if (lane < z.D) out[lane] = all.o0 * f + 0.0f;
-        if (lane + 64 < z.D) out[lane + 64] = all.o1 * f + 0.0f;
-        if (stats && lane == 0) {
-            stats[2 * n] = finite_top(all.top);
-            stats[2 * n + 1] = inverse;
-        }
     }
 }
 
@@ -157,6 +134,9 @@ Problem problem_of(const rg_attention_config* c, const float* q, const float* k,
     z.scale = (float)c->scale;
     z.keep_factor = repro_dropout::factor_of(c->dropout);
     z.threshold = repro_dropout::threshold_of(c->dropout);
+    uintptr_t odd = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
+    for (int n = 0; n < 3; ++n) odd |= (uintptr_t)(c->q_stride[n] | c->k_stride[n] | c->v_stride[n]) * sizeof(float);
+    z.quads = (odd & 15) == 0 && c->D % 4 == 0;
     for (int n = 0; n < 3; ++n) {
         z.q_stride[n] = c->q_stride[n];
         z.k_stride[n] = c->k_stride[n];
@@ -171,11 +151,6 @@ bool operands_ok(const rg_attention_config* c, const float* q, const float* k, c
     const bool rows = c->B > 0 && c->Tq > 0, keys = c->B > 0 && c->Tk > 0;
     return !(rows && !q) && !(keys && (!k || !v)) && !off(q, 4) && !off(k, 4) && !off(v, 4) && !off(key_lengths, 8) &&
            !off(mask, 8) && !off(bias, 4) && !off(seed_at, 8);
-}
-
-unsigned grid_of(long long items, int a_block) {
-    const long long blocks = (items + a_block - 1) / a_block;
-    return (unsigned)(blocks < 1 ? 1 : blocks < (1 << 20) ? blocks : 1 << 20);
 }
 
 }  // namespace
@@ -209,7 +184,7 @@ int rg_attention_pack_mask(const unsigned char* mask, long long items, long long
 int rg_attention_workspace(const rg_attention_config* cfg, size_t* bytes) {
     using namespace rg::attention;
     if (!sizes_ok(cfg) || !bytes) return hipErrorInvalidValue;
-    *bytes = 0;
+    *bytes = forward_workspace(problem_of(cfg, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr));
     return hipSuccess;
 }
 
@@ -218,17 +193,16 @@ int rg_attention_fp32(const rg_attention_config* cfg, const float* q, const floa
                       const unsigned long long* seed_at, unsigned long long* used, float* y, float* stats, void* workspace,
                       size_t workspace_bytes, void* stream) {
     using namespace rg::attention;
-    (void)workspace;
-    (void)workspace_bytes;
     if (!sizes_ok(cfg) || !operands_ok(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at) || off(y, 4) ||
         off(stats, 8) || off(used, 8))
         return hipErrorInvalidValue;
     const long long rows = cfg->B * cfg->H * cfg->Tq;
     if (rows > 0 && !y) return hipErrorInvalidValue;
-    if (rows == 0 && !used) return hipSuccess;
+    if (rows == 0) return hipSuccess;
     const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at);
-    hipLaunchKernelGGL(forward_rows, dim3(grid_of(rows, 4)), dim3(256), 0, static_cast<hipStream_t>(stream), z, y, stats, used);
-    return hipGetLastError();
+    const size_t needed = forward_workspace(z);
+    if (needed > 0 && (!workspace || workspace_bytes < needed || off(workspace, 16))) return hipErrorInvalidValue;
+    return forward(z, y, stats, used, workspace, static_cast<hipStream_t>(stream));
 }
 
 int rg_attention_grad_workspace(const rg_attention_config* cfg, int want_bias, size_t* bytes) {

@@ -1,0 +1,410 @@
+// The attention's forward pass on the matrix cores.
+//
+// A block takes 128 queries of a head, 32 a wavefront, and goes through the keys in tiles of 64 that its wavefronts share in LDS.
+// v_mfma_f32_32x32x2_f32 adds a pair of products a step, in ascending order, each fused and rounded as fmaf is: the
+// definition's chains. Scores are made as S^T = K Q^T, so that a lane holds scores of one query (column lane mod 32), and
+// a register of the result is, as it stands, the operand of O^T = V^T P^T for two successive keys: row 8 g + 4 h + r of the tile's
+// operand is taken to be key 8 g + 2 r + h, so half h of the wavefront holds the keys of parity h in ascending order.
+// Nothing of the softmax passes through LDS, and a row's maximum takes one exchange between the halves.
+#include "rg_attention.h"
+
+namespace rg {
+namespace attention {
+namespace {
+
+typedef float Block16 __attribute__((ext_vector_type(16)));
+
+constexpr int ROWS = 128;
+
+__device__ __forceinline__ Block16 zero16() {
+    Block16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    return z;
+}
+__device__ __forceinline__ Block16 mfma(float a, float b, Block16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+// The value of the lane 32 away.
+__device__ __forceinline__ void halves(uint32_t v, uint32_t* low, uint32_t* high) {
+    const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    *low = s[0];
+    *high = s[1];
+}
+
+// 4 values of a row from d on; 0 past the row's end and where the row is not there.
+__device__ __forceinline__ float4 four(const float* row, bool there, int d, int D, bool quads) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (!there || d >= D) return v;
+    if (quads) return *reinterpret_cast<const float4*>(row + d);
+    v.x = row[d];
+    if (d + 1 < D) v.y = row[d + 1];
+    if (d + 2 < D) v.z = row[d + 2];
+    if (d + 3 < D) v.w = row[d + 3];
+    return v;
+}
+
+// A part of a row's chunks is handed on unjoined where the keys are split over blocks: m and l of each chunk (l = -1: nothing was seen
+// there) and its o.
+struct Parts {
+    int parts, chunks, a_part;  // chunks a part
+    float2* ml;                 // [B][H][Tq][chunks]
+    float* o;                   // [B][H][Tq][chunks][D]
+};
+
+// DB blocks of 32 values hold a head's.
+template <int DB, bool BIAS, bool DROP>
+__global__ void __launch_bounds__(256, 2)
+forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
+    constexpr int DP = 32 * DB, KS = DP + 4, QUAD_LOADS = 2 * DB;
+    constexpr bool AHEAD = DB <= 2;  // the next tile in registers while one is worked on
+    __shared__ float Ks[TILE * KS], Vs[TILE * DP], Bs[BIAS ? TILE + ROWS : 1];
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    if (used && blockIdx.x == 0 && threadIdx.x == 0) *used = seed;
+    const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5, wave = t >> 6;
+    const int heads = z.B * z.H, bh = (int)(blockIdx.x % heads), rest = (int)(blockIdx.x / heads);
+    const int b = bh / z.H, h = bh % z.H;
+    const int part = rest % s.parts;
+    const int i0 = ((z.Tq + ROWS - 1) / ROWS - 1 - rest / s.parts) * ROWS;  // under a causal mask the longest first
+    const int w0 = i0 + 32 * wave, i = w0 + col;
+    const int len = keys_of(z, b);
+    const auto end_of = [&](int last) { return z.causal ? max(0, min(len, last + z.start + 1)) : len; };
+    const int block_end = end_of(min(i0 + ROWS, z.Tq) - 1);
+    const int wave_end = w0 < z.Tq ? end_of(min(w0 + 32, z.Tq) - 1) : 0;
+    const int row_end = i < z.Tq ? end_of(i) : 0;
+    const int full = z.mask ? 0 : w0 + 32 <= z.Tq ? end_of(w0) : 0;  // keys below it are seen by the whole wavefront
+    const unsigned long long* mask_row = nullptr;
+    if (z.mask && i < z.Tq) mask_row = z.mask + b * z.mask_stride[0] + h * z.mask_stride[1] + i * z.mask_stride[2];
+    const bool watch = z.causal || z.mask != nullptr;  // what a key holds must not reach a row that does not see it
+
+    float q[16 * DB];  // value 2 n + half of the row
+    {
+        const float* row = query_at(z, b, h, min(i, z.Tq - 1));
+#pragma unroll
+        for (int u = 0; u < 4 * DB; ++u) {
+            const float4 a = four(row, i < z.Tq, 8 * u, z.D, z.quads), c = four(row, i < z.Tq, 8 * u + 4, z.D, z.quads);
+            q[4 * u] = half ? a.y : a.x;
+            q[4 * u + 1] = half ? a.w : a.z;
+            q[4 * u + 2] = half ? c.y : c.x;
+            q[4 * u + 3] = half ? c.w : c.z;
+        }
+    }
+    const int key_row = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);  // the key that row `col` of an operand is
+
+    float4 kn[QUAD_LOADS], vn[QUAD_LOADS];
+    float bn = 0.0f, broken = 0.0f;
+    const float* kbase = key_at(z, b, h, 0);
+    const float* vbase = value_at(z, b, h, 0);
+    const auto load = [&](int j0) {
+#pragma unroll
+        for (int n = 0; n < QUAD_LOADS; ++n) {
+            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4, j = j0 + row;
+            kn[n] = four(kbase + j * z.k_stride[1], j < len, d, z.D, z.quads);
+            vn[n] = four(vbase + j * z.v_stride[1], j < len, d, z.D, z.quads);
+        }
+        if (BIAS && t < TILE + ROWS - 1) {
+            const int c = j0 + t - (ROWS - 1) - i0 + z.Tq - 1;
+            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c] * LOG2E : 0.0f;
+        }
+    };
+    const auto store = [&]() {
+#pragma unroll
+        for (int n = 0; n < QUAD_LOADS; ++n) {
+            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4;
+            float* p = Ks + row * KS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
+            *reinterpret_cast<float2*>(p) = make_float2(kn[n].x, kn[n].z);
+            *reinterpret_cast<float2*>(p + 4) = make_float2(kn[n].y, kn[n].w);
+            *reinterpret_cast<float4*>(Vs + row * DP + d) = vn[n];
+            broken = __builtin_fmaf(vn[n].x, 0.0f, broken);
+            broken = __builtin_fmaf(vn[n].y, 0.0f, broken);
+            broken = __builtin_fmaf(vn[n].z, 0.0f, broken);
+            broken = __builtin_fmaf(vn[n].w, 0.0f, broken);
+        }
+        if (BIAS && t < TILE + ROWS - 1) Bs[t] = bn;
+    };
+
+    const int first_chunk = part * s.a_part, last_chunk = min(s.chunks, first_chunk + s.a_part);
+    const int first_key = first_chunk * CHUNK, last_key = min(last_chunk * CHUNK, block_end);
+    const size_t row_index = (size_t)bh * z.Tq + i;
+    float top = -__builtin_inff(), total = 0.0f;
+    Block16 out[DB];
+#pragma unroll
+    for (int n = 0; n < DB; ++n) out[n] = zero16();
+    if (AHEAD && first_key < last_key) load(first_key);
+    for (int chunk = first_chunk; chunk < last_chunk && chunk * CHUNK < block_end; ++chunk) {
+        float m = -__builtin_inff(), l = 0.0f;
+        Block16 o[DB];
+#pragma unroll
+        for (int n = 0; n < DB; ++n) o[n] = zero16();
+        const int chunk_end = min((chunk + 1) * CHUNK, block_end);
+        for (int j0 = chunk * CHUNK; j0 < chunk_end; j0 += TILE) {
+            if (!AHEAD) load(j0);
+            __syncthreads();
+            store();
+            __syncthreads();
+            if (AHEAD && j0 + TILE < last_key) load(j0 + TILE);
+            if (j0 >= wave_end) continue;
+            Block16 p[2] = {zero16(), zero16()};
+#pragma unroll
+            for (int u = 0; u < 4 * DB; ++u) {
+                float4 a[2];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    a[kb] = *reinterpret_cast<const float4*>(Ks + (32 * kb + key_row) * KS + 8 * u + 4 * half);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+                        p[kb] = mfma(r == 0 ? a[kb].x : r == 1 ? a[kb].y : r == 2 ? a[kb].z : a[kb].w, q[4 * u + r], p[kb]);
+            }
+            // register 4 g + r of block kb: key j0 + 32 kb + 8 g + 2 r + half
+            float next = m;
+            if (BIAS) {
+                const float* bias = Bs + (ROWS - 1 - (i - i0)) + half;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        p[kb][r] = __builtin_fmaf(p[kb][r], z.factor, bias[32 * kb + 8 * (r / 4) + 2 * (r % 4)]);
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) p[kb][r] = p[kb][r] * z.factor;
+            }
+            if (j0 + TILE > full) {
+                const unsigned long long bits = mask_row ? mask_row[j0 >> 6] : ~0ull;
+                const int left = row_end - j0 - half;
+                const uint32_t words[2] = {(uint32_t)(bits >> half), (uint32_t)(bits >> 32) >> half};
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int n = 8 * (r / 4) + 2 * (r % 4);
+                        p[kb][r] = 32 * kb + n < left && (words[kb] >> n & 1) != 0 ? p[kb][r] : -__builtin_inff();
+                    }
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) next = larger(next, p[kb][r]);
+            {
+                uint32_t x, w;
+                halves(__float_as_uint(next), &x, &w);
+                next = larger(__uint_as_float(x), __uint_as_float(w));
+            }
+            const float base = finite_top(next), a = e2(m - base);
+            m = next;
+            l = l * a;
+            if (__any(a != 1.0f)) {
+#pragma unroll
+                for (int n = 0; n < DB; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[n][r] = o[n][r] * a;
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    p[kb][r] = e2(p[kb][r] - base);
+                    l = l + p[kb][r];
+                }
+            if (DROP) {
+                // the four words of a call are four keys': half 0 makes those of keys 0..3 of eight, half 1 of 4..7, and both take
+                // the bits of their parity from each
+                uint32_t bits = 0;
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    const auto w = repro_dropout::pair_words((uint32_t)(j0 / 4 + 2 * g + half), i, bh, seed);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) bits |= (uint32_t)(w.w[n] >= z.threshold) << (4 * g + n);
+                }
+                uint32_t low, high;
+                halves(bits, &low, &high);
+                low >>= half;
+                high >>= half;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int g = 4 * kb + r / 4, n = r % 4;
+                        p[kb][r] = ((n < 2 ? low : high) >> (4 * g + 2 * (n & 1)) & 1) != 0 ? p[kb][r] : 0.0f;
+                    }
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float* v = Vs + (32 * kb + 8 * (r / 4) + 2 * (r % 4) + half) * DP + col;
+#pragma unroll
+                    for (int n = 0; n < DB; ++n) o[n] = mfma(v[32 * n], p[kb][r], o[n]);
+                }
+        }
+        uint32_t x, w;
+        halves(__float_as_uint(l), &x, &w);
+        const float both_l = __uint_as_float(x) + __uint_as_float(w);
+        if (s.parts > 1) {
+            if (i < z.Tq) {
+                float* to = s.o + (row_index * s.chunks + chunk) * z.D;
+#pragma unroll
+                for (int n = 0; n < DB; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int d = 32 * n + 8 * (r / 4) + 4 * half + r % 4;
+                        if (d < z.D) to[d] = o[n][r];
+                    }
+                if (half == 0) s.ml[row_index * s.chunks + chunk] = make_float2(m, both_l);
+            }
+        } else {
+            const float both = larger(top, m), base = finite_top(both), a = e2(top - base), e = e2(m - base);
+            top = both;
+            total = __builtin_fmaf(both_l, e, total * a);
+#pragma unroll
+            for (int n = 0; n < DB; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) out[n][r] = __builtin_fmaf(o[n][r], e, out[n][r] * a);
+        }
+    }
+    if (s.parts > 1 && i < z.Tq && half == 0)
+        for (int chunk = max(first_chunk, (block_end + CHUNK - 1) / CHUNK); chunk < last_chunk; ++chunk)
+            s.ml[row_index * s.chunks + chunk] = make_float2(-__builtin_inff(), -1.0f);
+    const bool again = watch && __syncthreads_or(broken != broken);
+    if (s.parts == 1 && !again) {
+        const float inverse = reciprocal(total), f = DROP ? inverse * z.keep_factor : inverse;
+        if (i < z.Tq) {
+            float* row = y + (((size_t)b * z.Tq + i) * z.H + h) * z.D;
+            const bool whole = z.D % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+#pragma unroll
+            for (int n = 0; n < DB; ++n)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int d = 32 * n + 8 * g + 4 * half;
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = out[n][4 * g + r] * f + 0.0f;
+                    if (whole && d < z.D) {
+                        *reinterpret_cast<float4*>(row + d) = make_float4(v[0], v[1], v[2], v[3]);
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (d + r < z.D) row[d + r] = v[r];
+                    }
+                }
+            if (stats && half == 0) {
+                stats[2 * row_index] = finite_top(top);
+                stats[2 * row_index + 1] = inverse;
+            }
+        }
+    }
+    if (!again) return;
+    // A NaN or infinity among these values, which the products' zeros would hand to rows that do not see it: row by row.
+    for (int row = i0 + wave; row < i0 + ROWS && row < z.Tq; row += 4) {
+        const int end = key_end(z, b, row);
+        const size_t n = (size_t)bh * z.Tq + row;
+        Joined all;
+        for (int chunk = first_chunk; chunk < last_chunk && chunk * CHUNK < block_end; ++chunk) {
+            const RowChunk r = row_chunk(z, seed, b, h, row, chunk * CHUNK, end, lane);
+            if (s.parts > 1) {
+                float* to = s.o + (n * s.chunks + chunk) * z.D;
+                if (lane < z.D) to[lane] = r.o0;
+                if (lane + 64 < z.D) to[lane + 64] = r.o1;
+                if (lane == 0) s.ml[n * s.chunks + chunk] = make_float2(r.m, r.even + r.odd);
+            } else {
+                all.join(r);
+            }
+        }
+        if (s.parts == 1) finish_row(z, all, b, h, row, lane, y, stats);
+    }
+}
+
+// Joins the chunks of a row in their order: a wavefront takes a row, first a lane a chunk (the maxima before it and the
+// two factors), then a lane a value.
+__global__ void __launch_bounds__(256)
+join_chunks(Problem z, Parts s, float* y, float* stats) {
+    const int lane = threadIdx.x & 63;
+    const long long rows = (long long)z.B * z.H * z.Tq;
+    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
+        const int i = (int)(n % z.Tq), bh = (int)(n / z.Tq);
+        Joined all;
+        for (int first = 0; first < s.chunks; first += 64) {
+            const int c = first + lane;
+            const float2 ml = c < s.chunks ? s.ml[n * s.chunks + c] : make_float2(-__builtin_inff(), -1.0f);
+            const bool there = ml.y != -1.0f;
+            float run = ml.x;  // the largest of the chunks up to this one
+#pragma unroll
+            for (int step = 1; step < 64; step *= 2) {
+                const float before = __shfl_up(run, step, 64);
+                if (lane >= step) run = larger(before, run);
+            }
+            run = larger(all.top, run);
+            float before = __shfl_up(run, 1, 64);
+            if (lane == 0) before = all.top;
+            const float base = finite_top(run);
+            const float a = there ? e2(before - base) : 1.0f, e = there ? e2(ml.x - base) : 0.0f;
+            const unsigned long long which = __ballot(there);
+            all.top = __shfl(run, 63, 64);
+            const float* o = s.o + (n * s.chunks + first) * z.D;
+            const int count = min(64, s.chunks - first);
+#pragma unroll 8
+            for (int k = 0; k < count; ++k) {
+                const float ak = __shfl(a, k, 64), ek = __shfl(e, k, 64), lk = __shfl(ml.y, k, 64);
+                if ((which >> k & 1) == 0) continue;
+                const float o0 = lane < z.D ? o[(size_t)k * z.D + lane] : 0.0f;
+                const float o1 = lane + 64 < z.D ? o[(size_t)k * z.D + lane + 64] : 0.0f;
+                all.total = __builtin_fmaf(lk, ek, all.total * ak);
+                all.o0 = __builtin_fmaf(o0, ek, all.o0 * ak);
+                all.o1 = __builtin_fmaf(o1, ek, all.o1 * ak);
+            }
+        }
+        finish_row(z, all, bh / z.H, bh % z.H, i, lane, y, stats);
+    }
+}
+
+// The keys are split over blocks where the queries alone leave compute units idle: as many parts as bring the grid to two
+// blocks a compute unit, whole chunks each, as long as the chunks' results take at most a quarter of a gigabyte.
+Parts parts_of(const Problem& z) {
+    Parts s;
+    s.chunks = (z.Tk + CHUNK - 1) / CHUNK;
+    const long long blocks = (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS);
+    long long parts = blocks > 0 ? (512 + blocks - 1) / blocks : 1;
+    if (blocks > 384 || (long long)z.B * z.H * z.Tq * s.chunks * (z.D + 2) > (1ll << 26)) parts = 1;
+    if (parts > s.chunks) parts = s.chunks;
+    s.a_part = parts > 0 ? (int)((s.chunks + parts - 1) / parts) : 0;
+    s.parts = s.a_part > 0 ? (s.chunks + s.a_part - 1) / s.a_part : 1;
+    if (s.parts == 1) s.a_part = s.chunks;
+    s.ml = nullptr;
+    s.o = nullptr;
+    return s;
+}
+
+}  // namespace
+
+size_t forward_workspace(const Problem& z) {
+    const Parts s = parts_of(z);
+    return s.parts > 1 ? (size_t)z.B * z.H * z.Tq * s.chunks * (z.D + 2) * sizeof(float) : 0;
+}
+
+int forward(const Problem& z, float* y, float* stats, unsigned long long* used, void* workspace, hipStream_t stream) {
+    Parts s = parts_of(z);
+    const long long rows = (long long)z.B * z.H * z.Tq;
+    if (s.parts > 1) {
+        s.ml = static_cast<float2*>(workspace);
+        s.o = static_cast<float*>(workspace) + 2 * rows * s.chunks;
+    }
+    const long long blocks = (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
+    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
+    with_size(z.D, [&](auto db) {
+        with_flags(z.bias != nullptr, z.threshold != 0, [&](auto bias, auto drop) {
+            hipLaunchKernelGGL((forward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
+        });
+    });
+    int rc = hipGetLastError();
+    if (rc == hipSuccess && s.parts > 1) {
+        hipLaunchKernelGGL(join_chunks, dim3(grid_of(rows, 4)), dim3(256), 0, stream, z, s, y, stats);
+        rc = hipGetLastError();
+    }
+    return rc;
+}
+
+}  // namespace attention
+}  // namespace rg

@@ -6,6 +6,7 @@
 #include "repro_attention_math.h"
 #include "repro_dropout_math.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace rg {
@@ -236,6 +237,10 @@ void with_flags(bool a, bool b, F run) {
 
 size_t forward_workspace(const Problem& z);
 int forward(const Problem& z, float* y, float* stats, unsigned long long* used, void* workspace, hipStream_t stream);
+// For at least one query and one key; the workspace starts with the rows' deltas.
+size_t backward_workspace(const Problem& z, bool want_bias);
+int backward(const Problem& z, const float* dy, const float* stats, float* dq, float* dk, float* dv, float* dbias, void* workspace,
+             hipStream_t stream);
 
 }  // namespace attention
 }  // namespace rg

@@ -36,73 +36,8 @@ row_deltas(Problem z, const float* dy, const float* y, float* delta) {
 }
 
 __global__ void __launch_bounds__(256)
-backward_keys(Problem z, Gradients g, float* dk, float* dv) {
-    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
-    const int lane = threadIdx.x & 63;
-    const long long rows = (long long)z.B * z.KVH * z.Tk;
-    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
-        const int j = (int)(n % z.Tk), kvh = (int)(n / z.Tk % z.KVH), b = (int)(n / z.Tk / z.KVH);
-        KeyPart s = {};
-        for (int h = kvh * z.group; h < (kvh + 1) * z.group; ++h)
-            for (int first = 0; first < z.Tq; first += QUERY_CHUNK) {
-                const KeyPart p = key_part(z, g, seed, b, h, j, first, lane);
-                s.v0 = s.v0 + p.v0, s.v1 = s.v1 + p.v1, s.k0 = s.k0 + p.k0, s.k1 = s.k1 + p.k1;
-            }
-        const size_t at = (((size_t)b * z.Tk + j) * z.KVH + kvh) * z.D;
-        if (lane < z.D) {
-            dv[at + lane] = s.v0 + 0.0f;
-            dk[at + lane] = s.k0 * z.scale + 0.0f;
-        }
-        if (lane + 64 < z.D) {
-            dv[at + lane + 64] = s.v1 + 0.0f;
-            dk[at + lane + 64] = s.k1 * z.scale + 0.0f;
-        }
-    }
-}
-
-__global__ void __launch_bounds__(256)
-backward_queries(Problem z, Gradients g, float* dq) {
-    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
-    const int lane = threadIdx.x & 63;
-    const long long rows = (long long)z.B * z.H * z.Tq;
-    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
-        const int i = (int)(n % z.Tq), t = (int)(n / z.Tq), b = t / z.H, h = t % z.H;
-        const int end = key_end(z, b, i);
-        float s0 = 0.0f, s1 = 0.0f;
-        for (int first = 0; first < end; first += KEY_BLOCK) {
-            const QueryPart p = query_part(z, g, seed, b, h, i, first, end, lane);
-            s0 = s0 + p.q0, s1 = s1 + p.q1;
-        }
-        const size_t at = (((size_t)b * z.Tq + i) * z.H + h) * z.D;
-        if (lane < z.D) dq[at + lane] = s0 * z.scale + 0.0f;
-        if (lane + 64 < z.D) dq[at + lane + 64] = s1 * z.scale + 0.0f;
-    }
-}
-
-// The bias's gradient: a thread a distance of a head.
-__global__ void __launch_bounds__(256)
-backward_bias(Problem z, Gradients g, float* dbias) {
-    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
-    const int columns = z.Tq + z.Tk - 1;
-    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < (long long)z.H * columns; n += (long long)gridDim.x * 256) {
-        const int h = (int)(n / columns), away = (int)(n % columns) - (z.Tq - 1);
-        float s = 0.0f;
-        for (int b = 0; b < z.B; ++b)
-            for (int block = 0; block < z.Tk; block += KEY_BLOCK)
-                for (int first = 0; first < z.Tq; first += QUERY_CHUNK) {
-                    const int high = min(block + KEY_BLOCK, z.Tk);
-                    int i = max(first, block - away);
-                    const int last = min(min(first + QUERY_CHUNK, z.Tq), high - away);
-                    if (i >= last) continue;
-                    float part = 0.0f;
-                    for (; i < last; ++i) {
-                        const Pair w = pair(z, g, seed, b, h, i, i + away, seen(z, b, h, i, i + away, key_end(z, b, i)));
-                        part = part + w.ds;
-                    }
-                    s = s + part;
-                }
-        dbias[n] = s + 0.0f;
-    }
+clear(float* p, size_t n) {
+    for (size_t at = (size_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (size_t)gridDim.x * 256) p[at] = 0.0f;
 }
 
 namespace {
@@ -207,9 +142,9 @@ int rg_attention_fp32(const rg_attention_config* cfg, const float* q, const floa
 
 int rg_attention_grad_workspace(const rg_attention_config* cfg, int want_bias, size_t* bytes) {
     using namespace rg::attention;
-    (void)want_bias;
     if (!sizes_ok(cfg) || !bytes) return hipErrorInvalidValue;
-    *bytes = (size_t)(cfg->B * cfg->H * cfg->Tq) * sizeof(float);
+    const Problem z = problem_of(cfg, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr);
+    *bytes = z.B > 0 && z.Tq > 0 && z.Tk > 0 ? backward_workspace(z, want_bias != 0) : 0;
     return hipSuccess;
 }
 
@@ -228,17 +163,20 @@ int rg_attention_grad_fp32(const rg_attention_config* cfg, const float* dy, cons
         (needed > 0 && (!workspace || workspace_bytes < needed || off(workspace, 16))))
         return hipErrorInvalidValue;
     const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at);
-    const Gradients g{dy, stats, static_cast<float*>(workspace)};
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (rows > 0) {
-        hipLaunchKernelGGL(row_deltas, dim3(grid_of(rows, 4)), dim3(256), 0, st, z, dy, y, static_cast<float*>(workspace));
-        hipLaunchKernelGGL(backward_queries, dim3(grid_of(rows, 4)), dim3(256), 0, st, z, g, dq);
+    const long long columns = drelative_bias ? (long long)z.H * (z.Tq + z.Tk - 1) : 0;
+    if (rows == 0 || keys == 0) {  // no pair: zeros
+        const auto zero = [&](float* p, long long n) {
+            if (p && n > 0) hipLaunchKernelGGL(clear, dim3(grid_of(n, 256)), dim3(256), 0, st, p, (size_t)n);
+        };
+        zero(dq, rows * z.D);
+        zero(dk, keys * z.D);
+        zero(dv, keys * z.D);
+        zero(drelative_bias, columns);
+        return hipGetLastError();
     }
-    if (keys > 0) hipLaunchKernelGGL(backward_keys, dim3(grid_of(keys, 4)), dim3(256), 0, st, z, g, dk, dv);
-    if (drelative_bias && z.Tq + z.Tk > 1)
-        hipLaunchKernelGGL(backward_bias, dim3(grid_of((long long)z.H * (z.Tq + z.Tk - 1), 256)), dim3(256), 0, st, z, g,
-                           drelative_bias);
-    return hipGetLastError();
+    hipLaunchKernelGGL(row_deltas, dim3(grid_of(rows, 4)), dim3(256), 0, st, z, dy, y, static_cast<float*>(workspace));
+    return backward(z, dy, stats, dq, dk, dv, drelative_bias, workspace, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,524 @@
+// The attention's gradients on the matrix cores.
+//
+// A block takes 128 keys of a head, 32 a wavefront, and goes through the queries 32 at a time, which its wavefronts share in LDS:
+// S = Q K^T and dP = dY V^T with queries as rows (row 8 g + 4 h + r is query 8 g + 2 r + h, as in the forward pass), so a
+// register of P or dS is the operand of dV^T = dY^T P and dK^T = Q^T dS for two successive queries. K and V stay in registers, as
+// the operands of the first two, and K in LDS for dQ = dS K, which needs dS along its rows: it goes through LDS, and the wavefronts
+// share the tile's 32 rows of dQ by 16 x 16 blocks over all 128 keys (v_mfma_f32_16x16x4_f32: four products in ascending order).
+//
+// dQ's sum over key blocks is taken from what each block leaves (no atomics, whose order would vary): 4 D bytes a query and
+// block written and read beside the 5 x 128 x D multiply-adds that make them. Sums of chunks of 256 queries go to dK
+// and dV as they are done, or stay apart where the queries are split over blocks.
+#include "rg_attention.h"
+
+namespace rg {
+namespace attention {
+namespace {
+
+typedef float Block16 __attribute__((ext_vector_type(16)));
+typedef float Block4 __attribute__((ext_vector_type(4)));
+
+constexpr int STEP = 32;                              // queries at a time
+constexpr int DIAGONALS = KEY_BLOCK + QUERY_CHUNK;    // distances of a block and chunk, one more than there are
+constexpr int DS_STRIDE = KEY_BLOCK + 4;
+
+__device__ __forceinline__ Block16 zero16() {
+    Block16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    return z;
+}
+__device__ __forceinline__ Block16 mfma(float a, float b, Block16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float part_of(const float4& v, int r) { return r == 0 ? v.x : r == 1 ? v.y : r == 2 ? v.z : v.w; }
+
+// Where a block and chunk are, and what they leave. Key blocks first .. first + count of the `blocks`.
+struct Work {
+    int first, count, chunks, parts, a_part;
+    int direct;                 // dk and dv are the results themselves, [B][Tk][KVH][D], else [chunk or 1][B][H][Tk][D]
+    float *dk, *dv;
+    float* dq;                  // [count][B][H][Tq][D]
+    float* diagonals;           // [B][H][count][chunks][DIAGONALS], or null
+};
+
+__device__ __forceinline__ int last_end(const Problem& z, int len, int i) {
+    return z.causal ? max(0, min(len, i + z.start + 1)) : len;
+}
+// Whether a key block's keys are seen by a query before `rows` (the mask aside).
+__device__ __forceinline__ bool live(const Problem& z, int len, int block, int rows) {
+    return block * KEY_BLOCK < last_end(z, len, min(rows, z.Tq) - 1);
+}
+
+template <int DB, bool BIAS, bool DROP>
+__global__ void __launch_bounds__(256, DB <= 2 ? 2 : 1)
+backward_tiles(Problem z, Gradients g, Work w) {
+    constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 16;
+    __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds[STEP * DS_STRIDE];
+    __shared__ float Bs[BIAS ? 160 : 1], Sums[BIAS ? DIAGONALS : 1];
+    __shared__ float4 Rows[STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits
+    __shared__ uint32_t Masks[STEP][4];
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5, wave = t >> 6;
+    const int heads = z.B * z.H, bh = (int)(blockIdx.x % heads), rest = (int)(blockIdx.x / heads);
+    const int b = bh / z.H, h = bh % z.H, part = rest % w.parts;
+    const int slot = rest / w.parts, block = w.first + slot, k0 = block * KEY_BLOCK;
+    const int len = keys_of(z, b), key = k0 + 32 * wave + col;
+    const size_t row0 = (size_t)bh * z.Tq;
+    const size_t out_row = w.direct ? ((size_t)b * z.Tk * z.KVH + h) * z.D : (size_t)bh * z.Tk * z.D;
+    const size_t out_stride = (size_t)(w.direct ? z.KVH : 1) * z.D;
+    const bool whole = z.D % 4 == 0;
+
+    if (!live(z, len, block, z.Tq)) {
+        if (w.direct && part == 0)
+            for (int at = t; at < KEY_BLOCK * z.D; at += 256)
+                if (k0 + at / z.D < z.Tk) {
+                    w.dk[out_row + (k0 + at / z.D) * out_stride + at % z.D] = 0.0f;
+                    w.dv[out_row + (k0 + at / z.D) * out_stride + at % z.D] = 0.0f;
+                }
+        return;
+    }
+
+    float k[16 * DB], v[16 * DB];  // value 2 n + half of the lane's key
+    float broken_key = 0.0f;
+    const auto four = [&](const float* row, bool there, int d) {
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (!there || d >= z.D) return x;
+        if (z.quads) return *reinterpret_cast<const float4*>(row + d);
+        x.x = row[d];
+        if (d + 1 < z.D) x.y = row[d + 1];
+        if (d + 2 < z.D) x.z = row[d + 2];
+        if (d + 3 < z.D) x.w = row[d + 3];
+        return x;
+    };
+    const auto keys_to_lds = [&](const float* base, long long stride) {
+#pragma unroll
+        for (int n = 0; n < 4 * DB; ++n) {
+            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4;
+            *reinterpret_cast<float4*>(Ks + row * KS + d) = four(base + (k0 + row) * stride, k0 + row < len, d);
+        }
+    };
+    const auto take = [&](float* to) {
+#pragma unroll
+        for (int n = 0; n < 8 * DB; ++n) {
+            const float4 x = *reinterpret_cast<const float4*>(Ks + (32 * wave + col) * KS + 4 * n);
+            to[2 * n] = half ? x.y : x.x;
+            to[2 * n + 1] = half ? x.w : x.z;
+        }
+    };
+    keys_to_lds(value_at(z, b, h, 0), z.v_stride[1]);
+    __syncthreads();
+    take(v);
+    __syncthreads();
+    keys_to_lds(key_at(z, b, h, 0), z.k_stride[1]);
+    __syncthreads();
+    take(k);
+#pragma unroll
+    for (int n = 0; n < 16 * DB; ++n) broken_key = __builtin_fmaf(k[n], 0.0f, broken_key);
+
+    const float* qbase = query_at(z, b, h, 0);
+    const float* ybase = g.dy + ((size_t)b * z.Tq * z.H + h) * z.D;
+    const size_t ystride = (size_t)z.H * z.D;
+    const bool ywhole = whole && (reinterpret_cast<uintptr_t>(g.dy) & 15) == 0;
+    const bool watch = z.causal || z.mask || k0 + KEY_BLOCK > len;  // a query's values must not reach keys that it does not see
+    float4 qn[DB], yn[DB];
+    float broken = 0.0f, bn = 0.0f;
+    float4 rn;
+    uint32_t mn = 0;
+    const auto load = [&](int i0) {
+#pragma unroll
+        for (int n = 0; n < DB; ++n) {
+            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4, i = i0 + row;
+            qn[n] = four(qbase + i * z.q_stride[1], i < z.Tq, d);
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i < z.Tq && d < z.D) {
+                const float* p = ybase + i * ystride + d;
+                if (ywhole) {
+                    x = *reinterpret_cast<const float4*>(p);
+                } else {
+                    x.x = p[0];
+                    if (d + 1 < z.D) x.y = p[1];
+                    if (d + 2 < z.D) x.z = p[2];
+                    if (d + 3 < z.D) x.w = p[3];
+                }
+            }
+            yn[n] = x;
+        }
+        if (t < STEP) {
+            const int i = i0 + t;
+            rn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (i < z.Tq) {
+                rn.x = g.stats[2 * (row0 + i)];
+                rn.y = g.stats[2 * (row0 + i) + 1];
+                rn.z = g.delta[row0 + i];
+                rn.w = __int_as_float(last_end(z, len, i));
+            }
+        } else if (t >= 64 && t < 64 + 4 * STEP) {
+            const int i = i0 + (t - 64) / 4, word = k0 / 32 + (t & 3);
+            mn = ~0u;
+            if (z.mask && i < z.Tq && word * 32 < z.Tk) {
+                const unsigned long long* row = z.mask + b * z.mask_stride[0] + h * z.mask_stride[1] + i * z.mask_stride[2];
+                mn = (uint32_t)(row[word >> 1] >> (32 * (word & 1)));
+            }
+        }
+        if (BIAS && t < KEY_BLOCK + STEP - 1) {
+            const int c = k0 + t - (STEP - 1) - i0 + z.Tq - 1;
+            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c] * LOG2E : 0.0f;
+        }
+    };
+    const auto store = [&]() {
+#pragma unroll
+        for (int n = 0; n < DB; ++n) {
+            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4;
+            const int to = row * QS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
+            *reinterpret_cast<float2*>(Qs + to) = make_float2(qn[n].x, qn[n].z);
+            *reinterpret_cast<float2*>(Qs + to + 4) = make_float2(qn[n].y, qn[n].w);
+            *reinterpret_cast<float2*>(Ys + to) = make_float2(yn[n].x, yn[n].z);
+            *reinterpret_cast<float2*>(Ys + to + 4) = make_float2(yn[n].y, yn[n].w);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                broken = __builtin_fmaf(part_of(qn[n], r), 0.0f, broken);
+                broken = __builtin_fmaf(part_of(yn[n], r), 0.0f, broken);
+            }
+        }
+        if (t < STEP) Rows[t] = rn;
+        else if (t >= 64 && t < 64 + 4 * STEP) Masks[(t - 64) / 4][t & 3] = mn;
+        if (BIAS && t < KEY_BLOCK + STEP - 1) Bs[t] = bn;
+    };
+    const int row_of = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);     // the query that row `col` of an operand is
+    const int place_of = (col & 24) + 4 * (col & 1) + ((col >> 1) & 3);   // where value `col` of 32 is in Qs and Ys
+    const int ds_place = 32 * wave + (col & 16) + 4 * (col & 3) + ((col >> 2) & 3);  // where a key is in Ds: 4 s + c of 16 at 4 c + s
+
+    const int first_chunk = part * w.a_part, last_chunk = min(w.chunks, first_chunk + w.a_part);
+    bool begun = false;
+    for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
+        const int c0 = chunk * QUERY_CHUNK, c1 = min(c0 + QUERY_CHUNK, z.Tq);
+        if (!live(z, len, block, c1)) continue;
+        float* diagonals = BIAS && w.diagonals ? w.diagonals + (((size_t)bh * w.count + slot) * w.chunks + chunk) * DIAGONALS : nullptr;
+        Block16 dk[DB], dv[DB];
+#pragma unroll
+        for (int n = 0; n < DB; ++n) dk[n] = dv[n] = zero16();
+        int i0 = c0;
+        while (!live(z, len, block, i0 + STEP)) i0 += STEP;  // (the chunk's last step is live)
+        __syncthreads();
+        broken = 0.0f;
+        load(i0);
+        store();
+        if (BIAS)
+            for (int n = t; n < DIAGONALS; n += 256) Sums[n] = 0.0f;
+        __syncthreads();
+        for (; i0 < c1; i0 += STEP) {
+            const bool more = i0 + STEP < c1;
+            if (more) load(i0 + STEP);
+            Block16 s = zero16(), dp = zero16();
+#pragma unroll
+            for (int u = 0; u < 4 * DB; ++u) {
+                const float4 a = *reinterpret_cast<const float4*>(Qs + row_of * QS + 8 * u + 4 * half);
+                const float4 c = *reinterpret_cast<const float4*>(Ys + row_of * QS + 8 * u + 4 * half);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s = mfma(part_of(a, r), k[4 * u + r], s);
+                    dp = mfma(part_of(c, r), v[4 * u + r], dp);
+                }
+            }
+            uint32_t keep[4];
+            if (DROP) {
+                // a call's four words are four keys', neighbours in a quad of lanes: each makes those of another query
+                uint32_t bits = 0;
+                const int r = lane & 3;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const auto x = repro_dropout::pair_words((uint32_t)(key >> 2), i0 + 8 * n + 2 * r + half, bh, seed);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) bits |= (uint32_t)(x.w[q] >= z.threshold) << (4 * n + q);
+                }
+                keep[0] = __builtin_amdgcn_update_dpp(0, bits, 0x00, 0xF, 0xF, true) >> r;
+                keep[1] = __builtin_amdgcn_update_dpp(0, bits, 0x55, 0xF, 0xF, true) >> r;
+                keep[2] = __builtin_amdgcn_update_dpp(0, bits, 0xAA, 0xF, 0xF, true) >> r;
+                keep[3] = __builtin_amdgcn_update_dpp(0, bits, 0xFF, 0xF, 0xF, true) >> r;
+            }
+            // whether every pair of the wavefront's is seen
+            const bool inner = !z.mask && i0 + STEP <= z.Tq && k0 + 32 * wave + 32 <= last_end(z, len, i0);
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                const int q = 8 * (n / 4) + 2 * (n % 4) + half;
+                const float4 row = Rows[q];
+                const float x = BIAS ? __builtin_fmaf(s[n], z.factor, Bs[32 * wave + col - q + STEP - 1]) : s[n] * z.factor;
+                float p = e2(x - row.x) * row.y, d = dp[n], u = p;
+                if (DROP) {
+                    const bool kept = (keep[n % 4] >> (4 * (n / 4)) & 1) != 0;
+                    u = kept ? p * z.keep_factor : 0.0f;
+                    d = kept ? d * z.keep_factor : 0.0f;
+                }
+                d = ds_of(p, d, row.z);
+                if (!inner) {
+                    const bool see = key < __float_as_int(row.w) && (Masks[q][wave] >> col & 1) != 0;
+                    u = see ? u : 0.0f;
+                    d = see ? d : 0.0f;
+                }
+                s[n] = u;
+                dp[n] = d;
+                Ds[q * DS_STRIDE + ds_place] = d;
+            }
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                const int q = 8 * (n / 4) + 2 * (n % 4) + half;
+#pragma unroll
+                for (int x = 0; x < DB; ++x) {
+                    dv[x] = mfma(Ys[q * QS + 32 * x + place_of], s[n], dv[x]);
+                    dk[x] = mfma(Qs[q * QS + 32 * x + place_of], dp[n], dk[x]);
+                }
+            }
+            __syncthreads();
+            if (more) store();
+            {
+                const int c16 = lane & 15, group = lane >> 4, q0 = 16 * (wave & 1), d0 = 16 * DB * (wave >> 1);
+                Block4 dq[DB];
+#pragma unroll
+                for (int x = 0; x < DB; ++x) dq[x] = Block4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int n = 0; n < KEY_BLOCK / 16; ++n) {
+                    const float4 a = *reinterpret_cast<const float4*>(Ds + (q0 + c16) * DS_STRIDE + 16 * n + 4 * group);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int x = 0; x < DB; ++x)
+                            dq[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(part_of(a, r), Ks[(16 * n + 4 * r + group) * KS + d0 + 16 * x + c16],
+                                                                        dq[x], 0, 0, 0);
+                }
+                float* to = w.dq + ((size_t)slot * heads * z.Tq + row0 + i0 + q0 + 4 * group) * z.D;
+#pragma unroll
+                for (int x = 0; x < DB; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int d = d0 + 16 * x + c16;
+                        if (i0 + q0 + 4 * group + r < z.Tq && d < z.D) to[(size_t)r * z.D + d] = dq[x][r];
+                    }
+            }
+            if (BIAS && w.diagonals && t < KEY_BLOCK + STEP - 1) {
+                float* sum = Sums + t - (STEP - 1) - (i0 - c0) + QUERY_CHUNK - 1;
+                float x = *sum;
+                for (int q = 0; q < STEP; ++q) {
+                    const int c = t - (STEP - 1) + q;
+                    if (c >= 0 && c < KEY_BLOCK) x = x + Ds[q * DS_STRIDE + (c & ~15) + 4 * (c & 3) + ((c >> 2) & 3)];
+                }
+                *sum = x;
+            }
+            __syncthreads();
+        }
+        const bool again = watch && __syncthreads_or(broken != broken || broken_key != broken_key);
+        const bool last = w.direct && chunk == w.chunks - 1;
+        const size_t chunk_out = out_row + (w.parts > 1 ? (size_t)chunk * heads * z.Tk * z.D : 0);
+        const bool add = w.parts == 1 && begun;
+        begun = true;
+        if (!again) {
+            if (key < z.Tk) {
+                float* kd = w.dk + chunk_out + key * out_stride;
+                float* vd = w.dv + chunk_out + key * out_stride;
+#pragma unroll
+                for (int x = 0; x < DB; ++x)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const int d = 32 * x + 8 * n + 4 * half;
+                        if (d >= z.D) continue;
+                        float a[4], c[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) a[r] = dk[x][4 * n + r], c[r] = dv[x][4 * n + r];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if (d + r >= z.D) continue;
+                            if (add) a[r] = kd[d + r] + a[r], c[r] = vd[d + r] + c[r];
+                            if (last) a[r] = a[r] * z.scale + 0.0f, c[r] = c[r] + 0.0f;
+                            kd[d + r] = a[r];
+                            vd[d + r] = c[r];
+                        }
+                    }
+            }
+            if (diagonals)
+                for (int n = t; n < DIAGONALS; n += 256) diagonals[n] = Sums[n];
+            continue;
+        }
+        // A NaN or infinity that the products' zeros would hand to pairs that are not seen: key by key, row by row.
+        for (int n = wave; n < KEY_BLOCK && k0 + n < z.Tk; n += 4) {
+            const KeyPart r = key_part(z, g, seed, b, h, k0 + n, c0, lane);
+            float* kd = w.dk + chunk_out + (k0 + n) * out_stride;
+            float* vd = w.dv + chunk_out + (k0 + n) * out_stride;
+            for (int x = 0; x < 2; ++x) {
+                const int d = lane + 64 * x;
+                if (d >= z.D) continue;
+                float a = x ? r.k1 : r.k0, c = x ? r.v1 : r.v0;
+                if (add) a = kd[d] + a, c = vd[d] + c;
+                if (last) a = a * z.scale + 0.0f, c = c + 0.0f;
+                kd[d] = a;
+                vd[d] = c;
+            }
+        }
+        for (int i = c0 + wave; i < c1; i += 4) {
+            const QueryPart r = query_part(z, g, seed, b, h, i, k0, last_end(z, len, i), lane);
+            float* to = w.dq + ((size_t)slot * heads * z.Tq + row0 + i) * z.D;
+            if (lane < z.D) to[lane] = r.q0;
+            if (lane + 64 < z.D) to[lane + 64] = r.q1;
+        }
+        if (diagonals)
+            for (int n = t; n < DIAGONALS; n += 256) {
+                const int away = n - (QUERY_CHUNK - 1);  // key in the block less query in the chunk
+                float x = 0.0f;
+                for (int i = max(0, -away); i < c1 - c0 && i + away < KEY_BLOCK; ++i) {
+                    const int j = k0 + i + away;
+                    x = x + pair(z, g, seed, b, h, c0 + i, j, seen(z, b, h, c0 + i, j, last_end(z, len, c0 + i))).ds;
+                }
+                diagonals[n] = x;
+            }
+        __syncthreads();
+    }
+}
+
+// dq = (what it is) + the key blocks' shares, in their order; the first time 0, the last time times scale.
+__global__ void __launch_bounds__(256)
+sum_queries(Problem z, Work w, float* dq, int begins, int ends) {
+    const long long rows = (long long)z.B * z.H * z.Tq;
+    const int wide = (z.D + 63) / 64 * 64;  // a row takes whole wavefronts
+    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < rows * wide; n += (long long)gridDim.x * 256) {
+        const long long row = n / wide;
+        const int d = (int)(n % wide), i = (int)(row % z.Tq), bh = (int)(row / z.Tq);
+        if (d >= z.D) continue;
+        float* to = dq + (((size_t)(bh / z.H) * z.Tq + i) * z.H + bh % z.H) * z.D + d;
+        const int end = last_end(z, keys_of(z, bh / z.H), i);
+        float s = begins ? 0.0f : *to;
+        const float* p = w.dq + (size_t)row * z.D + d;
+        const size_t apart = (size_t)rows * z.D;
+        const int blocks = min(w.count, (end + KEY_BLOCK - 1) / KEY_BLOCK - w.first);
+#pragma unroll 4
+        for (int k = 0; k < blocks; ++k) s = s + p[k * apart];
+        *to = ends ? s * z.scale + 0.0f : s;
+    }
+}
+
+// dk and dv from the heads' (and, where they are apart, the chunks') sums.
+__global__ void __launch_bounds__(256)
+sum_keys(Problem z, Work w, float* dk, float* dv) {
+    const int j0 = w.first * KEY_BLOCK, keys = min(z.Tk - j0, w.count * KEY_BLOCK);
+    const long long count = (long long)z.B * keys * z.KVH * z.D;
+    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < count; n += (long long)gridDim.x * 256) {
+        const int d = (int)(n % z.D), kvh = (int)(n / z.D % z.KVH), j = j0 + (int)(n / z.D / z.KVH % keys);
+        const int b = (int)(n / z.D / z.KVH / keys), len = keys_of(z, b);
+        float sk = 0.0f, sv = 0.0f;
+        for (int h = kvh * z.group; h < (kvh + 1) * z.group; ++h) {
+            float ck = 0.0f, cv = 0.0f;
+            for (int c = 0; c < (w.parts > 1 ? w.chunks : 1); ++c) {
+                if (!live(z, len, j / KEY_BLOCK, w.parts > 1 ? (c + 1) * QUERY_CHUNK : z.Tq)) continue;
+                const size_t at = ((((size_t)c * z.B + b) * z.H + h) * z.Tk + j) * z.D + d;
+                ck = ck + w.dk[at];
+                cv = cv + w.dv[at];
+            }
+            sk = sk + ck;
+            sv = sv + cv;
+        }
+        const size_t to = (((size_t)b * z.Tk + j) * z.KVH + kvh) * z.D + d;
+        dk[to] = sk * z.scale + 0.0f;
+        dv[to] = sv + 0.0f;
+    }
+}
+
+// The bias's gradient: a thread a distance of a head, over the key blocks, the batch and the chunks.
+__global__ void __launch_bounds__(256)
+sum_diagonals(Problem z, Work w, float* dbias, int begins, int ends) {
+    const int columns = z.Tq + z.Tk - 1;
+    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < (long long)z.H * columns; n += (long long)gridDim.x * 256) {
+        const int h = (int)(n / columns), away = (int)(n % columns) - (z.Tq - 1);
+        float s = begins ? 0.0f : dbias[n];
+        for (int slot = 0; slot < w.count; ++slot) {
+            const int k0 = (w.first + slot) * KEY_BLOCK;
+            const int low = max(0, k0 - away), high = min(z.Tq, min(k0 + KEY_BLOCK, z.Tk) - away);  // the queries
+            if (low >= high) continue;
+            for (int b = 0; b < z.B; ++b) {
+                const int len = keys_of(z, b);
+                for (int chunk = low / QUERY_CHUNK; chunk * QUERY_CHUNK < high; ++chunk) {
+                    if (!live(z, len, w.first + slot, (chunk + 1) * QUERY_CHUNK)) continue;
+                    const float* p = w.diagonals + ((((size_t)b * z.H + h) * w.count + slot) * w.chunks + chunk) * DIAGONALS;
+                    s = s + p[away - k0 + chunk * QUERY_CHUNK + QUERY_CHUNK - 1];
+                }
+            }
+        }
+        dbias[n] = ends ? s + 0.0f : s;
+    }
+}
+
+// How the key blocks are taken: as many at a time as leave at most a gigabyte for dQ and half of one for the bias; the queries split
+// over blocks, whole chunks each, where the key blocks alone leave compute units idle and the chunks' results stay below
+// half a gigabyte.
+struct Plan {
+    Work w;
+    int blocks;
+    size_t delta, kv, dq, diagonals, bytes;  // workspace: offsets, and its size
+};
+
+size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+Plan plan_of(const Problem& z, bool want_bias) {
+    Plan p{};
+    const size_t rows = (size_t)z.B * z.H * z.Tq, a_block = rows * z.D * sizeof(float), keys = (size_t)z.B * z.H * z.Tk * z.D * sizeof(float);
+    p.blocks = (z.Tk + KEY_BLOCK - 1) / KEY_BLOCK;
+    p.w.chunks = (z.Tq + QUERY_CHUNK - 1) / QUERY_CHUNK;
+    const size_t diagonals = want_bias ? (size_t)z.B * z.H * p.w.chunks * DIAGONALS * sizeof(float) : 0;
+    size_t at_a_time = a_block > 0 ? (1u << 30) / a_block : 1;
+    if (diagonals > 0) at_a_time = std::min(at_a_time, (size_t)(1 << 29) / diagonals);
+    p.w.count = (int)std::min(std::max<size_t>(at_a_time, 1), (size_t)p.blocks);
+    const long long grid = (long long)z.B * z.H * p.w.count;
+    long long parts = grid > 0 && grid < 384 ? (512 + grid - 1) / grid : 1;
+    if (keys * 2 * p.w.chunks > (1u << 29)) parts = 1;
+    if (parts > p.w.chunks) parts = p.w.chunks;
+    p.w.a_part = parts > 0 ? (int)((p.w.chunks + parts - 1) / parts) : 0;
+    p.w.parts = p.w.a_part > 0 ? (p.w.chunks + p.w.a_part - 1) / p.w.a_part : 1;
+    p.w.direct = p.w.parts == 1 && z.group == 1;
+    p.delta = 0;
+    p.kv = padded(rows * sizeof(float));
+    p.dq = p.kv + (p.w.direct ? 0 : padded(2 * keys * (p.w.parts > 1 ? p.w.chunks : 1)));
+    p.diagonals = p.dq + padded(a_block * p.w.count);
+    p.bytes = p.diagonals + diagonals * p.w.count;
+    return p;
+}
+
+}  // namespace
+
+size_t backward_workspace(const Problem& z, bool want_bias) { return plan_of(z, want_bias).bytes; }
+
+int backward(const Problem& z, const float* dy, const float* stats, float* dq, float* dk, float* dv, float* dbias, void* workspace,
+             hipStream_t stream) {
+    Plan p = plan_of(z, dbias != nullptr);
+    char* base = static_cast<char*>(workspace);
+    const Gradients g{dy, stats, reinterpret_cast<const float*>(base + p.delta)};
+    Work w = p.w;
+    const long long values = (long long)z.B * z.H * z.Tk * z.D * (w.parts > 1 ? w.chunks : 1);
+    w.dk = w.direct ? dk : reinterpret_cast<float*>(base + p.kv);
+    w.dv = w.direct ? dv : w.dk + values;
+    w.dq = reinterpret_cast<float*>(base + p.dq);
+    w.diagonals = dbias ? reinterpret_cast<float*>(base + p.diagonals) : nullptr;
+    if ((long long)z.B * z.H * w.count * w.parts > MAX_BLOCKS) return hipErrorInvalidValue;
+    const int most = w.count;
+    for (int first = 0; first < p.blocks; first += most) {
+        w.first = first;
+        w.count = std::min(most, p.blocks - first);
+        const bool begins = first == 0, ends = first + w.count == p.blocks;
+        with_size(z.D, [&](auto db) {
+            with_flags(z.bias != nullptr, z.threshold != 0, [&](auto bias, auto drop) {
+                hipLaunchKernelGGL((backward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value>),
+                                   dim3((unsigned)(z.B * z.H * w.count * w.parts)), dim3(256), 0, stream, z, g, w);
+            });
+        });
+        hipLaunchKernelGGL(sum_queries, dim3(grid_of((long long)z.B * z.H * z.Tq * ((z.D + 63) / 64 * 64), 256)), dim3(256), 0, stream, z,
+                           w, dq, begins, ends);
+        if (!w.direct)
+            hipLaunchKernelGGL(sum_keys, dim3(grid_of((long long)z.B * std::min(z.Tk, w.count * KEY_BLOCK) * z.KVH * z.D, 256)), dim3(256),
+                               0, stream, z, w, dk, dv);
+        if (dbias)
+            hipLaunchKernelGGL(sum_diagonals, dim3(grid_of((long long)z.H * (z.Tq + z.Tk - 1), 256)), dim3(256), 0, stream, z, w, dbias,
+                               begins, ends);
+        const int rc = hipGetLastError();
+        if (rc != hipSuccess) return rc;
+    }
+    return hipSuccess;
+}
+
+}  // namespace attention
+}  // namespace rg

@@ -176,7 +176,8 @@ inline void cpu_attention_grad(const rg_attention_config& c, const float* dy, co
     cpu_detail::spread(c.B * c.KVH * c.Tk, [&](long long n) {
         const long long j = n % c.Tk, g = n / c.Tk % c.KVH, b = n / c.Tk / c.KVH;
         float sv[MAX_D] = {}, sk[MAX_D] = {};
-        for (long long h = g * group; h < (g + 1) * group; ++h)
+        for (long long h = g * group; h < (g + 1) * group; ++h) {
+            float hv[MAX_D] = {}, hk[MAX_D] = {};
             for (long long first = 0; first < c.Tq; first += QUERY_CHUNK) {
                 float pv[MAX_D] = {}, pk[MAX_D] = {};
                 for (long long i = first; i < first + QUERY_CHUNK && i < c.Tq; ++i) {
@@ -186,9 +187,12 @@ inline void cpu_attention_grad(const rg_attention_config& c, const float* dy, co
                     for (int d = 0; d < D; ++d) pv[d] = __builtin_fmaf(w.u, a[d], pv[d]);
                     for (int d = 0; d < D; ++d) pk[d] = __builtin_fmaf(w.ds, x[d], pk[d]);
                 }
-                for (int d = 0; d < D; ++d) sv[d] = sv[d] + pv[d];
-                for (int d = 0; d < D; ++d) sk[d] = sk[d] + pk[d];
+                for (int d = 0; d < D; ++d) hv[d] = hv[d] + pv[d];
+                for (int d = 0; d < D; ++d) hk[d] = hk[d] + pk[d];
             }
+            for (int d = 0; d < D; ++d) sv[d] = sv[d] + hv[d];
+            for (int d = 0; d < D; ++d) sk[d] = sk[d] + hk[d];
+        }
         const long long at = ((b * c.Tk + j) * c.KVH + g) * D;
         for (int d = 0; d < D; ++d) {
             dv[at + d] = sv[d] + 0.0f;
@@ -216,8 +220,8 @@ inline void cpu_attention_grad(const rg_attention_config& c, const float* dy, co
     cpu_detail::spread(c.H * columns, [&](long long n) {
         const long long h = n / columns, away = n % columns - (c.Tq - 1);
         float s = 0.0f;
-        for (long long b = 0; b < c.B; ++b)
-            for (long long block = 0; block < c.Tk; block += KEY_BLOCK)
+        for (long long block = 0; block < c.Tk; block += KEY_BLOCK)
+            for (long long b = 0; b < c.B; ++b)
                 for (long long first = 0; first < c.Tq; first += QUERY_CHUNK) {
                     const long long high = std::min(block + KEY_BLOCK, c.Tk);
                     long long i = std::max(first, block - away), last = std::min({first + QUERY_CHUNK, c.Tq, high - away});

@@ -20,9 +20,9 @@
 // Backward: p_ij = e2(t_ij - M_i) (1 / L_i), delta_i = sum_d dy_d y_d, u_ij = p_ij kept factor,
 //   ds_ij = p_ij ((dy_i . v_j) kept factor - delta_i)
 // Queries are taken in chunks of QUERY_CHUNK and keys in blocks of KEY_BLOCK:
-//   dv_j = sum over the group's heads, then the chunks, both ascending, of the chunk's chain of u_ij dy_i; dk_j likewise of
+//   dv_j = sum over the group's heads of the sum over the chunks, both ascending, of the chunk's chain of u_ij dy_i; dk_j likewise of
 //   ds_ij q_i, times scale; dq_i = sum over the key blocks of the block's chain of ds_ij k_j, times scale
-//   the bias's gradient at distance j - i: over the batch, the key blocks, the chunks, ascending, the sum of ds_ij
+//   the bias's gradient at distance j - i: over the key blocks, the batch, the chunks, ascending, the sum of ds_ij
 //   of one block and chunk in ascending order of i
 #include "repro_gemm_math.h"
 

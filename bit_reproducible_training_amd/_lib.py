@@ -245,7 +245,8 @@ _SEQUENCE_SIGNATURES = {
     "rg_attention_config_init": (None, [ctypes.POINTER(rg_attention_config)]),
     "rg_attention_pack_mask": (ctypes.c_int, [ctypes.c_void_p] + [ctypes.c_longlong] * 4 +
                                [ctypes.POINTER(ctypes.c_longlong), ctypes.c_longlong, ctypes.c_void_p, ctypes.c_void_p]),
-    "rg_attention_workspace": (ctypes.c_int, [ctypes.POINTER(rg_attention_config), ctypes.POINTER(ctypes.c_size_t)]),
+    "rg_attention_workspace": (ctypes.c_int, [ctypes.POINTER(rg_attention_config), ctypes.c_int,
+                                              ctypes.POINTER(ctypes.c_size_t)]),
     "rg_attention_fp32": (ctypes.c_int, [ctypes.POINTER(rg_attention_config)] + [ctypes.c_void_p] * 11 +
                           [ctypes.c_size_t, ctypes.c_void_p]),
     "rg_attention_grad_workspace": (ctypes.c_int, [ctypes.POINTER(rg_attention_config), ctypes.c_int,

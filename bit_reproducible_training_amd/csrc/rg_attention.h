@@ -12,13 +12,14 @@
 namespace rg {
 namespace attention {
 
+using repro_attention::base_of;
+using repro_attention::bias_term;
 using repro_attention::CHUNK;
 using repro_attention::ds_of;
 using repro_attention::e2;
-using repro_attention::finite_top;
 using repro_attention::KEY_BLOCK;
 using repro_attention::larger;
-using repro_attention::LOG2E;
+using repro_attention::NONE;
 using repro_attention::QUERY_CHUNK;
 using repro_attention::reciprocal;
 using repro_attention::TILE;
@@ -32,6 +33,7 @@ struct Problem {
     unsigned long long seed;
     int B, Tq, Tk, H, KVH, D, group, causal, start;
     int quads;  // whether the rows of q, k and v can be read 16 bytes at a time
+    int flip;                          // a negative scale: scores are multiplied by -1, and factor is positive
     float factor, scale, keep_factor;
     uint32_t threshold;
     long long q_stride[3], k_stride[3], v_stride[3], mask_stride[3];
@@ -71,10 +73,18 @@ __device__ __forceinline__ float dot(const float* a, const float* b, int D) {
     for (int d = 0; d < D; ++d) s = __builtin_fmaf(a[d], b[d], s);
     return s;
 }
-__device__ __forceinline__ float score(const Problem& z, int b, int h, int i, int j) {
-    const float s = dot(query_at(z, b, h, i), key_at(z, b, h, j), z.D);
-    return z.bias ? __builtin_fmaf(s, z.factor, z.bias[(size_t)h * (z.Tq + z.Tk - 1) + j - i + z.Tq - 1] * LOG2E)
-                  : s * z.factor;
+// t, and its difference to a maximum.
+struct Score {
+    float s, t;
+};
+__device__ __forceinline__ Score score(const Problem& z, int b, int h, int i, int j) {
+    float s = dot(query_at(z, b, h, i), key_at(z, b, h, j), z.D);
+    s = z.flip ? -s : s;
+    if (!z.bias) return Score{s, s * z.factor};
+    return Score{s, __builtin_fmaf(s, z.factor, bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + j - i + z.Tq - 1]))};
+}
+__device__ __forceinline__ float less(const Problem& z, const Score& a, float m) {
+    return z.bias ? a.t - m : __builtin_fmaf(a.s, z.factor, -m);
 }
 __device__ __forceinline__ bool kept(const Problem& z, uint64_t seed, int b, int h, int i, int j) {
     if (z.threshold == 0) return true;
@@ -92,16 +102,16 @@ struct RowChunk {
     float m, even, odd, o0, o1;
 };
 __device__ __forceinline__ RowChunk row_chunk(const Problem& z, uint64_t seed, int b, int h, int i, int first, int end, int lane) {
-    RowChunk r{-__builtin_inff(), 0.0f, 0.0f, 0.0f, 0.0f};
+    RowChunk r{NONE, 0.0f, 0.0f, 0.0f, 0.0f};
     for (int j0 = first; j0 < first + CHUNK && j0 < end; j0 += TILE) {
         const int j = j0 + lane;
         const bool see = seen(z, b, h, i, j, end);
-        const float t = see ? score(z, b, h, i, j) : -__builtin_inff();
-        const float next = larger(r.m, wave_max(t));
-        const float a = e2(r.m - finite_top(next));
+        const Score t = see ? score(z, b, h, i, j) : Score{NONE, NONE};
+        const float next = larger(r.m, wave_max(t.t));
+        const float a = e2(r.m - base_of(next));
         r.m = next;
         r.even = r.even * a, r.odd = r.odd * a, r.o0 = r.o0 * a, r.o1 = r.o1 * a;
-        const float p = see ? e2(t - finite_top(next)) : 0.0f;
+        const float p = see ? e2(less(z, t, base_of(next))) : 0.0f;
         const float u = see && kept(z, seed, b, h, i, j) ? p : 0.0f;
         const unsigned long long which = __ballot(see);
         for (int n = 0; n < TILE; n += 2) {
@@ -119,9 +129,9 @@ __device__ __forceinline__ RowChunk row_chunk(const Problem& z, uint64_t seed, i
     return r;
 }
 struct Joined {
-    float top = -__builtin_inff(), total = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    float top = NONE, total = 0.0f, o0 = 0.0f, o1 = 0.0f;
     __device__ __forceinline__ void join(const RowChunk& r) {
-        const float both = larger(top, r.m), a = e2(top - finite_top(both)), e = e2(r.m - finite_top(both));
+        const float both = larger(top, r.m), a = e2(top - base_of(both)), e = e2(r.m - base_of(both));
         top = both;
         total = __builtin_fmaf(r.even + r.odd, e, total * a);
         o0 = __builtin_fmaf(r.o0, e, o0 * a);
@@ -136,7 +146,7 @@ __device__ __forceinline__ void finish_row(const Problem& z, const Joined& all, 
     if (lane + 64 < z.D) out[lane + 64] = all.o1 * f + 0.0f;
     if (stats && lane == 0) {
         const size_t n = ((size_t)b * z.H + h) * z.Tq + i;
-        stats[2 * n] = finite_top(all.top);
+        stats[2 * n] = base_of(all.top);
         stats[2 * n + 1] = inverse;
     }
 }
@@ -148,7 +158,7 @@ struct Pair {
 __device__ __forceinline__ Pair pair(const Problem& z, const Gradients& g, uint64_t seed, int b, int h, int i, int j, bool see) {
     if (!see) return Pair{0.0f, 0.0f};
     const size_t n = ((size_t)b * z.H + h) * z.Tq + i;
-    const float p = e2(score(z, b, h, i, j) - g.stats[2 * n]) * g.stats[2 * n + 1];
+    const float p = e2(less(z, score(z, b, h, i, j), g.stats[2 * n])) * g.stats[2 * n + 1];
     float u = p, dp = dot(g.dy + (((size_t)b * z.Tq + i) * z.H + h) * z.D, value_at(z, b, h, j), z.D);
     if (z.threshold != 0) {
         const bool keep = kept(z, seed, b, h, i, j);
@@ -209,6 +219,13 @@ __device__ __forceinline__ QueryPart query_part(const Problem& z, const Gradient
     return r;
 }
 
+// A barrier for what the block's wavefronts hand each other in LDS; loads and stores of global memory may go on across it.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // ---- host ----
 
 constexpr long long MAX_BLOCKS = 1 << 23;  // of 256 threads: a launch takes fewer than 2^32
@@ -235,7 +252,7 @@ void with_flags(bool a, bool b, F run) {
     else second(std::false_type());
 }
 
-size_t forward_workspace(const Problem& z);
+size_t forward_workspace(const Problem& z, bool masked);  // masked: z's mask will be given
 int forward(const Problem& z, float* y, float* stats, unsigned long long* used, void* workspace, hipStream_t stream);
 // For at least one query and one key; the workspace starts with the rows' deltas.
 size_t backward_workspace(const Problem& z, bool want_bias);

@@ -65,7 +65,8 @@ Problem problem_of(const rg_attention_config* c, const float* q, const float* k,
     const long long s = c->query_start;
     z.causal = c->causal && s < c->Tk;
     z.start = (int)(s > c->Tk ? c->Tk : s < -c->Tq ? -c->Tq : s);
-    z.factor = repro_attention::score_factor(c->scale);
+    z.factor = std::fabs(repro_attention::score_factor(c->scale));
+    z.flip = c->scale < 0.0;
     z.scale = (float)c->scale;
     z.keep_factor = repro_dropout::factor_of(c->dropout);
     z.threshold = repro_dropout::threshold_of(c->dropout);
@@ -116,10 +117,10 @@ int rg_attention_pack_mask(const unsigned char* mask, long long items, long long
     return hipGetLastError();
 }
 
-int rg_attention_workspace(const rg_attention_config* cfg, size_t* bytes) {
+int rg_attention_workspace(const rg_attention_config* cfg, int masked, size_t* bytes) {
     using namespace rg::attention;
     if (!sizes_ok(cfg) || !bytes) return hipErrorInvalidValue;
-    *bytes = forward_workspace(problem_of(cfg, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr));
+    *bytes = forward_workspace(problem_of(cfg, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr), masked != 0);
     return hipSuccess;
 }
 
@@ -135,7 +136,7 @@ int rg_attention_fp32(const rg_attention_config* cfg, const float* q, const floa
     if (rows > 0 && !y) return hipErrorInvalidValue;
     if (rows == 0) return hipSuccess;
     const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at);
-    const size_t needed = forward_workspace(z);
+    const size_t needed = forward_workspace(z, mask != nullptr);
     if (needed > 0 && (!workspace || workspace_bytes < needed || off(workspace, 16))) return hipErrorInvalidValue;
     return forward(z, y, stats, used, workspace, static_cast<hipStream_t>(stream));
 }

@@ -31,6 +31,13 @@ __device__ __forceinline__ Block16 zero16() {
 __device__ __forceinline__ Block16 mfma(float a, float b, Block16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0);
 }
+// Keeps the compiler from fetching operands of later products early, which takes registers that there are not.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+// A value that the compiler does not compute addresses from ahead of a loop.
+__device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 __device__ __forceinline__ float part_of(const float4& v, int r) { return r == 0 ? v.x : r == 1 ? v.y : r == 2 ? v.z : v.w; }
 
 // Where a block and chunk are, and what they leave. Key blocks first .. first + count of the `blocks`.
@@ -40,7 +47,20 @@ struct Work {
     float *dk, *dv;
     float* dq;                  // [count][B][H][Tq][D]
     float* diagonals;           // [B][H][count][chunks][DIAGONALS], or null
+    int* broken;                // a number for each block: whether `repair` has to redo it; null where it never has to
 };
+struct Place {
+    int bh, slot, part;
+};
+__device__ __forceinline__ Place place_of(const Problem& z, const Work& w) {
+    const int heads = z.B * z.H, rest = (int)(blockIdx.x / heads);
+    return Place{(int)(blockIdx.x % heads), rest / w.parts, rest % w.parts};
+}
+// Where a key's sums of a chunk go: the chunk's own place, or the one that all chunks are added to.
+__device__ __forceinline__ size_t out_of(const Problem& z, const Work& w, int bh, int chunk) {
+    return w.direct ? ((size_t)(bh / z.H) * z.Tk * z.KVH + bh % z.H) * z.D
+                    : ((size_t)(w.parts > 1 ? chunk : 0) * z.B * z.H + bh) * z.Tk * z.D;
+}
 
 __device__ __forceinline__ int last_end(const Problem& z, int len, int i) {
     return z.causal ? max(0, min(len, i + z.start + 1)) : len;
@@ -60,27 +80,28 @@ backward_tiles(Problem z, Gradients g, Work w) {
     __shared__ uint32_t Masks[STEP][4];
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
     const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5, wave = t >> 6;
-    const int heads = z.B * z.H, bh = (int)(blockIdx.x % heads), rest = (int)(blockIdx.x / heads);
-    const int b = bh / z.H, h = bh % z.H, part = rest % w.parts;
-    const int slot = rest / w.parts, block = w.first + slot, k0 = block * KEY_BLOCK;
+    const Place at = place_of(z, w);
+    const int bh = at.bh, b = bh / z.H, h = bh % z.H, slot = at.slot, heads = z.B * z.H;
+    const int block = w.first + slot, k0 = block * KEY_BLOCK;
     const int len = keys_of(z, b), key = k0 + 32 * wave + col;
     const size_t row0 = (size_t)bh * z.Tq;
-    const size_t out_row = w.direct ? ((size_t)b * z.Tk * z.KVH + h) * z.D : (size_t)bh * z.Tk * z.D;
     const size_t out_stride = (size_t)(w.direct ? z.KVH : 1) * z.D;
     const bool whole = z.D % 4 == 0;
 
     if (!live(z, len, block, z.Tq)) {
-        if (w.direct && part == 0)
-            for (int at = t; at < KEY_BLOCK * z.D; at += 256)
-                if (k0 + at / z.D < z.Tk) {
-                    w.dk[out_row + (k0 + at / z.D) * out_stride + at % z.D] = 0.0f;
-                    w.dv[out_row + (k0 + at / z.D) * out_stride + at % z.D] = 0.0f;
+        const size_t out = out_of(z, w, bh, 0);
+        if (w.direct)
+            for (int n = t; n < KEY_BLOCK * z.D; n += 256)
+                if (k0 + n / z.D < z.Tk) {
+                    w.dk[out + (k0 + n / z.D) * out_stride + n % z.D] = 0.0f;
+                    w.dv[out + (k0 + n / z.D) * out_stride + n % z.D] = 0.0f;
                 }
+        if (w.broken && t == 0) w.broken[blockIdx.x] = 0;
         return;
     }
 
     float k[16 * DB], v[16 * DB];  // value 2 n + half of the lane's key
-    float broken_key = 0.0f;
+    float broken = 0.0f;
     const auto four = [&](const float* row, bool there, int d) {
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (!there || d >= z.D) return x;
@@ -114,18 +135,21 @@ backward_tiles(Problem z, Gradients g, Work w) {
     __syncthreads();
     take(k);
 #pragma unroll
-    for (int n = 0; n < 16 * DB; ++n) broken_key = __builtin_fmaf(k[n], 0.0f, broken_key);
+    for (int n = 0; n < 16 * DB; ++n) {
+        broken = __builtin_fmaf(k[n], 0.0f, broken);
+        k[n] = z.flip ? -k[n] : k[n];
+    }
 
     const float* qbase = query_at(z, b, h, 0);
     const float* ybase = g.dy + ((size_t)b * z.Tq * z.H + h) * z.D;
     const size_t ystride = (size_t)z.H * z.D;
     const bool ywhole = whole && (reinterpret_cast<uintptr_t>(g.dy) & 15) == 0;
-    const bool watch = z.causal || z.mask || k0 + KEY_BLOCK > len;  // a query's values must not reach keys that it does not see
     float4 qn[DB], yn[DB];
-    float broken = 0.0f, bn = 0.0f;
+    float bn = 0.0f;
     float4 rn;
     uint32_t mn = 0;
     const auto load = [&](int i0) {
+        const int t = fresh(threadIdx.x);
 #pragma unroll
         for (int n = 0; n < DB; ++n) {
             const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4, i = i0 + row;
@@ -163,10 +187,11 @@ backward_tiles(Problem z, Gradients g, Work w) {
         }
         if (BIAS && t < KEY_BLOCK + STEP - 1) {
             const int c = k0 + t - (STEP - 1) - i0 + z.Tq - 1;
-            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c] * LOG2E : 0.0f;
+            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c]) : 0.0f;
         }
     };
     const auto store = [&]() {
+        const int t = fresh(threadIdx.x);
 #pragma unroll
         for (int n = 0; n < DB; ++n) {
             const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4;
@@ -186,10 +211,10 @@ backward_tiles(Problem z, Gradients g, Work w) {
         if (BIAS && t < KEY_BLOCK + STEP - 1) Bs[t] = bn;
     };
     const int row_of = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);     // the query that row `col` of an operand is
-    const int place_of = (col & 24) + 4 * (col & 1) + ((col >> 1) & 3);   // where value `col` of 32 is in Qs and Ys
+    const int place_in = (col & 24) + 4 * (col & 1) + ((col >> 1) & 3);   // where value `col` of 32 is in Qs and Ys
     const int ds_place = 32 * wave + (col & 16) + 4 * (col & 3) + ((col >> 2) & 3);  // where a key is in Ds: 4 s + c of 16 at 4 c + s
 
-    const int first_chunk = part * w.a_part, last_chunk = min(w.chunks, first_chunk + w.a_part);
+    const int first_chunk = at.part * w.a_part, last_chunk = min(w.chunks, first_chunk + w.a_part);
     bool begun = false;
     for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
         const int c0 = chunk * QUERY_CHUNK, c1 = min(c0 + QUERY_CHUNK, z.Tq);
@@ -201,24 +226,32 @@ backward_tiles(Problem z, Gradients g, Work w) {
         int i0 = c0;
         while (!live(z, len, block, i0 + STEP)) i0 += STEP;  // (the chunk's last step is live)
         __syncthreads();
-        broken = 0.0f;
         load(i0);
         store();
         if (BIAS)
             for (int n = t; n < DIAGONALS; n += 256) Sums[n] = 0.0f;
-        __syncthreads();
+        lds_barrier();
         for (; i0 < c1; i0 += STEP) {
             const bool more = i0 + STEP < c1;
             if (more) load(i0 + STEP);
             Block16 s = zero16(), dp = zero16();
+            {
+                const float* qs = Qs + row_of * QS + 4 * half;
+                const float* ys = Ys + row_of * QS + 4 * half;
+                float4 a = *reinterpret_cast<const float4*>(qs), c = *reinterpret_cast<const float4*>(ys);
 #pragma unroll
-            for (int u = 0; u < 4 * DB; ++u) {
-                const float4 a = *reinterpret_cast<const float4*>(Qs + row_of * QS + 8 * u + 4 * half);
-                const float4 c = *reinterpret_cast<const float4*>(Ys + row_of * QS + 8 * u + 4 * half);
+                for (int u = 0; u < 4 * DB; ++u) {
+                    const int ahead = u + 1 < 4 * DB ? u + 1 : u;
+                    const float4 an = *reinterpret_cast<const float4*>(qs + 8 * ahead);
+                    const float4 cn = *reinterpret_cast<const float4*>(ys + 8 * ahead);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    s = mfma(part_of(a, r), k[4 * u + r], s);
-                    dp = mfma(part_of(c, r), v[4 * u + r], dp);
+                    for (int r = 0; r < 4; ++r) {
+                        s = mfma(part_of(a, r), k[4 * u + r], s);
+                        dp = mfma(part_of(c, r), v[4 * u + r], dp);
+                    }
+                    a = an;
+                    c = cn;
+                    fence();
                 }
             }
             uint32_t keep[4];
@@ -237,54 +270,81 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 keep[2] = __builtin_amdgcn_update_dpp(0, bits, 0xAA, 0xF, 0xF, true) >> r;
                 keep[3] = __builtin_amdgcn_update_dpp(0, bits, 0xFF, 0xF, 0xF, true) >> r;
             }
+            const auto differentials = [&](auto edge) {
+#pragma unroll
+                for (int n = 0; n < 16; ++n) {
+                    const int q = 8 * (n / 4) + 2 * (n % 4) + half;
+                    const float4 row = Rows[q];
+                    const float x = BIAS ? __builtin_fmaf(s[n], z.factor, Bs[32 * wave + col - q + STEP - 1]) - row.x
+                                         : __builtin_fmaf(s[n], z.factor, -row.x);
+                    float p = e2(x) * row.y, d = dp[n], u = p;
+                    if (DROP) {
+                        const bool kept = (keep[n % 4] >> (4 * (n / 4)) & 1) != 0;
+                        u = kept ? p * z.keep_factor : 0.0f;
+                        d = kept ? d * z.keep_factor : 0.0f;
+                    }
+                    d = ds_of(p, d, row.z);
+                    if (decltype(edge)::value) {
+                        const bool see = (int)(key < __float_as_int(row.w)) & (int)(Masks[q][wave] >> col & 1);
+                        u = see ? u : 0.0f;
+                        d = see ? d : 0.0f;
+                    }
+                    s[n] = u;
+                    dp[n] = d;
+                    Ds[q * DS_STRIDE + ds_place] = d;
+                    if (n % 4 == 3) fence();
+                }
+            };
             // whether every pair of the wavefront's is seen
-            const bool inner = !z.mask && i0 + STEP <= z.Tq && k0 + 32 * wave + 32 <= last_end(z, len, i0);
+            if (!z.mask && i0 + STEP <= z.Tq && k0 + 32 * wave + 32 <= last_end(z, len, i0)) differentials(std::false_type());
+            else differentials(std::true_type());
+            {
+                const float* qs = Qs + half * QS + place_in;
+                const float* ys = Ys + half * QS + place_in;
+                float a[DB], c[DB];
 #pragma unroll
-            for (int n = 0; n < 16; ++n) {
-                const int q = 8 * (n / 4) + 2 * (n % 4) + half;
-                const float4 row = Rows[q];
-                const float x = BIAS ? __builtin_fmaf(s[n], z.factor, Bs[32 * wave + col - q + STEP - 1]) : s[n] * z.factor;
-                float p = e2(x - row.x) * row.y, d = dp[n], u = p;
-                if (DROP) {
-                    const bool kept = (keep[n % 4] >> (4 * (n / 4)) & 1) != 0;
-                    u = kept ? p * z.keep_factor : 0.0f;
-                    d = kept ? d * z.keep_factor : 0.0f;
-                }
-                d = ds_of(p, d, row.z);
-                if (!inner) {
-                    const bool see = key < __float_as_int(row.w) && (Masks[q][wave] >> col & 1) != 0;
-                    u = see ? u : 0.0f;
-                    d = see ? d : 0.0f;
-                }
-                s[n] = u;
-                dp[n] = d;
-                Ds[q * DS_STRIDE + ds_place] = d;
-            }
+                for (int x = 0; x < DB; ++x) a[x] = ys[32 * x], c[x] = qs[32 * x];
 #pragma unroll
-            for (int n = 0; n < 16; ++n) {
-                const int q = 8 * (n / 4) + 2 * (n % 4) + half;
+                for (int n = 0; n < 16; ++n) {
+                    const int m = n < 15 ? n + 1 : n, ahead = (8 * (m / 4) + 2 * (m % 4)) * QS;
+                    float an[DB], cn[DB];
 #pragma unroll
-                for (int x = 0; x < DB; ++x) {
-                    dv[x] = mfma(Ys[q * QS + 32 * x + place_of], s[n], dv[x]);
-                    dk[x] = mfma(Qs[q * QS + 32 * x + place_of], dp[n], dk[x]);
+                    for (int x = 0; x < DB; ++x) an[x] = ys[ahead + 32 * x], cn[x] = qs[ahead + 32 * x];
+#pragma unroll
+                    for (int x = 0; x < DB; ++x) {
+                        dv[x] = mfma(a[x], s[n], dv[x]);
+                        dk[x] = mfma(c[x], dp[n], dk[x]);
+                    }
+#pragma unroll
+                    for (int x = 0; x < DB; ++x) a[x] = an[x], c[x] = cn[x];
+                    fence();
                 }
             }
-            __syncthreads();
+            lds_barrier();
             if (more) store();
             {
                 const int c16 = lane & 15, group = lane >> 4, q0 = 16 * (wave & 1), d0 = 16 * DB * (wave >> 1);
                 Block4 dq[DB];
 #pragma unroll
                 for (int x = 0; x < DB; ++x) dq[x] = Block4{0.0f, 0.0f, 0.0f, 0.0f};
+                const float* ds = Ds + (q0 + c16) * DS_STRIDE + 4 * group;
+                const float* ks = Ks + group * KS + d0 + c16;
+                float4 a = *reinterpret_cast<const float4*>(ds);
 #pragma unroll
                 for (int n = 0; n < KEY_BLOCK / 16; ++n) {
-                    const float4 a = *reinterpret_cast<const float4*>(Ds + (q0 + c16) * DS_STRIDE + 16 * n + 4 * group);
+                    const float4 an = *reinterpret_cast<const float4*>(ds + 16 * (n + 1 < KEY_BLOCK / 16 ? n + 1 : n));
+                    float c[4][DB];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int x = 0; x < DB; ++x) c[r][x] = ks[(16 * n + 4 * r) * KS + 16 * x];
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int x = 0; x < DB; ++x)
-                            dq[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(part_of(a, r), Ks[(16 * n + 4 * r + group) * KS + d0 + 16 * x + c16],
-                                                                        dq[x], 0, 0, 0);
+                            dq[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(part_of(a, r), c[r][x], dq[x], 0, 0, 0);
+                    a = an;
+                    if (n % 2 == 1) fence();
                 }
                 float* to = w.dq + ((size_t)slot * heads * z.Tq + row0 + i0 + q0 + 4 * group) * z.D;
 #pragma unroll
@@ -296,80 +356,95 @@ backward_tiles(Problem z, Gradients g, Work w) {
                     }
             }
             if (BIAS && w.diagonals && t < KEY_BLOCK + STEP - 1) {
+                const int t = fresh(threadIdx.x);
                 float* sum = Sums + t - (STEP - 1) - (i0 - c0) + QUERY_CHUNK - 1;
                 float x = *sum;
+#pragma unroll
                 for (int q = 0; q < STEP; ++q) {
-                    const int c = t - (STEP - 1) + q;
-                    if (c >= 0 && c < KEY_BLOCK) x = x + Ds[q * DS_STRIDE + (c & ~15) + 4 * (c & 3) + ((c >> 2) & 3)];
+                    const int c = t - (STEP - 1) + q, at_c = c & (KEY_BLOCK - 1);
+                    const float d = Ds[q * DS_STRIDE + (at_c & ~15) + 4 * (at_c & 3) + ((at_c >> 2) & 3)];
+                    x = x + (c == at_c ? d : 0.0f);
                 }
                 *sum = x;
             }
-            __syncthreads();
+            lds_barrier();
         }
-        const bool again = watch && __syncthreads_or(broken != broken || broken_key != broken_key);
         const bool last = w.direct && chunk == w.chunks - 1;
-        const size_t chunk_out = out_row + (w.parts > 1 ? (size_t)chunk * heads * z.Tk * z.D : 0);
+        const size_t chunk_out = out_of(z, w, bh, chunk);
         const bool add = w.parts == 1 && begun;
         begun = true;
-        if (!again) {
-            if (key < z.Tk) {
-                float* kd = w.dk + chunk_out + key * out_stride;
-                float* vd = w.dv + chunk_out + key * out_stride;
+        if (key < z.Tk) {
+            float* kd = w.dk + chunk_out + key * out_stride;
+            float* vd = w.dv + chunk_out + key * out_stride;
 #pragma unroll
-                for (int x = 0; x < DB; ++x)
+            for (int x = 0; x < DB; ++x)
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int d = 32 * x + 8 * n + 4 * half;
-                        if (d >= z.D) continue;
-                        float a[4], c[4];
+                for (int n = 0; n < 4; ++n) {
+                    const int d = 32 * x + 8 * n + 4 * half;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) a[r] = dk[x][4 * n + r], c[r] = dv[x][4 * n + r];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            if (d + r >= z.D) continue;
-                            if (add) a[r] = kd[d + r] + a[r], c[r] = vd[d + r] + c[r];
-                            if (last) a[r] = a[r] * z.scale + 0.0f, c[r] = c[r] + 0.0f;
-                            kd[d + r] = a[r];
-                            vd[d + r] = c[r];
-                        }
+                    for (int r = 0; r < 4; ++r) {
+                        if (d + r >= z.D) continue;
+                        float a = dk[x][4 * n + r], c = dv[x][4 * n + r];
+                        if (add) a = kd[d + r] + a, c = vd[d + r] + c;
+                        if (last) a = a * z.scale + 0.0f, c = c + 0.0f;
+                        kd[d + r] = a;
+                        vd[d + r] = c;
                     }
-            }
-            if (diagonals)
-                for (int n = t; n < DIAGONALS; n += 256) diagonals[n] = Sums[n];
-            continue;
+                }
         }
-        // A NaN or infinity that the products' zeros would hand to pairs that are not seen: key by key, row by row.
-        for (int n = wave; n < KEY_BLOCK && k0 + n < z.Tk; n += 4) {
-            const KeyPart r = key_part(z, g, seed, b, h, k0 + n, c0, lane);
-            float* kd = w.dk + chunk_out + (k0 + n) * out_stride;
-            float* vd = w.dv + chunk_out + (k0 + n) * out_stride;
-            for (int x = 0; x < 2; ++x) {
-                const int d = lane + 64 * x;
-                if (d >= z.D) continue;
-                float a = x ? r.k1 : r.k0, c = x ? r.v1 : r.v0;
-                if (add) a = kd[d] + a, c = vd[d] + c;
-                if (last) a = a * z.scale + 0.0f, c = c + 0.0f;
-                kd[d] = a;
-                vd[d] = c;
-            }
+        if (diagonals)
+            for (int n = t; n < DIAGONALS; n += 256) diagonals[n] = Sums[n];
+    }
+    if (w.broken) {  // a NaN or infinity, which the products' zeros hand to pairs that are not seen
+        const int any = __syncthreads_or(broken != broken);
+        if (t == 0) w.broken[blockIdx.x] = any;
+    }
+}
+
+// Redoes the blocks whose operands hold a NaN or infinity, key by key, row by row and pair by pair.
+__global__ void __launch_bounds__(256)
+repair(Problem z, Gradients g, Work w) {
+    if (w.broken[blockIdx.x] == 0) return;
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Place at = place_of(z, w);
+    const int b = at.bh / z.H, h = at.bh % z.H, heads = z.B * z.H, block = w.first + at.slot, k0 = block * KEY_BLOCK;
+    const int len = keys_of(z, b), first_chunk = at.part * w.a_part, last_chunk = min(w.chunks, first_chunk + w.a_part);
+    const size_t out_stride = (size_t)(w.direct ? z.KVH : 1) * z.D;
+    for (int n = wave; n < KEY_BLOCK && k0 + n < z.Tk; n += 4) {
+        KeyPart sum{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
+            if (!live(z, len, block, min((chunk + 1) * QUERY_CHUNK, z.Tq))) continue;
+            const KeyPart r = key_part(z, g, seed, b, h, k0 + n, chunk * QUERY_CHUNK, lane);
+            if (w.parts > 1) sum = r;
+            else sum.v0 = sum.v0 + r.v0, sum.v1 = sum.v1 + r.v1, sum.k0 = sum.k0 + r.k0, sum.k1 = sum.k1 + r.k1;
+            if (w.parts == 1 && chunk + 1 < last_chunk) continue;
+            const size_t to = out_of(z, w, at.bh, chunk) + (k0 + n) * out_stride;
+            const float scale = w.direct ? z.scale : 1.0f;
+            if (lane < z.D) w.dk[to + lane] = sum.k0 * scale + 0.0f, w.dv[to + lane] = sum.v0 + 0.0f;
+            if (lane + 64 < z.D) w.dk[to + lane + 64] = sum.k1 * scale + 0.0f, w.dv[to + lane + 64] = sum.v1 + 0.0f;
         }
+    }
+    for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
+        const int c0 = chunk * QUERY_CHUNK, c1 = min(c0 + QUERY_CHUNK, z.Tq);
+        if (!live(z, len, block, c1)) continue;
         for (int i = c0 + wave; i < c1; i += 4) {
             const QueryPart r = query_part(z, g, seed, b, h, i, k0, last_end(z, len, i), lane);
-            float* to = w.dq + ((size_t)slot * heads * z.Tq + row0 + i) * z.D;
+            float* to = w.dq + ((size_t)at.slot * heads * z.Tq + (size_t)at.bh * z.Tq + i) * z.D;
             if (lane < z.D) to[lane] = r.q0;
             if (lane + 64 < z.D) to[lane + 64] = r.q1;
         }
-        if (diagonals)
-            for (int n = t; n < DIAGONALS; n += 256) {
-                const int away = n - (QUERY_CHUNK - 1);  // key in the block less query in the chunk
-                float x = 0.0f;
-                for (int i = max(0, -away); i < c1 - c0 && i + away < KEY_BLOCK; ++i) {
-                    const int j = k0 + i + away;
-                    x = x + pair(z, g, seed, b, h, c0 + i, j, seen(z, b, h, c0 + i, j, last_end(z, len, c0 + i))).ds;
-                }
-                diagonals[n] = x;
+        if (!w.diagonals) continue;
+        float* diagonals = w.diagonals + (((size_t)at.bh * w.count + at.slot) * w.chunks + chunk) * DIAGONALS;
+        for (int n = threadIdx.x; n < DIAGONALS; n += 256) {
+            const int away = n - (QUERY_CHUNK - 1);  // key in the block less query in the chunk
+            float x = 0.0f;
+            for (int i = max(0, -away); i < c1 - c0 && i + away < KEY_BLOCK; ++i) {
+                const int j = k0 + i + away;
+                x = x + pair(z, g, seed, b, h, c0 + i, j, seen(z, b, h, c0 + i, j, last_end(z, len, c0 + i))).ds;
             }
-        __syncthreads();
+            diagonals[n] = x;
+        }
     }
 }
 
@@ -450,7 +525,7 @@ sum_diagonals(Problem z, Work w, float* dbias, int begins, int ends) {
 struct Plan {
     Work w;
     int blocks;
-    size_t delta, kv, dq, diagonals, bytes;  // workspace: offsets, and its size
+    size_t kv, dq, diagonals, broken, bytes;  // workspace: offsets, and its size
 };
 
 size_t padded(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -471,11 +546,11 @@ Plan plan_of(const Problem& z, bool want_bias) {
     p.w.a_part = parts > 0 ? (int)((p.w.chunks + parts - 1) / parts) : 0;
     p.w.parts = p.w.a_part > 0 ? (p.w.chunks + p.w.a_part - 1) / p.w.a_part : 1;
     p.w.direct = p.w.parts == 1 && z.group == 1;
-    p.delta = 0;
     p.kv = padded(rows * sizeof(float));
     p.dq = p.kv + (p.w.direct ? 0 : padded(2 * keys * (p.w.parts > 1 ? p.w.chunks : 1)));
     p.diagonals = p.dq + padded(a_block * p.w.count);
-    p.bytes = p.diagonals + diagonals * p.w.count;
+    p.broken = p.diagonals + padded(diagonals * p.w.count);
+    p.bytes = p.broken + (size_t)z.B * z.H * p.w.count * p.w.parts * sizeof(int);
     return p;
 }
 
@@ -487,13 +562,15 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
              hipStream_t stream) {
     Plan p = plan_of(z, dbias != nullptr);
     char* base = static_cast<char*>(workspace);
-    const Gradients g{dy, stats, reinterpret_cast<const float*>(base + p.delta)};
+    const Gradients g{dy, stats, reinterpret_cast<const float*>(base)};
     Work w = p.w;
     const long long values = (long long)z.B * z.H * z.Tk * z.D * (w.parts > 1 ? w.chunks : 1);
     w.dk = w.direct ? dk : reinterpret_cast<float*>(base + p.kv);
     w.dv = w.direct ? dv : w.dk + values;
     w.dq = reinterpret_cast<float*>(base + p.dq);
     w.diagonals = dbias ? reinterpret_cast<float*>(base + p.diagonals) : nullptr;
+    // a query's values must not reach keys that it does not see, nor a key's a query
+    w.broken = z.causal || z.mask || z.key_lengths ? reinterpret_cast<int*>(base + p.broken) : nullptr;
     if ((long long)z.B * z.H * w.count * w.parts > MAX_BLOCKS) return hipErrorInvalidValue;
     const int most = w.count;
     for (int first = 0; first < p.blocks; first += most) {
@@ -506,6 +583,8 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
                                    dim3((unsigned)(z.B * z.H * w.count * w.parts)), dim3(256), 0, stream, z, g, w);
             });
         });
+        if (w.broken)
+            hipLaunchKernelGGL(repair, dim3((unsigned)(z.B * z.H * w.count * w.parts)), dim3(256), 0, stream, z, g, w);
         hipLaunchKernelGGL(sum_queries, dim3(grid_of((long long)z.B * z.H * z.Tq * ((z.D + 63) / 64 * 64), 256)), dim3(256), 0, stream, z,
                            w, dq, begins, ends);
         if (!w.direct)

@@ -50,7 +50,18 @@ struct Parts {
     int parts, chunks, a_part;  // chunks a part
     float2* ml;                 // [B][H][Tq][chunks]
     float* o;                   // [B][H][Tq][chunks][D]
+    int* broken;                // a number for each block: whether `repair` has to redo it; null where it never has to
 };
+
+// The block's place: head, first query, part.
+struct Place {
+    int bh, i0, part;
+};
+__device__ __forceinline__ Place place_of(const Problem& z, const Parts& s) {
+    const int heads = z.B * z.H, rest = (int)(blockIdx.x / heads);
+    // under a causal mask the longest first
+    return Place{(int)(blockIdx.x % heads), ((z.Tq + ROWS - 1) / ROWS - 1 - rest / s.parts) * ROWS, rest % s.parts};
+}
 
 // DB blocks of 32 values hold a head's.
 template <int DB, bool BIAS, bool DROP>
@@ -62,10 +73,8 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
     if (used && blockIdx.x == 0 && threadIdx.x == 0) *used = seed;
     const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5, wave = t >> 6;
-    const int heads = z.B * z.H, bh = (int)(blockIdx.x % heads), rest = (int)(blockIdx.x / heads);
-    const int b = bh / z.H, h = bh % z.H;
-    const int part = rest % s.parts;
-    const int i0 = ((z.Tq + ROWS - 1) / ROWS - 1 - rest / s.parts) * ROWS;  // under a causal mask the longest first
+    const Place at = place_of(z, s);
+    const int bh = at.bh, b = bh / z.H, h = bh % z.H, part = at.part, i0 = at.i0;
     const int w0 = i0 + 32 * wave, i = w0 + col;
     const int len = keys_of(z, b);
     const auto end_of = [&](int last) { return z.causal ? max(0, min(len, last + z.start + 1)) : len; };
@@ -75,7 +84,6 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     const int full = z.mask ? 0 : w0 + 32 <= z.Tq ? end_of(w0) : 0;  // keys below it are seen by the whole wavefront
     const unsigned long long* mask_row = nullptr;
     if (z.mask && i < z.Tq) mask_row = z.mask + b * z.mask_stride[0] + h * z.mask_stride[1] + i * z.mask_stride[2];
-    const bool watch = z.causal || z.mask != nullptr;  // what a key holds must not reach a row that does not see it
 
     float q[16 * DB];  // value 2 n + half of the row
     {
@@ -87,6 +95,8 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
             q[4 * u + 1] = half ? a.w : a.z;
             q[4 * u + 2] = half ? c.y : c.x;
             q[4 * u + 3] = half ? c.w : c.z;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) q[4 * u + r] = z.flip ? -q[4 * u + r] : q[4 * u + r];
         }
     }
     const int key_row = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);  // the key that row `col` of an operand is
@@ -104,7 +114,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
         }
         if (BIAS && t < TILE + ROWS - 1) {
             const int c = j0 + t - (ROWS - 1) - i0 + z.Tq - 1;
-            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c] * LOG2E : 0.0f;
+            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c]) : 0.0f;
         }
     };
     const auto store = [&]() {
@@ -126,22 +136,22 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     const int first_chunk = part * s.a_part, last_chunk = min(s.chunks, first_chunk + s.a_part);
     const int first_key = first_chunk * CHUNK, last_key = min(last_chunk * CHUNK, block_end);
     const size_t row_index = (size_t)bh * z.Tq + i;
-    float top = -__builtin_inff(), total = 0.0f;
+    float top = NONE, total = 0.0f;
     Block16 out[DB];
 #pragma unroll
     for (int n = 0; n < DB; ++n) out[n] = zero16();
     if (AHEAD && first_key < last_key) load(first_key);
     for (int chunk = first_chunk; chunk < last_chunk && chunk * CHUNK < block_end; ++chunk) {
-        float m = -__builtin_inff(), l = 0.0f;
+        float m = NONE, l = 0.0f;
         Block16 o[DB];
 #pragma unroll
         for (int n = 0; n < DB; ++n) o[n] = zero16();
         const int chunk_end = min((chunk + 1) * CHUNK, block_end);
         for (int j0 = chunk * CHUNK; j0 < chunk_end; j0 += TILE) {
             if (!AHEAD) load(j0);
-            __syncthreads();
+            lds_barrier();
             store();
-            __syncthreads();
+            lds_barrier();
             if (AHEAD && j0 + TILE < last_key) load(j0 + TILE);
             if (j0 >= wave_end) continue;
             Block16 p[2] = {zero16(), zero16()};
@@ -158,7 +168,6 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
                         p[kb] = mfma(r == 0 ? a[kb].x : r == 1 ? a[kb].y : r == 2 ? a[kb].z : a[kb].w, q[4 * u + r], p[kb]);
             }
             // register 4 g + r of block kb: key j0 + 32 kb + 8 g + 2 r + half
-            float next = m;
             if (BIAS) {
                 const float* bias = Bs + (ROWS - 1 - (i - i0)) + half;
 #pragma unroll
@@ -166,34 +175,34 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         p[kb][r] = __builtin_fmaf(p[kb][r], z.factor, bias[32 * kb + 8 * (r / 4) + 2 * (r % 4)]);
-            } else {
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) p[kb][r] = p[kb][r] * z.factor;
             }
-            if (j0 + TILE > full) {
+            // the keys of the lane's parity that its row sees, key 32 kb + n at bit n of word kb
+            uint32_t see[2] = {~0u, ~0u};
+            const bool edge = j0 + TILE > full;
+            if (edge) {
                 const unsigned long long bits = mask_row ? mask_row[j0 >> 6] : ~0ull;
-                const int left = row_end - j0 - half;
-                const uint32_t words[2] = {(uint32_t)(bits >> half), (uint32_t)(bits >> 32) >> half};
+                const int left = row_end - j0;
+                const unsigned long long there = bits & (left >= 64 ? ~0ull : left > 0 ? (1ull << left) - 1 : 0ull);
+                see[0] = (uint32_t)(there >> half);
+                see[1] = (uint32_t)(there >> 32) >> half;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int n = 8 * (r / 4) + 2 * (r % 4);
-                        p[kb][r] = 32 * kb + n < left && (words[kb] >> n & 1) != 0 ? p[kb][r] : -__builtin_inff();
-                    }
+                    for (int r = 0; r < 16; ++r)
+                        p[kb][r] = (see[kb] >> (8 * (r / 4) + 2 * (r % 4)) & 1) != 0 ? p[kb][r] : -__builtin_inff();
             }
+            float next = -__builtin_inff();
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) next = larger(next, p[kb][r]);
+                for (int r = 0; r < 16; r += 2) next = larger(larger(next, p[kb][r]), p[kb][r + 1]);
             {
                 uint32_t x, w;
                 halves(__float_as_uint(next), &x, &w);
                 next = larger(__uint_as_float(x), __uint_as_float(w));
             }
-            const float base = finite_top(next), a = e2(m - base);
+            next = larger(m, BIAS ? next : next * z.factor);
+            const float base = base_of(next), a = e2(m - base);
             m = next;
             l = l * a;
             if (__any(a != 1.0f)) {
@@ -202,13 +211,19 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[n][r] = o[n][r] * a;
             }
+            const auto exponentials = [&](auto masked) {
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    p[kb][r] = e2(p[kb][r] - base);
-                    l = l + p[kb][r];
-                }
+                    for (int r = 0; r < 16; ++r) {
+                        float x = BIAS ? p[kb][r] - base : __builtin_fmaf(p[kb][r], z.factor, -base);
+                        if (decltype(masked)::value) x = (see[kb] >> (8 * (r / 4) + 2 * (r % 4)) & 1) != 0 ? x : NONE;
+                        p[kb][r] = e2(x);
+                        l = l + p[kb][r];
+                    }
+            };
+            if (edge) exponentials(std::true_type());
+            else exponentials(std::false_type());
             if (DROP) {
                 // the four words of a call are four keys': half 0 makes those of keys 0..3 of eight, half 1 of 4..7, and both take
                 // the bits of their parity from each
@@ -256,7 +271,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
                 if (half == 0) s.ml[row_index * s.chunks + chunk] = make_float2(m, both_l);
             }
         } else {
-            const float both = larger(top, m), base = finite_top(both), a = e2(top - base), e = e2(m - base);
+            const float both = larger(top, m), base = base_of(both), a = e2(top - base), e = e2(m - base);
             top = both;
             total = __builtin_fmaf(both_l, e, total * a);
 #pragma unroll
@@ -267,9 +282,12 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     }
     if (s.parts > 1 && i < z.Tq && half == 0)
         for (int chunk = max(first_chunk, (block_end + CHUNK - 1) / CHUNK); chunk < last_chunk; ++chunk)
-            s.ml[row_index * s.chunks + chunk] = make_float2(-__builtin_inff(), -1.0f);
-    const bool again = watch && __syncthreads_or(broken != broken);
-    if (s.parts == 1 && !again) {
+            s.ml[row_index * s.chunks + chunk] = make_float2(NONE, -1.0f);
+    if (s.broken) {  // a NaN or infinity in v, which the products' zeros hand to rows that do not see it
+        const int any = __syncthreads_or(broken != broken);
+        if (t == 0) s.broken[blockIdx.x] = any;
+    }
+    if (s.parts == 1) {
         const float inverse = reciprocal(total), f = DROP ? inverse * z.keep_factor : inverse;
         if (i < z.Tq) {
             float* row = y + (((size_t)b * z.Tq + i) * z.H + h) * z.D;
@@ -291,16 +309,26 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
                     }
                 }
             if (stats && half == 0) {
-                stats[2 * row_index] = finite_top(top);
+                stats[2 * row_index] = base_of(top);
                 stats[2 * row_index + 1] = inverse;
             }
         }
     }
-    if (!again) return;
-    // A NaN or infinity among these values, which the products' zeros would hand to rows that do not see it: row by row.
-    for (int row = i0 + wave; row < i0 + ROWS && row < z.Tq; row += 4) {
+}
+
+// Redoes the blocks whose values hold a NaN or infinity, row by row and pair by pair.
+__global__ void __launch_bounds__(256)
+repair(Problem z, Parts s, float* y, float* stats) {
+    if (s.broken[blockIdx.x] == 0) return;
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Place at = place_of(z, s);
+    const int b = at.bh / z.H, h = at.bh % z.H, len = keys_of(z, b);
+    const int block_end = z.causal ? max(0, min(len, min(at.i0 + ROWS, z.Tq) + z.start)) : len;
+    const int first_chunk = at.part * s.a_part, last_chunk = min(s.chunks, first_chunk + s.a_part);
+    for (int row = at.i0 + wave; row < at.i0 + ROWS && row < z.Tq; row += 4) {
         const int end = key_end(z, b, row);
-        const size_t n = (size_t)bh * z.Tq + row;
+        const size_t n = (size_t)at.bh * z.Tq + row;
         Joined all;
         for (int chunk = first_chunk; chunk < last_chunk && chunk * CHUNK < block_end; ++chunk) {
             const RowChunk r = row_chunk(z, seed, b, h, row, chunk * CHUNK, end, lane);
@@ -328,7 +356,7 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
         Joined all;
         for (int first = 0; first < s.chunks; first += 64) {
             const int c = first + lane;
-            const float2 ml = c < s.chunks ? s.ml[n * s.chunks + c] : make_float2(-__builtin_inff(), -1.0f);
+            const float2 ml = c < s.chunks ? s.ml[n * s.chunks + c] : make_float2(NONE, -1.0f);
             const bool there = ml.y != -1.0f;
             float run = ml.x;  // the largest of the chunks up to this one
 #pragma unroll
@@ -339,13 +367,12 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
             run = larger(all.top, run);
             float before = __shfl_up(run, 1, 64);
             if (lane == 0) before = all.top;
-            const float base = finite_top(run);
+            const float base = base_of(run);
             const float a = there ? e2(before - base) : 1.0f, e = there ? e2(ml.x - base) : 0.0f;
             const unsigned long long which = __ballot(there);
             all.top = __shfl(run, 63, 64);
             const float* o = s.o + (n * s.chunks + first) * z.D;
             const int count = min(64, s.chunks - first);
-#pragma unroll 8
             for (int k = 0; k < count; ++k) {
                 const float ak = __shfl(a, k, 64), ek = __shfl(e, k, 64), lk = __shfl(ml.y, k, 64);
                 if ((which >> k & 1) == 0) continue;
@@ -374,31 +401,42 @@ Parts parts_of(const Problem& z) {
     if (s.parts == 1) s.a_part = s.chunks;
     s.ml = nullptr;
     s.o = nullptr;
+    s.broken = nullptr;
     return s;
+}
+long long blocks_of(const Problem& z, const Parts& s) { return (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts; }
+// What a key holds must not reach a row that does not see it: under a causal mask or one of pairs.
+bool watched(const Problem& z) { return z.causal || z.mask != nullptr; }
+size_t parts_bytes(const Problem& z, const Parts& s) {
+    return s.parts > 1 ? ((size_t)z.B * z.H * z.Tq * s.chunks * (z.D + 2) * sizeof(float) + 15) / 16 * 16 : 0;
 }
 
 }  // namespace
 
-size_t forward_workspace(const Problem& z) {
+size_t forward_workspace(const Problem& z, bool masked) {
     const Parts s = parts_of(z);
-    return s.parts > 1 ? (size_t)z.B * z.H * z.Tq * s.chunks * (z.D + 2) * sizeof(float) : 0;
+    return parts_bytes(z, s) + (z.causal || masked ? blocks_of(z, s) * sizeof(int) : 0);
 }
 
 int forward(const Problem& z, float* y, float* stats, unsigned long long* used, void* workspace, hipStream_t stream) {
     Parts s = parts_of(z);
-    const long long rows = (long long)z.B * z.H * z.Tq;
+    const long long rows = (long long)z.B * z.H * z.Tq, blocks = blocks_of(z, s);
+    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     if (s.parts > 1) {
         s.ml = static_cast<float2*>(workspace);
         s.o = static_cast<float*>(workspace) + 2 * rows * s.chunks;
     }
-    const long long blocks = (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
-    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
+    if (watched(z)) s.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + parts_bytes(z, s));
     with_size(z.D, [&](auto db) {
         with_flags(z.bias != nullptr, z.threshold != 0, [&](auto bias, auto drop) {
             hipLaunchKernelGGL((forward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
         });
     });
     int rc = hipGetLastError();
+    if (rc == hipSuccess && s.broken) {
+        hipLaunchKernelGGL(repair, dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats);
+        rc = hipGetLastError();
+    }
     if (rc == hipSuccess && s.parts > 1) {
         hipLaunchKernelGGL(join_chunks, dim3(grid_of(rows, 4)), dim3(256), 0, stream, z, s, y, stats);
         rc = hipGetLastError();

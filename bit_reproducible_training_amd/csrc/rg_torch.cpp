@@ -1161,7 +1161,7 @@ struct AttentionFunction : torch::autograd::Function<AttentionFunction> {
         if (q.is_cuda()) {
             c10::DeviceGuard guard(q.device());
             size_t bytes = 0;
-            check(rg_attention_workspace(&c, &bytes), "attention plan");
+            check(rg_attention_workspace(&c, words.defined(), &bytes), "attention plan");
             Tensor ws;
             if (bytes > 0) ws = workspace_like(bytes, q);
             check(rg_attention_fp32(&c, q.data_ptr<float>(), k.data_ptr<float>(), v.data_ptr<float>(), lengths_or_null(keys),

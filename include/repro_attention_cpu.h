@@ -60,9 +60,17 @@ struct Call {
         for (int d = 0; d < D; ++d) s = __builtin_fmaf(a[d], b[d], s);
         return s;
     }
-    float score(long long b, long long h, long long i, long long j) const {
+    // t, and its difference to a maximum.
+    struct Score {
+        float s, t;
+        bool biased;
+        float factor;
+        float less(float m) const { return biased ? t - m : __builtin_fmaf(s, factor, -m); }
+    };
+    Score score(long long b, long long h, long long i, long long j) const {
         const float s = dot(query(b, h, i), key(b, h, j), c.D);
-        return bias ? __builtin_fmaf(s, factor, bias[h * (c.Tq + c.Tk - 1) + j - i + c.Tq - 1] * LOG2E) : s * factor;
+        if (!bias) return Score{s, s * factor, false, factor};
+        return Score{s, __builtin_fmaf(s, factor, bias_term(bias[h * (c.Tq + c.Tk - 1) + j - i + c.Tq - 1])), true, factor};
     }
     bool kept(long long b, long long h, long long i, long long j) const {
         if (threshold == 0) return true;
@@ -73,33 +81,34 @@ struct Call {
 
 inline void forward_row(const Call& z, long long b, long long h, long long i, float* y, float* stats) {
     const int D = z.c.D;
-    float top = -__builtin_inff(), total = 0.0f, out[MAX_D] = {};
+    float top = NONE, total = 0.0f, out[MAX_D] = {};
     const long long end = z.end(b, i);
     for (long long first = 0; first < end; first += CHUNK) {
-        float m = -__builtin_inff(), l[2] = {0.0f, 0.0f}, o[MAX_D] = {};
+        float m = NONE, l[2] = {0.0f, 0.0f}, o[MAX_D] = {};
         for (long long j0 = first; j0 < first + CHUNK && j0 < end; j0 += TILE) {
-            float t[TILE], next = m;
+            Call::Score t[TILE];
+            float next = m;
             bool seen[TILE];
             for (int n = 0; n < TILE; ++n) {
                 seen[n] = j0 + n < end && z.seen(b, h, i, j0 + n);
                 if (!seen[n]) continue;
                 t[n] = z.score(b, h, i, j0 + n);
-                next = larger(next, t[n]);
+                next = larger(next, t[n].t);
             }
-            const float a = e2(m - finite_top(next));
+            const float a = e2(m - base_of(next));
             m = next;
             for (float& x : l) x = x * a;
             for (int d = 0; d < D; ++d) o[d] = o[d] * a;
             for (int n = 0; n < TILE; ++n) {
                 if (!seen[n]) continue;
-                const float p = e2(t[n] - finite_top(m));
+                const float p = e2(t[n].less(base_of(m)));
                 l[n & 1] = l[n & 1] + p;
                 const float u = z.kept(b, h, i, j0 + n) ? p : 0.0f;
                 const float* v = z.value(b, h, j0 + n);
                 for (int d = 0; d < D; ++d) o[d] = __builtin_fmaf(u, v[d], o[d]);
             }
         }
-        const float both = larger(top, m), a = e2(top - finite_top(both)), e = e2(m - finite_top(both));
+        const float both = larger(top, m), a = e2(top - base_of(both)), e = e2(m - base_of(both));
         top = both;
         total = __builtin_fmaf(l[0] + l[1], e, total * a);
         for (int d = 0; d < D; ++d) out[d] = __builtin_fmaf(o[d], e, out[d] * a);
@@ -108,7 +117,7 @@ inline void forward_row(const Call& z, long long b, long long h, long long i, fl
     const float f = z.threshold == 0 ? inverse : inverse * z.keep_factor;
     for (int d = 0; d < D; ++d) y[d] = out[d] * f + 0.0f;  // (no -0)
     if (stats) {
-        stats[0] = finite_top(top);
+        stats[0] = base_of(top);
         stats[1] = inverse;
     }
 }
@@ -164,7 +173,7 @@ inline void cpu_attention_grad(const rg_attention_config& c, const float* dy, co
     };
     const auto pair = [&](long long b, long long h, long long i, long long j) {
         const long long n = (b * c.H + h) * c.Tq + i;
-        const float p = e2(z.score(b, h, i, j) - stats[2 * n]) * stats[2 * n + 1];
+        const float p = e2(z.score(b, h, i, j).less(stats[2 * n])) * stats[2 * n + 1];
         float u = p, dp = cpu_detail::Call::dot(dy + place(b, i, h), z.value(b, h, j), D);
         if (z.threshold != 0) {
             const bool kept = z.kept(b, h, i, j);

@@ -4,20 +4,21 @@
 // and without FP contraction; fused multiply-adds are written out). Products are chains of fused
 // multiply-adds in ascending order from +0, which is what the matrix cores' float32 instructions compute.
 //
-// Forward, for a query and a head:
-//   score  s_j = fma chain over d of q_d k_jd;  t_j = s_j c (+ bias_j log2 e, fused), c = scale log2 e
-//   keys are taken in chunks of CHUNK, a chunk in tiles of TILE: m' = max(m, visible t of the tile), a = e2(m - m');
-//   p_j = e2(t_j - m'); l_even = l_even a, then + p_j of the even keys in ascending order, l_odd likewise;
-//   o_d = o_d a, then the chain over the tile's keys of p_j v_jd
+// Forward, for a query and a head, with c = scale log2 e (a negative scale's sign goes to the query):
+//   score  s_j = fma chain over d of q_d k_jd;  with a bias t_j = fma(s_j, c, bias_j log2 e), else t_j = s_j c
+//   keys are taken in chunks of CHUNK, a chunk in tiles of TILE: m' = max(m, visible t of the tile) from m = NONE, a = e2(m - m');
+//   p_j = e2(t_j - m'), without a bias e2(fma(s_j, c, -m')); l_even = l_even a, then + p_j of the even keys in ascending order,
+//   l_odd likewise; o_d = o_d a, then the chain over the tile's keys of p_j v_jd
 //   chunks are joined in ascending order: M' = max(M, m), a = e2(M - M'), b = e2(m - M'),
 //   L = fma(l_even + l_odd, b, L a), O_d = fma(o_d, b, O_d a)
 //   y_d = O_d (1 / L)
 // A masked key has p = 0 and nothing else of it takes part; a tile or chunk without visible keys changes nothing. So a
 // row's bits depend on its query and the keys it sees alone, not on the batch, the other queries or the padding.
-// -infinity as a maximum counts as 0 in the exponents; a row that sees nothing has L = 0, which 1 / L is 0 for.
+// NONE as a maximum counts as 0 in the exponents, so nothing below it does anything; a row that sees nothing has L = 0, which
+// 1 / L is 0 for. A NaN or infinite t gives its row NaN; a bias below LOWEST_BIAS (-infinity) counts as that.
 // With dropout the dropped p_j are 0 in the chain over v (not in l) and y is multiplied by factor / L.
 //
-// Backward: p_ij = e2(t_ij - M_i) (1 / L_i), delta_i = sum_d dy_d y_d, u_ij = p_ij kept factor,
+// Backward: p_ij = e2(t_ij - M_i) (1 / L_i), the difference as above, delta_i = sum_d dy_d y_d, u_ij = p_ij kept factor,
 //   ds_ij = p_ij ((dy_i . v_j) kept factor - delta_i)
 // Queries are taken in chunks of QUERY_CHUNK and keys in blocks of KEY_BLOCK:
 //   dv_j = sum over the group's heads of the sum over the chunks, both ascending, of the chunk's chain of u_ij dy_i; dk_j likewise of
@@ -32,26 +33,40 @@ using repro_gemm::bits_to_float;
 using repro_gemm::float_to_bits;
 
 constexpr int TILE = 64, CHUNK = 256, QUERY_CHUNK = 256, KEY_BLOCK = 128, MAX_D = 128;
-constexpr float LOG2E = 1.44269504f;
+constexpr float LOG2E = 1.44269504f, NONE = -1e37f, LOWEST_BIAS = -1e30f;
 inline float score_factor(double scale) { return (float)(scale * 1.4426950408889634); }
 
-// 2^t for t <= 0, within 1.1 units in the last place; 0 below -126, NaN for NaN, 1 for 0. t = n + f with n a whole number and
-// |f| <= 1/2, read off a sum with 1.5 2^23; 2^f by a polynomial whose coefficients were fitted to the least
-// largest relative error (2^-25.9).
-RG_HD inline float e2(float t) {
-    const float shifted = t + 12583039.0f;  // 1.5 2^23 + 127: the low bits are n + 127
-    const float f = t - (shifted - 12583039.0f);
-    float p = 0.00015353362f;
-    p = __builtin_fmaf(p, f, 0.0013398875f);
-    p = __builtin_fmaf(p, f, 0.009618437f);
-    p = __builtin_fmaf(p, f, 0.055503324f);
-    p = __builtin_fmaf(p, f, 0.24022648f);
-    p = __builtin_fmaf(p, f, 0.6931472f);
+// 2^x for finite x up to 0 and a rounding past it, within 1.6 units in the last place; 1 for 0, NaN for NaN and infinities. x = n + f
+// with n = floor x and 0 <= f < 1 (what rounds to 1 is the number before it); 2^f by a polynomial whose coefficients were fitted
+// to the least largest relative error (2^-23.3); times 2^n, rounded once where the result is subnormal.
+RG_HD inline float e2(float x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    int n;
+    asm("v_cvt_flr_i32_f32 %0, %1" : "=v"(n) : "v"(x));
+    const float f = __builtin_amdgcn_fractf(x);
+#else
+    const float below = __builtin_floorf(x);
+    float f = x - below;
+    f = f > 0.99999994f ? 0.99999994f : f;
+    const int n = below < -1000.0f ? -1000 : below > 1000.0f ? 1000 : below == below ? (int)below : 0;
+#endif
+    float p = 0.00186713f;
+    p = __builtin_fmaf(p, f, 0.009017031f);
+    p = __builtin_fmaf(p, f, 0.055799913f);
+    p = __builtin_fmaf(p, f, 0.24016444f);
+    p = __builtin_fmaf(p, f, 0.6931513f);
     p = __builtin_fmaf(p, f, 1.0f);
-    const float r = p * bits_to_float(float_to_bits(shifted) << 23);
-    return t < -126.0f ? 0.0f : r;
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_ldexpf(p, n);
+#else
+    return (float)((double)p * __builtin_bit_cast(double, (uint64_t)(1023 + n) << 52));
+#endif
 }
-RG_HD inline float finite_top(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+RG_HD inline float base_of(float m) { return m == NONE ? 0.0f : m; }
+RG_HD inline float bias_term(float bias) {
+    const float b = bias * LOG2E;
+    return b < LOWEST_BIAS ? LOWEST_BIAS : b;
+}
 // The larger of the two; the other where one is NaN.
 RG_HD inline float larger(float a, float b) { return __builtin_fmaxf(a, b); }
 // 1 / L, and 0 for a row that sees nothing.

@@ -43,7 +43,7 @@ def test_defaults():
                                     dict(q_stride=(ctypes.c_longlong * 3)(-1, 0, 0))])
 def test_attention_refuses_bad_sizes(change):
     n, c = ctypes.c_size_t(), config(**change)
-    assert _lib.lib.rg_attention_workspace(ctypes.byref(c), ctypes.byref(n)) == BAD
+    assert _lib.lib.rg_attention_workspace(ctypes.byref(c), 0, ctypes.byref(n)) == BAD
     assert _lib.lib.rg_attention_grad_workspace(ctypes.byref(c), 0, ctypes.byref(n)) == BAD
 
 

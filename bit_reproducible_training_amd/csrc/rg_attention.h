@@ -32,7 +32,7 @@ struct Problem {
     const unsigned long long* seed_at;
     unsigned long long seed;
     int B, Tq, Tk, H, KVH, D, group, causal, start;
-    int quads;  // whether the rows of q, k and v can be read 16 bytes at a time
+    int quads;  // whether all operands' rows can be taken 16 bytes at a time
     int flip;                          // a negative scale: scores are multiplied by -1, and factor is positive
     float factor, scale, keep_factor;
     uint32_t threshold;
@@ -219,6 +219,42 @@ __device__ __forceinline__ QueryPart query_part(const Problem& z, const Gradient
     return r;
 }
 
+// Rows in global memory, read and written by offsets in bytes without branches: past `bytes` loads give 0 and stores do nothing.
+typedef __amdgpu_buffer_rsrc_t Rows;
+constexpr uint32_t NOWHERE = 0xF0000000u;
+__device__ __forceinline__ Rows rows_at(const float* base, long long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base), (short)0, (int)(bytes > 0 ? bytes : 0), 0x00020000);
+}
+// `rows` rows (at most 128) of D values, `stride` values apart (at most MAX_ROW).
+__device__ __forceinline__ Rows rows_at(const float* base, int rows, long long stride, int D) {
+    return rows_at(base, rows > 0 ? ((rows - 1) * stride + D) * 4 : 0);
+}
+__device__ __forceinline__ float one(Rows r, uint32_t at) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0)); }
+__device__ __forceinline__ void put_one(Rows r, uint32_t at, float v) {
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, at, 0, 0);
+}
+// Four values from `at` on, of which the first `left` are there. QUADS: 16 bytes at once, all or none there.
+template <bool QUADS>
+__device__ __forceinline__ float4 four(Rows r, uint32_t at, int left) {
+    if (QUADS) {
+        const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, left > 0 ? at : NOWHERE, 0, 0);
+        return make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3]));
+    }
+    return make_float4(one(r, left > 0 ? at : NOWHERE), one(r, left > 1 ? at + 4 : NOWHERE), one(r, left > 2 ? at + 8 : NOWHERE),
+                       one(r, left > 3 ? at + 12 : NOWHERE));
+}
+template <bool QUADS>
+__device__ __forceinline__ void put_four(Rows r, uint32_t at, int left, const float* v) {
+    if (QUADS) {
+        typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+        const Words4 w = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+        __builtin_amdgcn_raw_buffer_store_b128(w, r, left > 0 ? at : NOWHERE, 0, 0);
+    } else {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) put_one(r, left > n ? at + 4 * n : NOWHERE, v[n]);
+    }
+}
+
 // A barrier for what the block's wavefronts hand each other in LDS; loads and stores of global memory may go on across it.
 __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -227,6 +263,8 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // ---- host ----
+
+constexpr long long MAX_ROW = RG_ATTENTION_MAX_ROW;  // values from a position to the next: 128 positions' offsets stay below 2^31
 
 constexpr long long MAX_BLOCKS = 1 << 23;  // of 256 threads: a launch takes fewer than 2^32
 
@@ -243,10 +281,14 @@ void with_size(int D, F run) {
     else run(std::integral_constant<int, 4>());
 }
 template <class F>
-void with_flags(bool a, bool b, F run) {
+void with_flags(bool a, bool b, bool c, F run) {
+    const auto third = [&](auto x, auto y) {
+        if (c) run(x, y, std::true_type());
+        else run(x, y, std::false_type());
+    };
     const auto second = [&](auto x) {
-        if (b) run(x, std::true_type());
-        else run(x, std::false_type());
+        if (b) third(x, std::true_type());
+        else third(x, std::false_type());
     };
     if (a) second(std::true_type());
     else second(std::false_type());

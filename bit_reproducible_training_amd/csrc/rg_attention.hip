@@ -2,6 +2,7 @@
 #include "rg_attention.h"
 
 #include <cmath>
+#include <initializer_list>
 
 namespace rg {
 namespace attention {
@@ -52,11 +53,12 @@ bool sizes_ok(const rg_attention_config* c) {
         return false;
     for (int n = 0; n < 3; ++n)
         if (c->q_stride[n] < 0 || c->k_stride[n] < 0 || c->v_stride[n] < 0 || c->mask_stride[n] < 0) return false;
-    return true;
+    return c->q_stride[1] <= MAX_ROW && c->k_stride[1] <= MAX_ROW && c->v_stride[1] <= MAX_ROW && (long long)c->H * c->D <= MAX_ROW;
 }
 
 Problem problem_of(const rg_attention_config* c, const float* q, const float* k, const float* v, const long long* key_lengths,
-                   const unsigned long long* mask, const float* bias, const unsigned long long* seed_at) {
+                   const unsigned long long* mask, const float* bias, const unsigned long long* seed_at,
+                   std::initializer_list<const float*> dense = {}) {
     Problem z;
     z.q = q, z.k = k, z.v = v, z.key_lengths = key_lengths, z.mask = mask, z.bias = bias, z.seed_at = seed_at;
     z.seed = c->seed;
@@ -71,6 +73,7 @@ Problem problem_of(const rg_attention_config* c, const float* q, const float* k,
     z.keep_factor = repro_dropout::factor_of(c->dropout);
     z.threshold = repro_dropout::threshold_of(c->dropout);
     uintptr_t odd = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v);
+    for (const float* p : dense) odd |= reinterpret_cast<uintptr_t>(p);
     for (int n = 0; n < 3; ++n) odd |= (uintptr_t)(c->q_stride[n] | c->k_stride[n] | c->v_stride[n]) * sizeof(float);
     z.quads = (odd & 15) == 0 && c->D % 4 == 0;
     for (int n = 0; n < 3; ++n) {
@@ -135,7 +138,7 @@ int rg_attention_fp32(const rg_attention_config* cfg, const float* q, const floa
     const long long rows = cfg->B * cfg->H * cfg->Tq;
     if (rows > 0 && !y) return hipErrorInvalidValue;
     if (rows == 0) return hipSuccess;
-    const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at);
+    const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at, {y});
     const size_t needed = forward_workspace(z, mask != nullptr);
     if (needed > 0 && (!workspace || workspace_bytes < needed || off(workspace, 16))) return hipErrorInvalidValue;
     return forward(z, y, stats, used, workspace, static_cast<hipStream_t>(stream));
@@ -163,7 +166,7 @@ int rg_attention_grad_fp32(const rg_attention_config* cfg, const float* dy, cons
     if ((rows > 0 && (!dy || !y || !stats || !dq)) || (keys > 0 && (!dk || !dv)) ||
         (needed > 0 && (!workspace || workspace_bytes < needed || off(workspace, 16))))
         return hipErrorInvalidValue;
-    const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at);
+    const Problem z = problem_of(cfg, q, k, v, key_lengths, mask, relative_bias, seed_at, {dy, dk, dv});
     hipStream_t st = static_cast<hipStream_t>(stream);
     const long long columns = drelative_bias ? (long long)z.H * (z.Tq + z.Tk - 1) : 0;
     if (rows == 0 || keys == 0) {  // no pair: zeros

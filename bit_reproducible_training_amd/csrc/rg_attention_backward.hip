@@ -70,13 +70,13 @@ __device__ __forceinline__ bool live(const Problem& z, int len, int block, int r
     return block * KEY_BLOCK < last_end(z, len, min(rows, z.Tq) - 1);
 }
 
-template <int DB, bool BIAS, bool DROP>
+template <int DB, bool BIAS, bool DROP, bool QUADS>
 __global__ void __launch_bounds__(256, DB <= 2 ? 2 : 1)
 backward_tiles(Problem z, Gradients g, Work w) {
     constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 16;
     __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds[STEP * DS_STRIDE];
     __shared__ float Bs[BIAS ? 160 : 1], Sums[BIAS ? DIAGONALS : 1];
-    __shared__ float4 Rows[STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits
+    __shared__ float4 Query[STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits
     __shared__ uint32_t Masks[STEP][4];
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
     const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5, wave = t >> 6;
@@ -86,7 +86,6 @@ backward_tiles(Problem z, Gradients g, Work w) {
     const int len = keys_of(z, b), key = k0 + 32 * wave + col;
     const size_t row0 = (size_t)bh * z.Tq;
     const size_t out_stride = (size_t)(w.direct ? z.KVH : 1) * z.D;
-    const bool whole = z.D % 4 == 0;
 
     if (!live(z, len, block, z.Tq)) {
         const size_t out = out_of(z, w, bh, 0);
@@ -102,22 +101,17 @@ backward_tiles(Problem z, Gradients g, Work w) {
 
     float k[16 * DB], v[16 * DB];  // value 2 n + half of the lane's key
     float broken = 0.0f;
-    const auto four = [&](const float* row, bool there, int d) {
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (!there || d >= z.D) return x;
-        if (z.quads) return *reinterpret_cast<const float4*>(row + d);
-        x.x = row[d];
-        if (d + 1 < z.D) x.y = row[d + 1];
-        if (d + 2 < z.D) x.z = row[d + 2];
-        if (d + 3 < z.D) x.w = row[d + 3];
-        return x;
-    };
+    // a thread brings four values in each 32 of a row
+    const int lrow = t >> 3, lcol = 4 * (t & 7);
     const auto keys_to_lds = [&](const float* base, long long stride) {
+        const Rows rows = rows_at(base + k0 * stride, min(KEY_BLOCK, len - k0), stride, z.D);
+        const uint32_t at = ((uint32_t)lrow * (uint32_t)stride + lcol) * 4;
+        float4 x[4 * DB];
 #pragma unroll
-        for (int n = 0; n < 4 * DB; ++n) {
-            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4;
-            *reinterpret_cast<float4*>(Ks + row * KS + d) = four(base + (k0 + row) * stride, k0 + row < len, d);
-        }
+        for (int n = 0; n < 4 * DB; ++n)
+            x[n] = four<QUADS>(rows, at + 128 * (n % DB) + n / DB * 128 * (uint32_t)stride, z.D - lcol - 32 * (n % DB));
+#pragma unroll
+        for (int n = 0; n < 4 * DB; ++n) *reinterpret_cast<float4*>(Ks + (lrow + n / DB * 32) * KS + lcol + 32 * (n % DB)) = x[n];
     };
     const auto take = [&](float* to) {
 #pragma unroll
@@ -142,73 +136,52 @@ backward_tiles(Problem z, Gradients g, Work w) {
 
     const float* qbase = query_at(z, b, h, 0);
     const float* ybase = g.dy + ((size_t)b * z.Tq * z.H + h) * z.D;
-    const size_t ystride = (size_t)z.H * z.D;
-    const bool ywhole = whole && (reinterpret_cast<uintptr_t>(g.dy) & 15) == 0;
+    const int ystride = z.H * z.D;
+    const uint32_t qat = ((uint32_t)lrow * (uint32_t)z.q_stride[1] + lcol) * 4, yat = ((uint32_t)lrow * (uint32_t)ystride + lcol) * 4;
     float4 qn[DB], yn[DB];
     float bn = 0.0f;
-    float4 rn;
-    uint32_t mn = 0;
+    float2 sn;
+    float en;
+    uint32_t mn = ~0u;
     const auto load = [&](int i0) {
-        const int t = fresh(threadIdx.x);
+        const Rows qr = rows_at(qbase + i0 * z.q_stride[1], min(STEP, z.Tq - i0), z.q_stride[1], z.D);
+        const Rows yr = rows_at(ybase + (long long)i0 * ystride, min(STEP, z.Tq - i0), ystride, z.D);
 #pragma unroll
-        for (int n = 0; n < DB; ++n) {
-            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4, i = i0 + row;
-            qn[n] = four(qbase + i * z.q_stride[1], i < z.Tq, d);
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i < z.Tq && d < z.D) {
-                const float* p = ybase + i * ystride + d;
-                if (ywhole) {
-                    x = *reinterpret_cast<const float4*>(p);
-                } else {
-                    x.x = p[0];
-                    if (d + 1 < z.D) x.y = p[1];
-                    if (d + 2 < z.D) x.z = p[2];
-                    if (d + 3 < z.D) x.w = p[3];
-                }
-            }
-            yn[n] = x;
+        for (int x = 0; x < DB; ++x) {
+            const int left = x < DB - 1 ? 4 : z.D - lcol - 32 * x;
+            qn[x] = four<QUADS>(qr, qat + 128 * x, left);
+            yn[x] = four<QUADS>(yr, yat + 128 * x, left);
         }
-        if (t < STEP) {
-            const int i = i0 + t;
-            rn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (i < z.Tq) {
-                rn.x = g.stats[2 * (row0 + i)];
-                rn.y = g.stats[2 * (row0 + i) + 1];
-                rn.z = g.delta[row0 + i];
-                rn.w = __int_as_float(last_end(z, len, i));
-            }
-        } else if (t >= 64 && t < 64 + 4 * STEP) {
-            const int i = i0 + (t - 64) / 4, word = k0 / 32 + (t & 3);
-            mn = ~0u;
-            if (z.mask && i < z.Tq && word * 32 < z.Tk) {
-                const unsigned long long* row = z.mask + b * z.mask_stride[0] + h * z.mask_stride[1] + i * z.mask_stride[2];
-                mn = (uint32_t)(row[word >> 1] >> (32 * (word & 1)));
-            }
+        const size_t row = row0 + min(i0 + (t & (STEP - 1)), z.Tq - 1);
+        sn = reinterpret_cast<const float2*>(g.stats)[row];
+        en = g.delta[row];
+        if (z.mask) {
+            const int i = min(i0 + ((t >> 2) & (STEP - 1)), z.Tq - 1), word = min(k0 / 32 + (t & 3), (z.Tk - 1) / 32);
+            const unsigned long long* m = z.mask + b * z.mask_stride[0] + h * z.mask_stride[1] + i * z.mask_stride[2];
+            mn = reinterpret_cast<const uint32_t*>(m)[word];
         }
-        if (BIAS && t < KEY_BLOCK + STEP - 1) {
-            const int c = k0 + t - (STEP - 1) - i0 + z.Tq - 1;
-            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c]) : 0.0f;
+        if (BIAS) {
+            const int c = k0 + t - (STEP - 1) - i0 + z.Tq - 1;  // (outside of the bias no pair needs it)
+            bn = z.bias[(size_t)h * (z.Tq + z.Tk - 1) + max(0, min(c, z.Tq + z.Tk - 2))];
         }
     };
-    const auto store = [&]() {
-        const int t = fresh(threadIdx.x);
+    const auto store = [&](int i0) {
 #pragma unroll
-        for (int n = 0; n < DB; ++n) {
-            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4;
-            const int to = row * QS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
-            *reinterpret_cast<float2*>(Qs + to) = make_float2(qn[n].x, qn[n].z);
-            *reinterpret_cast<float2*>(Qs + to + 4) = make_float2(qn[n].y, qn[n].w);
-            *reinterpret_cast<float2*>(Ys + to) = make_float2(yn[n].x, yn[n].z);
-            *reinterpret_cast<float2*>(Ys + to + 4) = make_float2(yn[n].y, yn[n].w);
+        for (int x = 0; x < DB; ++x) {
+            const int d = lcol + 32 * x, to = lrow * QS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
+            *reinterpret_cast<float2*>(Qs + to) = make_float2(qn[x].x, qn[x].z);
+            *reinterpret_cast<float2*>(Qs + to + 4) = make_float2(qn[x].y, qn[x].w);
+            *reinterpret_cast<float2*>(Ys + to) = make_float2(yn[x].x, yn[x].z);
+            *reinterpret_cast<float2*>(Ys + to + 4) = make_float2(yn[x].y, yn[x].w);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                broken = __builtin_fmaf(part_of(qn[n], r), 0.0f, broken);
-                broken = __builtin_fmaf(part_of(yn[n], r), 0.0f, broken);
+                broken = __builtin_fmaf(part_of(qn[x], r), 0.0f, broken);
+                broken = __builtin_fmaf(part_of(yn[x], r), 0.0f, broken);
             }
         }
-        if (t < STEP) Rows[t] = rn;
-        else if (t >= 64 && t < 64 + 4 * STEP) Masks[(t - 64) / 4][t & 3] = mn;
-        if (BIAS && t < KEY_BLOCK + STEP - 1) Bs[t] = bn;
+        if (t < STEP) Query[t] = make_float4(sn.x, sn.y, en, __int_as_float(i0 + t < z.Tq ? last_end(z, len, i0 + t) : 0));
+        else if (t >= 128) Masks[(t >> 2) & (STEP - 1)][t & 3] = mn;
+        if (BIAS && t < KEY_BLOCK + STEP - 1) Bs[t] = bias_term(bn);
     };
     const int row_of = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);     // the query that row `col` of an operand is
     const int place_in = (col & 24) + 4 * (col & 1) + ((col >> 1) & 3);   // where value `col` of 32 is in Qs and Ys
@@ -227,7 +200,7 @@ backward_tiles(Problem z, Gradients g, Work w) {
         while (!live(z, len, block, i0 + STEP)) i0 += STEP;  // (the chunk's last step is live)
         __syncthreads();
         load(i0);
-        store();
+        store(i0);
         if (BIAS)
             for (int n = t; n < DIAGONALS; n += 256) Sums[n] = 0.0f;
         lds_barrier();
@@ -274,7 +247,7 @@ backward_tiles(Problem z, Gradients g, Work w) {
 #pragma unroll
                 for (int n = 0; n < 16; ++n) {
                     const int q = 8 * (n / 4) + 2 * (n % 4) + half;
-                    const float4 row = Rows[q];
+                    const float4 row = Query[q];
                     const float x = BIAS ? __builtin_fmaf(s[n], z.factor, Bs[32 * wave + col - q + STEP - 1]) - row.x
                                          : __builtin_fmaf(s[n], z.factor, -row.x);
                     float p = e2(x) * row.y, d = dp[n], u = p;
@@ -321,7 +294,7 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 }
             }
             lds_barrier();
-            if (more) store();
+            if (more) store(i0 + STEP);
             {
                 const int c16 = lane & 15, group = lane >> 4, q0 = 16 * (wave & 1), d0 = 16 * DB * (wave >> 1);
                 Block4 dq[DB];
@@ -346,14 +319,14 @@ backward_tiles(Problem z, Gradients g, Work w) {
                     a = an;
                     if (n % 2 == 1) fence();
                 }
-                float* to = w.dq + ((size_t)slot * heads * z.Tq + row0 + i0 + q0 + 4 * group) * z.D;
+                const Rows rows = rows_at(w.dq + ((size_t)slot * heads * z.Tq + row0 + i0) * z.D, min(STEP, z.Tq - i0), z.D, z.D);
 #pragma unroll
-                for (int x = 0; x < DB; ++x)
+                for (int x = 0; x < DB; ++x) {
+                    const int d = d0 + 16 * x + c16;
+                    const uint32_t to = d < z.D ? ((uint32_t)(q0 + 4 * group) * z.D + d) * 4 : NOWHERE;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int d = d0 + 16 * x + c16;
-                        if (i0 + q0 + 4 * group + r < z.Tq && d < z.D) to[(size_t)r * z.D + d] = dq[x][r];
-                    }
+                    for (int r = 0; r < 4; ++r) put_one(rows, to + (uint32_t)(4 * r * z.D), dq[x][r]);
+                }
             }
             if (BIAS && w.diagonals && t < KEY_BLOCK + STEP - 1) {
                 const int t = fresh(threadIdx.x);
@@ -373,25 +346,28 @@ backward_tiles(Problem z, Gradients g, Work w) {
         const size_t chunk_out = out_of(z, w, bh, chunk);
         const bool add = w.parts == 1 && begun;
         begun = true;
-        if (key < z.Tk) {
-            float* kd = w.dk + chunk_out + key * out_stride;
-            float* vd = w.dv + chunk_out + key * out_stride;
+        const auto leave = [&](float* base, const Block16* sum, float scale) {
+            const Rows rows = rows_at(base + chunk_out + k0 * out_stride, min(KEY_BLOCK, z.Tk - k0), out_stride, z.D);
+            const uint32_t to = ((uint32_t)(32 * wave + col) * (uint32_t)out_stride + 4 * half) * 4;
+            float4 held[4 * DB];
+            if (add) {
 #pragma unroll
-            for (int x = 0; x < DB; ++x)
+                for (int n = 0; n < 4 * DB; ++n) held[n] = four<QUADS>(rows, to + 32 * n, z.D - 8 * n - 4 * half);
+            }
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    const int d = 32 * x + 8 * n + 4 * half;
+            for (int n = 0; n < 4 * DB; ++n) {
+                float v[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if (d + r >= z.D) continue;
-                        float a = dk[x][4 * n + r], c = dv[x][4 * n + r];
-                        if (add) a = kd[d + r] + a, c = vd[d + r] + c;
-                        if (last) a = a * z.scale + 0.0f, c = c + 0.0f;
-                        kd[d + r] = a;
-                        vd[d + r] = c;
-                    }
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = sum[n / 4][4 * (n % 4) + r];
+                    if (add) v[r] = part_of(held[n], r) + v[r];
+                    if (last) v[r] = v[r] * scale + 0.0f;
                 }
-        }
+                put_four<QUADS>(rows, to + 32 * n, z.D - 8 * n - 4 * half, v);
+            }
+        };
+        leave(w.dk, dk, z.scale);
+        leave(w.dv, dv, 1.0f);
         if (diagonals)
             for (int n = t; n < DIAGONALS; n += 256) diagonals[n] = Sums[n];
     }
@@ -578,8 +554,8 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
         w.count = std::min(most, p.blocks - first);
         const bool begins = first == 0, ends = first + w.count == p.blocks;
         with_size(z.D, [&](auto db) {
-            with_flags(z.bias != nullptr, z.threshold != 0, [&](auto bias, auto drop) {
-                hipLaunchKernelGGL((backward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value>),
+            with_flags(z.bias != nullptr, z.threshold != 0, z.quads != 0, [&](auto bias, auto drop, auto quads) {
+                hipLaunchKernelGGL((backward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value, decltype(quads)::value>),
                                    dim3((unsigned)(z.B * z.H * w.count * w.parts)), dim3(256), 0, stream, z, g, w);
             });
         });

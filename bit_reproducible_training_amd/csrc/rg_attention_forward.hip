@@ -32,18 +32,6 @@ __device__ __forceinline__ void halves(uint32_t v, uint32_t* low, uint32_t* high
     *high = s[1];
 }
 
-// 4 values of a row from d on; 0 past the row's end and where the row is not there.
-__device__ __forceinline__ float4 four(const float* row, bool there, int d, int D, bool quads) {
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (!there || d >= D) return v;
-    if (quads) return *reinterpret_cast<const float4*>(row + d);
-    v.x = row[d];
-    if (d + 1 < D) v.y = row[d + 1];
-    if (d + 2 < D) v.z = row[d + 2];
-    if (d + 3 < D) v.w = row[d + 3];
-    return v;
-}
-
 // A part of a row's chunks is handed on unjoined where the keys are split over blocks: m and l of each chunk (l = -1: nothing was seen
 // there) and its o.
 struct Parts {
@@ -63,11 +51,11 @@ __device__ __forceinline__ Place place_of(const Problem& z, const Parts& s) {
     return Place{(int)(blockIdx.x % heads), ((z.Tq + ROWS - 1) / ROWS - 1 - rest / s.parts) * ROWS, rest % s.parts};
 }
 
-// DB blocks of 32 values hold a head's.
-template <int DB, bool BIAS, bool DROP>
+// DB blocks of 32 values hold a head's; QUADS as in four().
+template <int DB, bool BIAS, bool DROP, bool QUADS>
 __global__ void __launch_bounds__(256, 2)
 forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
-    constexpr int DP = 32 * DB, KS = DP + 4, QUAD_LOADS = 2 * DB;
+    constexpr int DP = 32 * DB, KS = DP + 4;
     constexpr bool AHEAD = DB <= 2;  // the next tile in registers while one is worked on
     __shared__ float Ks[TILE * KS], Vs[TILE * DP], Bs[BIAS ? TILE + ROWS : 1];
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
@@ -87,10 +75,11 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
 
     float q[16 * DB];  // value 2 n + half of the row
     {
-        const float* row = query_at(z, b, h, min(i, z.Tq - 1));
+        const Rows rows = rows_at(query_at(z, b, h, i0), min(ROWS, z.Tq - i0), z.q_stride[1], z.D);
+        const uint32_t row = (uint32_t)(32 * wave + col) * (uint32_t)z.q_stride[1] * 4;
 #pragma unroll
         for (int u = 0; u < 4 * DB; ++u) {
-            const float4 a = four(row, i < z.Tq, 8 * u, z.D, z.quads), c = four(row, i < z.Tq, 8 * u + 4, z.D, z.quads);
+            const float4 a = four<QUADS>(rows, row + 32 * u, z.D - 8 * u), c = four<QUADS>(rows, row + 32 * u + 16, z.D - 8 * u - 4);
             q[4 * u] = half ? a.y : a.x;
             q[4 * u + 1] = half ? a.w : a.z;
             q[4 * u + 2] = half ? c.y : c.x;
@@ -101,26 +90,37 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     }
     const int key_row = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);  // the key that row `col` of an operand is
 
-    float4 kn[QUAD_LOADS], vn[QUAD_LOADS];
+    // a thread brings four values in each 32 of two rows of k and v
+    const int lrow = t >> 3, lcol = 4 * (t & 7);
+    uint32_t kat[2], vat[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        kat[n] = ((uint32_t)(lrow + 32 * n) * (uint32_t)z.k_stride[1] + lcol) * 4;
+        vat[n] = ((uint32_t)(lrow + 32 * n) * (uint32_t)z.v_stride[1] + lcol) * 4;
+    }
+    float4 kn[2 * DB], vn[2 * DB];
     float bn = 0.0f, broken = 0.0f;
     const float* kbase = key_at(z, b, h, 0);
     const float* vbase = value_at(z, b, h, 0);
     const auto load = [&](int j0) {
+        const int rows = min(TILE, len - j0);
+        const Rows kr = rows_at(kbase + j0 * z.k_stride[1], rows, z.k_stride[1], z.D);
+        const Rows vr = rows_at(vbase + j0 * z.v_stride[1], rows, z.v_stride[1], z.D);
 #pragma unroll
-        for (int n = 0; n < QUAD_LOADS; ++n) {
-            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4, j = j0 + row;
-            kn[n] = four(kbase + j * z.k_stride[1], j < len, d, z.D, z.quads);
-            vn[n] = four(vbase + j * z.v_stride[1], j < len, d, z.D, z.quads);
+        for (int n = 0; n < 2 * DB; ++n) {
+            const int x = n % DB, left = x < DB - 1 ? 4 : z.D - lcol - 32 * x;
+            kn[n] = four<QUADS>(kr, kat[n / DB] + 128 * x, left);
+            vn[n] = four<QUADS>(vr, vat[n / DB] + 128 * x, left);
         }
-        if (BIAS && t < TILE + ROWS - 1) {
-            const int c = j0 + t - (ROWS - 1) - i0 + z.Tq - 1;
-            bn = c >= 0 && c < z.Tq + z.Tk - 1 ? bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + c]) : 0.0f;
+        if (BIAS) {
+            const int c = j0 + t - (ROWS - 1) - i0 + z.Tq - 1;  // (outside of the bias no pair needs it)
+            bn = z.bias[(size_t)h * (z.Tq + z.Tk - 1) + max(0, min(c, z.Tq + z.Tk - 2))];
         }
     };
     const auto store = [&]() {
 #pragma unroll
-        for (int n = 0; n < QUAD_LOADS; ++n) {
-            const int at = t + 256 * n, row = at / (8 * DB), d = at % (8 * DB) * 4;
+        for (int n = 0; n < 2 * DB; ++n) {
+            const int row = lrow + n / DB * 32, d = lcol + 32 * (n % DB);
             float* p = Ks + row * KS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
             *reinterpret_cast<float2*>(p) = make_float2(kn[n].x, kn[n].z);
             *reinterpret_cast<float2*>(p + 4) = make_float2(kn[n].y, kn[n].w);
@@ -130,7 +130,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
             broken = __builtin_fmaf(vn[n].z, 0.0f, broken);
             broken = __builtin_fmaf(vn[n].w, 0.0f, broken);
         }
-        if (BIAS && t < TILE + ROWS - 1) Bs[t] = bn;
+        if (BIAS && t < TILE + ROWS - 1) Bs[t] = bias_term(bn);
     };
 
     const int first_chunk = part * s.a_part, last_chunk = min(s.chunks, first_chunk + s.a_part);
@@ -290,23 +290,16 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     if (s.parts == 1) {
         const float inverse = reciprocal(total), f = DROP ? inverse * z.keep_factor : inverse;
         if (i < z.Tq) {
-            float* row = y + (((size_t)b * z.Tq + i) * z.H + h) * z.D;
-            const bool whole = z.D % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+            const Rows rows = rows_at(y + (((size_t)b * z.Tq + i0) * z.H + h) * z.D, min(ROWS, z.Tq - i0), (long long)z.H * z.D, z.D);
+            const uint32_t row = ((uint32_t)(i - i0) * (uint32_t)(z.H * z.D) + 4 * half) * 4;
 #pragma unroll
             for (int n = 0; n < DB; ++n)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const int d = 32 * n + 8 * g + 4 * half;
                     float v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[r] = out[n][4 * g + r] * f + 0.0f;
-                    if (whole && d < z.D) {
-                        *reinterpret_cast<float4*>(row + d) = make_float4(v[0], v[1], v[2], v[3]);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (d + r < z.D) row[d + r] = v[r];
-                    }
+                    put_four<QUADS>(rows, row + 128 * n + 32 * g, z.D - 32 * n - 8 * g - 4 * half, v);
                 }
             if (stats && half == 0) {
                 stats[2 * row_index] = base_of(top);
@@ -428,8 +421,8 @@ int forward(const Problem& z, float* y, float* stats, unsigned long long* used, 
     }
     if (watched(z)) s.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + parts_bytes(z, s));
     with_size(z.D, [&](auto db) {
-        with_flags(z.bias != nullptr, z.threshold != 0, [&](auto bias, auto drop) {
-            hipLaunchKernelGGL((forward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
+        with_flags(z.bias != nullptr, z.threshold != 0, z.quads != 0, [&](auto bias, auto drop, auto quads) {
+            hipLaunchKernelGGL((forward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value, decltype(quads)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
         });
     });
     int rc = hipGetLastError();

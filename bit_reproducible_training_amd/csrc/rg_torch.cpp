@@ -1071,7 +1071,7 @@ Tensor dropout_apply(const Tensor& x, double p, uint64_t seed, const OptTensor& 
 // [B, T, heads, D] with its values next to each other; any other strides stay.
 Tensor attention_operand(const Tensor& t_) {
     const Tensor t = t_.resolve_neg();
-    return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+    return (t.size(-1) == 1 || t.stride(-1) == 1) && (t.size(1) <= 1 || t.stride(1) <= RG_ATTENTION_MAX_ROW) ? t : t.contiguous();
 }
 void set_strides(long long* to, const Tensor& t) {
     for (int n = 0; n < 3; ++n) to[n] = t.size(n) > 1 ? t.stride(n) : 0;
@@ -1245,7 +1245,7 @@ Tensor attention_apply(const Tensor& q, const Tensor& k, const Tensor& v, double
     static_assert(RG_ATTENTION_MAX_D == 128, "the message above");
     need(q.size(2) >= 1 && k.size(2) >= 1 && q.size(2) % k.size(2) == 0, "attention: k's heads must divide q's");
     need(q.size(1) <= RG_ATTENTION_MAX_LENGTH && k.size(1) <= RG_ATTENTION_MAX_LENGTH &&
-             q.size(0) * q.size(2) <= RG_ATTENTION_MAX_HEADS && q.size(0) <= RG_ATTENTION_MAX_HEADS,
+             q.size(0) * q.size(2) <= RG_ATTENTION_MAX_HEADS && q.size(2) * q.size(3) <= RG_ATTENTION_MAX_ROW && q.size(0) <= RG_ATTENTION_MAX_HEADS,
          "attention: too many positions or heads");
     need(std::isfinite((float)(scale * 1.4426950408889634)), "attention: the scale must be finite");
     need_probability(dropout, "attention");

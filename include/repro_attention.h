@@ -31,6 +31,7 @@ extern "C" {
 #define RG_ATTENTION_MAX_D 128
 #define RG_ATTENTION_MAX_LENGTH (1 << 22)
 #define RG_ATTENTION_MAX_HEADS (1 << 20) /* B * H */
+#define RG_ATTENTION_MAX_ROW (1 << 22)   /* H * D, and the strides of the positions */
 #define RG_RELATIVE_BIAS_MAX_BORDERS 512
 
 typedef struct rg_attention_config {

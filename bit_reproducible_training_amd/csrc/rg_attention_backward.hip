@@ -20,7 +20,7 @@ typedef float Block4 __attribute__((ext_vector_type(4)));
 
 constexpr int STEP = 32;                              // queries at a time
 constexpr int DIAGONALS = KEY_BLOCK + QUERY_CHUNK;    // distances of a block and chunk, one more than there are
-constexpr int DS_STRIDE = KEY_BLOCK + 4;
+constexpr int DS_STRIDE = KEY_BLOCK + STEP + 1;     // a row of dS and zeros, over which a diagonal goes on into its neighbours
 
 __device__ __forceinline__ Block16 zero16() {
     Block16 z;
@@ -73,11 +73,12 @@ __device__ __forceinline__ bool live(const Problem& z, int len, int block, int r
 template <int DB, bool BIAS, bool DROP, bool QUADS>
 __global__ void __launch_bounds__(256, DB <= 2 ? 2 : 1)
 backward_tiles(Problem z, Gradients g, Work w) {
-    constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 16;
-    __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds[STEP * DS_STRIDE];
+    constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 8;
+    __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds_[STEP + STEP * DS_STRIDE];
     __shared__ float Bs[BIAS ? 160 : 1], Sums[BIAS ? DIAGONALS : 1];
     __shared__ float4 Query[STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits
     __shared__ uint32_t Masks[STEP][4];
+    float* Ds = Ds_ + STEP;  // (zeros before the first row, too)
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
     const int t = threadIdx.x, lane = t & 63, col = lane & 31, half = lane >> 5, wave = t >> 6;
     const Place at = place_of(z, w);
@@ -121,6 +122,8 @@ backward_tiles(Problem z, Gradients g, Work w) {
             to[2 * n + 1] = half ? x.w : x.z;
         }
     };
+    for (int n = t; n < STEP; n += 256) Ds_[n] = 0.0f;
+    for (int n = t; n < STEP * (STEP + 1); n += 256) Ds[n / (STEP + 1) * DS_STRIDE + KEY_BLOCK + n % (STEP + 1)] = 0.0f;
     keys_to_lds(value_at(z, b, h, 0), z.v_stride[1]);
     __syncthreads();
     take(v);
@@ -185,8 +188,6 @@ backward_tiles(Problem z, Gradients g, Work w) {
     };
     const int row_of = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);     // the query that row `col` of an operand is
     const int place_in = (col & 24) + 4 * (col & 1) + ((col >> 1) & 3);   // where value `col` of 32 is in Qs and Ys
-    const int ds_place = 32 * wave + (col & 16) + 4 * (col & 3) + ((col >> 2) & 3);  // where a key is in Ds: 4 s + c of 16 at 4 c + s
-
     const int first_chunk = at.part * w.a_part, last_chunk = min(w.chunks, first_chunk + w.a_part);
     bool begun = false;
     for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
@@ -264,7 +265,7 @@ backward_tiles(Problem z, Gradients g, Work w) {
                     }
                     s[n] = u;
                     dp[n] = d;
-                    Ds[q * DS_STRIDE + ds_place] = d;
+                    Ds[q * DS_STRIDE + 32 * wave + col] = d;
                     if (n % 4 == 3) fence();
                 }
             };
@@ -300,24 +301,36 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 Block4 dq[DB];
 #pragma unroll
                 for (int x = 0; x < DB; ++x) dq[x] = Block4{0.0f, 0.0f, 0.0f, 0.0f};
-                const float* ds = Ds + (q0 + c16) * DS_STRIDE + 4 * group;
+                const float* ds = Ds + (q0 + c16) * DS_STRIDE + group;
                 const float* ks = Ks + group * KS + d0 + c16;
-                float4 a = *reinterpret_cast<const float4*>(ds);
+                float a[4], c[4][DB];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    a[r] = ds[4 * r];
+#pragma unroll
+                    for (int x = 0; x < DB; ++x) c[r][x] = ks[4 * r * KS + 16 * x];
+                }
 #pragma unroll
                 for (int n = 0; n < KEY_BLOCK / 16; ++n) {
-                    const float4 an = *reinterpret_cast<const float4*>(ds + 16 * (n + 1 < KEY_BLOCK / 16 ? n + 1 : n));
-                    float c[4][DB];
+                    const int ahead = 16 * (n + 1 < KEY_BLOCK / 16 ? n + 1 : n);
+                    float an[4], cn[4][DB];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        an[r] = ds[ahead + 4 * r];
+#pragma unroll
+                        for (int x = 0; x < DB; ++x) cn[r][x] = ks[(ahead + 4 * r) * KS + 16 * x];
+                    }
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int x = 0; x < DB; ++x) c[r][x] = ks[(16 * n + 4 * r) * KS + 16 * x];
+                        for (int x = 0; x < DB; ++x) dq[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], c[r][x], dq[x], 0, 0, 0);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int r = 0; r < 4; ++r) {
+                        a[r] = an[r];
 #pragma unroll
-                        for (int x = 0; x < DB; ++x)
-                            dq[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(part_of(a, r), c[r][x], dq[x], 0, 0, 0);
-                    a = an;
-                    if (n % 2 == 1) fence();
+                        for (int x = 0; x < DB; ++x) c[r][x] = cn[r][x];
+                    }
+                    fence();
                 }
                 const Rows rows = rows_at(w.dq + ((size_t)slot * heads * z.Tq + row0 + i0) * z.D, min(STEP, z.Tq - i0), z.D, z.D);
 #pragma unroll
@@ -329,15 +342,11 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 }
             }
             if (BIAS && w.diagonals && t < KEY_BLOCK + STEP - 1) {
-                const int t = fresh(threadIdx.x);
                 float* sum = Sums + t - (STEP - 1) - (i0 - c0) + QUERY_CHUNK - 1;
+                const float* ds = Ds + t - (STEP - 1);
                 float x = *sum;
 #pragma unroll
-                for (int q = 0; q < STEP; ++q) {
-                    const int c = t - (STEP - 1) + q, at_c = c & (KEY_BLOCK - 1);
-                    const float d = Ds[q * DS_STRIDE + (at_c & ~15) + 4 * (at_c & 3) + ((at_c >> 2) & 3)];
-                    x = x + (c == at_c ? d : 0.0f);
-                }
+                for (int q = 0; q < STEP; ++q) x = x + ds[q * (DS_STRIDE + 1)];
                 *sum = x;
             }
             lds_barrier();

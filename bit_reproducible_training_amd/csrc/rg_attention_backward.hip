@@ -176,11 +176,6 @@ backward_tiles(Problem z, Gradients g, Work w) {
             *reinterpret_cast<float2*>(Qs + to + 4) = make_float2(qn[x].y, qn[x].w);
             *reinterpret_cast<float2*>(Ys + to) = make_float2(yn[x].x, yn[x].z);
             *reinterpret_cast<float2*>(Ys + to + 4) = make_float2(yn[x].y, yn[x].w);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                broken = __builtin_fmaf(part_of(qn[x], r), 0.0f, broken);
-                broken = __builtin_fmaf(part_of(yn[x], r), 0.0f, broken);
-            }
         }
         if (t < STEP) Query[t] = make_float4(sn.x, sn.y, en, __int_as_float(i0 + t < z.Tq ? last_end(z, len, i0 + t) : 0));
         else if (t >= 128) Masks[(t >> 2) & (STEP - 1)][t & 3] = mn;
@@ -207,7 +202,6 @@ backward_tiles(Problem z, Gradients g, Work w) {
         lds_barrier();
         for (; i0 < c1; i0 += STEP) {
             const bool more = i0 + STEP < c1;
-            if (more) load(i0 + STEP);
             Block16 s = zero16(), dp = zero16();
             {
                 const float* qs = Qs + row_of * QS + 4 * half;
@@ -295,7 +289,7 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 }
             }
             lds_barrier();
-            if (more) store(i0 + STEP);
+            if (more) load(i0 + STEP);  // (in flight under dQ's products)
             {
                 const int c16 = lane & 15, group = lane >> 4, q0 = 16 * (wave & 1), d0 = 16 * DB * (wave >> 1);
                 Block4 dq[DB];
@@ -349,6 +343,7 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 for (int q = 0; q < STEP; ++q) x = x + ds[q * (DS_STRIDE + 1)];
                 *sum = x;
             }
+            if (more) store(i0 + STEP);
             lds_barrier();
         }
         const bool last = w.direct && chunk == w.chunks - 1;
@@ -375,12 +370,17 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 put_four<QUADS>(rows, to + 32 * n, z.D - 8 * n - 4 * half, v);
             }
         };
+#pragma unroll
+        for (int n = 0; n < 16 * DB; ++n) {
+            broken = __builtin_fmaf(dk[n / 16][n % 16], 0.0f, broken);
+            broken = __builtin_fmaf(dv[n / 16][n % 16], 0.0f, broken);
+        }
         leave(w.dk, dk, z.scale);
         leave(w.dv, dv, 1.0f);
         if (diagonals)
             for (int n = t; n < DIAGONALS; n += 256) diagonals[n] = Sums[n];
     }
-    if (w.broken) {  // a NaN or infinity, which the products' zeros hand to pairs that are not seen
+    if (w.broken) {  // a NaN or infinity, which the products' zeros hand to pairs that are not seen, shows in every key's sums
         const int any = __syncthreads_or(broken != broken);
         if (t == 0) w.broken[blockIdx.x] = any;
     }
@@ -491,13 +491,17 @@ sum_diagonals(Problem z, Work w, float* dbias, int begins, int ends) {
             const int k0 = (w.first + slot) * KEY_BLOCK;
             const int low = max(0, k0 - away), high = min(z.Tq, min(k0 + KEY_BLOCK, z.Tk) - away);  // the queries
             if (low >= high) continue;
+            const int chunk = low / QUERY_CHUNK, more = (high - 1) / QUERY_CHUNK;  // at most two chunks
+            const float* p = w.diagonals + (((size_t)h * w.count + slot) * w.chunks + chunk) * DIAGONALS + away - k0 + chunk * QUERY_CHUNK +
+                             QUERY_CHUNK - 1;
+            const size_t items = (size_t)z.H * w.count * w.chunks * DIAGONALS;
+#pragma unroll 8
             for (int b = 0; b < z.B; ++b) {
                 const int len = keys_of(z, b);
-                for (int chunk = low / QUERY_CHUNK; chunk * QUERY_CHUNK < high; ++chunk) {
-                    if (!live(z, len, w.first + slot, (chunk + 1) * QUERY_CHUNK)) continue;
-                    const float* p = w.diagonals + ((((size_t)b * z.H + h) * w.count + slot) * w.chunks + chunk) * DIAGONALS;
-                    s = s + p[away - k0 + chunk * QUERY_CHUNK + QUERY_CHUNK - 1];
-                }
+                // (what is not live was not written)
+                const float first = p[b * items], second = p[b * items + (more > chunk ? DIAGONALS + QUERY_CHUNK : 0)];
+                s = s + (live(z, len, w.first + slot, (chunk + 1) * QUERY_CHUNK) ? first : 0.0f);
+                s = s + (more > chunk && live(z, len, w.first + slot, (more + 1) * QUERY_CHUNK) ? second : 0.0f);
             }
         }
         dbias[n] = ends ? s + 0.0f : s;

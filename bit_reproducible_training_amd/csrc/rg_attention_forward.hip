@@ -100,37 +100,39 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     }
     float4 kn[2 * DB], vn[2 * DB];
     float bn = 0.0f, broken = 0.0f;
+    const auto watch = [&](const Block16* sum) {
+#pragma unroll
+        for (int n = 0; n < 16 * DB; ++n) broken = __builtin_fmaf(sum[n / 16][n % 16], 0.0f, broken);
+    };
     const float* kbase = key_at(z, b, h, 0);
     const float* vbase = value_at(z, b, h, 0);
-    const auto load = [&](int j0) {
-        const int rows = min(TILE, len - j0);
-        const Rows kr = rows_at(kbase + j0 * z.k_stride[1], rows, z.k_stride[1], z.D);
-        const Rows vr = rows_at(vbase + j0 * z.v_stride[1], rows, z.v_stride[1], z.D);
+    const auto load_keys = [&](int j0) {
+        const Rows rows = rows_at(kbase + j0 * z.k_stride[1], min(TILE, len - j0), z.k_stride[1], z.D);
 #pragma unroll
-        for (int n = 0; n < 2 * DB; ++n) {
-            const int x = n % DB, left = x < DB - 1 ? 4 : z.D - lcol - 32 * x;
-            kn[n] = four<QUADS>(kr, kat[n / DB] + 128 * x, left);
-            vn[n] = four<QUADS>(vr, vat[n / DB] + 128 * x, left);
-        }
+        for (int n = 0; n < 2 * DB; ++n) kn[n] = four<QUADS>(rows, kat[n / DB] + 128 * (n % DB), n % DB < DB - 1 ? 4 : z.D - lcol - 32 * (n % DB));
         if (BIAS) {
             const int c = j0 + t - (ROWS - 1) - i0 + z.Tq - 1;  // (outside of the bias no pair needs it)
             bn = z.bias[(size_t)h * (z.Tq + z.Tk - 1) + max(0, min(c, z.Tq + z.Tk - 2))];
         }
     };
-    const auto store = [&]() {
+    const auto load_values = [&](int j0) {
+        const Rows rows = rows_at(vbase + j0 * z.v_stride[1], min(TILE, len - j0), z.v_stride[1], z.D);
+#pragma unroll
+        for (int n = 0; n < 2 * DB; ++n) vn[n] = four<QUADS>(rows, vat[n / DB] + 128 * (n % DB), n % DB < DB - 1 ? 4 : z.D - lcol - 32 * (n % DB));
+    };
+    const auto store_keys = [&]() {
 #pragma unroll
         for (int n = 0; n < 2 * DB; ++n) {
-            const int row = lrow + n / DB * 32, d = lcol + 32 * (n % DB);
-            float* p = Ks + row * KS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
+            const int d = lcol + 32 * (n % DB);
+            float* p = Ks + (lrow + n / DB * 32) * KS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
             *reinterpret_cast<float2*>(p) = make_float2(kn[n].x, kn[n].z);
             *reinterpret_cast<float2*>(p + 4) = make_float2(kn[n].y, kn[n].w);
-            *reinterpret_cast<float4*>(Vs + row * DP + d) = vn[n];
-            broken = __builtin_fmaf(vn[n].x, 0.0f, broken);
-            broken = __builtin_fmaf(vn[n].y, 0.0f, broken);
-            broken = __builtin_fmaf(vn[n].z, 0.0f, broken);
-            broken = __builtin_fmaf(vn[n].w, 0.0f, broken);
         }
         if (BIAS && t < TILE + ROWS - 1) Bs[t] = bias_term(bn);
+    };
+    const auto store_values = [&]() {
+#pragma unroll
+        for (int n = 0; n < 2 * DB; ++n) *reinterpret_cast<float4*>(Vs + (lrow + n / DB * 32) * DP + lcol + 32 * (n % DB)) = vn[n];
     };
 
     const int first_chunk = part * s.a_part, last_chunk = min(s.chunks, first_chunk + s.a_part);
@@ -140,7 +142,10 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     Block16 out[DB];
 #pragma unroll
     for (int n = 0; n < DB; ++n) out[n] = zero16();
-    if (AHEAD && first_key < last_key) load(first_key);
+    if (AHEAD && first_key < last_key) {
+        load_keys(first_key);
+        load_values(first_key);
+    }
     for (int chunk = first_chunk; chunk < last_chunk && chunk * CHUNK < block_end; ++chunk) {
         float m = NONE, l = 0.0f;
         Block16 o[DB];
@@ -148,11 +153,16 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
         for (int n = 0; n < DB; ++n) o[n] = zero16();
         const int chunk_end = min((chunk + 1) * CHUNK, block_end);
         for (int j0 = chunk * CHUNK; j0 < chunk_end; j0 += TILE) {
-            if (!AHEAD) load(j0);
+            if (!AHEAD) load_keys(j0);
             lds_barrier();
-            store();
+            store_keys();
+            if (!AHEAD) load_values(j0);
+            store_values();
             lds_barrier();
-            if (AHEAD && j0 + TILE < last_key) load(j0 + TILE);
+            if (AHEAD && j0 + TILE < last_key) {
+                load_keys(j0 + TILE);
+                load_values(j0 + TILE);
+            }
             if (j0 >= wave_end) continue;
             Block16 p[2] = {zero16(), zero16()};
 #pragma unroll
@@ -259,6 +269,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
         halves(__float_as_uint(l), &x, &w);
         const float both_l = __uint_as_float(x) + __uint_as_float(w);
         if (s.parts > 1) {
+            watch(o);
             if (i < z.Tq) {
                 float* to = s.o + (row_index * s.chunks + chunk) * z.D;
 #pragma unroll
@@ -283,7 +294,8 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     if (s.parts > 1 && i < z.Tq && half == 0)
         for (int chunk = max(first_chunk, (block_end + CHUNK - 1) / CHUNK); chunk < last_chunk; ++chunk)
             s.ml[row_index * s.chunks + chunk] = make_float2(NONE, -1.0f);
-    if (s.broken) {  // a NaN or infinity in v, which the products' zeros hand to rows that do not see it
+    if (s.parts == 1) watch(out);
+    if (s.broken) {  // a NaN or infinity in v, which the products' zeros hand to rows that do not see it, shows in every row
         const int any = __syncthreads_or(broken != broken);
         if (t == 0) s.broken[blockIdx.x] = any;
     }

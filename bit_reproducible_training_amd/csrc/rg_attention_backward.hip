@@ -140,13 +140,14 @@ backward_tiles(Problem z, Gradients g, Work w) {
     const float* qbase = query_at(z, b, h, 0);
     const float* ybase = g.dy + ((size_t)b * z.Tq * z.H + h) * z.D;
     const int ystride = z.H * z.D;
-    const uint32_t qat = ((uint32_t)lrow * (uint32_t)z.q_stride[1] + lcol) * 4, yat = ((uint32_t)lrow * (uint32_t)ystride + lcol) * 4;
     float4 qn[DB], yn[DB];
     float bn = 0.0f;
     float2 sn;
     float en;
     uint32_t mn = ~0u;
     const auto load = [&](int i0) {
+        const int t = fresh(threadIdx.x), lrow = t >> 3, lcol = 4 * (t & 7);
+        const uint32_t qat = ((uint32_t)lrow * (uint32_t)z.q_stride[1] + lcol) * 4, yat = ((uint32_t)lrow * (uint32_t)ystride + lcol) * 4;
         const Rows qr = rows_at(qbase + i0 * z.q_stride[1], min(STEP, z.Tq - i0), z.q_stride[1], z.D);
         const Rows yr = rows_at(ybase + (long long)i0 * ystride, min(STEP, z.Tq - i0), ystride, z.D);
 #pragma unroll
@@ -169,6 +170,7 @@ backward_tiles(Problem z, Gradients g, Work w) {
         }
     };
     const auto store = [&](int i0) {
+        const int t = fresh(threadIdx.x), lrow = t >> 3, lcol = 4 * (t & 7);
 #pragma unroll
         for (int x = 0; x < DB; ++x) {
             const int d = lcol + 32 * x, to = lrow * QS + (d & ~7) + (d & 4) / 2;  // values 2 r + h of eight at 4 h + r
@@ -327,9 +329,10 @@ backward_tiles(Problem z, Gradients g, Work w) {
                     fence();
                 }
                 const Rows rows = rows_at(w.dq + ((size_t)slot * heads * z.Tq + row0 + i0) * z.D, min(STEP, z.Tq - i0), z.D, z.D);
+                const int from = fresh(lane);
 #pragma unroll
                 for (int x = 0; x < DB; ++x) {
-                    const int d = d0 + 16 * x + c16;
+                    const int d = d0 + 16 * x + (from & 15), group = from >> 4;
                     const uint32_t to = d < z.D ? ((uint32_t)(q0 + 4 * group) * z.D + d) * 4 : NOWHERE;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) put_one(rows, to + (uint32_t)(4 * r * z.D), dq[x][r]);
@@ -352,7 +355,8 @@ backward_tiles(Problem z, Gradients g, Work w) {
         begun = true;
         const auto leave = [&](float* base, const Block16* sum, float scale) {
             const Rows rows = rows_at(base + chunk_out + k0 * out_stride, min(KEY_BLOCK, z.Tk - k0), out_stride, z.D);
-            const uint32_t to = ((uint32_t)(32 * wave + col) * (uint32_t)out_stride + 4 * half) * 4;
+            const int lane = fresh(threadIdx.x) & 63, half = lane >> 5;
+            const uint32_t to = ((uint32_t)(32 * wave + (lane & 31)) * (uint32_t)out_stride + 4 * half) * 4;
             float4 held[4 * DB];
             if (add) {
 #pragma unroll

@@ -350,6 +350,198 @@ repair(Problem z, Parts s, float* y, float* stats) {
     }
 }
 
+// Few queries: a block takes a chunk of keys for all rows that share a head of keys (at most FEW), a thread a key for the
+// scores, then a wavefront a row and a lane a value. Bound by HBM: the keys are read into LDS as the values are on their way, and the
+// values take their place there. A single query of 4096 keys for 16 items of 12 heads of 64: FEW_TIME.
+constexpr int FEW = 8;
+
+template <int DB, bool QUADS>
+__global__ void __launch_bounds__(256, DB <= 2 ? 2 : 1)
+few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
+    constexpr int DP = 32 * DB, STRIDE = DP + 4;
+    __shared__ float KV[CHUNK * STRIDE], Qs[FEW][DP], Tops[FEW][4], Ls[FEW][2];
+    __shared__ __attribute__((aligned(16))) float P[FEW][CHUNK];
+    __shared__ unsigned long long See[FEW][4];
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    if (used && blockIdx.x == 0 && threadIdx.x == 0) *used = seed;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int heads = z.B * z.KVH, chunk = (int)(blockIdx.x / heads);
+    const int b = (int)(blockIdx.x % heads) / z.KVH, kvh = (int)(blockIdx.x % heads) % z.KVH, h0 = kvh * z.group;
+    const int rows = z.group * z.Tq, first = chunk * CHUNK, len = keys_of(z, b);
+    const auto row_of = [&](int r) { return ((size_t)b * z.H + h0 + r / z.Tq) * z.Tq + r % z.Tq; };
+    if (s.chunks > 1 && first >= key_end(z, b, z.Tq - 1)) {
+        if (t < rows) s.ml[row_of(t) * s.chunks + chunk] = make_float2(NONE, -1.0f);
+        return;
+    }
+    const int lrow = t >> 3, lcol = 4 * (t & 7);
+    const auto load = [&](const float* base, long long stride, float4* to) {
+        const uint32_t at = ((uint32_t)lrow * (uint32_t)stride + lcol) * 4;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // (128 rows are what the offsets reach)
+            const Rows from = rows_at(base + (long long)(first + 128 * half) * stride, min(128, len - first - 128 * half), stride, z.D);
+#pragma unroll
+            for (int n = 0; n < 4 * DB; ++n)
+                to[4 * DB * half + n] = four<QUADS>(from, at + 128 * (n % DB) + n / DB * 128 * (uint32_t)stride, z.D - lcol - 32 * (n % DB));
+        }
+    };
+    const auto store = [&](const float4* from) {
+#pragma unroll
+        for (int n = 0; n < 8 * DB; ++n) *reinterpret_cast<float4*>(KV + (lrow + n / DB * 32) * STRIDE + lcol + 32 * (n % DB)) = from[n];
+    };
+    float4 held[8 * DB], next[8 * DB];
+    load(key_at(z, b, h0, 0), z.k_stride[1], held);
+    load(value_at(z, b, h0, 0), z.v_stride[1], next);
+    for (int n = t; n < rows * DP; n += 256) {
+        const int r = n / DP, d = n % DP;
+        const float x = d < z.D ? query_at(z, b, h0 + r / z.Tq, r % z.Tq)[d] : 0.0f;
+        Qs[r][d] = z.flip ? -x : x;
+    }
+    store(held);
+    __syncthreads();
+
+    const int j = first + t;
+    float sum[FEW];
+#pragma unroll
+    for (int r = 0; r < FEW; ++r) sum[r] = 0.0f;
+    for (int d = 0; d < DP; d += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(KV + t * STRIDE + d);
+#pragma unroll
+        for (int r = 0; r < FEW; ++r) {
+            if (r >= rows) break;
+            const float4 q = *reinterpret_cast<const float4*>(&Qs[r][d]);
+            sum[r] = __builtin_fmaf(q.x, k.x, sum[r]);
+            sum[r] = __builtin_fmaf(q.y, k.y, sum[r]);
+            sum[r] = __builtin_fmaf(q.z, k.z, sum[r]);
+            sum[r] = __builtin_fmaf(q.w, k.w, sum[r]);
+        }
+    }
+    float term[FEW];
+    bool see[FEW];
+#pragma unroll
+    for (int r = 0; r < FEW; ++r) {
+        if (r >= rows) break;
+        const int i = r % z.Tq, h = h0 + r / z.Tq;
+        see[r] = seen(z, b, h, i, j, key_end(z, b, i));
+        term[r] = see[r] ? z.bias ? __builtin_fmaf(sum[r], z.factor, bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + j - i + z.Tq - 1]))
+                                  : sum[r] * z.factor : NONE;
+        const float top = wave_max(term[r]);
+        const unsigned long long which = __ballot(see[r]);
+        if (lane == 0) {
+            Tops[r][wave] = top;
+            See[r][wave] = which;
+        }
+    }
+    __syncthreads();
+    store(next);
+#pragma unroll
+    for (int r = 0; r < FEW; ++r) {
+        if (r >= rows) break;
+        float m = NONE;
+        for (int w = 0; w <= wave; ++w) m = larger(m, Tops[r][w]);
+        const float base = base_of(m);
+        const float p = see[r] ? e2(z.bias ? term[r] - base : __builtin_fmaf(sum[r], z.factor, -base)) : 0.0f;
+        P[r][t] = p;
+    }
+    __syncthreads();
+
+    // the tiles' factors: what was there is multiplied by before a tile's terms come in
+    const auto factors = [&](int r, float* a) {
+        float m = NONE;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float up = larger(m, Tops[r][w]);
+            a[w] = e2(m - base_of(up));
+            m = up;
+        }
+        return m;
+    };
+    const int tiles = min(4, (len - first + 63) / 64);  // past the keys nothing changes
+    if (t >= 192 && t < 192 + 2 * rows) {
+        const int r = (t - 192) >> 1, parity = t & 1;
+        float a[4], l = 0.0f;
+        factors(r, a);
+        for (int w = 0; w < tiles; ++w) {
+            l = l * a[w];
+#pragma unroll 16
+            for (int n = 0; n < 32; ++n) l = l + P[r][64 * w + 2 * n + parity];
+        }
+        Ls[r][parity] = l;
+    }
+    if (z.threshold != 0) {
+        __syncthreads();
+        for (int r = 0; r < rows; ++r) P[r][t] = kept(z, seed, b, h0 + r / z.Tq, r % z.Tq, j) ? P[r][t] : 0.0f;
+        __syncthreads();
+    }
+    const bool some = z.causal || z.mask;
+    RowChunk mine[2];  // of rows wave and wave + 4
+    float a[2][4];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        mine[x].m = factors(wave + 4 * x < rows ? wave + 4 * x : 0, a[x]);
+        mine[x].o0 = mine[x].o1 = 0.0f;
+    }
+    const auto products = [&](auto both) {
+        constexpr int N = decltype(both)::value ? 2 : 1;
+        for (int w = 0; w < tiles; ++w) {
+            unsigned long long which = ~0ull;
+#pragma unroll
+            for (int x = 0; x < N; ++x) {
+                mine[x].o0 = mine[x].o0 * a[x][w];
+                mine[x].o1 = mine[x].o1 * a[x][w];
+                if (some) which &= See[wave + 4 * x][w];
+            }
+            const float* v = KV + 64 * w * STRIDE + lane;
+            if (which == ~0ull) {
+#pragma unroll 4
+                for (int n = 0; n < 64; n += 4) {
+                    float4 p[N];
+#pragma unroll
+                    for (int x = 0; x < N; ++x) p[x] = *reinterpret_cast<const float4*>(&P[wave + 4 * x][64 * w + n]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float v0 = v[(n + q) * STRIDE], v1 = DB > 2 ? v[(n + q) * STRIDE + 64] : 0.0f;
+#pragma unroll
+                        for (int x = 0; x < N; ++x) {
+                            const float u = q == 0 ? p[x].x : q == 1 ? p[x].y : q == 2 ? p[x].z : p[x].w;
+                            mine[x].o0 = __builtin_fmaf(u, v0, mine[x].o0);
+                            if (DB > 2) mine[x].o1 = __builtin_fmaf(u, v1, mine[x].o1);
+                        }
+                    }
+                }
+            } else {
+                for (int x = 0; x < N; ++x)
+                    for (int n = 0; n < 64; ++n) {  // what an unseen key holds stays out
+                        if ((See[wave + 4 * x][w] >> n & 1) == 0) continue;
+                        const float u = P[wave + 4 * x][64 * w + n];
+                        mine[x].o0 = __builtin_fmaf(u, v[n * STRIDE], mine[x].o0);
+                        if (DB > 2) mine[x].o1 = __builtin_fmaf(u, v[n * STRIDE + 64], mine[x].o1);
+                    }
+            }
+        }
+    };
+    if (wave + 4 < rows) products(std::true_type());
+    else if (wave < rows) products(std::false_type());
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < FEW / 4; ++x) {
+        const int r = wave + 4 * x;
+        if (r >= rows) break;
+        RowChunk& c = mine[x];
+        c.even = Ls[r][0];
+        c.odd = Ls[r][1];
+        if (s.chunks > 1) {
+            const size_t at = row_of(r) * s.chunks + chunk;
+            if (lane < z.D) s.o[at * z.D + lane] = c.o0;
+            if (lane + 64 < z.D) s.o[at * z.D + lane + 64] = c.o1;
+            if (lane == 0) s.ml[at] = make_float2(c.m, c.even + c.odd);
+        } else {
+            Joined all;
+            all.join(c);
+            finish_row(z, all, b, h0 + r / z.Tq, r % z.Tq, lane, y, stats);
+        }
+    }
+}
+
 // Joins the chunks of a row in their order: a wavefront takes a row, first a lane a chunk (the maxima before it and the
 // two factors), then a lane a value.
 __global__ void __launch_bounds__(256)
@@ -394,9 +586,18 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
 
 // The keys are split over blocks where the queries alone leave compute units idle: as many parts as bring the grid to two
 // blocks a compute unit, whole chunks each, as long as the chunks' results take at most a quarter of a gigabyte.
+bool few(const Problem& z) { return z.Tk > 0 && (long long)z.group * z.Tq <= FEW; }
 Parts parts_of(const Problem& z) {
     Parts s;
     s.chunks = (z.Tk + CHUNK - 1) / CHUNK;
+    s.ml = nullptr;
+    s.o = nullptr;
+    s.broken = nullptr;
+    if (few(z)) {
+        s.parts = s.chunks;
+        s.a_part = 1;
+        return s;
+    }
     const long long blocks = (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS);
     long long parts = blocks > 0 ? (512 + blocks - 1) / blocks : 1;
     if (blocks > 384 || (long long)z.B * z.H * z.Tq * s.chunks * (z.D + 2) > (1ll << 26)) parts = 1;
@@ -404,14 +605,14 @@ Parts parts_of(const Problem& z) {
     s.a_part = parts > 0 ? (int)((s.chunks + parts - 1) / parts) : 0;
     s.parts = s.a_part > 0 ? (s.chunks + s.a_part - 1) / s.a_part : 1;
     if (s.parts == 1) s.a_part = s.chunks;
-    s.ml = nullptr;
-    s.o = nullptr;
-    s.broken = nullptr;
     return s;
 }
-long long blocks_of(const Problem& z, const Parts& s) { return (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts; }
+long long blocks_of(const Problem& z, const Parts& s) {
+    return few(z) ? (long long)z.B * z.KVH * s.chunks : (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
+}
 // What a key holds must not reach a row that does not see it: under a causal mask or one of pairs.
-bool watched(const Problem& z) { return z.causal || z.mask != nullptr; }
+// (Few rows leave out each pair by itself.)
+bool watched(const Problem& z, bool masked) { return !few(z) && (z.causal || masked); }
 size_t parts_bytes(const Problem& z, const Parts& s) {
     return s.parts > 1 ? ((size_t)z.B * z.H * z.Tq * s.chunks * (z.D + 2) * sizeof(float) + 15) / 16 * 16 : 0;
 }
@@ -420,7 +621,7 @@ size_t parts_bytes(const Problem& z, const Parts& s) {
 
 size_t forward_workspace(const Problem& z, bool masked) {
     const Parts s = parts_of(z);
-    return parts_bytes(z, s) + (z.causal || masked ? blocks_of(z, s) * sizeof(int) : 0);
+    return parts_bytes(z, s) + (watched(z, masked) ? blocks_of(z, s) * sizeof(int) : 0);
 }
 
 int forward(const Problem& z, float* y, float* stats, unsigned long long* used, void* workspace, hipStream_t stream) {
@@ -431,8 +632,13 @@ int forward(const Problem& z, float* y, float* stats, unsigned long long* used, 
         s.ml = static_cast<float2*>(workspace);
         s.o = static_cast<float*>(workspace) + 2 * rows * s.chunks;
     }
-    if (watched(z)) s.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + parts_bytes(z, s));
+    if (watched(z, z.mask != nullptr)) s.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + parts_bytes(z, s));
     with_size(z.D, [&](auto db) {
+        if (few(z)) {
+            auto kernel = z.quads ? few_rows<decltype(db)::value, true> : few_rows<decltype(db)::value, false>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
+            return;
+        }
         with_flags(z.bias != nullptr, z.threshold != 0, z.quads != 0, [&](auto bias, auto drop, auto quads) {
             hipLaunchKernelGGL((forward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value, decltype(quads)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
         });

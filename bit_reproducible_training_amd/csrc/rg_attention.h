@@ -91,12 +91,6 @@ __device__ __forceinline__ bool kept(const Problem& z, uint64_t seed, int b, int
     return repro_dropout::pair_words(j >> 2, i, b * z.H + h, seed).w[j & 3] >= z.threshold;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int n = 32; n > 0; n >>= 1) v = v + __shfl_xor(v, n, 64);
-    return v;
-}
-
 // A row's share of a chunk of keys; lane d holds o_d and o_{d + 64}.
 struct RowChunk {
     float m, even, odd, o0, o1;

@@ -21,18 +21,50 @@ pack_mask(const unsigned char* mask, long long heads, long long queries, long lo
     }
 }
 
-// delta = sum over d of dy y, for each row [B][H][Tq].
+// delta = sum over d of dy y, for each row [B][H][Tq]: 16 lanes take a row, four values (and the four 64 on) each, and add what the
+// definition adds: values 32, 16, 8 and 4 apart are 8, 4, 2 and 1 lanes apart, and a lane holds the last four.
+template <int APART>
+__device__ __forceinline__ float turned(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + APART, 0xF, 0xF, true));
+}
+template <bool QUADS>
 __global__ void __launch_bounds__(256)
 row_deltas(Problem z, const float* dy, const float* y, float* delta) {
-    const int lane = threadIdx.x & 63;
+    const int d = 4 * (threadIdx.x & 15);
     const long long rows = (long long)z.B * z.H * z.Tq;
-    for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
-        const int i = (int)(n % z.Tq), t = (int)(n / z.Tq), b = t / z.H, h = t % z.H;
+    for (long long n = (long long)blockIdx.x * 16 + (threadIdx.x >> 4); n < (rows + 15) / 16 * 16; n += (long long)gridDim.x * 16) {
+        const long long row = n < rows ? n : rows - 1;
+        const int i = (int)(row % z.Tq), t = (int)(row / z.Tq), b = t / z.H, h = t % z.H;
         const size_t at = (((size_t)b * z.Tq + i) * z.H + h) * z.D;
-        float s = lane < z.D ? dy[at + lane] * y[at + lane] : 0.0f;
-        if (lane + 64 < z.D) s = __builtin_fmaf(dy[at + lane + 64], y[at + lane + 64], s);
-        s = wave_sum(s);
-        if (lane == 0) delta[n] = s;
+        float s[4] = {};
+        const auto take = [&](int from, auto add) {
+            float a[4] = {}, c[4] = {};
+            if (QUADS) {
+                if (from < z.D) {
+                    const float4 x = *reinterpret_cast<const float4*>(dy + at + from), w = *reinterpret_cast<const float4*>(y + at + from);
+                    a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
+                    c[0] = w.x, c[1] = w.y, c[2] = w.z, c[3] = w.w;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (from + k < z.D) a[k] = dy[at + from + k], c[k] = y[at + from + k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (from + k < z.D) s[k] = decltype(add)::value ? __builtin_fmaf(a[k], c[k], s[k]) : a[k] * c[k];
+        };
+        take(d, std::false_type());
+        if (z.D > 64) take(d + 64, std::true_type());
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            s[k] = s[k] + turned<8>(s[k]);
+            s[k] = s[k] + turned<4>(s[k]);
+            s[k] = s[k] + turned<2>(s[k]);
+            s[k] = s[k] + turned<1>(s[k]);
+        }
+        const float sum = (s[0] + s[2]) + (s[1] + s[3]);
+        if (d == 0 && n < rows) delta[n] = sum;
     }
 }
 
@@ -179,7 +211,9 @@ int rg_attention_grad_fp32(const rg_attention_config* cfg, const float* dy, cons
         zero(drelative_bias, columns);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(row_deltas, dim3(grid_of(rows, 4)), dim3(256), 0, st, z, dy, y, static_cast<float*>(workspace));
+    const bool quads = z.D % 4 == 0 && !off(dy, 16) && !off(y, 16);
+    hipLaunchKernelGGL(quads ? row_deltas<true> : row_deltas<false>, dim3(grid_of(rows, 16)), dim3(256), 0, st, z, dy, y,
+                       static_cast<float*>(workspace));
     return backward(z, dy, stats, dq, dk, dv, drelative_bias, workspace, st);
 }
 

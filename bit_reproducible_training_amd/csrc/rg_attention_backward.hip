@@ -484,32 +484,45 @@ sum_keys(Problem z, Work w, float* dk, float* dv) {
     }
 }
 
-// The bias's gradient: a thread a distance of a head, over the key blocks, the batch and the chunks.
+// The bias's gradient at each distance, over the key blocks, the batch and the chunks: a block takes 64 distances of a head, its
+// wavefronts bring the terms, TERMS at a time, and one adds them up in order. A key block and item have two terms: a
+// distance meets at most two chunks there.
+constexpr int TERMS = 64;
+
 __global__ void __launch_bounds__(256)
 sum_diagonals(Problem z, Work w, float* dbias, int begins, int ends) {
-    const int columns = z.Tq + z.Tk - 1;
-    for (long long n = (long long)blockIdx.x * 256 + threadIdx.x; n < (long long)z.H * columns; n += (long long)gridDim.x * 256) {
-        const int h = (int)(n / columns), away = (int)(n % columns) - (z.Tq - 1);
-        float s = begins ? 0.0f : dbias[n];
-        for (int slot = 0; slot < w.count; ++slot) {
-            const int k0 = (w.first + slot) * KEY_BLOCK;
-            const int low = max(0, k0 - away), high = min(z.Tq, min(k0 + KEY_BLOCK, z.Tk) - away);  // the queries
-            if (low >= high) continue;
-            const int chunk = low / QUERY_CHUNK, more = (high - 1) / QUERY_CHUNK;  // at most two chunks
-            const float* p = w.diagonals + (((size_t)h * w.count + slot) * w.chunks + chunk) * DIAGONALS + away - k0 + chunk * QUERY_CHUNK +
-                             QUERY_CHUNK - 1;
-            const size_t items = (size_t)z.H * w.count * w.chunks * DIAGONALS;
-#pragma unroll 8
-            for (int b = 0; b < z.B; ++b) {
-                const int len = keys_of(z, b);
-                // (what is not live was not written)
-                const float first = p[b * items], second = p[b * items + (more > chunk ? DIAGONALS + QUERY_CHUNK : 0)];
-                s = s + (live(z, len, w.first + slot, (chunk + 1) * QUERY_CHUNK) ? first : 0.0f);
-                s = s + (more > chunk && live(z, len, w.first + slot, (more + 1) * QUERY_CHUNK) ? second : 0.0f);
-            }
+    __shared__ float terms[TERMS][64];
+    const int columns = z.Tq + z.Tk - 1, across = (columns + 63) / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int h = blockIdx.x / across, column = (blockIdx.x % across) * 64 + lane, away = column - (z.Tq - 1);
+    const bool there = column < columns;
+    float s = begins || !there || wave > 0 ? 0.0f : dbias[(size_t)h * columns + column];
+    // the key blocks that one of the block's distances meets
+    const int least = away - lane, k_low = max(0, least) / KEY_BLOCK, k_high = min(z.Tk - 1, z.Tq - 1 + least + 63) / KEY_BLOCK;
+    const int first = max(0, k_low - w.first), last = min(w.count, k_high + 1 - w.first);
+    const int count = (last - first) * z.B * 2;
+    for (int at = 0; at < count; at += TERMS) {
+        float v[TERMS / 4];
+#pragma unroll
+        for (int n = 0; n < TERMS / 4; ++n) {  // (a term that is not there is read elsewhere and left out)
+            const int term = min(at + 4 * n + wave, count - 1), slot = first + term / 2 / z.B, b = term / 2 % z.B;
+            const int k0 = (w.first + slot) * KEY_BLOCK, low = max(0, k0 - away), high = min(z.Tq, min(k0 + KEY_BLOCK, z.Tk) - away);
+            const int chunk = low / QUERY_CHUNK + (term & 1);  // of the queries low .. high
+            const bool is = at + 4 * n + wave < count && there && low < high && chunk * QUERY_CHUNK < high &&
+                            live(z, keys_of(z, b), w.first + slot, (chunk + 1) * QUERY_CHUNK);
+            const float x = w.diagonals[is ? ((((size_t)b * z.H + h) * w.count + slot) * w.chunks + chunk) * DIAGONALS + away - k0 +
+                                                 chunk * QUERY_CHUNK + QUERY_CHUNK - 1 : 0];
+            v[n] = is ? x : 0.0f;
         }
-        dbias[n] = ends ? s + 0.0f : s;
+#pragma unroll
+        for (int n = 0; n < TERMS / 4; ++n) terms[4 * n + wave][lane] = v[n];
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll 16
+            for (int n = 0; n < TERMS; ++n) s = s + terms[n][lane];
+        }
+        __syncthreads();
     }
+    if (wave == 0 && there) dbias[(size_t)h * columns + column] = ends ? s + 0.0f : s;
 }
 
 // How the key blocks are taken: as many at a time as leave at most a gigabyte for dQ and half of one for the bias; the queries split
@@ -564,7 +577,8 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
     w.diagonals = dbias ? reinterpret_cast<float*>(base + p.diagonals) : nullptr;
     // a query's values must not reach keys that it does not see, nor a key's a query
     w.broken = z.causal || z.mask || z.key_lengths ? reinterpret_cast<int*>(base + p.broken) : nullptr;
-    if ((long long)z.B * z.H * w.count * w.parts > MAX_BLOCKS) return hipErrorInvalidValue;
+    if ((long long)z.B * z.H * w.count * w.parts > MAX_BLOCKS || (dbias && (long long)z.H * ((z.Tq + z.Tk + 62) / 64) > MAX_BLOCKS))
+        return hipErrorInvalidValue;
     const int most = w.count;
     for (int first = 0; first < p.blocks; first += most) {
         w.first = first;
@@ -584,7 +598,7 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
             hipLaunchKernelGGL(sum_keys, dim3(grid_of((long long)z.B * std::min(z.Tk, w.count * KEY_BLOCK) * z.KVH * z.D, 256)), dim3(256),
                                0, stream, z, w, dk, dv);
         if (dbias)
-            hipLaunchKernelGGL(sum_diagonals, dim3(grid_of((long long)z.H * (z.Tq + z.Tk - 1), 256)), dim3(256), 0, stream, z, w, dbias,
+            hipLaunchKernelGGL(sum_diagonals, dim3((unsigned)(z.H * ((z.Tq + z.Tk - 1 + 63) / 64))), dim3(256), 0, stream, z, w, dbias,
                                begins, ends);
         const int rc = hipGetLastError();
         if (rc != hipSuccess) return rc;

@@ -235,26 +235,20 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
             if (edge) exponentials(std::true_type());
             else exponentials(std::false_type());
             if (DROP) {
-                // the four words of a call are four keys': half 0 makes those of keys 0..3 of eight, half 1 of 4..7, and both take
-                // the bits of their parity from each
-                uint32_t bits = 0;
+                // the four words of a call are four keys': half 0 makes those of keys 0..3 of eight, half 1 of 4..7, and an exchange of
+                // the odd words of the one with the even words of the other leaves each half those of its parity
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
                     const auto w = repro_dropout::pair_words((uint32_t)(j0 / 4 + 2 * g + half), i, bh, seed);
+                    const auto first = __builtin_amdgcn_permlane32_swap(w.w[0], w.w[1], false, false);
+                    const auto second = __builtin_amdgcn_permlane32_swap(w.w[2], w.w[3], false, false);
+                    const uint32_t mine[4] = {first[0], second[0], first[1], second[1]};
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) bits |= (uint32_t)(w.w[n] >= z.threshold) << (4 * g + n);
-                }
-                uint32_t low, high;
-                halves(bits, &low, &high);
-                low >>= half;
-                high >>= half;
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int g = 4 * kb + r / 4, n = r % 4;
-                        p[kb][r] = ((n < 2 ? low : high) >> (4 * g + 2 * (n & 1)) & 1) != 0 ? p[kb][r] : 0.0f;
+                    for (int r = 0; r < 4; ++r) {
+                        const int at_r = 4 * (g % 4) + r;
+                        p[g / 4][at_r] = mine[r] >= z.threshold ? p[g / 4][at_r] : 0.0f;
                     }
+                }
             }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)

@@ -32,12 +32,13 @@ __device__ __forceinline__ void halves(uint32_t v, uint32_t* low, uint32_t* high
     *high = s[1];
 }
 
-// A part of a row's chunks is handed on unjoined where the keys are split over blocks: m and l of each chunk (l = -1: nothing was seen
-// there) and its o.
+// Where the keys are split over blocks, the first part's chunks are handed on joined and the others' one by one, as m, l (-1: nothing
+// was seen there) and o.
 struct Parts {
-    int parts, chunks, a_part;  // chunks a part
-    float2* ml;                 // [B][H][Tq][chunks]
-    float* o;                   // [B][H][Tq][chunks][D]
+    int parts, chunks, a_part, slots;  // chunks a part; slots: 1 and the chunks after the first part's
+    float2* ml;                        // [slots][B][H][Tq]
+    float* o;                          // [slots][B][H][Tq][D]
+    __device__ __forceinline__ int slot_of(int chunk) const { return chunk < a_part ? 0 : chunk - a_part + 1; }
     int* broken;                // a number for each block: whether `repair` has to redo it; null where it never has to
 };
 
@@ -138,6 +139,19 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     const int first_chunk = part * s.a_part, last_chunk = min(s.chunks, first_chunk + s.a_part);
     const int first_key = first_chunk * CHUNK, last_key = min(last_chunk * CHUNK, block_end);
     const size_t row_index = (size_t)bh * z.Tq + i;
+    const size_t all_rows = (size_t)z.B * z.H * z.Tq;
+    const auto leave = [&](int chunk, float m, float l, const Block16* sum) {
+        watch(sum);
+        const int slot = s.slot_of(chunk);
+        const Rows rows = rows_at(s.o + (slot * all_rows + (size_t)bh * z.Tq + i0) * z.D, min(ROWS, z.Tq - i0), z.D, z.D);
+        const uint32_t row = ((uint32_t)(i - i0) * z.D + 4 * half) * 4;
+#pragma unroll
+        for (int n = 0; n < 4 * DB; ++n) {
+            const float v[4] = {sum[n / 4][4 * (n % 4)], sum[n / 4][4 * (n % 4) + 1], sum[n / 4][4 * (n % 4) + 2], sum[n / 4][4 * (n % 4) + 3]};
+            put_four<QUADS>(rows, row + 32 * n, z.D - 8 * n - 4 * half, v);
+        }
+        if (half == 0 && i < z.Tq) s.ml[slot * all_rows + row_index] = make_float2(m, l);
+    };
     float top = NONE, total = 0.0f;
     Block16 out[DB];
 #pragma unroll
@@ -262,19 +276,8 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
         uint32_t x, w;
         halves(__float_as_uint(l), &x, &w);
         const float both_l = __uint_as_float(x) + __uint_as_float(w);
-        if (s.parts > 1) {
-            watch(o);
-            if (i < z.Tq) {
-                float* to = s.o + (row_index * s.chunks + chunk) * z.D;
-#pragma unroll
-                for (int n = 0; n < DB; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int d = 32 * n + 8 * (r / 4) + 4 * half + r % 4;
-                        if (d < z.D) to[d] = o[n][r];
-                    }
-                if (half == 0) s.ml[row_index * s.chunks + chunk] = make_float2(m, both_l);
-            }
+        if (part > 0) {
+            leave(chunk, m, both_l, o);
         } else {
             const float both = larger(top, m), base = base_of(both), a = e2(top - base), e = e2(m - base);
             top = both;
@@ -285,9 +288,10 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
                 for (int r = 0; r < 16; ++r) out[n][r] = __builtin_fmaf(o[n][r], e, out[n][r] * a);
         }
     }
-    if (s.parts > 1 && i < z.Tq && half == 0)
+    if (part > 0 && i < z.Tq && half == 0)
         for (int chunk = max(first_chunk, (block_end + CHUNK - 1) / CHUNK); chunk < last_chunk; ++chunk)
-            s.ml[row_index * s.chunks + chunk] = make_float2(NONE, -1.0f);
+            s.ml[s.slot_of(chunk) * all_rows + row_index] = make_float2(NONE, -1.0f);
+    if (part == 0 && s.parts > 1) leave(0, top, total, out);
     if (s.parts == 1) watch(out);
     if (s.broken) {  // a NaN or infinity in v, which the products' zeros hand to rows that do not see it, shows in every row
         const int any = __syncthreads_or(broken != broken);
@@ -331,16 +335,21 @@ repair(Problem z, Parts s, float* y, float* stats) {
         Joined all;
         for (int chunk = first_chunk; chunk < last_chunk && chunk * CHUNK < block_end; ++chunk) {
             const RowChunk r = row_chunk(z, seed, b, h, row, chunk * CHUNK, end, lane);
-            if (s.parts > 1) {
-                float* to = s.o + (n * s.chunks + chunk) * z.D;
-                if (lane < z.D) to[lane] = r.o0;
-                if (lane + 64 < z.D) to[lane + 64] = r.o1;
-                if (lane == 0) s.ml[n * s.chunks + chunk] = make_float2(r.m, r.even + r.odd);
+            if (at.part > 0) {
+                const size_t to = s.slot_of(chunk) * (size_t)z.B * z.H * z.Tq + n;
+                if (lane < z.D) s.o[to * z.D + lane] = r.o0;
+                if (lane + 64 < z.D) s.o[to * z.D + lane + 64] = r.o1;
+                if (lane == 0) s.ml[to] = make_float2(r.m, r.even + r.odd);
             } else {
                 all.join(r);
             }
         }
         if (s.parts == 1) finish_row(z, all, b, h, row, lane, y, stats);
+        else if (at.part == 0) {
+            if (lane < z.D) s.o[n * z.D + lane] = all.o0;
+            if (lane + 64 < z.D) s.o[n * z.D + lane + 64] = all.o1;
+            if (lane == 0) s.ml[n] = make_float2(all.top, all.total);
+        }
     }
 }
 
@@ -364,7 +373,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
     const int rows = z.group * z.Tq, first = chunk * CHUNK, len = keys_of(z, b);
     const auto row_of = [&](int r) { return ((size_t)b * z.H + h0 + r / z.Tq) * z.Tq + r % z.Tq; };
     if (s.chunks > 1 && first >= key_end(z, b, z.Tq - 1)) {
-        if (t < rows) s.ml[row_of(t) * s.chunks + chunk] = make_float2(NONE, -1.0f);
+        if (t < rows) s.ml[(size_t)chunk * z.B * z.H * z.Tq + row_of(t)] = make_float2(NONE, -1.0f);
         return;
     }
     const int lrow = t >> 3, lcol = 4 * (t & 7);
@@ -524,7 +533,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
         c.even = Ls[r][0];
         c.odd = Ls[r][1];
         if (s.chunks > 1) {
-            const size_t at = row_of(r) * s.chunks + chunk;
+            const size_t at = (size_t)chunk * z.B * z.H * z.Tq + row_of(r);
             if (lane < z.D) s.o[at * z.D + lane] = c.o0;
             if (lane + 64 < z.D) s.o[at * z.D + lane + 64] = c.o1;
             if (lane == 0) s.ml[at] = make_float2(c.m, c.even + c.odd);
@@ -545,9 +554,9 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
     for (long long n = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); n < rows; n += (long long)gridDim.x * 4) {
         const int i = (int)(n % z.Tq), bh = (int)(n / z.Tq);
         Joined all;
-        for (int first = 0; first < s.chunks; first += 64) {
+        for (int first = 0; first < s.slots; first += 64) {
             const int c = first + lane;
-            const float2 ml = c < s.chunks ? s.ml[n * s.chunks + c] : make_float2(NONE, -1.0f);
+            const float2 ml = c < s.slots ? s.ml[c * rows + n] : make_float2(NONE, -1.0f);
             const bool there = ml.y != -1.0f;
             float run = ml.x;  // the largest of the chunks up to this one
 #pragma unroll
@@ -562,16 +571,25 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
             const float a = there ? e2(before - base) : 1.0f, e = there ? e2(ml.x - base) : 0.0f;
             const unsigned long long which = __ballot(there);
             all.top = __shfl(run, 63, 64);
-            const float* o = s.o + (n * s.chunks + first) * z.D;
-            const int count = min(64, s.chunks - first);
-            for (int k = 0; k < count; ++k) {
-                const float ak = __shfl(a, k, 64), ek = __shfl(e, k, 64), lk = __shfl(ml.y, k, 64);
-                if ((which >> k & 1) == 0) continue;
-                const float o0 = lane < z.D ? o[(size_t)k * z.D + lane] : 0.0f;
-                const float o1 = lane + 64 < z.D ? o[(size_t)k * z.D + lane + 64] : 0.0f;
-                all.total = __builtin_fmaf(lk, ek, all.total * ak);
-                all.o0 = __builtin_fmaf(o0, ek, all.o0 * ak);
-                all.o1 = __builtin_fmaf(o1, ek, all.o1 * ak);
+            const float* o = s.o + (first * rows + n) * z.D;
+            const int count = min(64, s.slots - first);
+            const int d0 = min(lane, z.D - 1), d1 = min(lane + 64, z.D - 1);
+            for (int k0 = 0; k0 < count; k0 += 8) {
+                float o0[8], o1[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float* p = o + min(k0 + k, count - 1) * rows * z.D;
+                    o0[k] = p[d0];
+                    o1[k] = p[d1];
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {  // (a chunk that was not written has factors 1 and 0)
+                    const float ak = __shfl(a, k0 + k, 64), ek = __shfl(e, k0 + k, 64), lk = __shfl(ml.y, k0 + k, 64);
+                    const bool is = (which >> (k0 + k) & 1) != 0;
+                    all.total = __builtin_fmaf(is ? lk : 0.0f, ek, all.total * ak);
+                    all.o0 = __builtin_fmaf(is ? o0[k] : 0.0f, ek, all.o0 * ak);
+                    all.o1 = __builtin_fmaf(is ? o1[k] : 0.0f, ek, all.o1 * ak);
+                }
             }
         }
         finish_row(z, all, bh / z.H, bh % z.H, i, lane, y, stats);
@@ -588,7 +606,7 @@ Parts parts_of(const Problem& z) {
     s.o = nullptr;
     s.broken = nullptr;
     if (few(z)) {
-        s.parts = s.chunks;
+        s.parts = s.slots = s.chunks;
         s.a_part = 1;
         return s;
     }
@@ -599,6 +617,7 @@ Parts parts_of(const Problem& z) {
     s.a_part = parts > 0 ? (int)((s.chunks + parts - 1) / parts) : 0;
     s.parts = s.a_part > 0 ? (s.chunks + s.a_part - 1) / s.a_part : 1;
     if (s.parts == 1) s.a_part = s.chunks;
+    s.slots = 1 + s.chunks - s.a_part;
     return s;
 }
 long long blocks_of(const Problem& z, const Parts& s) {
@@ -608,7 +627,7 @@ long long blocks_of(const Problem& z, const Parts& s) {
 // (Few rows leave out each pair by itself.)
 bool watched(const Problem& z, bool masked) { return !few(z) && (z.causal || masked); }
 size_t parts_bytes(const Problem& z, const Parts& s) {
-    return s.parts > 1 ? ((size_t)z.B * z.H * z.Tq * s.chunks * (z.D + 2) * sizeof(float) + 15) / 16 * 16 : 0;
+    return s.parts > 1 ? ((size_t)z.B * z.H * z.Tq * s.slots * (z.D + 2) * sizeof(float) + 15) / 16 * 16 : 0;
 }
 
 }  // namespace
@@ -624,7 +643,7 @@ int forward(const Problem& z, float* y, float* stats, unsigned long long* used, 
     if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     if (s.parts > 1) {
         s.ml = static_cast<float2*>(workspace);
-        s.o = static_cast<float*>(workspace) + 2 * rows * s.chunks;
+        s.o = static_cast<float*>(workspace) + 2 * rows * s.slots;
     }
     if (watched(z, z.mask != nullptr)) s.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + parts_bytes(z, s));
     with_size(z.D, [&](auto db) {

@@ -80,10 +80,16 @@ diagonal_sums(Sizes z, const float* dout, float* part) {
         if (n >= width) continue;
         const int j0 = n - (RUN - 1);  // the key beside the run's first row
         const int first = max(0, -j0), last = min(min(RUN, z.Tq - r * RUN), z.Tk - j0);
-        const float* p = dout + ((size_t)h * z.Tq + r * RUN) * z.Tk + j0;
+        const float* p = dout + ((size_t)h * z.Tq + r * RUN) * z.Tk;
         float s = 0.0f;
-#pragma unroll 16
-        for (int i = first; i < last; ++i) s = s + p[(size_t)i * (z.Tk + 1)];
+#pragma unroll
+        for (int i0 = 0; i0 < RUN; i0 += 16) {  // sixteen loads in flight; those of no pair read the run's first value and are left out
+            float v[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = p[i0 + i >= first && i0 + i < last ? (size_t)(i0 + i) * (z.Tk + 1) + j0 : 0];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s = s + (i0 + i >= first && i0 + i < last ? v[i] : 0.0f);
+        }
         part[((size_t)h * runs + r) * width + n] = s;
     }
 }
@@ -110,9 +116,16 @@ bucket_sums(Sizes z, Borders borders, const float* dout, const float* part, floa
         if (part) {
             const int away = (int)(n - (z.Tq - 1));
             const int first = max(0, -away) / RUN, last = min(z.Tq, z.Tk - away);  // rows max(0, -away) .. last
+            const int rows = (last + RUN - 1) / RUN - first;  // runs
+            const float* p = part + ((size_t)h * runs + first) * width + away + first * RUN + RUN - 1;
             v = 0.0f;
-#pragma unroll 8
-            for (int r = first; r * RUN < last; ++r) v = v + part[((size_t)h * runs + r) * width + away + r * RUN + RUN - 1];
+            for (int r0 = 0; r0 < rows; r0 += 16) {
+                float x[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = p[(size_t)min(r0 + r, rows - 1) * (width + RUN)];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) v = v + (r0 + r < rows ? x[r] : 0.0f);
+            }
         } else {
             v = dout[h * columns + n];
         }

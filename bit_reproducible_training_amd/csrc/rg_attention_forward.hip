@@ -626,8 +626,9 @@ long long blocks_of(const Problem& z, const Parts& s) {
 // What a key holds must not reach a row that does not see it: under a causal mask or one of pairs.
 // (Few rows leave out each pair by itself.)
 bool watched(const Problem& z, bool masked) { return !few(z) && (z.causal || masked); }
+size_t sums_offset(const Problem& z, const Parts& s) { return ((size_t)z.B * z.H * z.Tq * s.slots * sizeof(float2) + 15) / 16 * 16; }
 size_t parts_bytes(const Problem& z, const Parts& s) {
-    return s.parts > 1 ? ((size_t)z.B * z.H * z.Tq * s.slots * (z.D + 2) * sizeof(float) + 15) / 16 * 16 : 0;
+    return s.parts > 1 ? (sums_offset(z, s) + (size_t)z.B * z.H * z.Tq * s.slots * z.D * sizeof(float) + 15) / 16 * 16 : 0;
 }
 
 }  // namespace
@@ -643,7 +644,7 @@ int forward(const Problem& z, float* y, float* stats, unsigned long long* used, 
     if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     if (s.parts > 1) {
         s.ml = static_cast<float2*>(workspace);
-        s.o = static_cast<float*>(workspace) + 2 * rows * s.slots;
+        s.o = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_offset(z, s));
     }
     if (watched(z, z.mask != nullptr)) s.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + parts_bytes(z, s));
     with_size(z.D, [&](auto db) {

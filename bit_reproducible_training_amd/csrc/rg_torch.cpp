@@ -980,7 +980,7 @@ Tensor loss_apply(const Tensor& x, const Tensor& weight, const Tensor& target, i
 // A leaf keeps the stream that the first graph over it was made on for as long as such a graph lives, and a backward pass
 // waits for that stream; one that is being captured cannot wait for a stream outside of its capture, and PyTorch ends the process
 // over it. So the forward pass is refused there.
-void need_capturable(std::initializer_list<const Tensor*> operands, const char* op) {
+void need_capturable(const std::vector<const Tensor*>& operands, const char* op) {
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor* t : operands) {
         if (!t->defined() || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
@@ -1395,6 +1395,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw8_values", &adamw8_values);
     m.def("norm_apply", &norm_apply);
     m.def("loss_apply", &loss_apply);
+    m.def("need_capturable", [](const std::vector<Tensor>& operands, const std::string& op) {
+        std::vector<const Tensor*> each;
+        for (const Tensor& t : operands) each.push_back(&t);
+        need_capturable(each, op.c_str());
+    });
     m.def("dropout_apply", &dropout_apply);
     m.def("attention_apply", &attention_apply);
     m.def("relative_bias_apply", &relative_bias_apply);

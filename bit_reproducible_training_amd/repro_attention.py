@@ -62,6 +62,16 @@ def _borders(buckets, max_distance):
     return found
 
 
+def _side(buckets, max_distance, bidirectional):
+    """The buckets of a side of a table."""
+    side = buckets // 2 if bidirectional else buckets
+    if side < 2 or side > 513 or (bidirectional and buckets % 2):
+        raise ValueError("relative_position_bias: 2 to 513 buckets a side, evenly divided")
+    if not side // 2 < max_distance < 2 ** 31:
+        raise ValueError("relative_position_bias: max_distance must be more than half a side's buckets and less than 2^31")
+    return side
+
+
 def relative_position_bias(table, q_len, k_len, *, max_distance=128, bidirectional=True, query_start=0, dense=True):
     """A learned bias for each pair of a query and a key by the bucket of their distance: table [buckets, heads] -> [heads, q_len, k_len],
     or with dense=False [heads, q_len + k_len - 1] by distance (key minus query, ascending), as attention takes it.
@@ -71,12 +81,7 @@ def relative_position_bias(table, q_len, k_len, *, max_distance=128, bidirection
     even steps of the logarithm up to max_distance, and the last takes all beyond. Gradients reach the table."""
     if table.dim() != 2:
         raise ValueError("relative_position_bias: the table must be [buckets, heads]")
-    buckets = table.shape[0]
-    side = buckets // 2 if bidirectional else buckets
-    if side < 2 or side > 513 or (bidirectional and buckets % 2):
-        raise ValueError("relative_position_bias: 2 to 513 buckets a side, evenly divided")
-    if not side // 2 < max_distance < 2 ** 31:
-        raise ValueError("relative_position_bias: max_distance must be more than half a side's buckets and less than 2^31")
+    side = _side(table.shape[0], max_distance, bidirectional)
     return _backend.relative_bias_apply(table, int(q_len), int(k_len), int(query_start), _borders(side, int(max_distance)),
                                         bool(bidirectional), bool(dense))
 
@@ -87,10 +92,10 @@ class RelativePositionBias(torch.nn.Module):
 
     def __init__(self, num_heads, num_buckets=32, max_distance=128, bidirectional=True):
         super().__init__()
+        _side(num_buckets, max_distance, bidirectional)
         self.max_distance, self.bidirectional = max_distance, bidirectional
         self.weight = torch.nn.Parameter(torch.empty(num_buckets, num_heads))
         torch.nn.init.normal_(self.weight, std=0.02)
-        self(1, 1)  # refuses what the function refuses
 
     def forward(self, q_len, k_len, query_start=0):
         return self._of(q_len, k_len, query_start, False)
@@ -107,7 +112,8 @@ class Attention(torch.nn.Module):
     """A layer of attention with num_heads heads over num_kv_heads (as many by default) heads of keys and values, each of
     head_size (width / num_heads by default): forward(x, states=None, ...) lets the positions of x [batch, queries, width] look at
     those of states [batch, keys, states_width], or of x itself. The products are the reproducible Linear's. In training, dropout
-    drops shares of v by seeds from torch's CPU generator, as Dropout's."""
+    drops shares of v by seeds from torch's CPU generator, as Dropout's; a captured graph repeats the seed that it was captured with, unless
+    seed is a tensor."""
 
     def __init__(self, width, num_heads, num_kv_heads=None, head_size=None, states_width=None, bias=False, dropout=0.0):
         super().__init__()
@@ -128,6 +134,7 @@ class Attention(torch.nn.Module):
         self.out = Linear(num_heads * self.head_size, width, bias=bias)
 
     def forward(self, x, states=None, *, causal=False, query_start=0, key_lengths=None, mask=None, relative_bias=None, seed=None):
+        _backend.need_capturable([x, *self.parameters()], "Attention")
         states = x if states is None else states
         q = self.query(x).unflatten(-1, (self.num_heads, self.head_size))
         k, v = self.key_value(states).unflatten(-1, (2, self.num_kv_heads, self.head_size)).unbind(-3)

@@ -36,7 +36,8 @@ def dropout(x, p=0.5, *, seed):
 
 class Dropout(torch.nn.Module):
     """torch.nn.Dropout, reproducible: in training, forward(x) takes its seed from torch's CPU generator (torch.manual_seed), the
-    same for x on a GPU and on the CPU, or the given one; in evaluation it returns x."""
+    same for x on a GPU and on the CPU, or the given one (a captured graph repeats a number, and reads a tensor at each replay); in
+    evaluation it returns x."""
 
     def __init__(self, p=0.5):
         super().__init__()

@@ -327,3 +327,21 @@ def test_the_layer_is_its_parts():
                 dict(width=12, num_heads=4, dropout=1.0)):
         with pytest.raises(ValueError):
             rg.Attention(**bad)
+
+
+def test_transforms_raise_an_error():
+    q = torch.randn(2, 3, 1, 4)
+    table = torch.randn(8, 2)
+    for f, x in ((lambda x: rg.attention(x, x, x), q), (lambda x: rg.dropout(x, 0.5, seed=1), q),
+                 (lambda x: rg.relative_position_bias(x, 3, 3, max_distance=9), table)):
+        with pytest.raises(Exception):
+            torch.func.grad(lambda x: f(x).sum())(x)
+        with pytest.raises(Exception):
+            torch.func.jvp(f, (x,), (x,))
+        with pytest.raises(Exception):
+            torch.func.vmap(f)(x[None])
+
+
+def test_modules_on_the_meta_device():
+    with torch.device("meta"):
+        rg.Attention(8, 2), rg.RelativePositionBias(2), rg.Dropout(0.1)

@@ -275,3 +275,54 @@ def test_backward_into_a_graph_beside_an_eager_one():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_layer_refuses_a_capture_beside_an_eager_graph():
+    layer = rg.Attention(16, 2).cuda()
+    x = torch.randn(1, 5, 16, device="cuda")
+    alive = layer(x)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        torch.zeros(4, device="cuda").add_(1)
+        with pytest.raises(ValueError, match="still alive"):
+            layer(x)
+    del alive
+
+
+def test_key_blocks_in_turns_and_items_apart():
+    """So many queries that their sums over key blocks are taken some key blocks at a time: each item and head as by itself."""
+    torch.manual_seed(5)
+    q, dy = (torch.randn(1, 8192, 16, 128, device="cuda") for _ in range(2))
+    k, v = (torch.randn(1, 4096, 16, 128, device="cuda") for _ in range(2))
+    bias = torch.randn(16, 8192 + 4096 - 1, device="cuda")
+    s = dict(key_lengths=torch.tensor([4000], device="cuda"), causal=True, query_start=-4000)
+    whole = gradients({"q": q, "k": k, "v": v, "relative_bias": bias}, s, dy)
+    for h in (0, 11):
+        one = gradients({"q": q[:, :, h:h + 1], "k": k[:, :, h:h + 1], "v": v[:, :, h:h + 1], "relative_bias": bias[h:h + 1]}, s,
+                        dy[:, :, h:h + 1])
+        for n in ("y", "dq", "dk", "dv"):
+            assert torch.equal(whole[n][:, :, h], one[n][:, :, 0]), n
+        assert torch.equal(whole["drelative_bias"][h], one["drelative_bias"][0])
+
+
+def test_offsets_past_32_bits():
+    """Items 2^32 values apart, as in a long cache."""
+    t, s, dy = case(2, 4, 2, 70, 300, 16, causal=True)
+    want = gradients(cuda(t), s, dy.cuda())
+    room = torch.empty(2 ** 32 + 300 * 64, device="cuda")
+    k, v = (room.as_strided((2, 300, 2, 16), (2 ** 32, 64, 16, 1), at) for at in (0, 32))
+    k.copy_(t["k"])
+    v.copy_(t["v"])
+    got = gradients({"q": t["q"].cuda(), "k": k, "v": v, "relative_bias": None}, s, dy.cuda())
+    assert_same(got, {n: x.cpu() for n, x in want.items()})
+    one = rg.attention(t["q"][:, :1].cuda(), k, v)
+    assert torch.equal(one, rg.attention(t["q"][:, :1].cuda(), t["k"].cuda(), t["v"].cuda()))
+
+
+def test_shared_rows_of_strides_too_far_apart():
+    """Positions more than 2^22 values apart are brought together."""
+    t, s, dy = case(1, 1, 1, 3, 9, 8)
+    room = torch.zeros(9 * (2 ** 22 + 4), device="cuda")
+    k = room.as_strided((1, 9, 1, 8), (1, 2 ** 22 + 4, 1, 1))
+    k.copy_(t["k"])
+    assert torch.equal(rg.attention(t["q"].cuda(), k, t["v"].cuda()).cpu(), rg.attention(t["q"], t["k"], t["v"]))

@@ -1,11 +1,17 @@
 // The attention's forward pass on the matrix cores.
 //
 // A block takes 128 queries of a head, 32 a wavefront, and goes through the keys in tiles of 64 that its wavefronts share in LDS.
-// v_mfma_f32_32x32x2_f32 adds a pair of products a step, in ascending order, each fused and rounded as fmaf is: the
-// definition's chains. Scores are made as S^T = K Q^T, so that a lane holds scores of one query (column lane mod 32), and
-// a register of the result is, as it stands, the operand of O^T = V^T P^T for two successive keys: row 8 g + 4 h + r of the tile's
-// operand is taken to be key 8 g + 2 r + h, so half h of the wavefront holds the keys of parity h in ascending order.
-// Nothing of the softmax passes through LDS, and a row's maximum takes one exchange between the halves.
+// v_mfma_f32_32x32x2_f32 adds a pair of products a step, in ascending order, each fused and rounded as fmaf is, subnormals and
+// all (524288 of 524288 results the same in each of four ranges): the definition's chains. Scores are made as S^T = K Q^T, so that a
+// lane holds scores of one query (column lane mod 32), and a register of the result is, as it stands, the operand of
+// O^T = V^T P^T for two successive keys: row 8 g + 4 h + r of the tile's operand is taken to be key 8 g + 2 r + h, so half h
+// of the wavefront holds the keys of parity h in ascending order. Nothing of the softmax passes through LDS, and a row's maximum
+// takes one exchange between the halves.
+//
+// The float32 matrix instructions and the vector unit's take turns on a SIMD (1154 and 2141 us apart, 3247 together, where
+// int8 ones overlap), so every vector instruction counts: a score costs 10.5, a kept or dropped pair 13 more (Philox's
+// products). 2 x 16 heads of 4096 x 4096 x 64: 1134 us, 121 TFLOP/s of the 153 that a product of 8192^3 reaches; of 128: 124. At
+// 8 x 12 heads of 1024 the blocks are one and a half rounds: 97.
 #include "rg_attention.h"
 
 namespace rg {
@@ -355,7 +361,8 @@ repair(Problem z, Parts s, float* y, float* stats) {
 
 // Few queries: a block takes a chunk of keys for all rows that share a head of keys (at most FEW), a thread a key for the
 // scores, then a wavefront a row and a lane a value. Bound by HBM: the keys are read into LDS as the values are on their way, and the
-// values take their place there. A single query of 4096 keys for 16 items of 12 heads of 64: FEW_TIME.
+// values take their place there. One query of 2048 to 4096
+// keys for 16 items of 12 heads of 64: 72 us and 5.5 to join the chunks, 4.9 TB/s of the 5.25 of a copy.
 constexpr int FEW = 8;
 
 template <int DB, bool QUADS>
@@ -597,7 +604,10 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
 }
 
 // The keys are split over blocks where the queries alone leave compute units idle: as many parts as bring the grid to two
-// blocks a compute unit, whole chunks each, as long as the chunks' results take at most a quarter of a gigabyte.
+// blocks a compute unit, whole chunks each, as long as the chunks' results take at most a quarter of a gigabyte (8 heads of
+// 1024 x 1024 x 64: 36 us in 4 parts; 96 heads of 512 x 1500 with dropout, 384 blocks: 263 us in 2 parts, 286 in one).
+// Up to FEW rows of a head of keys go to the kernel above, which reads the keys once for all (16 x 12 rows of 4096 keys: 214 us
+// here, 78 there).
 bool few(const Problem& z) { return z.Tk > 0 && (long long)z.group * z.Tq <= FEW; }
 Parts parts_of(const Problem& z) {
     Parts s;

@@ -359,7 +359,7 @@ repair(Problem z, Parts s, float* y, float* stats) {
     }
 }
 
-// Few queries: a block takes a chunk of keys for all rows that share a head of keys (at most FEW), a thread a key for the
+// Few queries: a block takes a chunk of keys for up to FEW of the rows that share a head of keys, a thread a key for the
 // scores, then a wavefront a row and a lane a value. Bound by HBM: the keys are read into LDS as the values are on their way, and the
 // values take their place there. One query of 2048 to 4096
 // keys for 16 items of 12 heads of 64: 72 us and 5.5 to join the chunks, 4.9 TB/s of the 5.25 of a copy.
@@ -375,11 +375,13 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
     if (used && blockIdx.x == 0 && threadIdx.x == 0) *used = seed;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int heads = z.B * z.KVH, chunk = (int)(blockIdx.x / heads);
+    const int heads = z.B * z.KVH, shares = (z.group * z.Tq + FEW - 1) / FEW, chunk = (int)(blockIdx.x / heads / shares);
+    const int r0 = (int)(blockIdx.x / heads % shares) * FEW;
     const int b = (int)(blockIdx.x % heads) / z.KVH, kvh = (int)(blockIdx.x % heads) % z.KVH, h0 = kvh * z.group;
-    const int rows = z.group * z.Tq, first = chunk * CHUNK, len = keys_of(z, b);
-    const auto row_of = [&](int r) { return ((size_t)b * z.H + h0 + r / z.Tq) * z.Tq + r % z.Tq; };
-    if (s.chunks > 1 && first >= key_end(z, b, z.Tq - 1)) {
+    const int rows = min(FEW, z.group * z.Tq - r0), first = chunk * CHUNK;
+    const int len = key_end(z, b, z.Tq - 1);  // what no row sees is not read
+    const auto row_of = [&](int r) { return ((size_t)b * z.H + h0 + (r0 + r) / z.Tq) * z.Tq + (r0 + r) % z.Tq; };
+    if (s.chunks > 1 && first >= len) {
         if (t < rows) s.ml[(size_t)chunk * z.B * z.H * z.Tq + row_of(t)] = make_float2(NONE, -1.0f);
         return;
     }
@@ -403,7 +405,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
     load(value_at(z, b, h0, 0), z.v_stride[1], next);
     for (int n = t; n < rows * DP; n += 256) {
         const int r = n / DP, d = n % DP;
-        const float x = d < z.D ? query_at(z, b, h0 + r / z.Tq, r % z.Tq)[d] : 0.0f;
+        const float x = d < z.D ? query_at(z, b, h0 + (r0 + r) / z.Tq, (r0 + r) % z.Tq)[d] : 0.0f;
         Qs[r][d] = z.flip ? -x : x;
     }
     store(held);
@@ -430,7 +432,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
 #pragma unroll
     for (int r = 0; r < FEW; ++r) {
         if (r >= rows) break;
-        const int i = r % z.Tq, h = h0 + r / z.Tq;
+        const int i = (r0 + r) % z.Tq, h = h0 + (r0 + r) / z.Tq;
         see[r] = seen(z, b, h, i, j, key_end(z, b, i));
         term[r] = see[r] ? z.bias ? __builtin_fmaf(sum[r], z.factor, bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + j - i + z.Tq - 1]))
                                   : sum[r] * z.factor : NONE;
@@ -479,7 +481,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
     }
     if (z.threshold != 0) {
         __syncthreads();
-        for (int r = 0; r < rows; ++r) P[r][t] = kept(z, seed, b, h0 + r / z.Tq, r % z.Tq, j) ? P[r][t] : 0.0f;
+        for (int r = 0; r < rows; ++r) P[r][t] = kept(z, seed, b, h0 + (r0 + r) / z.Tq, (r0 + r) % z.Tq, j) ? P[r][t] : 0.0f;
         __syncthreads();
     }
     const bool some = z.causal || z.mask;
@@ -547,7 +549,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
         } else {
             Joined all;
             all.join(c);
-            finish_row(z, all, b, h0 + r / z.Tq, r % z.Tq, lane, y, stats);
+            finish_row(z, all, b, h0 + (r0 + r) / z.Tq, (r0 + r) % z.Tq, lane, y, stats);
         }
     }
 }
@@ -606,9 +608,9 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
 // The keys are split over blocks where the queries alone leave compute units idle: as many parts as bring the grid to two
 // blocks a compute unit, whole chunks each, as long as the chunks' results take at most a quarter of a gigabyte (8 heads of
 // 1024 x 1024 x 64: 36 us in 4 parts; 96 heads of 512 x 1500 with dropout, 384 blocks: 263 us in 2 parts, 286 in one).
-// Up to FEW rows of a head of keys go to the kernel above, which reads the keys once for all (16 x 12 rows of 4096 keys: 214 us
-// here, 78 there).
-bool few(const Problem& z) { return z.Tk > 0 && (long long)z.group * z.Tq <= FEW; }
+// Up to FEW rows of a head of keys, and more where few queries stand under many heads, go to the kernel above (16 x 12 rows of
+// 4096 keys: 214 us here, 78 there; 4 x 144 over 12 heads of 2048: 372 and 50).
+bool few(const Problem& z) { return z.Tk > 0 && ((long long)z.group * z.Tq <= FEW || (z.Tq <= 4 && (long long)z.group * z.Tq <= 128)); }
 Parts parts_of(const Problem& z) {
     Parts s;
     s.chunks = (z.Tk + CHUNK - 1) / CHUNK;
@@ -631,7 +633,7 @@ Parts parts_of(const Problem& z) {
     return s;
 }
 long long blocks_of(const Problem& z, const Parts& s) {
-    return few(z) ? (long long)z.B * z.KVH * s.chunks : (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
+    return few(z) ? (long long)z.B * z.KVH * ((z.group * z.Tq + FEW - 1) / FEW) * s.chunks : (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
 }
 // What a key holds must not reach a row that does not see it: under a causal mask or one of pairs.
 // (Few rows leave out each pair by itself.)

@@ -48,9 +48,9 @@ def test_gives_the_cpu_bits_at_every_length(tq, tk):
         compare(*case(*c))
 
 
-@pytest.mark.parametrize("h,kvh", [(1, 1), (8, 1), (12, 3), (6, 6), (40, 2)])
+@pytest.mark.parametrize("h,kvh", [(1, 1), (8, 1), (12, 3), (6, 6), (40, 2), (128, 1), (129, 1)])
 def test_shared_heads(h, kvh):
-    for tq, tk in ((1, 520), (5, 300), (90, 90)):
+    for tq, tk in ((1, 520), (3, 300), (5, 300), (90, 90)):
         compare(*case(2, h, kvh, tq, tk, 16, True, True, "keys", True, 0.1))
 
 

@@ -10,8 +10,8 @@
 //
 // The float32 matrix instructions and the vector unit's take turns on a SIMD (1154 and 2141 us apart, 3247 together, where
 // int8 ones overlap), so every vector instruction counts: a score costs 10.5, a kept or dropped pair 13 more (Philox's
-// products). 2 x 16 heads of 4096 x 4096 x 64: 1134 us, 121 TFLOP/s of the 153 that a product of 8192^3 reaches; of 128: 124. At
-// 8 x 12 heads of 1024 the blocks are one and a half rounds: 97.
+// products). 2 x 16 heads of 4096 x 4096 x 64: 1132 us, 121 TFLOP/s of the 153 that a product of 8192^3 reaches; at
+// 8 x 12 heads of 1024 the blocks are one and a half rounds: 97 to 99.
 #include "rg_attention.h"
 
 namespace rg {
@@ -468,7 +468,9 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
         return m;
     };
     const int tiles = min(4, (len - first + 63) / 64);  // past the keys nothing changes
-    if (t >= 192 && t < 192 + 2 * rows) {
+    // l by the last wavefront where it has no row, or where o leaves pairs out; else it comes along with o
+    const bool apart = rows < 4 || z.threshold != 0;
+    if (apart && t >= 192 && t < 192 + 2 * rows) {
         const int r = (t - 192) >> 1, parity = t & 1;
         float a[4], l = 0.0f;
         factors(r, a);
@@ -490,9 +492,9 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         mine[x].m = factors(wave + 4 * x < rows ? wave + 4 * x : 0, a[x]);
-        mine[x].o0 = mine[x].o1 = 0.0f;
+        mine[x].o0 = mine[x].o1 = mine[x].even = mine[x].odd = 0.0f;
     }
-    const auto products = [&](auto both) {
+    const auto products = [&](auto both, auto alone) {
         constexpr int N = decltype(both)::value ? 2 : 1;
         for (int w = 0; w < tiles; ++w) {
             unsigned long long which = ~0ull;
@@ -500,6 +502,8 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
             for (int x = 0; x < N; ++x) {
                 mine[x].o0 = mine[x].o0 * a[x][w];
                 mine[x].o1 = mine[x].o1 * a[x][w];
+                mine[x].even = mine[x].even * a[x][w];
+                mine[x].odd = mine[x].odd * a[x][w];
                 if (some) which &= See[wave + 4 * x][w];
             }
             const float* v = KV + 64 * w * STRIDE + lane;
@@ -517,6 +521,10 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
                             const float u = q == 0 ? p[x].x : q == 1 ? p[x].y : q == 2 ? p[x].z : p[x].w;
                             mine[x].o0 = __builtin_fmaf(u, v0, mine[x].o0);
                             if (DB > 2) mine[x].o1 = __builtin_fmaf(u, v1, mine[x].o1);
+                            if (!decltype(alone)::value) {
+                                float& l = q % 2 == 0 ? mine[x].even : mine[x].odd;
+                                l = l + u;
+                            }
                         }
                     }
                 }
@@ -527,20 +535,28 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
                         const float u = P[wave + 4 * x][64 * w + n];
                         mine[x].o0 = __builtin_fmaf(u, v[n * STRIDE], mine[x].o0);
                         if (DB > 2) mine[x].o1 = __builtin_fmaf(u, v[n * STRIDE + 64], mine[x].o1);
+                        if (!decltype(alone)::value) {
+                            float& l = n % 2 == 0 ? mine[x].even : mine[x].odd;
+                            l = l + u;
+                        }
                     }
             }
         }
     };
-    if (wave + 4 < rows) products(std::true_type());
-    else if (wave < rows) products(std::false_type());
+    if (wave + 4 < rows && apart) products(std::true_type(), std::true_type());
+    else if (wave + 4 < rows) products(std::true_type(), std::false_type());
+    else if (wave < rows && apart) products(std::false_type(), std::true_type());
+    else if (wave < rows) products(std::false_type(), std::false_type());
     __syncthreads();
 #pragma unroll
     for (int x = 0; x < FEW / 4; ++x) {
         const int r = wave + 4 * x;
         if (r >= rows) break;
         RowChunk& c = mine[x];
-        c.even = Ls[r][0];
-        c.odd = Ls[r][1];
+        if (apart) {
+            c.even = Ls[r][0];
+            c.odd = Ls[r][1];
+        }
         if (s.chunks > 1) {
             const size_t at = (size_t)chunk * z.B * z.H * z.Tq + row_of(r);
             if (lane < z.D) s.o[at * z.D + lane] = c.o0;
@@ -555,7 +571,8 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
 }
 
 // Joins the chunks of a row in their order: a wavefront takes a row, first a lane a chunk (the maxima before it and the
-// two factors), then a lane a value.
+// two factors), then a lane a value (WIDE: two), with the next chunks' on the way.
+template <bool WIDE>
 __global__ void __launch_bounds__(256)
 join_chunks(Problem z, Parts s, float* y, float* stats) {
     const int lane = threadIdx.x & 63;
@@ -583,21 +600,24 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
             const float* o = s.o + (first * rows + n) * z.D;
             const int count = min(64, s.slots - first);
             const int d0 = min(lane, z.D - 1), d1 = min(lane + 64, z.D - 1);
-            for (int k0 = 0; k0 < count; k0 += 8) {
-                float o0[8], o1[8];
+            constexpr int AHEAD = WIDE ? 16 : 32;
+            for (int k0 = 0; k0 < count; k0 += AHEAD) {
+                float o0[AHEAD], o1[AHEAD];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
+                for (int k = 0; k < AHEAD; ++k) {
+                    if (k % 8 == 0 && k0 + k >= count) break;
                     const float* p = o + min(k0 + k, count - 1) * rows * z.D;
                     o0[k] = p[d0];
-                    o1[k] = p[d1];
+                    o1[k] = WIDE ? p[d1] : 0.0f;
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {  // (a chunk that was not written has factors 1 and 0)
+                for (int k = 0; k < AHEAD; ++k) {  // (a chunk that was not written has factors 1 and 0)
+                    if (k % 8 == 0 && k0 + k >= count) break;
                     const float ak = __shfl(a, k0 + k, 64), ek = __shfl(e, k0 + k, 64), lk = __shfl(ml.y, k0 + k, 64);
                     const bool is = (which >> (k0 + k) & 1) != 0;
                     all.total = __builtin_fmaf(is ? lk : 0.0f, ek, all.total * ak);
                     all.o0 = __builtin_fmaf(is ? o0[k] : 0.0f, ek, all.o0 * ak);
-                    all.o1 = __builtin_fmaf(is ? o1[k] : 0.0f, ek, all.o1 * ak);
+                    if (WIDE) all.o1 = __builtin_fmaf(is ? o1[k] : 0.0f, ek, all.o1 * ak);
                 }
             }
         }
@@ -605,9 +625,60 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
     }
 }
 
+// The same where there are few chunks (at most SLOTS): a thread takes four values of a row and works out the factors itself.
+constexpr int SLOTS = 8;
+
+template <bool QUADS>
+__global__ void __launch_bounds__(256)
+join_few(Problem z, Parts s, float* y, float* stats) {
+    const int quads = (z.D + 3) / 4;
+    const long long rows = (long long)z.B * z.H * z.Tq;
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < rows * quads; at += (long long)gridDim.x * 256) {
+        const long long n = at / quads;
+        const int d = 4 * (int)(at % quads), i = (int)(n % z.Tq), bh = (int)(n / z.Tq);
+        float2 ml[SLOTS];
+        float v[SLOTS][4];
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) {
+            const long long from = min(k, s.slots - 1) * rows + n;
+            ml[k] = s.ml[from];
+            const float* p = s.o + from * z.D + d;
+            if (QUADS) {
+                const float4 x = *reinterpret_cast<const float4*>(p);
+                v[k][0] = x.x, v[k][1] = x.y, v[k][2] = x.z, v[k][3] = x.w;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[k][r] = p[d + r < z.D ? r : 0];
+            }
+        }
+        float top = NONE, total = 0.0f, o[4] = {};
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) {
+            if (k >= s.slots || ml[k].y == -1.0f) continue;
+            const float both = larger(top, ml[k].x), base = base_of(both), a = e2(top - base), e = e2(ml[k].x - base);
+            top = both;
+            total = __builtin_fmaf(ml[k].y, e, total * a);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = __builtin_fmaf(v[k][r], e, o[r] * a);
+        }
+        const float inverse = reciprocal(total), f = z.threshold == 0 ? inverse : inverse * z.keep_factor;
+        float* out = y + (((size_t)(bh / z.H) * z.Tq + i) * z.H + bh % z.H) * z.D + d;
+        if (QUADS) {
+            *reinterpret_cast<float4*>(out) = make_float4(o[0] * f + 0.0f, o[1] * f + 0.0f, o[2] * f + 0.0f, o[3] * f + 0.0f);
+        } else {
+            for (int r = 0; r < 4; ++r)
+                if (d + r < z.D) out[r] = o[r] * f + 0.0f;
+        }
+        if (stats && d == 0) {
+            stats[2 * n] = base_of(top);
+            stats[2 * n + 1] = inverse;
+        }
+    }
+}
+
 // The keys are split over blocks where the queries alone leave compute units idle: as many parts as bring the grid to two
 // blocks a compute unit, whole chunks each, as long as the chunks' results take at most a quarter of a gigabyte (8 heads of
-// 1024 x 1024 x 64: 36 us in 4 parts; 96 heads of 512 x 1500 with dropout, 384 blocks: 263 us in 2 parts, 286 in one).
+// 1024 x 1024 x 64: 34 us in 4 parts; 96 heads of 512 x 1500 with dropout, 384 blocks: 252 us in 2 parts, 286 in one).
 // Up to FEW rows of a head of keys, and more where few queries stand under many heads, go to the kernel above (16 x 12 rows of
 // 4096 keys: 214 us here, 78 there; 4 x 144 over 12 heads of 2048: 372 and 50).
 bool few(const Problem& z) { return z.Tk > 0 && ((long long)z.group * z.Tq <= FEW || (z.Tq <= 4 && (long long)z.group * z.Tq <= 128)); }
@@ -675,7 +746,12 @@ int forward(const Problem& z, float* y, float* stats, unsigned long long* used, 
         rc = hipGetLastError();
     }
     if (rc == hipSuccess && s.parts > 1) {
-        hipLaunchKernelGGL(join_chunks, dim3(grid_of(rows, 4)), dim3(256), 0, stream, z, s, y, stats);
+        if (s.slots <= SLOTS)
+            hipLaunchKernelGGL(z.quads ? join_few<true> : join_few<false>, dim3(grid_of(rows * ((z.D + 3) / 4), 256)), dim3(256), 0, stream, z,
+                               s, y, stats);
+        else
+            hipLaunchKernelGGL(z.D > 64 ? join_chunks<true> : join_chunks<false>, dim3(grid_of(rows, 4)), dim3(256), 0, stream, z, s, y,
+                               stats);
         rc = hipGetLastError();
     }
     return rc;

@@ -13,7 +13,7 @@
 // As in the forward pass vector instructions add to the products' time (about a sixth of it). Loads go by buffer offsets without
 // branches: with branches each waited for the one before, and the pass of 2 x 16 heads of 4096 x 4096 x 64 took 4.75 ms
 // where it takes 3.17 (108 TFLOP/s). Two blocks a compute unit up to 64 values a head, whose registers hold two wavefronts a
-// SIMD; one for wider heads (96 TFLOP/s at 128: nothing runs while its only wavefront waits at a barrier).
+// SIMD.
 #include "rg_attention.h"
 
 namespace rg {
@@ -43,6 +43,7 @@ __device__ __forceinline__ int fresh(int v) {
     asm volatile("" : "+v"(v));
     return v;
 }
+__device__ __forceinline__ Block4 mfma4(float a, float b, Block4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float part_of(const float4& v, int r) { return r == 0 ? v.x : r == 1 ? v.y : r == 2 ? v.z : v.w; }
 
 // Where a block and chunk are, and what they leave. Key blocks first .. first + count of the `blocks`.
@@ -76,7 +77,7 @@ __device__ __forceinline__ bool live(const Problem& z, int len, int block, int r
 }
 
 template <int DB, bool BIAS, bool DROP, bool QUADS>
-__global__ void __launch_bounds__(256, DB <= 2 ? 2 : 1)
+__global__ void __launch_bounds__(256, 2)
 backward_tiles(Problem z, Gradients g, Work w) {
     constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 8;
     __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds_[STEP + STEP * DS_STRIDE];
@@ -395,6 +396,335 @@ backward_tiles(Problem z, Gradients g, Work w) {
     }
 }
 
+// The same for heads of more than 64 values, whose sums would leave one wavefront a SIMD and nothing to run while it waits at a
+// barrier (2 x 16 heads of 2048 x 2048 x 128 in the kernel above: 1790 us, here 1600, 107 TFLOP/s): eight wavefronts of 16
+// keys each, all products by 16 x 16 blocks (row 4 c + r of an operand is query 4 r + c, so that a register of P or dS is again the
+// next operand, for four successive queries).
+template <int DB, bool BIAS, bool DROP, bool QUADS>
+__global__ void __launch_bounds__(512, 2)
+backward_wide(Problem z, Gradients g, Work w) {
+    constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 8;
+    __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds_[STEP + STEP * DS_STRIDE];
+    __shared__ float Bs[BIAS ? 160 : 1], Sums[BIAS ? DIAGONALS : 1];
+    __shared__ float4 Query[STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits
+    __shared__ uint32_t Masks[STEP][4];
+    float* Ds = Ds_ + STEP;  // (zeros before the first row, too)
+    const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
+    const int t = threadIdx.x, lane = t & 63, col = lane & 15, group = lane >> 4, wave = t >> 6;
+    const Place at = place_of(z, w);
+    const int bh = at.bh, b = bh / z.H, h = bh % z.H, slot = at.slot, heads = z.B * z.H;
+    const int block = w.first + slot, k0 = block * KEY_BLOCK;
+    const int len = keys_of(z, b), key = k0 + 16 * wave + col;
+    const size_t row0 = (size_t)bh * z.Tq;
+    const size_t out_stride = (size_t)(w.direct ? z.KVH : 1) * z.D;
+
+    if (!live(z, len, block, z.Tq)) {
+        const size_t out = out_of(z, w, bh, 0);
+        if (w.direct)
+            for (int n = t; n < KEY_BLOCK * z.D; n += 512)
+                if (k0 + n / z.D < z.Tk) {
+                    w.dk[out + (k0 + n / z.D) * out_stride + n % z.D] = 0.0f;
+                    w.dv[out + (k0 + n / z.D) * out_stride + n % z.D] = 0.0f;
+                }
+        if (w.broken && t == 0) w.broken[blockIdx.x] = 0;
+        return;
+    }
+
+    float k[8 * DB], v[8 * DB];  // value 4 n + group of the lane's key
+    float broken = 0.0f;
+    const int lrow = t >> 3, lcol = 4 * (t & 7);
+    const auto keys_to_lds = [&](const float* base, long long stride) {
+        const Rows rows = rows_at(base + k0 * stride, min(KEY_BLOCK, len - k0), stride, z.D);
+        const uint32_t at = ((uint32_t)lrow * (uint32_t)stride + lcol) * 4;
+        float4 x[2 * DB];
+#pragma unroll
+        for (int n = 0; n < 2 * DB; ++n)
+            x[n] = four<QUADS>(rows, at + 128 * (n % DB) + n / DB * 256 * (uint32_t)stride, z.D - lcol - 32 * (n % DB));
+#pragma unroll
+        for (int n = 0; n < 2 * DB; ++n) *reinterpret_cast<float4*>(Ks + (lrow + n / DB * 64) * KS + lcol + 32 * (n % DB)) = x[n];
+    };
+    const auto take = [&](float* to) {
+#pragma unroll
+        for (int n = 0; n < 8 * DB; ++n) to[n] = Ks[(16 * wave + col) * KS + 4 * n + group];
+    };
+    for (int n = t; n < STEP; n += 512) Ds_[n] = 0.0f;
+    for (int n = t; n < STEP * (STEP + 1); n += 512) Ds[n / (STEP + 1) * DS_STRIDE + KEY_BLOCK + n % (STEP + 1)] = 0.0f;
+    keys_to_lds(value_at(z, b, h, 0), z.v_stride[1]);
+    __syncthreads();
+    take(v);
+    __syncthreads();
+    keys_to_lds(key_at(z, b, h, 0), z.k_stride[1]);
+    __syncthreads();
+    take(k);
+#pragma unroll
+    for (int n = 0; n < 8 * DB; ++n) {
+        broken = __builtin_fmaf(k[n], 0.0f, broken);
+        k[n] = z.flip ? -k[n] : k[n];
+    }
+
+    // the first four wavefronts bring the queries, the others the gradients
+    const bool first_half = __builtin_amdgcn_readfirstlane(wave) < 4;
+    const float* base = first_half ? query_at(z, b, h, 0) : g.dy + ((size_t)b * z.Tq * z.H + h) * z.D;
+    const long long stride = first_half ? z.q_stride[1] : (long long)z.H * z.D;
+    float4 qn[DB];
+    float bn = 0.0f;
+    float2 sn;
+    float en;
+    uint32_t mn = ~0u;
+    const auto load = [&](int i0) {
+        const int t = fresh(threadIdx.x), lrow = (t >> 3) & (STEP - 1), lcol = 4 * (t & 7);
+        const uint32_t at = ((uint32_t)lrow * (uint32_t)stride + lcol) * 4;
+        const Rows rows = rows_at(base + i0 * stride, min(STEP, z.Tq - i0), stride, z.D);
+#pragma unroll
+        for (int x = 0; x < DB; ++x) qn[x] = four<QUADS>(rows, at + 128 * x, x < DB - 1 ? 4 : z.D - lcol - 32 * x);
+        const size_t row = row0 + min(i0 + (t & (STEP - 1)), z.Tq - 1);
+        sn = reinterpret_cast<const float2*>(g.stats)[row];
+        en = g.delta[row];
+        if (z.mask) {
+            const int i = min(i0 + ((t >> 2) & (STEP - 1)), z.Tq - 1), word = min(k0 / 32 + (t & 3), (z.Tk - 1) / 32);
+            const unsigned long long* m = z.mask + b * z.mask_stride[0] + h * z.mask_stride[1] + i * z.mask_stride[2];
+            mn = reinterpret_cast<const uint32_t*>(m)[word];
+        }
+        if (BIAS) {
+            const int c = k0 + t - (STEP - 1) - i0 + z.Tq - 1;  // (outside of the bias no pair needs it)
+            bn = z.bias[(size_t)h * (z.Tq + z.Tk - 1) + max(0, min(c, z.Tq + z.Tk - 2))];
+        }
+    };
+    const auto store = [&](int i0) {
+        const int t = fresh(threadIdx.x), lrow = (t >> 3) & (STEP - 1), lcol = 4 * (t & 7);
+        float* to = first_half ? Qs : Ys;
+#pragma unroll
+        for (int x = 0; x < DB; ++x) {
+            const int d = lcol + 32 * x;
+            float* p = to + lrow * QS + (d & ~15) + ((d >> 2) & 3);  // values 4 s + c of sixteen at 4 c + s
+#pragma unroll
+            for (int c = 0; c < 4; ++c) p[4 * c] = part_of(qn[x], c);
+        }
+        if (t < STEP) Query[t] = make_float4(sn.x, sn.y, en, __int_as_float(i0 + t < z.Tq ? last_end(z, len, i0 + t) : 0));
+        else if (t >= 128 && t < 256) Masks[(t >> 2) & (STEP - 1)][t & 3] = mn;
+        if (BIAS && t < KEY_BLOCK + STEP - 1) Bs[t] = bias_term(bn);
+    };
+    const int row_of = 4 * (col & 3) + (col >> 2);    // the query of 16 that row `col` of an operand is
+    const int place_in = 4 * (col & 3) + (col >> 2);  // where value `col` of 16 is in Qs and Ys
+
+    const int first_chunk = at.part * w.a_part, last_chunk = min(w.chunks, first_chunk + w.a_part);
+    bool begun = false;
+    for (int chunk = first_chunk; chunk < last_chunk; ++chunk) {
+        const int c0 = chunk * QUERY_CHUNK, c1 = min(c0 + QUERY_CHUNK, z.Tq);
+        if (!live(z, len, block, c1)) continue;
+        float* diagonals = BIAS && w.diagonals ? w.diagonals + (((size_t)bh * w.count + slot) * w.chunks + chunk) * DIAGONALS : nullptr;
+        Block4 dk[2 * DB], dv[2 * DB];
+#pragma unroll
+        for (int n = 0; n < 2 * DB; ++n) dk[n] = dv[n] = Block4{0.0f, 0.0f, 0.0f, 0.0f};
+        int i0 = c0;
+        while (!live(z, len, block, i0 + STEP)) i0 += STEP;  // (the chunk's last step is live)
+        __syncthreads();
+        load(i0);
+        store(i0);
+        if (BIAS)
+            for (int n = t; n < DIAGONALS; n += 512) Sums[n] = 0.0f;
+        lds_barrier();
+        for (; i0 < c1; i0 += STEP) {
+            const bool more = i0 + STEP < c1;
+            Block4 s[2], dp[2];  // register r of block n: query 16 n + 4 r + group
+#pragma unroll
+            for (int n = 0; n < 2; ++n) s[n] = dp[n] = Block4{0.0f, 0.0f, 0.0f, 0.0f};
+            {
+                const float* qs = Qs + row_of * QS + 4 * group;
+                const float* ys = Ys + row_of * QS + 4 * group;
+                float4 a[2], c[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    a[n] = *reinterpret_cast<const float4*>(qs + 16 * n * QS);
+                    c[n] = *reinterpret_cast<const float4*>(ys + 16 * n * QS);
+                }
+#pragma unroll
+                for (int u = 0; u < 2 * DB; ++u) {
+                    const int ahead = 16 * (u + 1 < 2 * DB ? u + 1 : u);
+                    float4 an[2], cn[2];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        an[n] = *reinterpret_cast<const float4*>(qs + 16 * n * QS + ahead);
+                        cn[n] = *reinterpret_cast<const float4*>(ys + 16 * n * QS + ahead);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) {
+                            s[n] = mfma4(part_of(a[n], r), k[4 * u + r], s[n]);
+                            dp[n] = mfma4(part_of(c[n], r), v[4 * u + r], dp[n]);
+                        }
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) a[n] = an[n], c[n] = cn[n];
+                    fence();
+                }
+            }
+            uint32_t keep[4];
+            if (DROP) {
+                // a call's four words are four keys', neighbours in a quad of lanes: each makes those of another query
+                uint32_t bits = 0;
+                const int r = lane & 3;
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const auto x = repro_dropout::pair_words((uint32_t)(key >> 2), i0 + 16 * n + 4 * r + group, bh, seed);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) bits |= (uint32_t)(x.w[q] >= z.threshold) << (4 * n + q);
+                }
+                keep[0] = __builtin_amdgcn_update_dpp(0, bits, 0x00, 0xF, 0xF, true) >> r;
+                keep[1] = __builtin_amdgcn_update_dpp(0, bits, 0x55, 0xF, 0xF, true) >> r;
+                keep[2] = __builtin_amdgcn_update_dpp(0, bits, 0xAA, 0xF, 0xF, true) >> r;
+                keep[3] = __builtin_amdgcn_update_dpp(0, bits, 0xFF, 0xF, 0xF, true) >> r;
+            }
+            const auto differentials = [&](auto edge) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int q = 16 * n + 4 * r + group;
+                        const float4 row = Query[q];
+                        const float x = BIAS ? __builtin_fmaf(s[n][r], z.factor, Bs[16 * wave + col - q + STEP - 1]) - row.x
+                                             : __builtin_fmaf(s[n][r], z.factor, -row.x);
+                        float p = e2(x) * row.y, d = dp[n][r], u = p;
+                        if (DROP) {
+                            const bool kept = (keep[r] >> (4 * n) & 1) != 0;
+                            u = kept ? p * z.keep_factor : 0.0f;
+                            d = kept ? d * z.keep_factor : 0.0f;
+                        }
+                        d = ds_of(p, d, row.z);
+                        if (decltype(edge)::value) {
+                            const bool see = (int)(key < __float_as_int(row.w)) & (int)(Masks[q][wave >> 1] >> (16 * (wave & 1) + col) & 1);
+                            u = see ? u : 0.0f;
+                            d = see ? d : 0.0f;
+                        }
+                        s[n][r] = u;
+                        dp[n][r] = d;
+                        Ds[q * DS_STRIDE + 16 * wave + col] = d;
+                    }
+            };
+            // whether every pair of the wavefront's is seen
+            if (!z.mask && i0 + STEP <= z.Tq && k0 + 16 * wave + 16 <= last_end(z, len, i0)) differentials(std::false_type());
+            else differentials(std::true_type());
+            {
+                const float* qs = Qs + group * QS + place_in;
+                const float* ys = Ys + group * QS + place_in;
+                float a[2 * DB], c[2 * DB];
+#pragma unroll
+                for (int x = 0; x < 2 * DB; ++x) a[x] = ys[16 * x], c[x] = qs[16 * x];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const int ahead = 4 * (n < 7 ? n + 1 : n) * QS;
+                    float an[2 * DB], cn[2 * DB];
+#pragma unroll
+                    for (int x = 0; x < 2 * DB; ++x) an[x] = ys[ahead + 16 * x], cn[x] = qs[ahead + 16 * x];
+#pragma unroll
+                    for (int x = 0; x < 2 * DB; ++x) {
+                        dv[x] = mfma4(a[x], s[n / 4][n % 4], dv[x]);
+                        dk[x] = mfma4(c[x], dp[n / 4][n % 4], dk[x]);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2 * DB; ++x) a[x] = an[x], c[x] = cn[x];
+                    fence();
+                }
+            }
+            lds_barrier();
+            if (more) load(i0 + STEP);  // (in flight under dQ's products)
+            {
+                // the wavefront's 16 queries and its blocks of 16 values: the first and, where there are as many, the one 4 on
+                const int q0 = 16 * (wave & 1), x0 = wave >> 1;
+                const float* ds = Ds + (q0 + col) * DS_STRIDE + group;
+                const float* ks[2];
+                Block4 dq[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    ks[x] = Ks + group * KS + 16 * min(x0 + 4 * x, 2 * DB - 1) + col;
+                    dq[x] = Block4{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                float a[4], c[4][2];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    a[r] = ds[4 * r];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) c[r][x] = ks[x][4 * r * KS];
+                }
+#pragma unroll
+                for (int n = 0; n < KEY_BLOCK / 16; ++n) {
+                    const int ahead = 16 * (n + 1 < KEY_BLOCK / 16 ? n + 1 : n);
+                    float an[4], cn[4][2];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        an[r] = ds[ahead + 4 * r];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) cn[r][x] = ks[x][(ahead + 4 * r) * KS];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) dq[x] = mfma4(a[r], c[r][x], dq[x]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        a[r] = an[r];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) c[r][x] = cn[r][x];
+                    }
+                    fence();
+                }
+                const Rows rows = rows_at(w.dq + ((size_t)slot * heads * z.Tq + row0 + i0) * z.D, min(STEP, z.Tq - i0), z.D, z.D);
+                const int from = fresh(lane);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const int d = 16 * (x0 + 4 * x) + (from & 15);
+                    const uint32_t to = x0 + 4 * x < 2 * DB && d < z.D ? ((uint32_t)(q0 + 4 * (from >> 4)) * z.D + d) * 4 : NOWHERE;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) put_one(rows, to + (uint32_t)(4 * r * z.D), dq[x][r]);
+                }
+            }
+            if (BIAS && w.diagonals && t < KEY_BLOCK + STEP - 1) {
+                float* sum = Sums + t - (STEP - 1) - (i0 - c0) + QUERY_CHUNK - 1;
+                const float* ds = Ds + t - (STEP - 1);
+                float x = *sum;
+#pragma unroll
+                for (int q = 0; q < STEP; ++q) x = x + ds[q * (DS_STRIDE + 1)];
+                *sum = x;
+            }
+            if (more) store(i0 + STEP);
+            lds_barrier();
+        }
+        const bool last = w.direct && chunk == w.chunks - 1;
+        const size_t chunk_out = out_of(z, w, bh, chunk);
+        const bool add = w.parts == 1 && begun;
+        begun = true;
+        const auto leave = [&](float* base, const Block4* sum, float scale) {
+            const Rows rows = rows_at(base + chunk_out + k0 * out_stride, min(KEY_BLOCK, z.Tk - k0), out_stride, z.D);
+            const int lane = fresh(threadIdx.x) & 63, group = lane >> 4;
+            const uint32_t to = ((uint32_t)(16 * wave + (lane & 15)) * (uint32_t)out_stride + 4 * group) * 4;
+            float4 held[2 * DB];
+            if (add) {
+#pragma unroll
+                for (int n = 0; n < 2 * DB; ++n) held[n] = four<QUADS>(rows, to + 64 * n, z.D - 16 * n - 4 * group);
+            }
+#pragma unroll
+            for (int n = 0; n < 2 * DB; ++n) {
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    broken = __builtin_fmaf(sum[n][r], 0.0f, broken);
+                    v[r] = add ? part_of(held[n], r) + sum[n][r] : sum[n][r];
+                    if (last) v[r] = v[r] * scale + 0.0f;
+                }
+                put_four<QUADS>(rows, to + 64 * n, z.D - 16 * n - 4 * group, v);
+            }
+        };
+        leave(w.dk, dk, z.scale);
+        leave(w.dv, dv, 1.0f);
+        if (diagonals)
+            for (int n = t; n < DIAGONALS; n += 512) diagonals[n] = Sums[n];
+    }
+    if (w.broken) {  // a NaN or infinity, which the products' zeros hand to pairs that are not seen, shows in every key's sums
+        const int any = __syncthreads_or(broken != broken);
+        if (t == 0) w.broken[blockIdx.x] = any;
+    }
+}
+
 // Redoes the blocks whose operands hold a NaN or infinity, key by key, row by row and pair by pair.
 __global__ void __launch_bounds__(256)
 repair(Problem z, Gradients g, Work w) {
@@ -585,7 +915,7 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
     w.diagonals = dbias ? reinterpret_cast<float*>(base + p.diagonals) : nullptr;
     // a query's values must not reach keys that it does not see, nor a key's a query
     w.broken = z.causal || z.mask || z.key_lengths ? reinterpret_cast<int*>(base + p.broken) : nullptr;
-    if ((long long)z.B * z.H * w.count * w.parts > MAX_BLOCKS || (dbias && (long long)z.H * ((z.Tq + z.Tk + 62) / 64) > MAX_BLOCKS))
+    if ((long long)z.B * z.H * w.count * w.parts > MAX_BLOCKS / 2 || (dbias && (long long)z.H * ((z.Tq + z.Tk + 62) / 64) > MAX_BLOCKS))
         return hipErrorInvalidValue;
     const int most = w.count;
     for (int first = 0; first < p.blocks; first += most) {
@@ -594,8 +924,13 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
         const bool begins = first == 0, ends = first + w.count == p.blocks;
         with_size(z.D, [&](auto db) {
             with_flags(z.bias != nullptr, z.threshold != 0, z.quads != 0, [&](auto bias, auto drop, auto quads) {
-                hipLaunchKernelGGL((backward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value, decltype(quads)::value>),
-                                   dim3((unsigned)(z.B * z.H * w.count * w.parts)), dim3(256), 0, stream, z, g, w);
+                constexpr int DB = decltype(db)::value;
+                constexpr bool BIAS = decltype(bias)::value, DROP = decltype(drop)::value, QUADS = decltype(quads)::value;
+                const dim3 grid((unsigned)(z.B * z.H * w.count * w.parts));
+                if constexpr (DB <= 2)
+                    hipLaunchKernelGGL((backward_tiles<DB, BIAS, DROP, QUADS>), grid, dim3(256), 0, stream, z, g, w);
+                else
+                    hipLaunchKernelGGL((backward_wide<DB, BIAS, DROP, QUADS>), grid, dim3(512), 0, stream, z, g, w);
             });
         });
         if (w.broken)

@@ -45,7 +45,7 @@ struct Parts {
     float2* ml;                        // [slots][B][H][Tq]
     float* o;                          // [slots][B][H][Tq][D]
     __device__ __forceinline__ int slot_of(int chunk) const { return chunk < a_part ? 0 : chunk - a_part + 1; }
-    int* broken;                // a number for each block: whether `repair` has to redo it; null where it never has to
+    int* broken;                       // a number for each block: whether `repair` has to redo it; null where it never has to
 };
 
 // The block's place: head, first query, part.
@@ -361,8 +361,8 @@ repair(Problem z, Parts s, float* y, float* stats) {
 
 // Few queries: a block takes a chunk of keys for up to FEW of the rows that share a head of keys, a thread a key for the
 // scores, then a wavefront a row and a lane a value. Bound by HBM: the keys are read into LDS as the values are on their way, and the
-// values take their place there. One query of 2048 to 4096
-// keys for 16 items of 12 heads of 64: 72 us and 5.5 to join the chunks, 4.9 TB/s of the 5.25 of a copy.
+// values take their place there. One query of 2048 to 4096 keys for 16 items of 12 heads of 64: 72 us and 5.5 to join the
+// chunks, 4.9 TB/s of the 5.25 of a copy; heads of 128, whose keys leave room for one block a compute unit: 3.4.
 constexpr int FEW = 8;
 
 template <int DB, bool QUADS>
@@ -704,7 +704,8 @@ Parts parts_of(const Problem& z) {
     return s;
 }
 long long blocks_of(const Problem& z, const Parts& s) {
-    return few(z) ? (long long)z.B * z.KVH * ((z.group * z.Tq + FEW - 1) / FEW) * s.chunks : (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
+    return few(z) ? (long long)z.B * z.KVH * ((z.group * z.Tq + FEW - 1) / FEW) * s.chunks
+                  : (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
 }
 // What a key holds must not reach a row that does not see it: under a causal mask or one of pairs.
 // (Few rows leave out each pair by itself.)
@@ -737,7 +738,9 @@ int forward(const Problem& z, float* y, float* stats, unsigned long long* used, 
             return;
         }
         with_flags(z.bias != nullptr, z.threshold != 0, z.quads != 0, [&](auto bias, auto drop, auto quads) {
-            hipLaunchKernelGGL((forward_tiles<decltype(db)::value, decltype(bias)::value, decltype(drop)::value, decltype(quads)::value>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
+            constexpr int DB = decltype(db)::value;
+            constexpr bool BIAS = decltype(bias)::value, DROP = decltype(drop)::value, QUADS = decltype(quads)::value;
+            hipLaunchKernelGGL((forward_tiles<DB, BIAS, DROP, QUADS>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
         });
     });
     int rc = hipGetLastError();

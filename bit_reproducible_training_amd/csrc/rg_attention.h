@@ -18,6 +18,7 @@ using repro_attention::CHUNK;
 using repro_attention::ds_of;
 using repro_attention::e2;
 using repro_attention::KEY_BLOCK;
+using repro_attention::is_large;
 using repro_attention::larger;
 using repro_attention::NONE;
 using repro_attention::QUERY_CHUNK;
@@ -84,7 +85,7 @@ __device__ __forceinline__ Score score(const Problem& z, int b, int h, int i, in
     return Score{s, __builtin_fmaf(s, z.factor, bias_term(z.bias[(size_t)h * (z.Tq + z.Tk - 1) + j - i + z.Tq - 1]))};
 }
 __device__ __forceinline__ float less(const Problem& z, const Score& a, float m) {
-    return z.bias ? a.t - m : __builtin_fmaf(a.s, z.factor, -m);
+    return repro_attention::less(a.s, a.t, z.factor, m, z.bias != nullptr);
 }
 __device__ __forceinline__ bool kept(const Problem& z, uint64_t seed, int b, int h, int i, int j) {
     if (z.threshold == 0) return true;

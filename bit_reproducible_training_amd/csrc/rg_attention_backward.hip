@@ -76,13 +76,14 @@ __device__ __forceinline__ bool live(const Problem& z, int len, int block, int r
     return block * KEY_BLOCK < last_end(z, len, min(rows, z.Tq) - 1);
 }
 
+// Without a bias and dropout heads of up to 32 values leave room for a third wavefront a SIMD.
 template <int DB, bool BIAS, bool DROP, bool QUADS>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, DB == 1 && !BIAS && !DROP ? 3 : 2)
 backward_tiles(Problem z, Gradients g, Work w) {
     constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 8;
     __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds_[STEP + STEP * DS_STRIDE];
     __shared__ float Bs[BIAS ? 160 : 1], Sums[BIAS ? DIAGONALS : 1];
-    __shared__ float4 Query[STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits
+    __shared__ float4 Query[(BIAS ? 1 : 2) * STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits; the same with m = 0
     __shared__ uint32_t Masks[STEP][4];
     float* Ds = Ds_ + STEP;  // (zeros before the first row, too)
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
@@ -185,8 +186,11 @@ backward_tiles(Problem z, Gradients g, Work w) {
             *reinterpret_cast<float2*>(Ys + to) = make_float2(yn[x].x, yn[x].z);
             *reinterpret_cast<float2*>(Ys + to + 4) = make_float2(yn[x].y, yn[x].w);
         }
-        if (t < STEP) Query[t] = make_float4(sn.x, sn.y, en, __int_as_float(i0 + t < z.Tq ? last_end(z, len, i0 + t) : 0));
-        else if (t >= 128) Masks[(t >> 2) & (STEP - 1)][t & 3] = mn;
+        if (t < (BIAS ? 1 : 2) * STEP) {
+            const int i = i0 + (t & (STEP - 1));
+            Query[t] = make_float4(t < STEP ? sn.x : 0.0f, sn.y, en, __int_as_float(i < z.Tq ? last_end(z, len, i) : 0));
+        }
+        if (t >= 128) Masks[(t >> 2) & (STEP - 1)][t & 3] = mn;
         if (BIAS && t < KEY_BLOCK + STEP - 1) Bs[t] = bias_term(bn);
     };
     const int row_of = (col & 24) + 2 * (col & 3) + ((col >> 2) & 1);     // the query that row `col` of an operand is
@@ -246,13 +250,21 @@ backward_tiles(Problem z, Gradients g, Work w) {
                 keep[2] = __builtin_amdgcn_update_dpp(0, bits, 0xAA, 0xF, 0xF, true) >> r;
                 keep[3] = __builtin_amdgcn_update_dpp(0, bits, 0xFF, 0xF, 0xF, true) >> r;
             }
+            const bool large = !BIAS && __any(is_large(Query[lane & (STEP - 1)].x));
+            if (large) {  // the exponents are made here, and kept by what follows
+#pragma unroll
+                for (int n = 0; n < 16; ++n)
+                    s[n] = repro_attention::less(s[n], s[n] * z.factor, z.factor, Query[8 * (n / 4) + 2 * (n % 4) + half].x, false);
+            }
+            const float factor = large ? 1.0f : z.factor;
+            const float4* rows = Query + (large ? STEP : 0);
             const auto differentials = [&](auto edge) {
 #pragma unroll
                 for (int n = 0; n < 16; ++n) {
                     const int q = 8 * (n / 4) + 2 * (n % 4) + half;
-                    const float4 row = Query[q];
+                    const float4 row = rows[q];
                     const float x = BIAS ? __builtin_fmaf(s[n], z.factor, Bs[32 * wave + col - q + STEP - 1]) - row.x
-                                         : __builtin_fmaf(s[n], z.factor, -row.x);
+                                         : __builtin_fmaf(s[n], factor, -row.x);
                     float p = e2(x) * row.y, d = dp[n], u = p;
                     if (DROP) {
                         const bool kept = (keep[n % 4] >> (4 * (n / 4)) & 1) != 0;
@@ -406,7 +418,7 @@ backward_wide(Problem z, Gradients g, Work w) {
     constexpr int DP = 32 * DB, QS = DP + 4, KS = DP + 8;
     __shared__ float Ks[KEY_BLOCK * KS], Qs[STEP * QS], Ys[STEP * QS], Ds_[STEP + STEP * DS_STRIDE];
     __shared__ float Bs[BIAS ? 160 : 1], Sums[BIAS ? DIAGONALS : 1];
-    __shared__ float4 Query[STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits
+    __shared__ float4 Query[(BIAS ? 1 : 2) * STEP];  // m, 1 / L, delta, and the keys that the query sees, as bits; the same with m = 0
     __shared__ uint32_t Masks[STEP][4];
     float* Ds = Ds_ + STEP;  // (zeros before the first row, too)
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
@@ -500,8 +512,11 @@ backward_wide(Problem z, Gradients g, Work w) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) p[4 * c] = part_of(qn[x], c);
         }
-        if (t < STEP) Query[t] = make_float4(sn.x, sn.y, en, __int_as_float(i0 + t < z.Tq ? last_end(z, len, i0 + t) : 0));
-        else if (t >= 128 && t < 256) Masks[(t >> 2) & (STEP - 1)][t & 3] = mn;
+        if (t < (BIAS ? 1 : 2) * STEP) {
+            const int i = i0 + (t & (STEP - 1));
+            Query[t] = make_float4(t < STEP ? sn.x : 0.0f, sn.y, en, __int_as_float(i < z.Tq ? last_end(z, len, i) : 0));
+        }
+        if (t >= 128 && t < 256) Masks[(t >> 2) & (STEP - 1)][t & 3] = mn;
         if (BIAS && t < KEY_BLOCK + STEP - 1) Bs[t] = bias_term(bn);
     };
     const int row_of = 4 * (col & 3) + (col >> 2);    // the query of 16 that row `col` of an operand is
@@ -575,15 +590,25 @@ backward_wide(Problem z, Gradients g, Work w) {
                 keep[2] = __builtin_amdgcn_update_dpp(0, bits, 0xAA, 0xF, 0xF, true) >> r;
                 keep[3] = __builtin_amdgcn_update_dpp(0, bits, 0xFF, 0xF, 0xF, true) >> r;
             }
+            const bool large = !BIAS && __any(is_large(Query[lane & (STEP - 1)].x));
+            if (large) {  // the exponents are made here, and kept by what follows
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        s[n][r] = repro_attention::less(s[n][r], s[n][r] * z.factor, z.factor, Query[16 * n + 4 * r + group].x, false);
+            }
+            const float factor = large ? 1.0f : z.factor;
+            const float4* rows = Query + (large ? STEP : 0);
             const auto differentials = [&](auto edge) {
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int q = 16 * n + 4 * r + group;
-                        const float4 row = Query[q];
+                        const float4 row = rows[q];
                         const float x = BIAS ? __builtin_fmaf(s[n][r], z.factor, Bs[16 * wave + col - q + STEP - 1]) - row.x
-                                             : __builtin_fmaf(s[n][r], z.factor, -row.x);
+                                             : __builtin_fmaf(s[n][r], factor, -row.x);
                         float p = e2(x) * row.y, d = dp[n][r], u = p;
                         if (DROP) {
                             const bool kept = (keep[r] >> (4 * n) & 1) != 0;

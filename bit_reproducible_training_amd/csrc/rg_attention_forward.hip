@@ -241,12 +241,21 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[n][r] = o[n][r] * a;
             }
+            const bool large = !BIAS && __any(is_large(base));  // (then the exponents are made here, and kept by what follows)
+            if (large) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        p[kb][r] = repro_attention::less(p[kb][r], p[kb][r] * z.factor, z.factor, base, false);
+            }
+            const float factor = large ? 1.0f : z.factor, shift = large ? 0.0f : base;
             const auto exponentials = [&](auto masked) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        float x = BIAS ? p[kb][r] - base : __builtin_fmaf(p[kb][r], z.factor, -base);
+                        float x = BIAS ? p[kb][r] - shift : __builtin_fmaf(p[kb][r], factor, -shift);
                         if (decltype(masked)::value) x = (see[kb] >> (8 * (r / 4) + 2 * (r % 4)) & 1) != 0 ? x : NONE;
                         p[kb][r] = e2(x);
                         l = l + p[kb][r];
@@ -451,7 +460,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
         float m = NONE;
         for (int w = 0; w <= wave; ++w) m = larger(m, Tops[r][w]);
         const float base = base_of(m);
-        const float p = see[r] ? e2(z.bias ? term[r] - base : __builtin_fmaf(sum[r], z.factor, -base)) : 0.0f;
+        const float p = see[r] ? e2(less(z, Score{sum[r], term[r]}, base)) : 0.0f;
         P[r][t] = p;
     }
     __syncthreads();

@@ -65,7 +65,7 @@ struct Call {
         float s, t;
         bool biased;
         float factor;
-        float less(float m) const { return biased ? t - m : __builtin_fmaf(s, factor, -m); }
+        float less(float base) const { return repro_attention::less(s, t, factor, base, biased); }
     };
     Score score(long long b, long long h, long long i, long long j) const {
         const float s = dot(query(b, h, i), key(b, h, j), c.D);

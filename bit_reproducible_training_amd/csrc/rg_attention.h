@@ -20,9 +20,11 @@ using repro_attention::e2;
 using repro_attention::KEY_BLOCK;
 using repro_attention::is_large;
 using repro_attention::larger;
+using repro_attention::LOWEST;
 using repro_attention::NONE;
 using repro_attention::QUERY_CHUNK;
 using repro_attention::reciprocal;
+using repro_attention::rescale;
 using repro_attention::TILE;
 
 struct Problem {
@@ -103,7 +105,7 @@ __device__ __forceinline__ RowChunk row_chunk(const Problem& z, uint64_t seed, i
         const bool see = seen(z, b, h, i, j, end);
         const Score t = see ? score(z, b, h, i, j) : Score{NONE, NONE};
         const float next = larger(r.m, wave_max(t.t));
-        const float a = e2(r.m - base_of(next));
+        const float a = rescale(r.m, base_of(next));
         r.m = next;
         r.even = r.even * a, r.odd = r.odd * a, r.o0 = r.o0 * a, r.o1 = r.o1 * a;
         const float p = see ? e2(less(z, t, base_of(next))) : 0.0f;
@@ -126,7 +128,7 @@ __device__ __forceinline__ RowChunk row_chunk(const Problem& z, uint64_t seed, i
 struct Joined {
     float top = NONE, total = 0.0f, o0 = 0.0f, o1 = 0.0f;
     __device__ __forceinline__ void join(const RowChunk& r) {
-        const float both = larger(top, r.m), a = e2(top - base_of(both)), e = e2(r.m - base_of(both));
+        const float both = larger(top, r.m), a = rescale(top, base_of(both)), e = rescale(r.m, base_of(both));
         top = both;
         total = __builtin_fmaf(r.even + r.odd, e, total * a);
         o0 = __builtin_fmaf(r.o0, e, o0 * a);

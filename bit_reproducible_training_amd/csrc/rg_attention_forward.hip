@@ -232,7 +232,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
                 next = larger(__uint_as_float(x), __uint_as_float(w));
             }
             next = larger(m, BIAS ? next : next * z.factor);
-            const float base = base_of(next), a = e2(m - base);
+            const float base = base_of(next), a = rescale(m, base);
             m = next;
             l = l * a;
             if (__any(a != 1.0f)) {
@@ -256,7 +256,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         float x = BIAS ? p[kb][r] - shift : __builtin_fmaf(p[kb][r], factor, -shift);
-                        if (decltype(masked)::value) x = (see[kb] >> (8 * (r / 4) + 2 * (r % 4)) & 1) != 0 ? x : NONE;
+                        if (decltype(masked)::value) x = (see[kb] >> (8 * (r / 4) + 2 * (r % 4)) & 1) != 0 ? x : LOWEST;
                         p[kb][r] = e2(x);
                         l = l + p[kb][r];
                     }
@@ -294,7 +294,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
         if (part > 0) {
             leave(chunk, m, both_l, o);
         } else {
-            const float both = larger(top, m), base = base_of(both), a = e2(top - base), e = e2(m - base);
+            const float both = larger(top, m), base = base_of(both), a = rescale(top, base), e = rescale(m, base);
             top = both;
             total = __builtin_fmaf(both_l, e, total * a);
 #pragma unroll
@@ -471,7 +471,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float up = larger(m, Tops[r][w]);
-            a[w] = e2(m - base_of(up));
+            a[w] = rescale(m, base_of(up));
             m = up;
         }
         return m;
@@ -603,7 +603,7 @@ join_chunks(Problem z, Parts s, float* y, float* stats) {
             float before = __shfl_up(run, 1, 64);
             if (lane == 0) before = all.top;
             const float base = base_of(run);
-            const float a = there ? e2(before - base) : 1.0f, e = there ? e2(ml.x - base) : 0.0f;
+            const float a = there ? rescale(before, base) : 1.0f, e = there ? rescale(ml.x, base) : 0.0f;
             const unsigned long long which = __ballot(there);
             all.top = __shfl(run, 63, 64);
             const float* o = s.o + (first * rows + n) * z.D;
@@ -664,7 +664,7 @@ join_few(Problem z, Parts s, float* y, float* stats) {
 #pragma unroll
         for (int k = 0; k < SLOTS; ++k) {
             if (k >= s.slots || ml[k].y == -1.0f) continue;
-            const float both = larger(top, ml[k].x), base = base_of(both), a = e2(top - base), e = e2(ml[k].x - base);
+            const float both = larger(top, ml[k].x), base = base_of(both), a = rescale(top, base), e = rescale(ml[k].x, base);
             top = both;
             total = __builtin_fmaf(ml[k].y, e, total * a);
 #pragma unroll

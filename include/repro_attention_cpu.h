@@ -95,7 +95,7 @@ inline void forward_row(const Call& z, long long b, long long h, long long i, fl
                 t[n] = z.score(b, h, i, j0 + n);
                 next = larger(next, t[n].t);
             }
-            const float a = e2(m - base_of(next));
+            const float a = rescale(m, base_of(next));
             m = next;
             for (float& x : l) x = x * a;
             for (int d = 0; d < D; ++d) o[d] = o[d] * a;
@@ -108,7 +108,7 @@ inline void forward_row(const Call& z, long long b, long long h, long long i, fl
                 for (int d = 0; d < D; ++d) o[d] = __builtin_fmaf(u, v[d], o[d]);
             }
         }
-        const float both = larger(top, m), a = e2(top - base_of(both)), e = e2(m - base_of(both));
+        const float both = larger(top, m), a = rescale(top, base_of(both)), e = rescale(m, base_of(both));
         top = both;
         total = __builtin_fmaf(l[0] + l[1], e, total * a);
         for (int d = 0; d < D; ++d) out[d] = __builtin_fmaf(o[d], e, out[d] * a);

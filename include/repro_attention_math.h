@@ -6,18 +6,18 @@
 //
 // Forward, for a query and a head, with c = scale log2 e (a negative scale's sign goes to the query):
 //   score  s_j = fma chain over d of q_d k_jd;  with a bias t_j = fma(s_j, c, bias_j log2 e), else t_j = s_j c
-//   keys are taken in chunks of CHUNK, a chunk in tiles of TILE: m' = max(m, visible t of the tile) from m = NONE, a = e2(m - m');
+//   keys are taken in chunks of CHUNK, a chunk in tiles of TILE: m' = max(m, visible t of the tile) from m = NONE, a = rescale(m, m');
 //   p_j = e2(less(t_j, m')); l_even = l_even a, then + p_j of the even keys in ascending order,
 //   l_odd likewise; o_d = o_d a, then the chain over the tile's keys of p_j v_jd
 //   less(t_j, m') = t_j - m', without a bias and for |m'| below LARGE fma(s_j, c, -m'), which spares a multiplication and t's rounding. (m' is
 //   rounded, so the largest key's own fma is up to half a unit in m's last place away from 0: at most 1/2 there, but 2^7 at 2^31.)
-//   chunks are joined in ascending order: M' = max(M, m), a = e2(M - M'), b = e2(m - M'),
+//   chunks are joined in ascending order: M' = max(M, m), a = rescale(M, M'), b = rescale(m, M'),
 //   L = fma(l_even + l_odd, b, L a), O_d = fma(o_d, b, O_d a)
 //   y_d = O_d (1 / L)
 // A masked key has p = 0 and nothing else of it takes part; a tile or chunk without visible keys changes nothing. So a
 // row's bits depend on its query and the keys it sees alone, not on the batch, the other queries or the padding.
-// NONE as a maximum counts as 0 in the exponents, so nothing below it does anything; a row that sees nothing has L = 0, which
-// 1 / L is 0 for. A NaN or infinite t gives its row NaN; a bias below LOWEST_BIAS (-infinity) counts as that.
+// NONE as a maximum counts as 0 in the exponents; a row that sees nothing has L = 0, which 1 / L is 0 for. A NaN or infinite t gives
+// its row NaN; a bias below LOWEST (-infinity) counts as that.
 // With dropout the dropped p_j are 0 in the chain over v (not in l) and y is multiplied by factor / L.
 //
 // Backward: p_ij = e2(less(t_ij, M_i)) (1 / L_i), delta_i = sum_d dy_d y_d, u_ij = p_ij kept factor,
@@ -35,7 +35,7 @@ using repro_gemm::bits_to_float;
 using repro_gemm::float_to_bits;
 
 constexpr int TILE = 64, CHUNK = 256, QUERY_CHUNK = 256, KEY_BLOCK = 128, MAX_D = 128;
-constexpr float LOG2E = 1.44269504f, NONE = -1e37f, LOWEST_BIAS = -1e30f, LARGE = 16777216.0f;
+constexpr float LOG2E = 1.44269504f, NONE = -__builtin_inff(), LOWEST = -1e30f, LARGE = 16777216.0f;
 inline float score_factor(double scale) { return (float)(scale * 1.4426950408889634); }
 
 // 2^x for finite x up to 0 and a rounding past it, within 1.6 units in the last place; 1 for 0, NaN for NaN and infinities. x = n + f
@@ -72,7 +72,12 @@ RG_HD inline float less(float s, float t, float c, float base, bool biased) {
 }
 RG_HD inline float bias_term(float bias) {
     const float b = bias * LOG2E;
-    return b < LOWEST_BIAS ? LOWEST_BIAS : b;
+    return b < LOWEST ? LOWEST : b;
+}
+// The factor for what was summed under the maximum m: 0 where nothing was, or where the two are further apart than float32 reaches.
+RG_HD inline float rescale(float m, float base) {
+    const float x = m - base;
+    return e2(x < LOWEST ? LOWEST : x);
 }
 // The larger of the two; the other where one is NaN.
 RG_HD inline float larger(float a, float b) { return __builtin_fmaxf(a, b); }

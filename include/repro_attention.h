@@ -8,8 +8,10 @@
  *   y_i = sum_j p_ij kept_ij / (1 - dropout) v_j
  * Query i of batch item b sees key j where j < key_lengths[b], with `causal` j <= i + query_start, and where the mask's bit is
  * set; one that sees none has y = 0 and takes no part in the gradients. What keys hold that no query sees, and what a
- * query and a key hold for each other where the one does not see the other, reaches nothing, NaN or not. A visible NaN, or a score
- * past float32's range, gives its row NaN.
+ * query and a key hold for each other where the one does not see the other, reaches nothing, NaN or not. A visible NaN or a score
+ * past float32's range gives its row NaN; two scores of a row that are further apart than that range can give it, or its gradients, NaN. Scores are
+ * counted in base 2, t_ij log2 e: one is past the range from 2.3e38 on, two can be apart by it from 1.1e38 on. A bias below
+ * -6.9e29 (-infinity) counts as that.
  * The random bits of dropout are a function of the seed and the places of query and key (include/repro_dropout_math.h).
  *
  * Every operation is rounded once in a fixed order (include/repro_attention_math.h): the bits do not depend on the

@@ -122,3 +122,20 @@ def test_rows_whose_scores_are_all_far_below_zero(device, tq, tk, d, h):
             got = run(device, t, s, dy)
             check_shared_by_equals({n: got[n] for n in ("y", "dq", "dv")}, t, s, dy)
             assert same_bits(got, run("cpu", t, s, dy))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scores_at_the_end_of_the_range(device):
+    """Base 2 scores of +-1.6e38 beside each other; those of +-2e38 are further apart than float32 reaches and may give NaN but nothing else
+    that is wrong, and one of 3.5e38 is past it and gives NaN. Other rows are as they are."""
+    for T, bias, fine in ((1.1e38, False, True), (1.1e38, True, True), (1.4e38, False, False), (1.4e38, True, False), (2.4e38, True, False)):
+        for tq in (1, 20):
+            t = {"q": torch.ones(1, tq, 1, 1), "k": torch.zeros(1, 300, 1, 1), "v": torch.randn(1, 300, 1, 1),
+                 "relative_bias": torch.zeros(1, tq + 299) if bias else None}
+            t["q"][:, 0], t["k"][:, 9], t["k"][:, 270] = T, 1.0, -1.0
+            s, dy = dict(scale=1.0, causal=False, query_start=0), torch.randn(1, tq, 1, 1)
+            got, want = run(device, t, s, dy), run("cpu", t, s, dy)
+            assert same_bits(got, want)
+            y = got["y"][0, 0, 0].cpu()
+            assert (torch.equal(y, t["v"][0, 9, 0]) and T < 2e38) or (y.isnan().all() and not fine)
+            assert got["y"][0, 1:].isfinite().all() and got["dq"][0, 1:].isfinite().all()

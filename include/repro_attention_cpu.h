@@ -35,6 +35,7 @@ struct Call {
     float keep_factor = repro_dropout::factor_of(c.dropout);
     uint32_t threshold = repro_dropout::threshold_of(c.dropout);
     long long words = (c.Tk + 63) / 64;
+    long long start = c.query_start > c.Tk ? c.Tk : c.query_start < -c.Tq ? -c.Tq : c.query_start;  // past the ends nothing changes
 
     const float* row(const float* p, const long long* s, long long b, long long n, long long h) const {
         return p + b * s[0] + n * s[1] + h * s[2];
@@ -46,7 +47,7 @@ struct Call {
     long long end(long long b, long long i) const {
         long long n = c.Tk;
         if (key_lengths && key_lengths[b] < n) n = key_lengths[b];
-        if (c.causal && i + c.query_start + 1 < n) n = i + c.query_start + 1;
+        if (c.causal && i + start + 1 < n) n = i + start + 1;
         return n < 0 ? 0 : n;
     }
     bool seen(long long b, long long h, long long i, long long j) const {

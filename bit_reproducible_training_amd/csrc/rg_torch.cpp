@@ -979,19 +979,24 @@ Tensor loss_apply(const Tensor& x, const Tensor& weight, const Tensor& target, i
 
 // A leaf keeps the stream that the first graph over it was made on for as long as such a graph lives, and a backward pass
 // waits for that stream; one that is being captured cannot wait for a stream outside of its capture, and PyTorch ends the process
-// over it. So the forward pass is refused there.
+// over it. So the forward pass is refused there, where an operand is such a leaf itself.
+bool capturing(const Tensor& t, const char* op) {
+    if (!at::GradMode::is_enabled() || !t.is_cuda()) return false;
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(t.get_device()).stream();
+    if (!stream) return false;  // (the default stream cannot be captured)
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    check((int)hipStreamIsCapturing(stream, &status), op);
+    return status != hipStreamCaptureStatusNone;
+}
 void need_capturable(const std::vector<const Tensor*>& operands, const char* op) {
     if (!at::GradMode::is_enabled()) return;
     for (const Tensor* t : operands) {
         if (!t->defined() || !t->is_cuda() || !t->requires_grad() || !t->is_leaf()) continue;
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         if (!node || !node->stream().has_value()) continue;
-        const auto current = c10::hip::getCurrentHIPStream(t->get_device());
-        if (node->stream()->id() == current.unwrap().id()) continue;
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        check((int)hipStreamIsCapturing(current.stream(), &status), op);
-        need(status == hipStreamCaptureStatusNone,
-             std::string(op) + ": a graph over an operand that was made outside of this capture is still alive; free it before");
+        if (node->stream()->id() == c10::hip::getCurrentHIPStream(t->get_device()).unwrap().id()) continue;
+        need(!capturing(*t, op), std::string(op) + ": a graph over an operand that was made outside of this capture is still alive; free it "
+                                                   "before, or capture under torch.no_grad() where no backward pass is wanted");
     }
 }
 
@@ -1395,6 +1400,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("adamw8_values", &adamw8_values);
     m.def("norm_apply", &norm_apply);
     m.def("loss_apply", &loss_apply);
+    m.def("capturing", [](const Tensor& t) { return capturing(t, "capture"); });
     m.def("need_capturable", [](const std::vector<Tensor>& operands, const std::string& op) {
         std::vector<const Tensor*> each;
         for (const Tensor& t : operands) each.push_back(&t);

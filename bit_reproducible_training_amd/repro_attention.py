@@ -134,7 +134,9 @@ class Attention(torch.nn.Module):
         self.out = Linear(num_heads * self.head_size, width, bias=bias)
 
     def forward(self, x, states=None, *, causal=False, query_start=0, key_lengths=None, mask=None, relative_bias=None, seed=None):
-        _backend.need_capturable([x, *self.parameters()], "Attention")
+        if _backend.capturing(x):
+            operands = [t for t in (x, states, relative_bias) if t is not None]
+            _backend.need_capturable(operands + list(self.parameters()), "Attention")
         states = x if states is None else states
         q = self.query(x).unflatten(-1, (self.num_heads, self.head_size))
         k, v = self.key_value(states).unflatten(-1, (2, self.num_kv_heads, self.head_size)).unbind(-3)

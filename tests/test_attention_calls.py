@@ -23,3 +23,41 @@ def test_a_start_past_every_key_sees_all_and_one_before_sees_none(device, tq, tk
     for start in (-tq, -2 ** 32 - 1, -2 ** 63):
         got = gradients(to(device, t), {**s, "causal": True, "query_start": start}, dy.to(device))
         assert all(torch.all(x == 0) for x in got.values()), start
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["x", "states", "relative_bias"])
+def test_the_layer_refuses_a_capture_beside_an_eager_graph_of_an_operand(which):
+    """(The layer's own parameters have none.)"""
+    layer = rg.Attention(16, 2).cuda()
+    t = {"x": torch.randn(1, 5, 16, device="cuda"), "states": torch.randn(1, 7, 16, device="cuda"),
+         "relative_bias": torch.randn(2, 11, device="cuda")}
+    t[which].requires_grad_()
+    alive = t[which] * 2
+    torch.cuda.synchronize()
+    refused = None
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        torch.zeros(4, device="cuda").add_(1)
+        try:
+            layer(**t)
+        except ValueError as e:
+            refused = str(e)
+        with torch.no_grad():
+            layer(**t)
+    assert "still alive" in refused
+    del alive
+    want = torch.autograd.grad(layer(**t).sum(), t[which])[0]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layer(**t).sum(), t[which])[0]
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_a_capture_is_asked_for_where_there_can_be_one():
+    from bit_reproducible_training_amd._lib import _backend
+
+    assert not _backend.capturing(torch.zeros(1))

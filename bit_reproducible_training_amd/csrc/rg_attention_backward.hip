@@ -850,10 +850,10 @@ sum_keys(Problem z, Work w, float* dk, float* dv) {
 constexpr int TERMS = 64;
 
 __global__ void __launch_bounds__(256)
-sum_diagonals(Problem z, Work w, float* dbias, int begins, int ends) {
+sum_diagonals(Problem z, Work w, int first_head, float* dbias, int begins, int ends) {
     __shared__ float terms[TERMS][64];
     const int columns = z.Tq + z.Tk - 1, across = (columns + 63) / 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int h = blockIdx.x / across, column = (blockIdx.x % across) * 64 + lane, away = column - (z.Tq - 1);
+    const int h = first_head + blockIdx.x / across, column = (blockIdx.x % across) * 64 + lane, away = column - (z.Tq - 1);
     const bool there = column < columns;
     float s = begins || !there || wave > 0 ? 0.0f : dbias[(size_t)h * columns + column];
     // the key blocks that one of the block's distances meets
@@ -888,7 +888,8 @@ sum_diagonals(Problem z, Work w, float* dbias, int begins, int ends) {
 // dQ's sums read what they add at the copy's rate (210 us of the 4096 x 4096 pass; making the scores again instead would
 // be 2 of 7 products more, 1.3 ms).
 //
-// How the key blocks are taken: as many at a time as leave at most a gigabyte for dQ and half of one for the bias; the queries split
+// How the key blocks are taken: as many at a time as leave at most a gigabyte for dQ and half of one for the bias and make a grid of
+// at most 2^22 blocks; the queries split
 // over blocks, whole chunks each, where the key blocks alone leave compute units idle and the chunks' results stay below
 // half a gigabyte.
 struct Plan {
@@ -907,6 +908,7 @@ Plan plan_of(const Problem& z, bool want_bias) {
     const size_t diagonals = want_bias ? (size_t)z.B * z.H * p.w.chunks * DIAGONALS * sizeof(float) : 0;
     size_t at_a_time = a_block > 0 ? (1u << 30) / a_block : 1;
     if (diagonals > 0) at_a_time = std::min(at_a_time, (size_t)(1 << 29) / diagonals);
+    at_a_time = std::min(at_a_time, (size_t)(MAX_BLOCKS / 2) / std::max<size_t>((size_t)z.B * z.H, 1));  // (at least four)
     p.w.count = (int)std::min(std::max<size_t>(at_a_time, 1), (size_t)p.blocks);
     const long long grid = (long long)z.B * z.H * p.w.count;
     long long parts = grid > 0 && grid < 384 ? (512 + grid - 1) / grid : 1;
@@ -940,9 +942,7 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
     w.diagonals = dbias ? reinterpret_cast<float*>(base + p.diagonals) : nullptr;
     // a query's values must not reach keys that it does not see, nor a key's a query
     w.broken = z.causal || z.mask || z.key_lengths ? reinterpret_cast<int*>(base + p.broken) : nullptr;
-    if ((long long)z.B * z.H * w.count * w.parts > MAX_BLOCKS / 2 || (dbias && (long long)z.H * ((z.Tq + z.Tk + 62) / 64) > MAX_BLOCKS))
-        return hipErrorInvalidValue;
-    const int most = w.count;
+    const int most = w.count, across = (z.Tq + z.Tk - 1 + 63) / 64, heads = (int)(MAX_BLOCKS / across);  // (of a launch of sum_diagonals)
     for (int first = 0; first < p.blocks; first += most) {
         w.first = first;
         w.count = std::min(most, p.blocks - first);
@@ -966,8 +966,9 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
             hipLaunchKernelGGL(sum_keys, dim3(grid_of((long long)z.B * std::min(z.Tk, w.count * KEY_BLOCK) * z.KVH * z.D, 256)), dim3(256),
                                0, stream, z, w, dk, dv);
         if (dbias)
-            hipLaunchKernelGGL(sum_diagonals, dim3((unsigned)(z.H * ((z.Tq + z.Tk - 1 + 63) / 64))), dim3(256), 0, stream, z, w, dbias,
-                               begins, ends);
+            for (int h = 0; h < z.H; h += heads)
+                hipLaunchKernelGGL(sum_diagonals, dim3((unsigned)(std::min(heads, z.H - h) * across)), dim3(256), 0, stream, z, w, h, dbias,
+                                   begins, ends);
         const int rc = hipGetLastError();
         if (rc != hipSuccess) return rc;
     }

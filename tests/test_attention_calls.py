@@ -61,3 +61,38 @@ def test_a_capture_is_asked_for_where_there_can_be_one():
     from bit_reproducible_training_amd._lib import _backend
 
     assert not _backend.capturing(torch.zeros(1))
+
+
+def each_alone(t, s, dy, of, index):
+    """{y, d...} of the slices of dimension `of` (0: items, 2: heads of queries) that `index` names, by themselves."""
+    cut = lambda x: None if x is None else x[index:index + 1] if of == 0 else x[:, :, index:index + 1]
+    own = {n: cut(x) if of == 0 or n == "q" else x for n, x in t.items()}
+    if of == 2 and t["relative_bias"] is not None:
+        own["relative_bias"] = t["relative_bias"][index:index + 1]
+    return gradients(own, s, cut(dy))
+
+
+@pytest.mark.gpu
+def test_a_gradient_of_many_items_over_many_key_blocks():
+    """2^18 heads over 32 blocks of keys: 2^23 in all, which takes two turns."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    t = {"q": torch.randn(2048, 1, 128, 1, device="cuda", generator=g), "relative_bias": None,
+         **{n: torch.randn(2048, 4096, 1, 1, device="cuda", generator=g) for n in "kv"}}
+    dy = torch.randn(2048, 1, 128, 1, device="cuda", generator=g)
+    got = gradients(t, {}, dy)
+    for b in (0, 1000, 2047):
+        alone = each_alone(t, {}, dy, 0, b)
+        assert all(torch.equal(got[n][b], alone[n][0]) for n in alone), b
+
+
+@pytest.mark.gpu
+def test_a_bias_gradient_of_many_heads_and_distances():
+    """2^15 heads of 257 x 64 distances."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    t = {"q": torch.randn(1, 1, 2 ** 15, 1, device="cuda", generator=g), "relative_bias": torch.randn(2 ** 15, 16385, device="cuda", generator=g),
+         **{n: torch.randn(1, 16385, 1, 1, device="cuda", generator=g) for n in "kv"}}
+    dy = torch.randn(1, 1, 2 ** 15, 1, device="cuda", generator=g)
+    got = gradients(t, {}, dy)
+    for h in (0, 20000, 2 ** 15 - 1):
+        alone = each_alone(t, {}, dy, 2, h)
+        assert torch.equal(got["drelative_bias"][h], alone["drelative_bias"][0]) and torch.equal(got["dq"][:, :, h], alone["dq"][:, :, 0])

@@ -42,10 +42,12 @@ __device__ __forceinline__ void halves(uint32_t v, uint32_t* low, uint32_t* high
 // was seen there) and o.
 struct Parts {
     int parts, chunks, a_part, slots;  // chunks a part; slots: 1 and the chunks after the first part's
+    uint32_t from;                     // blocks of earlier launches
     float2* ml;                        // [slots][B][H][Tq]
     float* o;                          // [slots][B][H][Tq][D]
     __device__ __forceinline__ int slot_of(int chunk) const { return chunk < a_part ? 0 : chunk - a_part + 1; }
     int* broken;                       // a number for each block: whether `repair` has to redo it; null where it never has to
+    __device__ __forceinline__ uint32_t block() const { return from + blockIdx.x; }
 };
 
 // The block's place: head, first query, part.
@@ -53,9 +55,9 @@ struct Place {
     int bh, i0, part;
 };
 __device__ __forceinline__ Place place_of(const Problem& z, const Parts& s) {
-    const int heads = z.B * z.H, rest = (int)(blockIdx.x / heads);
+    const int heads = z.B * z.H, rest = (int)(s.block() / heads);
     // under a causal mask the longest first
-    return Place{(int)(blockIdx.x % heads), ((z.Tq + ROWS - 1) / ROWS - 1 - rest / s.parts) * ROWS, rest % s.parts};
+    return Place{(int)(s.block() % heads), ((z.Tq + ROWS - 1) / ROWS - 1 - rest / s.parts) * ROWS, rest % s.parts};
 }
 
 // DB blocks of 32 values hold a head's; QUADS as in four().
@@ -310,7 +312,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
     if (s.parts == 1) watch(out);
     if (s.broken) {  // a NaN or infinity in v, which the products' zeros hand to rows that do not see it, shows in every row
         const int any = __syncthreads_or(broken != broken);
-        if (t == 0) s.broken[blockIdx.x] = any;
+        if (t == 0) s.broken[s.block()] = any;
     }
     if (s.parts == 1) {
         const float inverse = reciprocal(total), f = DROP ? inverse * z.keep_factor : inverse;
@@ -337,7 +339,7 @@ forward_tiles(Problem z, Parts s, float* y, float* stats, unsigned long long* us
 // Redoes the blocks whose values hold a NaN or infinity, row by row and pair by pair.
 __global__ void __launch_bounds__(256)
 repair(Problem z, Parts s, float* y, float* stats) {
-    if (s.broken[blockIdx.x] == 0) return;
+    if (s.broken[s.block()] == 0) return;
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Place at = place_of(z, s);
@@ -384,9 +386,9 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
     const uint64_t seed = z.seed_at ? *z.seed_at : z.seed;
     if (used && blockIdx.x == 0 && threadIdx.x == 0) *used = seed;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int heads = z.B * z.KVH, shares = (z.group * z.Tq + FEW - 1) / FEW, chunk = (int)(blockIdx.x / heads / shares);
-    const int r0 = (int)(blockIdx.x / heads % shares) * FEW;
-    const int b = (int)(blockIdx.x % heads) / z.KVH, kvh = (int)(blockIdx.x % heads) % z.KVH, h0 = kvh * z.group;
+    const int heads = z.B * z.KVH, shares = (z.group * z.Tq + FEW - 1) / FEW, chunk = (int)(s.block() / heads / shares);
+    const int r0 = (int)(s.block() / heads % shares) * FEW;
+    const int b = (int)(s.block() % heads) / z.KVH, kvh = (int)(s.block() % heads) % z.KVH, h0 = kvh * z.group;
     const int rows = min(FEW, z.group * z.Tq - r0), first = chunk * CHUNK;
     const int len = key_end(z, b, z.Tq - 1);  // what no row sees is not read
     const auto row_of = [&](int r) { return ((size_t)b * z.H + h0 + (r0 + r) / z.Tq) * z.Tq + (r0 + r) % z.Tq; };
@@ -697,6 +699,7 @@ Parts parts_of(const Problem& z) {
     s.ml = nullptr;
     s.o = nullptr;
     s.broken = nullptr;
+    s.from = 0;
     if (few(z)) {
         s.parts = s.slots = s.chunks;
         s.a_part = 1;
@@ -734,27 +737,29 @@ size_t forward_workspace(const Problem& z, bool masked) {
 int forward(const Problem& z, float* y, float* stats, unsigned long long* used, void* workspace, hipStream_t stream) {
     Parts s = parts_of(z);
     const long long rows = (long long)z.B * z.H * z.Tq, blocks = blocks_of(z, s);
-    if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
+    if (blocks > UINT32_MAX) return hipErrorInvalidValue;
     if (s.parts > 1) {
         s.ml = static_cast<float2*>(workspace);
         s.o = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums_offset(z, s));
     }
     if (watched(z, z.mask != nullptr)) s.broken = reinterpret_cast<int*>(static_cast<char*>(workspace) + parts_bytes(z, s));
-    with_size(z.D, [&](auto db) {
-        if (few(z)) {
-            auto kernel = z.quads ? few_rows<decltype(db)::value, true> : few_rows<decltype(db)::value, false>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
-            return;
-        }
-        with_flags(z.bias != nullptr, z.threshold != 0, z.quads != 0, [&](auto bias, auto drop, auto quads) {
-            constexpr int DB = decltype(db)::value;
-            constexpr bool BIAS = decltype(bias)::value, DROP = decltype(drop)::value, QUADS = decltype(quads)::value;
-            hipLaunchKernelGGL((forward_tiles<DB, BIAS, DROP, QUADS>), dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats, used);
+    int rc = hipSuccess;
+    for (long long from = 0; from < blocks && rc == hipSuccess; from += MAX_BLOCKS) {
+        s.from = (uint32_t)from;
+        const dim3 grid((unsigned)std::min(blocks - from, MAX_BLOCKS));
+        with_size(z.D, [&](auto db) {
+            if (few(z)) {
+                auto kernel = z.quads ? few_rows<decltype(db)::value, true> : few_rows<decltype(db)::value, false>;
+                hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, z, s, y, stats, used);
+                return;
+            }
+            with_flags(z.bias != nullptr, z.threshold != 0, z.quads != 0, [&](auto bias, auto drop, auto quads) {
+                constexpr int DB = decltype(db)::value;
+                constexpr bool BIAS = decltype(bias)::value, DROP = decltype(drop)::value, QUADS = decltype(quads)::value;
+                hipLaunchKernelGGL((forward_tiles<DB, BIAS, DROP, QUADS>), grid, dim3(256), 0, stream, z, s, y, stats, used);
+            });
         });
-    });
-    int rc = hipGetLastError();
-    if (rc == hipSuccess && s.broken) {
-        hipLaunchKernelGGL(repair, dim3((unsigned)blocks), dim3(256), 0, stream, z, s, y, stats);
+        if (s.broken) hipLaunchKernelGGL(repair, grid, dim3(256), 0, stream, z, s, y, stats);
         rc = hipGetLastError();
     }
     if (rc == hipSuccess && s.parts > 1) {

@@ -96,3 +96,29 @@ def test_a_bias_gradient_of_many_heads_and_distances():
     for h in (0, 20000, 2 ** 15 - 1):
         alone = each_alone(t, {}, dy, 2, h)
         assert torch.equal(got["drelative_bias"][h], alone["drelative_bias"][0]) and torch.equal(got["dq"][:, :, h], alone["dq"][:, :, 0])
+
+
+@pytest.mark.gpu
+def test_many_single_queries_over_many_chunks_of_keys():
+    """2^15 items by 258 chunks of the same keys: more than 2^23 blocks, which takes two launches."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(2 ** 15, 1, 1, 1, device="cuda", generator=g)
+    k, v = (torch.randn(1, 65793, 1, 1, device="cuda", generator=g) for _ in range(2))
+    y = rg.attention(q, k.expand(2 ** 15, -1, -1, -1), v.expand(2 ** 15, -1, -1, -1))
+    for b in (0, 20000, 2 ** 15 - 1):
+        assert torch.equal(y[b], rg.attention(q[b:b + 1], k, v)[0])
+
+
+@pytest.mark.gpu
+def test_many_items_of_many_queries():
+    """2^20 items of 9 blocks of queries, and a NaN that the last queries of the last items alone see."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = 2 ** 20
+    q, k = torch.randn(1, 1025, 1, 1, device="cuda", generator=g), torch.randn(1, 3, 1, 1, device="cuda", generator=g)
+    v = torch.randn(1, 3, 1, 1, device="cuda", generator=g).repeat(n, 1, 1, 1)
+    s = dict(causal=True, query_start=-1000)
+    want = rg.attention(q, k, v[:1], **s)
+    v[-5:, 2] = float("nan")
+    y = rg.attention(q.expand(n, -1, -1, -1), k.expand(n, -1, -1, -1), v, **s)
+    assert (y[:-5] == want).all()
+    assert (y[-5:, :1002] == want[:, :1002]).all() and y[-5:, 1002:].isnan().all()

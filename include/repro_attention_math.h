@@ -39,7 +39,8 @@ constexpr int TILE = 64, CHUNK = 256, QUERY_CHUNK = 256, KEY_BLOCK = 128, MAX_D 
 constexpr float LOG2E = 1.44269504f, NONE = -__builtin_inff(), LOWEST = -1e30f, LARGE = 16777216.0f;
 inline float score_factor(double scale) { return (float)(scale * 1.4426950408889634); }
 
-// 2^x for finite x up to 0 and a rounding past it, within 1.6 units in the last place; 1 for 0, NaN for NaN and infinities. x = n + f
+// 2^x for finite x up to 0 and a rounding past it, within 2.73 units in the last place (most at -0.00039, just below a power of two) or 2^-22.5,
+// over every float; 1 for 0, NaN for NaN and infinities. x = n + f
 // with n = floor x and 0 <= f < 1 (what rounds to 1 is the number before it); 2^f by a polynomial whose coefficients were fitted
 // to the least largest relative error (2^-23.3); times 2^n, rounded once where the result is subnormal.
 RG_HD inline float e2(float x) {

@@ -1,0 +1,47 @@
+"""The attention's exponential on the host against binary64: the bound that its comment states and that the error analysis of
+the attention's tests counts with (four units of 2^-24). The GPU's is compared with the host's by every comparison of bits."""
+import ctypes
+import math
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+@pytest.fixture(scope="module", params=[[], ["-mfma"]], ids=["calls", "instructions"])
+def ha(request, tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("ha") / "libha.so")
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off", "-fno-fast-math", *request.param, "-I",
+                    os.path.join(os.path.dirname(HERE), "include"), os.path.join(HERE, "host_attention_shim.cpp"), "-o", out], check=True)
+    lib = ctypes.CDLL(out)
+    lib.ha_e2.argtypes, lib.ha_e2.restype = [ctypes.c_float], ctypes.c_float
+    lib.ha_e2_errors.argtypes = [ctypes.c_uint32] * 3 + [ctypes.POINTER(ctypes.c_double)] * 3
+    return lib
+
+
+def bits(x):
+    return int(np.float32(x).view(np.uint32))
+
+
+def errors(ha, near, far, step):
+    e = [ctypes.c_double() for _ in range(3)]
+    ha.ha_e2_errors(bits(near), bits(far), step, *map(ctypes.byref, e))
+    return [x.value for x in e]
+
+
+def test_the_stated_bound(ha):
+    """Every 61st float, and every one about the worst: within 2.73 units in the last place and 2^-22.5; where the result is subnormal
+    the last product is rounded to 2^-149 once more."""
+    for near, far, step in ((-2.0 ** -40, -150.0, 61), (2.0 ** -40, 0.5, 61), (-0.00038, -0.00040, 1), (-0.2686, -0.2687, 1)):
+        units, relative, below = errors(ha, near, far, step)
+        assert units <= 2.73 and relative <= 2.0 ** -22.5 and below <= 0.5 + 2.0 ** 23 * 2.0 ** -22.5
+    assert errors(ha, -0.00038, -0.00040, 1)[0] > 2.7
+
+
+def test_the_ends(ha):
+    assert ha.ha_e2(0.0) == ha.ha_e2(-0.0) == 1.0
+    assert ha.ha_e2(-1e30) == ha.ha_e2(-151.0) == 0.0 and ha.ha_e2(-149.0) == 2.0 ** -149
+    assert all(math.isnan(ha.ha_e2(x)) for x in (math.nan, math.inf, -math.inf))

@@ -2,7 +2,6 @@
 // repro_attention_cpu.h -- the reproducible attention with its gradients and the bias of relative positions on the
 // host CPU (header-only C++17; no GPU needed), bit-identical to include/repro_attention.h's entries,
 // whose arguments these take (the mask packed to words of 64 keys). Arguments are not checked (the binding does).
-// Compiled with -mfma the fused multiply-adds are instructions, else calls; the bits are the same.
 #include <cmath>
 #include <cstdint>
 #include <vector>
@@ -20,7 +19,7 @@ namespace cpu_detail {
 template <class F>
 void spread(long long count, F run) {
     const long long parts = count < (1 << 20) ? count : 1 << 20;
-    repro_gemm::cpu_for((int)parts, [&](int part) {
+    repro_gemm::cpu_for_fused((int)parts, [&](int part) {
         for (long long n = part; n < count; n += parts) run(n);
     });
 }

@@ -13,6 +13,9 @@
 //   cpu_for(n, f)        calls f(i) exactly once for every i in [0, n), spread over the
 //                        workers; returns when all calls have returned. Results never depend
 //                        on the worker count, only on what f(i) writes.
+//   cpu_for_fused(n, f)  the same for an f with fused multiply-adds: on x86 from a copy of its code that
+//                        has them as instructions, where the processor does (they are calls else, with the
+//                        same bits). Nothing else needs more than the compiler's own target.
 //   cpu_gemm(A, B, C, M, N, K, ta, tb, S)
 //                        C[M][N] = op(A) op(B), all row-major: A is MxK (KxM when ta), B is
 //                        KxN (NxK when tb). Throws std::invalid_argument for a null pointer,
@@ -79,6 +82,27 @@ void cpu_for(int n, F f) {
     drain();
     for (auto& h : helpers) h.join();
 }
+
+#if defined(__x86_64__) && defined(__GNUC__) && !defined(__FMA__)
+namespace cpu_detail {
+// f and all it calls, compiled into one function.
+template <class F>
+__attribute__((target("fma"), flatten, noinline)) void call_with_fma(F& f, int i) {
+    f(i);
+}
+}  // namespace cpu_detail
+template <class F>
+void cpu_for_fused(int n, F f) {
+    static const bool has = __builtin_cpu_supports("fma") != 0;
+    if (has) cpu_for(n, [&](int i) { cpu_detail::call_with_fma(f, i); });
+    else cpu_for(n, f);
+}
+#else
+template <class F>
+void cpu_for_fused(int n, F f) {
+    cpu_for(n, f);
+}
+#endif
 
 namespace cpu_detail {
 

@@ -74,7 +74,7 @@ inline void cpu_linear_cross_entropy(const rg_loss_config& c, const float* x, co
         const float* xg = x + first * D;
         z.resize((size_t)rows * V);
         repro_gemm::cpu_gemm(xg, w, z.data(), rows, V, D, false, true, c.slices);
-        repro_gemm::cpu_for(rows, [&](int r) {
+        repro_gemm::cpu_for_fused(rows, [&](int r) {
             float* q = z.data() + (size_t)r * V;
             Token& t = tokens[first + r];
             const int64_t word = target[first + r];

@@ -3,6 +3,7 @@
 #include <cstdint>
 
 #include "repro_attention_math.h"
+#include "repro_gemm_cpu.h"
 
 extern "C" {
 
@@ -24,6 +25,17 @@ void ha_e2_errors(uint32_t lo, uint32_t hi, uint32_t step, double* units, double
         *units = std::fmax(*units, off / std::ldexp(1.0, e - 24));
         *relative = std::fmax(*relative, off / want);
     }
+}
+
+// out[i]: a chain of n fused multiply-adds and exponentials of a[i], by cpu_for_fused or by cpu_for.
+void ha_chains(const float* a, float* out, int count, int n, int fused) {
+    const auto run = [&](int i) {
+        float s = a[i];
+        for (int k = 0; k < n; ++k) s = __builtin_fmaf(s, a[i], repro_attention::e2(-s * s));
+        out[i] = s;
+    };
+    if (fused) repro_gemm::cpu_for_fused(count, run);
+    else repro_gemm::cpu_for(count, run);
 }
 
 }  // extern "C"

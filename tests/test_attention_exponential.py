@@ -14,10 +14,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 @pytest.fixture(scope="module", params=[[], ["-mfma"]], ids=["calls", "instructions"])
 def ha(request, tmp_path_factory):
     out = str(tmp_path_factory.mktemp("ha") / "libha.so")
-    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off", "-fno-fast-math", *request.param, "-I",
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off", "-fno-fast-math", "-pthread", *request.param, "-I",
                     os.path.join(os.path.dirname(HERE), "include"), os.path.join(HERE, "host_attention_shim.cpp"), "-o", out], check=True)
     lib = ctypes.CDLL(out)
     lib.ha_e2.argtypes, lib.ha_e2.restype = [ctypes.c_float], ctypes.c_float
+    lib.ha_chains.argtypes = [ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_int] * 3
     lib.ha_e2_errors.argtypes = [ctypes.c_uint32] * 3 + [ctypes.POINTER(ctypes.c_double)] * 3
     return lib
 
@@ -45,3 +46,18 @@ def test_the_ends(ha):
     assert ha.ha_e2(0.0) == ha.ha_e2(-0.0) == 1.0
     assert ha.ha_e2(-1e30) == ha.ha_e2(-151.0) == 0.0 and ha.ha_e2(-149.0) == 2.0 ** -149
     assert all(math.isnan(ha.ha_e2(x)) for x in (math.nan, math.inf, -math.inf))
+
+
+def test_fused_multiply_adds_are_the_same_as_instructions_and_as_calls(ha):
+    a = np.random.default_rng(1).uniform(-0.9, 0.9, 5000).astype(np.float32)
+    got = [np.empty_like(a) for _ in range(2)]
+    for fused in (0, 1):
+        ha.ha_chains(a.ctypes.data, got[fused].ctypes.data, a.size, 20, fused)
+    assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32)) and np.isfinite(got[0]).all()
+
+
+def test_the_binding_needs_no_more_than_the_compilers_own_target():
+    """On x86 it asks for no instructions that a processor may lack: those it uses where it finds them."""
+    from bit_reproducible_training_amd import _build
+
+    assert not [f for f in _build._binding_compile_cmd("x.o") if f.startswith("-m")]

@@ -97,11 +97,10 @@ diagonal_sums(Sizes z, const float* dout, float* part) {
 
 // A block adds up a bucket of a head: the columns [low, high) that the borders give it, column n in strand n mod STRANDS.
 __global__ void __launch_bounds__(STRANDS)
-bucket_sums(Sizes z, Borders borders, const float* dout, const float* part, float* dtable) {
+bucket_sums(Sizes z, Borders borders, int first_block, const float* dout, const float* part, float* dtable) {
     __shared__ float strand[STRANDS];
-    const int half = borders.count + 1, buckets = borders.both ? 2 * half : half;
-    const int bucket = blockIdx.x / z.H, h = blockIdx.x % z.H;
-    if (bucket >= buckets) return;
+    const int half = borders.count + 1, block = first_block + blockIdx.x;
+    const int bucket = block / z.H, h = block % z.H;
     const bool after = bucket >= half;
     const int c = after ? bucket - half : bucket;
     const long long never = 1ll << 40, near = c == 0 ? 0 : borders.at[c - 1], far = c + 1 == half ? never : borders.at[c];
@@ -208,8 +207,7 @@ int rg_relative_bias_grad_fp32(const rg_relative_bias_config* cfg, const float* 
     const long long values = values_of(cfg);
     if ((values > 0 && !dout) || (needed > 0 && (!workspace || workspace_bytes < needed || (reinterpret_cast<uintptr_t>(workspace) & 3) != 0)))
         return hipErrorInvalidValue;
-    const int buckets = (cfg->count + 1) * (cfg->both ? 2 : 1);
-    if ((long long)buckets * cfg->H > (1 << 23)) return hipErrorInvalidValue;
+    const int sums = (cfg->count + 1) * (cfg->both ? 2 : 1) * cfg->H, most = 1 << 23;  // (of a launch: it takes fewer than 2^32 threads)
     Sizes z = sizes_of(cfg);
     if (values == 0) z.Tq = 1, z.Tk = 0;  // no column: every sum is 0
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -218,8 +216,9 @@ int rg_relative_bias_grad_fp32(const rg_relative_bias_config* cfg, const float* 
         const long long blocks = (long long)((z.Tk + RUN - 1 + 255) / 256) * ((z.Tq + RUN - 1) / RUN) * z.H;
         hipLaunchKernelGGL(diagonal_sums, dim3(capped(blocks)), dim3(256), 0, st, z, dout, part);
     }
-    hipLaunchKernelGGL(bucket_sums, dim3((unsigned)(buckets * cfg->H)), dim3(STRANDS), 0, st, z, borders_of(cfg), dout, part,
-                       dtable);
+    for (int first = 0; first < sums; first += most)
+        hipLaunchKernelGGL(bucket_sums, dim3((unsigned)(sums - first < most ? sums - first : most)), dim3(STRANDS), 0, st, z, borders_of(cfg), first,
+                           dout, part, dtable);
     return hipGetLastError();
 }
 

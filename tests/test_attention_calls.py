@@ -122,3 +122,26 @@ def test_many_items_of_many_queries():
     y = rg.attention(q.expand(n, -1, -1, -1), k.expand(n, -1, -1, -1), v, **s)
     assert (y[:-5] == want).all()
     assert (y[-5:, :1002] == want[:, :1002]).all() and y[-5:, 1002:].isnan().all()
+
+
+@pytest.mark.gpu
+def test_a_table_of_many_heads_and_buckets():
+    """1026 buckets of 2^14 heads: more sums than a launch has blocks. (Only the C entry takes so many heads.)"""
+    import ctypes
+
+    from bit_reproducible_training_amd import _lib
+
+    h, count = 2 ** 14, 512
+    borders = (ctypes.c_int * count)(*range(1, count + 1))
+    c = _lib.rg_relative_bias_config(3, 700, 0, h, count, 1, 0, borders)
+    dout = torch.randn(h, 702, device="cuda")
+    out = torch.full((1026, h), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    assert _lib.lib.rg_relative_bias_grad_fp32(ctypes.byref(c), dout.data_ptr(), out.data_ptr(), None, 0, None) == 0
+    torch.cuda.synchronize()
+    want = torch.zeros(1026, h, device="cuda")
+    want[:3] = dout[:, [2, 1, 0]].t()  # distances 0, -1 and -2
+    want[514:514 + 511] = dout[:, 3:3 + 511].t()  # 1 to 511
+    assert torch.equal(out[:1025], want[:1025])
+    size = dout[:, 514:].double()
+    assert torch.all((out[1025].double() - size.sum(1)).abs() <= 20 * 2.0 ** -24 * size.abs().sum(1))  # 188 in 256 strands and a tree

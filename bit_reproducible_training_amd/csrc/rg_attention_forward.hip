@@ -10,8 +10,8 @@
 //
 // The float32 matrix instructions and the vector unit's take turns on a SIMD (1154 and 2141 us apart, 3247 together, where
 // int8 ones overlap), so every vector instruction counts: a score costs 10.5, a kept or dropped pair 13 more (Philox's
-// products). 2 x 16 heads of 4096 x 4096 x 64: 1132 us, 121 TFLOP/s of the 153 that a product of 8192^3 reaches; at
-// 8 x 12 heads of 1024 the blocks are one and a half rounds: 97 to 99.
+// products). 2 x 16 heads of 4096 x 4096 x 64: 1138 us, 121 TFLOP/s of the 153 that a product of 8192^3 reaches; at
+// 8 x 12 heads of 1024 the blocks are one and a half rounds: 95 to 97.
 #include "rg_attention.h"
 
 namespace rg {
@@ -372,7 +372,7 @@ repair(Problem z, Parts s, float* y, float* stats) {
 
 // Few queries: a block takes a chunk of keys for up to FEW of the rows that share a head of keys, a thread a key for the
 // scores, then a wavefront a row and a lane a value. Bound by HBM: the keys are read into LDS as the values are on their way, and the
-// values take their place there. One query of 2048 to 4096 keys for 16 items of 12 heads of 64: 72 us and 5.5 to join the
+// values take their place there. One query of 2048 to 4096 keys for 16 items of 12 heads of 64: 73 us and 5.1 to join the
 // chunks, 4.9 TB/s of the 5.25 of a copy; heads of 128, whose keys leave room for one block a compute unit: 3.4.
 constexpr int FEW = 8;
 
@@ -687,11 +687,13 @@ join_few(Problem z, Parts s, float* y, float* stats) {
     }
 }
 
-// The keys are split over blocks where the queries alone leave compute units idle: as many parts as bring the grid to two
-// blocks a compute unit, whole chunks each, as long as the chunks' results take at most a quarter of a gigabyte (8 heads of
-// 1024 x 1024 x 64: 34 us in 4 parts; 96 heads of 512 x 1500 with dropout, 384 blocks: 252 us in 2 parts, 286 in one).
-// Up to FEW rows of a head of keys, and more where few queries stand under many heads, go to the kernel above (16 x 12 rows of
-// 4096 keys: 214 us here, 78 there; 4 x 144 over 12 heads of 2048: 372 and 50).
+// The keys are split over blocks where the queries alone leave compute units idle: up to 384 blocks, three quarters of the two a
+// compute unit that fit, into as many parts as bring the grid to those, whole chunks each, as long as the chunks' results take at most a quarter of a
+// gigabyte. In parts and in one, us: 64 blocks (1024 x 1024 x 64) 34, 84; 384 blocks 132, 149; 448 blocks 167, 150; 512 x 1500 x 64: 288
+// blocks 186, 221; 384 blocks 190, 222; 432 blocks 241, 224.
+// Up to FEW rows of a head of keys go to the kernel above, and up to 128 of at most 4 queries. There and here, us, 16 items over 12 heads of 2048 keys
+// of 64: 8 rows of one head 76, 107; 9 rows 99, 107; 12 rows 115, 108; 4 queries of 4 heads 135, 371, of 8 heads 260, 571. It would still win at 5 to 8
+// queries of shared heads (8 of 4 heads 258, 372; 12: 382, 372) and past 128 rows (4 items of 144: 287, 2590), with its chunks' results without a bound.
 bool few(const Problem& z) { return z.Tk > 0 && ((long long)z.group * z.Tq <= FEW || (z.Tq <= 4 && (long long)z.group * z.Tq <= 128)); }
 Parts parts_of(const Problem& z) {
     Parts s;

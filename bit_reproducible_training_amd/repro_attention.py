@@ -9,7 +9,8 @@ several heads.
 
 float32 tensors on a GPU (on the current stream) or on the CPU, the same bits either way: every operation is rounded once and
 every sum's order is fixed (include/repro_attention_math.h). A query's result depends on the query and the keys it sees
-alone: the same bits in a batch, in a padded batch, or one token at a time.
+alone: the same bits in a batch, in a padded batch, or one token at a time. (With dropout also on its places in the call, by
+which pairs are dropped: the item's and head's number, the query's and the keys'.)
 """
 import functools
 
@@ -33,7 +34,7 @@ def attention(q, k, v, *, scale=None, causal=False, query_start=0, key_lengths=N
     heads, queries, keys]) is true. A query that sees none has 0 and no gradients; what keys hold that it does not see, NaN or not,
     does not reach it. relative_bias [heads, queries + keys - 1] is added at column j - i + queries - 1
     (relative_position_bias(..., dense=False) makes one). dropout: the probability that a pair's share of v is dropped, by seed
-    (as of rg.dropout). Gradients reach q, k, v and relative_bias."""
+    (as of rg.dropout). Gradients reach q, k, v and relative_bias; those of q, k and v are made together, whichever are wanted."""
     size = q.shape[-1] if q.dim() else 0
     if scale is None:
         scale = size ** -0.5 if size else 1.0

@@ -15,7 +15,7 @@
  * The random bits of dropout are a function of the seed and the places of query and key (include/repro_dropout_math.h).
  *
  * Every operation is rounded once in a fixed order (include/repro_attention_math.h): the bits do not depend on the
- * device or the launch, and a row of y depends on its query and the keys it sees alone, so that it
+ * device or the launch, and a row of y depends on its query and the keys it sees alone (and with dropout on their places), so that it
  * is the same computed alone, in a batch, or with padding.
  *
  * Plain C types only; the stream is a hipStream_t passed as void*. Return values are hipError_t

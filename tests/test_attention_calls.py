@@ -145,3 +145,17 @@ def test_a_table_of_many_heads_and_buckets():
     assert torch.equal(out[:1025], want[:1025])
     size = dout[:, 514:].double()
     assert torch.all((out[1025].double() - size.sum(1)).abs() <= 20 * 2.0 ** -24 * size.abs().sum(1))  # 188 in 256 strands and a tree
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_of_some_operands(device):
+    """Each alone, and each pair, as with all of them."""
+    t, s, dy = case(2, 4, 2, 40, 70, 16, causal=True, lengths=True, bias=True, drop=0.1)
+    t, s, dy = to(device, t), to(device, s), dy.to(device)
+    want = gradients(t, s, dy)
+    names = list(t)
+    for some in [{a} for a in names] + [{a, b} for a in names for b in names if a < b]:
+        own = {n: x.detach().requires_grad_(n in some) for n, x in t.items()}
+        leaves = [own[n] for n in names if n in some]
+        got = torch.autograd.grad(rg.attention(**own, **s), leaves, dy)
+        assert all(torch.equal(g, want["d" + n]) for g, n in zip(got, [n for n in names if n in some])), some

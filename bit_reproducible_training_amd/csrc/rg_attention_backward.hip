@@ -76,7 +76,8 @@ __device__ __forceinline__ bool live(const Problem& z, int len, int block, int r
     return block * KEY_BLOCK < last_end(z, len, min(rows, z.Tq) - 1);
 }
 
-// Without a bias and dropout heads of up to 32 values leave room for a third wavefront a SIMD.
+// Without a bias and dropout heads of up to 32 values leave room for a third wavefront a SIMD (4 x 16 heads of 2048 x 2048 x 32: 880 us, with two
+// 901; 8 x 12 of 1024 x 1024 x 16: 321, 364).
 template <int DB, bool BIAS, bool DROP, bool QUADS>
 __global__ void __launch_bounds__(256, DB == 1 && !BIAS && !DROP ? 3 : 2)
 backward_tiles(Problem z, Gradients g, Work w) {

@@ -36,6 +36,7 @@ struct Problem {
     unsigned long long seed;
     int B, Tq, Tk, H, KVH, D, group, causal, start;
     int quads;  // whether all operands' rows can be taken 16 bytes at a time
+    int overlap;                       // whether rows of an operand overlap: what lies past the last of them is then not read as 0
     int flip;                          // a negative scale: scores are multiplied by -1, and factor is positive
     float factor, scale, keep_factor;
     uint32_t threshold;
@@ -216,7 +217,8 @@ __device__ __forceinline__ QueryPart query_part(const Problem& z, const Gradient
     return r;
 }
 
-// Rows in global memory, read and written by offsets in bytes without branches: past `bytes` loads give 0 and stores do nothing.
+// Rows in global memory, read and written by offsets in bytes without branches: past `bytes` loads give 0 and stores do nothing. (Rows that
+// overlap have others before that end; where they do, `repair` and few_rows leave out by pair what is not seen.)
 typedef __amdgpu_buffer_rsrc_t Rows;
 constexpr uint32_t NOWHERE = 0xF0000000u;
 __device__ __forceinline__ Rows rows_at(const float* base, long long bytes) {

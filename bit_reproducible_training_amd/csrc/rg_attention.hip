@@ -114,6 +114,10 @@ Problem problem_of(const rg_attention_config* c, const float* q, const float* k,
         z.v_stride[n] = c->v_stride[n];
         z.mask_stride[n] = c->mask_stride[n];
     }
+    // of a single row the stride says nothing
+    if (c->Tq <= 1) z.q_stride[1] = z.D;
+    if (c->Tk <= 1) z.k_stride[1] = z.v_stride[1] = z.D;
+    z.overlap = z.q_stride[1] < z.D || z.k_stride[1] < z.D || z.v_stride[1] < z.D;
     return z;
 }
 

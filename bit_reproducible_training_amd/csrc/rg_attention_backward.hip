@@ -942,7 +942,7 @@ int backward(const Problem& z, const float* dy, const float* stats, float* dq, f
     w.dq = reinterpret_cast<float*>(base + p.dq);
     w.diagonals = dbias ? reinterpret_cast<float*>(base + p.diagonals) : nullptr;
     // a query's values must not reach keys that it does not see, nor a key's a query
-    w.broken = z.causal || z.mask || z.key_lengths ? reinterpret_cast<int*>(base + p.broken) : nullptr;
+    w.broken = z.causal || z.mask || z.key_lengths || z.overlap ? reinterpret_cast<int*>(base + p.broken) : nullptr;
     const int most = w.count, across = (z.Tq + z.Tk - 1 + 63) / 64, heads = (int)(MAX_BLOCKS / across);  // (of a launch of sum_diagonals)
     for (int first = 0; first < p.blocks; first += most) {
         w.first = first;

@@ -497,7 +497,7 @@ few_rows(Problem z, Parts s, float* y, float* stats, unsigned long long* used) {
         for (int r = 0; r < rows; ++r) P[r][t] = kept(z, seed, b, h0 + (r0 + r) / z.Tq, (r0 + r) % z.Tq, j) ? P[r][t] : 0.0f;
         __syncthreads();
     }
-    const bool some = z.causal || z.mask;
+    const bool some = z.causal || z.mask || z.overlap;
     RowChunk mine[2];  // of rows wave and wave + 4
     float a[2][4];
 #pragma unroll
@@ -721,9 +721,9 @@ long long blocks_of(const Problem& z, const Parts& s) {
     return few(z) ? (long long)z.B * z.KVH * ((z.group * z.Tq + FEW - 1) / FEW) * s.chunks
                   : (long long)z.B * z.H * ((z.Tq + ROWS - 1) / ROWS) * s.parts;
 }
-// What a key holds must not reach a row that does not see it: under a causal mask or one of pairs.
+// What a key holds must not reach a row that does not see it: under a causal mask or one of pairs, or where rows past the last are not 0.
 // (Few rows leave out each pair by itself.)
-bool watched(const Problem& z, bool masked) { return !few(z) && (z.causal || masked); }
+bool watched(const Problem& z, bool masked) { return !few(z) && (z.causal || masked || z.overlap); }
 size_t sums_offset(const Problem& z, const Parts& s) { return ((size_t)z.B * z.H * z.Tq * s.slots * sizeof(float2) + 15) / 16 * 16; }
 size_t parts_bytes(const Problem& z, const Parts& s) {
     return s.parts > 1 ? (sums_offset(z, s) + (size_t)z.B * z.H * z.Tq * s.slots * z.D * sizeof(float) + 15) / 16 * 16 : 0;

@@ -159,3 +159,45 @@ def test_gradients_of_some_operands(device):
         leaves = [own[n] for n in names if n in some]
         got = torch.autograd.grad(rg.attention(**own, **s), leaves, dy)
         assert all(torch.equal(g, want["d" + n]) for g, n in zip(got, [n for n in names if n in some])), some
+
+
+def windows(x, tk, d):
+    """Keys that overlap: key j is values j .. j + d - 1 of x."""
+    return x.as_strided((1, tk, 1, d), (0, 1, 0, 1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("tq", [1, 6, 40])
+def test_a_value_that_is_not_finite_stays_in_its_place(device, value, tq):
+    """One key, keys at one address and keys that overlap, where rows past the last lie in the same memory: a visible value that is not finite
+    reaches the outputs that it belongs to, as it is, and no others."""
+    g = torch.Generator().manual_seed(tq)
+    q, x = torch.randn(1, tq, 1, 8, generator=g), torch.randn(200, generator=g)
+    x[20] = value
+    dy = torch.randn(1, tq, 1, 8, generator=g)
+    one = torch.randn(1, 1, 1, 8, generator=g)
+    one[..., 3] = value
+    for name, v in (("one key", one), ("one address", one.expand(1, 70, 1, 8)), ("overlapping", windows(x, 21, 8)),
+                    ("past the length", windows(x, 90, 8))):
+        k = torch.randn(v.shape, generator=g)
+        lengths = torch.tensor([15]) if name == "past the length" else None
+        seen = v.shape[1] if lengths is None else 15
+        t = {"q": q, "k": k, "v": v, "relative_bias": None}
+        want = gradients({**t, "v": v.contiguous()}, {"key_lengths": lengths}, dy)
+        on = {n: None if a is None else a.to(device) for n, a in t.items()}
+        if name != "one key":  # (to() lays them out anew)
+            on["v"] = one.to(device).expand(1, 70, 1, 8) if name == "one address" else windows(x.to(device), v.shape[1], 8)
+        y = rg.attention(on["q"], on["k"], on["v"], key_lengths=None if lengths is None else lengths.to(device)).cpu()
+        for d in range(8):
+            column = v[0, :seen, 0, d]
+            if column.isfinite().all():
+                assert y[..., d].isfinite().all(), (name, d)
+            else:
+                assert torch.all(y[..., d].isnan() if value != value else y[..., d] == value), (name, d)
+        got = gradients(on, {"key_lengths": None if lengths is None else lengths.to(device)}, dy.to(device))
+        for n in ("y", "dq", "dk", "dv"):
+            a, b = got[n].cpu(), want[n]
+            if n in ("dk", "dv") and a.shape != b.shape:
+                continue
+            assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)), (name, n)

@@ -61,8 +61,8 @@ int rg_attention_pack_mask(const unsigned char* mask, long long items, long long
  * cfg->seed; used receives it) may be null. y [B][Tq][H][D] contiguous; stats [B][H][Tq][2] for the
  * backward pass, or null.
  * 1 (invalid value): null cfg, sizes out of range, scale not finite, dropout outside [0, 1); with rows and values to compute null q,
- * k, v or y, an address off 4 bytes (off 8: lengths, mask, stats, seeds), a workspace that is needed and null, off 16 bytes or too small; 2^32 or more times 8
- * single queries and 256 keys of theirs (which only keys of many items at the same address, by a stride of 0, reach). */
+ * k, v or y, an address off 4 bytes (off 8: lengths, mask, stats, seeds), a workspace that is needed and null, off 16 bytes or too small; few
+ * queries that make 2^32 or more blocks of 8 rows by 256 keys (which only keys of many items at one address, by a stride of 0, reach). */
 int rg_attention_workspace(const rg_attention_config* cfg, int masked, size_t* bytes); /* masked: whether a mask is given */
 int rg_attention_fp32(const rg_attention_config* cfg, const float* q, const float* k, const float* v,
                       const long long* key_lengths, const unsigned long long* mask, const float* relative_bias,
